@@ -402,6 +402,7 @@ void register_comm_ops(torch::Library& m);
 void register_seq_ops(torch::Library& m);      // bindings_seq.cpp
 void register_state_ops(torch::Library& m);    // bindings_state.cpp
 void register_mix_ops(torch::Library& m);      // bindings_mix.cpp
+void register_vocab_ops(torch::Library& m);    // bindings_vocab.cpp
 
 static int64_t set_pdl(int64_t on) { const int old = rb_get_pdl(); if (on >= 0) rb_set_pdl((int)on); return old; }
 
@@ -434,4 +435,5 @@ TORCH_LIBRARY(realhf_b200, m) {
   register_seq_ops(m);
   register_state_ops(m);
   register_mix_ops(m);
+  register_vocab_ops(m);
 }

@@ -1,0 +1,180 @@
+// torch bindings for the operators on rows of logits: token statistics, top alternatives, distillation.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/library.h>
+#include <torch/types.h>
+
+#include <vector>
+
+using at::Tensor;
+using OptT = c10::optional<Tensor>;
+
+extern "C" {
+int rb_token_stats(const void*, int64_t, const int64_t*, const uint8_t*, int64_t, float*, float*, float*, int64_t, int, float, int, cudaStream_t);
+int rb_token_stats_bwd(const void*, int64_t, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*, void*, int64_t,
+                       int64_t, int, float, int, cudaStream_t);
+int rb_top_logprobs_max();
+int rb_top_logprobs(const void*, int64_t, const int64_t*, const uint8_t*, int64_t, float*, float*, float*, int64_t*, float*, int64_t, int, int, float, int,
+                    cudaStream_t);
+int rb_distill_max_listed();
+int64_t rb_distill_max_vocab();
+int rb_distill_fwd(const void*, int64_t, const int64_t*, const float*, const float*, int, float*, float*, float*, float*, int*, int64_t, int, int, float, int,
+                   cudaStream_t);
+int rb_distill_bwd(const void*, int64_t, const float*, const float*, const float*, const int*, const float*, void*, int64_t, int64_t, int, int, float, int,
+                   cudaStream_t);
+}
+
+namespace {
+
+cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+int dtype_code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return 0;
+    case at::kBFloat16: return 1;
+    case at::kHalf: return 2;
+    default: TORCH_CHECK(false, "unsupported dtype ", t.scalar_type(), " (float32, bfloat16 or float16)");
+  }
+}
+
+void check_logits(const Tensor& logits, const char* op, double inv_temp) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, op, ": logits are a CUDA matrix [rows, vocabulary] with unit inner stride");
+  TORCH_CHECK(logits.size(1) > 0 && logits.size(1) <= 0x7fffff00LL && logits.size(0) <= 0x7fffffffLL, op, ": bad size ", logits.sizes());
+  TORCH_CHECK(inv_temp > 0, op, ": the inverse temperature is positive");
+}
+
+// a contiguous tensor of this device, of one value a row (or [rows, k])
+const void* row_values(const OptT& t, at::ScalarType type, const Tensor& logits, int64_t k, const char* op, const char* name) {
+  if (!t.has_value()) return nullptr;
+  TORCH_CHECK(t->device() == logits.device() && t->scalar_type() == type && t->is_contiguous() && t->size(0) == logits.size(0) &&
+                  (k < 0 ? t->dim() == 1 : t->dim() == 2 && t->size(1) == k),
+              op, ": ", name, " has to be contiguous, of type ", type, ", on the logits' device and of ", logits.size(0), " rows");
+  return t->data_ptr();
+}
+
+const uint8_t* mask_rows(const OptT& mask, const Tensor& logits, const char* op) {
+  if (!mask.has_value()) return nullptr;
+  TORCH_CHECK(mask->device() == logits.device() && mask->scalar_type() == at::kByte && mask->dim() == 2 && mask->is_contiguous() &&
+                  mask->size(0) == logits.size(0) && mask->size(1) * 8 >= logits.size(1),
+              op, ": the mask is a packed uint8 matrix [rows, at least vocabulary / 8] on the logits' device");
+  return mask->data_ptr<uint8_t>();
+}
+
+int64_t mask_bytes(const OptT& mask) { return mask.has_value() ? mask->size(1) : 0; }
+
+// the gradient's destination: a new matrix, or `out` (the logits themselves, or one like them)
+Tensor gradient_like(const Tensor& logits, const OptT& out, const char* op) {
+  if (!out.has_value()) return at::empty({logits.size(0), logits.size(1)}, logits.options());
+  TORCH_CHECK(out->device() == logits.device() && out->scalar_type() == logits.scalar_type() && out->sizes() == logits.sizes() && out->stride(1) == 1, op,
+              ": the gradient's destination is like the logits");
+  return *out;
+}
+
+std::vector<Tensor> token_stats(const Tensor& logits, const Tensor& labels, const OptT& mask, double inv_temp) {
+  check_logits(logits, "token_stats", inv_temp);
+  const int64_t rows = logits.size(0);
+  const auto* lab = static_cast<const int64_t*>(row_values(labels, at::kLong, logits, -1, "token_stats", "labels"));
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto f = logits.options().dtype(at::kFloat);
+  Tensor logp = at::empty({rows}, f), entropy = at::empty({rows}, f), lse = at::empty({rows}, f);
+  const int rc = rb_token_stats(logits.data_ptr(), logits.stride(0), lab, mask_rows(mask, logits, "token_stats"), mask_bytes(mask), logp.data_ptr<float>(),
+                                entropy.data_ptr<float>(), lse.data_ptr<float>(), rows, (int)logits.size(1), (float)inv_temp, dtype_code(logits), stream());
+  TORCH_CHECK(rc == 0, "token_stats failed with code ", rc);
+  return {logp, entropy, lse};
+}
+
+Tensor token_stats_bwd(const Tensor& logits, const Tensor& labels, const OptT& mask, const Tensor& lse, const Tensor& entropy, const OptT& g_logp,
+                       const OptT& g_entropy, double inv_temp, const OptT& out) {
+  const char* op = "token_stats_bwd";
+  check_logits(logits, op, inv_temp);
+  const auto* lab = static_cast<const int64_t*>(row_values(labels, at::kLong, logits, -1, op, "labels"));
+  const auto* l = static_cast<const float*>(row_values(lse, at::kFloat, logits, -1, op, "lse"));
+  const auto* h = static_cast<const float*>(row_values(entropy, at::kFloat, logits, -1, op, "entropy"));
+  const auto* gl = static_cast<const float*>(row_values(g_logp, at::kFloat, logits, -1, op, "the log-probability's gradient"));
+  const auto* ge = static_cast<const float*>(row_values(g_entropy, at::kFloat, logits, -1, op, "the entropy's gradient"));
+  c10::cuda::CUDAGuard guard(logits.device());
+  Tensor d = gradient_like(logits, out, op);
+  const int rc = rb_token_stats_bwd(logits.data_ptr(), logits.stride(0), lab, mask_rows(mask, logits, op), mask_bytes(mask), l, h, gl, ge, d.data_ptr(),
+                                    d.stride(0), logits.size(0), (int)logits.size(1), (float)inv_temp, dtype_code(logits), stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+  return d;
+}
+
+std::vector<Tensor> top_logprobs(const Tensor& logits, int64_t k, const OptT& labels, const OptT& mask, double inv_temp) {
+  const char* op = "top_logprobs";
+  check_logits(logits, op, inv_temp);
+  const int64_t rows = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(k >= 1 && k <= V && k <= rb_top_logprobs_max(), op, ": between 1 and min(vocabulary, ", rb_top_logprobs_max(), ") alternatives, not ", k);
+  const auto* lab = static_cast<const int64_t*>(row_values(labels, at::kLong, logits, -1, op, "labels"));
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto f = logits.options().dtype(at::kFloat);
+  Tensor entropy = at::empty({rows}, f), rest = at::empty({rows}, f), top = at::empty({rows, k}, f), ids = at::empty({rows, k}, f.dtype(at::kLong));
+  Tensor logp = labels.has_value() ? at::empty({rows}, f) : Tensor();
+  const int rc = rb_top_logprobs(logits.data_ptr(), logits.stride(0), lab, mask_rows(mask, logits, op), mask_bytes(mask),
+                                 labels.has_value() ? logp.data_ptr<float>() : nullptr, entropy.data_ptr<float>(), top.data_ptr<float>(), ids.data_ptr<int64_t>(),
+                                 rest.data_ptr<float>(), rows, (int)V, (int)k, (float)inv_temp, dtype_code(logits), stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+  std::vector<Tensor> r{top, ids, rest, entropy};
+  if (labels.has_value()) r.push_back(logp);
+  return r;
+}
+
+std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& ids, const Tensor& top_logp, const OptT& rest_logp, bool reverse, double inv_temp,
+                                bool need_grad) {
+  const char* op = "distill_fwd";
+  check_logits(logits, op, inv_temp);
+  const int64_t rows = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(ids.dim() == 2 && ids.size(1) >= 1 && ids.size(1) <= rb_distill_max_listed(), op, ": between 1 and ", rb_distill_max_listed(), " tokens a row");
+  TORCH_CHECK(V <= rb_distill_max_vocab(), op, ": a vocabulary of at most ", rb_distill_max_vocab(), " tokens");
+  TORCH_CHECK(!reverse || rest_logp.has_value(), op, ": the reverse divergence needs the teacher's rest");
+  const int64_t k = ids.size(1);
+  const auto* id = static_cast<const int64_t*>(row_values(ids, at::kLong, logits, k, op, "the tokens"));
+  const auto* t = static_cast<const float*>(row_values(top_logp, at::kFloat, logits, k, op, "the tokens' log-probabilities"));
+  const auto* tr = static_cast<const float*>(row_values(rest_logp, at::kFloat, logits, -1, op, "the rest's log-probability"));
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto f = logits.options().dtype(at::kFloat);
+  Tensor loss = at::empty({rows}, f), lse_rest, g_rest, g_listed, ids_out;
+  if (need_grad) {
+    lse_rest = at::empty({rows}, f);
+    g_rest = at::empty({rows}, f);
+    g_listed = at::empty({rows, k}, f);
+    ids_out = at::empty({rows, k}, f.dtype(at::kInt));
+  }
+  const int rc = rb_distill_fwd(logits.data_ptr(), logits.stride(0), id, t, tr, reverse, loss.data_ptr<float>(), need_grad ? lse_rest.data_ptr<float>() : nullptr,
+                                need_grad ? g_rest.data_ptr<float>() : nullptr, need_grad ? g_listed.data_ptr<float>() : nullptr,
+                                need_grad ? ids_out.data_ptr<int>() : nullptr, rows, (int)V, (int)k, (float)inv_temp, dtype_code(logits), stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+  if (!need_grad) return {loss};
+  return {loss, lse_rest, g_rest, g_listed, ids_out};
+}
+
+Tensor distill_bwd(const Tensor& logits, const Tensor& lse_rest, const Tensor& g_rest, const Tensor& g_listed, const Tensor& ids, const Tensor& g_loss,
+                   double inv_temp, const OptT& out) {
+  const char* op = "distill_bwd";
+  check_logits(logits, op, inv_temp);
+  TORCH_CHECK(ids.dim() == 2, op, ": the tokens are a matrix");
+  const int64_t k = ids.size(1);
+  const auto* id = static_cast<const int*>(row_values(ids, at::kInt, logits, k, op, "the tokens"));
+  const auto* gk = static_cast<const float*>(row_values(g_listed, at::kFloat, logits, k, op, "the tokens' gradients"));
+  const auto* lr = static_cast<const float*>(row_values(lse_rest, at::kFloat, logits, -1, op, "lse_rest"));
+  const auto* gr = static_cast<const float*>(row_values(g_rest, at::kFloat, logits, -1, op, "the rest's gradient"));
+  const auto* g = static_cast<const float*>(row_values(g_loss, at::kFloat, logits, -1, op, "the loss's gradient"));
+  c10::cuda::CUDAGuard guard(logits.device());
+  Tensor d = gradient_like(logits, out, op);
+  const int rc = rb_distill_bwd(logits.data_ptr(), logits.stride(0), lr, gr, gk, id, g, d.data_ptr(), d.stride(0), logits.size(0), (int)logits.size(1), (int)k,
+                                (float)inv_temp, dtype_code(logits), stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+  return d;
+}
+
+}  // namespace
+
+void register_vocab_ops(torch::Library& m) {
+  m.def("token_stats(Tensor logits, Tensor labels, Tensor? mask, float inv_temp) -> Tensor[]", &token_stats);
+  m.def("token_stats_bwd(Tensor logits, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
+        "Tensor(a!)? out) -> Tensor", &token_stats_bwd);
+  m.def("top_logprobs(Tensor logits, int k, Tensor? labels, Tensor? mask, float inv_temp) -> Tensor[]", &top_logprobs);
+  m.def("distill_fwd(Tensor logits, Tensor ids, Tensor top_logp, Tensor? rest_logp, bool reverse, float inv_temp, bool need_grad) -> Tensor[]", &distill_fwd);
+  m.def("distill_bwd(Tensor logits, Tensor lse_rest, Tensor g_rest, Tensor g_listed, Tensor ids, Tensor g_loss, float inv_temp, Tensor(a!)? out) -> Tensor",
+        &distill_bwd);
+}

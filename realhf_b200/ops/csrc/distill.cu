@@ -1,0 +1,205 @@
+// Kullback-Leibler divergence between a teacher known by some tokens' log-probabilities and a student's logits, forward and backward.
+//
+// Outcomes b: the listed tokens one by one and, as one more, all tokens that are not listed.  Teacher: t_b, p_b = e^{t_b}; student, from
+// y_j = x_j inv_temp - lse: y_b = y_id, y_rest = lse over the unlisted tokens - lse, q_b = e^{y_b}.
+//   forward  L = sum_b p_b (t_b - y_b)     d L / d z_b = P q_b - p_b,       P = sum_b p_b
+//   reverse  L = sum_b q_b (y_b - t_b)     d L / d z_b = q_b (y_b - t_b - L)
+// and an unlisted token has the rest's times its share e^{x_j inv_temp - lse_rest} of it (a share is at most 1: dividing by q_rest could overflow).
+// Without a rest the teacher is renormalised over its tokens and p_rest = 0 (forward only).
+// The rest's mass is summed over the tokens it consists of, from a bitmap of the listed ones: 1 - sum q_b would cancel.
+// A negative id is an unused place; an id given again counts where it stands first; an id beyond the vocabulary makes the row's loss NaN.
+// p_b = 0 and q_b = 0 contribute 0.
+#include "vocab_rows.cuh"
+
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kMaxListed = 1024;
+constexpr int kBwdThreads = 256, kBwdVecs = 4;
+
+struct DistillShared {
+  float red[96];
+  int dup;
+  int ids[kMaxListed];
+  float y[kMaxListed], t[kMaxListed];
+};
+
+RB_DEVICE float block_sum(float v, float* red) { return rb::block_reduce<false>(v, red); }
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const T* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ ids,
+                                                               const float* __restrict__ top_logp, const float* __restrict__ rest_logp, int reverse,
+                                                               float* __restrict__ loss, float* __restrict__ lse_rest_out, float* __restrict__ grad_rest,
+                                                               float* __restrict__ grad_listed, int* __restrict__ ids_out, int V, int k, float inv_temp) {
+  __shared__ DistillShared sh;
+  extern __shared__ uint32_t listed[];                  // a bit a token
+  const int64_t row = blockIdx.x;
+  const T* lr = logits + row * row_stride;
+  const float kk = inv_temp * rb::kLog2e;
+  for (int i = threadIdx.x; i < RB_CEIL_DIV(V, 32); i += kThreads) listed[i] = 0;
+  if (threadIdx.x == 0) sh.dup = 0;
+  __syncthreads();
+  bool beyond = false;
+  for (int i = threadIdx.x; i < k; i += kThreads) {
+    const int64_t id = ids[row * k + i];
+    const bool ok = id >= 0 && id < V;
+    beyond |= id >= V;
+    sh.ids[i] = ok ? (int)id : -1;
+    sh.t[i] = ok ? top_logp[row * k + i] : -INFINITY;
+    sh.y[i] = ok ? rb::to_f(lr[id]) * inv_temp : -INFINITY;
+    if (ok && (atomicOr(&listed[id >> 5], 1u << (id & 31)) >> (id & 31)) & 1) sh.dup = 1;
+  }
+  beyond = __syncthreads_or(beyond);
+  if (sh.dup) {                                         // the first place of an id stands
+    for (int i = threadIdx.x; i < k; i += kThreads) {
+      bool again = false;
+      const int id = sh.ids[i];
+      for (int e = 0; e < i && id >= 0; ++e) again |= ids[row * k + e] == id;
+      if (again) { sh.ids[i] = -1; sh.t[i] = -INFINITY; sh.y[i] = -INFINITY; }
+    }
+    __syncthreads();
+  }
+  // the row: every unlisted token's part of the rest
+  rb::RowStats others;
+  for (int j = threadIdx.x; j < V; j += kThreads)
+    if (!((listed[j >> 5] >> (j & 31)) & 1)) others.one(rb::to_f(lr[j]), kk);
+  others = rb::block_stats(others, kk, sh.red);
+  const bool rest_empty = others.m == -INFINITY;
+  const float lse_rest = others.m < INFINITY ? (rest_empty ? -INFINITY : fmaf(others.m, inv_temp, logf(others.s))) : NAN;
+  // lse over the listed tokens and the rest; the teacher's over its listed ones where it is to be renormalised
+  rb::RowStats all, teach;
+  for (int i = threadIdx.x; i < k; i += kThreads) {
+    all.one(sh.y[i], rb::kLog2e);
+    teach.one(sh.t[i], rb::kLog2e);
+  }
+  if (threadIdx.x == 0) all.one(lse_rest, rb::kLog2e);
+  all = rb::block_stats(all, rb::kLog2e, sh.red);
+  const float lse = all.m < INFINITY ? (all.m == -INFINITY ? -INFINITY : all.m + logf(all.s)) : NAN;
+  float tr = -INFINITY, shift = 0.f;
+  if (rest_logp) {
+    tr = rest_logp[row];
+  } else {
+    teach = rb::block_stats(teach, rb::kLog2e, sh.red);
+    shift = teach.m == -INFINITY ? 0.f : teach.m + logf(teach.s);
+  }
+  const float base = lse == -INFINITY ? 0.f : lse;      // a row without a token: every y is -inf
+  const float yr = lse_rest - base;
+  float part = 0.f, mass = 0.f;
+  for (int i = threadIdx.x; i <= k; i += kThreads) {
+    const float y = i < k ? sh.y[i] - base : yr, t = i < k ? sh.t[i] - shift : tr;
+    const float w = expf(reverse ? y : t);
+    const float f = reverse ? y - t : t - y;
+    if (w != 0.f) part += w * f;                        // (NaN included)
+    mass += w;
+  }
+  float L = block_sum(part, sh.red);
+  const float P = block_sum(mass, sh.red);
+  if (beyond || lse != lse) L = NAN;
+  auto grad = [&](float y, float t) {
+    const float q = expf(y);
+    if (!reverse) return P * q - expf(t);
+    return q == 0.f ? 0.f : q * (y - t - L);
+  };
+  if (threadIdx.x == 0) {
+    loss[row] = L;
+    if (grad_rest) {
+      lse_rest_out[row] = lse_rest;
+      grad_rest[row] = L != L ? NAN : (rest_empty ? 0.f : grad(yr, tr));
+    }
+  }
+  if (grad_rest)
+    for (int i = threadIdx.x; i < k; i += kThreads) {
+      ids_out[row * k + i] = sh.ids[i];
+      grad_listed[row * k + i] = L != L ? NAN : grad(sh.y[i] - base, sh.t[i] - shift);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logits, int64_t row_stride, const float* __restrict__ lse_rest_in,
+                                                                  const float* __restrict__ grad_rest, const float* __restrict__ grad_listed,
+                                                                  const int* __restrict__ ids, const float* __restrict__ g_loss, T* out, int64_t out_stride,
+                                                                  int V, int k, float inv_temp, int segs) {
+  constexpr int VEC = rb::RowSpan<T>::VEC, kPer = kBwdThreads * kBwdVecs * VEC;
+  const int64_t row = blockIdx.x / segs;
+  const int seg = blockIdx.x - (int)(row * segs);
+  const T* lr = logits + row * row_stride;
+  T* orow = out + row * out_stride;
+  const float g = g_loss[row] * inv_temp;
+  const bool zero = g == 0.f;
+  const float a = zero ? 0.f : g * grad_rest[row], lr_rest = lse_rest_in[row];
+  const float ref = lr_rest == -INFINITY ? 0.f : lr_rest;
+  auto grad = [&](float x) {
+    const float e = rb::exp2_fast(fmaf(x, inv_temp, -ref) * rb::kLog2e);
+    return zero || e == 0.f ? 0.f : a * e;
+  };
+  const rb::RowSpan<T> span(lr, V);
+  const bool same = ((reinterpret_cast<uintptr_t>(lr) ^ reinterpret_cast<uintptr_t>(orow)) & 15) == 0;
+  int lo, hi;                                           // the elements of this block
+  if (same) {
+    const rb::Pack<T, VEC>* vecs = reinterpret_cast<const rb::Pack<T, VEC>*>(lr + span.head);
+    rb::Pack<T, VEC>* outs = reinterpret_cast<rb::Pack<T, VEC>*>(orow + span.head);
+    lo = seg == 0 ? 0 : span.head + seg * kPer;
+    hi = seg == segs - 1 ? V : min(V, span.head + (seg + 1) * kPer);
+#pragma unroll
+    for (int u = 0; u < kBwdVecs; ++u) {
+      const int i = (seg * kBwdVecs + u) * kBwdThreads + threadIdx.x;
+      if (i >= span.nvec) break;
+      rb::Pack<T, VEC> p = vecs[i];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) p.v[e] = rb::from_f<T>(grad(rb::to_f(p.v[e])));
+      outs[i] = p;
+    }
+    const int j = span.edge(threadIdx.x, V);
+    if (j >= lo && j < hi) orow[j] = rb::from_f<T>(grad(rb::to_f(lr[j])));
+  } else {
+    lo = seg * kPer;
+    hi = seg == segs - 1 ? V : min(V, (seg + 1) * kPer);
+    for (int j = lo + threadIdx.x; j < hi; j += kBwdThreads) orow[j] = rb::from_f<T>(grad(rb::to_f(lr[j])));
+  }
+  __syncthreads();                                      // the listed tokens over what was just written
+  for (int i = threadIdx.x; i < k; i += kBwdThreads) {
+    const int id = ids[row * k + i];
+    if (id >= lo && id < hi) orow[id] = rb::from_f<T>(zero ? 0.f : g * grad_listed[row * k + i]);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int rb_distill_max_listed() { return kMaxListed; }
+int64_t rb_distill_max_vocab() { return 1 << 20; }
+
+// grad_rest null: no gradient asked for (then lse_rest, grad_listed and ids_out are null too).
+int rb_distill_fwd(const void* logits, int64_t row_stride, const int64_t* ids, const float* top_logp, const float* rest_logp, int reverse, float* loss,
+                   float* lse_rest, float* grad_rest, float* grad_listed, int* ids_out, int64_t rows, int V, int k, float inv_temp, int dt, cudaStream_t s) {
+  if (rows == 0) return 0;
+  if (k < 0 || k > kMaxListed || V > rb_distill_max_vocab() || (reverse && !rest_logp)) return -1;
+  const int smem = RB_CEIL_DIV(V, 32) * 4;
+#define RB_L(T)                                                                                                                                     \
+  {                                                                                                                                                 \
+    if (smem > 32768 && cudaFuncSetAttribute(distill_fwd_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2;     \
+    distill_fwd_kernel<T><<<(unsigned)rows, kThreads, smem, s>>>((const T*)logits, row_stride, ids, top_logp, rest_logp, reverse, loss, lse_rest,     \
+                                                                 grad_rest, grad_listed, ids_out, V, k, inv_temp);                                   \
+  }
+  if (dt == 0) RB_L(float) else if (dt == 1) RB_L(__nv_bfloat16) else if (dt == 2) RB_L(__half) else return -1;
+#undef RB_L
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+// out: [rows, V], may be the logits themselves
+int rb_distill_bwd(const void* logits, int64_t row_stride, const float* lse_rest, const float* grad_rest, const float* grad_listed, const int* ids,
+                   const float* g_loss, void* out, int64_t out_stride, int64_t rows, int V, int k, float inv_temp, int dt, cudaStream_t s) {
+  if (rows == 0) return 0;
+  const int per = kBwdThreads * kBwdVecs * (dt == 0 ? 4 : 8);
+  const int64_t segs = RB_CEIL_DIV((int64_t)V, per);
+  if (rows * segs > 0x7fffffffLL) return -3;
+#define RB_L(T)                                                                                                                                        \
+  distill_bwd_kernel<T><<<(unsigned)(rows * segs), kBwdThreads, 0, s>>>((const T*)logits, row_stride, lse_rest, grad_rest, grad_listed, ids, g_loss,     \
+                                                                        (T*)out, out_stride, V, k, inv_temp, (int)segs)
+  if (dt == 0) RB_L(float); else if (dt == 1) RB_L(__nv_bfloat16); else if (dt == 2) RB_L(__half); else return -1;
+#undef RB_L
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+}  // extern "C"

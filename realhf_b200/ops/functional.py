@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import os
 
-from typing import List, Optional, Tuple
+from typing import List, NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -428,6 +428,389 @@ def lm_head_logprobs(hidden, weight, labels, mask_bits=None, temperature: float 
 def lm_head_logprobs_ref(hidden, weight, labels, mask_bits=None, temperature: float = 1.0):
     logits = hidden.float() @ weight.float().t()
     return logprob_from_logits_ref(logits, labels, mask_bits, 1.0 / temperature)[0]
+
+
+# ------------------------------------------------------------------------------------------------ token statistics, alternatives, distillation
+
+
+def _ref_logits(logits, mask_bits, inv_temp):
+    x = (logits if logits.dtype == torch.float64 else logits.float()) * inv_temp
+    return x if mask_bits is None else x.masked_fill(unpack_mask_bits(mask_bits, x.shape[1]), float("-inf"))
+
+
+def _ref_lse(x):
+    """log sum exp of every row: -inf with zero gradients for a row of -inf alone, NaN for one that holds a NaN or +inf."""
+    none = (x == float("-inf")).all(-1)
+    lse = torch.logsumexp(x.masked_fill(none.unsqueeze(-1), 0.0), -1)
+    return torch.where(lse == float("inf"), torch.full_like(lse, float("nan")), lse).masked_fill(none, float("-inf"))
+
+
+def logprob_entropy_from_logits_ref(logits, labels, mask_bits=None, inv_temp: float = 1.0):
+    x = _ref_logits(logits, mask_bits, inv_temp)
+    V, labels = x.shape[1], labels.long()
+    lse = _ref_lse(x)
+    none = lse == float("-inf")
+    y = x - lse.masked_fill(none, 0.0).unsqueeze(-1)
+    gone = y == float("-inf")
+    entropy = -(torch.exp(y).masked_fill(gone, 0.0) * y.masked_fill(gone, 0.0)).sum(-1)
+    logp = y.gather(-1, labels.clamp(0, V - 1).unsqueeze(-1)).squeeze(-1)
+    logp = logp.masked_fill(none, float("-inf")).masked_fill(lse.isnan() | (labels >= V), float("nan")).masked_fill(labels < 0, 0.0)
+    return logp, entropy.masked_fill(lse.isnan(), float("nan"))
+
+
+def _check_rows(op: str, logits, inv_temp, **rows):
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"{op}: logits are a matrix [rows, vocabulary], not {tuple(logits.shape)}")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16) and (logits.is_cuda or logits.dtype != torch.float64):
+        raise ValueError(f"{op}: logits of type {logits.dtype} (float32, bfloat16 or float16)")
+    if not inv_temp > 0:
+        raise ValueError(f"{op}: the inverse temperature is positive, not {inv_temp}")
+    _check_row_values(op, logits.shape[0], logits.device, **rows)
+
+
+def _check_row_values(op: str, T: int, device, **rows):
+    for name, t in rows.items():
+        if t is not None and (t.dim() == 0 or t.shape[0] != T or t.device != device):
+            raise ValueError(f"{op}: {name} has to be on the logits' device with one row a row of logits ({T}), not {tuple(t.shape)} on {t.device}")
+    for name in ("labels", "ids", "top_ids"):
+        t = rows.get(name)
+        if t is not None and (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool):
+            raise ValueError(f"{op}: {name} are whole numbers, not {t.dtype}")
+
+
+def _check_labels(op: str, labels):
+    if labels is not None and labels.dim() != 1:
+        raise ValueError(f"{op}: labels are a vector, not {tuple(labels.shape)}")
+
+
+def _check_mask(op: str, mask_bits, V: int):
+    if mask_bits is not None and (mask_bits.dim() != 2 or mask_bits.dtype != torch.uint8 or mask_bits.shape[1] * 8 < V):
+        raise ValueError(f"{op}: the mask is a packed uint8 matrix [rows, at least {-(-V // 8)}] (`pack_mask_bits`)")
+
+
+def _rows_f32(t):
+    return None if t is None else t.float().contiguous()
+
+
+def _unit_rows(logits):
+    return logits if logits.stride(1) == 1 else logits.clone(memory_format=torch.contiguous_format)   # (`contiguous()` keeps a single column as it lies)
+
+
+class _TokenStats(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, mask_bits, inv_temp):
+        ctx.set_materialize_grads(False)
+        logp, entropy, lse = lib().token_stats(logits, labels, mask_bits, inv_temp)
+        ctx.save_for_backward(logits, labels, mask_bits, lse, entropy)
+        ctx.inv_temp = inv_temp
+        return logp, entropy
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy):
+        logits, labels, mask_bits, lse, entropy = ctx.saved_tensors
+        if g_logp is None and g_entropy is None:
+            return None, None, None, None
+        return lib().token_stats_bwd(logits, labels, mask_bits, lse, entropy, _rows_f32(g_logp), _rows_f32(g_entropy), ctx.inv_temp, None), None, None, None
+
+
+def logprob_entropy_from_logits(logits, labels, mask_bits=None, inv_temp: float = 1.0):
+    """(log p(label), entropy of p) per row of logits [T, V], fp32, both differentiable in the logits; p = softmax(logits * inv_temp) over
+    the tokens that `mask_bits` (`pack_mask_bits`, set = filtered out) keeps.  A negative label is no token: 0 without a gradient;
+    a label of V or more gives NaN.  A row that keeps no token gives -inf and 0, one that holds a NaN or +inf NaN.  A row whose incoming
+    gradients are 0 gets zeros, whatever it holds."""
+    op = "logprob_entropy_from_logits"
+    _check_rows(op, logits, inv_temp, labels=labels, mask_bits=mask_bits)
+    _check_labels(op, labels)
+    _check_mask(op, mask_bits, logits.shape[1])
+    if not use_native(logits):
+        return logprob_entropy_from_logits_ref(logits, labels, mask_bits, inv_temp)
+    logits, labels = _unit_rows(logits), labels.long().contiguous()
+    mask_bits = mask_bits.contiguous() if mask_bits is not None else None
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TokenStats.apply(logits, labels, mask_bits, float(inv_temp))
+    return tuple(lib().token_stats(logits.detach(), labels, mask_bits, inv_temp)[:2])
+
+
+class TopLogprobs(NamedTuple):
+    """The k most likely tokens of every row and what surrounds them (all fp32 but the ids)."""
+
+    top_logp: torch.Tensor            # [T, k], descending; -inf where a row keeps fewer than k tokens
+    top_ids: torch.Tensor             # [T, k] int64, equal logits by the lower id; -1 where a row keeps fewer than k tokens
+    rest_logp: torch.Tensor           # [T], log of the mass of all other tokens
+    entropy: torch.Tensor             # [T]
+    logp: Optional[torch.Tensor]      # [T], of the given labels
+
+
+def top_logprobs_from_logits_ref(logits, k: int, labels=None, mask_bits=None, inv_temp: float = 1.0) -> TopLogprobs:
+    x = _ref_logits(logits, mask_bits, inv_temp)
+    lse = _ref_lse(x)
+    raw = logits if mask_bits is None else logits.masked_fill(unpack_mask_bits(mask_bits, x.shape[1]), float("-inf"))
+    ids = torch.sort(raw + 0.0, dim=-1, descending=True, stable=True).indices[:, :k]
+    bad = (lse.isnan() | (lse == float("-inf"))).unsqueeze(-1)
+    rest = _ref_lse(x.scatter(1, ids, float("-inf"))) - lse
+    top = x.gather(1, ids)
+    ids = ids.masked_fill(bad | (top == float("-inf")), -1)
+    logp, entropy = logprob_entropy_from_logits_ref(logits, labels if labels is not None else ids.new_zeros(x.shape[0]), mask_bits, inv_temp)
+    return TopLogprobs(torch.where(bad, lse.unsqueeze(-1), top - lse.unsqueeze(-1)), ids, torch.where(bad.squeeze(-1), lse, rest), entropy,
+                       logp if labels is not None else None)
+
+
+def top_logprobs_from_logits(logits, k: int, labels=None, mask_bits=None, inv_temp: float = 1.0) -> TopLogprobs:
+    """The k most likely tokens of every row of logits [T, V], the log of the others' mass, the entropy and, with `labels`, their
+    log-probabilities: one read of the logits.  No gradients.  What `distill_loss_from_logits` takes as its teacher.  k is at most
+    min(V, 1024); -0 counts as 0; masked tokens are no alternatives; labels as in `logprob_entropy_from_logits`."""
+    op = "top_logprobs_from_logits"
+    _check_rows(op, logits, inv_temp, labels=labels, mask_bits=mask_bits)
+    _check_labels(op, labels)
+    _check_mask(op, mask_bits, logits.shape[1])
+    if not 1 <= k <= min(logits.shape[1], 1024):
+        raise ValueError(f"{op}: between 1 and min(vocabulary, 1024) alternatives, not {k}")
+    logits = logits.detach()
+    if not use_native(logits):
+        return top_logprobs_from_logits_ref(logits, k, labels, mask_bits, inv_temp)
+    r = lib().top_logprobs(_unit_rows(logits), k, labels.long().contiguous() if labels is not None else None,
+                           mask_bits.contiguous() if mask_bits is not None else None, inv_temp)
+    return TopLogprobs(r[0], r[1], r[2], r[3], r[4] if labels is not None else None)
+
+
+def distill_loss_from_logits_ref(logits, top_ids, top_logp, rest_logp=None, reverse: bool = False, inv_temp: float = 1.0):
+    x = _ref_logits(logits, None, inv_temp)
+    V, ids, inf = x.shape[1], top_ids.long(), float("inf")
+    again = ((ids.unsqueeze(2) == ids.unsqueeze(1)) & torch.ones(ids.shape[1], ids.shape[1], dtype=torch.bool, device=ids.device).tril(-1)).any(-1)
+    used = (ids >= 0) & (ids < V) & ~again
+    at = ids.clamp(0, V - 1)
+    listed = torch.zeros_like(x, dtype=torch.int32).scatter_add_(1, at, used.int()) > 0
+    lse, lse_rest = _ref_lse(x), _ref_lse(x.masked_fill(listed, -inf))
+    y = torch.cat([x.gather(1, at).masked_fill(~used, -inf), lse_rest.unsqueeze(-1)], 1) - lse.masked_fill(lse == -inf, 0.0).unsqueeze(-1)
+    t = top_logp.to(x.dtype).masked_fill(~used, -inf)
+    if rest_logp is None:
+        lt = _ref_lse(t)
+        t = torch.cat([t - lt.masked_fill(lt == -inf, 0.0).unsqueeze(-1), torch.full_like(lt, -inf).unsqueeze(-1)], 1)
+    else:
+        t = torch.cat([t, rest_logp.to(x.dtype).unsqueeze(-1)], 1)
+    w, f = (torch.exp(y), y - t) if reverse else (torch.exp(t), t - y)
+    nothing = w == 0
+    loss = (w.masked_fill(nothing, 0.0) * f.masked_fill(nothing, 0.0)).sum(-1)
+    return loss.masked_fill((ids >= V).any(-1) | lse.isnan(), float("nan"))
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_ids, top_logp, rest_logp, reverse, inv_temp):
+        loss, *saved = lib().distill_fwd(logits, top_ids, top_logp, rest_logp, reverse, inv_temp, True)
+        ctx.save_for_backward(logits, *saved)
+        ctx.inv_temp = inv_temp
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return lib().distill_bwd(*ctx.saved_tensors, _rows_f32(g), ctx.inv_temp, None), None, None, None, None, None
+
+
+def _check_teacher(op: str, T: int, V: int, device, top_ids, top_logp, rest_logp, reverse):
+    _check_row_values(op, T, device, top_ids=top_ids, top_logp=top_logp, rest_logp=rest_logp)
+    if top_ids.dim() != 2 or top_ids.shape != top_logp.shape or not 1 <= top_ids.shape[1] <= 1024:
+        raise ValueError(f"{op}: the teacher's tokens and their log-probabilities are matrices [rows, 1 .. 1024], not {tuple(top_ids.shape)} and "
+                         f"{tuple(top_logp.shape)}")
+    if rest_logp is not None and rest_logp.dim() != 1:
+        raise ValueError(f"{op}: the rest's log-probability is a vector")
+    if reverse and rest_logp is None:
+        raise ValueError(f"{op}: the reverse divergence needs the teacher's rest (a token that the teacher gives nothing costs infinitely much)")
+    if V > 1 << 20:
+        raise ValueError(f"{op}: a vocabulary of at most {1 << 20} tokens, not {V}")
+    if any(t is not None and t.requires_grad for t in (top_logp, rest_logp)) and torch.is_grad_enabled():
+        raise ValueError(f"{op}: the teacher's log-probabilities get no gradient (detach them)")
+
+
+def distill_loss_from_logits(logits, top_ids, top_logp, rest_logp=None, reverse: bool = False, inv_temp: float = 1.0):
+    """Divergence per row between a teacher known by its most likely tokens (`top_logprobs_from_logits`: ids [T, k], log-probabilities
+    [T, k], the others' log-mass [T]) and p = softmax(logits * inv_temp), fp32 [T], differentiable in the logits.  The k tokens are one outcome
+    each, all others together one more; without `rest_logp` the teacher is renormalised over its k tokens.  `reverse` False:
+    KL(teacher || p); True: KL(p || teacher), which needs `rest_logp`.  A negative id is an unused place, an id given again counts where it stands
+    first, an id of V or more makes the loss NaN.  A row whose incoming gradient is 0 gets zeros, whatever it holds."""
+    op = "distill_loss_from_logits"
+    _check_rows(op, logits, inv_temp)
+    _check_teacher(op, logits.shape[0], logits.shape[1], logits.device, top_ids, top_logp, rest_logp, reverse)
+    if not use_native(logits):
+        return distill_loss_from_logits_ref(logits, top_ids, top_logp, rest_logp, reverse, inv_temp)
+    logits, ids, t, tr = _unit_rows(logits), top_ids.long().contiguous(), _rows_f32(top_logp), _rows_f32(rest_logp)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _Distill.apply(logits, ids, t, tr, bool(reverse), float(inv_temp))
+    return lib().distill_fwd(logits.detach(), ids, t, tr, bool(reverse), float(inv_temp), False)[0]
+
+
+# ---- the same through the LM head: no [T, V] logits beyond a chunk of rows
+
+
+def _head_gemm(h, w):
+    """The tcgen05 GEMM module when it takes the head's three products as they are (any number of rows and tokens), else None."""
+    if not h.is_cuda or gemm_impl() is None or h.dtype not in (torch.bfloat16, torch.float16) or w.dtype != h.dtype:
+        return None
+    from realhf_b200.ops import gemm as G
+    ok = gemm_impl() is G.linear and h.shape[1] % 8 == 0 and w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0
+    return G if ok else None
+
+
+def _pitched(rows: int, cols: int, dtype, device):
+    """[rows, cols] with rows a multiple of 8 elements apart, as a TMA descriptor wants them."""
+    return torch.empty(rows, -(-cols // 8) * 8, dtype=dtype, device=device)[:, :cols]
+
+
+def _head_logits(h, w):
+    """fp32 logits of the head: 16-bit operands keep the accumulator, others multiply in fp32."""
+    G = _head_gemm(h, w)
+    if G is None:
+        return h.float() @ w.float().t()
+    return G.gemm(G.tma_rows(h), w, out=_pitched(h.shape[0], w.shape[0], torch.float32, h.device))
+
+
+def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
+    """(d hidden, d weight) of a head whose rows [s, e) have the logits' gradient dlogits_of(s, e), of the hidden states' type."""
+    T = hidden.shape[0]
+    dh = torch.empty_like(hidden, memory_format=torch.contiguous_format) if needs[0] else None
+    G = _head_gemm(hidden, weight)
+    dw = whole = None
+    if needs[1]:
+        mg = getattr(weight, "main_grad", None)
+        if G is not None and mg is None and T <= chunk and getattr(weight, "_grad_in_flat_buffer", False) and weight.grad is not None \
+                and weight.grad.dtype == weight.dtype:
+            dw = weight.grad
+        elif G is not None and mg is not None and mg.dtype == torch.float32:
+            dw = mg
+        elif G is None or T > chunk or T == 0:
+            dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device)
+    for s in range(0, T, chunk):
+        e = min(T, s + chunk)
+        d = dlogits_of(s, e)
+        if G is None:
+            if dh is not None:
+                dh[s:e] = (d.float() @ weight.float()).to(dh.dtype)
+            if dw is not None:
+                dw += d.float().t() @ hidden[s:e].float()
+            continue
+        if dh is not None:
+            G.gemm(d, weight, out=dh[s:e], b_mn=True)                                        # [t, V] x [V, H]
+        if needs[1]:
+            h = G.tma_rows(hidden[s:e])
+            if dw is None:
+                whole = G.gemm(d, h, a_mn=True, b_mn=True)                                   # [t, V]^T x [t, H], rounded once
+            else:
+                G.gemm(d, h, out=dw.view(weight.shape), a_mn=True, b_mn=True, accumulate=True)
+    if dw is not None and dw is not getattr(weight, "main_grad", None) and dw is not weight.grad:
+        whole = dw.to(weight.dtype)
+    return dh, whole
+
+
+class _LMHeadTokenStats(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, mask_bits, inv_temp, chunk):
+        ctx.set_materialize_grads(False)
+        T = hidden.shape[0]
+        logp, entropy, lse = (torch.empty(T, dtype=torch.float32, device=hidden.device) for _ in range(3))
+        for s in range(0, T, chunk):
+            e = min(T, s + chunk)
+            logp[s:e], entropy[s:e], lse[s:e] = lib().token_stats(_head_logits(hidden[s:e], weight), labels[s:e], None if mask_bits is None else mask_bits[s:e],
+                                                                  inv_temp)
+        ctx.save_for_backward(hidden, weight, labels, mask_bits, lse, entropy)
+        ctx.inv_temp, ctx.chunk = inv_temp, chunk
+        return logp, entropy
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy):
+        hidden, weight, labels, mask_bits, lse, entropy = ctx.saved_tensors
+        if g_logp is None and g_entropy is None:
+            return (None,) * 6
+        gl, ge = _rows_f32(g_logp), _rows_f32(g_entropy)
+
+        def dlogits(s, e):
+            x = _head_logits(hidden[s:e], weight)
+            lib().token_stats_bwd(x, labels[s:e], None if mask_bits is None else mask_bits[s:e], lse[s:e], entropy[s:e], None if gl is None else gl[s:e],
+                                  None if ge is None else ge[s:e], ctx.inv_temp, x)
+            return _pitched(e - s, x.shape[1], hidden.dtype, x.device).copy_(x)
+
+        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None)
+
+
+def _check_head(op: str, hidden, weight, temperature, chunk, **rows):
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1] or weight.shape[0] == 0:
+        raise ValueError(f"{op}: hidden states [T, H] and a head [V, H], not {tuple(hidden.shape)} and {tuple(weight.shape)}")
+    if hidden.dtype != weight.dtype or hidden.device != weight.device:
+        raise ValueError(f"{op}: hidden states and head of one type and device, not {hidden.dtype} on {hidden.device} and {weight.dtype} on {weight.device}")
+    if not temperature > 0 or chunk < 1:
+        raise ValueError(f"{op}: the temperature is positive and a chunk one row at least")
+    _check_row_values(op, hidden.shape[0], hidden.device, **rows)
+    _check_mask(op, rows.get("mask_bits"), weight.shape[0])
+
+
+def lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits=None, temperature: float = 1.0):
+    return logprob_entropy_from_logits_ref(hidden.float() @ weight.float().t(), labels, mask_bits, 1.0 / temperature)
+
+
+def lm_head_logprobs_entropy(hidden, weight, labels, mask_bits=None, temperature: float = 1.0, chunk: int = 8192):
+    """(log p(label), entropy) of p = softmax(hidden @ weight^T / temperature): hidden [T, H], weight [V, H], labels [T] -> fp32 [T] each,
+    differentiable in hidden and weight.  Logits stay in fp32 (`lm_head_logprobs` rounds them to the weights' type) and their gradient
+    exists for `chunk` rows at a time.  Labels and mask as in `logprob_entropy_from_logits`."""
+    op = "lm_head_logprobs_entropy"
+    _check_head(op, hidden, weight, temperature, chunk, labels=labels, mask_bits=mask_bits)
+    _check_labels(op, labels)
+    if not use_native(hidden):
+        return lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits, temperature)
+    return _LMHeadTokenStats.apply(hidden, weight, labels.long().contiguous(), mask_bits.contiguous() if mask_bits is not None else None, 1.0 / temperature,
+                                   int(chunk))
+
+
+def lm_head_top_logprobs(hidden, weight, k: int, labels=None, mask_bits=None, temperature: float = 1.0, chunk: int = 4096) -> TopLogprobs:
+    """`top_logprobs_from_logits` of hidden @ weight^T / temperature, `chunk` rows at a time: what a teacher's inference keeps.  No gradients."""
+    op = "lm_head_top_logprobs"
+    _check_head(op, hidden, weight, temperature, chunk, labels=labels, mask_bits=mask_bits)
+    parts, cut = [], lambda t, s: None if t is None else t[s: s + chunk]
+    for s in range(0, max(1, hidden.shape[0]), chunk):
+        parts.append(top_logprobs_from_logits(_head_logits(hidden.detach()[s: s + chunk], weight.detach()), k, cut(labels, s), cut(mask_bits, s),
+                                              1.0 / temperature))
+    return parts[0] if len(parts) == 1 else TopLogprobs(*(None if p[0] is None else torch.cat(p) for p in zip(*parts)))
+
+
+class _LMHeadDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, t, tr, reverse, inv_temp, chunk):
+        need, T = any(ctx.needs_input_grad[:2]), hidden.shape[0]
+        parts = []
+        for s in range(0, max(1, T), chunk):
+            e = min(T, s + chunk)
+            parts.append(lib().distill_fwd(_head_logits(hidden[s:e], weight), ids[s:e], t[s:e], None if tr is None else tr[s:e], reverse, inv_temp, need))
+        loss, *saved = parts[0] if len(parts) == 1 else [torch.cat(p) for p in zip(*parts)]
+        if need:
+            ctx.save_for_backward(hidden, weight, *saved)
+            ctx.inv_temp, ctx.chunk = inv_temp, chunk
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        hidden, weight, lse_rest, g_rest, g_listed, ids = ctx.saved_tensors
+        g = _rows_f32(g)
+
+        def dlogits(s, e):
+            x = _head_logits(hidden[s:e], weight)
+            lib().distill_bwd(x, lse_rest[s:e], g_rest[s:e], g_listed[s:e], ids[s:e], g[s:e], ctx.inv_temp, x)
+            return _pitched(e - s, x.shape[1], hidden.dtype, x.device).copy_(x)
+
+        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None, None, None)
+
+
+def lm_head_distill_loss(hidden, weight, top_ids, top_logp, rest_logp=None, reverse: bool = False, temperature: float = 1.0, chunk: int = 4096):
+    """`distill_loss_from_logits` of hidden @ weight^T / temperature, differentiable in hidden and weight; fp32 logits and their gradient
+    exist for `chunk` rows at a time."""
+    op = "lm_head_distill_loss"
+    _check_head(op, hidden, weight, temperature, chunk)
+    _check_teacher(op, hidden.shape[0], weight.shape[0], hidden.device, top_ids, top_logp, rest_logp, reverse)
+    if not use_native(hidden):
+        return distill_loss_from_logits_ref(hidden.float() @ weight.float().t(), top_ids, top_logp, rest_logp, reverse, 1.0 / temperature)
+    return _LMHeadDistill.apply(hidden, weight, top_ids.long().contiguous(), _rows_f32(top_logp), _rows_f32(rest_logp), bool(reverse), 1.0 / temperature,
+                                int(chunk))
 
 
 # ------------------------------------------------------------------------------------------------ GEMM
