@@ -13,9 +13,10 @@
 
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kMaxListed = 1024;
 constexpr int kBwdThreads = 256, kBwdVecs = 4;
+
+__host__ __device__ constexpr int bitmap_words(int V) { return (V + 16 + 31) / 32; }
 
 struct DistillShared {
   float red[96];
@@ -26,17 +27,19 @@ struct DistillShared {
 
 RB_DEVICE float block_sum(float v, float* red) { return rb::block_reduce<false>(v, red); }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const T* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ ids,
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_fwd_kernel(const T* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ ids,
                                                                const float* __restrict__ top_logp, const float* __restrict__ rest_logp, int reverse,
                                                                float* __restrict__ loss, float* __restrict__ lse_rest_out, float* __restrict__ grad_rest,
                                                                float* __restrict__ grad_listed, int* __restrict__ ids_out, int V, int k, float inv_temp) {
   __shared__ DistillShared sh;
-  extern __shared__ uint32_t listed[];                  // a bit a token
+  constexpr int VEC = rb::RowSpan<T>::VEC;
+  extern __shared__ uint32_t listed[];                  // a bit a token: bit 8 + j - head, so that a 16-byte piece's bits lie in one byte
   const int64_t row = blockIdx.x;
   const T* lr = logits + row * row_stride;
   const float kk = inv_temp * rb::kLog2e;
-  for (int i = threadIdx.x; i < RB_CEIL_DIV(V, 32); i += kThreads) listed[i] = 0;
+  const rb::RowSpan<T> span(lr, V);
+  for (int i = threadIdx.x; i < bitmap_words(V); i += kThreads) listed[i] = 0;
   if (threadIdx.x == 0) sh.dup = 0;
   __syncthreads();
   bool beyond = false;
@@ -47,7 +50,8 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const T* __restri
     sh.ids[i] = ok ? (int)id : -1;
     sh.t[i] = ok ? top_logp[row * k + i] : -INFINITY;
     sh.y[i] = ok ? rb::to_f(lr[id]) * inv_temp : -INFINITY;
-    if (ok && (atomicOr(&listed[id >> 5], 1u << (id & 31)) >> (id & 31)) & 1) sh.dup = 1;
+    const int bit = ok ? 8 + (int)id - span.head : 0;
+    if (ok && (atomicOr(&listed[bit >> 5], 1u << (bit & 31)) >> (bit & 31)) & 1) sh.dup = 1;
   }
   beyond = __syncthreads_or(beyond);
   if (sh.dup) {                                         // the first place of an id stands
@@ -60,9 +64,19 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const T* __restri
     __syncthreads();
   }
   // the row: every unlisted token's part of the rest
-  rb::RowStats others;
-  for (int j = threadIdx.x; j < V; j += kThreads)
-    if (!((listed[j >> 5] >> (j & 31)) & 1)) others.one(rb::to_f(lr[j]), kk);
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(listed);
+  rb::RunningStats<T, false> run;
+  rb::walk_groups<T, kThreads>(
+      lr + span.head, span.nvec,
+      [&](int4 v, int i) {
+        if (i >= span.nvec) return v;
+        const uint32_t gone = VEC == 8 ? bytes[1 + i] : bytes[1 + (i >> 1)] >> ((i & 1) * 4) & 15;
+        return gone ? rb::mask_piece<T>(v, gone) : v;
+      },
+      [&](const int4 (&raw)[rb::kPieces], int, bool) { run.add(raw, kk, false); });
+  rb::RowStats others = run.stats();
+  const int ej = span.edge(threadIdx.x, V);
+  if (ej >= 0 && !((listed[(8 + ej - span.head) >> 5] >> ((8 + ej - span.head) & 31)) & 1)) others.one(rb::to_f(lr[ej]), kk);
   others = rb::block_stats(others, kk, sh.red);
   const bool rest_empty = others.m == -INFINITY;
   const float lse_rest = others.m < INFINITY ? (rest_empty ? -INFINITY : fmaf(others.m, inv_temp, logf(others.s))) : NAN;
@@ -175,15 +189,18 @@ int rb_distill_fwd(const void* logits, int64_t row_stride, const int64_t* ids, c
                    float* lse_rest, float* grad_rest, float* grad_listed, int* ids_out, int64_t rows, int V, int k, float inv_temp, int dt, cudaStream_t s) {
   if (rows == 0) return 0;
   if (k < 0 || k > kMaxListed || V > rb_distill_max_vocab() || (reverse && !rest_logp)) return -1;
-  const int smem = RB_CEIL_DIV(V, 32) * 4;
-#define RB_L(T)                                                                                                                                     \
-  {                                                                                                                                                 \
-    if (smem > 32768 && cudaFuncSetAttribute(distill_fwd_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2;     \
-    distill_fwd_kernel<T><<<(unsigned)rows, kThreads, smem, s>>>((const T*)logits, row_stride, ids, top_logp, rest_logp, reverse, loss, lse_rest,     \
-                                                                 grad_rest, grad_listed, ids_out, V, k, inv_temp);                                   \
+  const int smem = bitmap_words(V) * 4;
+  const int nt = rb::row_threads(rows, V / (dt == 0 ? 4 : 8));
+#define RB_L2(T, NT)                                                                                                                                       \
+  {                                                                                                                                                        \
+    if (smem > 32768 && cudaFuncSetAttribute(distill_fwd_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2;       \
+    distill_fwd_kernel<T, NT><<<(unsigned)rows, NT, smem, s>>>((const T*)logits, row_stride, ids, top_logp, rest_logp, reverse, loss, lse_rest, grad_rest,  \
+                                                               grad_listed, ids_out, V, k, inv_temp);                                                       \
   }
-  if (dt == 0) RB_L(float) else if (dt == 1) RB_L(__nv_bfloat16) else if (dt == 2) RB_L(__half) else return -1;
+#define RB_L(T) if (nt == 32) RB_L2(T, 32) else if (nt == 128) RB_L2(T, 128) else if (nt == 256) RB_L2(T, 256) else RB_L2(T, 512)
+  if (dt == 0) { RB_L(float) } else if (dt == 1) { RB_L(__nv_bfloat16) } else if (dt == 2) { RB_L(__half) } else return -1;
 #undef RB_L
+#undef RB_L2
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

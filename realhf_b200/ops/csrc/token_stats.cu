@@ -7,13 +7,13 @@
 
 namespace {
 
-constexpr int kThreads = 512, kUnroll = 4;
 constexpr int kBwdThreads = 256, kBwdVecs = 4;
 
-template <typename T, bool kMask>
-__global__ void __launch_bounds__(kThreads) token_stats_kernel(const T* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ labels,
-                                                               const uint8_t* __restrict__ mask, int64_t mask_stride, float* __restrict__ logp,
-                                                               float* __restrict__ entropy, float* __restrict__ lse, int V, float inv_temp) {
+template <typename T, bool kMask, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_stats_kernel(const T* __restrict__ logits, int64_t row_stride,
+                                                                                const int64_t* __restrict__ labels, const uint8_t* __restrict__ mask,
+                                                                                int64_t mask_stride, float* __restrict__ logp, float* __restrict__ entropy,
+                                                                                float* __restrict__ lse, int V, float inv_temp) {
   constexpr int VEC = rb::RowSpan<T>::VEC;
   __shared__ float red[96];
   const int64_t row = blockIdx.x;
@@ -21,27 +21,15 @@ __global__ void __launch_bounds__(kThreads) token_stats_kernel(const T* __restri
   const uint8_t* mr = kMask ? mask + row * mask_stride : nullptr;
   const float k = inv_temp * rb::kLog2e;
   const rb::RowSpan<T> span(lr, V);
-  const rb::Pack<T, VEC>* vecs = reinterpret_cast<const rb::Pack<T, VEC>*>(lr + span.head);
-  rb::RowStats st;
-  for (int i0 = threadIdx.x; i0 < span.nvec; i0 += kThreads * kUnroll) {
-    float x[kUnroll * VEC];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int i = i0 + u * kThreads;
-      if (i < span.nvec) {
-        const rb::Pack<T, VEC> p = vecs[i];
-        const uint32_t gone = kMask ? rb::mask8(mr, mask_stride, span.head + i * VEC) : 0u;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[u * VEC + e] = (gone >> e) & 1 ? -INFINITY : rb::to_f(p.v[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[u * VEC + e] = -INFINITY;
-      }
-    }
-    float m, s, w;
-    rb::group_stats(x, k, m, s, w);
-    st.add(m, s, w, k);
+  rb::RunningStats<T, true> run;
+  auto adjust = [&](int4 v, int i) { return kMask && i < span.nvec ? rb::mask_piece<T>(v, rb::mask8(mr, mask_stride, span.head + i * VEC)) : v; };
+  rb::walk_groups<T, kThreads>(lr + span.head, span.nvec, adjust, [&](const int4 (&raw)[rb::kPieces], int, bool whole) { run.add(raw, k, kMask || !whole); });
+  if (run.again()) {
+    run.sums = rb::Sums();
+    rb::walk_groups<T, kThreads>(lr + span.head, span.nvec, adjust,
+                                 [&](const int4 (&raw)[rb::kPieces], int, bool) { rb::group_add<T, true, true>(raw, run.m, k, run.sums); });
   }
+  rb::RowStats st = run.stats();
   const int j = span.edge(threadIdx.x, V);
   if (j >= 0 && !(kMask && (mr[j >> 3] >> (j & 7)) & 1)) st.one(rb::to_f(lr[j]), k);
   st = rb::block_stats(st, k, red);
@@ -115,8 +103,10 @@ extern "C" {
 int rb_token_stats(const void* logits, int64_t row_stride, const int64_t* labels, const uint8_t* mask, int64_t mask_stride, float* logp, float* entropy,
                    float* lse, int64_t rows, int V, float inv_temp, int dt, cudaStream_t s) {
   if (rows == 0) return 0;
-#define RB_L2(T, M) token_stats_kernel<T, M><<<(unsigned)rows, kThreads, 0, s>>>((const T*)logits, row_stride, labels, mask, mask_stride, logp, entropy, lse, V, inv_temp)
-#define RB_L(T) if (mask) RB_L2(T, true); else RB_L2(T, false)
+  const int nt = rb::row_threads(rows, V / (dt == 0 ? 4 : 8));
+#define RB_L3(T, M, NT) token_stats_kernel<T, M, NT><<<(unsigned)rows, NT, 0, s>>>((const T*)logits, row_stride, labels, mask, mask_stride, logp, entropy, lse, V, inv_temp);
+#define RB_L2(T, M) if (nt == 32) RB_L3(T, M, 32) else if (nt == 128) RB_L3(T, M, 128) else if (nt == 256) RB_L3(T, M, 256) else RB_L3(T, M, 512)
+#define RB_L(T) if (mask) { RB_L2(T, true) } else { RB_L2(T, false) }
   if (dt == 0) { RB_L(float); } else if (dt == 1) { RB_L(__nv_bfloat16); } else if (dt == 2) { RB_L(__half); } else return -1;
 #undef RB_L
 #undef RB_L2

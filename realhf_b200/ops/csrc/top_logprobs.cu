@@ -5,14 +5,21 @@
 // token fills holds id -1 and -inf.  The rest's mass is summed over the tokens it consists of: 1 - sum of the chosen would cancel where they
 // hold nearly all of it.
 //
-// The k-th largest value by a radix descent over its bits (four digits of 8 bits, a histogram in shared memory each), the elements above it in any order, of
-// those equal to it the first in index order, sorted by (value, index).
+// The row is read once.  Every thread keeps the maximum and the sum of each of its groups (vocab_rows.cuh) in shared memory.  The k-th largest of the
+// maxima of 512 shares of the row, to 16 bits, is a lower bound of the k-th largest logit: k shares hold an element at least as large; only some k .. 2 k elements
+// reach it.  The groups whose maximum does are looked at again, a lane a piece, and give the candidates; the mass of the rest is what these groups leave plus the sums
+// of all others.  A candidate's place is the number of candidates before it in the order: counted among all of them where they are few, else among those of its
+// bucket, 512 equal intervals of the value (a bitonic sort of 128, a barrier for each of its 28 stages, took 7400 cycles; counting among 400 by 128 threads 28000).
+// More than 256 alternatives, more than 1024 groups or candidates at the bound (ties), and rows of more than 12288 groups take a radix descent instead:
+// the k-th largest value by its bits (four digits of 8 bits, a histogram in shared memory each), the elements above it in any order, of those equal to it the
+// first in index order.
+// Sums have a fixed order whichever way candidates arrive.
 #include "vocab_rows.cuh"
 
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kMaxTop = 1024;
+constexpr int kShares = 512;
 
 RB_DEVICE uint32_t order_key(float x) {  // order-preserving float -> uint, -0 as 0
   const uint32_t u = __float_as_uint(x + 0.f);
@@ -21,12 +28,22 @@ RB_DEVICE uint32_t order_key(float x) {  // order-preserving float -> uint, -0 a
 RB_DEVICE float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 constexpr uint32_t kKeyNone = 0x007fffffu;  // order_key(-inf)
 
+constexpr int kFastTop = 256, kMaxRecords = 12288;
+
 struct TopShared {
   float red[96];
-  uint32_t hist[256];
-  uint32_t warp_n[kThreads / 32];
-  uint32_t digit, above, count;
-  uint64_t list[kMaxTop];   // key << 32 | ~index: descending order is the order wanted
+  union {
+    uint32_t hist[kShares];
+    uint32_t keys[kShares];
+  };
+  uint32_t warp_n[32];
+  uint32_t digit, above, count, selected, kth;
+  int last;
+  alignas(16) uint64_t list[kMaxTop];   // key << 32 | ~index: descending order is the order wanted
+  union {
+    uint16_t group[kMaxTop];            // groups to look at again: number * threads + thread
+    uint64_t ordered[kMaxTop];          // the list by buckets
+  };
 };
 
 template <typename T> struct TopRow {
@@ -37,8 +54,8 @@ template <typename T> struct TopRow {
 };
 
 // The k largest (key, ~index) of the row -> sh.list in any order; returns how many there are (less than k where the row keeps fewer tokens), and in
-// `kth` / `last` the smallest chosen value's key and the highest index that is chosen among those equal to it.
-template <typename T> RB_DEVICE int select_radix(const TopRow<T>& r, int k, TopShared& sh, uint32_t& kth, int& last) {
+// sh.kth the k-th largest value's key.
+template <int kThreads, typename T> RB_DEVICE int select_radix(const TopRow<T>& r, int k, TopShared& sh) {
   uint32_t prefix = 0, want = k;      // the want-th largest among the elements whose high digits are `prefix`
   for (int shift = 24; shift >= 0; shift -= 8) {
     for (int b = threadIdx.x; b < 256; b += kThreads) sh.hist[b] = 0;
@@ -60,9 +77,11 @@ template <typename T> RB_DEVICE int select_radix(const TopRow<T>& r, int k, TopS
     want = sh.above;
     __syncthreads();
   }
-  kth = prefix;
-  last = -1;
-  if (threadIdx.x == 0) sh.count = 0;
+  const uint32_t kth = prefix;
+  if (threadIdx.x == 0) {
+    sh.count = 0;
+    sh.kth = max(kth, kKeyNone);
+  }
   __syncthreads();
   for (int j = threadIdx.x; j < r.V; j += kThreads) {
     const uint32_t key = order_key(r.at(j));
@@ -86,33 +105,104 @@ template <typename T> RB_DEVICE int select_radix(const TopRow<T>& r, int k, TopS
       all += n;
     }
     at += __popc(b & ((1u << lane) - 1u));
-    if (hit && at < need) {
-      sh.list[above + at] = (uint64_t)kth << 32 | (uint32_t)~j;
-      if (at == need - 1) sh.digit = j;
-    }
+    if (hit && at < need) sh.list[above + at] = (uint64_t)kth << 32 | (uint32_t)~j;
     found += all;
     __syncthreads();
   }
-  if (need > 0) last = (int)sh.digit;
   return above + need;
 }
 
-template <typename T, bool kMask>
-__global__ void __launch_bounds__(kThreads) top_logprobs_kernel(const T* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ labels,
-                                                                const uint8_t* __restrict__ mask, int64_t mask_stride, float* __restrict__ logp,
-                                                                float* __restrict__ entropy, float* __restrict__ top_logp, int64_t* __restrict__ top_ids,
-                                                                float* __restrict__ rest, int V, int k, float inv_temp) {
+// The largest t, to the upper 16 bits of a key, that at least k of the shares' keys reach; by warp 0, N keys a lane (kShares / 32 / N shares taken together:
+// k of the fewer and larger ones bound as well while k is a quarter of them at most).  Only the bits in which the keys differ are searched.
+template <int N> RB_DEVICE uint32_t bound_of(int k, const uint32_t* keys) {
+  uint32_t key[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    key[i] = 0;
+#pragma unroll
+    for (int e = 0; e < kShares / 32 / N; ++e) key[i] = max(key[i], keys[(e * N + i) * 32 + threadIdx.x] >> 16);
+  }
+  uint32_t hi = 0, lo = ~0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    hi = max(hi, key[i]);
+    lo = min(lo, key[i]);
+  }
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  const int bits = 32 - __clz(hi ^ lo);
+  uint32_t t = hi >> bits << bits;
+#pragma unroll 1
+  for (int bit = bits - 1; bit >= 0; --bit) {
+    const uint32_t c = t | 1u << bit;
+    int n[2] = {};
+#pragma unroll
+    for (int i = 0; i < N; ++i) n[i & 1] += key[i] >= c;
+    if (__reduce_add_sync(0xffffffffu, n[0] + n[1]) >= k) t = c;
+  }
+  return t << 16;
+}
+
+// how many of list[0, n) are larger than `mine`; the list is padded with zeros to an even number
+RB_DEVICE int larger_than(uint64_t mine, const uint64_t* list, int n) {
+  int rank = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; i += 2) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(list + i);
+    rank += v.x > mine;
+    rank += v.y > mine;
+  }
+  return rank;
+}
+
+template <typename T, bool kMask, int kThreads, int P>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel(const T* __restrict__ logits, int64_t row_stride,
+                                                                                 const int64_t* __restrict__ labels, const uint8_t* __restrict__ mask,
+                                                                                 int64_t mask_stride, float* __restrict__ logp, float* __restrict__ entropy,
+                                                                                 float* __restrict__ top_logp, int64_t* __restrict__ top_ids,
+                                                                                 float* __restrict__ rest, int V, int k, float inv_temp, int records) {
+  constexpr int VEC = rb::RowSpan<T>::VEC, kStep = P * kThreads;
   __shared__ TopShared sh;
+  extern __shared__ float2 rec[];           // [group][thread]: maximum and sum
   const int64_t row = blockIdx.x;
   const TopRow<T> r{logits + row * row_stride, kMask ? mask + row * mask_stride : nullptr, V};
   const float kk = inv_temp * rb::kLog2e;
-  rb::RowStats st;
-  for (int j = threadIdx.x; j < V; j += kThreads) st.one(r.at(j), kk);
+  const rb::RowSpan<T> span(r.lr, V);
+  const int lane = threadIdx.x & 31;
+  const bool fast = records > 0;
+  rb::RunningStats<T, true> run;
+  auto adjust = [&](int4 v, int i) { return kMask && i < span.nvec ? rb::mask_piece<T>(v, rb::mask8(r.mr, mask_stride, span.head + i * VEC)) : v; };
+  rb::walk_groups<T, kThreads, P>(r.lr + span.head, span.nvec, adjust, [&](const int4 (&raw)[P], int i0, bool whole) {
+    const float mg = rb::group_max<T>(raw);
+    run.raise(mg, kk);
+    rb::Sums g;
+    if (kMask || !whole) rb::group_add<T, true, true>(raw, run.reference(), kk, g);
+    else rb::group_add<T, true, false>(raw, run.reference(), kk, g);
+    run.sums.s2 = rb::add2(run.sums.s2, g.s2);
+    run.sums.w2 = rb::add2(run.sums.w2, g.w2);
+    if (fast) rec[i0 / kStep * kThreads + threadIdx.x] = make_float2(mg, g.s());
+  });
+  if (run.again()) {
+    run.sums.w2 = 0;
+    rb::walk_groups<T, kThreads, P>(r.lr + span.head, span.nvec, adjust, [&](const int4 (&raw)[P], int, bool) {
+      rb::Sums g;
+      rb::group_add<T, true, true>(raw, run.m, kk, g);
+      run.sums.w2 = rb::add2(run.sums.w2, g.w2);
+    });
+  }
+  rb::RowStats st = run.stats();
+  const int ej = span.edge(threadIdx.x, V);
+  const float ex = ej >= 0 ? r.at(ej) : -INFINITY;
+  st.one(ex, kk);
+  const int groups = RB_CEIL_DIV(max(0, span.nvec - (int)threadIdx.x), kStep);
   st = rb::block_stats(st, kk, sh.red);
   const rb::RowResult res(st, inv_temp);
   if (threadIdx.x == 0) {
     entropy[row] = res.entropy;
     if (logp) logp[row] = rb::label_logp(r.lr, labels[row], r.mr, V, inv_temp, res.lse);
+    sh.count = sh.selected = 0;
+    sh.kth = kKeyNone;      // where fewer than k tokens are kept there is no rest
+    sh.last = V;
   }
   if (!(fabsf(res.lse) < INFINITY)) {     // no softmax, or no token
     for (int i = threadIdx.x; i < k; i += kThreads) {
@@ -122,33 +212,185 @@ __global__ void __launch_bounds__(kThreads) top_logprobs_kernel(const T* __restr
     if (threadIdx.x == 0) rest[row] = res.lse;
     return;
   }
-  uint32_t kth;
-  int last;
-  const int n = select_radix(r, k, sh, kth, last);
-  int size = 1;
-  while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += kThreads) sh.list[i] = 0;
-  __syncthreads();
-  for (int len = 2; len <= size; len <<= 1)
-    for (int d = len >> 1; d > 0; d >>= 1) {
-      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-        const int lo = 2 * d * (i / d) + i % d, hi = lo + d;
-        const uint64_t a = sh.list[lo], b = sh.list[hi];
-        if ((a < b) == ((lo & len) == 0)) { sh.list[lo] = b; sh.list[hi] = a; }
+  float left = 0.f;                         // the rest's sum against the row's maximum
+  int n = kMaxTop + 1;
+  float lowest = 0.f;                       // no candidate lies below
+  if (fast) {
+    // a group's sum was taken against the thread's largest value so far: bring it to the row's; the thread's kShares / kThreads shares: every so many-th group,
+    // the edge with the first
+    constexpr int B = kShares / kThreads;
+    float share[B], so_far = -INFINITY;
+    share[0] = ex;
+#pragma unroll
+    for (int b = 1; b < B; ++b) share[b] = -INFINITY;
+    for (int g0 = 0; g0 < groups; g0 += B) {
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        if (g0 + b < groups) {
+          float2& v = rec[(g0 + b) * kThreads + threadIdx.x];
+          so_far = fmaxf(so_far, v.x);
+          share[b] = fmaxf(share[b], v.x);
+          v.y *= rb::exp2_fast(fmaxf((so_far - st.m) * kk, -1000.f));
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b) sh.keys[b * kThreads + threadIdx.x] = order_key(share[b]);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const uint32_t t = k <= 32 ? bound_of<4>(k, sh.keys) : bound_of<kShares / 32>(k, sh.keys);
+      if (threadIdx.x == 0) sh.digit = max(t, kKeyNone + 1);
+    }
+    __syncthreads();
+    const float bound_x = lowest = key_value(sh.digit);
+    // places in `group` or `list` for the bits set in a lane's mask: one addition a warp
+    auto places = [&](uint32_t hits, uint32_t& count) {
+      const int mine = __popc(hits);
+      int before = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+      }
+      uint32_t at = 0;
+      if (lane == 31 && before) at = atomicAdd(&count, (uint32_t)before);
+      return __shfl_sync(0xffffffffu, at, 31) + before - mine;
+    };
+    const int all_groups = RB_CEIL_DIV(span.nvec, kStep);
+    for (int g0 = 0; g0 < all_groups; g0 += 32) {
+      uint32_t hits = 0;
+      for (int g = g0; g < min(groups, g0 + 32); ++g) hits |= (uint32_t)(rec[g * kThreads + threadIdx.x].x >= bound_x) << (g - g0);
+      uint32_t at = places(hits, sh.selected);
+      for (; hits; hits &= hits - 1, ++at)
+        if (at < kMaxTop) sh.group[at] = (uint16_t)((g0 + __ffs(hits) - 1) * kThreads + threadIdx.x);
+    }
+    if (threadIdx.x < 32) {
+      const uint32_t at = places(ex >= bound_x, sh.count);
+      if (ex >= bound_x) sh.list[at] = (uint64_t)order_key(ex) << 32 | (uint32_t)~ej;
+    }
+    __syncthreads();
+    const int selected = sh.selected;
+    if (selected <= kMaxTop) {
+      // a lane a piece of a chosen group, P lanes a group: the pieces' sums add up in a fixed order
+      for (int q0 = 0; q0 < selected * P; q0 += kThreads) {
+        const int q = q0 + threadIdx.x, u = q % P;
+        const bool on = q < selected * P;
+        const int id = on ? sh.group[q / P] : 0, piece = id / kThreads * kStep + id % kThreads + u * kThreads;
+        uint32_t hits = 0;
+        float s = 0.f;
+        const int j0 = span.head + piece * VEC;
+        if (on && piece < span.nvec) {
+          int4 raw = reinterpret_cast<const int4*>(r.lr + span.head)[piece];
+          if (kMask) raw = rb::mask_piece<T>(raw, rb::mask8(r.mr, mask_stride, j0));
+          const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) {
+            const float x = rb::to_f(e[c]);
+            const bool hit = x >= bound_x;
+            hits |= (uint32_t)hit << c;
+            s += hit ? 0.f : rb::exp2_fast(fmaxf((x - st.m) * kk, -1000.f));
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < P; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        uint32_t at = places(hits, sh.count);
+        for (; hits; hits &= hits - 1, ++at) {
+          const int j = j0 + __ffs(hits) - 1;
+          if (at < kMaxTop) sh.list[at] = (uint64_t)order_key(rb::to_f(r.lr[j])) << 32 | (uint32_t)~j;
+        }
+        if (on && u == 0) rec[id].y = s;
       }
       __syncthreads();
+      n = sh.count;
     }
-  for (int i = threadIdx.x; i < k; i += kThreads) {
-    const uint64_t c = i < n ? sh.list[i] : 0;
-    top_logp[row * k + i] = i < n ? fmaf(key_value((uint32_t)(c >> 32)), inv_temp, -res.lse) : -INFINITY;
-    top_ids[row * k + i] = i < n ? (int64_t)(int)~(uint32_t)c : -1;
+    if (n <= kMaxTop) {
+      for (int g = 0; g < groups; ++g) left += rec[g * kThreads + threadIdx.x].y;
+      if (ex != -INFINITY && !(ex >= bound_x)) left += rb::exp2_fast((ex - st.m) * kk);
+    }
   }
-  // the others: below the k-th value, or equal to it behind the last chosen index
+  const bool listed = n <= kMaxTop;
+  if (!listed) {
+    __syncthreads();
+    n = select_radix<kThreads>(r, k, sh);
+    lowest = key_value(sh.kth);
+    __syncthreads();
+  }
+  auto place = [&](uint64_t c, int at, float* after) {
+    const float x = key_value((uint32_t)(c >> 32));
+    const int j = (int)~(uint32_t)c;
+    if (at < k) {
+      top_logp[row * k + at] = fmaf(x, inv_temp, -res.lse);
+      top_ids[row * k + at] = j;
+      if (at == k - 1) { sh.kth = (uint32_t)(c >> 32); sh.last = j; }
+    } else {
+      after[at - k] = x;
+    }
+  };
+  float* after;                             // candidates that are not chosen, in order
+  if (n <= 96) {
+    after = reinterpret_cast<float*>(sh.ordered);
+    if (threadIdx.x == 0 && (n & 1)) sh.list[n] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) place(sh.list[i], larger_than(sh.list[i], sh.list, n), after);
+  } else {
+    after = reinterpret_cast<float*>(sh.list);
+    const float width = st.m - lowest, scale = width > 0.f && width < INFINITY ? (kShares - 1) / width : 0.f;
+    auto bucket = [&](uint64_t c) { return min(kShares - 1, (int)((st.m - key_value((uint32_t)(c >> 32))) * scale)); };
+    for (int b = threadIdx.x; b < kShares; b += kThreads) sh.hist[b] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) atomicAdd(&sh.hist[bucket(sh.list[i])], 1u);
+    __syncthreads();
+    if (threadIdx.x < 32) {                 // counts -> where the buckets begin
+      uint32_t c[kShares / 32], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kShares / 32; ++i) {
+        c[i] = sh.hist[lane * (kShares / 32) + i];
+        sum += c[i];
+      }
+      uint32_t before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+      }
+      before -= sum;
+#pragma unroll
+      for (int i = 0; i < kShares / 32; ++i) {
+        sh.hist[lane * (kShares / 32) + i] = before;
+        before += c[i];
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) sh.ordered[atomicAdd(&sh.hist[bucket(sh.list[i])], 1u)] = sh.list[i];
+    __syncthreads();                        // hist: where the buckets end
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const uint64_t c = sh.ordered[i];
+      const int b = bucket(c), begin = b > 0 ? sh.hist[b - 1] : 0, end = sh.hist[b];
+      int at = begin;
+      for (int e = begin; e < end; ++e) at += sh.ordered[e] > c;
+      place(c, at, after);
+    }
+  }
+  for (int i = n + threadIdx.x; i < k; i += kThreads) {
+    top_logp[row * k + i] = -INFINITY;
+    top_ids[row * k + i] = -1;
+  }
+  if (listed && n > k) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < n - k; i += kThreads) left += rb::exp2_fast(fmaxf((after[i] - st.m) * kk, -1000.f));
+  }
+  left = rb::block_reduce<false>(left, sh.red);
+  if (listed && left > 1e-18f) {
+    if (threadIdx.x == 0) rest[row] = logf(left) - logf(st.s);
+    return;
+  }
+  // the others one by one, below the k-th value or equal to it behind the last chosen index: after a descent, and where they are too small beside the largest
+  // logit to be summed against it
   rb::RowStats others;
   for (int j = threadIdx.x; j < V; j += kThreads) {
     const float x = r.at(j);
     const uint32_t key = order_key(x);
-    if (key < kth || (key == kth && j > last)) others.one(x, kk);
+    if (key < sh.kth || (key == sh.kth && j > sh.last)) others.one(x, kk);
   }
   others = rb::block_stats(others, kk, sh.red);
   if (threadIdx.x == 0) rest[row] = rb::RowResult(others, inv_temp).lse - res.lse;
@@ -165,11 +407,28 @@ int rb_top_logprobs(const void* logits, int64_t row_stride, const int64_t* label
                     float* top_logp, int64_t* top_ids, float* rest, int64_t rows, int V, int k, float inv_temp, int dt, cudaStream_t s) {
   if (rows == 0) return 0;
   if (k < 1 || k > kMaxTop || k > V) return -1;
-#define RB_L2(T, M) top_logprobs_kernel<T, M><<<(unsigned)rows, kThreads, 0, s>>>((const T*)logits, row_stride, labels, mask, mask_stride, logp, entropy, top_logp, top_ids, rest, V, k, inv_temp)
-#define RB_L(T) if (mask) RB_L2(T, true); else RB_L2(T, false)
-  if (dt == 0) { RB_L(float); } else if (dt == 1) { RB_L(__nv_bfloat16); } else if (dt == 2) { RB_L(__half); } else return -1;
+  // pieces a group: one where groups of four are too few to bound the k-th logit
+  const int vec = V / (dt == 0 ? 4 : 8), p = vec >= 8 * k ? 4 : 1;
+  // threads: as for the statistics, but no fewer than keep 1024 resident beside what a block has in shared memory, and all of them for few rows
+  const int64_t bytes = sizeof(TopShared) + 1024 + (int64_t)vec / p * 8;
+  const int nt = rows < 4 * rb::kNumSMs ? 512 : bytes <= 45 << 10 ? 128 : 256;
+#define RB_L4(T, M, NT, P)                                                                                                                                 \
+  {                                                                                                                                                        \
+    const int groups = RB_CEIL_DIV(vec, P * NT);                                                                                                           \
+    const bool fast = k <= kFastTop && groups * NT <= kMaxRecords;                                                                                         \
+    const int smem = fast ? groups * NT * (int)sizeof(float2) : 0;                                                                                         \
+    if (smem > 26000 && cudaFuncSetAttribute(top_logprobs_kernel<T, M, NT, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2; \
+    top_logprobs_kernel<T, M, NT, P><<<(unsigned)rows, NT, smem, s>>>((const T*)logits, row_stride, labels, mask, mask_stride, logp, entropy, top_logp,     \
+                                                                      top_ids, rest, V, k, inv_temp, fast ? groups : 0);                                    \
+  }
+#define RB_L3(T, M, NT) if (p == 4) RB_L4(T, M, NT, 4) else RB_L4(T, M, NT, 1)
+#define RB_L2(T, M) if (nt == 128) { RB_L3(T, M, 128) } else if (nt == 256) { RB_L3(T, M, 256) } else { RB_L3(T, M, 512) }
+#define RB_L(T) if (mask) { RB_L2(T, true) } else { RB_L2(T, false) }
+  if (dt == 0) { RB_L(float) } else if (dt == 1) { RB_L(__nv_bfloat16) } else if (dt == 2) { RB_L(__half) } else return -1;
 #undef RB_L
 #undef RB_L2
+#undef RB_L3
+#undef RB_L4
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

@@ -4,6 +4,9 @@
 //   log-sum-exp  lse = M inv_temp + ln S          entropy  H = ln S - ln 2 * W / S
 // S >= 1 and W <= 0, so the entropy is a sum of two terms >= 0 and nothing cancels (lse - sum p x would).  All in fp32.
 // A masked token and a logit of -inf weigh nothing.  A row that holds a NaN or +inf has no softmax: its statistics are NaN.
+//
+// A thread takes the row in groups of four 16-byte pieces (32 16-bit or 16 fp32 logits), the next group's loads on their way while one is worked on.
+// Per 16-bit logit: half an instruction for the maximum (two at once), one to unpack, half each for difference, scale and the two sums (f32x2), one exponential.
 #pragma once
 #include "common.cuh"
 
@@ -21,6 +24,65 @@ RB_DEVICE float max_nan(float a, float b) {  // a NaN wins
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
+RB_DEVICE float warp_max_nan(float v) {
+  float y;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
+  return y;
+}
+
+// two fp32 numbers in one instruction
+RB_DEVICE uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+RB_DEVICE void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+RB_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+RB_DEVICE uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+RB_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// A 32-bit word of a row: two 16-bit logits, or one fp32.
+template <typename T> struct Word;
+template <> struct Word<__nv_bfloat16> {
+  static constexpr int N = 2;
+  static constexpr uint32_t kNone = 0xff80ff80u;  // -inf twice
+  RB_DEVICE static uint32_t max(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  RB_DEVICE static void values(uint32_t a, float& lo, float& hi) { lo = __uint_as_float(a << 16); hi = __uint_as_float(a & 0xffff0000u); }
+};
+template <> struct Word<__half> {
+  static constexpr int N = 2;
+  static constexpr uint32_t kNone = 0xfc00fc00u;
+  RB_DEVICE static uint32_t max(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  RB_DEVICE static void values(uint32_t a, float& lo, float& hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    lo = f.x;
+    hi = f.y;
+  }
+};
+template <> struct Word<float> {
+  static constexpr int N = 1;
+  static constexpr uint32_t kNone = 0xff800000u;
+};
 
 // Where the 16-byte pieces of a row lie: `head` elements before the first 16-byte boundary, `nvec` whole pieces, then the tail.
 template <typename T> struct RowSpan {
@@ -46,6 +108,19 @@ RB_DEVICE uint32_t mask8(const uint8_t* m, int64_t bytes, int j) {
   return b >> (j & 7);
 }
 
+// a 16-byte piece whose elements with a bit set in `gone` become -inf
+template <typename T> RB_DEVICE int4 mask_piece(int4 v, uint32_t gone) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t m;
+    if constexpr (Word<T>::N == 1) m = 0u - ((gone >> i) & 1u);
+    else m = ((gone >> (2 * i)) & 1u) * 0xffffu + ((gone >> (2 * i + 1)) & 1u) * 0xffff0000u;
+    w[i] = (w[i] & ~m) | (Word<T>::kNone & m);
+  }
+  return v;
+}
+
 struct RowStats {
   float m = -INFINITY, s = 0.f, w = 0.f;
   // merge another part of the same row; an empty part has s == 0
@@ -58,43 +133,142 @@ struct RowStats {
     m = mn;
   }
   RB_DEVICE void one(float x, float k) { if (x != -INFINITY) add(x, 1.f, 0.f, k); }
+  // bring the sums to another maximum `mn` >= m
+  RB_DEVICE void to(float mn, float k) {
+    const float d = m == mn ? 0.f : fmaxf((m - mn) * k, -1000.f), f = exp2_fast(d);
+    w = f * fmaf(d, s, w);
+    s *= f;
+    m = mn;
+  }
 };
 
-// N values of one thread at once: their maximum, then the sums against it
-template <int N> RB_DEVICE void group_stats(const float (&x)[N], float k, float& m, float& s, float& w) {
-  m = x[0];
+constexpr int kPieces = 4;  // 16-byte pieces of a group (the functions below take any number)
+
+template <typename T, int P> RB_DEVICE float group_max(const int4 (&raw)[P]) {
+  constexpr int NW = P * 4;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+  if constexpr (Word<T>::N == 2) {
+    uint32_t m = w[0];
 #pragma unroll
-  for (int i = 1; i < N; ++i) m = max_nan(m, x[i]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  s = 0.f; w = 0.f;
+    for (int i = 1; i < NW; ++i) m = Word<T>::max(m, w[i]);
+    float a, b;
+    Word<T>::values(m, a, b);
+    return max_nan(a, b);
+  } else {
+    float m = __uint_as_float(w[0]);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    // the difference first: the largest token weighs exactly 1, a row of one token has an entropy of 0.  (-inf: weight 2^-1000 = 0, and 0 times a finite d)
-    const float d = fmaxf((x[i] - ref) * k, -1000.f);
-    const float e = exp2_fast(d);
-    s += e;
-    w = fmaf(d, e, w);
+    for (int i = 1; i < NW; ++i) m = max_nan(m, __uint_as_float(w[i]));
+    return m;
+  }
+}
+
+// A thread's sums against a reference, two at a time.
+struct Sums {
+  uint64_t s2 = 0, w2 = 0;
+  RB_DEVICE float s() const { float a, b; unpack2(s2, a, b); return a + b; }
+  RB_DEVICE float w() const { float a, b; unpack2(w2, a, b); return a + b; }
+};
+
+// Adds a group to sums against `ref`.  The difference comes before the scale: the largest token weighs exactly 1, and a row of one token has an
+// entropy of 0.  Unless differences are clamped, a logit of -inf (or one further from the reference than fp32 reaches) adds nothing to S and makes W a NaN.
+template <typename T, bool kEntropy, bool kClamp, int P> RB_DEVICE void group_add(const int4 (&raw)[P], float ref, float k, Sums& to) {
+  constexpr int NW = P * 4, STEP = Word<T>::N == 2 ? 1 : 2;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+  const uint64_t k2 = pack2(k, k), ref2 = pack2(-ref, -ref);
+#pragma unroll
+  for (int i = 0; i < NW; i += STEP) {
+    float a, b;
+    if constexpr (Word<T>::N == 2) Word<T>::values(w[i], a, b);
+    else { a = __uint_as_float(w[i]); b = __uint_as_float(w[i + 1]); }
+    uint64_t d = mul2(add2(pack2(a, b), ref2), k2);
+    unpack2(d, a, b);
+    if (kClamp) {
+      a = fmaxf(a, -1000.f);
+      b = fmaxf(b, -1000.f);
+      d = pack2(a, b);
+    }
+    const uint64_t e = pack2(exp2_fast(a), exp2_fast(b));
+    to.s2 = add2(to.s2, e);
+    if (kEntropy) to.w2 = fma2(d, e, to.w2);
+  }
+}
+
+// A thread's statistics over groups: the sums run against the largest value so far (a merge of each group's own statistics cost 20 instructions a group).
+template <typename T, bool kEntropy> struct RunningStats {
+  float m = -INFINITY;
+  Sums sums;
+  RB_DEVICE float reference() const { return m == -INFINITY ? 0.f : m; }
+  // make room for a group with the maximum mg
+  RB_DEVICE void raise(float mg, float k) {
+    if (!(mg <= m)) {
+      const float mn = max_nan(m, mg), d = fmaxf((m - mn) * k, -1000.f), f = exp2_fast(d);
+      const uint64_t f2 = pack2(f, f);
+      if (kEntropy) sums.w2 = mul2(f2, fma2(pack2(d, d), sums.s2, sums.w2));
+      sums.s2 = mul2(f2, sums.s2);
+      m = mn;
+    }
+  }
+  // `clamp`: the group may hold -inf
+  template <int P> RB_DEVICE void add(const int4 (&raw)[P], float k, bool clamp) {
+    raise(group_max<T>(raw), k);
+    if (kEntropy && clamp) group_add<T, kEntropy, true>(raw, reference(), k, sums);
+    else group_add<T, kEntropy, false>(raw, reference(), k, sums);
+  }
+  // W met a -inf: the row again, clamped
+  RB_DEVICE bool again() const { const float w = sums.w(); return kEntropy && w != w && m < INFINITY; }
+  RB_DEVICE RowStats stats() const {
+    RowStats r;
+    r.m = m;
+    r.s = sums.s();
+    r.w = sums.w();
+    return r;
+  }
+};
+
+// A row group by group: `adjust(piece, i)` may change the i-th piece of the row, `use(raw, i0, whole)` gets the group whose first piece is i0 (the others
+// are i0 + n threads, ...); in a group that is not whole, pieces behind the row's end are -inf.
+template <typename T, int kThreads, int P = kPieces, typename Adjust, typename Use> RB_DEVICE void walk_groups(const T* aligned, int nvec, Adjust adjust, Use use) {
+  const int4* v = reinterpret_cast<const int4*>(aligned);
+  int4 raw[P], next[P];
+  constexpr int none = (int)Word<T>::kNone;
+  auto fetch = [&](int4 (&r)[P], int i0) {
+    if (i0 + (P - 1) * kThreads < nvec) {
+#pragma unroll
+      for (int u = 0; u < P; ++u) r[u] = ld_stream(v + i0 + u * kThreads);
+    } else {
+#pragma unroll
+      for (int u = 0; u < P; ++u) r[u] = i0 + u * kThreads < nvec ? ld_stream(v + i0 + u * kThreads) : make_int4(none, none, none, none);
+    }
+  };
+  int i0 = threadIdx.x;
+  if (i0 < nvec) fetch(raw, i0);
+  while (i0 < nvec) {
+    const int i1 = i0 + P * kThreads;
+    if (i1 < nvec) fetch(next, i1);
+#pragma unroll
+    for (int u = 0; u < P; ++u) raw[u] = adjust(raw[u], i0 + u * kThreads);
+    use(raw, i0, i0 + (P - 1) * kThreads < nvec);
+#pragma unroll
+    for (int u = 0; u < P; ++u) raw[u] = next[u];
+    i0 = i1;
   }
 }
 
 // all threads' parts, in a fixed order, to every thread; red: 3 * 32 floats
 RB_DEVICE RowStats block_stats(RowStats a, float k, float* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m = __shfl_xor_sync(0xffffffffu, a.m, o), s = __shfl_xor_sync(0xffffffffu, a.s, o), w = __shfl_xor_sync(0xffffffffu, a.w, o);
-    a.add(m, s, w, k);
-  }
+  const float wm = warp_max_nan(a.m);
+  a.to(wm, k);
+  a.s = warp_sum(a.s);
+  a.w = warp_sum(a.w);
   __syncthreads();
-  if (lane == 0) { red[warp] = a.m; red[32 + warp] = a.s; red[64 + warp] = a.w; }
+  if (lane == 0) { red[warp] = wm; red[32 + warp] = a.s; red[64 + warp] = a.w; }
   __syncthreads();
   RowStats r;
   if (lane < nwarp) { r.m = red[lane]; r.s = red[32 + lane]; r.w = red[64 + lane]; }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m = __shfl_xor_sync(0xffffffffu, r.m, o), s = __shfl_xor_sync(0xffffffffu, r.s, o), w = __shfl_xor_sync(0xffffffffu, r.w, o);
-    r.add(m, s, w, k);
-  }
+  r.to(warp_max_nan(r.m), k);
+  r.s = warp_sum(r.s);
+  r.w = warp_sum(r.w);
   return r;
 }
 
@@ -108,6 +282,14 @@ struct RowResult {
     entropy = bad ? NAN : (r.m == -INFINITY ? 0.f : ls - kLn2 * (r.w / r.s));
   }
 };
+
+// Threads a row.  Small blocks overlap the rows' ends, large ones shorten a row.  us, 16-bit logits, 128 / 256 / 512 threads: 8192 x 32000 94 / 100 / 115,
+// 2048 x 131072 100 / 96 / 102, 300 x 32000 11.1 / 11.0 / 10.9, 1 x 131072 20.7 / 14.5 / 11.4 (launch included); 8192 x 2048 20.7 / 36.4 / 60.3: a group a thread.
+inline int row_threads(int64_t rows, int64_t pieces) {
+  if (pieces <= 256) return 32;
+  if (pieces <= 1024 || rows >= 16 * kNumSMs) return 128;
+  return rows >= 4 * kNumSMs ? 256 : 512;
+}
 
 // log-probability of a label: 0 for a negative one (no token), NaN for one beyond the vocabulary
 template <typename T> RB_DEVICE float label_logp(const T* row, int64_t label, const uint8_t* mask, int V, float inv_temp, float lse) {

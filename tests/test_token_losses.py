@@ -671,28 +671,35 @@ def test_nothing_beside_the_rows_is_written_gpu():
 
 @gpu
 def test_offsets_beyond_32_bits_gpu():
-    """Rows whose first element lies beyond 2^31: the last rows of a matrix of 33000 x 70001 in 16 bits equal the same rows alone (eight, so that
-    their addresses modulo 16, and with them the order of their sums, are the same)."""
+    """Rows whose first element lies beyond 2^31: the last rows of a matrix of 33000 x 70001 in 16 bits against the same rows alone.  A block has another number of
+    threads for few rows and with it another order of sums: two results of the bounds above."""
     T, V = 33000, 70001
     x = torch.empty(T, V, dtype=torch.bfloat16, device="cuda").normal_(0, 2)
     labels = torch.arange(T, device="cuda") % V
     o = OF.top_logprobs_from_logits(x, 3, labels)
-    few = OF.top_logprobs_from_logits(x[-8:].clone(), 3, labels[-8:])
-    for a, b in zip(o, few):
-        assert torch.equal(a[-8:], b)
+    last = x[-8:].clone()
+    few = OF.top_logprobs_from_logits(last, 3, labels[-8:])
+    z = scaled(last, None, 1.0)
+    y, p, _, H = stats64(z, labels[-8:].cpu())
+    e, r = err(z, V), half_step(x.dtype)
+    assert torch.equal(o.top_ids[-8:], few.top_ids)
+    for a, b in ((o.top_logp, few.top_logp), (o.rest_logp, few.rest_logp), (o.logp, few.logp), (o.entropy, few.entropy)):
+        assert ((a[-8:] - b).abs() <= 4 * e * (1 + b.abs())).all()
     leaf = x.requires_grad_(True)
     logp, ent = OF.logprob_entropy_from_logits(leaf, labels)
     (d,) = torch.autograd.grad([logp, ent], [leaf], [torch.ones_like(logp), torch.ones_like(ent)])
-    last = x.detach()[-8:].clone().requires_grad_(True)
+    last = last.requires_grad_(True)
     lp, en = OF.logprob_entropy_from_logits(last, labels[-8:])
     (dl,) = torch.autograd.grad([lp, en], [last], [torch.ones_like(lp), torch.ones_like(en)])
-    assert torch.equal(logp[-8:], lp) and torch.equal(d[-8:], dl)
+    slack = 2 * (r * dl.cpu().double().abs() + p * (2 - y + H[:, None]) * 4 * e + U)
+    assert ((logp[-8:] - lp).abs() <= 4 * e * (1 + lp.abs())).all() and ((d[-8:] - dl).abs().cpu().double() <= slack).all()
     del d
     loss = OF.distill_loss_from_logits(leaf, o.top_ids, o.top_logp, o.rest_logp)
     (d,) = torch.autograd.grad([loss], [leaf], [torch.ones_like(loss)])
     l8 = OF.distill_loss_from_logits(last, few.top_ids, few.top_logp, few.rest_logp)
     (d8,) = torch.autograd.grad([l8], [last], [torch.ones_like(l8)])
-    assert torch.equal(loss[-8:], l8) and torch.equal(d[-8:], d8)
+    # the teacher is the student: a loss of 0 but for the roundings of log-probabilities up to 12, and a gradient of as little
+    assert (loss[-8:].abs() <= 8 * e * 12).all() and (l8.abs() <= 8 * e * 12).all() and (d[-8:].abs() <= 8 * e * 12).all() and (d8.abs() <= 8 * e * 12).all()
 
 
 def check_no_rows(dev):
