@@ -14,7 +14,7 @@
 namespace {
 
 constexpr int kMaxListed = 1024;
-constexpr int kBwdThreads = 256, kBwdVecs = 4;
+constexpr int kBwdThreads = 128, kBwdVecs = 4;
 
 __host__ __device__ constexpr int bitmap_words(int V) { return (V + 16 + 31) / 32; }
 
@@ -66,13 +66,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_fwd_kernel(
   // the row: every unlisted token's part of the rest
   const uint8_t* bytes = reinterpret_cast<const uint8_t*>(listed);
   rb::RunningStats<T, false> run;
-  rb::walk_groups<T, kThreads>(
-      lr + span.head, span.nvec,
-      [&](int4 v, int i) {
-        if (i >= span.nvec) return v;
-        const uint32_t gone = VEC == 8 ? bytes[1 + i] : bytes[1 + (i >> 1)] >> ((i & 1) * 4) & 15;
-        return gone ? rb::mask_piece<T>(v, gone) : v;
-      },
+  rb::walk_groups<T, kThreads, rb::kPieces, true>(
+      lr + span.head, span.nvec, [&](int i) -> uint32_t { return VEC == 8 ? bytes[1 + i] : bytes[1 + (i >> 1)] >> ((i & 1) * 4) & 15; },
       [&](const int4 (&raw)[rb::kPieces], int, bool) { run.add(raw, kk, false); });
   rb::RowStats others = run.stats();
   const int ej = span.edge(threadIdx.x, V);
@@ -144,7 +139,7 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
   const float ref = lr_rest == -INFINITY ? 0.f : lr_rest;
   auto grad = [&](float x) {
     const float e = rb::exp2_fast(fmaf(x, inv_temp, -ref) * rb::kLog2e);
-    return zero || e == 0.f ? 0.f : a * e;
+    return zero ? 0.f : a * e;
   };
   const rb::RowSpan<T> span(lr, V);
   const bool same = ((reinterpret_cast<uintptr_t>(lr) ^ reinterpret_cast<uintptr_t>(orow)) & 15) == 0;
@@ -154,14 +149,31 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
     rb::Pack<T, VEC>* outs = reinterpret_cast<rb::Pack<T, VEC>*>(orow + span.head);
     lo = seg == 0 ? 0 : span.head + seg * kPer;
     hi = seg == segs - 1 ? V : min(V, span.head + (seg + 1) * kPer);
+    rb::Pack<T, VEC> p[kBwdVecs];                       // all loads before the first use
+    const uint64_t c2 = rb::pack2(inv_temp, inv_temp), r2 = rb::pack2(-ref, -ref), e2 = rb::pack2(rb::kLog2e, rb::kLog2e), a2 = rb::pack2(a, a);
+    const int i0 = seg * kBwdVecs * kBwdThreads + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < kBwdVecs; ++u)
+      if (i0 + u * kBwdThreads < span.nvec) {
+        const int4 v = rb::ld_once(reinterpret_cast<const int4*>(vecs + i0 + u * kBwdThreads));
+        p[u] = *reinterpret_cast<const rb::Pack<T, VEC>*>(&v);
+      }
 #pragma unroll
     for (int u = 0; u < kBwdVecs; ++u) {
-      const int i = (seg * kBwdVecs + u) * kBwdThreads + threadIdx.x;
-      if (i >= span.nvec) break;
-      rb::Pack<T, VEC> p = vecs[i];
+      const int i = i0 + u * kBwdThreads;
+      if (zero && i < span.nvec) {
+        __stcs(reinterpret_cast<int4*>(outs + i), make_int4(0, 0, 0, 0));
+      } else if (i < span.nvec) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) p.v[e] = rb::from_f<T>(grad(rb::to_f(p.v[e])));
-      outs[i] = p;
+        for (int e = 0; e < VEC; e += 2) {
+          float x0, x1;
+          rb::unpack2(rb::mul2(rb::fma2(rb::pack2(rb::to_f(p[u].v[e]), rb::to_f(p[u].v[e + 1])), c2, r2), e2), x0, x1);
+          rb::unpack2(rb::mul2(rb::pack2(rb::exp2_fast(x0), rb::exp2_fast(x1)), a2), x0, x1);
+          p[u].v[e] = rb::from_f<T>(x0);
+          p[u].v[e + 1] = rb::from_f<T>(x1);
+        }
+        __stcs(reinterpret_cast<int4*>(outs + i), *reinterpret_cast<const int4*>(&p[u]));
+      }
     }
     const int j = span.edge(threadIdx.x, V);
     if (j >= lo && j < hi) orow[j] = rb::from_f<T>(grad(rb::to_f(lr[j])));

@@ -7,7 +7,7 @@
 
 namespace {
 
-constexpr int kBwdThreads = 256, kBwdVecs = 4;
+constexpr int kBwdThreads = 64, kBwdVecs = 4;
 
 template <typename T, bool kMask, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_stats_kernel(const T* __restrict__ logits, int64_t row_stride,
@@ -22,11 +22,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_stats_kernel(
   const float k = inv_temp * rb::kLog2e;
   const rb::RowSpan<T> span(lr, V);
   rb::RunningStats<T, true> run;
-  auto adjust = [&](int4 v, int i) { return kMask && i < span.nvec ? rb::mask_piece<T>(v, rb::mask8(mr, mask_stride, span.head + i * VEC)) : v; };
-  rb::walk_groups<T, kThreads>(lr + span.head, span.nvec, adjust, [&](const int4 (&raw)[rb::kPieces], int, bool whole) { run.add(raw, k, kMask || !whole); });
+  auto bits = [&](int i) { return rb::mask_bits<VEC>(mr, mask_stride, span.head + i * VEC); };
+  rb::walk_groups<T, kThreads, rb::kPieces, kMask>(lr + span.head, span.nvec, bits, [&](const int4 (&raw)[rb::kPieces], int, bool whole) { run.add(raw, k, kMask || !whole); });
   if (run.again()) {
     run.sums = rb::Sums();
-    rb::walk_groups<T, kThreads>(lr + span.head, span.nvec, adjust,
+    rb::walk_groups<T, kThreads, rb::kPieces, kMask>(lr + span.head, span.nvec, bits,
                                  [&](const int4 (&raw)[rb::kPieces], int, bool) { rb::group_add<T, true, true>(raw, run.m, k, run.sums); });
   }
   rb::RowStats st = run.stats();
@@ -54,44 +54,80 @@ __global__ void __launch_bounds__(kBwdThreads) token_stats_bwd_kernel(const T* l
   T* orow = out + row * out_stride;
   const uint8_t* mr = kMask ? mask + row * mask_stride : nullptr;
   const float lse = lse_in[row], H = entropy[row];
-  const int64_t label = labels[row];
+  const int64_t given = labels[row];
   const float ge = g_entropy ? g_entropy[row] * inv_temp : 0.f;
-  float gl = g_logp && label >= 0 ? g_logp[row] * inv_temp : 0.f;
-  if (gl != 0.f && label >= V) gl = NAN;
+  float gl = g_logp && given >= 0 ? g_logp[row] * inv_temp : 0.f;
+  if (gl != 0.f && given >= V) gl = NAN;
   const bool zero = (gl == 0.f && ge == 0.f) || lse == -INFINITY;   // nothing asked of the row, or no token in it
+  const bool kept = given >= 0 && given < V && !(kMask && (mr[given >> 3] >> (given & 7)) & 1);
+  const int label = kept ? (int)given : -1;
   const float a = -(gl + ge * H);
-  auto grad = [&](float x, int j, bool gone) {
-    // d = a p - ge p y (+ gl at the label); a weight of 0 is 0 however low its logit
-    const float y = fmaf(x, inv_temp, -lse);
-    const float p = rb::exp2_fast(y * rb::kLog2e);
-    float d = p == 0.f ? 0.f : p * fmaf(-ge, y, a);
-    if (j == label) d += gl;
-    return zero || gone ? 0.f : d;
+  // a p - ge p y; a weight of 0 is 0 however low its logit
+  auto grad = [&](float x) {
+    const float y = fmaxf(fmaf(x, inv_temp, -lse), -1000.f);
+    return zero ? 0.f : rb::exp2_fast(y * rb::kLog2e) * fmaf(-ge, y, a);
+  };
+  auto edge = [&](int j) {
+    const float d = kMask && (mr[j >> 3] >> (j & 7)) & 1 ? (lse != lse && !zero ? NAN : 0.f) : grad(rb::to_f(lr[j]));
+    return rb::from_f<T>(j == label && !zero ? d + gl : d);
   };
   const rb::RowSpan<T> span(lr, V);
   const bool same = ((reinterpret_cast<uintptr_t>(lr) ^ reinterpret_cast<uintptr_t>(orow)) & 15) == 0;
   if (same) {
-    const rb::Pack<T, VEC>* vecs = reinterpret_cast<const rb::Pack<T, VEC>*>(lr + span.head);
-    rb::Pack<T, VEC>* outs = reinterpret_cast<rb::Pack<T, VEC>*>(orow + span.head);
+    const int4* vecs = reinterpret_cast<const int4*>(lr + span.head);
+    int4* outs = reinterpret_cast<int4*>(orow + span.head);
+    int4 p[kBwdVecs];                        // all loads before the first use
+    const int i0 = seg * kBwdVecs * kBwdThreads + threadIdx.x;
+    if (zero) {
 #pragma unroll
-    for (int u = 0; u < kBwdVecs; ++u) {
-      const int i = (seg * kBwdVecs + u) * kBwdThreads + threadIdx.x;
-      if (i >= span.nvec) break;
-      rb::Pack<T, VEC> p = vecs[i];
-      const int j0 = span.head + i * VEC;
-      const uint32_t gone = kMask ? rb::mask8(mr, mask_stride, j0) : 0u;
+      for (int u = 0; u < kBwdVecs; ++u)
+        if (i0 + u * kBwdThreads < span.nvec) __stcs(outs + i0 + u * kBwdThreads, make_int4(0, 0, 0, 0));
+    } else {
+      uint32_t gone[kBwdVecs];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) p.v[e] = rb::from_f<T>(grad(rb::to_f(p.v[e]), j0 + e, (gone >> e) & 1));
-      outs[i] = p;
+      for (int u = 0; u < kBwdVecs; ++u) {
+        const int i = i0 + u * kBwdThreads;
+        if (i < span.nvec) {
+          p[u] = rb::ld_once(vecs + i);
+          if (kMask) gone[u] = rb::mask_bits<VEC>(mr, mask_stride, span.head + i * VEC);
+        }
+      }
+      const uint64_t c2 = rb::pack2(inv_temp, inv_temp), l2 = rb::pack2(-lse, -lse), e2 = rb::pack2(rb::kLog2e, rb::kLog2e), g2 = rb::pack2(-ge, -ge),
+                     a2 = rb::pack2(a, a);
+#pragma unroll
+      for (int u = 0; u < kBwdVecs; ++u) {
+        const int i = i0 + u * kBwdThreads;
+        if (i < span.nvec) {
+          if (kMask) p[u] = rb::mask_piece<T>(p[u], gone[u]);
+          T* v = reinterpret_cast<T*>(&p[u]);
+          float d[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; e += 2) {
+            float x0, x1;
+            rb::unpack2(rb::fma2(rb::pack2(rb::to_f(v[e]), rb::to_f(v[e + 1])), c2, l2), x0, x1);
+            const uint64_t y = rb::pack2(fmaxf(x0, -1000.f), fmaxf(x1, -1000.f));
+            rb::unpack2(rb::mul2(y, e2), x0, x1);
+            rb::unpack2(rb::mul2(rb::pack2(rb::exp2_fast(x0), rb::exp2_fast(x1)), rb::fma2(g2, y, a2)), d[e], d[e + 1]);
+          }
+          const int at = label - (span.head + i * VEC);
+          if (at >= 0 && at < VEC) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) d[e] += e == at ? gl : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] = rb::from_f<T>(d[e]);
+          __stcs(outs + i, p[u]);
+        }
+      }
     }
     if (seg == 0) {
       const int j = span.edge(threadIdx.x, V);
-      if (j >= 0) orow[j] = rb::from_f<T>(grad(rb::to_f(lr[j]), j, kMask && (mr[j >> 3] >> (j & 7)) & 1));
+      if (j >= 0) orow[j] = edge(j);
     }
   } else {
     constexpr int per = kBwdThreads * kBwdVecs * VEC;
     const int j1 = seg == segs - 1 ? V : min(V, (seg + 1) * per);
-    for (int j = seg * per + threadIdx.x; j < j1; j += kBwdThreads) orow[j] = rb::from_f<T>(grad(rb::to_f(lr[j]), j, kMask && (mr[j >> 3] >> (j & 7)) & 1));
+    for (int j = seg * per + threadIdx.x; j < j1; j += kBwdThreads) orow[j] = edge(j);
   }
 }
 

@@ -171,8 +171,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
   const int lane = threadIdx.x & 31;
   const bool fast = records > 0;
   rb::RunningStats<T, true> run;
-  auto adjust = [&](int4 v, int i) { return kMask && i < span.nvec ? rb::mask_piece<T>(v, rb::mask8(r.mr, mask_stride, span.head + i * VEC)) : v; };
-  rb::walk_groups<T, kThreads, P>(r.lr + span.head, span.nvec, adjust, [&](const int4 (&raw)[P], int i0, bool whole) {
+  auto bits = [&](int i) { return rb::mask_bits<VEC>(r.mr, mask_stride, span.head + i * VEC); };
+  rb::walk_groups<T, kThreads, P, kMask>(r.lr + span.head, span.nvec, bits, [&](const int4 (&raw)[P], int i0, bool whole) {
     const float mg = rb::group_max<T>(raw);
     run.raise(mg, kk);
     rb::Sums g;
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
   });
   if (run.again()) {
     run.sums.w2 = 0;
-    rb::walk_groups<T, kThreads, P>(r.lr + span.head, span.nvec, adjust, [&](const int4 (&raw)[P], int, bool) {
+    rb::walk_groups<T, kThreads, P, kMask>(r.lr + span.head, span.nvec, bits, [&](const int4 (&raw)[P], int, bool) {
       rb::Sums g;
       rb::group_add<T, true, true>(raw, run.m, kk, g);
       run.sums.w2 = rb::add2(run.sums.w2, g.w2);
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
         const int j0 = span.head + piece * VEC;
         if (on && piece < span.nvec) {
           int4 raw = reinterpret_cast<const int4*>(r.lr + span.head)[piece];
-          if (kMask) raw = rb::mask_piece<T>(raw, rb::mask8(r.mr, mask_stride, j0));
+          if (kMask) raw = rb::mask_piece<T>(raw, rb::mask_bits<VEC>(r.mr, mask_stride, j0));
           const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
           for (int c = 0; c < VEC; ++c) {

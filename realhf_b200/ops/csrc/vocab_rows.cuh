@@ -101,22 +101,27 @@ template <typename T> struct RowSpan {
   }
 };
 
-// bits [j, j + 8) of a packed mask row of `bytes` bytes
-RB_DEVICE uint32_t mask8(const uint8_t* m, int64_t bytes, int j) {
+// bits [j, j + N) of a packed mask row of `bytes` bytes, N <= 8
+template <int N> RB_DEVICE uint32_t mask_bits(const uint8_t* m, int64_t bytes, int j) {
   uint32_t b = m[j >> 3];
-  if ((j & 7) && (j >> 3) + 1 < bytes) b |= (uint32_t)m[(j >> 3) + 1] << 8;
+  if ((j & 7) + N > 8 && (j >> 3) + 1 < bytes) b |= (uint32_t)m[(j >> 3) + 1] << 8;
   return b >> (j & 7);
 }
+
+// a piece that is read once; not through the read-only path, as gradients may take the logits' place
+RB_DEVICE int4 ld_once(const int4* p) { return __ldcs(p); }
 
 // a 16-byte piece whose elements with a bit set in `gone` become -inf
 template <typename T> RB_DEVICE int4 mask_piece(int4 v, uint32_t gone) {
   uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t m;
-    if constexpr (Word<T>::N == 1) m = 0u - ((gone >> i) & 1u);
-    else m = ((gone >> (2 * i)) & 1u) * 0xffffu + ((gone >> (2 * i + 1)) & 1u) * 0xffff0000u;
-    w[i] = (w[i] & ~m) | (Word<T>::kNone & m);
+    if constexpr (Word<T>::N == 1) {
+      if ((gone >> i) & 1) w[i] = Word<T>::kNone;
+    } else {                                 // one half at a time (a mask built from two bits took twice the instructions)
+      if ((gone >> (2 * i)) & 1) w[i] = __byte_perm(w[i], Word<T>::kNone, 0x3254);
+      if ((gone >> (2 * i + 1)) & 1) w[i] = __byte_perm(w[i], Word<T>::kNone, 0x7610);
+    }
   }
   return v;
 }
@@ -225,31 +230,44 @@ template <typename T, bool kEntropy> struct RunningStats {
   }
 };
 
-// A row group by group: `adjust(piece, i)` may change the i-th piece of the row, `use(raw, i0, whole)` gets the group whose first piece is i0 (the others
-// are i0 + n threads, ...); in a group that is not whole, pieces behind the row's end are -inf.
-template <typename T, int kThreads, int P = kPieces, typename Adjust, typename Use> RB_DEVICE void walk_groups(const T* aligned, int nvec, Adjust adjust, Use use) {
+// A row group by group.  `use(raw, i0, whole)` gets the group whose first piece is i0 (the others are i0 + n threads, ...); in a group that is not whole, pieces
+// behind the row's end are -inf.  kBits: `bits(i)` gives the elements of piece i that become -inf.
+template <typename T, int kThreads, int P, bool kBits, typename Bits, typename Use> RB_DEVICE void walk_groups(const T* aligned, int nvec, Bits bits, Use use) {
   const int4* v = reinterpret_cast<const int4*>(aligned);
   int4 raw[P], next[P];
+  uint32_t gone[P], gone_next[P];
   constexpr int none = (int)Word<T>::kNone;
-  auto fetch = [&](int4 (&r)[P], int i0) {
+  auto fetch = [&](int4 (&r)[P], uint32_t (&g)[P], int i0) {
     if (i0 + (P - 1) * kThreads < nvec) {
 #pragma unroll
-      for (int u = 0; u < P; ++u) r[u] = ld_stream(v + i0 + u * kThreads);
+      for (int u = 0; u < P; ++u) {
+        r[u] = ld_stream(v + i0 + u * kThreads);
+        if (kBits) g[u] = bits(i0 + u * kThreads);
+      }
     } else {
 #pragma unroll
-      for (int u = 0; u < P; ++u) r[u] = i0 + u * kThreads < nvec ? ld_stream(v + i0 + u * kThreads) : make_int4(none, none, none, none);
+      for (int u = 0; u < P; ++u) {
+        const int i = i0 + u * kThreads;
+        r[u] = i < nvec ? ld_stream(v + i) : make_int4(none, none, none, none);
+        if (kBits) g[u] = i < nvec ? bits(i) : 0u;
+      }
     }
   };
   int i0 = threadIdx.x;
-  if (i0 < nvec) fetch(raw, i0);
+  if (i0 < nvec) fetch(raw, gone, i0);
   while (i0 < nvec) {
     const int i1 = i0 + P * kThreads;
-    if (i1 < nvec) fetch(next, i1);
+    if (i1 < nvec) fetch(next, gone_next, i1);
+    if (kBits) {
 #pragma unroll
-    for (int u = 0; u < P; ++u) raw[u] = adjust(raw[u], i0 + u * kThreads);
+      for (int u = 0; u < P; ++u) raw[u] = mask_piece<T>(raw[u], gone[u]);
+    }
     use(raw, i0, i0 + (P - 1) * kThreads < nvec);
 #pragma unroll
-    for (int u = 0; u < P; ++u) raw[u] = next[u];
+    for (int u = 0; u < P; ++u) {
+      raw[u] = next[u];
+      if (kBits) gone[u] = gone_next[u];
+    }
     i0 = i1;
   }
 }
