@@ -16,6 +16,11 @@ int rb_token_stats_bwd(const void*, int64_t, const int64_t*, const uint8_t*, int
 int rb_top_logprobs_max();
 int rb_top_logprobs(const void*, int64_t, const int64_t*, const uint8_t*, int64_t, float*, float*, float*, int64_t*, float*, int64_t, int, int, float, int,
                     cudaStream_t);
+int64_t rb_head_stats_scratch(int);
+int rb_head_stats(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, float*, float*, float*, float*, int, int, int, float, int,
+                  int, cudaStream_t);
+int rb_head_stats_bwd(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*,
+                      void*, int64_t, int, int, int, float, int, int, cudaStream_t);
 int rb_distill_max_listed();
 int64_t rb_distill_max_vocab();
 int rb_distill_fwd(const void*, int64_t, const int64_t*, const float*, const float*, int, float*, float*, float*, float*, int*, int64_t, int, int, float, int,
@@ -167,6 +172,54 @@ Tensor distill_bwd(const Tensor& logits, const Tensor& lse_rest, const Tensor& g
   return d;
 }
 
+void check_head(const Tensor& h, const Tensor& w, const char* op, double inv_temp) {
+  TORCH_CHECK(h.is_cuda() && w.device() == h.device() && h.dim() == 2 && w.dim() == 2 && h.size(1) == w.size(1) && h.stride(1) == 1 && w.stride(1) == 1, op,
+              ": hidden states [rows, H] and a head [vocabulary, H] on one CUDA device, unit inner stride");
+  TORCH_CHECK(h.scalar_type() == w.scalar_type() && h.element_size() == 2, op, ": 16-bit operands of one type");
+  TORCH_CHECK(w.size(0) > 0 && w.size(0) <= 0x7fffff00LL && h.size(0) <= 0x7fffff00LL && inv_temp > 0, op, ": bad sizes or temperature");
+}
+
+// mask rows beside hidden states: [rows, at least vocabulary / 8]
+const uint8_t* head_mask(const OptT& mask, const Tensor& h, int64_t V, const char* op) {
+  if (!mask.has_value()) return nullptr;
+  TORCH_CHECK(mask->device() == h.device() && mask->scalar_type() == at::kByte && mask->dim() == 2 && mask->is_contiguous() && mask->size(0) == h.size(0) &&
+                  mask->size(1) * 8 >= V, op, ": the mask is a packed uint8 matrix [rows, at least vocabulary / 8]");
+  return mask->data_ptr<uint8_t>();
+}
+
+std::vector<Tensor> head_stats(const Tensor& h, const Tensor& w, const Tensor& labels, const OptT& mask, double inv_temp, int64_t num_sms) {
+  const char* op = "head_stats";
+  check_head(h, w, op, inv_temp);
+  const int64_t rows = h.size(0), V = w.size(0);
+  const auto* lab = static_cast<const int64_t*>(row_values(labels, at::kLong, h, -1, op, "labels"));
+  c10::cuda::CUDAGuard guard(h.device());
+  auto f = h.options().dtype(at::kFloat);
+  Tensor logp = at::empty({rows}, f), entropy = at::empty({rows}, f), lse = at::empty({rows}, f), scratch = at::empty({rows * rb_head_stats_scratch((int)V)}, f);
+  const int rc = rb_head_stats(h.data_ptr(), w.data_ptr(), h.stride(0), w.stride(0), lab, head_mask(mask, h, V, op), mask_bytes(mask), scratch.data_ptr<float>(),
+                               logp.data_ptr<float>(), entropy.data_ptr<float>(), lse.data_ptr<float>(), (int)rows, (int)V, (int)h.size(1), (float)inv_temp,
+                               dtype_code(h), (int)num_sms, stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+  return {logp, entropy, lse};
+}
+
+void head_stats_bwd(const Tensor& h, const Tensor& w, const Tensor& labels, const OptT& mask, const Tensor& lse, const Tensor& entropy, const OptT& g_logp,
+                    const OptT& g_entropy, double inv_temp, Tensor out, int64_t num_sms) {
+  const char* op = "head_stats_bwd";
+  check_head(h, w, op, inv_temp);
+  const int64_t rows = h.size(0), V = w.size(0);
+  const auto* lab = static_cast<const int64_t*>(row_values(labels, at::kLong, h, -1, op, "labels"));
+  const auto* l = static_cast<const float*>(row_values(lse, at::kFloat, h, -1, op, "lse"));
+  const auto* e = static_cast<const float*>(row_values(entropy, at::kFloat, h, -1, op, "entropy"));
+  const auto* gl = static_cast<const float*>(row_values(g_logp, at::kFloat, h, -1, op, "the log-probability's gradient"));
+  const auto* ge = static_cast<const float*>(row_values(g_entropy, at::kFloat, h, -1, op, "the entropy's gradient"));
+  TORCH_CHECK(out.device() == h.device() && out.scalar_type() == h.scalar_type() && out.dim() == 2 && out.size(0) == rows && out.size(1) == V &&
+                  out.stride(1) == 1, op, ": the destination is [rows, vocabulary] of the operands' type");
+  c10::cuda::CUDAGuard guard(h.device());
+  const int rc = rb_head_stats_bwd(h.data_ptr(), w.data_ptr(), h.stride(0), w.stride(0), lab, head_mask(mask, h, V, op), mask_bytes(mask), l, e, gl, ge,
+                                   out.data_ptr(), out.stride(0), (int)rows, (int)V, (int)h.size(1), (float)inv_temp, dtype_code(h), (int)num_sms, stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+}
+
 }  // namespace
 
 void register_vocab_ops(torch::Library& m) {
@@ -174,6 +227,9 @@ void register_vocab_ops(torch::Library& m) {
   m.def("token_stats_bwd(Tensor logits, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
         "Tensor(a!)? out) -> Tensor", &token_stats_bwd);
   m.def("top_logprobs(Tensor logits, int k, Tensor? labels, Tensor? mask, float inv_temp) -> Tensor[]", &top_logprobs);
+  m.def("head_stats(Tensor h, Tensor w, Tensor labels, Tensor? mask, float inv_temp, int num_sms) -> Tensor[]", &head_stats);
+  m.def("head_stats_bwd(Tensor h, Tensor w, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
+        "Tensor(a!) out, int num_sms) -> ()", &head_stats_bwd);
   m.def("distill_fwd(Tensor logits, Tensor ids, Tensor top_logp, Tensor? rest_logp, bool reverse, float inv_temp, bool need_grad) -> Tensor[]", &distill_fwd);
   m.def("distill_bwd(Tensor logits, Tensor lse_rest, Tensor g_rest, Tensor g_listed, Tensor ids, Tensor g_loss, float inv_temp, Tensor(a!)? out) -> Tensor",
         &distill_bwd);

@@ -667,7 +667,7 @@ def _head_logits(h, w):
 
 
 def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
-    """(d hidden, d weight) of a head whose rows [s, e) have the logits' gradient dlogits_of(s, e), of the hidden states' type."""
+    """(d hidden, d weight) of a head whose rows [s, e) have the logits' gradient dlogits_of(s, e)."""
     T = hidden.shape[0]
     dh = torch.empty_like(hidden, memory_format=torch.contiguous_format) if needs[0] else None
     G = _head_gemm(hidden, weight)
@@ -709,10 +709,15 @@ class _LMHeadTokenStats(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         T = hidden.shape[0]
         logp, entropy, lse = (torch.empty(T, dtype=torch.float32, device=hidden.device) for _ in range(3))
+        G = _head_gemm(hidden, weight)
         for s in range(0, T, chunk):
             e = min(T, s + chunk)
-            logp[s:e], entropy[s:e], lse[s:e] = lib().token_stats(_head_logits(hidden[s:e], weight), labels[s:e], None if mask_bits is None else mask_bits[s:e],
-                                                                  inv_temp)
+            mb = None if mask_bits is None else mask_bits[s:e]
+            if G is not None:
+                r = lib().head_stats(G.tma_rows(hidden[s:e]), weight, labels[s:e], mb, inv_temp, G._sms(hidden.device))
+            else:
+                r = lib().token_stats(_head_logits(hidden[s:e], weight), labels[s:e], mb, inv_temp)
+            logp[s:e], entropy[s:e], lse[s:e] = r
         ctx.save_for_backward(hidden, weight, labels, mask_bits, lse, entropy)
         ctx.inv_temp, ctx.chunk = inv_temp, chunk
         return logp, entropy
@@ -724,12 +729,17 @@ class _LMHeadTokenStats(torch.autograd.Function):
         if g_logp is None and g_entropy is None:
             return (None,) * 6
         gl, ge = _rows_f32(g_logp), _rows_f32(g_entropy)
+        G = _head_gemm(hidden, weight)
 
         def dlogits(s, e):
+            rows = (labels[s:e], None if mask_bits is None else mask_bits[s:e], lse[s:e], entropy[s:e], None if gl is None else gl[s:e],
+                    None if ge is None else ge[s:e], ctx.inv_temp)
+            if G is not None:
+                d = _pitched(e - s, weight.shape[0], hidden.dtype, hidden.device)
+                lib().head_stats_bwd(G.tma_rows(hidden[s:e]), weight, *rows, d, G._sms(hidden.device))
+                return d
             x = _head_logits(hidden[s:e], weight)
-            lib().token_stats_bwd(x, labels[s:e], None if mask_bits is None else mask_bits[s:e], lse[s:e], entropy[s:e], None if gl is None else gl[s:e],
-                                  None if ge is None else ge[s:e], ctx.inv_temp, x)
-            return _pitched(e - s, x.shape[1], hidden.dtype, x.device).copy_(x)
+            return lib().token_stats_bwd(x, *rows, x)
 
         return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None)
 
@@ -796,7 +806,7 @@ class _LMHeadDistill(torch.autograd.Function):
         def dlogits(s, e):
             x = _head_logits(hidden[s:e], weight)
             lib().distill_bwd(x, lse_rest[s:e], g_rest[s:e], g_listed[s:e], ids[s:e], g[s:e], ctx.inv_temp, x)
-            return _pitched(e - s, x.shape[1], hidden.dtype, x.device).copy_(x)
+            return x if _head_gemm(hidden, weight) is None else _pitched(e - s, x.shape[1], hidden.dtype, x.device).copy_(x)
 
         return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None, None, None)
 
