@@ -21,6 +21,8 @@ int rb_head_stats(const void*, const void*, int64_t, int64_t, const int64_t*, co
                   int, cudaStream_t);
 int rb_head_stats_bwd(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*,
                       void*, int64_t, int, int, int, float, int, int, cudaStream_t);
+int rb_head_dhidden_splits(int, int, int, int);
+int rb_head_dhidden(const void*, const void*, int64_t, int64_t, float*, void*, int, int, int, int, int, int, cudaStream_t);
 int rb_distill_max_listed();
 int64_t rb_distill_max_vocab();
 int rb_distill_fwd(const void*, int64_t, const int64_t*, const float*, const float*, int, float*, float*, float*, float*, int*, int64_t, int, int, float, int,
@@ -220,6 +222,19 @@ void head_stats_bwd(const Tensor& h, const Tensor& w, const Tensor& labels, cons
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
 }
 
+// out [rows, H] = d [rows, vocabulary] x w [vocabulary, H], the sum in `splits` parts
+void head_dhidden(const Tensor& d, const Tensor& w, Tensor out, int64_t splits, int64_t num_sms) {
+  const char* op = "head_dhidden";
+  TORCH_CHECK(d.is_cuda() && w.device() == d.device() && out.device() == d.device() && d.dim() == 2 && w.dim() == 2 && d.size(1) == w.size(0) && d.stride(1) == 1 &&
+                  w.stride(1) == 1 && out.is_contiguous() && out.dim() == 2 && out.size(0) == d.size(0) && out.size(1) == w.size(1), op, ": bad shapes");
+  TORCH_CHECK(d.scalar_type() == w.scalar_type() && out.scalar_type() == w.scalar_type() && w.element_size() == 2, op, ": 16-bit operands of one type");
+  c10::cuda::CUDAGuard guard(d.device());
+  Tensor parts = at::empty({splits, d.size(0), w.size(1)}, d.options().dtype(at::kFloat));
+  const int rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), d.stride(0), w.stride(0), parts.data_ptr<float>(), out.data_ptr(), (int)d.size(0), (int)w.size(1),
+                                 (int)d.size(1), (int)splits, dtype_code(d), (int)num_sms, stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+}
+
 }  // namespace
 
 void register_vocab_ops(torch::Library& m) {
@@ -230,6 +245,9 @@ void register_vocab_ops(torch::Library& m) {
   m.def("head_stats(Tensor h, Tensor w, Tensor labels, Tensor? mask, float inv_temp, int num_sms) -> Tensor[]", &head_stats);
   m.def("head_stats_bwd(Tensor h, Tensor w, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
         "Tensor(a!) out, int num_sms) -> ()", &head_stats_bwd);
+  m.def("head_dhidden(Tensor d, Tensor w, Tensor(a!) out, int splits, int num_sms) -> ()", &head_dhidden);
+  m.def("head_dhidden_splits(int rows, int width, int vocab, int num_sms) -> int",
+        [](int64_t m, int64_t n, int64_t v, int64_t sms) -> int64_t { return rb_head_dhidden_splits((int)m, (int)n, (int)v, (int)sms); });
   m.def("distill_fwd(Tensor logits, Tensor ids, Tensor top_logp, Tensor? rest_logp, bool reverse, float inv_temp, bool need_grad) -> Tensor[]", &distill_fwd);
   m.def("distill_bwd(Tensor logits, Tensor lse_rest, Tensor g_rest, Tensor g_listed, Tensor ids, Tensor g_loss, float inv_temp, Tensor(a!)? out) -> Tensor",
         &distill_bwd);

@@ -1,11 +1,12 @@
 // Language-model head with token statistics in its epilogue: logits X = h W^T (h [T, H], W [V, H], 16 bits, fp32 accumulators) never leave the chip.
 //
-// Forward: a CTA pair forms a 256 x 256 tile of X (tcgen05.mma.cta_group::2, operands by TMA, two accumulators in tensor memory); while the next tile is multiplied, four
-// warps a CTA read theirs, a lane a row, and leave three numbers a row and tile: maximum, sum and weighted sum (vocab_rows.cuh).  A second kernel merges a row's V / 256
+// Forward: a CTA pair forms a 256 x 256 tile of X (tcgen05.mma.cta_group::2, operands by TMA, two accumulators in tensor memory); while the next tile is multiplied, eight
+// warps a CTA read theirs, a lane a row of 128 columns, and leave three numbers: maximum, sum and weighted sum (vocab_rows.cuh).  A second kernel merges a row's V / 128
 // triples.  Logits are what fp32 accumulators hold; stored in 16 bits they would move a log-probability by up to 2^-9 of the logit.
 // Backward: the product again, d logits formed in the epilogue from the row's log-sum-exp and entropy and stored in 16 bits (rounded once), as operand of the
 // products for d h and d W.
-// An epilogue takes 32768 exponentials a CTA, 2048 cycles at least, beside 8 H cycles of products: it hides behind them from H = 512 on.
+// d h with few tiles: the sum over the vocabulary in parts, fp32 tiles that a second kernel adds up in order (16 rows of 4096 x 32000: 167 us undivided).
+// An epilogue takes 32768 exponentials a CTA, 2048 cycles at least, beside 8 H cycles of products.
 #include "attn_common.cuh"
 #include "cta_pair.cuh"
 #include "vocab_rows.cuh"
@@ -15,7 +16,8 @@ namespace {
 constexpr int HN = 256;                                     // logits of a tile
 constexpr int kHeadStages = 6;
 constexpr int kHeadA = BM * BK * 2, kHeadB = HN / 2 * BK * 2, kHeadStage = kHeadA + kHeadB;
-constexpr int kHeadOut = kHeadStages * kHeadStage, kHeadBars = kHeadOut + 4 * 4096, kHeadSmem = kHeadBars + 1024 + 256;
+constexpr int kEpiWarps = 8, kHeadThreads = 64 + 32 * kEpiWarps;
+constexpr int kHeadOut = kHeadStages * kHeadStage, kHeadBars = kHeadOut + kEpiWarps * 4096, kHeadSmem = kHeadBars + 1024 + 256;
 constexpr int kHeadBand = 8;                                // row tiles walked together, so that the tiles in flight share operands in L2
 
 struct HeadParams {
@@ -24,12 +26,13 @@ struct HeadParams {
   const int64_t* labels;
   const uint8_t* mask;
   int64_t mask_stride;
-  // forward: [tiles_n, M] each, and the label's logit [M]
+  // forward: [2 tiles_n, M] each, and the label's logit [M]
   float *part_m, *part_s, *part_w, *target;
   // backward
   const float *lse, *entropy, *g_logp, *g_entropy;
   void* out;
   int64_t ld_out;
+  int splits;           // d hidden: parts of the sum over the vocabulary, out fp32 [splits, M, N]
   int* status;
 };
 
@@ -51,8 +54,10 @@ RB_DEVICE uint32_t gone32(const uint8_t* m, int64_t bytes, int col, int N) {
   return n >= 32 ? b : n <= 0 ? ~0u : b | ~0u << n;
 }
 
-template <typename T, int kFmt, bool kBwd>
-__global__ void __launch_bounds__(kThreads, 1) head_stats_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+enum HeadMode { kStats, kLogitGrad, kHiddenGrad };
+
+template <typename T, int kFmt, HeadMode kMode>
+__global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                                                                  const HeadParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint32_t dead;
@@ -62,10 +67,20 @@ __global__ void __launch_bounds__(kThreads, 1) head_stats_kernel(const __grid_co
   uint64_t *full_bar = bars, *empty_bar = bars + kHeadStages, *tmem_full = bars + 2 * kHeadStages, *tmem_empty = tmem_full + 2;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr bool kBwd = kMode == kLogitGrad, kSplit = kMode == kHiddenGrad;
+  constexpr int kCols = kBwd ? 64 : 32;                     // columns an epilogue warp holds at once
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-  const int tiles_m = RB_CEIL_DIV(p.M, 2 * BM), tiles_n = RB_CEIL_DIV(p.N, HN), num_tiles = tiles_m * tiles_n, num_kb = RB_CEIL_DIV(p.K, BK);
+  const int tiles_m = RB_CEIL_DIV(p.M, 2 * BM), tiles_n = RB_CEIL_DIV(p.N, HN), all_kb = RB_CEIL_DIV(p.K, BK);
+  const int num_tiles = tiles_m * tiles_n * (kSplit ? p.splits : 1);
+  // a work item: a tile, and with splits the part [kb0, kb1) of the sum
+  auto item = [&](int i, int& mt, int& nt, int& part, int& kb0, int& kb1) {
+    part = kSplit ? i / (tiles_m * tiles_n) : 0;
+    head_tile(kSplit ? i - part * (tiles_m * tiles_n) : i, tiles_m, tiles_n, mt, nt);
+    kb0 = kSplit ? (int)((int64_t)all_kb * part / p.splits) : 0;
+    kb1 = kSplit ? (int)((int64_t)all_kb * (part + 1) / p.splits) : all_kb;
+  };
 
   if (threadIdx.x == 0) dead = 0;
   if (warp == 0 && lane == 0) {
@@ -77,7 +92,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_stats_kernel(const __grid_co
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(ptx::smem_u32(&tmem_full[i]), 1);
-      ptx::mbar_init(ptx::smem_u32(&tmem_empty[i]), 8);
+      ptx::mbar_init(ptx::smem_u32(&tmem_empty[i]), 2 * kEpiWarps);
     }
     ptx::fence_barrier_init();
   }
@@ -97,23 +112,30 @@ __global__ void __launch_bounds__(kThreads, 1) head_stats_kernel(const __grid_co
       int stage = 0;
       uint32_t phase = 0;
       for (int tile = pair; tile < num_tiles; tile += num_pairs) {
-        int mt, nt;
-        head_tile(tile, tiles_m, tiles_n, mt, nt);
+        int mt, nt, part, kb0, kb1;
+        item(tile, mt, nt, part, kb0, kb1);
         const int m0 = mt * 2 * BM + (int)rank * BM, n0 = nt * HN + (int)rank * (HN / 2);
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           bounded_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1, &dead);
           const uint32_t fb_local = ptx::smem_u32(&full_bar[stage]);
           if (leader) ptx::mbar_arrive_expect_tx(fb_local, 2 * kHeadStage);
           const uint32_t fb = mapa_u32(fb_local, 0);
           tma_load_2d_cg2(ptx::smem_u32(smem_a + stage * kHeadA), &tma_a, fb, kb * BK, m0);
-          tma_load_2d_cg2(ptx::smem_u32(smem_b + stage * kHeadB), &tma_b, fb, kb * BK, n0);
+          const uint32_t sb = ptx::smem_u32(smem_b + stage * kHeadB);
+          if constexpr (kSplit) {          // W as [V, H]: the sum runs over its rows
+#pragma unroll
+            for (int j = 0; j < HN / 2 / 64; ++j) tma_load_2d_cg2(sb + j * (BK * 128), &tma_b, fb, n0 + 64 * j, kb * BK);
+          } else {
+            tma_load_2d_cg2(sb, &tma_b, fb, kb * BK, n0);
+          }
           if (++stage == kHeadStages) { stage = 0; phase ^= 1; }
         }
       }
     }
   } else if (warp == 1) {
     if (leader) {      // the warp runs converged, one elected lane issues
-      constexpr uint32_t idesc = ptx::make_idesc_f16(kFmt, 2 * BM, HN, 0, 0);
+      constexpr uint32_t idesc = ptx::make_idesc_f16(kFmt, 2 * BM, HN, 0, kSplit ? 1 : 0);
+      constexpr uint32_t kBStep = (kSplit ? 2048 : 32) >> 4;          // 16 elements of the sum further, in descriptor units
       const uint32_t tm = (uint32_t)ptx::uniform((int)tmem_base);
       int stage = 0, as = 0;
       uint32_t phase = 0, aphase = 0;
@@ -122,15 +144,18 @@ __global__ void __launch_bounds__(kThreads, 1) head_stats_kernel(const __grid_co
         __syncwarp();
         ptx::tc_fence_after();
         const uint32_t d_tmem = tm + as * HN;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        int mt, nt, part, kb0, kb1;
+        item(tile, mt, nt, part, kb0, kb1);
+        const int n_kb = ptx::uniform(kb1 - kb0);
+        for (int kb = 0; kb < n_kb; ++kb) {
           bounded_wait(ptx::smem_u32(&full_bar[stage]), phase, &dead);
           __syncwarp();
           ptx::tc_fence_after();
           const uint64_t da = ptx::make_smem_desc_sw128(ptx::smem_u32(smem_a + stage * kHeadA), 16, 1024);
-          const uint64_t db = ptx::make_smem_desc_sw128(ptx::smem_u32(smem_b + stage * kHeadB), 16, 1024);
+          const uint64_t db = ptx::make_smem_desc_sw128(ptx::smem_u32(smem_b + stage * kHeadB), kSplit ? BK * 128 : 16, 1024);
           if (ptx::elect_one()) {
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k) tc_mma_f16_cg2(d_tmem, da + k * 2, db + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) tc_mma_f16_cg2(d_tmem, da + k * 2, db + k * kBStep, idesc, (kb | k) != 0 ? 1u : 0u);
             tc_commit_cg2(ptx::smem_u32(&empty_bar[stage]), 0b11);
           }
           __syncwarp();
@@ -142,17 +167,17 @@ __global__ void __launch_bounds__(kThreads, 1) head_stats_kernel(const __grid_co
       }
     }
   } else {
-    const int quad = warp & 3;
-    const uint32_t stage_out = ptx::smem_u32(smem + kHeadOut + quad * 4096);
+    const int quad = warp & 3, half = (warp - 2) >> 2;        // 32 rows, 128 columns
+    const uint32_t stage_out = ptx::smem_u32(smem + kHeadOut + (warp - 2) * 4096);
     const float k = p.inv_temp * rb::kLog2e;
     int as = 0;
     uint32_t aphase = 0;
     for (int tile = pair; tile < num_tiles; tile += num_pairs) {
-      int mt, nt;
-      head_tile(tile, tiles_m, tiles_n, mt, nt);
+      int mt, nt, part, kb0, kb1;
+      item(tile, mt, nt, part, kb0, kb1);
       const int n0 = nt * HN, row0 = mt * 2 * BM + (int)rank * BM + quad * 32, row = row0 + lane;
       const bool on = row < p.M;
-      const int64_t given = on ? p.labels[row] : -1;
+      const int64_t given = !kSplit && on ? p.labels[row] : -1;
       const uint8_t* mr = p.mask && on ? p.mask + row * p.mask_stride : nullptr;
       const int label = given >= n0 && given < min(p.N, n0 + HN) ? (int)(given - n0) : -1;       // within this tile
       float lse = 0.f, H = 0.f, gl = 0.f, ge = 0.f;
@@ -171,21 +196,28 @@ __global__ void __launch_bounds__(kThreads, 1) head_stats_kernel(const __grid_co
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + as * HN;
       float m = -INFINITY, s = 0.f, w = 0.f;
 #pragma unroll 1
-      for (int c = 0; c < HN; c += 32) {
-        uint32_t r[32];
+      for (int c = half * (HN / 2); c < (half + 1) * (HN / 2); c += kCols) {
+        uint32_t r[kCols];
         __syncwarp();
         ptx::tc_ld_32x32(taddr + c, r);
+        if (kCols == 64) ptx::tc_ld_32x32(taddr + c + 32, r + kCols - 32);
         const int col = n0 + c;
-        uint32_t gone = 0;
-        if (p.mask || col + 32 > p.N) gone = gone32(mr, p.mask_stride, col, p.N);
+        uint32_t gone = 0, gone_hi = 0;
+        if (!kSplit && (p.mask || col + kCols > p.N)) {
+          gone = gone32(mr, p.mask_stride, col, p.N);
+          if (kCols == 64) gone_hi = gone32(mr, p.mask_stride, col + 32, p.N);
+        }
         __syncwarp();
         ptx::tc_wait_ld();
         if (row0 >= p.M || col >= p.N) continue;
-        float x[32];
+        float x[kCols];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+        for (int i = 0; i < kCols; ++i) x[i] = __uint_as_float(r[i]);
         const int at = label - c;
-        if constexpr (!kBwd) {
+        if constexpr (kSplit) {
+          store_rows32<float>(stage_out, x, reinterpret_cast<float*>(p.out) + ((int64_t)part * p.M + row0) * p.N + col, p.N, p.M - row0, min(32, p.N - col), true,
+                              false);
+        } else if constexpr (!kBwd) {
           if (gone) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -225,31 +257,44 @@ __global__ void __launch_bounds__(kThreads, 1) head_stats_kernel(const __grid_co
           const uint64_t c2 = rb::pack2(p.inv_temp, p.inv_temp), l2 = rb::pack2(-lse, -lse), e2 = rb::pack2(rb::kLog2e, rb::kLog2e), g2 = rb::pack2(-ge, -ge),
                          a2 = rb::pack2(a, a);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
+          for (int i = 0; i < kCols; i += 2) {
             float u, v;
             rb::unpack2(rb::fma2(rb::pack2(x[i], x[i + 1]), c2, l2), u, v);
             const uint64_t y = rb::pack2(fmaxf(u, -1000.f), fmaxf(v, -1000.f));
             rb::unpack2(rb::mul2(y, e2), u, v);
             rb::unpack2(rb::mul2(rb::pack2(rb::exp2_fast(u), rb::exp2_fast(v)), rb::fma2(g2, y, a2)), x[i], x[i + 1]);
           }
-          if (at >= 0 && at < 32) {
+          if (at >= 0 && at < kCols) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] += i == at ? gl : 0.f;
+            for (int i = 0; i < kCols; ++i) x[i] += i == at ? gl : 0.f;
           }
-          if (p.mask && gone) {
+          if (p.mask && (gone | gone_hi)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if ((gone >> i) & 1) x[i] = lse != lse ? NAN : 0.f;
+            for (int i = 0; i < kCols; ++i)
+              if (((i < 32 ? gone : gone_hi) >> (i & 31)) & 1) x[i] = lse != lse ? NAN : 0.f;
           }
           if (zero) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = 0.f;
+            for (int i = 0; i < kCols; ++i) x[i] = 0.f;
           }
-          store_rows32<T>(stage_out, x, reinterpret_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col, p.ld_out, p.M - row0, min(32, p.N - col), true, false);
+          T* dst = reinterpret_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
+          if (col + kCols <= p.N && row0 + 32 <= p.M) {
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) r[i] = __float_as_uint(x[i]);
+            if constexpr (kCols == 64) store_rows64<T>(stage_out, r, dst, p.ld_out);
+          } else {
+#pragma unroll
+            for (int part = 0; part < kCols; part += 32) {
+              float v[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = x[part + i];
+              if (col + part < p.N) store_rows32<T>(stage_out, v, dst + part, p.ld_out, p.M - row0, min(32, p.N - col - part), true, false);
+            }
+          }
         }
       }
-      if (!kBwd && on) {
-        const int64_t to = (int64_t)nt * p.M + row;
+      if (kMode == kStats && on) {
+        const int64_t to = (int64_t)(2 * nt + half) * p.M + row;
         p.part_m[to] = m;
         p.part_s[to] = s;
         p.part_w[to] = w;
@@ -272,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_stats_kernel(const __grid_co
 
 // A row's triples -> its results: 32 rows a block, 16 threads a row over the tiles in turn, merged in a fixed order.
 constexpr int kMergeSlices = 16;
-__global__ void __launch_bounds__(32 * kMergeSlices) head_merge_kernel(const HeadParams p, int tiles_n, float* __restrict__ logp, float* __restrict__ entropy,
+__global__ void __launch_bounds__(32 * kMergeSlices) head_merge_kernel(const HeadParams p, int parts, float* __restrict__ logp, float* __restrict__ entropy,
                                                                       float* __restrict__ lse) {
   __shared__ float sm[3][kMergeSlices][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
@@ -280,7 +325,7 @@ __global__ void __launch_bounds__(32 * kMergeSlices) head_merge_kernel(const Hea
   rb::RowStats st;
   if (row < p.M) {
 #pragma unroll 4
-    for (int t = slice; t < tiles_n; t += kMergeSlices) {
+    for (int t = slice; t < parts; t += kMergeSlices) {
       const int64_t at = (int64_t)t * p.M + row;
       st.add(p.part_m[at], p.part_s[at], p.part_w[at], k);
     }
@@ -305,13 +350,30 @@ __global__ void __launch_bounds__(32 * kMergeSlices) head_merge_kernel(const Hea
   }
 }
 
-template <typename T, int kFmt, bool kBwd> int launch_head(const CUtensorMap& ta, const CUtensorMap& tb, const HeadParams& p, int num_sms, cudaStream_t s) {
-  auto kern = head_stats_kernel<T, kFmt, kBwd>;
+// parts [splits, n] -> their sum, rounded once; n a multiple of 8
+template <typename T> __global__ void __launch_bounds__(256) head_sum_kernel(const float* __restrict__ parts, T* __restrict__ out, int splits, int64_t n) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (i >= n) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float4 u = *reinterpret_cast<const float4*>(parts + s * n + i), v = *reinterpret_cast<const float4*>(parts + s * n + i + 4);
+    a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+    b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+  }
+  rb::Pack<T, 8> o;
+  o.v[0] = rb::from_f<T>(a.x); o.v[1] = rb::from_f<T>(a.y); o.v[2] = rb::from_f<T>(a.z); o.v[3] = rb::from_f<T>(a.w);
+  o.v[4] = rb::from_f<T>(b.x); o.v[5] = rb::from_f<T>(b.y); o.v[6] = rb::from_f<T>(b.z); o.v[7] = rb::from_f<T>(b.w);
+  *reinterpret_cast<rb::Pack<T, 8>*>(out + i) = o;
+}
+
+template <typename T, int kFmt, HeadMode kMode> int launch_head(const CUtensorMap& ta, const CUtensorMap& tb, const HeadParams& p, int num_sms, cudaStream_t s) {
+  auto kern = head_stats_kernel<T, kFmt, kMode>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeadSmem) != cudaSuccess) return -2;
-  const int tiles = RB_CEIL_DIV(p.M, 2 * BM) * RB_CEIL_DIV(p.N, HN), pairs = num_sms / 2;
+  const int tiles = RB_CEIL_DIV(p.M, 2 * BM) * RB_CEIL_DIV(p.N, HN) * (kMode == kHiddenGrad ? p.splits : 1), pairs = num_sms / 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * (tiles < pairs ? tiles : pairs));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kHeadThreads);
   cfg.dynamicSmemBytes = kHeadSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -338,7 +400,7 @@ int head_maps(const void* h, const void* w, int64_t ld_h, int64_t ld_w, int M, i
 extern "C" {
 
 // fp32 numbers a row that the forward pass leaves beside its results
-int64_t rb_head_stats_scratch(int N) { return 3LL * RB_CEIL_DIV(N, HN) + 1; }
+int64_t rb_head_stats_scratch(int N) { return 6LL * RB_CEIL_DIV(N, HN) + 1; }
 
 // h [M, K], w [N, K], in_dt 1 bf16 / 2 fp16, rows 16-byte aligned; labels [M]; scratch: fp32 [rb_head_stats_scratch(N) * M].
 int rb_head_stats(const void* h, const void* w, int64_t ld_h, int64_t ld_w, const int64_t* labels, const uint8_t* mask, int64_t mask_stride, float* scratch,
@@ -352,14 +414,14 @@ int rb_head_stats(const void* h, const void* w, int64_t ld_h, int64_t ld_w, cons
   p.inv_temp = inv_temp;
   p.labels = labels; p.mask = mask; p.mask_stride = mask_stride;
   p.part_m = scratch;
-  p.part_s = scratch + (int64_t)tiles_n * M;
-  p.part_w = scratch + 2LL * tiles_n * M;
-  p.target = scratch + 3LL * tiles_n * M;
+  p.part_s = scratch + 2LL * tiles_n * M;
+  p.part_w = scratch + 4LL * tiles_n * M;
+  p.target = scratch + 6LL * tiles_n * M;
   p.status = rb_attn_status();
   if (p.status == nullptr) return -14;
-  const int rc = in_dt == 1 ? launch_head<__nv_bfloat16, 1, false>(ta, tb, p, num_sms, s) : launch_head<__half, 0, false>(ta, tb, p, num_sms, s);
+  const int rc = in_dt == 1 ? launch_head<__nv_bfloat16, 1, kStats>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kStats>(ta, tb, p, num_sms, s);
   if (rc) return rc;
-  head_merge_kernel<<<RB_CEIL_DIV(M, 32), 32 * kMergeSlices, 0, s>>>(p, tiles_n, logp, entropy, lse);
+  head_merge_kernel<<<RB_CEIL_DIV(M, 32), 32 * kMergeSlices, 0, s>>>(p, 2 * tiles_n, logp, entropy, lse);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -379,7 +441,46 @@ int rb_head_stats_bwd(const void* h, const void* w, int64_t ld_h, int64_t ld_w, 
   p.out = out; p.ld_out = ld_out;
   p.status = rb_attn_status();
   if (p.status == nullptr) return -14;
-  return in_dt == 1 ? launch_head<__nv_bfloat16, 1, true>(ta, tb, p, num_sms, s) : launch_head<__half, 0, true>(ta, tb, p, num_sms, s);
+  return in_dt == 1 ? launch_head<__nv_bfloat16, 1, kLogitGrad>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kLogitGrad>(ta, tb, p, num_sms, s);
+}
+
+// How many parts the sum over the vocabulary is cut into for d h = d logits W, [M, V] x [V, N]: 1 where the tiles of d h fill the GPU (or nearly), so that the general product
+// takes them.  A k-block of a tile takes 0.28 us; a part costs its fp32 tile once out and once in.
+int rb_head_dhidden_splits(int M, int N, int V, int num_sms) {
+  const int pairs = num_sms / 2, tiles = RB_CEIL_DIV(M, 2 * BM) * RB_CEIL_DIV(N, HN), kb = RB_CEIL_DIV(V, BK);
+  if (tiles * 10 >= pairs * 7) return 1;
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 64 && s * 4 <= kb; ++s) {
+    const double t = (double)RB_CEIL_DIV(tiles * s, pairs) * RB_CEIL_DIV(kb, s) * 0.28 + (double)s * M * N * 8 / 5e6;
+    if (t < least) { least = t; best = s; }
+  }
+  return best;
+}
+
+// d [M, V] (rows ld_d apart, a multiple of 8), w [V, N], parts: fp32 [splits, M, N], out [M, N] contiguous; N a multiple of 8.
+int rb_head_dhidden(const void* d, const void* w, int64_t ld_d, int64_t ld_w, float* parts, void* out, int M, int N, int V, int splits, int in_dt, int num_sms,
+                    cudaStream_t s) {
+  if (M <= 0) return 0;
+  if (in_dt != 1 && in_dt != 2) return -10;
+  if (N % 8 || ld_d % 8 || ld_w % 8 || ((reinterpret_cast<uintptr_t>(d) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 15)) return -11;
+  if (splits < 1 || splits > RB_CEIL_DIV(V, BK)) return -12;
+  CUtensorMap ta, tb;
+  if (!make_tmap(&ta, d, in_dt == 1, (uint64_t)M, (uint64_t)V, (uint64_t)ld_d, BK, (uint32_t)BM)) return -13;
+  if (!make_tmap(&tb, w, in_dt == 1, (uint64_t)V, (uint64_t)N, (uint64_t)ld_w, 64, BK)) return -13;
+  HeadParams p{};
+  p.M = M; p.N = N; p.K = V;
+  p.out = parts;
+  p.splits = splits;
+  p.status = rb_attn_status();
+  if (p.status == nullptr) return -14;
+  const int rc = in_dt == 1 ? launch_head<__nv_bfloat16, 1, kHiddenGrad>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kHiddenGrad>(ta, tb, p, num_sms, s);
+  if (rc) return rc;
+  const int64_t n = (int64_t)M * N;
+  const unsigned blocks = (unsigned)RB_CEIL_DIV(n, 256 * 8);
+  if (in_dt == 1) head_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(parts, (__nv_bfloat16*)out, splits, n);
+  else head_sum_kernel<__half><<<blocks, 256, 0, s>>>(parts, (__half*)out, splits, n);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 }  // extern "C"

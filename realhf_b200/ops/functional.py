@@ -690,8 +690,13 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
             if dw is not None:
                 dw += d.float().t() @ hidden[s:e].float()
             continue
-        if dh is not None:
-            G.gemm(d, weight, out=dh[s:e], b_mn=True)                                        # [t, V] x [V, H]
+        if dh is not None:                                                                   # [t, V] x [V, H]
+            sms = G._sms(weight.device)
+            splits = lib().head_dhidden_splits(e - s, weight.shape[1], weight.shape[0], sms)
+            if splits > 1:
+                lib().head_dhidden(d, weight, dh[s:e], splits, sms)
+            else:
+                G.gemm(d, weight, out=dh[s:e], b_mn=True)
         if needs[1]:
             h = G.tma_rows(hidden[s:e])
             if dw is None:
@@ -713,7 +718,7 @@ class _LMHeadTokenStats(torch.autograd.Function):
         for s in range(0, T, chunk):
             e = min(T, s + chunk)
             mb = None if mask_bits is None else mask_bits[s:e]
-            if G is not None:
+            if G is not None and e - s > 256:      # (a row tile or less leaves half of the pairs idle: 16 / 256 rows of 4096 x 32000 66 / 78 us through logits, 87 / 97 fused)
                 r = lib().head_stats(G.tma_rows(hidden[s:e]), weight, labels[s:e], mb, inv_temp, G._sms(hidden.device))
             else:
                 r = lib().token_stats(_head_logits(hidden[s:e], weight), labels[s:e], mb, inv_temp)
