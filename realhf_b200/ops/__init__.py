@@ -46,6 +46,9 @@ class _LaunchCounter:
         n = torch.ops.realhf_b200.native_launches() if _lib is not None else 0
         if n:
             self.add("embedding_grad_", n)
+        n = torch.ops.realhf_b200.native_vocab_launches() if _lib is not None else 0
+        if n:
+            self.add("logit_gradients", n)
 
     @property
     def total(self) -> int:

@@ -1,13 +1,19 @@
 // torch bindings for the operators on rows of logits: token statistics, top alternatives, distillation.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 #include <torch/types.h>
 
+#include <atomic>
 #include <vector>
 
 using at::Tensor;
 using OptT = c10::optional<Tensor>;
+
+// kernels launched where Python does not see the call (in a native backward pass), since the last question
+static std::atomic<int64_t> unseen_launches{0};
 
 extern "C" {
 int rb_token_stats(const void*, int64_t, const int64_t*, const uint8_t*, int64_t, float*, float*, float*, int64_t, int, float, int, cudaStream_t);
@@ -17,8 +23,10 @@ int rb_top_logprobs_max();
 int rb_top_logprobs(const void*, int64_t, const int64_t*, const uint8_t*, int64_t, float*, float*, float*, int64_t*, float*, int64_t, int, int, float, int,
                     cudaStream_t);
 int64_t rb_head_stats_scratch(int);
-int rb_head_stats(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, float*, float*, float*, float*, int, int, int, float, int,
-                  int, cudaStream_t);
+int rb_head_stats(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, float*, void*, int64_t, float*, float*, float*, int, int, int,
+                  float, int, int, cudaStream_t);
+int rb_head_grad(const void*, int64_t, const float*, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*, void*, int64_t,
+                 int, int, int, int, float, int, cudaStream_t);
 int rb_head_stats_bwd(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*,
                       void*, int64_t, int, int, int, float, int, int, cudaStream_t);
 int rb_head_dhidden_splits(int, int, int, int);
@@ -40,28 +48,28 @@ int dtype_code(const Tensor& t) {
     case at::kFloat: return 0;
     case at::kBFloat16: return 1;
     case at::kHalf: return 2;
-    default: TORCH_CHECK(false, "unsupported dtype ", t.scalar_type(), " (float32, bfloat16 or float16)");
+    default: TORCH_CHECK_VALUE(false, "unsupported dtype ", t.scalar_type(), " (float32, bfloat16 or float16)");
   }
 }
 
 void check_logits(const Tensor& logits, const char* op, double inv_temp) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, op, ": logits are a CUDA matrix [rows, vocabulary] with unit inner stride");
-  TORCH_CHECK(logits.size(1) > 0 && logits.size(1) <= 0x7fffff00LL && logits.size(0) <= 0x7fffffffLL, op, ": bad size ", logits.sizes());
-  TORCH_CHECK(inv_temp > 0, op, ": the inverse temperature is positive");
+  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, op, ": logits are a CUDA matrix [rows, vocabulary] with unit inner stride");
+  TORCH_CHECK_VALUE(logits.size(1) > 0 && logits.size(1) <= 0x7fffff00LL && logits.size(0) <= 0x7fffffffLL, op, ": bad size ", logits.sizes());
+  TORCH_CHECK_VALUE(inv_temp > 0, op, ": the inverse temperature is positive");
 }
 
 // a contiguous tensor of this device, of one value a row (or [rows, k])
 const void* row_values(const OptT& t, at::ScalarType type, const Tensor& logits, int64_t k, const char* op, const char* name) {
   if (!t.has_value()) return nullptr;
-  TORCH_CHECK(t->device() == logits.device() && t->scalar_type() == type && t->is_contiguous() && t->size(0) == logits.size(0) &&
-                  (k < 0 ? t->dim() == 1 : t->dim() == 2 && t->size(1) == k),
+  TORCH_CHECK_VALUE(t->device() == logits.device() && t->scalar_type() == type && t->is_contiguous() && (k < 0 ? t->dim() == 1 : t->dim() == 2 && t->size(1) == k) &&
+                  t->size(0) == logits.size(0),
               op, ": ", name, " has to be contiguous, of type ", type, ", on the logits' device and of ", logits.size(0), " rows");
   return t->data_ptr();
 }
 
 const uint8_t* mask_rows(const OptT& mask, const Tensor& logits, const char* op) {
   if (!mask.has_value()) return nullptr;
-  TORCH_CHECK(mask->device() == logits.device() && mask->scalar_type() == at::kByte && mask->dim() == 2 && mask->is_contiguous() &&
+  TORCH_CHECK_VALUE(mask->device() == logits.device() && mask->scalar_type() == at::kByte && mask->dim() == 2 && mask->is_contiguous() &&
                   mask->size(0) == logits.size(0) && mask->size(1) * 8 >= logits.size(1),
               op, ": the mask is a packed uint8 matrix [rows, at least vocabulary / 8] on the logits' device");
   return mask->data_ptr<uint8_t>();
@@ -76,6 +84,17 @@ Tensor gradient_like(const Tensor& logits, const OptT& out, const char* op) {
               ": the gradient's destination is like the logits");
   return *out;
 }
+
+// whole numbers as contiguous int64
+Tensor whole_numbers(const Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK_VALUE(at::isIntegralType(t.scalar_type(), false), op, ": ", name, " are whole numbers, not ", t.scalar_type());
+  return t.to(at::kLong).contiguous();
+}
+Tensor fp32(const Tensor& t) { return t.to(at::kFloat).contiguous(); }
+OptT fp32(const OptT& t) { return t.has_value() ? OptT(fp32(*t)) : t; }
+OptT packed(const OptT& t) { return t.has_value() ? OptT(t->contiguous()) : t; }
+// rows with unit inner stride (`contiguous()` keeps a single column as it lies)
+Tensor unit_rows(const Tensor& x) { return x.dim() != 2 || x.stride(1) == 1 ? x : x.clone(at::MemoryFormat::Contiguous); }
 
 std::vector<Tensor> token_stats(const Tensor& logits, const Tensor& labels, const OptT& mask, double inv_temp) {
   check_logits(logits, "token_stats", inv_temp);
@@ -107,11 +126,13 @@ Tensor token_stats_bwd(const Tensor& logits, const Tensor& labels, const OptT& m
   return d;
 }
 
-std::vector<Tensor> top_logprobs(const Tensor& logits, int64_t k, const OptT& labels, const OptT& mask, double inv_temp) {
-  const char* op = "top_logprobs";
+std::vector<Tensor> top_logprobs(const Tensor& logits_in, int64_t k, const OptT& labels_in, const OptT& mask_in, double inv_temp) {
+  const char* op = "top_logprobs_from_logits";
+  const Tensor logits = unit_rows(logits_in);
+  const OptT labels = labels_in.has_value() ? OptT(whole_numbers(*labels_in, op, "labels")) : labels_in, mask = packed(mask_in);
   check_logits(logits, op, inv_temp);
   const int64_t rows = logits.size(0), V = logits.size(1);
-  TORCH_CHECK(k >= 1 && k <= V && k <= rb_top_logprobs_max(), op, ": between 1 and min(vocabulary, ", rb_top_logprobs_max(), ") alternatives, not ", k);
+  TORCH_CHECK_VALUE(k >= 1 && k <= V && k <= rb_top_logprobs_max(), op, ": between 1 and min(vocabulary, ", rb_top_logprobs_max(), ") alternatives, not ", k);
   const auto* lab = static_cast<const int64_t*>(row_values(labels, at::kLong, logits, -1, op, "labels"));
   c10::cuda::CUDAGuard guard(logits.device());
   auto f = logits.options().dtype(at::kFloat);
@@ -126,18 +147,25 @@ std::vector<Tensor> top_logprobs(const Tensor& logits, int64_t k, const OptT& la
   return r;
 }
 
+void check_teacher(const Tensor& logits, const Tensor& ids, const Tensor& t, const OptT& rest, bool reverse, const char* op) {
+  TORCH_CHECK_VALUE(ids.dim() == 2 && ids.sizes() == t.sizes() && ids.size(1) >= 1 && ids.size(1) <= rb_distill_max_listed(), op,
+                    ": the teacher's tokens and their log-probabilities are matrices [rows, 1 .. ", rb_distill_max_listed(), "], not ", ids.sizes(), " and ", t.sizes());
+  TORCH_CHECK_VALUE(logits.size(1) <= rb_distill_max_vocab(), op, ": a vocabulary of at most ", rb_distill_max_vocab(), " tokens");
+  TORCH_CHECK_VALUE(!reverse || rest.has_value(), op, ": the reverse divergence needs the teacher's rest (a token that the teacher gives nothing costs infinitely much)");
+  row_values(ids, at::kLong, logits, ids.size(1), op, "the teacher's tokens");
+  row_values(t, at::kFloat, logits, ids.size(1), op, "the tokens' log-probabilities");
+  row_values(rest, at::kFloat, logits, -1, op, "the rest's log-probability");
+}
+
 std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& ids, const Tensor& top_logp, const OptT& rest_logp, bool reverse, double inv_temp,
                                 bool need_grad) {
   const char* op = "distill_fwd";
   check_logits(logits, op, inv_temp);
   const int64_t rows = logits.size(0), V = logits.size(1);
-  TORCH_CHECK(ids.dim() == 2 && ids.size(1) >= 1 && ids.size(1) <= rb_distill_max_listed(), op, ": between 1 and ", rb_distill_max_listed(), " tokens a row");
-  TORCH_CHECK(V <= rb_distill_max_vocab(), op, ": a vocabulary of at most ", rb_distill_max_vocab(), " tokens");
-  TORCH_CHECK(!reverse || rest_logp.has_value(), op, ": the reverse divergence needs the teacher's rest");
+  check_teacher(logits, ids, top_logp, rest_logp, reverse, op);
   const int64_t k = ids.size(1);
-  const auto* id = static_cast<const int64_t*>(row_values(ids, at::kLong, logits, k, op, "the tokens"));
-  const auto* t = static_cast<const float*>(row_values(top_logp, at::kFloat, logits, k, op, "the tokens' log-probabilities"));
-  const auto* tr = static_cast<const float*>(row_values(rest_logp, at::kFloat, logits, -1, op, "the rest's log-probability"));
+  const auto* id = ids.data_ptr<int64_t>();
+  const auto *t = top_logp.data_ptr<float>(), *tr = rest_logp.has_value() ? rest_logp->data_ptr<float>() : nullptr;
   c10::cuda::CUDAGuard guard(logits.device());
   auto f = logits.options().dtype(at::kFloat);
   Tensor loss = at::empty({rows}, f), lse_rest, g_rest, g_listed, ids_out;
@@ -181,6 +209,75 @@ void check_head(const Tensor& h, const Tensor& w, const char* op, double inv_tem
   TORCH_CHECK(w.size(0) > 0 && w.size(0) <= 0x7fffff00LL && h.size(0) <= 0x7fffff00LL && inv_temp > 0, op, ": bad sizes or temperature");
 }
 
+// A first derivative that is asked for with a graph (create_graph) and then differentiated again is an error, not a zero.
+Tensor once(const Tensor& d, const char* op) {
+  if (!at::GradMode::is_enabled()) return d;
+  Tensor t = d.detach();
+  t.set_requires_grad(true);
+  return (*std::make_shared<torch::autograd::DelayedError>(std::string(op) + " has no second derivative", 1))({t})[0];
+}
+
+// Native, as short batches wait for the host: as Python functions forward and backward of 16 x 32000 logits took 75 (statistics) and 100 us (distillation).
+class LogprobEntropy : public torch::autograd::Function<LogprobEntropy> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const OptT& mask, double inv_temp) {
+    auto r = token_stats(logits, labels, mask, inv_temp);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, labels, mask.has_value() ? *mask : Tensor(), r[2], r[1]});
+    ctx->saved_data["inv_temp"] = inv_temp;
+    return {r[0], r[1]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    if (!g[0].defined() && !g[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto s = ctx->get_saved_variables();
+    auto given = [](const Tensor& t) { return t.defined() ? OptT(t) : OptT(); };
+    ++unseen_launches;
+    return {once(token_stats_bwd(s[0], s[1], given(s[2]), s[3], s[4], fp32(given(g[0])), fp32(given(g[1])), ctx->saved_data["inv_temp"].toDouble(), OptT()),
+                 "logprob_entropy_from_logits"), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::vector<Tensor> logprob_entropy(const Tensor& logits_in, const Tensor& labels_in, const OptT& mask, double inv_temp) {
+  const char* op = "logprob_entropy_from_logits";
+  const Tensor logits = unit_rows(logits_in), labels = whole_numbers(labels_in, op, "labels");
+  check_logits(logits, op, inv_temp);
+  row_values(labels, at::kLong, logits, -1, op, "labels");
+  const OptT m = packed(mask);
+  mask_rows(m, logits, op);
+  if (at::GradMode::is_enabled() && logits.requires_grad()) return LogprobEntropy::apply(logits, labels, m, inv_temp);
+  auto r = token_stats(logits, labels, m, inv_temp);
+  r.pop_back();
+  return r;
+}
+
+class DistillLoss : public torch::autograd::Function<DistillLoss> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& ids, const Tensor& t, const OptT& rest, bool reverse, double inv_temp) {
+    auto r = distill_fwd(logits, ids, t, rest, reverse, inv_temp, true);
+    ctx->save_for_backward({logits, r[1], r[2], r[3], r[4]});
+    ctx->saved_data["inv_temp"] = inv_temp;
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    ++unseen_launches;
+    return {once(distill_bwd(s[0], s[1], s[2], s[3], s[4], fp32(g[0]), ctx->saved_data["inv_temp"].toDouble(), OptT()), "distill_loss_from_logits"), Tensor(), Tensor(),
+            Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor distill_loss(const Tensor& logits_in, const Tensor& ids_in, const Tensor& t_in, const OptT& rest_in, bool reverse, double inv_temp) {
+  const char* op = "distill_loss_from_logits";
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(t_in.requires_grad() || (rest_in.has_value() && rest_in->requires_grad())), op,
+                    ": the teacher's log-probabilities get no gradient (detach them)");
+  const Tensor logits = unit_rows(logits_in), ids = whole_numbers(ids_in, op, "the teacher's tokens"), t = fp32(t_in);
+  const OptT rest = fp32(rest_in);
+  check_logits(logits, op, inv_temp);
+  check_teacher(logits, ids, t, rest, reverse, op);
+  if (at::GradMode::is_enabled() && logits.requires_grad()) return DistillLoss::apply(logits, ids, t, rest, reverse, inv_temp);
+  return distill_fwd(logits, ids, t, rest, reverse, inv_temp, false)[0];
+}
+
 // mask rows beside hidden states: [rows, at least vocabulary / 8]
 const uint8_t* head_mask(const OptT& mask, const Tensor& h, int64_t V, const char* op) {
   if (!mask.has_value()) return nullptr;
@@ -189,7 +286,8 @@ const uint8_t* head_mask(const OptT& mask, const Tensor& h, int64_t V, const cha
   return mask->data_ptr<uint8_t>();
 }
 
-std::vector<Tensor> head_stats(const Tensor& h, const Tensor& w, const Tensor& labels, const OptT& mask, double inv_temp, int64_t num_sms) {
+// keep: also the weights fp16 [rows, vocabulary] and the maxima that they stand against, for head_grad
+std::vector<Tensor> head_stats(const Tensor& h, const Tensor& w, const Tensor& labels, const OptT& mask, double inv_temp, bool keep, int64_t num_sms) {
   const char* op = "head_stats";
   check_head(h, w, op, inv_temp);
   const int64_t rows = h.size(0), V = w.size(0);
@@ -197,11 +295,34 @@ std::vector<Tensor> head_stats(const Tensor& h, const Tensor& w, const Tensor& l
   c10::cuda::CUDAGuard guard(h.device());
   auto f = h.options().dtype(at::kFloat);
   Tensor logp = at::empty({rows}, f), entropy = at::empty({rows}, f), lse = at::empty({rows}, f), scratch = at::empty({rows * rb_head_stats_scratch((int)V)}, f);
+  const int64_t pitch = (V + 7) / 8 * 8;
+  Tensor kept = keep ? at::empty({rows, pitch}, f.dtype(at::kHalf)) : Tensor();
   const int rc = rb_head_stats(h.data_ptr(), w.data_ptr(), h.stride(0), w.stride(0), lab, head_mask(mask, h, V, op), mask_bytes(mask), scratch.data_ptr<float>(),
-                               logp.data_ptr<float>(), entropy.data_ptr<float>(), lse.data_ptr<float>(), (int)rows, (int)V, (int)h.size(1), (float)inv_temp,
+                               keep ? kept.data_ptr() : nullptr, pitch, logp.data_ptr<float>(), entropy.data_ptr<float>(), lse.data_ptr<float>(), (int)rows, (int)V, (int)h.size(1), (float)inv_temp,
                                dtype_code(h), (int)num_sms, stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
-  return {logp, entropy, lse};
+  if (!keep) return {logp, entropy, lse};
+  return {logp, entropy, lse, kept, scratch.slice(0, 0, rows * ((V + 255) / 256 * 2)).clone()};
+}
+
+// d logits of rows [row0, row0 + out.size(0)) from what head_stats kept
+void head_grad(const Tensor& kept, const Tensor& maxima, const Tensor& labels, const OptT& mask, const Tensor& lse, const Tensor& entropy, const OptT& g_logp,
+               const OptT& g_entropy, double inv_temp, Tensor out, int64_t row0) {
+  const char* op = "head_grad";
+  const int64_t all = kept.size(0), rows = out.size(0), V = out.size(1);
+  TORCH_CHECK(kept.is_cuda() && kept.dim() == 2 && kept.is_contiguous() && kept.scalar_type() == at::kHalf && kept.size(1) == (V + 7) / 8 * 8 && row0 >= 0 &&
+                  row0 + rows <= all, op, ": the kept weights are fp16 rows of the vocabulary");
+  TORCH_CHECK(out.device() == kept.device() && out.element_size() == 2 && out.dim() == 2 && out.stride(1) == 1, op, ": a 16-bit destination");
+  TORCH_CHECK(maxima.device() == kept.device() && maxima.scalar_type() == at::kFloat && maxima.numel() == all * ((V + 255) / 256 * 2), op, ": bad maxima");
+  const auto* lab = static_cast<const int64_t*>(row_values(labels, at::kLong, kept, -1, op, "labels"));
+  const auto* l = static_cast<const float*>(row_values(lse, at::kFloat, kept, -1, op, "lse"));
+  const auto* e = static_cast<const float*>(row_values(entropy, at::kFloat, kept, -1, op, "entropy"));
+  const auto* gl = static_cast<const float*>(row_values(g_logp, at::kFloat, kept, -1, op, "the log-probability's gradient"));
+  const auto* ge = static_cast<const float*>(row_values(g_entropy, at::kFloat, kept, -1, op, "the entropy's gradient"));
+  c10::cuda::CUDAGuard guard(kept.device());
+  const int rc = rb_head_grad(kept.data_ptr<at::Half>() + row0 * kept.size(1), kept.size(1), maxima.data_ptr<float>(), lab, head_mask(mask, kept, V, op), mask_bytes(mask),
+                              l, e, gl, ge, out.data_ptr(), out.stride(0), (int)row0, (int)rows, (int)all, (int)V, (float)inv_temp, dtype_code(out), stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
 }
 
 void head_stats_bwd(const Tensor& h, const Tensor& w, const Tensor& labels, const OptT& mask, const Tensor& lse, const Tensor& entropy, const OptT& g_logp,
@@ -238,11 +359,16 @@ void head_dhidden(const Tensor& d, const Tensor& w, Tensor out, int64_t splits, 
 }  // namespace
 
 void register_vocab_ops(torch::Library& m) {
+  m.def("native_vocab_launches() -> int", []() -> int64_t { return unseen_launches.exchange(0); });
+  m.def("logprob_entropy(Tensor logits, Tensor labels, Tensor? mask, float inv_temp) -> Tensor[]", &logprob_entropy);
+  m.def("distill_loss(Tensor logits, Tensor ids, Tensor top_logp, Tensor? rest_logp, bool reverse, float inv_temp) -> Tensor", &distill_loss);
   m.def("token_stats(Tensor logits, Tensor labels, Tensor? mask, float inv_temp) -> Tensor[]", &token_stats);
   m.def("token_stats_bwd(Tensor logits, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
         "Tensor(a!)? out) -> Tensor", &token_stats_bwd);
   m.def("top_logprobs(Tensor logits, int k, Tensor? labels, Tensor? mask, float inv_temp) -> Tensor[]", &top_logprobs);
-  m.def("head_stats(Tensor h, Tensor w, Tensor labels, Tensor? mask, float inv_temp, int num_sms) -> Tensor[]", &head_stats);
+  m.def("head_stats(Tensor h, Tensor w, Tensor labels, Tensor? mask, float inv_temp, bool keep, int num_sms) -> Tensor[]", &head_stats);
+  m.def("head_grad(Tensor kept, Tensor maxima, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, Tensor(a!) out, "
+        "int row0) -> ()", &head_grad);
   m.def("head_stats_bwd(Tensor h, Tensor w, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
         "Tensor(a!) out, int num_sms) -> ()", &head_stats_bwd);
   m.def("head_dhidden(Tensor d, Tensor w, Tensor(a!) out, int splits, int num_sms) -> ()", &head_dhidden);

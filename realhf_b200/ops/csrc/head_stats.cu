@@ -3,8 +3,10 @@
 // Forward: a CTA pair forms a 256 x 256 tile of X (tcgen05.mma.cta_group::2, operands by TMA, two accumulators in tensor memory); while the next tile is multiplied, eight
 // warps a CTA read theirs, a lane a row of 128 columns, and leave three numbers: maximum, sum and weighted sum (vocab_rows.cuh).  A second kernel merges a row's V / 128
 // triples.  Logits are what fp32 accumulators hold; stored in 16 bits they would move a log-probability by up to 2^-9 of the logit.
-// Backward: the product again, d logits formed in the epilogue from the row's log-sum-exp and entropy and stored in 16 bits (rounded once), as operand of the
-// products for d h and d W.
+// Backward: d logits, in 16 bits (rounded once) as operand of the products for d h and d W, from the row's log-sum-exp and entropy, either
+//   from the product formed again, in its epilogue (2 T V H more operations, no memory), or
+//   from the weights e^{x - m} that the forward pass kept, m the maximum of the lane's 128 columns, as fp16 times 2^15: 11 bits for weights down to 2^-29, so that what is kept is
+//   rounded by an eighth of what d logits in bf16 are (T V more numbers of 16 bits between the passes).
 // d h with few tiles: the sum over the vocabulary in parts, fp32 tiles that a second kernel adds up in order (16 rows of 4096 x 32000: 167 us undivided).
 // An epilogue takes 32768 exponentials a CTA, 2048 cycles at least, beside 8 H cycles of products.
 #include "attn_common.cuh"
@@ -54,7 +56,28 @@ RB_DEVICE uint32_t gone32(const uint8_t* m, int64_t bytes, int col, int N) {
   return n >= 32 ? b : n <= 0 ? ~0u : b | ~0u << n;
 }
 
-enum HeadMode { kStats, kLogitGrad, kHiddenGrad };
+// 64 columns of a warp's 32 rows, a lane a row, to 16-bit memory; rows, cols: how many there are from the first on
+template <typename T> RB_DEVICE void store_cols(uint32_t stage, const float (&x)[64], T* dst, int64_t ld, int rows, int cols) {
+  if (cols >= 64 && rows >= 32) {
+    uint32_t r[64];
+#pragma unroll
+    for (int i = 0; i < 64; ++i) r[i] = __float_as_uint(x[i]);
+    store_rows64<T>(stage, r, dst, ld);
+  } else {
+#pragma unroll
+    for (int part = 0; part < 64; part += 32) {
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = x[part + i];
+      if (part < cols) store_rows32<T>(stage, v, dst + part, ld, rows, min(32, cols - part), true, false);
+    }
+  }
+}
+// (kernels that have no 64 columns)
+template <typename T> RB_DEVICE void store_cols(uint32_t, const float (&)[32], T*, int64_t, int, int) {}
+
+enum HeadMode { kStats, kStatsKeep, kLogitGrad, kHiddenGrad };
+constexpr float kKeepScale = 32768.f;
 
 template <typename T, int kFmt, HeadMode kMode>
 __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
@@ -68,7 +91,8 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr bool kBwd = kMode == kLogitGrad, kSplit = kMode == kHiddenGrad;
-  constexpr int kCols = kBwd ? 64 : 32;                     // columns an epilogue warp holds at once
+  constexpr bool kKeep = kMode == kStatsKeep;
+  constexpr int kCols = kBwd || kKeep ? 64 : 32;            // columns an epilogue warp holds at once
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
@@ -195,6 +219,24 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
       ptx::tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + as * HN;
       float m = -INFINITY, s = 0.f, w = 0.f;
+      if constexpr (kKeep) {           // the maximum of the lane's columns first
+#pragma unroll 1
+        for (int c = half * (HN / 2); c < (half + 1) * (HN / 2); c += 32) {
+          uint32_t r[32];
+          __syncwarp();
+          ptx::tc_ld_32x32(taddr + c, r);
+          const uint32_t gone = p.mask || n0 + c + 32 > p.N ? gone32(mr, p.mask_stride, n0 + c, p.N) : 0u;
+          __syncwarp();
+          ptx::tc_wait_ld();
+          if (gone) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if ((gone >> i) & 1) r[i] = 0xff800000u;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) m = rb::max_nan(m, __uint_as_float(r[i]));
+        }
+      }
 #pragma unroll 1
       for (int c = half * (HN / 2); c < (half + 1) * (HN / 2); c += kCols) {
         uint32_t r[kCols];
@@ -217,6 +259,35 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
         if constexpr (kSplit) {
           store_rows32<float>(stage_out, x, reinterpret_cast<float*>(p.out) + ((int64_t)part * p.M + row0) * p.N + col, p.N, p.M - row0, min(32, p.N - col), true,
                               false);
+        } else if constexpr (kKeep) {
+          if (gone | gone_hi) {
+#pragma unroll
+            for (int i = 0; i < kCols; ++i)
+              if (((i < 32 ? gone : gone_hi) >> (i & 31)) & 1) x[i] = -INFINITY;
+          }
+          if (at >= 0 && at < kCols) {
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) t = i == at ? x[i] : t;
+            p.target[row] = t;
+          }
+          const float ref = m == -INFINITY ? 0.f : m;
+          const uint64_t k2 = rb::pack2(k, k), ref2 = rb::pack2(-ref, -ref), scale2 = rb::pack2(kKeepScale, kKeepScale);
+          rb::Sums g;
+#pragma unroll
+          for (int i = 0; i < kCols; i += 2) {
+            float u, v;
+            rb::unpack2(rb::mul2(rb::add2(rb::pack2(x[i], x[i + 1]), ref2), k2), u, v);
+            u = fmaxf(u, -1000.f);
+            v = fmaxf(v, -1000.f);
+            const uint64_t e = rb::pack2(rb::exp2_fast(u), rb::exp2_fast(v));
+            g.s2 = rb::add2(g.s2, e);
+            g.w2 = rb::fma2(rb::pack2(u, v), e, g.w2);
+            rb::unpack2(rb::mul2(e, scale2), x[i], x[i + 1]);
+          }
+          s += g.s();
+          w += g.w();
+          store_cols<__half>(stage_out, x, reinterpret_cast<__half*>(p.out) + (int64_t)row0 * p.ld_out + col, p.ld_out, p.M - row0, p.N - col);
         } else if constexpr (!kBwd) {
           if (gone) {
 #pragma unroll
@@ -277,23 +348,10 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < kCols; ++i) x[i] = 0.f;
           }
-          T* dst = reinterpret_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col;
-          if (col + kCols <= p.N && row0 + 32 <= p.M) {
-#pragma unroll
-            for (int i = 0; i < kCols; ++i) r[i] = __float_as_uint(x[i]);
-            if constexpr (kCols == 64) store_rows64<T>(stage_out, r, dst, p.ld_out);
-          } else {
-#pragma unroll
-            for (int part = 0; part < kCols; part += 32) {
-              float v[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = x[part + i];
-              if (col + part < p.N) store_rows32<T>(stage_out, v, dst + part, p.ld_out, p.M - row0, min(32, p.N - col - part), true, false);
-            }
-          }
+          store_cols<T>(stage_out, x, reinterpret_cast<T*>(p.out) + (int64_t)row0 * p.ld_out + col, p.ld_out, p.M - row0, p.N - col);
         }
       }
-      if (kMode == kStats && on) {
+      if ((kMode == kStats || kKeep) && on) {
         const int64_t to = (int64_t)(2 * nt + half) * p.M + row;
         p.part_m[to] = m;
         p.part_s[to] = s;
@@ -350,6 +408,82 @@ __global__ void __launch_bounds__(32 * kMergeSlices) head_merge_kernel(const Hea
   }
 }
 
+// d logits from kept weights: rows of `kept` belong to rows row0, row0 + 1, ... of the forward pass; in segments of a row
+constexpr int kGradThreads = 128, kGradPieces = 4;
+template <typename T>
+__global__ void __launch_bounds__(kGradThreads) head_grad_kernel(const __half* __restrict__ kept, int64_t ld_kept, const HeadParams p, int row0, int all_rows, int segs) {
+  const int row = blockIdx.x / segs, seg = blockIdx.x - row * segs, whole = row0 + row;
+  const float lse = p.lse[whole], H = p.entropy[whole];
+  const int64_t given = p.labels[whole];
+  const float ge = p.g_entropy ? p.g_entropy[whole] * p.inv_temp : 0.f;
+  float gl = p.g_logp && given >= 0 ? p.g_logp[whole] * p.inv_temp : 0.f;
+  if (gl != 0.f && given >= p.N) gl = NAN;
+  const bool zero = (gl == 0.f && ge == 0.f) || lse == -INFINITY;
+  const bool gone = p.mask && given >= 0 && given < p.N && (p.mask[whole * p.mask_stride + (given >> 3)] >> (given & 7)) & 1;
+  const int label = given >= 0 && given < p.N && !gone ? (int)given : -1;
+  const float a = -(gl + ge * H);
+  const int pieces = RB_CEIL_DIV(p.N, 8);
+  const int4* in = reinterpret_cast<const int4*>(kept + row * ld_kept);
+  int4* out = reinterpret_cast<int4*>(reinterpret_cast<T*>(p.out) + row * p.ld_out);
+  const int i0 = seg * kGradPieces * kGradThreads + threadIdx.x;
+  int4 v[kGradPieces];
+  float y0[kGradPieces];                                    // log-probability of a kept number of 1
+  const bool plain = zero || lse != lse;
+#pragma unroll
+  for (int u = 0; u < kGradPieces; ++u) {
+    const int i = i0 + u * kGradThreads;
+    if (i < pieces && !plain) {
+      v[u] = rb::ld_once(in + i);
+      y0[u] = p.part_m[(int64_t)(i / (HN / 2 / 8)) * all_rows + whole];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kGradPieces; ++u) {
+    const int i = i0 + u * kGradThreads;
+    if (i >= pieces) continue;
+    float d[8];
+    if (plain) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = zero ? 0.f : NAN;
+    } else {
+      const __half2* h = reinterpret_cast<const __half2*>(&v[u]);
+      const float y1 = y0[u] == -INFINITY ? 0.f : fmaf(y0[u], p.inv_temp, -lse) - 15.f * rb::kLn2, f = rb::exp2_fast(y1 * rb::kLog2e);
+      const uint64_t f2 = rb::pack2(f, f), ln2 = rb::pack2(rb::kLn2, rb::kLn2), y2 = rb::pack2(y1, y1), g2 = rb::pack2(-ge, -ge), a2 = rb::pack2(a, a);
+      if (ge != 0.f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = __half22float2(h[e]);
+          // y = ln x + y1; a weight of 0 is 0 whatever its logarithm
+          const uint64_t y = rb::fma2(rb::pack2(fmaxf(__log2f(x.x), -100.f), fmaxf(__log2f(x.y), -100.f)), ln2, y2);
+          rb::unpack2(rb::mul2(rb::mul2(rb::pack2(x.x, x.y), f2), rb::fma2(g2, y, a2)), d[2 * e], d[2 * e + 1]);
+        }
+      } else {
+        const uint64_t af = rb::mul2(f2, a2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = __half22float2(h[e]);
+          rb::unpack2(rb::mul2(rb::pack2(x.x, x.y), af), d[2 * e], d[2 * e + 1]);
+        }
+      }
+      const int at = label - i * 8;
+      if (at >= 0 && at < 8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] += e == at ? gl : 0.f;
+      }
+    }
+    rb::Pack<T, 8> o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.v[e] = rb::from_f<T>(d[e]);
+    if (i * 8 + 8 <= p.N) {
+      out[i] = *reinterpret_cast<const int4*>(&o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i * 8 + e < p.N) reinterpret_cast<T*>(out + i)[e] = o.v[e];
+    }
+  }
+}
+
 // parts [splits, n] -> their sum, rounded once; n a multiple of 8
 template <typename T> __global__ void __launch_bounds__(256) head_sum_kernel(const float* __restrict__ parts, T* __restrict__ out, int splits, int64_t n) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
@@ -402,9 +536,10 @@ extern "C" {
 // fp32 numbers a row that the forward pass leaves beside its results
 int64_t rb_head_stats_scratch(int N) { return 6LL * RB_CEIL_DIV(N, HN) + 1; }
 
-// h [M, K], w [N, K], in_dt 1 bf16 / 2 fp16, rows 16-byte aligned; labels [M]; scratch: fp32 [rb_head_stats_scratch(N) * M].
+// h [M, K], w [N, K], in_dt 1 bf16 / 2 fp16, rows 16-byte aligned; labels [M]; scratch: fp32 [rb_head_stats_scratch(N) * M]; its first M * ceil(N / 256) * 2 numbers are the
+// maxima of 128 columns.  kept: fp16 [M, N] for the weights, rows ld_kept apart (a multiple of 8), or null.
 int rb_head_stats(const void* h, const void* w, int64_t ld_h, int64_t ld_w, const int64_t* labels, const uint8_t* mask, int64_t mask_stride, float* scratch,
-                  float* logp, float* entropy, float* lse, int M, int N, int K, float inv_temp, int in_dt, int num_sms, cudaStream_t s) {
+                  void* kept, int64_t ld_kept, float* logp, float* entropy, float* lse, int M, int N, int K, float inv_temp, int in_dt, int num_sms, cudaStream_t s) {
   if (M <= 0) return 0;
   CUtensorMap ta, tb;
   if (const int rc = head_maps(h, w, ld_h, ld_w, M, N, K, in_dt, ta, tb)) return rc;
@@ -419,7 +554,11 @@ int rb_head_stats(const void* h, const void* w, int64_t ld_h, int64_t ld_w, cons
   p.target = scratch + 6LL * tiles_n * M;
   p.status = rb_attn_status();
   if (p.status == nullptr) return -14;
-  const int rc = in_dt == 1 ? launch_head<__nv_bfloat16, 1, kStats>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kStats>(ta, tb, p, num_sms, s);
+  if (kept && (ld_kept % 8 || (reinterpret_cast<uintptr_t>(kept) & 15))) return -12;
+  p.out = kept;
+  p.ld_out = ld_kept;
+  const int rc = kept ? (in_dt == 1 ? launch_head<__nv_bfloat16, 1, kStatsKeep>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kStatsKeep>(ta, tb, p, num_sms, s))
+                      : (in_dt == 1 ? launch_head<__nv_bfloat16, 1, kStats>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kStats>(ta, tb, p, num_sms, s));
   if (rc) return rc;
   head_merge_kernel<<<RB_CEIL_DIV(M, 32), 32 * kMergeSlices, 0, s>>>(p, 2 * tiles_n, logp, entropy, lse);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
@@ -442,6 +581,27 @@ int rb_head_stats_bwd(const void* h, const void* w, int64_t ld_h, int64_t ld_w, 
   p.status = rb_attn_status();
   if (p.status == nullptr) return -14;
   return in_dt == 1 ? launch_head<__nv_bfloat16, 1, kLogitGrad>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kLogitGrad>(ta, tb, p, num_sms, s);
+}
+
+// d logits [rows, N] of rows row0 .. of a forward pass over all_rows rows, from what it kept (`kept`: these rows; part_m, labels, mask and values a row: all rows); out as above
+int rb_head_grad(const void* kept, int64_t ld_kept, const float* part_m, const int64_t* labels, const uint8_t* mask, int64_t mask_stride, const float* lse,
+                 const float* entropy, const float* g_logp, const float* g_entropy, void* out, int64_t ld_out, int row0, int rows, int all_rows, int N, float inv_temp,
+                 int dt, cudaStream_t s) {
+  if (rows <= 0) return 0;
+  if (ld_out % 8 || ld_kept % 8 || ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(kept)) & 15) || row0 < 0 || row0 + rows > all_rows) return -12;
+  HeadParams p{};
+  p.M = rows; p.N = N;
+  p.inv_temp = inv_temp;
+  p.labels = labels; p.mask = mask; p.mask_stride = mask_stride;
+  p.part_m = const_cast<float*>(part_m);
+  p.lse = lse; p.entropy = entropy; p.g_logp = g_logp; p.g_entropy = g_entropy;
+  p.out = out; p.ld_out = ld_out;
+  const int64_t segs = RB_CEIL_DIV(RB_CEIL_DIV(N, 8), kGradThreads * kGradPieces);
+  if (rows * segs > 0x7fffffffLL) return -3;
+  if (dt == 1) head_grad_kernel<__nv_bfloat16><<<(unsigned)(rows * segs), kGradThreads, 0, s>>>((const __half*)kept, ld_kept, p, row0, all_rows, (int)segs);
+  else if (dt == 2) head_grad_kernel<__half><<<(unsigned)(rows * segs), kGradThreads, 0, s>>>((const __half*)kept, ld_kept, p, row0, all_rows, (int)segs);
+  else return -10;
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 // How many parts the sum over the vocabulary is cut into for d h = d logits W, [M, V] x [V, N]: 1 where the tiles of d h fill the GPU (or nearly), so that the general product

@@ -492,26 +492,9 @@ def _rows_f32(t):
     return None if t is None else t.float().contiguous()
 
 
-def _unit_rows(logits):
-    return logits if logits.stride(1) == 1 else logits.clone(memory_format=torch.contiguous_format)   # (`contiguous()` keeps a single column as it lies)
-
-
-class _TokenStats(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, mask_bits, inv_temp):
-        ctx.set_materialize_grads(False)
-        logp, entropy, lse = lib().token_stats(logits, labels, mask_bits, inv_temp)
-        ctx.save_for_backward(logits, labels, mask_bits, lse, entropy)
-        ctx.inv_temp = inv_temp
-        return logp, entropy
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logp, g_entropy):
-        logits, labels, mask_bits, lse, entropy = ctx.saved_tensors
-        if g_logp is None and g_entropy is None:
-            return None, None, None, None
-        return lib().token_stats_bwd(logits, labels, mask_bits, lse, entropy, _rows_f32(g_logp), _rows_f32(g_entropy), ctx.inv_temp, None), None, None, None
+def _plain_autograd() -> bool:
+    """Inside function transforms and forward-mode differentiation, which the native autograd functions do not answer for."""
+    return torch.autograd.forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None
 
 
 def logprob_entropy_from_logits(logits, labels, mask_bits=None, inv_temp: float = 1.0):
@@ -519,17 +502,13 @@ def logprob_entropy_from_logits(logits, labels, mask_bits=None, inv_temp: float 
     the tokens that `mask_bits` (`pack_mask_bits`, set = filtered out) keeps.  A negative label is no token: 0 without a gradient;
     a label of V or more gives NaN.  A row that keeps no token gives -inf and 0, one that holds a NaN or +inf NaN.  A row whose incoming
     gradients are 0 gets zeros, whatever it holds."""
+    if use_native(logits) and not _plain_autograd():       # (the native functions check their arguments themselves)
+        return tuple(lib().logprob_entropy(logits, labels, mask_bits, inv_temp))
     op = "logprob_entropy_from_logits"
     _check_rows(op, logits, inv_temp, labels=labels, mask_bits=mask_bits)
     _check_labels(op, labels)
     _check_mask(op, mask_bits, logits.shape[1])
-    if not use_native(logits):
-        return logprob_entropy_from_logits_ref(logits, labels, mask_bits, inv_temp)
-    logits, labels = _unit_rows(logits), labels.long().contiguous()
-    mask_bits = mask_bits.contiguous() if mask_bits is not None else None
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _TokenStats.apply(logits, labels, mask_bits, float(inv_temp))
-    return tuple(lib().token_stats(logits.detach(), labels, mask_bits, inv_temp)[:2])
+    return logprob_entropy_from_logits_ref(logits, labels, mask_bits, inv_temp)
 
 
 class TopLogprobs(NamedTuple):
@@ -560,18 +539,16 @@ def top_logprobs_from_logits(logits, k: int, labels=None, mask_bits=None, inv_te
     """The k most likely tokens of every row of logits [T, V], the log of the others' mass, the entropy and, with `labels`, their
     log-probabilities: one read of the logits.  No gradients.  What `distill_loss_from_logits` takes as its teacher.  k is at most
     min(V, 1024); -0 counts as 0; masked tokens are no alternatives; labels as in `logprob_entropy_from_logits`."""
+    if use_native(logits):
+        r = lib().top_logprobs(logits.detach(), k, labels, mask_bits, inv_temp)
+        return TopLogprobs(r[0], r[1], r[2], r[3], r[4] if labels is not None else None)
     op = "top_logprobs_from_logits"
     _check_rows(op, logits, inv_temp, labels=labels, mask_bits=mask_bits)
     _check_labels(op, labels)
     _check_mask(op, mask_bits, logits.shape[1])
     if not 1 <= k <= min(logits.shape[1], 1024):
         raise ValueError(f"{op}: between 1 and min(vocabulary, 1024) alternatives, not {k}")
-    logits = logits.detach()
-    if not use_native(logits):
-        return top_logprobs_from_logits_ref(logits, k, labels, mask_bits, inv_temp)
-    r = lib().top_logprobs(_unit_rows(logits), k, labels.long().contiguous() if labels is not None else None,
-                           mask_bits.contiguous() if mask_bits is not None else None, inv_temp)
-    return TopLogprobs(r[0], r[1], r[2], r[3], r[4] if labels is not None else None)
+    return top_logprobs_from_logits_ref(logits.detach(), k, labels, mask_bits, inv_temp)
 
 
 def distill_loss_from_logits_ref(logits, top_ids, top_logp, rest_logp=None, reverse: bool = False, inv_temp: float = 1.0):
@@ -595,20 +572,6 @@ def distill_loss_from_logits_ref(logits, top_ids, top_logp, rest_logp=None, reve
     return loss.masked_fill((ids >= V).any(-1) | lse.isnan(), float("nan"))
 
 
-class _Distill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, top_ids, top_logp, rest_logp, reverse, inv_temp):
-        loss, *saved = lib().distill_fwd(logits, top_ids, top_logp, rest_logp, reverse, inv_temp, True)
-        ctx.save_for_backward(logits, *saved)
-        ctx.inv_temp = inv_temp
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        return lib().distill_bwd(*ctx.saved_tensors, _rows_f32(g), ctx.inv_temp, None), None, None, None, None, None
-
-
 def _check_teacher(op: str, T: int, V: int, device, top_ids, top_logp, rest_logp, reverse):
     _check_row_values(op, T, device, top_ids=top_ids, top_logp=top_logp, rest_logp=rest_logp)
     if top_ids.dim() != 2 or top_ids.shape != top_logp.shape or not 1 <= top_ids.shape[1] <= 1024:
@@ -630,15 +593,12 @@ def distill_loss_from_logits(logits, top_ids, top_logp, rest_logp=None, reverse:
     each, all others together one more; without `rest_logp` the teacher is renormalised over its k tokens.  `reverse` False:
     KL(teacher || p); True: KL(p || teacher), which needs `rest_logp`.  A negative id is an unused place, an id given again counts where it stands
     first, an id of V or more makes the loss NaN.  A row whose incoming gradient is 0 gets zeros, whatever it holds."""
+    if use_native(logits) and not _plain_autograd():
+        return lib().distill_loss(logits, top_ids, top_logp, rest_logp, reverse, inv_temp)
     op = "distill_loss_from_logits"
     _check_rows(op, logits, inv_temp)
     _check_teacher(op, logits.shape[0], logits.shape[1], logits.device, top_ids, top_logp, rest_logp, reverse)
-    if not use_native(logits):
-        return distill_loss_from_logits_ref(logits, top_ids, top_logp, rest_logp, reverse, inv_temp)
-    logits, ids, t, tr = _unit_rows(logits), top_ids.long().contiguous(), _rows_f32(top_logp), _rows_f32(rest_logp)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _Distill.apply(logits, ids, t, tr, bool(reverse), float(inv_temp))
-    return lib().distill_fwd(logits.detach(), ids, t, tr, bool(reverse), float(inv_temp), False)[0]
+    return distill_loss_from_logits_ref(logits, top_ids, top_logp, rest_logp, reverse, inv_temp)
 
 
 # ---- the same through the LM head: no [T, V] logits beyond a chunk of rows
@@ -671,14 +631,12 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
     T = hidden.shape[0]
     dh = torch.empty_like(hidden, memory_format=torch.contiguous_format) if needs[0] else None
     G = _head_gemm(hidden, weight)
-    dw = whole = None
+    dw = whole = buffer = None
     if needs[1]:
-        mg = getattr(weight, "main_grad", None)
-        if G is not None and mg is None and T <= chunk and getattr(weight, "_grad_in_flat_buffer", False) and weight.grad is not None \
-                and weight.grad.dtype == weight.dtype:
-            dw = weight.grad
-        elif G is not None and mg is not None and mg.dtype == torch.float32:
-            dw = mg
+        own = bool(getattr(weight, "_main_grad_hooked", False)) and len(weight._post_accumulate_grad_hooks or ()) == 1
+        buffer = _row_grad_buffer(weight) if G is not None and weight.is_leaf and lib().gradient_goes_past(weight, own) else None
+        if buffer is not None and (buffer.dtype == torch.float32 or (buffer.dtype == weight.dtype and T <= chunk)):
+            dw = buffer              # the products' fp32 sums are added to it; one of 16 bits would be rounded once a chunk
         elif G is None or T > chunk or T == 0:
             dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device)
     for s in range(0, T, chunk):
@@ -702,51 +660,60 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
             if dw is None:
                 whole = G.gemm(d, h, a_mn=True, b_mn=True)                                   # [t, V]^T x [t, H], rounded once
             else:
-                G.gemm(d, h, out=dw.view(weight.shape), a_mn=True, b_mn=True, accumulate=True)
-    if dw is not None and dw is not getattr(weight, "main_grad", None) and dw is not weight.grad:
+                G.gemm(d, h, out=dw, a_mn=True, b_mn=True, accumulate=True)
+    if dw is not None and dw is not buffer:
         whole = dw.to(weight.dtype)
     return dh, whole
 
 
 class _LMHeadTokenStats(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, labels, mask_bits, inv_temp, chunk):
+    def forward(ctx, hidden, weight, labels, mask_bits, inv_temp, chunk, keep_bytes):
         ctx.set_materialize_grads(False)
-        T = hidden.shape[0]
-        logp, entropy, lse = (torch.empty(T, dtype=torch.float32, device=hidden.device) for _ in range(3))
-        G = _head_gemm(hidden, weight)
-        for s in range(0, T, chunk):
-            e = min(T, s + chunk)
-            mb = None if mask_bits is None else mask_bits[s:e]
-            if G is not None and e - s > 256:      # (a row tile or less leaves half of the pairs idle: 16 / 256 rows of 4096 x 32000 66 / 78 us through logits, 87 / 97 fused)
-                r = lib().head_stats(G.tma_rows(hidden[s:e]), weight, labels[s:e], mb, inv_temp, G._sms(hidden.device))
-            else:
-                r = lib().token_stats(_head_logits(hidden[s:e], weight), labels[s:e], mb, inv_temp)
-            logp[s:e], entropy[s:e], lse[s:e] = r
-        ctx.save_for_backward(hidden, weight, labels, mask_bits, lse, entropy)
+        T, G = hidden.shape[0], _head_gemm(hidden, weight)
+        cut = lambda t, s, e: None if t is None else t[s:e]
+        kept = maxima = None
+        # keep the weights from width 1024 on: forming and reading them costs what the product of width 512 does (us, both passes up to d logits, kept / formed again:
+        # 8192 x 4096 x 32000 1583 / 2715, 2047 x 1024 x 50257 352 / 408, 8192 x 512 x 32000 484 / 486)
+        if (G is not None and T > 256 and hidden.shape[1] >= 1024 and any(ctx.needs_input_grad[:2]) and 2 * T * weight.shape[0] <= keep_bytes):
+            logp, entropy, lse, kept, maxima = lib().head_stats(G.tma_rows(hidden), weight, labels, mask_bits, inv_temp, True, G._sms(hidden.device))
+        else:
+            parts = []
+            for s in range(0, max(1, T), chunk):
+                e = min(T, s + chunk)
+                if G is not None and e - s > 256:
+                    # (a row tile or less leaves half of the pairs idle: 16 / 256 rows of 4096 x 32000 66 / 78 us through logits, 87 / 97 fused)
+                    parts.append(lib().head_stats(G.tma_rows(hidden[s:e]), weight, labels[s:e], cut(mask_bits, s, e), inv_temp, False, G._sms(hidden.device)))
+                else:
+                    parts.append(lib().token_stats(_head_logits(hidden[s:e], weight), labels[s:e], cut(mask_bits, s, e), inv_temp))
+            logp, entropy, lse = parts[0] if len(parts) == 1 else [torch.cat(p) for p in zip(*parts)]
+        ctx.save_for_backward(hidden, weight, labels, mask_bits, lse, entropy, kept, maxima)
         ctx.inv_temp, ctx.chunk = inv_temp, chunk
         return logp, entropy
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy):
-        hidden, weight, labels, mask_bits, lse, entropy = ctx.saved_tensors
+        hidden, weight, labels, mask_bits, lse, entropy, kept, maxima = ctx.saved_tensors
         if g_logp is None and g_entropy is None:
-            return (None,) * 6
+            return (None,) * 7
         gl, ge = _rows_f32(g_logp), _rows_f32(g_entropy)
         G = _head_gemm(hidden, weight)
+        cut = lambda t, s, e: None if t is None else t[s:e]
 
         def dlogits(s, e):
-            rows = (labels[s:e], None if mask_bits is None else mask_bits[s:e], lse[s:e], entropy[s:e], None if gl is None else gl[s:e],
-                    None if ge is None else ge[s:e], ctx.inv_temp)
+            d = _pitched(e - s, weight.shape[0], hidden.dtype, hidden.device) if G is not None else None
+            if kept is not None:
+                lib().head_grad(kept, maxima, labels, mask_bits, lse, entropy, gl, ge, ctx.inv_temp, d, s)
+                return d
+            rows = [cut(t, s, e) for t in (labels, mask_bits, lse, entropy, gl, ge)]
             if G is not None:
-                d = _pitched(e - s, weight.shape[0], hidden.dtype, hidden.device)
-                lib().head_stats_bwd(G.tma_rows(hidden[s:e]), weight, *rows, d, G._sms(hidden.device))
+                lib().head_stats_bwd(G.tma_rows(hidden[s:e]), weight, *rows, ctx.inv_temp, d, G._sms(hidden.device))
                 return d
             x = _head_logits(hidden[s:e], weight)
-            return lib().token_stats_bwd(x, *rows, x)
+            return lib().token_stats_bwd(x, *rows, ctx.inv_temp, x)
 
-        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None)
+        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None, None)
 
 
 def _check_head(op: str, hidden, weight, temperature, chunk, **rows):
@@ -764,17 +731,19 @@ def lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits=None, tempera
     return logprob_entropy_from_logits_ref(hidden.float() @ weight.float().t(), labels, mask_bits, 1.0 / temperature)
 
 
-def lm_head_logprobs_entropy(hidden, weight, labels, mask_bits=None, temperature: float = 1.0, chunk: int = 8192):
+def lm_head_logprobs_entropy(hidden, weight, labels, mask_bits=None, temperature: float = 1.0, chunk: int = 8192, keep_bytes: int = 1 << 31):
     """(log p(label), entropy) of p = softmax(hidden @ weight^T / temperature): hidden [T, H], weight [V, H], labels [T] -> fp32 [T] each,
-    differentiable in hidden and weight.  Logits stay in fp32 (`lm_head_logprobs` rounds them to the weights' type) and their gradient
-    exists for `chunk` rows at a time.  Labels and mask as in `logprob_entropy_from_logits`."""
+    differentiable in hidden and weight.  16-bit logits never exist (`lm_head_logprobs` rounds them to the weights' type): the
+    statistics come from the product's fp32 accumulators.  Their gradient exists for `chunk` rows at a time, from the weights of the softmax where these
+    take at most `keep_bytes` (2 T V) between the passes and H is 1024 or more, else (0: always) from the product formed again.  Labels and mask as in
+    `logprob_entropy_from_logits`."""
     op = "lm_head_logprobs_entropy"
     _check_head(op, hidden, weight, temperature, chunk, labels=labels, mask_bits=mask_bits)
     _check_labels(op, labels)
     if not use_native(hidden):
         return lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits, temperature)
     return _LMHeadTokenStats.apply(hidden, weight, labels.long().contiguous(), mask_bits.contiguous() if mask_bits is not None else None, 1.0 / temperature,
-                                   int(chunk))
+                                   int(chunk), int(keep_bytes))
 
 
 def lm_head_top_logprobs(hidden, weight, k: int, labels=None, mask_bits=None, temperature: float = 1.0, chunk: int = 4096) -> TopLogprobs:

@@ -476,7 +476,7 @@ def head_errors(h, w, c, V):
     return z, size * (h.shape[1] / 16 + 4) * 2.0 ** -22 + U * z.abs()
 
 
-def check_head(dev, T, H, V, dtype, masked, temp, chunk, seed, buffer=None, top=None):
+def check_head(dev, T, H, V, dtype, masked, temp, chunk, seed, buffer=None, keep=1 << 31):
     h, w, labels = make_head(T, H, V, dtype, seed)
     c = 1.0 / temp
     mask = bits = None
@@ -498,7 +498,7 @@ def check_head(dev, T, H, V, dtype, masked, temp, chunk, seed, buffer=None, top=
         else:
             wd.main_grad = old.to(dev).clone()
         old = old.double()
-    logp, ent = OF.lm_head_logprobs_entropy(hd, wd, labels.to(dev), bits, temperature=temp, chunk=chunk)
+    logp, ent = OF.lm_head_logprobs_entropy(hd, wd, labels.to(dev), bits, temperature=temp, chunk=chunk, keep_bytes=keep)
     torch.autograd.backward([logp, ent], [gl.to(dev), ge.to(dev)])
     z, ez = head_errors(h, w, c, V)
     if mask is not None:
@@ -514,7 +514,12 @@ def check_head(dev, T, H, V, dtype, masked, temp, chunk, seed, buffer=None, top=
     d = grad64(y, p, want_H, labels, gl.double(), ge.double(), c).masked_fill(empty[:, None], 0.0)
     size = c * p * (gl.abs()[:, None] + ge.abs()[:, None] * (torch.where(p > 0, -y, 0.0) + want_H[:, None] + 1)) * 4 * e + c * U * (gl.abs()[:, None] + 1)
     r = half_step(dtype)
-    ed = (r * d.abs() + size + torch.finfo(dtype).tiny).masked_fill(empty[:, None], 0.0)
+    # kept weights e, relative to the largest of 128 columns, are rounded by at most 2^-12 of e or, below 2^-29, 2^-40 (their logarithm by as much more): of a
+    # probability p e^(their distance) <= p_max that is within 2 * 2^-12 of the size of the gradient's parts and 2^-40 of what a probability of 1 would give
+    kept = T > 256 and H >= 1024 and keep > 0 and dtype != torch.float32
+    whole = c * (gl.abs()[:, None] + ge.abs()[:, None] * (want_H[:, None] + 30))
+    more = (2.0 ** -11 * (size / (4 * e)) + 2.0 ** -40 * whole) if kept else 0.0
+    ed = (r * d.abs() + size + more + torch.finfo(dtype).tiny).masked_fill(empty[:, None], 0.0)
     W, Hh = w.double(), h.double()
     for got, want, slack, n in ((hd.grad, d @ W, ed @ W.abs() + (d.abs() @ W.abs()) * (V / 16 + 4) * 2.0 ** -22, 1),
                                 (wd.main_grad if buffer == "fp32" else wd.grad, d.t() @ Hh + old, ed.t() @ Hh.abs() + (d.abs().t() @ Hh.abs()) * (T / 16 + 4) * 2.0 ** -22,
@@ -536,9 +541,12 @@ def test_head_cpu(T, H, V, masked, temp, chunk):
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,H,V,masked,temp,chunk", HEADS + [(1, 64, 1000, False, 1.0, 8192), (130, 256, 1001, True, 1.3, 8192), (300, 136, 5003, False, 1.0, 128),
-                                                             (257, 512, 2048, True, 1.0, 8192), (513, 64, 32000, False, 1.0, 8192), (40, 60, 100, False, 1.0, 8192)])
+                                                             (257, 512, 2048, True, 1.0, 8192), (513, 64, 32000, False, 1.0, 8192), (40, 60, 100, False, 1.0, 8192),
+                                                             (270, 1032, 1001, True, 0.8, 8192), (300, 1024, 4096, False, 1.0, 128)])
 def test_head_gpu(T, H, V, masked, temp, chunk, dtype):
     check_head("cuda", T, H, V, dtype, masked, temp, chunk, seed=T)
+    if T > 256:
+        check_head("cuda", T, H, V, dtype, masked, temp, chunk, seed=T, keep=0)
 
 
 @gpu
@@ -548,6 +556,37 @@ def test_head_gradient_into_a_buffer_gpu(T, chunk, buffer):
     if buffer == "weight_type" and T > chunk:
         pytest.skip("several chunks keep an fp32 sum and leave the buffer to autograd")
     check_head("cuda", T, 128, 1000, torch.bfloat16, False, 1.0, chunk, 7, buffer=buffer)
+
+
+@gpu
+@pytest.mark.parametrize("buffer", ["weight_type", "fp32"])
+def test_head_gradient_is_given_to_who_asks_for_it_gpu(buffer):
+    """With a gradient buffer on the weight, `torch.autograd.grad` returns the gradient and leaves the buffer as it was."""
+    h, w, labels = make_head(70, 64, 500, torch.bfloat16, 3, "cuda")
+    w = torch.nn.Parameter(w)
+    logp, ent = OF.lm_head_logprobs_entropy(h, w, labels)
+    (want,) = torch.autograd.grad(logp.sum() + ent.sum(), [w])
+    old = torch.ones(500, 64, dtype=w.dtype if buffer == "weight_type" else torch.float32, device="cuda")
+    if buffer == "weight_type":
+        w.grad, w._grad_in_flat_buffer = old.clone(), True
+    else:
+        w.main_grad = old.clone()
+    logp, ent = OF.lm_head_logprobs_entropy(h, w, labels)
+    (got,) = torch.autograd.grad(logp.sum() + ent.sum(), [w])
+    assert torch.equal(got, want) and torch.equal(w.grad if buffer == "weight_type" else w.main_grad, old)
+
+
+@gpu
+def test_inside_function_transforms_gpu():
+    x, labels = make_logits(3, 50, torch.float32, 1, "cuda")
+    o = OF.top_logprobs_from_logits(x, 4)
+    e = err(x.cpu().double(), 50)
+    for f in (lambda v: OF.logprob_entropy_from_logits(v, labels)[1].sum(), lambda v: OF.distill_loss_from_logits(v * 0.5, o.top_ids, o.top_logp, o.rest_logp).sum()):
+        got = torch.func.grad(f)(x)
+        leaf = x.clone().requires_grad_(True)
+        f(leaf).backward()
+        # two results of the bounds above for gradients whose parts are at most 1 + the entropy's 4
+        assert ((got - leaf.grad).abs() <= 2 * 4 * e * 5 + 8 * U).all()
 
 
 @gpu
