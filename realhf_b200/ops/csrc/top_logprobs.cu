@@ -28,7 +28,7 @@ RB_DEVICE uint32_t order_key(float x) {  // order-preserving float -> uint, -0 a
 RB_DEVICE float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 constexpr uint32_t kKeyNone = 0x007fffffu;  // order_key(-inf)
 
-constexpr int kFastTop = 256, kMaxRecords = 12288;
+constexpr int kFastTop = 256, kMaxRecords = 12288, kCountAll = 128;
 
 struct TopShared {
   float red[96];
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
     for (int b = 0; b < B; ++b) sh.keys[b * kThreads + threadIdx.x] = order_key(share[b]);
     __syncthreads();
     if (threadIdx.x < 32) {
-      const uint32_t t = k <= 32 ? bound_of<4>(k, sh.keys) : bound_of<kShares / 32>(k, sh.keys);
+      const uint32_t t = k <= 32 ? bound_of<4>(k, sh.keys) : k <= 64 ? bound_of<8>(k, sh.keys) : bound_of<kShares / 32>(k, sh.keys);
       if (threadIdx.x == 0) sh.digit = max(t, kKeyNone + 1);
     }
     __syncthreads();
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
     }
   };
   float* after;                             // candidates that are not chosen, in order
-  if (n <= 96) {
+  if (n <= kCountAll) {
     after = reinterpret_cast<float*>(sh.ordered);
     if (threadIdx.x == 0 && (n & 1)) sh.list[n] = 0;
     __syncthreads();
@@ -409,9 +409,9 @@ int rb_top_logprobs(const void* logits, int64_t row_stride, const int64_t* label
   if (k < 1 || k > kMaxTop || k > V) return -1;
   // pieces a group: one where groups of four are too few to bound the k-th logit
   const int vec = V / (dt == 0 ? 4 : 8), p = vec >= 8 * k ? 4 : 1;
-  // threads: as for the statistics, but no fewer than keep 1024 resident beside what a block has in shared memory, and all of them for few rows
+  // threads: as for the statistics, but no fewer than keep 1024 resident beside what a block has in shared memory
   const int64_t bytes = sizeof(TopShared) + 1024 + (int64_t)vec / p * 8;
-  const int nt = rows < 4 * rb::kNumSMs ? 512 : bytes <= 45 << 10 ? 128 : 256;
+  const int nt = rows < 4 * rb::kNumSMs ? 512 : rows >= 16 * rb::kNumSMs && bytes <= 45 << 10 ? 128 : 256;
 #define RB_L4(T, M, NT, P)                                                                                                                                 \
   {                                                                                                                                                        \
     const int groups = RB_CEIL_DIV(vec, P * NT);                                                                                                           \
