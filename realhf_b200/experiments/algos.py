@@ -155,6 +155,7 @@ class PPOHyperparameters:
     reward_output_scaling: float = 1.0
     reward_output_bias: float = 0.0
     early_stop_imp_ratio: float = 5.0
+    entropy_coef: float = 0.0
     use_adaptive_kl_ctl: bool = False
     adv_norm: bool = True
     value_norm: bool = True
@@ -203,7 +204,8 @@ class PPOConfig(CommonExperimentConfig):
         p = self.ppo
         kw = self.ppo_kwargs
         actor_itf = ModelInterfaceAbstraction("ppo_actor", args={**copy.deepcopy(kw), "generation_config": dataclasses.asdict(p.gen),
-                                                                 "early_stop_imp_ratio": p.early_stop_imp_ratio, "adv_norm": p.adv_norm})
+                                                                 "early_stop_imp_ratio": p.early_stop_imp_ratio, "entropy_coef": p.entropy_coef,
+                                                                 "adv_norm": p.adv_norm})
         ref_itf = copy.deepcopy(actor_itf)
         ref_itf.args["enable_save"] = False
         critic_kw = {k: v for k, v in kw.items() if k != "eps_clip"}

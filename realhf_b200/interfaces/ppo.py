@@ -50,16 +50,24 @@ def _save_hf(model: Model, save_dir: str):
 
 
 def _actor_loss_from_output(out: ModelOutput, mb: SequenceSample, *, kl_adapter, eps_clip: float, temperature: float,
-                            early_stop_imp_ratio: Optional[float], early_stop_kl: Optional[float]):
+                            early_stop_imp_ratio: Optional[float], early_stop_kl: Optional[float], entropy_coef: float = 0.0):
     seqlens = mb.flat_seqlens("packed_input_ids")
     rows, labels = IF.shifted_rows_and_labels(seqlens, mb.data["packed_input_ids"])
     mask_bits = mb.data.get("packed_logits_mask")
-    logp = out.logprobs(labels, mask_bits, temperature, rows)
     loss_mask = mb.data["ppo_loss_mask"].bool()
+    entropy = None
+    if entropy_coef != 0.0:     # mean entropy of the answer's distributions (over the tokens that sampling could choose) as a bonus
+        logp, entropy = out.logprobs_entropy(labels, mask_bits, temperature, rows)
+    else:
+        logp = out.logprobs(labels, mask_bits, temperature, rows)
     loss, stat = IF.actor_loss_fn(logp, mb.data["old_logp"], mb.data["advantages"], eps_clip, loss_mask)
     n = loss_mask.count_nonzero().clamp(min=1)
     stat = dict(ppo_approx_kl=stat["approx_kl"], actor_clip_ratio=stat["clip_ratio"],
                 importance_weight=stat["importance_weight"], actor_loss=loss.detach())
+    if entropy is not None:
+        entropy = torch.where(loss_mask, entropy, torch.zeros_like(entropy)).sum() / n
+        stat["entropy"] = entropy.detach()
+        loss = loss - entropy_coef * entropy
     # early stopping: zero the loss on the device (no host sync) when the policy drifted too far
     if early_stop_imp_ratio is not None:
         loss = loss * (stat["importance_weight"] <= early_stop_imp_ratio).float()
@@ -96,6 +104,7 @@ class PPOActorInterface(ModelInterface):
     max_reward_clip: float = 5.0
     early_stop_kl: Optional[float] = None
     early_stop_imp_ratio: Optional[float] = None
+    entropy_coef: float = 0.0
     adaptive_kl_ctl: bool = False
     adaptive_kl_target: Optional[float] = 6
     adaptive_kl_horizon: Optional[float] = 10000
@@ -213,7 +222,7 @@ class PPOActorInterface(ModelInterface):
                     prompt_len=prompt_mask.count_nonzero(), seq_len=float(sum(seqlens)))
         loss_fn = functools.partial(_actor_loss_from_output, kl_adapter=self.kl_adapter, eps_clip=self.eps_clip,
                                     temperature=self.gconfig.temperature, early_stop_imp_ratio=self.early_stop_imp_ratio,
-                                    early_stop_kl=self.early_stop_kl)
+                                    early_stop_kl=self.early_stop_kl, entropy_coef=self.entropy_coef)
         train_stats: Dict[str, torch.Tensor] = collections.defaultdict(float)
         for mb in minibatches:
             st = eng.train_batch(mb, loss_fn, version_steps=model.version.global_step, num_micro_batches=n_mbs)

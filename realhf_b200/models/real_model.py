@@ -117,6 +117,53 @@ class ModelOutput:
             return TP.vocab_parallel_logprobs(local, labels, self.ctx, temperature, mask_bits)
         return OF.lm_head_logprobs(h, self.head_weight, labels, mask_bits, temperature)
 
+    def _whole_logits(self, rows: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        """The rows' logits over the whole vocabulary where the head's operators cannot form them themselves (a vocabulary-sharded head, a soft cap; the cap
+        and a fixed factor are applied), else None."""
+        tp = self.ctx is not None and self.ctx.tp_size > 1
+        if not tp and self.softcap is None:
+            return None
+        h = self.hidden if rows is None else self.hidden.index_select(0, rows)
+        lg = OF.linear(TP.copy_to_tp(h, self.ctx) if tp else h, self.head_weight)
+        lg = TP.gather_last_dim(lg, self.ctx) if tp else lg
+        if self.logit_scale is not None:
+            lg = lg.float() * self.logit_scale
+        if self.softcap is not None:    # (the cap's kernel has no gradient)
+            lg = self.softcap * torch.tanh(lg.float() / self.softcap) if torch.is_grad_enabled() and lg.requires_grad else OF.softcap_logits(lg, self.softcap)
+        return lg
+
+    def _head_rows(self, rows, temperature: float):
+        assert not self.is_critic, "a value head has no token distribution"
+        h = self.hidden if rows is None else self.hidden.index_select(0, rows)
+        return h, self.head_weight, temperature if self.logit_scale is None else temperature / self.logit_scale
+
+    def logprobs_entropy(self, labels: torch.Tensor, mask_bits: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                         rows: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """fp32 log p(labels[i] | hidden[rows[i]]) and the entropy of that distribution, both differentiable (`OF.lm_head_logprobs_entropy`)."""
+        lg = self._whole_logits(rows)
+        if lg is not None:
+            return OF.logprob_entropy_from_logits(lg, labels, mask_bits, 1.0 / temperature)
+        h, w, temperature = self._head_rows(rows, temperature)
+        return OF.lm_head_logprobs_entropy(h, w, labels, mask_bits, temperature)
+
+    def top_logprobs(self, k: int, labels: Optional[torch.Tensor] = None, mask_bits: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                     rows: Optional[torch.Tensor] = None) -> "OF.TopLogprobs":
+        """The k most likely next tokens of hidden[rows], their log-probabilities and the log of the others' mass: what a teacher hands over."""
+        lg = self._whole_logits(rows)
+        if lg is not None:
+            return OF.top_logprobs_from_logits(lg, k, labels, mask_bits, 1.0 / temperature)
+        h, w, temperature = self._head_rows(rows, temperature)
+        return OF.lm_head_top_logprobs(h, w, k, labels, mask_bits, temperature)
+
+    def distill_loss(self, top_ids: torch.Tensor, top_logp: torch.Tensor, rest_logp: Optional[torch.Tensor] = None, reverse: bool = False,
+                     temperature: float = 1.0, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Divergence per row of hidden[rows] from a teacher known by `top_logprobs` (`OF.distill_loss_from_logits`), differentiable."""
+        lg = self._whole_logits(rows)
+        if lg is not None:
+            return OF.distill_loss_from_logits(lg, top_ids, top_logp, rest_logp, reverse, 1.0 / temperature)
+        h, w, temperature = self._head_rows(rows, temperature)
+        return OF.lm_head_distill_loss(h, w, top_ids, top_logp, rest_logp, reverse, temperature)
+
 
 class ReaLModel(nn.Module):
     def __init__(self, config: ReaLModelConfig, ctx: Optional[ParallelContext] = None, dtype=torch.bfloat16,

@@ -644,6 +644,142 @@ def test_chain_gpu(dtype):
     check_chain("cuda", dtype)
 
 
+# ------------------------------------------------------------------------------------------------ a model's output, the actor's entropy bonus
+
+
+def check_model_output(dev, dtype, softcap, scale):
+    """`ModelOutput`'s calls against 64 bits, with a soft cap on the logits, a fixed factor, both and neither.  Bound: as for the head; a cap forms
+    cap tanh(z / cap) in fp32, 8 u of it, from logits that the capped path rounds to the model's type."""
+    from realhf_b200.models.real_model import ModelOutput
+    T, H, V, k = 11, 64, 300, 6
+    h, w, labels = make_head(T, H, V, dtype, 5, dev)
+    rows = torch.tensor([0, 3, 4, 10], device=dev)
+    lab = labels[rows]
+
+    def z64(hidden):
+        z = hidden.cpu().double()[rows.cpu()] @ w.cpu().double().t()
+        z = z * (1.0 if scale is None else scale)
+        return (z if softcap is None else softcap * torch.tanh(z / softcap)) / 0.9
+
+    rounding = half_step(dtype) if softcap is not None and dtype != torch.float32 else 0.0
+    z = z64(h)
+    slack = 4 * (err(z, V) + float(z.abs().max()) * (2.0 ** -19 + rounding))
+    out = ModelOutput(hidden=h.clone().requires_grad_(True), head_weight=w, ctx=None, softcap=softcap, logit_scale=scale)
+    logp, ent = out.logprobs_entropy(lab, None, 0.9, rows)
+    y, p, want_logp, want_H = stats64(z, lab.cpu())
+    assert ((logp.detach().cpu().double() - want_logp).abs() <= slack * 2).all() and ((ent.detach().cpu().double() - want_H).abs() <= slack * (1 + want_H) * 2).all()
+    top = out.top_logprobs(k, lab, None, 0.9, rows)
+    assert ((top.top_logp.cpu().double() - torch.sort(y, -1, descending=True).values[:, :k]).abs() <= 2 * slack).all()
+    assert ((top.logp.cpu().double() - want_logp).abs() <= 2 * slack).all()
+    assert ((top.top_logp.exp().sum(-1) + top.rest_logp.exp() - 1).abs() <= 1e-5).all()
+    ids, t, tr = make_teacher(z, k, 3, True)
+    loss = out.distill_loss(ids.to(dev), t.to(dev), tr.to(dev), False, 0.9, rows)
+    want = distill64(z, ids, t, tr, False)[0]
+    assert ((loss.detach().cpu().double() - want).abs() <= slack * 4).all()
+    (d,) = torch.autograd.grad([logp.sum() + ent.sum() + loss.sum()], [out.hidden])
+    # against a difference quotient of the 64-bit function along a direction; the parts' gradients are rounded twice to the type on the way
+    v = torch.randn(T, H, generator=torch.Generator().manual_seed(6)).double()
+
+    def f(hidden):
+        z = z64(hidden)
+        return stats64(z, lab.cpu())[2].sum() + stats64(z, lab.cpu())[3].sum() + distill64(z, ids, t, tr, False)[0].sum()
+
+    s = 1e-5
+    want = (f(h.cpu().double() + s * v) - f(h.cpu().double() - s * v)) / (2 * s)
+    got = (d.cpu().double() * v).sum()
+    size = float((d.cpu().double().abs() * v.abs()).sum())
+    assert abs(float(got - want)) <= size * (6 * half_step(dtype) + 20 * slack) + 1e-6
+    assert not d[1].any()
+
+
+@pytest.mark.parametrize("softcap,scale", [(None, None), (20.0, None), (None, 0.5), (20.0, 0.5)])
+def test_model_output_cpu(softcap, scale):
+    check_model_output("cpu", torch.float32, softcap, scale)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("softcap,scale", [(None, None), (20.0, None), (None, 0.5), (20.0, 0.5)])
+def test_model_output_gpu(softcap, scale, dtype):
+    check_model_output("cuda", dtype, softcap, scale)
+
+
+def _sharded_output(rank, world):
+    """Every rank's share of a vocabulary-sharded head: the calls and the gradient of the whole hidden states."""
+    from realhf_b200.base.topology import ParallelContext, ProcessTopology
+    from realhf_b200.models.real_model import ModelOutput
+    ctx = ParallelContext.build(ProcessTopology(1, 1, world), list(range(world)), rank, backend="gloo")
+    h, w, labels = make_head(9, 32, 64, torch.float32, 2)
+    per = 64 // world
+    hidden, shard = h.clone().requires_grad_(True), w[rank * per: (rank + 1) * per].clone().requires_grad_(True)
+    out = ModelOutput(hidden=hidden, head_weight=shard, ctx=ctx)
+    logp, ent = out.logprobs_entropy(labels)
+    top = out.top_logprobs(5, labels)
+    loss = out.distill_loss(top.top_ids, top.top_logp - 0.1, top.rest_logp)
+    (logp.sum() + ent.sum() + loss.sum()).backward()
+    return [t.detach().tolist() for t in (logp, ent, loss, top.top_logp, top.top_ids, hidden.grad, shard.grad)]
+
+
+@pytest.mark.distributed
+def test_model_output_with_a_sharded_head_cpu():
+    from realhf_b200.base.testing import run_distributed
+    one = run_distributed(_sharded_output, 1)[0]
+    two = run_distributed(_sharded_output, 2)
+    for r, got in enumerate(two):
+        for a, b in zip(one[:6], got[:6]):
+            torch.testing.assert_close(torch.tensor(a), torch.tensor(b), atol=1e-5, rtol=1e-5)
+        torch.testing.assert_close(torch.tensor(one[6][32 * r: 32 * r + 32]), torch.tensor(got[6]), atol=1e-5, rtol=1e-5)
+
+
+def test_actor_loss_with_an_entropy_bonus_cpu():
+    """The bonus is the masked mean entropy times its coefficient; without one the loss is what it was."""
+    from types import SimpleNamespace
+    from realhf_b200.interfaces import ppo
+    from realhf_b200.models.real_model import ModelOutput
+    T, H, V = 12, 32, 50
+    h, w, _ = make_head(T, H, V, torch.float32, 1)
+    ids = torch.arange(T) % V
+    n = T - 2
+    mask = torch.ones(n, dtype=torch.bool)
+    mask[:3] = False
+    data = dict(packed_input_ids=ids, old_logp=torch.full((n,), -3.0), advantages=torch.linspace(-1, 1, n), ppo_loss_mask=mask)
+    mb = SimpleNamespace(data=data, flat_seqlens=lambda key: [5, 7])
+    kw = dict(kl_adapter=None, eps_clip=0.2, temperature=1.0, early_stop_imp_ratio=None, early_stop_kl=None)
+    grads = []
+    for coef in (0.0, 0.3):
+        hidden = h.clone().requires_grad_(True)
+        loss, stat = ppo._actor_loss_from_output(ModelOutput(hidden=hidden, head_weight=w, ctx=None), mb, entropy_coef=coef, **kw)
+        loss.backward()
+        grads.append((loss.detach(), stat, hidden.grad))
+    rows = torch.tensor([0, 1, 2, 3, 5, 6, 7, 8, 9, 10])
+    hidden = h.clone().requires_grad_(True)
+    p = torch.softmax(hidden[rows] @ w.t(), -1)
+    mean = (torch.special.entr(p).sum(-1) * mask).sum() / mask.sum()
+    mean.backward()
+    assert "entropy" not in grads[0][1] and abs(float(grads[1][1]["entropy"] - mean.detach())) < 1e-5
+    assert abs(float(grads[1][0] - (grads[0][0] - 0.3 * mean.detach()))) < 1e-5
+    torch.testing.assert_close(grads[1][2], grads[0][2] - 0.3 * hidden.grad, atol=1e-6, rtol=1e-4)
+
+
+def test_ppo_iterations_with_an_entropy_bonus_cpu():
+    from test_engine_cpu import make_model
+    from realhf_b200.api.data import SequenceSample
+    from realhf_b200.interfaces import basic, ppo
+    torch.manual_seed(0)
+    actor, critic = make_model("actor"), make_model("critic", critic=True)
+    ref, rew = make_model("ref", train=False), make_model("reward", critic=True, train=False, seed=7)
+    a = ppo.PPOActorInterface(n_minibatches=2, generation_config=dict(max_new_tokens=6, min_new_tokens=2, top_k=50, top_p=0.9), entropy_coef=0.01)
+    c = ppo.PPOCriticInterface(n_minibatches=2)
+    plens = [5, 7, 4, 6]
+    prompts = SequenceSample.from_default(seqlens=plens, ids=list(range(4)), data=dict(packed_prompts=torch.randint(2, 128, (sum(plens),))))
+    d = a.generate(actor, prompts, n_mbs=1)
+    d.update_(a.inference(ref, d))
+    d.update_(c.inference(critic, d))
+    d.update_(basic.PairedRewardInterface().inference(rew, d))
+    st = a.train_step(actor, d, n_mbs=1)
+    assert 0 < st["entropy"] < math.log(128) and st["actor_loss"] == st["actor_loss"]
+
+
 # ------------------------------------------------------------------------------------------------ streams, graphs, sizes, refusals
 
 
