@@ -5,16 +5,20 @@
 // token fills holds id -1 and -inf.  The rest's mass is summed over the tokens it consists of: 1 - sum of the chosen would cancel where they
 // hold nearly all of it.
 //
-// The row is read once.  Every thread keeps the maximum and the sum of each of its groups (vocab_rows.cuh) in shared memory.  The k-th largest of the
-// maxima of 512 shares of the row, to 16 bits, is a lower bound of the k-th largest logit: k shares hold an element at least as large; only some k .. 2 k elements
-// reach it.  The groups whose maximum does are looked at again, a lane a piece, and give the candidates; the mass of the rest is what these groups leave plus the sums
-// of all others.  A candidate's place is the number of candidates before it in the order: counted among all of them where they are few, else among those of its
-// bucket, 512 equal intervals of the value (a bitonic sort of 128, a barrier for each of its 28 stages, took 7400 cycles; counting among 400 by 128 threads 28000).
-// More than 256 alternatives, more than 1024 groups or candidates at the bound (ties), and rows of more than 12288 groups take a radix descent instead:
+// The row is read once.  Every thread keeps, for each of its groups (vocab_rows.cuh), the maxima of its two halves (fp32: of the group) and its sum in shared
+// memory.  The k-th largest of the maxima of 512 shares of the row, to 16 bits, is a lower bound of the k-th largest logit: k shares hold an element at least as large;
+// only some k .. 2 k elements reach it.  The halves whose maximum does are read again, a lane a half, and give the candidates; the mass of the rest is the groups'
+// sums less their candidates', or, where candidates are more than 64 times what is left, the group's other elements added up again.  (With whole groups read
+// again, pieces of 64 bytes in memory that the cache had dropped, 256 alternatives of 8192 x 32000 read 1.6 times the logits.)  A candidate's place is the number of
+// candidates before it in the order: counted among all of them where they are few, else among those of its bucket, 512 equal intervals of the value (a bitonic sort of
+// 128, a barrier for each of its 28 stages, took 7400 cycles; counting among 400 by 128 threads 28000).
+// More than 256 alternatives, more than 768 halves or 1024 candidates at the bound (ties), and rows of more than 12288 groups take a radix descent instead:
 // the k-th largest value by its bits (four digits of 8 bits, a histogram in shared memory each), the elements above it in any order, of those equal to it the
 // first in index order.
 // Sums have a fixed order whichever way candidates arrive.
 #include "vocab_rows.cuh"
+
+#include <algorithm>
 
 namespace {
 
@@ -28,23 +32,55 @@ RB_DEVICE uint32_t order_key(float x) {  // order-preserving float -> uint, -0 a
 RB_DEVICE float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 constexpr uint32_t kKeyNone = 0x007fffffu;  // order_key(-inf)
 
-constexpr int kFastTop = 256, kMaxRecords = 12288, kCountAll = 128;
+constexpr int kFastTop = 256, kMaxRecords = 12288, kMaxHalves = 768, kCountAll = 128;
 
 struct TopShared {
   float red[96];
-  union {
-    uint32_t hist[kShares];
-    uint32_t keys[kShares];
-  };
   uint32_t warp_n[32];
   uint32_t digit, above, count, selected, kth;
   int last;
   alignas(16) uint64_t list[kMaxTop];   // key << 32 | ~index: descending order is the order wanted
-  union {
-    uint16_t group[kMaxTop];            // groups to look at again: number * threads + thread
-    uint64_t ordered[kMaxTop];          // the list by buckets
+  union {                               // one after the other
+    uint32_t keys[kShares];
+    struct {
+      uint32_t half[kMaxHalves];        // halves to look at again: 2 * group + which, groups numbered step * threads + thread
+      float hit_sum[kMaxHalves];        // their candidates' sums
+    };
+    uint32_t hist[kShares];
+    float after[kCountAll * 2];
   };
 };
+
+// What a group's record says of its maxima: of 16-bit types those of the first and the second half of its pieces, side by side; of fp32 the whole group's.  Returns the
+// group's maximum.
+template <typename T, int P> constexpr int kHalfPieces = rb::Word<T>::N == 2 && P > 1 ? P / 2 : P;
+template <typename T, int P> RB_DEVICE float half_maxima(const int4 (&raw)[P], uint32_t& halves) {
+  if constexpr (rb::Word<T>::N == 1) {
+    const float m = rb::group_max<T>(raw);
+    halves = __float_as_uint(m);
+    return m;
+  } else {
+    constexpr int NW = P * 4, HW = kHalfPieces<T, P> * 4;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+    uint32_t a = w[0], b = HW == NW ? rb::Word<T>::kNone : w[HW % NW];
+#pragma unroll
+    for (int i = 1; i < HW; ++i) a = rb::Word<T>::max(a, w[i]);
+#pragma unroll
+    for (int i = HW + 1; i < NW; ++i) b = rb::Word<T>::max(b, w[i]);
+    halves = rb::Word<T>::max(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+    float lo, hi;
+    rb::Word<T>::values(halves, lo, hi);
+    return rb::max_nan(lo, hi);
+  }
+}
+template <typename T> RB_DEVICE void half_values(uint32_t halves, float& lo, float& hi) {
+  if constexpr (rb::Word<T>::N == 2) {
+    rb::Word<T>::values(halves, lo, hi);
+  } else {
+    lo = __uint_as_float(halves);
+    hi = -INFINITY;
+  }
+}
 
 template <typename T> struct TopRow {
   const T* lr;
@@ -163,24 +199,35 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
                                                                                  float* __restrict__ rest, int V, int k, float inv_temp, int records) {
   constexpr int VEC = rb::RowSpan<T>::VEC, kStep = P * kThreads;
   __shared__ TopShared sh;
-  extern __shared__ float2 rec[];           // [group][thread]: maximum and sum
+  extern __shared__ uint2 rec[];            // [step][thread]: maxima of a group's halves, its sum; later the list by buckets
   const int64_t row = blockIdx.x;
   const TopRow<T> r{logits + row * row_stride, kMask ? mask + row * mask_stride : nullptr, V};
   const float kk = inv_temp * rb::kLog2e;
   const rb::RowSpan<T> span(r.lr, V);
   const int lane = threadIdx.x & 31;
   const bool fast = records > 0;
+  constexpr int B = kShares / kThreads;
+  float share[B];                           // maxima of the thread's shares: every so many-th group each, the edge with the first
+#pragma unroll
+  for (int b = 0; b < B; ++b) share[b] = -INFINITY;
   rb::RunningStats<T, true> run;
   auto bits = [&](int i) { return rb::mask_bits<VEC>(r.mr, mask_stride, span.head + i * VEC); };
   rb::walk_groups<T, kThreads, P, kMask>(r.lr + span.head, span.nvec, bits, [&](const int4 (&raw)[P], int i0, bool whole) {
-    const float mg = rb::group_max<T>(raw);
+    uint32_t halves;
+    const float mg = half_maxima<T>(raw, halves);
     run.raise(mg, kk);
     rb::Sums g;
     if (kMask || !whole) rb::group_add<T, true, true>(raw, run.reference(), kk, g);
     else rb::group_add<T, true, false>(raw, run.reference(), kk, g);
     run.sums.s2 = rb::add2(run.sums.s2, g.s2);
     run.sums.w2 = rb::add2(run.sums.w2, g.w2);
-    if (fast) rec[i0 / kStep * kThreads + threadIdx.x] = make_float2(mg, g.s());
+    if (fast) {
+      const int step = i0 / kStep;
+      rec[step * kThreads + threadIdx.x] = make_uint2(halves, __float_as_uint(g.s()));
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (step % B == b) share[b] = fmaxf(share[b], mg);
+    }
   });
   if (run.again()) {
     run.sums.w2 = 0;
@@ -216,26 +263,17 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
   int n = kMaxTop + 1;
   float lowest = 0.f;                       // no candidate lies below
   if (fast) {
-    // a group's sum was taken against the thread's largest value so far: bring it to the row's; the thread's kShares / kThreads shares: every so many-th group,
-    // the edge with the first
-    constexpr int B = kShares / kThreads;
-    float share[B], so_far = -INFINITY;
-    share[0] = ex;
 #pragma unroll
-    for (int b = 1; b < B; ++b) share[b] = -INFINITY;
-    for (int g0 = 0; g0 < groups; g0 += B) {
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        if (g0 + b < groups) {
-          float2& v = rec[(g0 + b) * kThreads + threadIdx.x];
-          so_far = fmaxf(so_far, v.x);
-          share[b] = fmaxf(share[b], v.x);
-          v.y *= rb::exp2_fast(fmaxf((so_far - st.m) * kk, -1000.f));
-        }
-      }
+    for (int b = 0; b < B; ++b) sh.keys[b * kThreads + threadIdx.x] = order_key(b == 0 ? fmaxf(share[0], ex) : share[b]);
+    // a group's sum was taken against the thread's largest value so far: bring it to the row's
+    float so_far = -INFINITY;
+    for (int g = 0; g < groups; ++g) {
+      uint2& v = rec[g * kThreads + threadIdx.x];
+      float lo, hi;
+      half_values<T>(v.x, lo, hi);
+      so_far = fmaxf(so_far, fmaxf(lo, hi));
+      v.y = __float_as_uint(__uint_as_float(v.y) * rb::exp2_fast(fmaxf((so_far - st.m) * kk, -1000.f)));
     }
-#pragma unroll
-    for (int b = 0; b < B; ++b) sh.keys[b * kThreads + threadIdx.x] = order_key(share[b]);
     __syncthreads();
     if (threadIdx.x < 32) {
       const uint32_t t = k <= 32 ? bound_of<4>(k, sh.keys) : k <= 64 ? bound_of<8>(k, sh.keys) : bound_of<kShares / 32>(k, sh.keys);
@@ -257,12 +295,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
       return __shfl_sync(0xffffffffu, at, 31) + before - mine;
     };
     const int all_groups = RB_CEIL_DIV(span.nvec, kStep);
-    for (int g0 = 0; g0 < all_groups; g0 += 32) {
+    for (int g0 = 0; g0 < all_groups; g0 += 16) {
       uint32_t hits = 0;
-      for (int g = g0; g < min(groups, g0 + 32); ++g) hits |= (uint32_t)(rec[g * kThreads + threadIdx.x].x >= bound_x) << (g - g0);
+      for (int g = g0; g < min(groups, g0 + 16); ++g) {
+        float lo, hi;
+        half_values<T>(rec[g * kThreads + threadIdx.x].x, lo, hi);
+        hits |= ((uint32_t)(lo >= bound_x) | (uint32_t)(hi >= bound_x) << 1) << (2 * (g - g0));
+      }
       uint32_t at = places(hits, sh.selected);
-      for (; hits; hits &= hits - 1, ++at)
-        if (at < kMaxTop) sh.group[at] = (uint16_t)((g0 + __ffs(hits) - 1) * kThreads + threadIdx.x);
+      for (; hits; hits &= hits - 1, ++at) {
+        const int b = __ffs(hits) - 1;
+        if (at < kMaxHalves) sh.half[at] = 2 * ((g0 + b / 2) * kThreads + threadIdx.x) + (b & 1);
+      }
     }
     if (threadIdx.x < 32) {
       const uint32_t at = places(ex >= bound_x, sh.count);
@@ -270,41 +314,71 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
     }
     __syncthreads();
     const int selected = sh.selected;
-    if (selected <= kMaxTop) {
-      // a lane a piece of a chosen group, P lanes a group: the pieces' sums add up in a fixed order
-      for (int q0 = 0; q0 < selected * P; q0 += kThreads) {
-        const int q = q0 + threadIdx.x, u = q % P;
-        const bool on = q < selected * P;
-        const int id = on ? sh.group[q / P] : 0, piece = id / kThreads * kStep + id % kThreads + u * kThreads;
+    if (selected <= kMaxHalves) {
+      constexpr int HP = kHalfPieces<T, P>;
+      const int4* v = reinterpret_cast<const int4*>(r.lr + span.head);
+      auto piece_of = [&](int id) { return id / kThreads * kStep + id % kThreads; };
+      auto fetch = [&](int i) {
+        constexpr int none = (int)rb::Word<T>::kNone;
+        int4 raw = i < span.nvec ? __ldg(v + i) : make_int4(none, none, none, none);
+        if (kMask && i < span.nvec) raw = rb::mask_piece<T>(raw, rb::mask_bits<VEC>(r.mr, mask_stride, span.head + i * VEC));
+        return raw;
+      };
+      for (int q0 = 0; q0 < selected; q0 += kThreads) {
+        const int q = q0 + threadIdx.x;
+        const bool on = q < selected;
+        const int what = on ? sh.half[q] : 0, first = piece_of(what >> 1) + (what & 1) * HP * kThreads;
+        int4 raw[HP];
+#pragma unroll
+        for (int u = 0; u < HP; ++u) raw[u] = fetch(on ? first + u * kThreads : span.nvec);
         uint32_t hits = 0;
         float s = 0.f;
-        const int j0 = span.head + piece * VEC;
-        if (on && piece < span.nvec) {
-          int4 raw = reinterpret_cast<const int4*>(r.lr + span.head)[piece];
-          if (kMask) raw = rb::mask_piece<T>(raw, rb::mask_bits<VEC>(r.mr, mask_stride, j0));
-          const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int u = 0; u < HP; ++u) {
+          const T* e = reinterpret_cast<const T*>(&raw[u]);
 #pragma unroll
           for (int c = 0; c < VEC; ++c) {
             const float x = rb::to_f(e[c]);
-            const bool hit = x >= bound_x;
-            hits |= (uint32_t)hit << c;
-            s += hit ? 0.f : rb::exp2_fast(fmaxf((x - st.m) * kk, -1000.f));
+            if (x >= bound_x) {
+              hits |= 1u << (u * VEC + c);
+              s += rb::exp2_fast((x - st.m) * kk);
+            }
           }
         }
-#pragma unroll
-        for (int o = 1; o < P; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (on) sh.hit_sum[q] = s;
         uint32_t at = places(hits, sh.count);
         for (; hits; hits &= hits - 1, ++at) {
-          const int j = j0 + __ffs(hits) - 1;
+          const int b = __ffs(hits) - 1, j = span.head + (first + b / VEC * kThreads) * VEC + b % VEC;
           if (at < kMaxTop) sh.list[at] = (uint64_t)order_key(rb::to_f(r.lr[j])) << 32 | (uint32_t)~j;
         }
-        if (on && u == 0) rec[id].y = s;
       }
       __syncthreads();
       n = sh.count;
+      // the groups' sums without their candidates; a group's halves lie side by side in the list
+      for (int q = threadIdx.x; q < selected; q += kThreads) {
+        const int id = sh.half[q] >> 1;
+        if (q > 0 && (int)(sh.half[q - 1] >> 1) == id) continue;
+        const float h = sh.hit_sum[q] + (q + 1 < selected && (int)(sh.half[q + 1] >> 1) == id ? sh.hit_sum[q + 1] : 0.f);
+        float s = __uint_as_float(rec[id].y) - h;
+        if (!(s * 64.f >= h)) {
+          s = 0.f;
+#pragma unroll
+          for (int u = 0; u < P; ++u) {
+            const int4 raw = fetch(piece_of(id) + u * kThreads);
+            const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) {
+              const float x = rb::to_f(e[c]);
+              s += x >= bound_x ? 0.f : rb::exp2_fast(fmaxf((x - st.m) * kk, -1000.f));
+            }
+          }
+        }
+        rec[id].y = __float_as_uint(s);
+      }
+      __syncthreads();
     }
     if (n <= kMaxTop) {
-      for (int g = 0; g < groups; ++g) left += rec[g * kThreads + threadIdx.x].y;
+      for (int g = 0; g < groups; ++g) left += __uint_as_float(rec[g * kThreads + threadIdx.x].y);
       if (ex != -INFINITY && !(ex >= bound_x)) left += rb::exp2_fast((ex - st.m) * kk);
     }
   }
@@ -315,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
     lowest = key_value(sh.kth);
     __syncthreads();
   }
+  uint64_t* ordered = reinterpret_cast<uint64_t*>(rec);
   auto place = [&](uint64_t c, int at, float* after) {
     const float x = key_value((uint32_t)(c >> 32));
     const int j = (int)~(uint32_t)c;
@@ -328,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
   };
   float* after;                             // candidates that are not chosen, in order
   if (n <= kCountAll) {
-    after = reinterpret_cast<float*>(sh.ordered);
+    after = sh.after;
     if (threadIdx.x == 0 && (n & 1)) sh.list[n] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kThreads) place(sh.list[i], larger_than(sh.list[i], sh.list, n), after);
@@ -361,13 +436,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) sh.ordered[atomicAdd(&sh.hist[bucket(sh.list[i])], 1u)] = sh.list[i];
+    for (int i = threadIdx.x; i < n; i += kThreads) ordered[atomicAdd(&sh.hist[bucket(sh.list[i])], 1u)] = sh.list[i];
     __syncthreads();                        // hist: where the buckets end
     for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint64_t c = sh.ordered[i];
+      const uint64_t c = ordered[i];
       const int b = bucket(c), begin = b > 0 ? sh.hist[b - 1] : 0, end = sh.hist[b];
       int at = begin;
-      for (int e = begin; e < end; ++e) at += sh.ordered[e] > c;
+      for (int e = begin; e < end; ++e) at += ordered[e] > c;
       place(c, at, after);
     }
   }
@@ -410,14 +485,14 @@ int rb_top_logprobs(const void* logits, int64_t row_stride, const int64_t* label
   // pieces a group: one where groups of four are too few to bound the k-th logit
   const int vec = V / (dt == 0 ? 4 : 8), p = vec >= 8 * k ? 4 : 1;
   // threads: as for the statistics, but no fewer than keep 1024 resident beside what a block has in shared memory
-  const int64_t bytes = sizeof(TopShared) + 1024 + (int64_t)vec / p * 8;
+  const int64_t bytes = sizeof(TopShared) + 1024 + std::max<int64_t>((int64_t)vec / p * 8, kMaxTop * 8);
   const int nt = rows < 4 * rb::kNumSMs ? 512 : rows >= 16 * rb::kNumSMs && bytes <= 45 << 10 ? 128 : 256;
 #define RB_L4(T, M, NT, P)                                                                                                                                 \
   {                                                                                                                                                        \
     const int groups = RB_CEIL_DIV(vec, P * NT);                                                                                                           \
     const bool fast = k <= kFastTop && groups * NT <= kMaxRecords;                                                                                         \
-    const int smem = fast ? groups * NT * (int)sizeof(float2) : 0;                                                                                         \
-    if (smem > 26000 && cudaFuncSetAttribute(top_logprobs_kernel<T, M, NT, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2; \
+    const int smem = std::max(fast ? groups * NT * (int)sizeof(uint2) : 0, kMaxTop * 8);                                                                                         \
+    if (smem > 30000 && cudaFuncSetAttribute(top_logprobs_kernel<T, M, NT, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2; \
     top_logprobs_kernel<T, M, NT, P><<<(unsigned)rows, NT, smem, s>>>((const T*)logits, row_stride, labels, mask, mask_stride, logp, entropy, top_logp,     \
                                                                       top_ids, rest, V, k, inv_temp, fast ? groups : 0);                                    \
   }
