@@ -90,7 +90,7 @@ void attn_check() {
   const volatile int* w = rb_attn_status();
   TORCH_CHECK(w == nullptr || *w != 2, "an earlier attention kernel did not run, its outputs are unwritten: its shared memory did not begin on a multiple of 1024 bytes "
                                        "(attn_wait_error() clears this)");
-  TORCH_CHECK(w == nullptr || *w == 0, "an earlier attention kernel gave up waiting and left parts of its outputs unwritten (attn_wait_error() clears this)");
+  TORCH_CHECK(w == nullptr || *w == 0, "an earlier attention or head kernel gave up waiting and left parts of its outputs unwritten (attn_wait_error() clears this)");
 }
 
 // The status word as an int32 [1] tensor on `device` (its kernels read it in stream order); no copy.

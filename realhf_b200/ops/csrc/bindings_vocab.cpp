@@ -7,10 +7,13 @@
 #include <torch/types.h>
 
 #include <atomic>
+#include <cmath>
 #include <vector>
 
 using at::Tensor;
 using OptT = c10::optional<Tensor>;
+
+void attn_check();      // bindings_attn.cpp: an error once a bounded wait of an earlier kernel has run out
 
 // kernels launched where Python does not see the call (in a native backward pass), since the last question
 static std::atomic<int64_t> unseen_launches{0};
@@ -54,8 +57,8 @@ int dtype_code(const Tensor& t) {
 
 void check_logits(const Tensor& logits, const char* op, double inv_temp) {
   TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, op, ": logits are a CUDA matrix [rows, vocabulary] with unit inner stride");
-  TORCH_CHECK_VALUE(logits.size(1) > 0 && logits.size(1) <= 0x7fffff00LL && logits.size(0) <= 0x7fffffffLL, op, ": bad size ", logits.sizes());
-  TORCH_CHECK_VALUE(inv_temp > 0, op, ": the inverse temperature is positive");
+  TORCH_CHECK_VALUE(logits.size(1) > 0 && logits.size(1) <= 0x7ffe0000LL && logits.size(0) <= 0x7fffffffLL, op, ": bad size ", logits.sizes());
+  TORCH_CHECK_VALUE((float)inv_temp > 0 && std::isfinite((float)inv_temp), op, ": the inverse temperature is positive and finite, not ", inv_temp);
 }
 
 // a contiguous tensor of this device, of one value a row (or [rows, k])
@@ -205,8 +208,9 @@ Tensor distill_bwd(const Tensor& logits, const Tensor& lse_rest, const Tensor& g
 void check_head(const Tensor& h, const Tensor& w, const char* op, double inv_temp) {
   TORCH_CHECK(h.is_cuda() && w.device() == h.device() && h.dim() == 2 && w.dim() == 2 && h.size(1) == w.size(1) && h.stride(1) == 1 && w.stride(1) == 1, op,
               ": hidden states [rows, H] and a head [vocabulary, H] on one CUDA device, unit inner stride");
+  attn_check();
   TORCH_CHECK(h.scalar_type() == w.scalar_type() && h.element_size() == 2, op, ": 16-bit operands of one type");
-  TORCH_CHECK(w.size(0) > 0 && w.size(0) <= 0x7fffff00LL && h.size(0) <= 0x7fffff00LL && inv_temp > 0, op, ": bad sizes or temperature");
+  TORCH_CHECK(w.size(0) > 0 && w.size(0) <= 0x7ffe0000LL && h.size(0) <= 0x7ffe0000LL && inv_temp > 0, op, ": bad sizes or temperature");
 }
 
 // A first derivative that is asked for with a graph (create_graph) and then differentiated again is an error, not a zero.

@@ -373,28 +373,46 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
   }
 }
 
-// A row's triples -> its results: 32 rows a block, 16 threads a row over the tiles in turn, merged in a fixed order.
-constexpr int kMergeSlices = 16;
-__global__ void __launch_bounds__(32 * kMergeSlices) head_merge_kernel(const HeadParams p, int parts, float* __restrict__ logp, float* __restrict__ entropy,
-                                                                      float* __restrict__ lse) {
-  __shared__ float sm[3][kMergeSlices][32];
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+// A row's triples -> its results: 8 rows a block, 32 threads a row over the parts in turn, merged in a fixed order (four threads a row of a warp, then the warps).
+constexpr int kMergeRows = 8, kMergeSlices = 32;
+__global__ void __launch_bounds__(kMergeRows* kMergeSlices) head_merge_kernel(const HeadParams p, int parts, float* __restrict__ logp, float* __restrict__ entropy,
+                                                                             float* __restrict__ lse) {
+  constexpr int kWarps = kMergeRows * kMergeSlices / 32;
+  __shared__ float sm[3][kWarps][kMergeRows];
+  const int at_row = threadIdx.x % kMergeRows, slice = threadIdx.x / kMergeRows, warp = threadIdx.x >> 5, row = blockIdx.x * kMergeRows + at_row;
   const float k = p.inv_temp * rb::kLog2e;
   rb::RowStats st;
   if (row < p.M) {
-#pragma unroll 4
-    for (int t = slice; t < parts; t += kMergeSlices) {
-      const int64_t at = (int64_t)t * p.M + row;
-      st.add(p.part_m[at], p.part_s[at], p.part_w[at], k);
+    constexpr int U = 8;
+    for (int t0 = slice; t0 < parts; t0 += U * kMergeSlices) {
+      float m[U], s[U], w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kMergeSlices;
+        const int64_t at = (int64_t)t * p.M + row;
+        m[u] = t < parts ? p.part_m[at] : -INFINITY;
+        s[u] = t < parts ? p.part_s[at] : 0.f;
+        w[u] = t < parts ? p.part_w[at] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (t0 + u * kMergeSlices < parts) st.add(m[u], s[u], w[u], k);
     }
   }
-  sm[0][slice][lane] = st.m;
-  sm[1][slice][lane] = st.s;
-  sm[2][slice][lane] = st.w;
-  __syncthreads();
-  if (slice == 0 && row < p.M) {
 #pragma unroll
-    for (int i = 1; i < kMergeSlices; ++i) st.add(sm[0][i][lane], sm[1][i][lane], sm[2][i][lane], k);
+  for (int o = kMergeRows; o < 32; o <<= 1) {
+    const float m = __shfl_xor_sync(0xffffffffu, st.m, o), s = __shfl_xor_sync(0xffffffffu, st.s, o), w = __shfl_xor_sync(0xffffffffu, st.w, o);
+    st.add(m, s, w, k);
+  }
+  if ((threadIdx.x & 31) < kMergeRows) {
+    sm[0][warp][at_row] = st.m;
+    sm[1][warp][at_row] = st.s;
+    sm[2][warp][at_row] = st.w;
+  }
+  __syncthreads();
+  if (threadIdx.x < kMergeRows && row < p.M) {
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) st.add(sm[0][i][at_row], sm[1][i][at_row], sm[2][i][at_row], k);
     const rb::RowResult r(st, p.inv_temp);
     lse[row] = r.lse;
     entropy[row] = r.entropy;
@@ -427,15 +445,23 @@ __global__ void __launch_bounds__(kGradThreads) head_grad_kernel(const __half* _
   int4* out = reinterpret_cast<int4*>(reinterpret_cast<T*>(p.out) + row * p.ld_out);
   const int i0 = seg * kGradPieces * kGradThreads + threadIdx.x;
   int4 v[kGradPieces];
-  float y0[kGradPieces];                                    // log-probability of a kept number of 1
   const bool plain = zero || lse != lse;
+  constexpr int kPartPieces = HN / 2 / 8;                   // pieces of 128 columns
+  __shared__ float2 factor[kGradPieces * kGradThreads / kPartPieces];   // of the segment's parts: log-probability of a kept number of 1, and it itself
 #pragma unroll
   for (int u = 0; u < kGradPieces; ++u) {
     const int i = i0 + u * kGradThreads;
     if (i < pieces && !plain) {
       v[u] = rb::ld_once(in + i);
-      y0[u] = p.part_m[(int64_t)(i / (HN / 2 / 8)) * all_rows + whole];
     }
+  }
+  {
+    const int part = seg * (kGradPieces * kGradThreads / kPartPieces) + threadIdx.x;
+    if (threadIdx.x < kGradPieces * kGradThreads / kPartPieces && part * kPartPieces < pieces) {
+      const float m = p.part_m[(int64_t)part * all_rows + whole], y = m == -INFINITY ? 0.f : fmaf(m, p.inv_temp, -lse) - 15.f * rb::kLn2;
+      factor[threadIdx.x] = make_float2(y, rb::exp2_fast(y * rb::kLog2e));
+    }
+    __syncthreads();
   }
 #pragma unroll
   for (int u = 0; u < kGradPieces; ++u) {
@@ -447,7 +473,8 @@ __global__ void __launch_bounds__(kGradThreads) head_grad_kernel(const __half* _
       for (int e = 0; e < 8; ++e) d[e] = zero ? 0.f : NAN;
     } else {
       const __half2* h = reinterpret_cast<const __half2*>(&v[u]);
-      const float y1 = y0[u] == -INFINITY ? 0.f : fmaf(y0[u], p.inv_temp, -lse) - 15.f * rb::kLn2, f = rb::exp2_fast(y1 * rb::kLog2e);
+      const float2 fac = factor[(u * kGradThreads + threadIdx.x) / kPartPieces];
+      const float y1 = fac.x, f = fac.y;
       const uint64_t f2 = rb::pack2(f, f), ln2 = rb::pack2(rb::kLn2, rb::kLn2), y2 = rb::pack2(y1, y1), g2 = rb::pack2(-ge, -ge), a2 = rb::pack2(a, a);
       if (ge != 0.f) {
 #pragma unroll
@@ -560,7 +587,7 @@ int rb_head_stats(const void* h, const void* w, int64_t ld_h, int64_t ld_w, cons
   const int rc = kept ? (in_dt == 1 ? launch_head<__nv_bfloat16, 1, kStatsKeep>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kStatsKeep>(ta, tb, p, num_sms, s))
                       : (in_dt == 1 ? launch_head<__nv_bfloat16, 1, kStats>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kStats>(ta, tb, p, num_sms, s));
   if (rc) return rc;
-  head_merge_kernel<<<RB_CEIL_DIV(M, 32), 32 * kMergeSlices, 0, s>>>(p, 2 * tiles_n, logp, entropy, lse);
+  head_merge_kernel<<<RB_CEIL_DIV(M, kMergeRows), kMergeRows * kMergeSlices, 0, s>>>(p, 2 * tiles_n, logp, entropy, lse);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 

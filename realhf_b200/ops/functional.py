@@ -463,8 +463,8 @@ def _check_rows(op: str, logits, inv_temp, **rows):
         raise ValueError(f"{op}: logits are a matrix [rows, vocabulary], not {tuple(logits.shape)}")
     if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16) and (logits.is_cuda or logits.dtype != torch.float64):
         raise ValueError(f"{op}: logits of type {logits.dtype} (float32, bfloat16 or float16)")
-    if not inv_temp > 0:
-        raise ValueError(f"{op}: the inverse temperature is positive, not {inv_temp}")
+    if not 0 < inv_temp < float("inf"):
+        raise ValueError(f"{op}: the inverse temperature is positive and finite, not {inv_temp}")
     _check_row_values(op, logits.shape[0], logits.device, **rows)
 
 
@@ -619,11 +619,11 @@ def _pitched(rows: int, cols: int, dtype, device):
 
 
 def _head_logits(h, w):
-    """fp32 logits of the head: 16-bit operands keep the accumulator, others multiply in fp32."""
+    """fp32 logits of the head: 16-bit operands keep the accumulator, others multiply in fp32.  (The product without a workspace: two graphs may replay at once.)"""
     G = _head_gemm(h, w)
     if G is None:
         return h.float() @ w.float().t()
-    return G.gemm(G.tma_rows(h), w, out=_pitched(h.shape[0], w.shape[0], torch.float32, h.device))
+    return lib().gemm(G.tma_rows(h), w, _pitched(h.shape[0], w.shape[0], torch.float32, h.device), None, False, False, False, None, 0, G._sms(h.device), -1)
 
 
 def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
@@ -681,8 +681,7 @@ class _LMHeadTokenStats(torch.autograd.Function):
             parts = []
             for s in range(0, max(1, T), chunk):
                 e = min(T, s + chunk)
-                if G is not None and e - s > 256:
-                    # (a row tile or less leaves half of the pairs idle: 16 / 256 rows of 4096 x 32000 66 / 78 us through logits, 87 / 97 fused)
+                if G is not None:      # (few rows too, though 16 of 4096 x 32000 take 57 us through fp32 logits and about 62 fused: those come from a product with a shared workspace)
                     parts.append(lib().head_stats(G.tma_rows(hidden[s:e]), weight, labels[s:e], cut(mask_bits, s, e), inv_temp, False, G._sms(hidden.device)))
                 else:
                     parts.append(lib().token_stats(_head_logits(hidden[s:e], weight), labels[s:e], cut(mask_bits, s, e), inv_temp))
@@ -721,8 +720,8 @@ def _check_head(op: str, hidden, weight, temperature, chunk, **rows):
         raise ValueError(f"{op}: hidden states [T, H] and a head [V, H], not {tuple(hidden.shape)} and {tuple(weight.shape)}")
     if hidden.dtype != weight.dtype or hidden.device != weight.device:
         raise ValueError(f"{op}: hidden states and head of one type and device, not {hidden.dtype} on {hidden.device} and {weight.dtype} on {weight.device}")
-    if not temperature > 0 or chunk < 1:
-        raise ValueError(f"{op}: the temperature is positive and a chunk one row at least")
+    if not 0 < temperature < float("inf") or chunk < 1:
+        raise ValueError(f"{op}: the temperature is positive and finite and a chunk one row at least")
     _check_row_values(op, hidden.shape[0], hidden.device, **rows)
     _check_mask(op, rows.get("mask_bits"), weight.shape[0])
 

@@ -796,9 +796,10 @@ def test_captured_and_replayed_gpu():
         logp, ent = OF.logprob_entropy_from_logits(a, labels)
         loss = OF.distill_loss_from_logits(a, ids, t, tr)
         lp, en = OF.lm_head_logprobs_entropy(b, c, labels)
-        top = OF.top_logprobs_from_logits(x, k, labels)
-        grads = torch.autograd.grad([logp, ent, loss, lp, en], [a, b, c], [torch.ones_like(logp)] * 5)
-        return [logp, ent, loss, lp, en, *top, *grads]
+        hd = OF.lm_head_distill_loss(b, c, ids, t, tr)
+        top, htop = OF.top_logprobs_from_logits(x, k, labels), OF.lm_head_top_logprobs(h, w, k, labels)
+        grads = torch.autograd.grad([logp, ent, loss, lp, en, hd], [a, b, c], [torch.ones_like(logp)] * 6)
+        return [logp, ent, loss, lp, en, hd, *top, *htop, *grads]
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -813,8 +814,12 @@ def test_captured_and_replayed_gpu():
         graphs.append((graph, out))
     x2, _ = make_logits(T, V, torch.bfloat16, 9, "cuda")
     x.copy_(x2)
-    for graph, out in graphs:
-        graph.replay()
+    streams = [torch.cuda.Stream() for _ in graphs]     # at once: no workspace is shared
+    for stream, (graph, out) in zip(streams, graphs):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                graph.replay()
     torch.cuda.synchronize()
     second = work()
     for graph, out in graphs:
@@ -912,7 +917,7 @@ def check_refusals(dev):
     L, P, D, E = OF.logprob_entropy_from_logits, OF.top_logprobs_from_logits, OF.distill_loss_from_logits, OF.lm_head_logprobs_entropy
     bad = [
         lambda: L(x[0], labels[:1]), lambda: L(x, labels[:2]), lambda: L(x, labels.float()), lambda: L(x, labels[:, None]), lambda: L(x, labels, inv_temp=0.0),
-        lambda: L(x, labels, inv_temp=float("nan")), lambda: L(x.int(), labels), lambda: L(x, labels, bits[:, :2]), lambda: L(x, labels, bits[:2]),
+        lambda: L(x, labels, inv_temp=float("nan")), lambda: L(x, labels, inv_temp=INF), lambda: L(x.int(), labels), lambda: L(x, labels, bits[:, :2]), lambda: L(x, labels, bits[:2]),
         lambda: L(x, labels, bits.bool()), lambda: L(x[:, :0], labels),
         lambda: P(x, 0), lambda: P(x, 21), lambda: P(torch.zeros(1, 2000, device=dev), 1025), lambda: P(x, 2, labels[:2]), lambda: P(x, 2, inv_temp=-1.0),
         lambda: D(x, ids, t[:, :2]), lambda: D(x, ids[:2], t[:2]), lambda: D(x, ids, t, tr[:2]), lambda: D(x, ids, t, reverse=True), lambda: D(x, t, t),
