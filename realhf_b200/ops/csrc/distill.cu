@@ -14,7 +14,7 @@
 namespace {
 
 constexpr int kMaxListed = 1024;
-constexpr int kBwdThreads = 128, kBwdVecs = 4;
+constexpr int kBwdThreads = 256, kBwdVecs = 4;
 
 __host__ __device__ constexpr int bitmap_words(int V) { return (V + 16 + 31) / 32; }
 
@@ -135,6 +135,8 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
   T* orow = out + row * out_stride;
   const float g = g_loss[row] * inv_temp;
   const bool zero = g == 0.f;
+  const int id0 = threadIdx.x < k ? ids[row * k + threadIdx.x] : -1;         // (asked for beside the logits, as the block ends with them)
+  const float listed0 = threadIdx.x < k ? grad_listed[row * k + threadIdx.x] : 0.f;
   const float a = zero ? 0.f : g * grad_rest[row], lr_rest = lse_rest_in[row];
   const float ref = lr_rest == -INFINITY ? 0.f : lr_rest;
   auto grad = [&](float x) {
@@ -183,7 +185,8 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
     for (int j = lo + threadIdx.x; j < hi; j += kBwdThreads) orow[j] = rb::from_f<T>(grad(rb::to_f(lr[j])));
   }
   __syncthreads();                                      // the listed tokens over what was just written
-  for (int i = threadIdx.x; i < k; i += kBwdThreads) {
+  if (id0 >= lo && id0 < hi) orow[id0] = rb::from_f<T>(zero ? 0.f : g * listed0);
+  for (int i = threadIdx.x + kBwdThreads; i < k; i += kBwdThreads) {
     const int id = ids[row * k + i];
     if (id >= lo && id < hi) orow[id] = rb::from_f<T>(zero ? 0.f : g * grad_listed[row * k + i]);
   }
