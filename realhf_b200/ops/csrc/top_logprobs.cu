@@ -16,6 +16,9 @@
 // the k-th largest value by its bits (four digits of 8 bits, a histogram in shared memory each), the elements above it in any order, of those equal to it the
 // first in index order.
 // Sums have a fixed order whichever way candidates arrive.
+//
+// bf16, us: 8192 x 32000 with 20 / 64 / 256 alternatives 130 / 150 / 207, 4096 x 131072 with 64 212 (5.1 TB/s); the statistics alone take 95 and 170.  Bound by issue slots (66 %):
+// ten instructions a logit, a fifth of them for bound, candidates and order.
 #include "vocab_rows.cuh"
 
 #include <algorithm>

@@ -514,8 +514,8 @@ def check_head(dev, T, H, V, dtype, masked, temp, chunk, seed, buffer=None, keep
     d = grad64(y, p, want_H, labels, gl.double(), ge.double(), c).masked_fill(empty[:, None], 0.0)
     size = c * p * (gl.abs()[:, None] + ge.abs()[:, None] * (torch.where(p > 0, -y, 0.0) + want_H[:, None] + 1)) * 4 * e + c * U * (gl.abs()[:, None] + 1)
     r = half_step(dtype)
-    # kept weights e, relative to the largest of 128 columns, are rounded by at most 2^-12 of e or, below 2^-29, 2^-40 (their logarithm by as much more): of a
-    # probability p e^(their distance) <= p_max that is within 2 * 2^-12 of the size of the gradient's parts and 2^-40 of what a probability of 1 would give
+    # kept weights e, relative to the largest of 128 columns, are rounded by at most 2^-11 of e (fp16), their logarithm by as much, which moves the gradient by at most
+    # 2^-11 of the size of its parts; below 2^-29 by 2^-40, which is no more than 2^-40 of what a probability of 1 would give
     kept = T > 256 and H >= 1024 and keep > 0 and dtype != torch.float32
     whole = c * (gl.abs()[:, None] + ge.abs()[:, None] * (want_H[:, None] + 30))
     more = (2.0 ** -11 * (size / (4 * e)) + 2.0 ** -40 * whole) if kept else 0.0
