@@ -6,6 +6,7 @@
 #include <torch/library.h>
 #include <torch/types.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <vector>
@@ -13,6 +14,7 @@
 using at::Tensor;
 using OptT = c10::optional<Tensor>;
 
+bool gradient_goes_past(const Tensor& leaf, bool own_hook);      // bindings.cpp
 void attn_check();      // bindings_attn.cpp: an error once a bounded wait of an earlier kernel has run out
 
 // kernels launched where Python does not see the call (in a native backward pass), since the last question
@@ -34,6 +36,7 @@ int rb_head_stats_bwd(const void*, const void*, int64_t, int64_t, const int64_t*
                       void*, int64_t, int, int, int, float, int, int, cudaStream_t);
 int rb_head_dhidden_splits(int, int, int, int);
 int rb_head_dhidden(const void*, const void*, int64_t, int64_t, float*, void*, int, int, int, int, int, int, cudaStream_t);
+int rb_gemm_tcgen05(const void*, const void*, void*, const void*, int, int, int, int64_t, int64_t, int64_t, int, int, int, int, int, int, int, int, cudaStream_t);
 int rb_distill_max_listed();
 int64_t rb_distill_max_vocab();
 int rb_distill_fwd(const void*, int64_t, const int64_t*, const float*, const float*, int, float*, float*, float*, float*, int*, int64_t, int, int, float, int,
@@ -360,6 +363,147 @@ void head_dhidden(const Tensor& d, const Tensor& w, Tensor out, int64_t splits, 
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
 }
 
+// rows that a TMA descriptor can describe: unit inner stride, 16-byte aligned rows
+Tensor tma_rows(const Tensor& x) {
+  if (x.stride(1) != 1 || x.stride(0) % 8 != 0 || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15)) return x.clone(at::MemoryFormat::Contiguous);
+  return x;
+}
+
+// The gradient buffer in a leaf's .grad that products can be added to, if its gradient may go past autograd's own accumulation
+Tensor flat_gradient(const Tensor& w, bool flat) {
+  if (!flat || !w.is_leaf()) return Tensor();
+  const Tensor g = w.grad();
+  const bool fits = g.defined() && g.device() == w.device() && g.sizes() == w.sizes() && g.is_contiguous() && (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15) == 0 &&
+                    (g.scalar_type() == at::kFloat || g.scalar_type() == w.scalar_type());
+  return fits && gradient_goes_past(w, false) ? g : Tensor();
+}
+
+// Native for the same reason as the functions on logits: a step of few rows waits for the host (64 rows forward and backward 190 us as a Python function).
+class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> {
+ public:
+  // log-probability, entropy, log-sum-exp and, where kept, the weights and the maxima that they stand against
+  static std::vector<Tensor> statistics(const Tensor& hidden, const Tensor& weight, const Tensor& labels, const OptT& mask, double inv_temp, int64_t chunk, bool keep,
+                                        int64_t num_sms) {
+    const char* op = "lm_head_logprobs_entropy";
+    const int64_t T = hidden.size(0), H = hidden.size(1), V = weight.size(0), mask_row = mask_bytes(mask);
+    c10::cuda::CUDAGuard guard(hidden.device());
+    const Tensor h = tma_rows(hidden);
+    const int64_t step = keep ? T : std::min(chunk, std::max<int64_t>(T, 1)), pitch = (V + 7) / 8 * 8;
+    auto f = h.options().dtype(at::kFloat);
+    Tensor logp = at::empty({T}, f), entropy = at::empty({T}, f), lse = at::empty({T}, f), scratch = at::empty({step * rb_head_stats_scratch((int)V)}, f);
+    const Tensor kept = keep ? at::empty({T, pitch}, f.dtype(at::kHalf)) : Tensor();
+    const uint8_t* m = head_mask(mask, h, V, op);
+    for (int64_t s = 0; s < T; s += step) {
+      const int rc = rb_head_stats(static_cast<const char*>(h.data_ptr()) + s * h.stride(0) * 2, weight.data_ptr(), h.stride(0), weight.stride(0),
+                                   labels.data_ptr<int64_t>() + s, m ? m + s * mask_row : nullptr, mask_row, scratch.data_ptr<float>(),
+                                   keep ? kept.data_ptr() : nullptr, pitch, logp.data_ptr<float>() + s, entropy.data_ptr<float>() + s, lse.data_ptr<float>() + s,
+                                   (int)std::min(step, T - s), (int)V, (int)H, (float)inv_temp, dtype_code(h), (int)num_sms, stream());
+      TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+    }
+    if (!keep) return {logp, entropy, lse, Tensor(), Tensor()};
+    return {logp, entropy, lse, kept, scratch.slice(0, 0, T * ((V + 255) / 256 * 2)).clone()};
+  }
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& labels, const OptT& mask,
+                                                double inv_temp, int64_t chunk, int64_t keep_bytes, bool flat, int64_t num_sms) {
+    // keep the weights from width 1024 on: forming and reading them costs what the product of width 512 does (us, both passes up to d logits, kept / formed again:
+    // 8192 x 4096 x 32000 1583 / 2715, 2047 x 1024 x 50257 352 / 408, 8192 x 512 x 32000 484 / 486)
+    const int64_t T = hidden.size(0);
+    const bool keep = T > 256 && hidden.size(1) >= 1024 && 2 * T * weight.size(0) <= keep_bytes;
+    const auto r = statistics(hidden, weight, labels, mask, inv_temp, chunk, keep, num_sms);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({hidden, weight, labels, mask.has_value() ? *mask : Tensor(), r[2], r[1], r[3], r[4]});
+    ctx->saved_data["inv_temp"] = inv_temp;
+    ctx->saved_data["chunk"] = chunk;
+    ctx->saved_data["flat"] = flat;
+    ctx->saved_data["num_sms"] = num_sms;
+    return {r[0], r[1]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const char* op = "lm_head_logprobs_entropy";
+    torch::autograd::variable_list out(9);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor h = tma_rows(saved[0]), w = saved[1], labels = saved[2], mask = saved[3], lse = saved[4], entropy = saved[5], kept = saved[6], maxima = saved[7];
+    const double inv_temp = ctx->saved_data["inv_temp"].toDouble();
+    const int num_sms = (int)ctx->saved_data["num_sms"].toInt();
+    const int64_t T = h.size(0), H = h.size(1), V = w.size(0), pitch = (V + 7) / 8 * 8, mask_row = mask.defined() ? mask.size(1) : 0;
+    const int64_t step = std::min<int64_t>(ctx->saved_data["chunk"].toInt(), std::max<int64_t>(T, 1));
+    const int dt = dtype_code(h);
+    c10::cuda::CUDAGuard guard(h.device());
+    attn_check();
+    const Tensor gl = g[0].defined() ? fp32(g[0]) : Tensor(), ge = g[1].defined() ? fp32(g[1]) : Tensor();
+    const Tensor d = at::empty({std::min(step, T), pitch}, h.options());
+    const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    Tensor dh = need_h ? at::empty({T, H}, h.options()) : Tensor(), dw, buffer, parts;
+    if (need_w) {
+      buffer = flat_gradient(w, ctx->saved_data["flat"].toBool());
+      if (buffer.defined() && buffer.scalar_type() != at::kFloat && T > step) buffer = Tensor();      // (16 bits would be rounded once a chunk)
+      dw = buffer.defined()   ? buffer
+           : T > step || T == 0 ? at::zeros({V, H}, h.options().dtype(at::kFloat))
+                                : at::empty({V, H}, h.options());
+    }
+    const bool add = need_w && (buffer.defined() || dw.scalar_type() == at::kFloat);
+    const int64_t* lab = labels.data_ptr<int64_t>();
+    const uint8_t* m = mask.defined() ? mask.data_ptr<uint8_t>() : nullptr;
+    auto at_row = [](const Tensor& t, int64_t s) { return t.defined() ? t.data_ptr<float>() + s : nullptr; };
+    for (int64_t s = 0; s < T; s += step) {
+      const int64_t n = std::min(step, T - s);
+      const char* hs = static_cast<const char*>(h.data_ptr()) + s * h.stride(0) * 2;
+      int rc;
+      if (kept.defined())
+        rc = rb_head_grad(kept.data_ptr<at::Half>() + s * pitch, pitch, maxima.data_ptr<float>(), lab, m, mask_row, at_row(lse, 0), at_row(entropy, 0), at_row(gl, 0),
+                          at_row(ge, 0), d.data_ptr(), pitch, (int)s, (int)n, (int)T, (int)V, (float)inv_temp, dt, stream());
+      else
+        rc = rb_head_stats_bwd(hs, w.data_ptr(), h.stride(0), w.stride(0), lab + s, m ? m + s * mask_row : nullptr, mask_row, at_row(lse, s), at_row(entropy, s),
+                               at_row(gl, s), at_row(ge, s), d.data_ptr(), pitch, (int)n, (int)V, (int)H, (float)inv_temp, dt, num_sms, stream());
+      TORCH_CHECK(rc == 0, op, ": d logits failed with code ", rc);
+      ++unseen_launches;
+      if (need_h) {       // [n, V] x [V, H]
+        void* to = static_cast<char*>(dh.data_ptr()) + s * H * 2;
+        const int splits = rb_head_dhidden_splits((int)n, (int)H, (int)V, num_sms);
+        if (splits > 1) {
+          if (!parts.defined() || parts.numel() < splits * n * H) parts = at::empty({splits * n * H}, h.options().dtype(at::kFloat));
+          rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), pitch, w.stride(0), parts.data_ptr<float>(), to, (int)n, (int)H, (int)V, splits, dt, num_sms, stream());
+        } else {
+          rc = rb_gemm_tcgen05(d.data_ptr(), w.data_ptr(), to, nullptr, (int)n, (int)H, (int)V, pitch, w.stride(0), H, 0, 1, dt, dt, 0, 0, num_sms, -1, stream());
+        }
+        TORCH_CHECK(rc == 0, op, ": d hidden failed with code ", rc);
+        unseen_launches += splits > 1 ? 2 : 1;
+      }
+      if (need_w) {       // [n, V]^T x [n, H]
+        rc = rb_gemm_tcgen05(d.data_ptr(), hs, dw.data_ptr(), nullptr, (int)V, (int)H, (int)n, pitch, h.stride(0), H, 1, 1, dt, dtype_code(dw), add, 0, num_sms, -1,
+                             stream());
+        TORCH_CHECK(rc == 0, op, ": d weight failed with code ", rc);
+        ++unseen_launches;
+      }
+    }
+    if (need_h) out[0] = once(dh, op);
+    if (need_w && !buffer.defined()) out[1] = once(dw.scalar_type() == w.scalar_type() ? dw : dw.to(w.scalar_type()), op);
+    return out;
+  }
+};
+
+// For 16-bit operands as a TMA descriptor takes them; flat: the weight's gradient buffer is its .grad
+torch::autograd::variable_list head_logprob_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& labels_in, const OptT& mask_in, double inv_temp, int64_t chunk,
+                                                    int64_t keep_bytes, bool flat, int64_t num_sms) {
+  const char* op = "lm_head_logprobs_entropy";
+  TORCH_CHECK_VALUE((float)inv_temp > 0 && std::isfinite((float)inv_temp) && chunk >= 1, op, ": the temperature is positive and finite and a chunk one row at least");
+  TORCH_CHECK_VALUE(hidden.dim() == 2 && weight.dim() == 2 && hidden.size(1) == weight.size(1) && weight.size(0) > 0 && hidden.device() == weight.device() &&
+                        hidden.scalar_type() == weight.scalar_type(), op, ": hidden states [T, H] and a head [V, H] of one type and device");
+  TORCH_CHECK(weight.element_size() == 2 && weight.stride(1) == 1 && weight.stride(0) % 8 == 0 && hidden.size(1) % 8 == 0 && weight.size(0) <= 0x7ffe0000LL &&
+                  hidden.size(0) <= 0x7ffe0000LL && (reinterpret_cast<uintptr_t>(weight.data_ptr()) & 15) == 0, op, ": operands that the products cannot take");
+  attn_check();
+  const Tensor labels = whole_numbers(labels_in, op, "labels");
+  const OptT mask = packed(mask_in);
+  row_values(labels, at::kLong, hidden, -1, op, "labels");
+  TORCH_CHECK_VALUE(!mask.has_value() || (mask->device() == hidden.device() && mask->scalar_type() == at::kByte && mask->dim() == 2 && mask->size(0) == hidden.size(0) &&
+                                          mask->size(1) * 8 >= weight.size(0)), op, ": the mask is a packed uint8 matrix [rows, at least vocabulary / 8]");
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))
+    return HeadLogprobEntropy::apply(hidden, weight, labels, mask, inv_temp, chunk, keep_bytes, flat, num_sms);
+  const auto r = HeadLogprobEntropy::statistics(hidden, weight, labels, mask, inv_temp, chunk, false, num_sms);
+  return {r[0], r[1]};
+}
+
 }  // namespace
 
 void register_vocab_ops(torch::Library& m) {
@@ -370,6 +514,8 @@ void register_vocab_ops(torch::Library& m) {
   m.def("token_stats_bwd(Tensor logits, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
         "Tensor(a!)? out) -> Tensor", &token_stats_bwd);
   m.def("top_logprobs(Tensor logits, int k, Tensor? labels, Tensor? mask, float inv_temp) -> Tensor[]", &top_logprobs);
+  m.def("head_logprob_entropy(Tensor hidden, Tensor weight, Tensor labels, Tensor? mask, float inv_temp, int chunk, int keep_bytes, bool flat, int num_sms) -> Tensor[]",
+        &head_logprob_entropy);
   m.def("head_stats(Tensor h, Tensor w, Tensor labels, Tensor? mask, float inv_temp, bool keep, int num_sms) -> Tensor[]", &head_stats);
   m.def("head_grad(Tensor kept, Tensor maxima, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, Tensor(a!) out, "
         "int row0) -> ()", &head_grad);

@@ -736,6 +736,12 @@ def lm_head_logprobs_entropy(hidden, weight, labels, mask_bits=None, temperature
     statistics come from the product's fp32 accumulators.  Their gradient exists for `chunk` rows at a time, from the weights of the softmax where these
     take at most `keep_bytes` (2 T V) between the passes and H is 1024 or more, else (0: always) from the product formed again.  Labels and mask as in
     `logprob_entropy_from_logits`."""
+    if (use_native(hidden) and hidden.dim() == weight.dim() == 2 and hidden.shape[1] == weight.shape[1] and weight.is_cuda and weight.shape[0] > 0
+            and temperature != 0 and getattr(weight, "main_grad", None) is None and not _plain_autograd()):
+        G = _head_gemm(hidden, weight)
+        if G is not None:        # (checks its arguments itself; a gradient buffer beside .grad is known to Python alone)
+            return tuple(lib().head_logprob_entropy(hidden, weight, labels, mask_bits, 1.0 / temperature, chunk, keep_bytes,
+                                                    bool(getattr(weight, "_grad_in_flat_buffer", False)), G._sms(hidden.device)))
     op = "lm_head_logprobs_entropy"
     _check_head(op, hidden, weight, temperature, chunk, labels=labels, mask_bits=mask_bits)
     _check_labels(op, labels)
