@@ -12,10 +12,14 @@
 // again, pieces of 64 bytes in memory that the cache had dropped, 256 alternatives of 8192 x 32000 read 1.6 times the logits.)  A candidate's place is the number of
 // candidates before it in the order: counted among all of them where they are few, else among those of its bucket, 512 equal intervals of the value (a bitonic sort of
 // 128, a barrier for each of its 28 stages, took 7400 cycles; counting among 400 by 128 threads 28000).
-// More than 256 alternatives, more than 768 halves or 1024 candidates at the bound (ties), and rows of more than 12288 groups take a radix descent instead:
-// the k-th largest value by its bits (four digits of 8 bits, a histogram in shared memory each), the elements above it in any order, of those equal to it the
-// first in index order.
+// More than 256 alternatives, or nearly as many as the row has pieces: room for 2048 candidates, and the bound from the halves' own maxima, counted by all threads bit by bit.
+// (300 of 4096 x 32000: 182 us, 1000: 373; the descent took 1080 and 1210.)
+// More candidates or halves than there is room for (ties) and rows of more than 12288 groups take a radix descent instead: the k-th largest value by its bits
+// (digits of 8 bits, a histogram in shared memory each: two in bf16, three in fp16, four in fp32), the elements above it in any order, of those equal to it the first in
+// index order.
 // Sums have a fixed order whichever way candidates arrive.
+//
+// A row of equal logits: 4096 x 32000 in 457 us, 896 before the descent left the digits out that a 16-bit type does not have.
 //
 // bf16, us: 8192 x 32000 with 20 / 64 / 256 alternatives 130 / 150 / 207, 4096 x 131072 with 64 212 (5.1 TB/s); the statistics alone take 95 and 170.  Bound by issue slots (66 %):
 // ten instructions a logit, a fifth of them for bound, candidates and order.
@@ -35,19 +39,22 @@ RB_DEVICE uint32_t order_key(float x) {  // order-preserving float -> uint, -0 a
 RB_DEVICE float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 constexpr uint32_t kKeyNone = 0x007fffffu;  // order_key(-inf)
 
-constexpr int kFastTop = 256, kMaxRecords = 12288, kMaxHalves = 768, kCountAll = 128;
+constexpr int kFastTop = 256, kMaxRecords = 12288, kCountAll = 128;
+constexpr int kCap = 1024, kBigCap = 2048;   // candidates of a block
 
-struct TopShared {
+template <int kCand> struct TopShared {
+  static constexpr int kHalves = kCand == kCap ? 768 : kCand;
   float red[96];
   uint32_t warp_n[32];
   uint32_t digit, above, count, selected, kth;
   int last;
-  alignas(16) uint64_t list[kMaxTop];   // key << 32 | ~index: descending order is the order wanted
+  int reach[16];
+  alignas(16) uint64_t list[kCand];   // key << 32 | ~index: descending order is the order wanted
   union {                               // one after the other
     uint32_t keys[kShares];
     struct {
-      uint32_t half[kMaxHalves];        // halves to look at again: 2 * group + which, groups numbered step * threads + thread
-      float hit_sum[kMaxHalves];        // their candidates' sums
+      uint32_t half[kHalves];           // halves to look at again: 2 * group + which, groups numbered step * threads + thread
+      float hit_sum[kHalves];           // their candidates' sums
     };
     uint32_t hist[kShares];
     float after[kCountAll * 2];
@@ -88,21 +95,49 @@ template <typename T> RB_DEVICE void half_values(uint32_t halves, float& lo, flo
 template <typename T> struct TopRow {
   const T* lr;
   const uint8_t* mr;
+  int64_t mask_row;
   int V;
   RB_DEVICE float at(int j) const { return mr && (mr[j >> 3] >> (j & 7)) & 1 ? -INFINITY : rb::to_f(lr[j]); }
 };
 
+// f(logit, index) for every element of the row, whole pieces a thread
+template <int kThreads, typename T, typename F> RB_DEVICE void for_each(const TopRow<T>& r, F f) {
+  constexpr int VEC = rb::RowSpan<T>::VEC;
+  const rb::RowSpan<T> span(r.lr, r.V);
+  const int4* v = reinterpret_cast<const int4*>(r.lr + span.head);
+  const int ej = span.edge(threadIdx.x, r.V);
+  if (ej >= 0) f(r.at(ej), ej);
+  for (int i = threadIdx.x; i < span.nvec; i += kThreads) {
+    int4 raw = __ldg(v + i);
+    const int j0 = span.head + i * VEC;
+    if (r.mr) raw = rb::mask_piece<T>(raw, rb::mask_bits<VEC>(r.mr, r.mask_row, j0));
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) f(rb::to_f(e[c]), j0 + c);
+  }
+}
+
 // The k largest (key, ~index) of the row -> sh.list in any order; returns how many there are (less than k where the row keeps fewer tokens), and in
 // sh.kth the k-th largest value's key.
-template <int kThreads, typename T> RB_DEVICE int select_radix(const TopRow<T>& r, int k, TopShared& sh) {
+template <int kThreads, typename T, typename Shared> RB_DEVICE int select_radix(const TopRow<T>& r, int k, Shared& sh) {
+  constexpr int kDigits = sizeof(T) == 4 ? 4 : rb::Word<T>::kNone == 0xfc00fc00u ? 3 : 2;      // the digits that differ: as fp32, 16-bit types end in zeros
   uint32_t prefix = 0, want = k;      // the want-th largest among the elements whose high digits are `prefix`
-  for (int shift = 24; shift >= 0; shift -= 8) {
+  for (int shift = 24; shift >= 32 - 8 * kDigits; shift -= 8) {
     for (int b = threadIdx.x; b < 256; b += kThreads) sh.hist[b] = 0;
     __syncthreads();
-    for (int j = threadIdx.x; j < r.V; j += kThreads) {
-      const uint32_t key = order_key(r.at(j));
-      if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&sh.hist[(key >> shift) & 255], 1u);
-    }
+    uint32_t same = 0, run = 0;       // a thread's equal digits in a row: one addition
+    for_each<kThreads>(r, [&](float x, int) {
+      const uint32_t key = order_key(x), digit = (key >> shift) & 255;
+      if (shift == 24 || (key >> (shift + 8)) == prefix) {
+        if (digit != same) {
+          if (run) atomicAdd(&sh.hist[same], run);
+          same = digit;
+          run = 0;
+        }
+        ++run;
+      }
+    });
+    if (run) atomicAdd(&sh.hist[same], run);
     __syncthreads();
     if (threadIdx.x == 0) {
       uint32_t left = want;
@@ -116,16 +151,20 @@ template <int kThreads, typename T> RB_DEVICE int select_radix(const TopRow<T>& 
     want = sh.above;
     __syncthreads();
   }
+  if constexpr (kDigits < 4) {        // (a negative number's key is its complement: ends in ones)
+    const bool positive = (prefix >> (8 * kDigits - 1)) & 1;
+    prefix = prefix << (32 - 8 * kDigits) | (positive ? 0u : (1u << (32 - 8 * kDigits)) - 1u);
+  }
   const uint32_t kth = prefix;
   if (threadIdx.x == 0) {
     sh.count = 0;
     sh.kth = max(kth, kKeyNone);
   }
   __syncthreads();
-  for (int j = threadIdx.x; j < r.V; j += kThreads) {
-    const uint32_t key = order_key(r.at(j));
+  for_each<kThreads>(r, [&](float x, int j) {
+    const uint32_t key = order_key(x);
     if (key > kth && key > kKeyNone) sh.list[atomicAdd(&sh.count, 1u)] = (uint64_t)key << 32 | (uint32_t)~j;
-  }
+  });
   __syncthreads();
   const int above = sh.count, need = kth > kKeyNone ? k - above : 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -194,17 +233,18 @@ RB_DEVICE int larger_than(uint64_t mine, const uint64_t* list, int n) {
   return rank;
 }
 
-template <typename T, bool kMask, int kThreads, int P>
+template <typename T, bool kMask, int kThreads, int P, int kCand>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel(const T* __restrict__ logits, int64_t row_stride,
                                                                                  const int64_t* __restrict__ labels, const uint8_t* __restrict__ mask,
                                                                                  int64_t mask_stride, float* __restrict__ logp, float* __restrict__ entropy,
                                                                                  float* __restrict__ top_logp, int64_t* __restrict__ top_ids,
                                                                                  float* __restrict__ rest, int V, int k, float inv_temp, int records) {
   constexpr int VEC = rb::RowSpan<T>::VEC, kStep = P * kThreads;
-  __shared__ TopShared sh;
+  constexpr int kHalves = TopShared<kCand>::kHalves;
+  __shared__ TopShared<kCand> sh;
   extern __shared__ uint2 rec[];            // [step][thread]: maxima of a group's halves, its sum; later the list by buckets
   const int64_t row = blockIdx.x;
-  const TopRow<T> r{logits + row * row_stride, kMask ? mask + row * mask_stride : nullptr, V};
+  const TopRow<T> r{logits + row * row_stride, kMask ? mask + row * mask_stride : nullptr, mask_stride, V};
   const float kk = inv_temp * rb::kLog2e;
   const rb::RowSpan<T> span(r.lr, V);
   const int lane = threadIdx.x & 31;
@@ -263,11 +303,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
     return;
   }
   float left = 0.f;                         // the rest's sum against the row's maximum
-  int n = kMaxTop + 1;
+  int n = kCand + 1;
   float lowest = 0.f;                       // no candidate lies below
   if (fast) {
+    if constexpr (kCand == kCap) {
 #pragma unroll
-    for (int b = 0; b < B; ++b) sh.keys[b * kThreads + threadIdx.x] = order_key(b == 0 ? fmaxf(share[0], ex) : share[b]);
+      for (int b = 0; b < B; ++b) sh.keys[b * kThreads + threadIdx.x] = order_key(b == 0 ? fmaxf(share[0], ex) : share[b]);
+    } else {
+      if (threadIdx.x < 16) sh.reach[threadIdx.x] = 0;
+    }
     // a group's sum was taken against the thread's largest value so far: bring it to the row's
     float so_far = -INFINITY;
     for (int g = 0; g < groups; ++g) {
@@ -278,13 +322,33 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
       v.y = __float_as_uint(__uint_as_float(v.y) * rb::exp2_fast(fmaxf((so_far - st.m) * kk, -1000.f)));
     }
     __syncthreads();
-    if (threadIdx.x < 32) {
-      const uint32_t t = k <= 32 ? bound_of<4>(k, sh.keys) : k <= 64 ? bound_of<8>(k, sh.keys) : bound_of<kShares / 32>(k, sh.keys);
-      if (threadIdx.x == 0) sh.digit = max(t, kKeyNone + 1);
+    uint32_t bound = 0;
+    if constexpr (kCand == kCap) {
+      if (threadIdx.x < 32) {
+        const uint32_t t = k <= 32 ? bound_of<4>(k, sh.keys) : k <= 64 ? bound_of<8>(k, sh.keys) : bound_of<kShares / 32>(k, sh.keys);
+        if (threadIdx.x == 0) sh.digit = t;
+      }
+      __syncthreads();
+      bound = sh.digit;
+    } else {
+      for (int bit = 15; bit >= 0; --bit) {   // (below -inf there are NaNs, which nothing reaches: the bound stays at 0)
+        const uint32_t c = bound | 1u << (16 + bit);
+        const float x = key_value(c);
+        int reach = ex >= x;
+        for (int g = 0; g < groups; ++g) {
+          float lo, hi;
+          half_values<T>(rec[g * kThreads + threadIdx.x].x, lo, hi);
+          reach += (lo >= x) + (hi >= x);
+        }
+        reach = __reduce_add_sync(0xffffffffu, reach);
+        if (lane == 0 && reach) atomicAdd(&sh.reach[bit], reach);
+        __syncthreads();
+        if (sh.reach[bit] >= k) bound = c;
+      }
     }
-    __syncthreads();
-    const float bound_x = lowest = key_value(sh.digit);
-    // places in `group` or `list` for the bits set in a lane's mask: one addition a warp
+    bound = max(bound, kKeyNone + 1);
+    const float bound_x = lowest = key_value(bound);
+    // places in `half` or `list` for the bits set in a lane's mask: one addition a warp
     auto places = [&](uint32_t hits, uint32_t& count) {
       const int mine = __popc(hits);
       int before = mine;
@@ -308,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
       uint32_t at = places(hits, sh.selected);
       for (; hits; hits &= hits - 1, ++at) {
         const int b = __ffs(hits) - 1;
-        if (at < kMaxHalves) sh.half[at] = 2 * ((g0 + b / 2) * kThreads + threadIdx.x) + (b & 1);
+        if (at < kHalves) sh.half[at] = 2 * ((g0 + b / 2) * kThreads + threadIdx.x) + (b & 1);
       }
     }
     if (threadIdx.x < 32) {
@@ -317,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
     }
     __syncthreads();
     const int selected = sh.selected;
-    if (selected <= kMaxHalves) {
+    if (selected <= kHalves) {
       constexpr int HP = kHalfPieces<T, P>;
       const int4* v = reinterpret_cast<const int4*>(r.lr + span.head);
       auto piece_of = [&](int id) { return id / kThreads * kStep + id % kThreads; };
@@ -352,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
         uint32_t at = places(hits, sh.count);
         for (; hits; hits &= hits - 1, ++at) {
           const int b = __ffs(hits) - 1, j = span.head + (first + b / VEC * kThreads) * VEC + b % VEC;
-          if (at < kMaxTop) sh.list[at] = (uint64_t)order_key(rb::to_f(r.lr[j])) << 32 | (uint32_t)~j;
+          if (at < kCand) sh.list[at] = (uint64_t)order_key(rb::to_f(r.lr[j])) << 32 | (uint32_t)~j;
         }
       }
       __syncthreads();
@@ -380,12 +444,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
       }
       __syncthreads();
     }
-    if (n <= kMaxTop) {
+    if (n <= kCand) {
       for (int g = 0; g < groups; ++g) left += __uint_as_float(rec[g * kThreads + threadIdx.x].y);
       if (ex != -INFINITY && !(ex >= bound_x)) left += rb::exp2_fast((ex - st.m) * kk);
     }
   }
-  const bool listed = n <= kMaxTop;
+  const bool listed = n <= kCand;
   if (!listed) {
     __syncthreads();
     n = select_radix<kThreads>(r, k, sh);
@@ -412,6 +476,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
     for (int i = threadIdx.x; i < n; i += kThreads) place(sh.list[i], larger_than(sh.list[i], sh.list, n), after);
   } else {
     after = reinterpret_cast<float*>(sh.list);
+    if (lowest <= key_value(kKeyNone + 1)) {  // every token: the buckets begin at the smallest one there is
+      __syncthreads();
+      float m = -INFINITY;
+      for (int i = threadIdx.x; i < n; i += kThreads) m = fmaxf(m, -key_value((uint32_t)(sh.list[i] >> 32)));
+      lowest = -rb::block_reduce<true>(m, sh.red);
+    }
     const float width = st.m - lowest, scale = width > 0.f && width < INFINITY ? (kShares - 1) / width : 0.f;
     auto bucket = [&](uint64_t c) { return min(kShares - 1, (int)((st.m - key_value((uint32_t)(c >> 32))) * scale)); };
     for (int b = threadIdx.x; b < kShares; b += kThreads) sh.hist[b] = 0;
@@ -453,23 +523,29 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) top_logprobs_kernel
     top_logp[row * k + i] = -INFINITY;
     top_ids[row * k + i] = -1;
   }
-  if (listed && n > k) {
-    __syncthreads();
+  __syncthreads();
+  // the others: below the k-th value, or equal to it behind the last chosen index
+  const uint32_t kth = sh.kth;
+  const int last = sh.last;
+  auto other = [&](float x, int j) {
+    const uint32_t key = order_key(x);
+    return key < kth || (key == kth && j > last);
+  };
+  if (listed) {
     for (int i = threadIdx.x; i < n - k; i += kThreads) left += rb::exp2_fast(fmaxf((after[i] - st.m) * kk, -1000.f));
+  } else {
+    for_each<kThreads>(r, [&](float x, int j) { left += other(x, j) ? rb::exp2_fast(fmaxf((x - st.m) * kk, -1000.f)) : 0.f; });
   }
   left = rb::block_reduce<false>(left, sh.red);
-  if (listed && left > 1e-18f) {
+  if (left > 1e-18f) {
     if (threadIdx.x == 0) rest[row] = logf(left) - logf(st.s);
     return;
   }
-  // the others one by one, below the k-th value or equal to it behind the last chosen index: after a descent, and where they are too small beside the largest
-  // logit to be summed against it
+  // too small beside the largest logit to be summed against it: against their own
   rb::RowStats others;
-  for (int j = threadIdx.x; j < V; j += kThreads) {
-    const float x = r.at(j);
-    const uint32_t key = order_key(x);
-    if (key < sh.kth || (key == sh.kth && j > sh.last)) others.one(x, kk);
-  }
+  for_each<kThreads>(r, [&](float x, int j) {
+    if (other(x, j)) others.one(x, kk);
+  });
   others = rb::block_stats(others, kk, sh.red);
   if (threadIdx.x == 0) rest[row] = rb::RowResult(others, inv_temp).lse - res.lse;
 }
@@ -485,22 +561,27 @@ int rb_top_logprobs(const void* logits, int64_t row_stride, const int64_t* label
                     float* top_logp, int64_t* top_ids, float* rest, int64_t rows, int V, int k, float inv_temp, int dt, cudaStream_t s) {
   if (rows == 0) return 0;
   if (k < 1 || k > kMaxTop || k > V) return -1;
-  // pieces a group: one where groups of four are too few to bound the k-th logit
-  const int vec = V / (dt == 0 ? 4 : 8), p = vec >= 8 * k ? 4 : 1;
+  const int vec = V / (dt == 0 ? 4 : 8);
+  const bool big = k > kFastTop || (V > kCap && vec < k + k / 8);
+  // pieces a group: one where groups of four (halves of them) are too few to bound the k-th logit
+  const int p = vec >= (!big ? 8 : dt == 0 ? 10 : 5) * k ? 4 : 1;
   // threads: as for the statistics, but no fewer than keep 1024 resident beside what a block has in shared memory
-  const int64_t bytes = sizeof(TopShared) + 1024 + std::max<int64_t>((int64_t)vec / p * 8, kMaxTop * 8);
-  const int nt = rows < 4 * rb::kNumSMs ? 512 : rows >= 16 * rb::kNumSMs && bytes <= 45 << 10 ? 128 : 256;
-#define RB_L4(T, M, NT, P)                                                                                                                                 \
+  const int64_t bytes = sizeof(TopShared<kCap>) + 1024 + std::max<int64_t>((int64_t)vec / p * 8, kCap * 8);
+  const int nt = big ? 256 : rows < 4 * rb::kNumSMs ? 512 : rows >= 16 * rb::kNumSMs && bytes <= 45 << 10 ? 128 : 256;
+#define RB_L4(T, M, NT, P, C)                                                                                                                              \
   {                                                                                                                                                        \
     const int groups = RB_CEIL_DIV(vec, P * NT);                                                                                                           \
-    const bool fast = k <= kFastTop && groups * NT <= kMaxRecords;                                                                                         \
-    const int smem = std::max(fast ? groups * NT * (int)sizeof(uint2) : 0, kMaxTop * 8);                                                                                         \
-    if (smem > 30000 && cudaFuncSetAttribute(top_logprobs_kernel<T, M, NT, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2; \
-    top_logprobs_kernel<T, M, NT, P><<<(unsigned)rows, NT, smem, s>>>((const T*)logits, row_stride, labels, mask, mask_stride, logp, entropy, top_logp,     \
-                                                                      top_ids, rest, V, k, inv_temp, fast ? groups : 0);                                    \
+    const bool fast = groups * NT <= kMaxRecords;                                                                                                          \
+    const int smem = std::max(fast ? groups * NT * (int)sizeof(uint2) : 0, C * 8);                                                                         \
+    if (smem + (int)sizeof(TopShared<C>) > 48 << 10 &&                                                                                                     \
+        cudaFuncSetAttribute(top_logprobs_kernel<T, M, NT, P, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)                        \
+      return -2;                                                                                                                                           \
+    top_logprobs_kernel<T, M, NT, P, C><<<(unsigned)rows, NT, smem, s>>>((const T*)logits, row_stride, labels, mask, mask_stride, logp, entropy, top_logp,  \
+                                                                         top_ids, rest, V, k, inv_temp, fast ? groups : 0);                                 \
   }
-#define RB_L3(T, M, NT) if (p == 4) RB_L4(T, M, NT, 4) else RB_L4(T, M, NT, 1)
-#define RB_L2(T, M) if (nt == 128) { RB_L3(T, M, 128) } else if (nt == 256) { RB_L3(T, M, 256) } else { RB_L3(T, M, 512) }
+#define RB_L3(T, M, NT, C) if (p == 4) RB_L4(T, M, NT, 4, C) else RB_L4(T, M, NT, 1, C)
+#define RB_L2(T, M) \
+  if (big) { RB_L3(T, M, 256, kBigCap) } else if (nt == 128) { RB_L3(T, M, 128, kCap) } else if (nt == 256) { RB_L3(T, M, 256, kCap) } else { RB_L3(T, M, 512, kCap) }
 #define RB_L(T) if (mask) { RB_L2(T, true) } else { RB_L2(T, false) }
   if (dt == 0) { RB_L(float) } else if (dt == 1) { RB_L(__nv_bfloat16) } else if (dt == 2) { RB_L(__half) } else return -1;
 #undef RB_L

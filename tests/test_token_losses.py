@@ -263,6 +263,39 @@ def test_top_ties_cpu():
     check_top("cpu", 9, 40, 11, torch.float32, "packed", False, 1.0, 3, x=tie_rows(40, torch.float32, "cpu"))
 
 
+# many alternatives: nearly every token of the row, more than its groups or pieces can bound, more than the room for candidates
+MANY = [(4, 257, 257, "packed", False, 1.0), (3, 1025, 1024, "odd", False, 0.7), (5, 1300, 256, "packed", True, 1.0), (3, 2000, 256, "wide", False, 1.0),
+        (3, 2048, 1000, "packed", True, 1.0), (3, 2049, 1024, "odd", False, 1.0), (2, 4500, 512, "odd", True, 1.5), (2, 9001, 1024, "packed", False, 1.0),
+        (2, 20481, 512, "odd", False, 1.0), (2, 50257, 300, "odd", True, 0.8), (2, 151936, 1024, "packed", False, 1.0), (1, 400003, 300, "packed", False, 1.0)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,V,k,layout,masked,temp", MANY)
+def test_top_many_gpu(T, V, k, layout, masked, temp, dtype):
+    check_top("cuda", T, V, k, dtype, layout, masked, temp, seed=V + k)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V,k", [(1500, 257), (2048, 1024), (5000, 300), (20000, 700), (450001, 257)])
+def test_top_many_ties_gpu(V, k, dtype):
+    check_top("cuda", 9, V, k, dtype, "packed", False, 1.0, 3, x=tie_rows(V, dtype, "cuda"))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_top_many_of_few_kept_gpu(dtype):
+    """Fewer tokens kept than alternatives asked for, of either sign."""
+    x, _ = make_logits(4, 33000, dtype, 5, "cuda")
+    keep = torch.randperm(33000, generator=torch.Generator().manual_seed(6))[:500].to("cuda")
+    few = torch.full_like(x, -INF)
+    few[:, keep] = x[:, keep]
+    few[1] = few[1].abs().neg()
+    few[2, keep] = -0.0
+    check_top("cuda", 4, 33000, 600, dtype, "packed", False, 1.0, 3, x=few)
+
+
 @gpu
 @pytest.mark.parametrize("V", [50, 30000])
 def test_top_rows_without_a_softmax_gpu(V):
