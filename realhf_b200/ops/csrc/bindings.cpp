@@ -3,6 +3,7 @@
 #include <atomic>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
@@ -367,6 +368,19 @@ bool gradient_goes_past(const Tensor& leaf, bool own_hook) {
   return it != info->end() && it->second.needed_ && !it->second.captures_;
 }
 
+// An error where a call with a gradient is being captured while an eager graph through the same leaf lives: the leaf's gradients are accumulated on the stream of that
+// graph, and the default stream cannot take part in a capture.  Left to the backward pass, the error comes up where nothing can hold it and ends the process.
+void check_capture(const Tensor& leaf, c10::string_view op) {
+  if (!at::GradMode::is_enabled() || !leaf.requires_grad() || !leaf.is_leaf() || !leaf.is_cuda()) return;
+  const auto acc = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (acc == nullptr) return;
+  const auto stream = acc->stream();
+  if (!stream.has_value() || *stream != at::cuda::getDefaultCUDAStream(leaf.get_device()).unwrap()) return;
+  c10::cuda::CUDAGuard guard(leaf.device());
+  TORCH_CHECK(at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None, op,
+              ": a backward pass is being captured while the graph of an eager call through the same leaf lives on the default stream; release that call's results first");
+}
+
 // table[ids] whose gradient is added to the table's .grad (a leaf's, looked up when the gradient comes; a gradient buffer keeps it there).  Native, as a training step
 // of few tokens waits for the host: as a Python function, forward and backward cost 20 us more than the library's lookup, which a step of 1200 us showed.
 class EmbeddingInto : public torch::autograd::Function<EmbeddingInto> {
@@ -426,6 +440,7 @@ TORCH_LIBRARY(realhf_b200, m) {
   m.def("embedding_rows(Tensor table, Tensor ids) -> Tensor", &embedding_rows);
   m.def("embedding_into(Tensor table, Tensor ids, Tensor? grad_ids=None) -> Tensor", &embedding_into);
   m.def("gradient_goes_past(Tensor leaf, bool own_hook) -> bool", &gradient_goes_past);
+  m.def("check_capture(Tensor leaf, str op) -> ()", &check_capture);
   m.def("native_launches() -> int", &native_launches);
   m.def("embedding_grad_tokens() -> int", &rb_embedding_grad_tokens);
   m.def("embedding_grad_(Tensor dy, Tensor ids, Tensor(a!) dst) -> ()", &embedding_grad_);

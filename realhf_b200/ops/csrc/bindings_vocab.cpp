@@ -15,6 +15,7 @@ using at::Tensor;
 using OptT = c10::optional<Tensor>;
 
 bool gradient_goes_past(const Tensor& leaf, bool own_hook);      // bindings.cpp
+void check_capture(const Tensor& leaf, c10::string_view op);     // bindings.cpp
 void attn_check();      // bindings_attn.cpp: an error once a bounded wait of an earlier kernel has run out
 
 // kernels launched where Python does not see the call (in a native backward pass), since the last question
@@ -251,7 +252,10 @@ std::vector<Tensor> logprob_entropy(const Tensor& logits_in, const Tensor& label
   row_values(labels, at::kLong, logits, -1, op, "labels");
   const OptT m = packed(mask);
   mask_rows(m, logits, op);
-  if (at::GradMode::is_enabled() && logits.requires_grad()) return LogprobEntropy::apply(logits, labels, m, inv_temp);
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    check_capture(logits, op);
+    return LogprobEntropy::apply(logits, labels, m, inv_temp);
+  }
   auto r = token_stats(logits, labels, m, inv_temp);
   r.pop_back();
   return r;
@@ -281,7 +285,10 @@ Tensor distill_loss(const Tensor& logits_in, const Tensor& ids_in, const Tensor&
   const OptT rest = fp32(rest_in);
   check_logits(logits, op, inv_temp);
   check_teacher(logits, ids, t, rest, reverse, op);
-  if (at::GradMode::is_enabled() && logits.requires_grad()) return DistillLoss::apply(logits, ids, t, rest, reverse, inv_temp);
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    check_capture(logits, op);
+    return DistillLoss::apply(logits, ids, t, rest, reverse, inv_temp);
+  }
   return distill_fwd(logits, ids, t, rest, reverse, inv_temp, false)[0];
 }
 
@@ -498,8 +505,11 @@ torch::autograd::variable_list head_logprob_entropy(const Tensor& hidden, const 
   row_values(labels, at::kLong, hidden, -1, op, "labels");
   TORCH_CHECK_VALUE(!mask.has_value() || (mask->device() == hidden.device() && mask->scalar_type() == at::kByte && mask->dim() == 2 && mask->size(0) == hidden.size(0) &&
                                           mask->size(1) * 8 >= weight.size(0)), op, ": the mask is a packed uint8 matrix [rows, at least vocabulary / 8]");
-  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
+    check_capture(hidden, op);
+    check_capture(weight, op);
     return HeadLogprobEntropy::apply(hidden, weight, labels, mask, inv_temp, chunk, keep_bytes, flat, num_sms);
+  }
   const auto r = HeadLogprobEntropy::statistics(hidden, weight, labels, mask, inv_temp, chunk, false, num_sms);
   return {r[0], r[1]};
 }

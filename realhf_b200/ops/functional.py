@@ -726,6 +726,12 @@ def _check_head(op: str, hidden, weight, temperature, chunk, **rows):
     _check_mask(op, rows.get("mask_bits"), weight.shape[0])
 
 
+def _check_capture(op: str, *leaves):
+    for t in leaves:
+        if t.is_leaf and t.requires_grad:
+            lib().check_capture(t, op)
+
+
 def lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits=None, temperature: float = 1.0):
     return logprob_entropy_from_logits_ref(hidden.float() @ weight.float().t(), labels, mask_bits, 1.0 / temperature)
 
@@ -747,6 +753,7 @@ def lm_head_logprobs_entropy(hidden, weight, labels, mask_bits=None, temperature
     _check_labels(op, labels)
     if not use_native(hidden):
         return lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits, temperature)
+    _check_capture(op, hidden, weight)
     return _LMHeadTokenStats.apply(hidden, weight, labels.long().contiguous(), mask_bits.contiguous() if mask_bits is not None else None, 1.0 / temperature,
                                    int(chunk), int(keep_bytes))
 
@@ -798,6 +805,7 @@ def lm_head_distill_loss(hidden, weight, top_ids, top_logp, rest_logp=None, reve
     _check_teacher(op, hidden.shape[0], weight.shape[0], hidden.device, top_ids, top_logp, rest_logp, reverse)
     if not use_native(hidden):
         return distill_loss_from_logits_ref(hidden.float() @ weight.float().t(), top_ids, top_logp, rest_logp, reverse, 1.0 / temperature)
+    _check_capture(op, hidden, weight)
     return _LMHeadDistill.apply(hidden, weight, top_ids.long().contiguous(), _rows_f32(top_logp), _rows_f32(rest_logp), bool(reverse), 1.0 / temperature,
                                 int(chunk))
 

@@ -862,6 +862,35 @@ def test_captured_and_replayed_gpu():
 
 
 @gpu
+def test_capture_beside_a_living_eager_graph_is_refused_gpu():
+    T, V, k = 5, 3000, 4
+    x, labels = make_logits(T, V, torch.bfloat16, 1, "cuda")
+    ids, t, tr = (v.cuda() for v in make_teacher(x, k, 3, True))
+    h, w, _ = make_head(T, 64, V, torch.bfloat16, 2, "cuda")
+    a, b, c, f, g = (v.detach().requires_grad_(True) for v in (x, h, w, h.float(), w.float()))
+    calls = [lambda: OF.logprob_entropy_from_logits(a, labels)[1], lambda: OF.distill_loss_from_logits(a, ids, t, tr), lambda: OF.lm_head_logprobs_entropy(b, w, labels)[0],
+             lambda: OF.lm_head_logprobs_entropy(h, c, labels)[0], lambda: OF.lm_head_logprobs_entropy(f, g, labels)[0], lambda: OF.lm_head_distill_loss(b, c, ids, t, tr)]
+    living = [call() for call in calls]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in calls:
+            with pytest.raises(RuntimeError, match="release that call's results first"):
+                call()
+            with torch.no_grad():
+                call()
+    torch.autograd.grad(living, [a, b, c, f, g], [torch.ones_like(y) for y in living])
+    want = [y.detach().clone() for y in living]
+    del living
+    again = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(again):
+        out = [call().detach() for call in calls]
+    again.replay()
+    torch.cuda.synchronize()
+    for y, z in zip(out, want):
+        assert torch.equal(y, z)
+
+
+@gpu
 def test_nothing_beside_the_rows_is_written_gpu():
     """Gradients of a slice of rows: what lies around inputs and outputs stays as it was."""
     T, V = 6, 1003
