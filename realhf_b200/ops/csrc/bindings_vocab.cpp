@@ -8,7 +8,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cmath>
 #include <vector>
 
 using at::Tensor;
@@ -59,10 +58,12 @@ int dtype_code(const Tensor& t) {
   }
 }
 
+bool good_factor(double inv_temp) { return inv_temp >= 1e-30 && inv_temp <= 1e30; }
+
 void check_logits(const Tensor& logits, const char* op, double inv_temp) {
   TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, op, ": logits are a CUDA matrix [rows, vocabulary] with unit inner stride");
   TORCH_CHECK_VALUE(logits.size(1) > 0 && logits.size(1) <= 0x7ffe0000LL && logits.size(0) <= 0x7fffffffLL, op, ": bad size ", logits.sizes());
-  TORCH_CHECK_VALUE((float)inv_temp > 0 && std::isfinite((float)inv_temp), op, ": the inverse temperature is positive and finite, not ", inv_temp);
+  TORCH_CHECK_VALUE(good_factor(inv_temp), op, ": the inverse temperature lies between 1e-30 and 1e30, not at ", inv_temp);
 }
 
 // a contiguous tensor of this device, of one value a row (or [rows, k])
@@ -214,7 +215,7 @@ void check_head(const Tensor& h, const Tensor& w, const char* op, double inv_tem
               ": hidden states [rows, H] and a head [vocabulary, H] on one CUDA device, unit inner stride");
   attn_check();
   TORCH_CHECK(h.scalar_type() == w.scalar_type() && h.element_size() == 2, op, ": 16-bit operands of one type");
-  TORCH_CHECK(w.size(0) > 0 && w.size(0) <= 0x7ffe0000LL && h.size(0) <= 0x7ffe0000LL && inv_temp > 0, op, ": bad sizes or temperature");
+  TORCH_CHECK(w.size(0) > 0 && w.size(0) <= 0x7ffe0000LL && h.size(0) <= 0x7ffe0000LL && good_factor(inv_temp), op, ": bad sizes or temperature");
 }
 
 // A first derivative that is asked for with a graph (create_graph) and then differentiated again is an error, not a zero.
@@ -494,7 +495,7 @@ class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> 
 torch::autograd::variable_list head_logprob_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& labels_in, const OptT& mask_in, double inv_temp, int64_t chunk,
                                                     int64_t keep_bytes, bool flat, int64_t num_sms) {
   const char* op = "lm_head_logprobs_entropy";
-  TORCH_CHECK_VALUE((float)inv_temp > 0 && std::isfinite((float)inv_temp) && chunk >= 1, op, ": the temperature is positive and finite and a chunk one row at least");
+  TORCH_CHECK_VALUE(good_factor(inv_temp) && chunk >= 1, op, ": the temperature lies between 1e-30 and 1e30 and a chunk is one row at least");
   TORCH_CHECK_VALUE(hidden.dim() == 2 && weight.dim() == 2 && hidden.size(1) == weight.size(1) && weight.size(0) > 0 && hidden.device() == weight.device() &&
                         hidden.scalar_type() == weight.scalar_type(), op, ": hidden states [T, H] and a head [V, H] of one type and device");
   TORCH_CHECK(weight.element_size() == 2 && weight.stride(1) == 1 && weight.stride(0) % 8 == 0 && hidden.size(1) % 8 == 0 && weight.size(0) <= 0x7ffe0000LL &&

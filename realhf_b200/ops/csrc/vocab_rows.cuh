@@ -294,10 +294,10 @@ RB_DEVICE RowStats block_stats(RowStats a, float k, float* red) {
 struct RowResult {
   float lse, entropy;
   RB_DEVICE RowResult(const RowStats& r, float inv_temp) {
-    const bool bad = !(r.m < INFINITY);
-    const float ls = logf(r.s);
-    lse = bad ? NAN : (r.m == -INFINITY ? -INFINITY : fmaf(r.m, inv_temp, ls));
-    entropy = bad ? NAN : (r.m == -INFINITY ? 0.f : ls - kLn2 * (r.w / r.s));
+    const float top = r.m * inv_temp, ls = logf(r.s);       // (may leave fp32's range by its scale)
+    const bool bad = !(top < INFINITY), none = top == -INFINITY;
+    lse = bad ? NAN : (none ? -INFINITY : fmaf(r.m, inv_temp, ls));
+    entropy = bad ? NAN : (none ? 0.f : ls - kLn2 * (r.w / r.s));
   }
 };
 

@@ -463,8 +463,8 @@ def _check_rows(op: str, logits, inv_temp, **rows):
         raise ValueError(f"{op}: logits are a matrix [rows, vocabulary], not {tuple(logits.shape)}")
     if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16) and (logits.is_cuda or logits.dtype != torch.float64):
         raise ValueError(f"{op}: logits of type {logits.dtype} (float32, bfloat16 or float16)")
-    if not 0 < inv_temp < float("inf"):
-        raise ValueError(f"{op}: the inverse temperature is positive and finite, not {inv_temp}")
+    if not 1e-30 <= inv_temp <= 1e30:
+        raise ValueError(f"{op}: the inverse temperature lies between 1e-30 and 1e30, not at {inv_temp}")
     _check_row_values(op, logits.shape[0], logits.device, **rows)
 
 
@@ -720,8 +720,8 @@ def _check_head(op: str, hidden, weight, temperature, chunk, **rows):
         raise ValueError(f"{op}: hidden states [T, H] and a head [V, H], not {tuple(hidden.shape)} and {tuple(weight.shape)}")
     if hidden.dtype != weight.dtype or hidden.device != weight.device:
         raise ValueError(f"{op}: hidden states and head of one type and device, not {hidden.dtype} on {hidden.device} and {weight.dtype} on {weight.device}")
-    if not 0 < temperature < float("inf") or chunk < 1:
-        raise ValueError(f"{op}: the temperature is positive and finite and a chunk one row at least")
+    if not (temperature > 0 and 1e-30 <= 1.0 / temperature <= 1e30) or chunk < 1:
+        raise ValueError(f"{op}: the temperature lies between 1e-30 and 1e30 and a chunk is one row at least")
     _check_row_values(op, hidden.shape[0], hidden.device, **rows)
     _check_mask(op, rows.get("mask_bits"), weight.shape[0])
 

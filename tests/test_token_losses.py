@@ -965,6 +965,32 @@ def test_no_rows_cpu():
     check_no_rows("cpu")
 
 
+def check_scales_beyond_fp32(dev, dtype):
+    """Logits whose scaled values leave fp32's range: above it no softmax, below it no token, and a row with its maximum at 0 has that token alone."""
+    x = torch.full((3, 700), -1e10)
+    x[0, 300], x[2, 301], x[2, 5] = 1e10, 0.0, -2e10
+    x, labels = x.to(dtype).to(dev), torch.tensor([300, 300, 301], device=dev)
+    leaf = x.clone().requires_grad_(True)
+    logp, ent = OF.logprob_entropy_from_logits(leaf, labels, inv_temp=1e30)
+    o = OF.top_logprobs_from_logits(x, 2, labels, inv_temp=1e30)
+    for lp, en in ((logp, ent), (o.logp, o.entropy)):
+        assert lp[0].isnan() and en[0].isnan() and lp[1] == -INF and lp[2] == 0 and en[1] == 0 and en[2] == 0
+    assert o.top_logp[0].isnan().all() and (o.top_logp[1] == -INF).all() and o.top_ids.tolist()[:2] == [[-1, -1]] * 2
+    assert o.top_logp[2, 0] == 0 and o.top_ids[2, 0] == 301 and o.rest_logp[2] == -INF
+    d, = torch.autograd.grad((logp + ent)[1:].sum(), leaf)
+    assert not d[1:].any()
+
+
+def test_scales_beyond_fp32_cpu():
+    check_scales_beyond_fp32("cpu", torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+def test_scales_beyond_fp32_gpu(dtype):
+    check_scales_beyond_fp32("cuda", dtype)
+
+
 @gpu
 def test_no_rows_gpu():
     check_no_rows("cuda")
@@ -979,13 +1005,13 @@ def check_refusals(dev):
     L, P, D, E = OF.logprob_entropy_from_logits, OF.top_logprobs_from_logits, OF.distill_loss_from_logits, OF.lm_head_logprobs_entropy
     bad = [
         lambda: L(x[0], labels[:1]), lambda: L(x, labels[:2]), lambda: L(x, labels.float()), lambda: L(x, labels[:, None]), lambda: L(x, labels, inv_temp=0.0),
-        lambda: L(x, labels, inv_temp=float("nan")), lambda: L(x, labels, inv_temp=INF), lambda: L(x.int(), labels), lambda: L(x, labels, bits[:, :2]), lambda: L(x, labels, bits[:2]),
+        lambda: L(x, labels, inv_temp=float("nan")), lambda: L(x, labels, inv_temp=INF), lambda: L(x, labels, inv_temp=1e38), lambda: L(x, labels, inv_temp=1e-40), lambda: L(x.int(), labels), lambda: L(x, labels, bits[:, :2]), lambda: L(x, labels, bits[:2]),
         lambda: L(x, labels, bits.bool()), lambda: L(x[:, :0], labels),
         lambda: P(x, 0), lambda: P(x, 21), lambda: P(torch.zeros(1, 2000, device=dev), 1025), lambda: P(x, 2, labels[:2]), lambda: P(x, 2, inv_temp=-1.0),
         lambda: D(x, ids, t[:, :2]), lambda: D(x, ids[:2], t[:2]), lambda: D(x, ids, t, tr[:2]), lambda: D(x, ids, t, reverse=True), lambda: D(x, t, t),
         lambda: D(x, ids[:, :0], t[:, :0]), lambda: D(x, ids, t, tr[:, None]), lambda: D(x, ids[0], t[0]), lambda: D(x, ids, t.clone().requires_grad_(True)),
         lambda: D(torch.zeros(3, (1 << 20) + 1, device=dev), ids, t),
-        lambda: E(h, w[:, :4], labels), lambda: E(h, w.to(torch.bfloat16), labels), lambda: E(h, w, labels, temperature=0.0), lambda: E(h, w, labels, chunk=0),
+        lambda: E(h, w[:, :4], labels), lambda: E(h, w.to(torch.bfloat16), labels), lambda: E(h, w, labels, temperature=0.0), lambda: E(h, w, labels, temperature=1e38), lambda: E(h, w, labels, chunk=0),
         lambda: E(h, w, labels[:2]), lambda: E(h, w, labels, bits[:, :1]), lambda: OF.lm_head_top_logprobs(h, w, 0), lambda: OF.lm_head_top_logprobs(h, w, 3, chunk=0),
         lambda: OF.lm_head_distill_loss(h, w, ids, t, reverse=True), lambda: OF.lm_head_distill_loss(h[:2], w, ids, t),
     ]
