@@ -41,7 +41,7 @@ int rb_distill_max_listed();
 int64_t rb_distill_max_vocab();
 int rb_distill_fwd(const void*, int64_t, const int64_t*, const float*, const float*, int, float*, float*, float*, float*, int*, int64_t, int, int, float, int,
                    cudaStream_t);
-int rb_distill_bwd(const void*, int64_t, const float*, const float*, const float*, const int*, const float*, void*, int64_t, int64_t, int, int, float, int,
+int rb_distill_bwd(const void*, int64_t, const float*, const float*, const float*, const int*, const float*, void*, int64_t, int64_t, int, int, float, int, int,
                    cudaStream_t);
 }
 
@@ -86,9 +86,9 @@ const uint8_t* mask_rows(const OptT& mask, const Tensor& logits, const char* op)
 int64_t mask_bytes(const OptT& mask) { return mask.has_value() ? mask->size(1) : 0; }
 
 // the gradient's destination: a new matrix, or `out` (the logits themselves, or one like them)
-Tensor gradient_like(const Tensor& logits, const OptT& out, const char* op) {
+Tensor gradient_like(const Tensor& logits, const OptT& out, const char* op, bool any_type = false) {
   if (!out.has_value()) return at::empty({logits.size(0), logits.size(1)}, logits.options());
-  TORCH_CHECK(out->device() == logits.device() && out->scalar_type() == logits.scalar_type() && out->sizes() == logits.sizes() && out->stride(1) == 1, op,
+  TORCH_CHECK(out->device() == logits.device() && (any_type || out->scalar_type() == logits.scalar_type()) && out->sizes() == logits.sizes() && out->stride(1) == 1, op,
               ": the gradient's destination is like the logits");
   return *out;
 }
@@ -203,9 +203,9 @@ Tensor distill_bwd(const Tensor& logits, const Tensor& lse_rest, const Tensor& g
   const auto* gr = static_cast<const float*>(row_values(g_rest, at::kFloat, logits, -1, op, "the rest's gradient"));
   const auto* g = static_cast<const float*>(row_values(g_loss, at::kFloat, logits, -1, op, "the loss's gradient"));
   c10::cuda::CUDAGuard guard(logits.device());
-  Tensor d = gradient_like(logits, out, op);
+  Tensor d = gradient_like(logits, out, op, logits.scalar_type() == at::kFloat);
   const int rc = rb_distill_bwd(logits.data_ptr(), logits.stride(0), lr, gr, gk, id, g, d.data_ptr(), d.stride(0), logits.size(0), (int)logits.size(1), (int)k,
-                                (float)inv_temp, dtype_code(logits), stream());
+                                (float)inv_temp, dtype_code(logits), dtype_code(d), stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
   return d;
 }

@@ -14,6 +14,8 @@
 // needs beside its logits: the listed tokens' own gradients, the rest's and its log-sum-exp.
 #include "vocab_rows.cuh"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int kMaxListed = 1024;
@@ -126,16 +128,22 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_fwd_kernel(
     }
 }
 
-template <typename T>
+// a piece of a row: as many elements of the gradient's type as 16 bytes of logits
+RB_DEVICE void store_once(void* p, const int4& v) { __stcs(reinterpret_cast<int4*>(p), v); }
+RB_DEVICE void store_once(void* p, const int2& v) { __stcs(reinterpret_cast<int2*>(p), v); }
+
+// O: the gradient's type, the logits' own or, of fp32 logits, a 16-bit one
+template <typename T, typename O>
 __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logits, int64_t row_stride, const float* __restrict__ lse_rest_in,
                                                                   const float* __restrict__ grad_rest, const float* __restrict__ grad_listed,
-                                                                  const int* __restrict__ ids, const float* __restrict__ g_loss, T* out, int64_t out_stride,
+                                                                  const int* __restrict__ ids, const float* __restrict__ g_loss, O* out, int64_t out_stride,
                                                                   int V, int k, float inv_temp, int segs) {
   constexpr int VEC = rb::RowSpan<T>::VEC, kPer = kBwdThreads * kBwdVecs * VEC;
+  using Raw = std::conditional_t<sizeof(O) == sizeof(T), int4, int2>;
   const int64_t row = blockIdx.x / segs;
   const int seg = blockIdx.x - (int)(row * segs);
   const T* lr = logits + row * row_stride;
-  T* orow = out + row * out_stride;
+  O* orow = out + row * out_stride;
   const float g = g_loss[row] * inv_temp;
   const bool zero = g == 0.f;
   const int id0 = threadIdx.x < k ? ids[row * k + threadIdx.x] : -1;         // (asked for beside the logits, as the block ends with them)
@@ -147,11 +155,11 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
     return zero ? 0.f : a * e;
   };
   const rb::RowSpan<T> span(lr, V);
-  const bool same = ((reinterpret_cast<uintptr_t>(lr) ^ reinterpret_cast<uintptr_t>(orow)) & 15) == 0;
+  const bool same = (reinterpret_cast<uintptr_t>(orow + span.head) & (sizeof(Raw) - 1)) == 0;
   int lo, hi;                                           // the elements of this block
   if (same) {
     const rb::Pack<T, VEC>* vecs = reinterpret_cast<const rb::Pack<T, VEC>*>(lr + span.head);
-    rb::Pack<T, VEC>* outs = reinterpret_cast<rb::Pack<T, VEC>*>(orow + span.head);
+    Raw* outs = reinterpret_cast<Raw*>(orow + span.head);
     lo = seg == 0 ? 0 : span.head + seg * kPer;
     hi = seg == segs - 1 ? V : min(V, span.head + (seg + 1) * kPer);
     rb::Pack<T, VEC> p[kBwdVecs];                       // all loads before the first use
@@ -167,31 +175,37 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
     for (int u = 0; u < kBwdVecs; ++u) {
       const int i = i0 + u * kBwdThreads;
       if (zero && i < span.nvec) {
-        __stcs(reinterpret_cast<int4*>(outs + i), make_int4(0, 0, 0, 0));
+        store_once(outs + i, Raw{});
       } else if (i < span.nvec) {
+        [[maybe_unused]] rb::Pack<O, VEC> o;
 #pragma unroll
         for (int e = 0; e < VEC; e += 2) {
           float x0, x1;
           rb::unpack2(rb::mul2(rb::fma2(rb::pack2(rb::to_f(p[u].v[e]), rb::to_f(p[u].v[e + 1])), c2, r2), e2), x0, x1);
           rb::unpack2(rb::mul2(rb::pack2(rb::exp2_fast(x0), rb::exp2_fast(x1)), a2), x0, x1);
-          p[u].v[e] = rb::from_f<T>(x0);
-          p[u].v[e + 1] = rb::from_f<T>(x1);
+          if constexpr (std::is_same_v<T, O>) {         // in the logits' registers: 8192 x 131072 656 us, 704 in others
+            p[u].v[e] = rb::from_f<O>(x0);
+            p[u].v[e + 1] = rb::from_f<O>(x1);
+          } else {
+            o.v[e] = rb::from_f<O>(x0);
+            o.v[e + 1] = rb::from_f<O>(x1);
+          }
         }
-        __stcs(reinterpret_cast<int4*>(outs + i), *reinterpret_cast<const int4*>(&p[u]));
+        store_once(outs + i, std::is_same_v<T, O> ? *reinterpret_cast<const Raw*>(&p[u]) : *reinterpret_cast<const Raw*>(&o));
       }
     }
     const int j = span.edge(threadIdx.x, V);
-    if (j >= lo && j < hi) orow[j] = rb::from_f<T>(grad(rb::to_f(lr[j])));
+    if (j >= lo && j < hi) orow[j] = rb::from_f<O>(grad(rb::to_f(lr[j])));
   } else {
     lo = seg * kPer;
     hi = seg == segs - 1 ? V : min(V, (seg + 1) * kPer);
-    for (int j = lo + threadIdx.x; j < hi; j += kBwdThreads) orow[j] = rb::from_f<T>(grad(rb::to_f(lr[j])));
+    for (int j = lo + threadIdx.x; j < hi; j += kBwdThreads) orow[j] = rb::from_f<O>(grad(rb::to_f(lr[j])));
   }
   __syncthreads();                                      // the listed tokens over what was just written
-  if (id0 >= lo && id0 < hi) orow[id0] = rb::from_f<T>(zero ? 0.f : g * listed0);
+  if (id0 >= lo && id0 < hi) orow[id0] = rb::from_f<O>(zero ? 0.f : g * listed0);
   for (int i = threadIdx.x + kBwdThreads; i < k; i += kBwdThreads) {
     const int id = ids[row * k + i];
-    if (id >= lo && id < hi) orow[id] = rb::from_f<T>(zero ? 0.f : g * grad_listed[row * k + i]);
+    if (id >= lo && id < hi) orow[id] = rb::from_f<O>(zero ? 0.f : g * grad_listed[row * k + i]);
   }
 }
 
@@ -222,17 +236,23 @@ int rb_distill_fwd(const void* logits, int64_t row_stride, const int64_t* ids, c
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-// out: [rows, V], may be the logits themselves
+// out: [rows, V] of type out_dt (dt, or a 16-bit one for fp32 logits), may be the logits themselves
 int rb_distill_bwd(const void* logits, int64_t row_stride, const float* lse_rest, const float* grad_rest, const float* grad_listed, const int* ids,
-                   const float* g_loss, void* out, int64_t out_stride, int64_t rows, int V, int k, float inv_temp, int dt, cudaStream_t s) {
+                   const float* g_loss, void* out, int64_t out_stride, int64_t rows, int V, int k, float inv_temp, int dt, int out_dt,
+                   cudaStream_t s) {
   if (rows == 0) return 0;
   const int per = kBwdThreads * kBwdVecs * (dt == 0 ? 4 : 8);
   const int64_t segs = RB_CEIL_DIV((int64_t)V, per);
   if (rows * segs > 0x7fffffffLL) return -3;
-#define RB_L(T)                                                                                                                                        \
-  distill_bwd_kernel<T><<<(unsigned)(rows * segs), kBwdThreads, 0, s>>>((const T*)logits, row_stride, lse_rest, grad_rest, grad_listed, ids, g_loss,     \
-                                                                        (T*)out, out_stride, V, k, inv_temp, (int)segs)
-  if (dt == 0) RB_L(float); else if (dt == 1) RB_L(__nv_bfloat16); else if (dt == 2) RB_L(__half); else return -1;
+#define RB_L(T, O)                                                                                                                                     \
+  distill_bwd_kernel<T, O><<<(unsigned)(rows * segs), kBwdThreads, 0, s>>>((const T*)logits, row_stride, lse_rest, grad_rest, grad_listed, ids, g_loss,  \
+                                                                           (O*)out, out_stride, V, k, inv_temp, (int)segs)
+  if (dt == 0 && out_dt == 0) RB_L(float, float);
+  else if (dt == 0 && out_dt == 1) RB_L(float, __nv_bfloat16);
+  else if (dt == 0 && out_dt == 2) RB_L(float, __half);
+  else if (dt == 1 && out_dt == 1) RB_L(__nv_bfloat16, __nv_bfloat16);
+  else if (dt == 2 && out_dt == 2) RB_L(__half, __half);
+  else return -1;
 #undef RB_L
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }

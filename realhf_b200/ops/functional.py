@@ -771,35 +771,44 @@ def lm_head_top_logprobs(hidden, weight, k: int, labels=None, mask_bits=None, te
 
 class _LMHeadDistill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, ids, t, tr, reverse, inv_temp, chunk):
+    def forward(ctx, hidden, weight, ids, t, tr, reverse, inv_temp, chunk, keep_bytes):
         need, T = any(ctx.needs_input_grad[:2]), hidden.shape[0]
-        parts = []
+        parts, kept, keep = [], [], need and 4 * T * weight.shape[0] <= keep_bytes
         for s in range(0, max(1, T), chunk):
             e = min(T, s + chunk)
-            parts.append(lib().distill_fwd(_head_logits(hidden[s:e], weight), ids[s:e], t[s:e], None if tr is None else tr[s:e], reverse, inv_temp, need))
+            x = _head_logits(hidden[s:e], weight)
+            parts.append(lib().distill_fwd(x, ids[s:e], t[s:e], None if tr is None else tr[s:e], reverse, inv_temp, need))
+            if keep:
+                kept.append(x)
+            del x
         loss, *saved = parts[0] if len(parts) == 1 else [torch.cat(p) for p in zip(*parts)]
         if need:
-            ctx.save_for_backward(hidden, weight, *saved)
+            ctx.save_for_backward(hidden, weight, *saved, *kept)
             ctx.inv_temp, ctx.chunk = inv_temp, chunk
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        hidden, weight, lse_rest, g_rest, g_listed, ids = ctx.saved_tensors
+        hidden, weight, lse_rest, g_rest, g_listed, ids, *kept = ctx.saved_tensors
         g = _rows_f32(g)
 
         def dlogits(s, e):
-            x = _head_logits(hidden[s:e], weight)
-            lib().distill_bwd(x, lse_rest[s:e], g_rest[s:e], g_listed[s:e], ids[s:e], g[s:e], ctx.inv_temp, x)
-            return x if _head_gemm(hidden, weight) is None else _pitched(e - s, x.shape[1], hidden.dtype, x.device).copy_(x)
+            x = kept[s // ctx.chunk] if kept else _head_logits(hidden[s:e], weight)
+            if _head_gemm(hidden, weight) is None:
+                d = None if kept else x
+            else:
+                d = _pitched(e - s, x.shape[1], hidden.dtype, x.device)     # (the products' operand: rounded once)
+            return lib().distill_bwd(x, lse_rest[s:e], g_rest[s:e], g_listed[s:e], ids[s:e], g[s:e], ctx.inv_temp, d)
 
-        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None, None, None)
+        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None, None, None, None)
 
 
-def lm_head_distill_loss(hidden, weight, top_ids, top_logp, rest_logp=None, reverse: bool = False, temperature: float = 1.0, chunk: int = 4096):
-    """`distill_loss_from_logits` of hidden @ weight^T / temperature, differentiable in hidden and weight; fp32 logits and their gradient
-    exist for `chunk` rows at a time."""
+def lm_head_distill_loss(hidden, weight, top_ids, top_logp, rest_logp=None, reverse: bool = False, temperature: float = 1.0, chunk: int = 4096,
+                         keep_bytes: int = 1 << 31):
+    """`distill_loss_from_logits` of hidden @ weight^T / temperature, differentiable in hidden and weight.  The logits' gradient exists for `chunk`
+    rows at a time, and so do the fp32 logits, unless a gradient is needed and all of them (4 T V) take at most `keep_bytes`: then they are kept
+    for the backward pass instead of formed again."""
     op = "lm_head_distill_loss"
     _check_head(op, hidden, weight, temperature, chunk)
     _check_teacher(op, hidden.shape[0], weight.shape[0], hidden.device, top_ids, top_logp, rest_logp, reverse)
@@ -807,7 +816,7 @@ def lm_head_distill_loss(hidden, weight, top_ids, top_logp, rest_logp=None, reve
         return distill_loss_from_logits_ref(hidden.float() @ weight.float().t(), top_ids, top_logp, rest_logp, reverse, 1.0 / temperature)
     _check_capture(op, hidden, weight)
     return _LMHeadDistill.apply(hidden, weight, top_ids.long().contiguous(), _rows_f32(top_logp), _rows_f32(rest_logp), bool(reverse), 1.0 / temperature,
-                                int(chunk))
+                                int(chunk), int(keep_bytes))
 
 
 # ------------------------------------------------------------------------------------------------ GEMM

@@ -667,6 +667,25 @@ def check_chain(dev, dtype):
         assert ws.grad.isfinite().all() and ws.grad.shape == w.shape
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distill_head_kept_logits_gpu(dtype):
+    """Logits kept for the backward pass or formed again: the same gradients, also when it runs twice."""
+    T, H, V, k = 37, 64, 501, 8
+    h, w, labels = make_head(T, H, V, dtype, 1, "cuda")
+    ids, t, tr = (v.cuda() for v in make_teacher(make_logits(T, V, torch.float32, 4)[0], k, 3, True))
+    g = torch.linspace(-1, 2, T, device="cuda")
+    results = []
+    for keep in (4 * T * V, 4 * T * V - 1, 0):
+        a, b = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        loss = OF.lm_head_distill_loss(a, b, ids, t, tr, temperature=1.2, chunk=16, keep_bytes=keep)
+        for _ in range(2):
+            results.append((loss.detach(), *torch.autograd.grad(loss, [a, b], g, retain_graph=True)))
+    for r in results[1:]:
+        for x, y in zip(results[0], r):
+            assert torch.equal(x, y)
+
+
 def test_chain_cpu():
     check_chain("cpu", torch.float32)
 
