@@ -30,19 +30,22 @@ int rb_top_logprobs(const void*, int64_t, const int64_t*, const uint8_t*, int64_
 int64_t rb_head_stats_scratch(int);
 int rb_head_stats(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, float*, void*, int64_t, float*, float*, float*, int, int, int,
                   float, int, int, cudaStream_t);
-int rb_head_grad(const void*, int64_t, const float*, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*, void*, int64_t,
-                 int, int, int, int, float, int, cudaStream_t);
+int rb_head_grad(const void*, int64_t, const float*, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*, const uint32_t*,
+                 void*, int64_t, int, int, int, int, float, int, cudaStream_t);
+int rb_head_grad_peak(const int64_t*, const float*, const float*, const float*, uint32_t*, int, float, cudaStream_t);
+int rb_head_unscale(const float*, const uint32_t*, void*, int64_t, int, int, cudaStream_t);
 int rb_head_stats_bwd(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*,
-                      void*, int64_t, int, int, int, float, int, int, cudaStream_t);
+                      const uint32_t*, void*, int64_t, int, int, int, float, int, int, cudaStream_t);
 int rb_head_dhidden_splits(int, int, int, int);
-int rb_head_dhidden(const void*, const void*, int64_t, int64_t, float*, void*, int, int, int, int, int, int, cudaStream_t);
+int rb_head_dhidden(const void*, const void*, int64_t, int64_t, const uint32_t*, float*, void*, int, int, int, int, int, int, cudaStream_t);
 int rb_gemm_tcgen05(const void*, const void*, void*, const void*, int, int, int, int64_t, int64_t, int64_t, int, int, int, int, int, int, int, int, cudaStream_t);
 int rb_distill_max_listed();
 int64_t rb_distill_max_vocab();
 int rb_distill_fwd(const void*, int64_t, const int64_t*, const float*, const float*, int, float*, float*, float*, float*, int*, int64_t, int, int, float, int,
                    cudaStream_t);
-int rb_distill_bwd(const void*, int64_t, const float*, const float*, const float*, const int*, const float*, void*, int64_t, int64_t, int, int, float, int, int,
-                   cudaStream_t);
+int rb_distill_peak(const float*, const float*, const float*, uint32_t*, int64_t, int, float, cudaStream_t);
+int rb_distill_bwd(const void*, int64_t, const float*, const float*, const float*, const int*, const float*, const uint32_t*, void*, int64_t, int64_t, int, int, float, int,
+                   int, cudaStream_t);
 }
 
 namespace {
@@ -92,6 +95,14 @@ Tensor gradient_like(const Tensor& logits, const OptT& out, const char* op, bool
               ": the gradient's destination is like the logits");
   return *out;
 }
+
+// the bound that gradients in fp16 are scaled by (`head_grad_peak`, `distill_peak`), or none
+const uint32_t* peak_of(const OptT& peak, const Tensor& like, const char* op) {
+  if (!peak.has_value()) return nullptr;
+  TORCH_CHECK(peak->device() == like.device() && peak->scalar_type() == at::kFloat && peak->numel() == 1, op, ": the peak is one fp32 number");
+  return static_cast<const uint32_t*>(peak->data_ptr());
+}
+Tensor new_peak(const Tensor& like) { return at::zeros({1}, like.options().dtype(at::kFloat)); }
 
 // whole numbers as contiguous int64
 Tensor whole_numbers(const Tensor& t, const char* op, const char* name) {
@@ -191,8 +202,23 @@ std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& ids, const T
   return {loss, lse_rest, g_rest, g_listed, ids_out};
 }
 
+// a bound of all gradients of the logits
+Tensor distill_peak(const Tensor& g_rest, const Tensor& g_listed, const Tensor& g_loss, double inv_temp) {
+  const char* op = "distill_peak";
+  TORCH_CHECK(g_rest.is_cuda() && g_listed.dim() == 2, op, ": gradients of rows on a CUDA device");
+  const int64_t k = g_listed.size(1);
+  const auto* gk = static_cast<const float*>(row_values(g_listed, at::kFloat, g_rest, k, op, "the tokens' gradients"));
+  const auto* gr = static_cast<const float*>(row_values(g_rest, at::kFloat, g_rest, -1, op, "the rest's gradient"));
+  const auto* g = static_cast<const float*>(row_values(g_loss, at::kFloat, g_rest, -1, op, "the loss's gradient"));
+  c10::cuda::CUDAGuard guard(g_rest.device());
+  Tensor peak = new_peak(g_rest);
+  const int rc = rb_distill_peak(gr, gk, g, static_cast<uint32_t*>(peak.data_ptr()), g_rest.size(0), (int)k, (float)inv_temp, stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+  return peak;
+}
+
 Tensor distill_bwd(const Tensor& logits, const Tensor& lse_rest, const Tensor& g_rest, const Tensor& g_listed, const Tensor& ids, const Tensor& g_loss,
-                   double inv_temp, const OptT& out) {
+                   double inv_temp, const OptT& out, const OptT& peak) {
   const char* op = "distill_bwd";
   check_logits(logits, op, inv_temp);
   TORCH_CHECK(ids.dim() == 2, op, ": the tokens are a matrix");
@@ -204,8 +230,8 @@ Tensor distill_bwd(const Tensor& logits, const Tensor& lse_rest, const Tensor& g
   const auto* g = static_cast<const float*>(row_values(g_loss, at::kFloat, logits, -1, op, "the loss's gradient"));
   c10::cuda::CUDAGuard guard(logits.device());
   Tensor d = gradient_like(logits, out, op, logits.scalar_type() == at::kFloat);
-  const int rc = rb_distill_bwd(logits.data_ptr(), logits.stride(0), lr, gr, gk, id, g, d.data_ptr(), d.stride(0), logits.size(0), (int)logits.size(1), (int)k,
-                                (float)inv_temp, dtype_code(logits), dtype_code(d), stream());
+  const int rc = rb_distill_bwd(logits.data_ptr(), logits.stride(0), lr, gr, gk, id, g, peak_of(peak, logits, op), d.data_ptr(), d.stride(0), logits.size(0),
+                                (int)logits.size(1), (int)k, (float)inv_temp, dtype_code(logits), dtype_code(d), stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
   return d;
 }
@@ -273,7 +299,7 @@ class DistillLoss : public torch::autograd::Function<DistillLoss> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
     const auto s = ctx->get_saved_variables();
     ++unseen_launches;
-    return {once(distill_bwd(s[0], s[1], s[2], s[3], s[4], fp32(g[0]), ctx->saved_data["inv_temp"].toDouble(), OptT()), "distill_loss_from_logits"), Tensor(), Tensor(),
+    return {once(distill_bwd(s[0], s[1], s[2], s[3], s[4], fp32(g[0]), ctx->saved_data["inv_temp"].toDouble(), OptT(), OptT()), "distill_loss_from_logits"), Tensor(), Tensor(),
             Tensor(), Tensor(), Tensor()};
   }
 };
@@ -320,9 +346,33 @@ std::vector<Tensor> head_stats(const Tensor& h, const Tensor& w, const Tensor& l
   return {logp, entropy, lse, kept, scratch.slice(0, 0, rows * ((V + 255) / 256 * 2)).clone()};
 }
 
+// a bound of all d logits
+Tensor head_grad_peak(const Tensor& labels, const Tensor& entropy, const OptT& g_logp, const OptT& g_entropy, double inv_temp) {
+  const char* op = "head_grad_peak";
+  const auto* lab = static_cast<const int64_t*>(row_values(labels, at::kLong, entropy, -1, op, "labels"));
+  const auto* e = static_cast<const float*>(row_values(entropy, at::kFloat, entropy, -1, op, "entropy"));
+  const auto* gl = static_cast<const float*>(row_values(g_logp, at::kFloat, entropy, -1, op, "the log-probability's gradient"));
+  const auto* ge = static_cast<const float*>(row_values(g_entropy, at::kFloat, entropy, -1, op, "the entropy's gradient"));
+  c10::cuda::CUDAGuard guard(entropy.device());
+  Tensor peak = new_peak(entropy);
+  const int rc = rb_head_grad_peak(lab, e, gl, ge, static_cast<uint32_t*>(peak.data_ptr()), (int)entropy.size(0), (float)inv_temp, stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+  return peak;
+}
+
+// out = x, or with `add` out += x, x fp32 products of scaled d logits taken back from their scale
+void head_unscale(const Tensor& x, const Tensor& peak, Tensor out, bool add) {
+  const char* op = "head_unscale";
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kFloat && x.is_contiguous() && out.device() == x.device() && out.is_contiguous() && out.sizes() == x.sizes(), op,
+              ": contiguous fp32 products and a destination of their shape");
+  c10::cuda::CUDAGuard guard(x.device());
+  const int rc = rb_head_unscale(x.data_ptr<float>(), peak_of(peak, x, op), out.data_ptr(), x.numel(), dtype_code(out), add, stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+}
+
 // d logits of rows [row0, row0 + out.size(0)) from what head_stats kept
 void head_grad(const Tensor& kept, const Tensor& maxima, const Tensor& labels, const OptT& mask, const Tensor& lse, const Tensor& entropy, const OptT& g_logp,
-               const OptT& g_entropy, double inv_temp, Tensor out, int64_t row0) {
+               const OptT& g_entropy, double inv_temp, Tensor out, int64_t row0, const OptT& peak) {
   const char* op = "head_grad";
   const int64_t all = kept.size(0), rows = out.size(0), V = out.size(1);
   TORCH_CHECK(kept.is_cuda() && kept.dim() == 2 && kept.is_contiguous() && kept.scalar_type() == at::kHalf && kept.size(1) == (V + 7) / 8 * 8 && row0 >= 0 &&
@@ -336,12 +386,13 @@ void head_grad(const Tensor& kept, const Tensor& maxima, const Tensor& labels, c
   const auto* ge = static_cast<const float*>(row_values(g_entropy, at::kFloat, kept, -1, op, "the entropy's gradient"));
   c10::cuda::CUDAGuard guard(kept.device());
   const int rc = rb_head_grad(kept.data_ptr<at::Half>() + row0 * kept.size(1), kept.size(1), maxima.data_ptr<float>(), lab, head_mask(mask, kept, V, op), mask_bytes(mask),
-                              l, e, gl, ge, out.data_ptr(), out.stride(0), (int)row0, (int)rows, (int)all, (int)V, (float)inv_temp, dtype_code(out), stream());
+                              l, e, gl, ge, peak_of(peak, kept, op), out.data_ptr(), out.stride(0), (int)row0, (int)rows, (int)all, (int)V, (float)inv_temp, dtype_code(out),
+                              stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
 }
 
 void head_stats_bwd(const Tensor& h, const Tensor& w, const Tensor& labels, const OptT& mask, const Tensor& lse, const Tensor& entropy, const OptT& g_logp,
-                    const OptT& g_entropy, double inv_temp, Tensor out, int64_t num_sms) {
+                    const OptT& g_entropy, double inv_temp, Tensor out, int64_t num_sms, const OptT& peak) {
   const char* op = "head_stats_bwd";
   check_head(h, w, op, inv_temp);
   const int64_t rows = h.size(0), V = w.size(0);
@@ -354,20 +405,20 @@ void head_stats_bwd(const Tensor& h, const Tensor& w, const Tensor& labels, cons
                   out.stride(1) == 1, op, ": the destination is [rows, vocabulary] of the operands' type");
   c10::cuda::CUDAGuard guard(h.device());
   const int rc = rb_head_stats_bwd(h.data_ptr(), w.data_ptr(), h.stride(0), w.stride(0), lab, head_mask(mask, h, V, op), mask_bytes(mask), l, e, gl, ge,
-                                   out.data_ptr(), out.stride(0), (int)rows, (int)V, (int)h.size(1), (float)inv_temp, dtype_code(h), (int)num_sms, stream());
+                                   peak_of(peak, h, op), out.data_ptr(), out.stride(0), (int)rows, (int)V, (int)h.size(1), (float)inv_temp, dtype_code(h), (int)num_sms, stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
 }
 
-// out [rows, H] = d [rows, vocabulary] x w [vocabulary, H], the sum in `splits` parts
-void head_dhidden(const Tensor& d, const Tensor& w, Tensor out, int64_t splits, int64_t num_sms) {
+// out [rows, H] = d [rows, vocabulary] x w [vocabulary, H], the sum in `splits` parts; peak: taken back from the scale of d
+void head_dhidden(const Tensor& d, const Tensor& w, Tensor out, int64_t splits, int64_t num_sms, const OptT& peak) {
   const char* op = "head_dhidden";
   TORCH_CHECK(d.is_cuda() && w.device() == d.device() && out.device() == d.device() && d.dim() == 2 && w.dim() == 2 && d.size(1) == w.size(0) && d.stride(1) == 1 &&
                   w.stride(1) == 1 && out.is_contiguous() && out.dim() == 2 && out.size(0) == d.size(0) && out.size(1) == w.size(1), op, ": bad shapes");
   TORCH_CHECK(d.scalar_type() == w.scalar_type() && out.scalar_type() == w.scalar_type() && w.element_size() == 2, op, ": 16-bit operands of one type");
   c10::cuda::CUDAGuard guard(d.device());
   Tensor parts = at::empty({splits, d.size(0), w.size(1)}, d.options().dtype(at::kFloat));
-  const int rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), d.stride(0), w.stride(0), parts.data_ptr<float>(), out.data_ptr(), (int)d.size(0), (int)w.size(1),
-                                 (int)d.size(1), (int)splits, dtype_code(d), (int)num_sms, stream());
+  const int rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), d.stride(0), w.stride(0), peak_of(peak, d, op), parts.data_ptr<float>(), out.data_ptr(), (int)d.size(0),
+                                 (int)w.size(1), (int)d.size(1), (int)splits, dtype_code(d), (int)num_sms, stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
 }
 
@@ -442,41 +493,49 @@ class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> 
     const Tensor gl = g[0].defined() ? fp32(g[0]) : Tensor(), ge = g[1].defined() ? fp32(g[1]) : Tensor();
     const Tensor d = at::empty({std::min(step, T), pitch}, h.options());
     const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    const int64_t* lab = labels.data_ptr<int64_t>();
+    // in fp16 d logits leave scaled by their largest size, as those of a mean lie below its smallest number: the products are taken back from it in fp32
+    const Tensor peak = dt == 2 && T > 0 ? new_peak(h) : Tensor();
+    const uint32_t* pk = peak.defined() ? static_cast<const uint32_t*>(peak.data_ptr()) : nullptr;
     Tensor dh = need_h ? at::empty({T, H}, h.options()) : Tensor(), dw, buffer, parts;
     if (need_w) {
       buffer = flat_gradient(w, ctx->saved_data["flat"].toBool());
-      if (buffer.defined() && buffer.scalar_type() != at::kFloat && T > step) buffer = Tensor();      // (16 bits would be rounded once a chunk)
-      dw = buffer.defined()   ? buffer
-           : T > step || T == 0 ? at::zeros({V, H}, h.options().dtype(at::kFloat))
-                                : at::empty({V, H}, h.options());
+      if (buffer.defined() && buffer.scalar_type() != at::kFloat && T > step && !pk) buffer = Tensor();      // (16 bits would be rounded once a chunk)
+      dw = buffer.defined() && !pk ? buffer
+           : T > step || T == 0    ? at::zeros({V, H}, h.options().dtype(at::kFloat))
+                                   : at::empty({V, H}, pk ? h.options().dtype(at::kFloat) : h.options());
     }
-    const bool add = need_w && (buffer.defined() || dw.scalar_type() == at::kFloat);
-    const int64_t* lab = labels.data_ptr<int64_t>();
+    const bool add = need_w && (pk ? T > step : buffer.defined() || dw.scalar_type() == at::kFloat);
     const uint8_t* m = mask.defined() ? mask.data_ptr<uint8_t>() : nullptr;
     auto at_row = [](const Tensor& t, int64_t s) { return t.defined() ? t.data_ptr<float>() + s : nullptr; };
+    if (pk) {
+      const int rc = rb_head_grad_peak(lab, at_row(entropy, 0), at_row(gl, 0), at_row(ge, 0), static_cast<uint32_t*>(peak.data_ptr()), (int)T, (float)inv_temp, stream());
+      TORCH_CHECK(rc == 0, op, ": the gradients' peak failed with code ", rc);
+      ++unseen_launches;
+    }
     for (int64_t s = 0; s < T; s += step) {
       const int64_t n = std::min(step, T - s);
       const char* hs = static_cast<const char*>(h.data_ptr()) + s * h.stride(0) * 2;
       int rc;
       if (kept.defined())
         rc = rb_head_grad(kept.data_ptr<at::Half>() + s * pitch, pitch, maxima.data_ptr<float>(), lab, m, mask_row, at_row(lse, 0), at_row(entropy, 0), at_row(gl, 0),
-                          at_row(ge, 0), d.data_ptr(), pitch, (int)s, (int)n, (int)T, (int)V, (float)inv_temp, dt, stream());
+                          at_row(ge, 0), pk, d.data_ptr(), pitch, (int)s, (int)n, (int)T, (int)V, (float)inv_temp, dt, stream());
       else
         rc = rb_head_stats_bwd(hs, w.data_ptr(), h.stride(0), w.stride(0), lab + s, m ? m + s * mask_row : nullptr, mask_row, at_row(lse, s), at_row(entropy, s),
-                               at_row(gl, s), at_row(ge, s), d.data_ptr(), pitch, (int)n, (int)V, (int)H, (float)inv_temp, dt, num_sms, stream());
+                               at_row(gl, s), at_row(ge, s), pk, d.data_ptr(), pitch, (int)n, (int)V, (int)H, (float)inv_temp, dt, num_sms, stream());
       TORCH_CHECK(rc == 0, op, ": d logits failed with code ", rc);
       ++unseen_launches;
       if (need_h) {       // [n, V] x [V, H]
         void* to = static_cast<char*>(dh.data_ptr()) + s * H * 2;
         const int splits = rb_head_dhidden_splits((int)n, (int)H, (int)V, num_sms);
-        if (splits > 1) {
+        if (splits > 1 || pk) {
           if (!parts.defined() || parts.numel() < splits * n * H) parts = at::empty({splits * n * H}, h.options().dtype(at::kFloat));
-          rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), pitch, w.stride(0), parts.data_ptr<float>(), to, (int)n, (int)H, (int)V, splits, dt, num_sms, stream());
+          rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), pitch, w.stride(0), pk, parts.data_ptr<float>(), to, (int)n, (int)H, (int)V, splits, dt, num_sms, stream());
         } else {
           rc = rb_gemm_tcgen05(d.data_ptr(), w.data_ptr(), to, nullptr, (int)n, (int)H, (int)V, pitch, w.stride(0), H, 0, 1, dt, dt, 0, 0, num_sms, -1, stream());
         }
         TORCH_CHECK(rc == 0, op, ": d hidden failed with code ", rc);
-        unseen_launches += splits > 1 ? 2 : 1;
+        unseen_launches += splits > 1 || pk ? 2 : 1;
       }
       if (need_w) {       // [n, V]^T x [n, H]
         rc = rb_gemm_tcgen05(d.data_ptr(), hs, dw.data_ptr(), nullptr, (int)V, (int)H, (int)n, pitch, h.stride(0), H, 1, 1, dt, dtype_code(dw), add, 0, num_sms, -1,
@@ -484,6 +543,13 @@ class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> 
         TORCH_CHECK(rc == 0, op, ": d weight failed with code ", rc);
         ++unseen_launches;
       }
+    }
+    if (need_w && pk) {
+      const Tensor to = buffer.defined() ? buffer : at::empty({V, H}, h.options());
+      const int rc = rb_head_unscale(dw.data_ptr<float>(), pk, to.data_ptr(), V * H, dtype_code(to), buffer.defined(), stream());
+      TORCH_CHECK(rc == 0, op, ": d weight failed with code ", rc);
+      ++unseen_launches;
+      dw = to;
     }
     if (need_h) out[0] = once(dh, op);
     if (need_w && !buffer.defined()) out[1] = once(dw.scalar_type() == w.scalar_type() ? dw : dw.to(w.scalar_type()), op);
@@ -529,13 +595,16 @@ void register_vocab_ops(torch::Library& m) {
         &head_logprob_entropy);
   m.def("head_stats(Tensor h, Tensor w, Tensor labels, Tensor? mask, float inv_temp, bool keep, int num_sms) -> Tensor[]", &head_stats);
   m.def("head_grad(Tensor kept, Tensor maxima, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, Tensor(a!) out, "
-        "int row0) -> ()", &head_grad);
+        "int row0, Tensor? peak=None) -> ()", &head_grad);
+  m.def("head_grad_peak(Tensor labels, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp) -> Tensor", &head_grad_peak);
+  m.def("head_unscale(Tensor x, Tensor peak, Tensor(a!) out, bool add) -> ()", &head_unscale);
   m.def("head_stats_bwd(Tensor h, Tensor w, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
-        "Tensor(a!) out, int num_sms) -> ()", &head_stats_bwd);
-  m.def("head_dhidden(Tensor d, Tensor w, Tensor(a!) out, int splits, int num_sms) -> ()", &head_dhidden);
+        "Tensor(a!) out, int num_sms, Tensor? peak=None) -> ()", &head_stats_bwd);
+  m.def("head_dhidden(Tensor d, Tensor w, Tensor(a!) out, int splits, int num_sms, Tensor? peak=None) -> ()", &head_dhidden);
   m.def("head_dhidden_splits(int rows, int width, int vocab, int num_sms) -> int",
         [](int64_t m, int64_t n, int64_t v, int64_t sms) -> int64_t { return rb_head_dhidden_splits((int)m, (int)n, (int)v, (int)sms); });
   m.def("distill_fwd(Tensor logits, Tensor ids, Tensor top_logp, Tensor? rest_logp, bool reverse, float inv_temp, bool need_grad) -> Tensor[]", &distill_fwd);
-  m.def("distill_bwd(Tensor logits, Tensor lse_rest, Tensor g_rest, Tensor g_listed, Tensor ids, Tensor g_loss, float inv_temp, Tensor(a!)? out) -> Tensor",
-        &distill_bwd);
+  m.def("distill_bwd(Tensor logits, Tensor lse_rest, Tensor g_rest, Tensor g_listed, Tensor ids, Tensor g_loss, float inv_temp, Tensor(a!)? out, "
+        "Tensor? peak=None) -> Tensor", &distill_bwd);
+  m.def("distill_peak(Tensor g_rest, Tensor g_listed, Tensor g_loss, float inv_temp) -> Tensor", &distill_peak);
 }

@@ -136,15 +136,16 @@ RB_DEVICE void store_once(void* p, const int2& v) { __stcs(reinterpret_cast<int2
 template <typename T, typename O>
 __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logits, int64_t row_stride, const float* __restrict__ lse_rest_in,
                                                                   const float* __restrict__ grad_rest, const float* __restrict__ grad_listed,
-                                                                  const int* __restrict__ ids, const float* __restrict__ g_loss, O* out, int64_t out_stride,
-                                                                  int V, int k, float inv_temp, int segs) {
+                                                                  const int* __restrict__ ids, const float* __restrict__ g_loss,
+                                                                  const uint32_t* __restrict__ peak, O* out, int64_t out_stride, int V, int k, float inv_temp,
+                                                                  int segs) {
   constexpr int VEC = rb::RowSpan<T>::VEC, kPer = kBwdThreads * kBwdVecs * VEC;
   using Raw = std::conditional_t<sizeof(O) == sizeof(T), int4, int2>;
   const int64_t row = blockIdx.x / segs;
   const int seg = blockIdx.x - (int)(row * segs);
   const T* lr = logits + row * row_stride;
   O* orow = out + row * out_stride;
-  const float g = g_loss[row] * inv_temp;
+  const float g = g_loss[row] * inv_temp * (peak ? rb::grad_scale(*peak) : 1.f);
   const bool zero = g == 0.f;
   const int id0 = threadIdx.x < k ? ids[row * k + threadIdx.x] : -1;         // (asked for beside the logits, as the block ends with them)
   const float listed0 = threadIdx.x < k ? grad_listed[row * k + threadIdx.x] : 0.f;
@@ -209,6 +210,20 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
   }
 }
 
+// The largest gradient of a row's logits into the peak of all rows, a warp a row: an unlisted token's is at most the rest's.
+__global__ void __launch_bounds__(128) distill_peak_kernel(const float* __restrict__ grad_rest, const float* __restrict__ grad_listed, const float* __restrict__ g_loss,
+                                                           uint32_t* peak, int64_t rows, int k, float inv_temp) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const float g = fabsf(g_loss[row]) * inv_temp;
+  float v = 0.f;
+  for (int i = (threadIdx.x & 31) - 1; i < k; i += 32) {
+    const float x = g * fabsf(i < 0 ? grad_rest[row] : grad_listed[row * k + i]);
+    if (x < INFINITY) v = fmaxf(v, x);
+  }
+  rb::raise_peak(peak, v);
+}
+
 }  // namespace
 
 extern "C" {
@@ -236,16 +251,23 @@ int rb_distill_fwd(const void* logits, int64_t row_stride, const int64_t* ids, c
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-// out: [rows, V] of type out_dt (dt, or a 16-bit one for fp32 logits), may be the logits themselves
+// peak (zeroed before): a bound of all rows' gradients, for grad_scale
+int rb_distill_peak(const float* grad_rest, const float* grad_listed, const float* g_loss, uint32_t* peak, int64_t rows, int k, float inv_temp, cudaStream_t s) {
+  if (rows == 0) return 0;
+  distill_peak_kernel<<<(unsigned)RB_CEIL_DIV(rows, 4), 128, 0, s>>>(grad_rest, grad_listed, g_loss, peak, rows, k, inv_temp);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+// out: [rows, V] of type out_dt (dt, or a 16-bit one for fp32 logits), may be the logits themselves; peak: gradients leave times grad_scale of it, or null
 int rb_distill_bwd(const void* logits, int64_t row_stride, const float* lse_rest, const float* grad_rest, const float* grad_listed, const int* ids,
-                   const float* g_loss, void* out, int64_t out_stride, int64_t rows, int V, int k, float inv_temp, int dt, int out_dt,
+                   const float* g_loss, const uint32_t* peak, void* out, int64_t out_stride, int64_t rows, int V, int k, float inv_temp, int dt, int out_dt,
                    cudaStream_t s) {
   if (rows == 0) return 0;
   const int per = kBwdThreads * kBwdVecs * (dt == 0 ? 4 : 8);
   const int64_t segs = RB_CEIL_DIV((int64_t)V, per);
   if (rows * segs > 0x7fffffffLL) return -3;
 #define RB_L(T, O)                                                                                                                                     \
-  distill_bwd_kernel<T, O><<<(unsigned)(rows * segs), kBwdThreads, 0, s>>>((const T*)logits, row_stride, lse_rest, grad_rest, grad_listed, ids, g_loss,  \
+  distill_bwd_kernel<T, O><<<(unsigned)(rows * segs), kBwdThreads, 0, s>>>((const T*)logits, row_stride, lse_rest, grad_rest, grad_listed, ids, g_loss, peak,  \
                                                                            (O*)out, out_stride, V, k, inv_temp, (int)segs)
   if (dt == 0 && out_dt == 0) RB_L(float, float);
   else if (dt == 0 && out_dt == 1) RB_L(float, __nv_bfloat16);

@@ -7,6 +7,8 @@
 //   from the product formed again, in its epilogue (2 T V H more operations, no memory), or
 //   from the weights e^{x - m} that the forward pass kept, m the maximum of the lane's 128 columns, as fp16 times 2^15: 11 bits for weights down to 2^-29, so that what is kept is
 //   rounded by an eighth of what d logits in bf16 are (T V more numbers of 16 bits between the passes).
+// In fp16 d logits are stored times a power of two that a bound of all of them gives (vocab_rows.cuh, grad_scale), and both products are taken back from it in fp32: with row gradients
+// of 1 / T nearly all of them lie below fp16's smallest number.
 // d h with few tiles: the sum over the vocabulary in parts, fp32 tiles that a second kernel adds up in order (16 rows of 4096 x 32000: 167 us undivided).
 // An epilogue takes 32768 exponentials a CTA, 2048 cycles at least, beside 8 H cycles of products.
 // 8192 x 4096 x 32000 bf16, us: forward 1320 .. 1350 (the plain product 1320 .. 1400), d logits 206 from kept weights, 1380 from the product.
@@ -33,6 +35,7 @@ struct HeadParams {
   float *part_m, *part_s, *part_w, *target;
   // backward
   const float *lse, *entropy, *g_logp, *g_entropy;
+  const uint32_t* peak; // d logits leave times grad_scale of it; null: as they are
   void* out;
   int64_t ld_out;
   int splits;           // d hidden: parts of the sum over the vocabulary, out fp32 [splits, M, N]
@@ -212,6 +215,11 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
         if (p.g_logp && given >= 0) gl = p.g_logp[row] * p.inv_temp;
         if (p.g_entropy) ge = p.g_entropy[row] * p.inv_temp;
         if (gl != 0.f && given >= p.N) gl = NAN;
+        if (p.peak) {
+          const float up = rb::grad_scale(*p.peak);
+          gl *= up;
+          ge *= up;
+        }
       }
       const bool zero = (gl == 0.f && ge == 0.f) || lse == -INFINITY;
       const float a = -(gl + ge * H);
@@ -434,9 +442,14 @@ __global__ void __launch_bounds__(kGradThreads) head_grad_kernel(const __half* _
   const int row = blockIdx.x / segs, seg = blockIdx.x - row * segs, whole = row0 + row;
   const float lse = p.lse[whole], H = p.entropy[whole];
   const int64_t given = p.labels[whole];
-  const float ge = p.g_entropy ? p.g_entropy[whole] * p.inv_temp : 0.f;
+  float ge = p.g_entropy ? p.g_entropy[whole] * p.inv_temp : 0.f;
   float gl = p.g_logp && given >= 0 ? p.g_logp[whole] * p.inv_temp : 0.f;
   if (gl != 0.f && given >= p.N) gl = NAN;
+  if (p.peak) {
+    const float up = rb::grad_scale(*p.peak);
+    gl *= up;
+    ge *= up;
+  }
   const bool zero = (gl == 0.f && ge == 0.f) || lse == -INFINITY;
   const bool gone = p.mask && given >= 0 && given < p.N && (p.mask[whole * p.mask_stride + (given >> 3)] >> (given & 7)) & 1;
   const int label = given >= 0 && given < p.N && !gone ? (int)given : -1;
@@ -512,8 +525,39 @@ __global__ void __launch_bounds__(kGradThreads) head_grad_kernel(const __half* _
   }
 }
 
-// parts [splits, n] -> their sum, rounded once; n a multiple of 8
-template <typename T> __global__ void __launch_bounds__(256) head_sum_kernel(const float* __restrict__ parts, T* __restrict__ out, int splits, int64_t n) {
+// A bound of a row's d logits, c (|g_logp| (1 - p) + |g_entropy| p |y + H|) with p |y| <= 1 / e, into the peak of all rows.
+__global__ void __launch_bounds__(256) head_grad_peak_kernel(const int64_t* __restrict__ labels, const float* __restrict__ entropy, const float* __restrict__ g_logp,
+                                                             const float* __restrict__ g_entropy, uint32_t* peak, int rows, float inv_temp) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  float v = 0.f;
+  if (row < rows) {
+    if (g_logp && labels[row] >= 0) v = fabsf(g_logp[row]);
+    if (g_entropy && g_entropy[row] != 0.f) v += fabsf(g_entropy[row]) * (entropy[row] + 0.37f);
+  }
+  rb::raise_peak(peak, v * inv_temp);
+}
+
+// out (+)= products, n numbers, taken back from the scale of their d logits; kAdd: to what `out` holds
+template <typename T, bool kAdd> __global__ void __launch_bounds__(256) head_unscale_kernel(const float* __restrict__ x, const uint32_t* __restrict__ peak, T* __restrict__ out,
+                                                                                            int64_t n) {
+  const float down = rb::grad_unscale(*peak);
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i + 4 <= n) {
+    const float4 v = *reinterpret_cast<const float4*>(x + i);
+    rb::Pack<T, 4> o;
+    if (kAdd) o = *reinterpret_cast<const rb::Pack<T, 4>*>(out + i);
+    const float a[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.v[e] = rb::from_f<T>(kAdd ? fmaf(a[e], down, rb::to_f(o.v[e])) : a[e] * down);
+    *reinterpret_cast<rb::Pack<T, 4>*>(out + i) = o;
+  } else {
+    for (int64_t j = i; j < n; ++j) out[j] = rb::from_f<T>(kAdd ? fmaf(x[j], down, rb::to_f(out[j])) : x[j] * down);
+  }
+}
+
+// parts [splits, n] -> their sum, rounded once; n a multiple of 8; peak: taken back from the scale of d logits
+template <typename T> __global__ void __launch_bounds__(256) head_sum_kernel(const float* __restrict__ parts, const uint32_t* __restrict__ peak, T* __restrict__ out, int splits,
+                                                                             int64_t n) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
   if (i >= n) return;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
@@ -522,6 +566,11 @@ template <typename T> __global__ void __launch_bounds__(256) head_sum_kernel(con
     const float4 u = *reinterpret_cast<const float4*>(parts + s * n + i), v = *reinterpret_cast<const float4*>(parts + s * n + i + 4);
     a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
     b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+  }
+  if (peak) {
+    const float down = rb::grad_unscale(*peak);
+    a.x *= down; a.y *= down; a.z *= down; a.w *= down;
+    b.x *= down; b.y *= down; b.z *= down; b.w *= down;
   }
   rb::Pack<T, 8> o;
   o.v[0] = rb::from_f<T>(a.x); o.v[1] = rb::from_f<T>(a.y); o.v[2] = rb::from_f<T>(a.z); o.v[3] = rb::from_f<T>(a.w);
@@ -592,9 +641,30 @@ int rb_head_stats(const void* h, const void* w, int64_t ld_h, int64_t ld_w, cons
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
-// out: d logits [M, N] of the operands' type, rows ld_out apart (a multiple of 8), 16-byte aligned
+// peak (zeroed before): a bound of the rows' d logits, for grad_scale; g_logp, g_entropy may be null
+int rb_head_grad_peak(const int64_t* labels, const float* entropy, const float* g_logp, const float* g_entropy, uint32_t* peak, int rows, float inv_temp, cudaStream_t s) {
+  if (rows <= 0) return 0;
+  head_grad_peak_kernel<<<RB_CEIL_DIV(rows, 256), 256, 0, s>>>(labels, entropy, g_logp, g_entropy, peak, rows, inv_temp);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+// out [n] of type dt (0 fp32, 2 fp16) = x, or add: += x, over the scale; both 16-byte aligned
+int rb_head_unscale(const float* x, const uint32_t* peak, void* out, int64_t n, int dt, int add, cudaStream_t s) {
+  if (n <= 0) return 0;
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) return -12;
+  const int64_t blocks = RB_CEIL_DIV(n, 256 * 4);
+  if (blocks > 0x7fffffffLL) return -3;
+#define RB_L(T, A) head_unscale_kernel<T, A><<<(unsigned)blocks, 256, 0, s>>>(x, peak, (T*)out, n)
+  if (dt == 0) { if (add) RB_L(float, true); else RB_L(float, false); }
+  else if (dt == 2) { if (add) RB_L(__half, true); else RB_L(__half, false); }
+  else return -10;
+#undef RB_L
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+// out: d logits [M, N] of the operands' type, rows ld_out apart (a multiple of 8), 16-byte aligned; peak: see HeadParams
 int rb_head_stats_bwd(const void* h, const void* w, int64_t ld_h, int64_t ld_w, const int64_t* labels, const uint8_t* mask, int64_t mask_stride, const float* lse,
-                      const float* entropy, const float* g_logp, const float* g_entropy, void* out, int64_t ld_out, int M, int N, int K, float inv_temp, int in_dt,
+                      const float* entropy, const float* g_logp, const float* g_entropy, const uint32_t* peak, void* out, int64_t ld_out, int M, int N, int K, float inv_temp, int in_dt,
                       int num_sms, cudaStream_t s) {
   if (M <= 0) return 0;
   if (ld_out % 8 || (reinterpret_cast<uintptr_t>(out) & 15)) return -12;
@@ -604,7 +674,7 @@ int rb_head_stats_bwd(const void* h, const void* w, int64_t ld_h, int64_t ld_w, 
   p.M = M; p.N = N; p.K = K;
   p.inv_temp = inv_temp;
   p.labels = labels; p.mask = mask; p.mask_stride = mask_stride;
-  p.lse = lse; p.entropy = entropy; p.g_logp = g_logp; p.g_entropy = g_entropy;
+  p.lse = lse; p.entropy = entropy; p.g_logp = g_logp; p.g_entropy = g_entropy; p.peak = peak;
   p.out = out; p.ld_out = ld_out;
   p.status = rb_attn_status();
   if (p.status == nullptr) return -14;
@@ -613,8 +683,8 @@ int rb_head_stats_bwd(const void* h, const void* w, int64_t ld_h, int64_t ld_w, 
 
 // d logits [rows, N] of rows row0 .. of a forward pass over all_rows rows, from what it kept (`kept`: these rows; part_m, labels, mask and values a row: all rows); out as above
 int rb_head_grad(const void* kept, int64_t ld_kept, const float* part_m, const int64_t* labels, const uint8_t* mask, int64_t mask_stride, const float* lse,
-                 const float* entropy, const float* g_logp, const float* g_entropy, void* out, int64_t ld_out, int row0, int rows, int all_rows, int N, float inv_temp,
-                 int dt, cudaStream_t s) {
+                 const float* entropy, const float* g_logp, const float* g_entropy, const uint32_t* peak, void* out, int64_t ld_out, int row0, int rows, int all_rows, int N,
+                 float inv_temp, int dt, cudaStream_t s) {
   if (rows <= 0) return 0;
   if (ld_out % 8 || ld_kept % 8 || ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(kept)) & 15) || row0 < 0 || row0 + rows > all_rows) return -12;
   HeadParams p{};
@@ -622,7 +692,7 @@ int rb_head_grad(const void* kept, int64_t ld_kept, const float* part_m, const i
   p.inv_temp = inv_temp;
   p.labels = labels; p.mask = mask; p.mask_stride = mask_stride;
   p.part_m = const_cast<float*>(part_m);
-  p.lse = lse; p.entropy = entropy; p.g_logp = g_logp; p.g_entropy = g_entropy;
+  p.lse = lse; p.entropy = entropy; p.g_logp = g_logp; p.g_entropy = g_entropy; p.peak = peak;
   p.out = out; p.ld_out = ld_out;
   const int64_t segs = RB_CEIL_DIV(RB_CEIL_DIV(N, 8), kGradThreads * kGradPieces);
   if (rows * segs > 0x7fffffffLL) return -3;
@@ -646,9 +716,9 @@ int rb_head_dhidden_splits(int M, int N, int V, int num_sms) {
   return best;
 }
 
-// d [M, V] (rows ld_d apart, a multiple of 8), w [V, N], parts: fp32 [splits, M, N], out [M, N] contiguous; N a multiple of 8.
-int rb_head_dhidden(const void* d, const void* w, int64_t ld_d, int64_t ld_w, float* parts, void* out, int M, int N, int V, int splits, int in_dt, int num_sms,
-                    cudaStream_t s) {
+// d [M, V] (rows ld_d apart, a multiple of 8), w [V, N], parts: fp32 [splits, M, N], out [M, N] contiguous; N a multiple of 8.  peak: that d is scaled by, or null.
+int rb_head_dhidden(const void* d, const void* w, int64_t ld_d, int64_t ld_w, const uint32_t* peak, float* parts, void* out, int M, int N, int V, int splits, int in_dt,
+                    int num_sms, cudaStream_t s) {
   if (M <= 0) return 0;
   if (in_dt != 1 && in_dt != 2) return -10;
   if (N % 8 || ld_d % 8 || ld_w % 8 || ((reinterpret_cast<uintptr_t>(d) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 15)) return -11;
@@ -666,8 +736,8 @@ int rb_head_dhidden(const void* d, const void* w, int64_t ld_d, int64_t ld_w, fl
   if (rc) return rc;
   const int64_t n = (int64_t)M * N;
   const unsigned blocks = (unsigned)RB_CEIL_DIV(n, 256 * 8);
-  if (in_dt == 1) head_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(parts, (__nv_bfloat16*)out, splits, n);
-  else head_sum_kernel<__half><<<blocks, 256, 0, s>>>(parts, (__half*)out, splits, n);
+  if (in_dt == 1) head_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(parts, peak, (__nv_bfloat16*)out, splits, n);
+  else head_sum_kernel<__half><<<blocks, 256, 0, s>>>(parts, peak, (__half*)out, splits, n);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 

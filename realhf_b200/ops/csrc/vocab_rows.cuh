@@ -317,4 +317,18 @@ template <typename T> RB_DEVICE float label_logp(const T* row, int64_t label, co
   return fmaf(to_f(row[label]), inv_temp, -lse);
 }
 
+// The power of two that brings `peak` (the bits of a finite fp32 number >= 0, a bound of all gradients of logits) into [2^14, 2^15), 1 for a peak of 0.  Of the type fp16 the
+// gradients of a mean over thousands of rows, a probability over thousands of tokens each, lie below the smallest number; scaled they keep 11 bits down to 2^-29 of the
+// largest.  Exact to apply and to take back: both it and its reciprocal are normal numbers.
+RB_DEVICE float grad_scale(uint32_t peak) {
+  const int e = peak ? min(max(268 - (int)(peak >> 23), 1), 253) : 127;
+  return __uint_as_float((uint32_t)e << 23);
+}
+RB_DEVICE float grad_unscale(uint32_t peak) { return __uint_as_float((254u << 23) - __float_as_uint(grad_scale(peak))); }
+// a gradient's size into the peak of all of them; one that is no number takes no part (its row is NaN whatever the scale)
+RB_DEVICE void raise_peak(uint32_t* peak, float v) {
+  const float most = warp_max(v < INFINITY ? v : 0.f);
+  if ((threadIdx.x & 31) == 0 && most > 0.f) atomicMax(peak, __float_as_uint(most));
+}
+
 }  // namespace rb

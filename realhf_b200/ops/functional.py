@@ -626,8 +626,8 @@ def _head_logits(h, w):
     return lib().gemm(G.tma_rows(h), w, _pitched(h.shape[0], w.shape[0], torch.float32, h.device), None, False, False, False, None, 0, G._sms(h.device), -1)
 
 
-def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
-    """(d hidden, d weight) of a head whose rows [s, e) have the logits' gradient dlogits_of(s, e)."""
+def _head_backward(hidden, weight, needs, chunk: int, dlogits_of, peak=None):
+    """(d hidden, d weight) of a head whose rows [s, e) have the logits' gradient dlogits_of(s, e), in fp16 times the scale that `peak` gives."""
     T = hidden.shape[0]
     dh = torch.empty_like(hidden, memory_format=torch.contiguous_format) if needs[0] else None
     G = _head_gemm(hidden, weight)
@@ -635,7 +635,10 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
     if needs[1]:
         own = bool(getattr(weight, "_main_grad_hooked", False)) and len(weight._post_accumulate_grad_hooks or ()) == 1
         buffer = _row_grad_buffer(weight) if G is not None and weight.is_leaf and lib().gradient_goes_past(weight, own) else None
-        if buffer is not None and (buffer.dtype == torch.float32 or (buffer.dtype == weight.dtype and T <= chunk)):
+        if peak is not None:
+            buffer = buffer if buffer is not None and buffer.dtype in (torch.float32, weight.dtype) else None
+            dw = (torch.zeros if T > chunk or T == 0 else torch.empty)(weight.shape, dtype=torch.float32, device=weight.device)
+        elif buffer is not None and (buffer.dtype == torch.float32 or T <= chunk):
             dw = buffer              # the products' fp32 sums are added to it; one of 16 bits would be rounded once a chunk
         elif G is None or T > chunk or T == 0:
             dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device)
@@ -651,8 +654,8 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
         if dh is not None:                                                                   # [t, V] x [V, H]
             sms = G._sms(weight.device)
             splits = lib().head_dhidden_splits(e - s, weight.shape[1], weight.shape[0], sms)
-            if splits > 1:
-                lib().head_dhidden(d, weight, dh[s:e], splits, sms)
+            if splits > 1 or peak is not None:
+                lib().head_dhidden(d, weight, dh[s:e], splits, sms, peak)
             else:
                 G.gemm(d, weight, out=dh[s:e], b_mn=True)
         if needs[1]:
@@ -660,8 +663,11 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of):
             if dw is None:
                 whole = G.gemm(d, h, a_mn=True, b_mn=True)                                   # [t, V]^T x [t, H], rounded once
             else:
-                G.gemm(d, h, out=dw, a_mn=True, b_mn=True, accumulate=True)
-    if dw is not None and dw is not buffer:
+                G.gemm(d, h, out=dw, a_mn=True, b_mn=True, accumulate=peak is None or T > chunk)
+    if peak is not None and dw is not None:
+        whole = None if buffer is not None else torch.empty_like(dw, dtype=weight.dtype)
+        lib().head_unscale(dw, peak, buffer if whole is None else whole, whole is None)
+    elif dw is not None and dw is not buffer:
         whole = dw.to(weight.dtype)
     return dh, whole
 
@@ -699,20 +705,21 @@ class _LMHeadTokenStats(torch.autograd.Function):
         gl, ge = _rows_f32(g_logp), _rows_f32(g_entropy)
         G = _head_gemm(hidden, weight)
         cut = lambda t, s, e: None if t is None else t[s:e]
+        peak = lib().head_grad_peak(labels, entropy, gl, ge, ctx.inv_temp) if G is not None and hidden.dtype == torch.float16 else None
 
         def dlogits(s, e):
             d = _pitched(e - s, weight.shape[0], hidden.dtype, hidden.device) if G is not None else None
             if kept is not None:
-                lib().head_grad(kept, maxima, labels, mask_bits, lse, entropy, gl, ge, ctx.inv_temp, d, s)
+                lib().head_grad(kept, maxima, labels, mask_bits, lse, entropy, gl, ge, ctx.inv_temp, d, s, peak)
                 return d
             rows = [cut(t, s, e) for t in (labels, mask_bits, lse, entropy, gl, ge)]
             if G is not None:
-                lib().head_stats_bwd(G.tma_rows(hidden[s:e]), weight, *rows, ctx.inv_temp, d, G._sms(hidden.device))
+                lib().head_stats_bwd(G.tma_rows(hidden[s:e]), weight, *rows, ctx.inv_temp, d, G._sms(hidden.device), peak)
                 return d
             x = _head_logits(hidden[s:e], weight)
             return lib().token_stats_bwd(x, *rows, ctx.inv_temp, x)
 
-        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None, None)
+        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits, peak), None, None, None, None, None)
 
 
 def _check_head(op: str, hidden, weight, temperature, chunk, **rows):
@@ -740,8 +747,8 @@ def lm_head_logprobs_entropy(hidden, weight, labels, mask_bits=None, temperature
     """(log p(label), entropy) of p = softmax(hidden @ weight^T / temperature): hidden [T, H], weight [V, H], labels [T] -> fp32 [T] each,
     differentiable in hidden and weight.  16-bit logits never exist (`lm_head_logprobs` rounds them to the weights' type): the
     statistics come from the product's fp32 accumulators.  Their gradient exists for `chunk` rows at a time, from the weights of the softmax where these
-    take at most `keep_bytes` (2 T V) between the passes and H is 1024 or more, else (0: always) from the product formed again.  Labels and mask as in
-    `logprob_entropy_from_logits`."""
+    take at most `keep_bytes` (2 T V) between the passes and H is 1024 or more, else (0: always) from the product formed again; in fp16 it is scaled on
+    its way by the largest of it, so that row gradients of 1 / T lose nothing.  Labels and mask as in `logprob_entropy_from_logits`."""
     if (use_native(hidden) and hidden.dim() == weight.dim() == 2 and hidden.shape[1] == weight.shape[1] and weight.is_cuda and weight.shape[0] > 0
             and temperature != 0 and getattr(weight, "main_grad", None) is None and not _plain_autograd()):
         G = _head_gemm(hidden, weight)
@@ -791,24 +798,25 @@ class _LMHeadDistill(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         hidden, weight, lse_rest, g_rest, g_listed, ids, *kept = ctx.saved_tensors
-        g = _rows_f32(g)
+        g, G = _rows_f32(g), _head_gemm(hidden, weight)
+        peak = lib().distill_peak(g_rest, g_listed, g, ctx.inv_temp) if G is not None and hidden.dtype == torch.float16 else None
 
         def dlogits(s, e):
             x = kept[s // ctx.chunk] if kept else _head_logits(hidden[s:e], weight)
-            if _head_gemm(hidden, weight) is None:
+            if G is None:
                 d = None if kept else x
             else:
                 d = _pitched(e - s, x.shape[1], hidden.dtype, x.device)     # (the products' operand: rounded once)
-            return lib().distill_bwd(x, lse_rest[s:e], g_rest[s:e], g_listed[s:e], ids[s:e], g[s:e], ctx.inv_temp, d)
+            return lib().distill_bwd(x, lse_rest[s:e], g_rest[s:e], g_listed[s:e], ids[s:e], g[s:e], ctx.inv_temp, d, peak)
 
-        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits), None, None, None, None, None, None, None)
+        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits, peak), None, None, None, None, None, None, None)
 
 
 def lm_head_distill_loss(hidden, weight, top_ids, top_logp, rest_logp=None, reverse: bool = False, temperature: float = 1.0, chunk: int = 4096,
                          keep_bytes: int = 1 << 31):
     """`distill_loss_from_logits` of hidden @ weight^T / temperature, differentiable in hidden and weight.  The logits' gradient exists for `chunk`
-    rows at a time, and so do the fp32 logits, unless a gradient is needed and all of them (4 T V) take at most `keep_bytes`: then they are kept
-    for the backward pass instead of formed again."""
+    rows at a time (fp16: scaled by the largest of it), and so do the fp32 logits, unless a gradient is needed and all of them (4 T V) take at most
+    `keep_bytes`: then they are kept for the backward pass instead of formed again."""
     op = "lm_head_distill_loss"
     _check_head(op, hidden, weight, temperature, chunk)
     _check_teacher(op, hidden.shape[0], weight.shape[0], hidden.device, top_ids, top_logp, rest_logp, reverse)
