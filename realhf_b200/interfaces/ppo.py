@@ -57,7 +57,7 @@ def _actor_loss_from_output(out: ModelOutput, mb: SequenceSample, *, kl_adapter,
     loss_mask = mb.data["ppo_loss_mask"].bool()
     entropy = None
     if entropy_coef != 0.0:     # mean entropy of the answer's distributions (over the tokens that sampling could choose) as a bonus
-        logp, entropy = out.logprobs_entropy(labels, mask_bits, temperature, rows)
+        logp, entropy = out.logprobs_entropy(labels, mask_bits, temperature, rows, rounded=True)    # (old_logp is of rounded logits)
     else:
         logp = out.logprobs(labels, mask_bits, temperature, rows)
     loss, stat = IF.actor_loss_fn(logp, mb.data["old_logp"], mb.data["advantages"], eps_clip, loss_mask)

@@ -138,13 +138,14 @@ class ModelOutput:
         return h, self.head_weight, temperature if self.logit_scale is None else temperature / self.logit_scale
 
     def logprobs_entropy(self, labels: torch.Tensor, mask_bits: Optional[torch.Tensor] = None, temperature: float = 1.0,
-                         rows: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-        """fp32 log p(labels[i] | hidden[rows[i]]) and the entropy of that distribution, both differentiable (`OF.lm_head_logprobs_entropy`)."""
+                         rows: Optional[torch.Tensor] = None, rounded: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+        """fp32 log p(labels[i] | hidden[rows[i]]) and the entropy of that distribution, both differentiable (`OF.lm_head_logprobs_entropy`).  `rounded`: of
+        logits rounded to the head's type, as `logprobs` and generation have them, which a ratio of the two needs (a sharded or capped head always rounds)."""
         lg = self._whole_logits(rows)
         if lg is not None:
             return OF.logprob_entropy_from_logits(lg, labels, mask_bits, 1.0 / temperature)
         h, w, temperature = self._head_rows(rows, temperature)
-        return OF.lm_head_logprobs_entropy(h, w, labels, mask_bits, temperature)
+        return OF.lm_head_logprobs_entropy(h, w, labels, mask_bits, temperature, rounded=rounded)
 
     def top_logprobs(self, k: int, labels: Optional[torch.Tensor] = None, mask_bits: Optional[torch.Tensor] = None, temperature: float = 1.0,
                      rows: Optional[torch.Tensor] = None) -> "OF.TopLogprobs":

@@ -29,13 +29,13 @@ int rb_top_logprobs(const void*, int64_t, const int64_t*, const uint8_t*, int64_
                     cudaStream_t);
 int64_t rb_head_stats_scratch(int);
 int rb_head_stats(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, float*, void*, int64_t, float*, float*, float*, int, int, int,
-                  float, int, int, cudaStream_t);
+                  float, int, int, int, cudaStream_t);
 int rb_head_grad(const void*, int64_t, const float*, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*, const uint32_t*,
                  void*, int64_t, int, int, int, int, float, int, cudaStream_t);
 int rb_head_grad_peak(const int64_t*, const float*, const float*, const float*, uint32_t*, int, float, cudaStream_t);
 int rb_head_unscale(const float*, const uint32_t*, void*, int64_t, int, int, cudaStream_t);
 int rb_head_stats_bwd(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*,
-                      const uint32_t*, void*, int64_t, int, int, int, float, int, int, cudaStream_t);
+                      const uint32_t*, void*, int64_t, int, int, int, float, int, int, int, cudaStream_t);
 int rb_head_dhidden_splits(int, int, int, int);
 int rb_head_dhidden(const void*, const void*, int64_t, int64_t, const uint32_t*, float*, void*, int, int, int, int, int, int, cudaStream_t);
 int rb_gemm_tcgen05(const void*, const void*, void*, const void*, int, int, int, int64_t, int64_t, int64_t, int, int, int, int, int, int, int, int, cudaStream_t);
@@ -328,7 +328,8 @@ const uint8_t* head_mask(const OptT& mask, const Tensor& h, int64_t V, const cha
 }
 
 // keep: also the weights fp16 [rows, vocabulary] and the maxima that they stand against, for head_grad
-std::vector<Tensor> head_stats(const Tensor& h, const Tensor& w, const Tensor& labels, const OptT& mask, double inv_temp, bool keep, int64_t num_sms) {
+std::vector<Tensor> head_stats(const Tensor& h, const Tensor& w, const Tensor& labels, const OptT& mask, double inv_temp, bool keep, int64_t num_sms,
+                               bool rounded) {
   const char* op = "head_stats";
   check_head(h, w, op, inv_temp);
   const int64_t rows = h.size(0), V = w.size(0);
@@ -340,7 +341,7 @@ std::vector<Tensor> head_stats(const Tensor& h, const Tensor& w, const Tensor& l
   Tensor kept = keep ? at::empty({rows, pitch}, f.dtype(at::kHalf)) : Tensor();
   const int rc = rb_head_stats(h.data_ptr(), w.data_ptr(), h.stride(0), w.stride(0), lab, head_mask(mask, h, V, op), mask_bytes(mask), scratch.data_ptr<float>(),
                                keep ? kept.data_ptr() : nullptr, pitch, logp.data_ptr<float>(), entropy.data_ptr<float>(), lse.data_ptr<float>(), (int)rows, (int)V, (int)h.size(1), (float)inv_temp,
-                               dtype_code(h), (int)num_sms, stream());
+                               rounded, dtype_code(h), (int)num_sms, stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
   if (!keep) return {logp, entropy, lse};
   return {logp, entropy, lse, kept, scratch.slice(0, 0, rows * ((V + 255) / 256 * 2)).clone()};
@@ -392,7 +393,7 @@ void head_grad(const Tensor& kept, const Tensor& maxima, const Tensor& labels, c
 }
 
 void head_stats_bwd(const Tensor& h, const Tensor& w, const Tensor& labels, const OptT& mask, const Tensor& lse, const Tensor& entropy, const OptT& g_logp,
-                    const OptT& g_entropy, double inv_temp, Tensor out, int64_t num_sms, const OptT& peak) {
+                    const OptT& g_entropy, double inv_temp, Tensor out, int64_t num_sms, const OptT& peak, bool rounded) {
   const char* op = "head_stats_bwd";
   check_head(h, w, op, inv_temp);
   const int64_t rows = h.size(0), V = w.size(0);
@@ -405,7 +406,8 @@ void head_stats_bwd(const Tensor& h, const Tensor& w, const Tensor& labels, cons
                   out.stride(1) == 1, op, ": the destination is [rows, vocabulary] of the operands' type");
   c10::cuda::CUDAGuard guard(h.device());
   const int rc = rb_head_stats_bwd(h.data_ptr(), w.data_ptr(), h.stride(0), w.stride(0), lab, head_mask(mask, h, V, op), mask_bytes(mask), l, e, gl, ge,
-                                   peak_of(peak, h, op), out.data_ptr(), out.stride(0), (int)rows, (int)V, (int)h.size(1), (float)inv_temp, dtype_code(h), (int)num_sms, stream());
+                                   peak_of(peak, h, op), out.data_ptr(), out.stride(0), (int)rows, (int)V, (int)h.size(1), (float)inv_temp, rounded, dtype_code(h),
+                                   (int)num_sms, stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
 }
 
@@ -442,7 +444,7 @@ class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> 
  public:
   // log-probability, entropy, log-sum-exp and, where kept, the weights and the maxima that they stand against
   static std::vector<Tensor> statistics(const Tensor& hidden, const Tensor& weight, const Tensor& labels, const OptT& mask, double inv_temp, int64_t chunk, bool keep,
-                                        int64_t num_sms) {
+                                        bool rounded, int64_t num_sms) {
     const char* op = "lm_head_logprobs_entropy";
     const int64_t T = hidden.size(0), H = hidden.size(1), V = weight.size(0), mask_row = mask_bytes(mask);
     c10::cuda::CUDAGuard guard(hidden.device());
@@ -456,35 +458,36 @@ class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> 
       const int rc = rb_head_stats(static_cast<const char*>(h.data_ptr()) + s * h.stride(0) * 2, weight.data_ptr(), h.stride(0), weight.stride(0),
                                    labels.data_ptr<int64_t>() + s, m ? m + s * mask_row : nullptr, mask_row, scratch.data_ptr<float>(),
                                    keep ? kept.data_ptr() : nullptr, pitch, logp.data_ptr<float>() + s, entropy.data_ptr<float>() + s, lse.data_ptr<float>() + s,
-                                   (int)std::min(step, T - s), (int)V, (int)H, (float)inv_temp, dtype_code(h), (int)num_sms, stream());
+                                   (int)std::min(step, T - s), (int)V, (int)H, (float)inv_temp, rounded, dtype_code(h), (int)num_sms, stream());
       TORCH_CHECK(rc == 0, op, " failed with code ", rc);
     }
     if (!keep) return {logp, entropy, lse, Tensor(), Tensor()};
     return {logp, entropy, lse, kept, scratch.slice(0, 0, T * ((V + 255) / 256 * 2)).clone()};
   }
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& labels, const OptT& mask,
-                                                double inv_temp, int64_t chunk, int64_t keep_bytes, bool flat, int64_t num_sms) {
+                                                double inv_temp, int64_t chunk, int64_t keep_bytes, bool flat, bool rounded, int64_t num_sms) {
     // keep the weights from width 1024 on: forming and reading them costs what the product of width 512 does (us, both passes up to d logits, kept / formed again:
     // 8192 x 4096 x 32000 1583 / 2715, 2047 x 1024 x 50257 352 / 408, 8192 x 512 x 32000 484 / 486)
     const int64_t T = hidden.size(0);
     const bool keep = T > 256 && hidden.size(1) >= 1024 && 2 * T * weight.size(0) <= keep_bytes;
-    const auto r = statistics(hidden, weight, labels, mask, inv_temp, chunk, keep, num_sms);
+    const auto r = statistics(hidden, weight, labels, mask, inv_temp, chunk, keep, rounded, num_sms);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({hidden, weight, labels, mask.has_value() ? *mask : Tensor(), r[2], r[1], r[3], r[4]});
     ctx->saved_data["inv_temp"] = inv_temp;
     ctx->saved_data["chunk"] = chunk;
     ctx->saved_data["flat"] = flat;
+    ctx->saved_data["rounded"] = rounded;
     ctx->saved_data["num_sms"] = num_sms;
     return {r[0], r[1]};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
     const char* op = "lm_head_logprobs_entropy";
-    torch::autograd::variable_list out(9);
+    torch::autograd::variable_list out(10);
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const Tensor h = tma_rows(saved[0]), w = saved[1], labels = saved[2], mask = saved[3], lse = saved[4], entropy = saved[5], kept = saved[6], maxima = saved[7];
     const double inv_temp = ctx->saved_data["inv_temp"].toDouble();
-    const int num_sms = (int)ctx->saved_data["num_sms"].toInt();
+    const int num_sms = (int)ctx->saved_data["num_sms"].toInt(), rounded = ctx->saved_data["rounded"].toBool();
     const int64_t T = h.size(0), H = h.size(1), V = w.size(0), pitch = (V + 7) / 8 * 8, mask_row = mask.defined() ? mask.size(1) : 0;
     const int64_t step = std::min<int64_t>(ctx->saved_data["chunk"].toInt(), std::max<int64_t>(T, 1));
     const int dt = dtype_code(h);
@@ -522,7 +525,7 @@ class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> 
                           at_row(ge, 0), pk, d.data_ptr(), pitch, (int)s, (int)n, (int)T, (int)V, (float)inv_temp, dt, stream());
       else
         rc = rb_head_stats_bwd(hs, w.data_ptr(), h.stride(0), w.stride(0), lab + s, m ? m + s * mask_row : nullptr, mask_row, at_row(lse, s), at_row(entropy, s),
-                               at_row(gl, s), at_row(ge, s), pk, d.data_ptr(), pitch, (int)n, (int)V, (int)H, (float)inv_temp, dt, num_sms, stream());
+                               at_row(gl, s), at_row(ge, s), pk, d.data_ptr(), pitch, (int)n, (int)V, (int)H, (float)inv_temp, rounded, dt, num_sms, stream());
       TORCH_CHECK(rc == 0, op, ": d logits failed with code ", rc);
       ++unseen_launches;
       if (need_h) {       // [n, V] x [V, H]
@@ -559,7 +562,7 @@ class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> 
 
 // For 16-bit operands as a TMA descriptor takes them; flat: the weight's gradient buffer is its .grad
 torch::autograd::variable_list head_logprob_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& labels_in, const OptT& mask_in, double inv_temp, int64_t chunk,
-                                                    int64_t keep_bytes, bool flat, int64_t num_sms) {
+                                                    int64_t keep_bytes, bool flat, int64_t num_sms, bool rounded) {
   const char* op = "lm_head_logprobs_entropy";
   TORCH_CHECK_VALUE(good_factor(inv_temp) && chunk >= 1, op, ": the temperature lies between 1e-30 and 1e30 and a chunk is one row at least");
   TORCH_CHECK_VALUE(hidden.dim() == 2 && weight.dim() == 2 && hidden.size(1) == weight.size(1) && weight.size(0) > 0 && hidden.device() == weight.device() &&
@@ -575,9 +578,9 @@ torch::autograd::variable_list head_logprob_entropy(const Tensor& hidden, const 
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
     check_capture(hidden, op);
     check_capture(weight, op);
-    return HeadLogprobEntropy::apply(hidden, weight, labels, mask, inv_temp, chunk, keep_bytes, flat, num_sms);
+    return HeadLogprobEntropy::apply(hidden, weight, labels, mask, inv_temp, chunk, keep_bytes, flat, rounded, num_sms);
   }
-  const auto r = HeadLogprobEntropy::statistics(hidden, weight, labels, mask, inv_temp, chunk, false, num_sms);
+  const auto r = HeadLogprobEntropy::statistics(hidden, weight, labels, mask, inv_temp, chunk, false, rounded, num_sms);
   return {r[0], r[1]};
 }
 
@@ -591,15 +594,16 @@ void register_vocab_ops(torch::Library& m) {
   m.def("token_stats_bwd(Tensor logits, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
         "Tensor(a!)? out) -> Tensor", &token_stats_bwd);
   m.def("top_logprobs(Tensor logits, int k, Tensor? labels, Tensor? mask, float inv_temp) -> Tensor[]", &top_logprobs);
-  m.def("head_logprob_entropy(Tensor hidden, Tensor weight, Tensor labels, Tensor? mask, float inv_temp, int chunk, int keep_bytes, bool flat, int num_sms) -> Tensor[]",
+  m.def("head_logprob_entropy(Tensor hidden, Tensor weight, Tensor labels, Tensor? mask, float inv_temp, int chunk, int keep_bytes, bool flat, int num_sms, "
+        "bool rounded=False) -> Tensor[]",
         &head_logprob_entropy);
-  m.def("head_stats(Tensor h, Tensor w, Tensor labels, Tensor? mask, float inv_temp, bool keep, int num_sms) -> Tensor[]", &head_stats);
+  m.def("head_stats(Tensor h, Tensor w, Tensor labels, Tensor? mask, float inv_temp, bool keep, int num_sms, bool rounded=False) -> Tensor[]", &head_stats);
   m.def("head_grad(Tensor kept, Tensor maxima, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, Tensor(a!) out, "
         "int row0, Tensor? peak=None) -> ()", &head_grad);
   m.def("head_grad_peak(Tensor labels, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp) -> Tensor", &head_grad_peak);
   m.def("head_unscale(Tensor x, Tensor peak, Tensor(a!) out, bool add) -> ()", &head_unscale);
   m.def("head_stats_bwd(Tensor h, Tensor w, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
-        "Tensor(a!) out, int num_sms, Tensor? peak=None) -> ()", &head_stats_bwd);
+        "Tensor(a!) out, int num_sms, Tensor? peak=None, bool rounded=False) -> ()", &head_stats_bwd);
   m.def("head_dhidden(Tensor d, Tensor w, Tensor(a!) out, int splits, int num_sms, Tensor? peak=None) -> ()", &head_dhidden);
   m.def("head_dhidden_splits(int rows, int width, int vocab, int num_sms) -> int",
         [](int64_t m, int64_t n, int64_t v, int64_t sms) -> int64_t { return rb_head_dhidden_splits((int)m, (int)n, (int)v, (int)sms); });

@@ -7,6 +7,7 @@
 //   from the product formed again, in its epilogue (2 T V H more operations, no memory), or
 //   from the weights e^{x - m} that the forward pass kept, m the maximum of the lane's 128 columns, as fp16 times 2^15: 11 bits for weights down to 2^-29, so that what is kept is
 //   rounded by an eighth of what d logits in bf16 are (T V more numbers of 16 bits between the passes).
+// `rounded`: each accumulator is rounded to the operands' type first, in both passes, so that log-probabilities are those of stored logits (a ratio of two has to be of one kind).
 // In fp16 d logits are stored times a power of two that a bound of all of them gives (vocab_rows.cuh, grad_scale), and both products are taken back from it in fp32: with row gradients
 // of 1 / T nearly all of them lie below fp16's smallest number.
 // d h with few tiles: the sum over the vocabulary in parts, fp32 tiles that a second kernel adds up in order (16 rows of 4096 x 32000: 167 us undivided).
@@ -15,6 +16,8 @@
 #include "attn_common.cuh"
 #include "cta_pair.cuh"
 #include "vocab_rows.cuh"
+
+#include <type_traits>
 
 namespace {
 
@@ -27,6 +30,7 @@ constexpr int kHeadBand = 8;                                // row tiles walked 
 
 struct HeadParams {
   int M, N, K;
+  int rounded;          // logits are rounded to the operands' type, as a product that stores them leaves them
   float inv_temp;
   const int64_t* labels;
   const uint8_t* mask;
@@ -46,6 +50,19 @@ RB_DEVICE void head_tile(int tile, int tiles_m, int tiles_n, int& mt, int& nt) {
   const int per = kHeadBand * tiles_n, band = tile / per, within = tile - band * per, m0 = band * kHeadBand, size = min(kHeadBand, tiles_m - m0);
   mt = m0 + within % size;
   nt = within / size;
+}
+
+// two logits as type T holds them
+template <typename T> RB_DEVICE void round_pair(float& a, float& b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const float2 f = __half22float2(__floats2half2_rn(a, b));
+    a = f.x;
+    b = f.y;
+  } else {
+    const float2 f = __bfloat1622float2(__floats2bfloat162_rn(a, b));
+    a = f.x;
+    b = f.y;
+  }
 }
 
 // bit i: column col + i of the row is masked out (or beyond the vocabulary)
@@ -245,6 +262,10 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < 32; ++i) m = rb::max_nan(m, __uint_as_float(r[i]));
         }
+        if (p.rounded) {
+          float same = m;
+          round_pair<T>(m, same);
+        }
       }
 #pragma unroll 1
       for (int c = half * (HN / 2); c < (half + 1) * (HN / 2); c += kCols) {
@@ -264,6 +285,10 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
         float x[kCols];
 #pragma unroll
         for (int i = 0; i < kCols; ++i) x[i] = __uint_as_float(r[i]);
+        if (!kSplit && p.rounded) {
+#pragma unroll
+          for (int i = 0; i < kCols; i += 2) round_pair<T>(x[i], x[i + 1]);
+        }
         const int at = label - c;
         if constexpr (kSplit) {
           store_rows32<float>(stage_out, x, reinterpret_cast<float*>(p.out) + ((int64_t)part * p.M + row0) * p.N + col, p.N, p.M - row0, min(32, p.N - col), true,
@@ -616,13 +641,15 @@ int64_t rb_head_stats_scratch(int N) { return 6LL * RB_CEIL_DIV(N, HN) + 1; }
 // h [M, K], w [N, K], in_dt 1 bf16 / 2 fp16, rows 16-byte aligned; labels [M]; scratch: fp32 [rb_head_stats_scratch(N) * M]; its first M * ceil(N / 256) * 2 numbers are the
 // maxima of 128 columns.  kept: fp16 [M, N] for the weights, rows ld_kept apart (a multiple of 8), or null.
 int rb_head_stats(const void* h, const void* w, int64_t ld_h, int64_t ld_w, const int64_t* labels, const uint8_t* mask, int64_t mask_stride, float* scratch,
-                  void* kept, int64_t ld_kept, float* logp, float* entropy, float* lse, int M, int N, int K, float inv_temp, int in_dt, int num_sms, cudaStream_t s) {
+                  void* kept, int64_t ld_kept, float* logp, float* entropy, float* lse, int M, int N, int K, float inv_temp, int rounded, int in_dt, int num_sms,
+                  cudaStream_t s) {
   if (M <= 0) return 0;
   CUtensorMap ta, tb;
   if (const int rc = head_maps(h, w, ld_h, ld_w, M, N, K, in_dt, ta, tb)) return rc;
   const int tiles_n = RB_CEIL_DIV(N, HN);
   HeadParams p{};
   p.M = M; p.N = N; p.K = K;
+  p.rounded = rounded;
   p.inv_temp = inv_temp;
   p.labels = labels; p.mask = mask; p.mask_stride = mask_stride;
   p.part_m = scratch;
@@ -664,14 +691,15 @@ int rb_head_unscale(const float* x, const uint32_t* peak, void* out, int64_t n, 
 
 // out: d logits [M, N] of the operands' type, rows ld_out apart (a multiple of 8), 16-byte aligned; peak: see HeadParams
 int rb_head_stats_bwd(const void* h, const void* w, int64_t ld_h, int64_t ld_w, const int64_t* labels, const uint8_t* mask, int64_t mask_stride, const float* lse,
-                      const float* entropy, const float* g_logp, const float* g_entropy, const uint32_t* peak, void* out, int64_t ld_out, int M, int N, int K, float inv_temp, int in_dt,
-                      int num_sms, cudaStream_t s) {
+                      const float* entropy, const float* g_logp, const float* g_entropy, const uint32_t* peak, void* out, int64_t ld_out, int M, int N, int K, float inv_temp,
+                      int rounded, int in_dt, int num_sms, cudaStream_t s) {
   if (M <= 0) return 0;
   if (ld_out % 8 || (reinterpret_cast<uintptr_t>(out) & 15)) return -12;
   CUtensorMap ta, tb;
   if (const int rc = head_maps(h, w, ld_h, ld_w, M, N, K, in_dt, ta, tb)) return rc;
   HeadParams p{};
   p.M = M; p.N = N; p.K = K;
+  p.rounded = rounded;
   p.inv_temp = inv_temp;
   p.labels = labels; p.mask = mask; p.mask_stride = mask_stride;
   p.lse = lse; p.entropy = entropy; p.g_logp = g_logp; p.g_entropy = g_entropy; p.peak = peak;

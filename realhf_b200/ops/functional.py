@@ -618,9 +618,12 @@ def _pitched(rows: int, cols: int, dtype, device):
     return torch.empty(rows, -(-cols // 8) * 8, dtype=dtype, device=device)[:, :cols]
 
 
-def _head_logits(h, w):
-    """fp32 logits of the head: 16-bit operands keep the accumulator, others multiply in fp32.  (The product without a workspace: two graphs may replay at once.)"""
+def _head_logits(h, w, rounded: bool = False):
+    """fp32 logits of the head: 16-bit operands keep the accumulator, others multiply in fp32.  (The product without a workspace: two graphs may replay at once.)
+    `rounded`: the values that `linear` leaves in the operands' type."""
     G = _head_gemm(h, w)
+    if rounded:
+        return linear(h, w).float()
     if G is None:
         return h.float() @ w.float().t()
     return lib().gemm(G.tma_rows(h), w, _pitched(h.shape[0], w.shape[0], torch.float32, h.device), None, False, False, False, None, 0, G._sms(h.device), -1)
@@ -674,7 +677,7 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of, peak=None):
 
 class _LMHeadTokenStats(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, labels, mask_bits, inv_temp, chunk, keep_bytes):
+    def forward(ctx, hidden, weight, labels, mask_bits, inv_temp, chunk, keep_bytes, rounded):
         ctx.set_materialize_grads(False)
         T, G = hidden.shape[0], _head_gemm(hidden, weight)
         cut = lambda t, s, e: None if t is None else t[s:e]
@@ -682,18 +685,20 @@ class _LMHeadTokenStats(torch.autograd.Function):
         # keep the weights from width 1024 on: forming and reading them costs what the product of width 512 does (us, both passes up to d logits, kept / formed again:
         # 8192 x 4096 x 32000 1583 / 2715, 2047 x 1024 x 50257 352 / 408, 8192 x 512 x 32000 484 / 486)
         if (G is not None and T > 256 and hidden.shape[1] >= 1024 and any(ctx.needs_input_grad[:2]) and 2 * T * weight.shape[0] <= keep_bytes):
-            logp, entropy, lse, kept, maxima = lib().head_stats(G.tma_rows(hidden), weight, labels, mask_bits, inv_temp, True, G._sms(hidden.device))
+            logp, entropy, lse, kept, maxima = lib().head_stats(G.tma_rows(hidden), weight, labels, mask_bits, inv_temp, True, G._sms(hidden.device),
+                                                                  rounded)
         else:
             parts = []
             for s in range(0, max(1, T), chunk):
                 e = min(T, s + chunk)
                 if G is not None:      # (few rows too, though 16 of 4096 x 32000 take 57 us through fp32 logits and about 62 fused: those come from a product with a shared workspace)
-                    parts.append(lib().head_stats(G.tma_rows(hidden[s:e]), weight, labels[s:e], cut(mask_bits, s, e), inv_temp, False, G._sms(hidden.device)))
+                    parts.append(lib().head_stats(G.tma_rows(hidden[s:e]), weight, labels[s:e], cut(mask_bits, s, e), inv_temp, False, G._sms(hidden.device),
+                                                  rounded))
                 else:
-                    parts.append(lib().token_stats(_head_logits(hidden[s:e], weight), labels[s:e], cut(mask_bits, s, e), inv_temp))
+                    parts.append(lib().token_stats(_head_logits(hidden[s:e], weight, rounded), labels[s:e], cut(mask_bits, s, e), inv_temp))
             logp, entropy, lse = parts[0] if len(parts) == 1 else [torch.cat(p) for p in zip(*parts)]
         ctx.save_for_backward(hidden, weight, labels, mask_bits, lse, entropy, kept, maxima)
-        ctx.inv_temp, ctx.chunk = inv_temp, chunk
+        ctx.inv_temp, ctx.chunk, ctx.rounded = inv_temp, chunk, rounded
         return logp, entropy
 
     @staticmethod
@@ -701,7 +706,7 @@ class _LMHeadTokenStats(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy):
         hidden, weight, labels, mask_bits, lse, entropy, kept, maxima = ctx.saved_tensors
         if g_logp is None and g_entropy is None:
-            return (None,) * 7
+            return (None,) * 8
         gl, ge = _rows_f32(g_logp), _rows_f32(g_entropy)
         G = _head_gemm(hidden, weight)
         cut = lambda t, s, e: None if t is None else t[s:e]
@@ -714,12 +719,12 @@ class _LMHeadTokenStats(torch.autograd.Function):
                 return d
             rows = [cut(t, s, e) for t in (labels, mask_bits, lse, entropy, gl, ge)]
             if G is not None:
-                lib().head_stats_bwd(G.tma_rows(hidden[s:e]), weight, *rows, ctx.inv_temp, d, G._sms(hidden.device), peak)
+                lib().head_stats_bwd(G.tma_rows(hidden[s:e]), weight, *rows, ctx.inv_temp, d, G._sms(hidden.device), peak, ctx.rounded)
                 return d
-            x = _head_logits(hidden[s:e], weight)
+            x = _head_logits(hidden[s:e], weight, ctx.rounded)
             return lib().token_stats_bwd(x, *rows, ctx.inv_temp, x)
 
-        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits, peak), None, None, None, None, None)
+        return (*_head_backward(hidden, weight, ctx.needs_input_grad, ctx.chunk, dlogits, peak), None, None, None, None, None, None)
 
 
 def _check_head(op: str, hidden, weight, temperature, chunk, **rows):
@@ -739,30 +744,33 @@ def _check_capture(op: str, *leaves):
             lib().check_capture(t, op)
 
 
-def lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits=None, temperature: float = 1.0):
-    return logprob_entropy_from_logits_ref(hidden.float() @ weight.float().t(), labels, mask_bits, 1.0 / temperature)
+def lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits=None, temperature: float = 1.0, rounded: bool = False):
+    logits = F.linear(hidden, weight) if rounded else hidden.float() @ weight.float().t()
+    return logprob_entropy_from_logits_ref(logits, labels, mask_bits, 1.0 / temperature)
 
 
-def lm_head_logprobs_entropy(hidden, weight, labels, mask_bits=None, temperature: float = 1.0, chunk: int = 8192, keep_bytes: int = 1 << 31):
+def lm_head_logprobs_entropy(hidden, weight, labels, mask_bits=None, temperature: float = 1.0, chunk: int = 8192, keep_bytes: int = 1 << 31,
+                             rounded: bool = False):
     """(log p(label), entropy) of p = softmax(hidden @ weight^T / temperature): hidden [T, H], weight [V, H], labels [T] -> fp32 [T] each,
     differentiable in hidden and weight.  16-bit logits never exist (`lm_head_logprobs` rounds them to the weights' type): the
     statistics come from the product's fp32 accumulators.  Their gradient exists for `chunk` rows at a time, from the weights of the softmax where these
     take at most `keep_bytes` (2 T V) between the passes and H is 1024 or more, else (0: always) from the product formed again; in fp16 it is scaled on
-    its way by the largest of it, so that row gradients of 1 / T lose nothing.  Labels and mask as in `logprob_entropy_from_logits`."""
+    its way by the largest of it, so that row gradients of 1 / T lose nothing.  Labels and mask as in `logprob_entropy_from_logits`.
+    `rounded`: p from logits rounded to the weights' type, as `lm_head_logprobs` has them: for a ratio to what that gave."""
     if (use_native(hidden) and hidden.dim() == weight.dim() == 2 and hidden.shape[1] == weight.shape[1] and weight.is_cuda and weight.shape[0] > 0
             and temperature != 0 and getattr(weight, "main_grad", None) is None and not _plain_autograd()):
         G = _head_gemm(hidden, weight)
         if G is not None:        # (checks its arguments itself; a gradient buffer beside .grad is known to Python alone)
             return tuple(lib().head_logprob_entropy(hidden, weight, labels, mask_bits, 1.0 / temperature, chunk, keep_bytes,
-                                                    bool(getattr(weight, "_grad_in_flat_buffer", False)), G._sms(hidden.device)))
+                                                    bool(getattr(weight, "_grad_in_flat_buffer", False)), G._sms(hidden.device), rounded))
     op = "lm_head_logprobs_entropy"
     _check_head(op, hidden, weight, temperature, chunk, labels=labels, mask_bits=mask_bits)
     _check_labels(op, labels)
     if not use_native(hidden):
-        return lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits, temperature)
+        return lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits, temperature, rounded)
     _check_capture(op, hidden, weight)
     return _LMHeadTokenStats.apply(hidden, weight, labels.long().contiguous(), mask_bits.contiguous() if mask_bits is not None else None, 1.0 / temperature,
-                                   int(chunk), int(keep_bytes))
+                                   int(chunk), int(keep_bytes), bool(rounded))
 
 
 def lm_head_top_logprobs(hidden, weight, k: int, labels=None, mask_bits=None, temperature: float = 1.0, chunk: int = 4096) -> TopLogprobs:
