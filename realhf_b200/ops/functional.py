@@ -766,7 +766,7 @@ def lm_head_logprobs_entropy(hidden, weight, labels, mask_bits=None, temperature
     op = "lm_head_logprobs_entropy"
     _check_head(op, hidden, weight, temperature, chunk, labels=labels, mask_bits=mask_bits)
     _check_labels(op, labels)
-    if not use_native(hidden):
+    if not use_native(hidden) or _plain_autograd():
         return lm_head_logprobs_entropy_ref(hidden, weight, labels, mask_bits, temperature, rounded)
     _check_capture(op, hidden, weight)
     return _LMHeadTokenStats.apply(hidden, weight, labels.long().contiguous(), mask_bits.contiguous() if mask_bits is not None else None, 1.0 / temperature,
@@ -828,7 +828,7 @@ def lm_head_distill_loss(hidden, weight, top_ids, top_logp, rest_logp=None, reve
     op = "lm_head_distill_loss"
     _check_head(op, hidden, weight, temperature, chunk)
     _check_teacher(op, hidden.shape[0], weight.shape[0], hidden.device, top_ids, top_logp, rest_logp, reverse)
-    if not use_native(hidden):
+    if not use_native(hidden) or _plain_autograd():
         return distill_loss_from_logits_ref(hidden.float() @ weight.float().t(), top_ids, top_logp, rest_logp, reverse, 1.0 / temperature)
     _check_capture(op, hidden, weight)
     return _LMHeadDistill.apply(hidden, weight, top_ids.long().contiguous(), _rows_f32(top_logp), _rows_f32(rest_logp), bool(reverse), 1.0 / temperature,
