@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr int kMaxListed = 1024;
+constexpr int kMaxListed = 1024, kMaxVocab = 1 << 20;
 constexpr int kBwdThreads = 256, kBwdVecs = 4;
 
 __host__ __device__ constexpr int bitmap_words(int V) { return (V + 16 + 31) / 32; }
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(128) distill_peak_kernel(const float* __restri
 extern "C" {
 
 int rb_distill_max_listed() { return kMaxListed; }
-int64_t rb_distill_max_vocab() { return 1 << 20; }
+int64_t rb_distill_max_vocab() { return kMaxVocab; }
 
 // grad_rest null: no gradient asked for (then lse_rest, grad_listed and ids_out are null too).
 int rb_distill_fwd(const void* logits, int64_t row_stride, const int64_t* ids, const float* top_logp, const float* rest_logp, int reverse, float* loss,
@@ -240,7 +240,9 @@ int rb_distill_fwd(const void* logits, int64_t row_stride, const int64_t* ids, c
   const int nt = rb::row_threads(rows, V / (dt == 0 ? 4 : 8));
 #define RB_L2(T, NT)                                                                                                                                       \
   {                                                                                                                                                        \
-    if (smem > 32768 && cudaFuncSetAttribute(distill_fwd_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2;       \
+    if (smem > 32768 && /* the most of any vocabulary: the limit is the process's, and another thread may be about to launch */                              \
+        cudaFuncSetAttribute(distill_fwd_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bitmap_words(kMaxVocab) * 4) != cudaSuccess)           \
+      return -2;                                                                                                                                           \
     distill_fwd_kernel<T, NT><<<(unsigned)rows, NT, smem, s>>>((const T*)logits, row_stride, ids, top_logp, rest_logp, reverse, loss, lse_rest, grad_rest,  \
                                                                grad_listed, ids_out, V, k, inv_temp);                                                       \
   }

@@ -41,6 +41,8 @@ constexpr uint32_t kKeyNone = 0x007fffffu;  // order_key(-inf)
 
 constexpr int kFastTop = 256, kMaxRecords = 12288, kCountAll = 128;
 constexpr int kCap = 1024, kBigCap = 2048;   // candidates of a block
+constexpr int kMaxSmem = kMaxRecords * 8;    // dynamic shared memory at most: records, later the candidates by buckets
+static_assert(kMaxSmem >= kBigCap * 8);
 
 template <int kCand> struct TopShared {
   static constexpr int kHalves = kCand == kCap ? 768 : kCand;
@@ -573,8 +575,8 @@ int rb_top_logprobs(const void* logits, int64_t row_stride, const int64_t* label
     const int groups = RB_CEIL_DIV(vec, P * NT);                                                                                                           \
     const bool fast = groups * NT <= kMaxRecords;                                                                                                          \
     const int smem = std::max(fast ? groups * NT * (int)sizeof(uint2) : 0, C * 8);                                                                         \
-    if (smem + (int)sizeof(TopShared<C>) > 48 << 10 &&                                                                                                     \
-        cudaFuncSetAttribute(top_logprobs_kernel<T, M, NT, P, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)                        \
+    if (smem + (int)sizeof(TopShared<C>) > 48 << 10 && /* the most of any length: the limit is the process's, and another thread may be about to launch */     \
+        cudaFuncSetAttribute(top_logprobs_kernel<T, M, NT, P, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)                    \
       return -2;                                                                                                                                           \
     top_logprobs_kernel<T, M, NT, P, C><<<(unsigned)rows, NT, smem, s>>>((const T*)logits, row_stride, labels, mask, mask_stride, logp, entropy, top_logp,  \
                                                                          top_ids, rest, V, k, inv_temp, fast ? groups : 0);                                 \
