@@ -54,7 +54,9 @@ _LEN_FULL = {"input_ids", "packed_seq", "seq", "prompt_mask",
 _LEN_MINUS1 = {"packed_logprobs", "logprobs", "packed_ref_logprobs", "ref_logprobs", "old_logp", "ref_logp",
                "advantages", "ppo_loss_mask", "kl_rewards", "returns",
                # bit-packed [L-1, V/8] here (aligned with the log-probs); the reference ships a bool [L, V]
-               "packed_logits_mask", "logits_mask"}
+               "packed_logits_mask", "logits_mask",
+               # a teacher's most likely next tokens (`ModelOutput.top_logprobs`): [L-1, k], [L-1, k], [L-1]
+               "top_ids", "top_logp", "rest_logp"}
 
 
 class SequenceSample:
