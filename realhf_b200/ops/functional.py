@@ -539,7 +539,7 @@ def top_logprobs_from_logits(logits, k: int, labels=None, mask_bits=None, inv_te
     """The k most likely tokens of every row of logits [T, V], the log of the others' mass, the entropy and, with `labels`, their
     log-probabilities: one read of the logits.  No gradients.  What `distill_loss_from_logits` takes as its teacher.  k is at most
     min(V, 1024); -0 counts as 0; masked tokens are no alternatives; labels as in `logprob_entropy_from_logits`."""
-    if use_native(logits):
+    if use_native(logits) and not _plain_autograd():
         r = lib().top_logprobs(logits.detach(), k, labels, mask_bits, inv_temp)
         return TopLogprobs(r[0], r[1], r[2], r[3], r[4] if labels is not None else None)
     op = "top_logprobs_from_logits"
@@ -621,7 +621,7 @@ def _pitched(rows: int, cols: int, dtype, device):
 def _head_logits(h, w, rounded: bool = False):
     """fp32 logits of the head: 16-bit operands keep the accumulator, others multiply in fp32.  (The product without a workspace: two graphs may replay at once.)
     `rounded`: the values that `linear` leaves in the operands' type."""
-    G = _head_gemm(h, w)
+    G = None if _plain_autograd() else _head_gemm(h, w)
     if rounded:
         return linear(h, w).float()
     if G is None:

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from realhf_b200.ops import functional as OF
-from test_token_losses import DTYPES, U, err, half_step, make_head, make_logits, make_teacher
+from test_token_losses import DTYPES, err, half_step, make_head, make_logits, make_teacher
 
 gpu = pytest.mark.gpu
 
@@ -45,3 +45,35 @@ def test_head_inside_function_transforms_cpu(dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_head_inside_function_transforms_gpu(dtype):
     check_transforms("cuda", dtype)
+
+
+def check_alternatives(dev, dtype):
+    """A list of alternatives taken inside a transform is that of the plain call, to the bounds of test_token_losses.py; what it is multiplied with has its gradient."""
+    h, w, labels = make_head(6, 64, 50, dtype, 1, dev)
+    x = make_logits(12, 50, dtype, 2, dev)[0].view(4, 3, 50)
+    e = 4 * (err(h.double() @ w.double().t(), 50) + 64 * 2.0 ** -22 * 40)
+    flat = OF.top_logprobs_from_logits(x.view(12, 50), 3, labels.repeat(2))
+    got = torch.func.vmap(lambda a, b: OF.top_logprobs_from_logits(a, 3, b))(x, labels.repeat(2).view(4, 3))
+    assert torch.equal(got.top_ids.view(12, 3), flat.top_ids)
+    for a, b in ((got.top_logp, flat.top_logp), (got.rest_logp, flat.rest_logp), (got.logp, flat.logp), (got.entropy, flat.entropy)):
+        assert ((a.reshape(b.shape) - b).abs() <= e * (1 + b.abs())).all()
+    plain = OF.lm_head_top_logprobs(h, w, 3, labels, chunk=4)
+    got = torch.func.vmap(lambda a: OF.lm_head_top_logprobs(a, w, 3, labels, chunk=4).top_logp)(torch.stack([h, h]))
+    assert ((got - plain.top_logp).abs() <= e * (1 + plain.top_logp.abs())).all()
+    top = torch.func.grad(lambda a: (a.float() * OF.lm_head_top_logprobs(a, w, 3).top_logp.sum()).sum())(h)
+    want = plain.top_logp.double().sum()
+    assert ((top.double() - want).abs() <= (18 * e * 21 + half_step(dtype) * want.abs())).all()
+    per = torch.func.grad(lambda a: (a.float() * OF.top_logprobs_from_logits(a, 3).top_logp.sum()).sum())(x[0])
+    want = flat.top_logp[:3].double().sum()
+    assert ((per.double() - want).abs() <= (9 * e * 21 + half_step(dtype) * want.abs())).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+def test_alternatives_inside_function_transforms_cpu(dtype):
+    check_alternatives("cpu", dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_alternatives_inside_function_transforms_gpu(dtype):
+    check_alternatives("cuda", dtype)
