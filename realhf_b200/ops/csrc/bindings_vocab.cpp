@@ -33,12 +33,12 @@ int rb_head_stats(const void*, const void*, int64_t, int64_t, const int64_t*, co
 int rb_head_grad(const void*, int64_t, const float*, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*, const uint32_t*,
                  void*, int64_t, int, int, int, int, float, int, cudaStream_t);
 int rb_head_grad_peak(const int64_t*, const float*, const float*, const float*, uint32_t*, int, float, cudaStream_t);
-int rb_head_unscale(const float*, const uint32_t*, void*, int64_t, int, int, cudaStream_t);
 int rb_head_stats_bwd(const void*, const void*, int64_t, int64_t, const int64_t*, const uint8_t*, int64_t, const float*, const float*, const float*, const float*,
                       const uint32_t*, void*, int64_t, int, int, int, float, int, int, int, cudaStream_t);
 int rb_head_dhidden_splits(int, int, int, int);
 int rb_head_dhidden(const void*, const void*, int64_t, int64_t, const uint32_t*, float*, void*, int, int, int, int, int, int, cudaStream_t);
 int rb_gemm_tcgen05(const void*, const void*, void*, const void*, int, int, int, int64_t, int64_t, int64_t, int, int, int, int, int, int, int, int, cudaStream_t);
+int rb_head_dweight(const void*, const void*, int64_t, int64_t, const uint32_t*, void*, int, int, int, int, int, int, int, cudaStream_t);
 int rb_distill_max_listed();
 int64_t rb_distill_max_vocab();
 int rb_distill_fwd(const void*, int64_t, const int64_t*, const float*, const float*, int, float*, float*, float*, float*, int*, int64_t, int, int, float, int,
@@ -361,16 +361,6 @@ Tensor head_grad_peak(const Tensor& labels, const Tensor& entropy, const OptT& g
   return peak;
 }
 
-// out = x, or with `add` out += x, x fp32 products of scaled d logits taken back from their scale
-void head_unscale(const Tensor& x, const Tensor& peak, Tensor out, bool add) {
-  const char* op = "head_unscale";
-  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kFloat && x.is_contiguous() && out.device() == x.device() && out.is_contiguous() && out.sizes() == x.sizes(), op,
-              ": contiguous fp32 products and a destination of their shape");
-  c10::cuda::CUDAGuard guard(x.device());
-  const int rc = rb_head_unscale(x.data_ptr<float>(), peak_of(peak, x, op), out.data_ptr(), x.numel(), dtype_code(out), add, stream());
-  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
-}
-
 // d logits of rows [row0, row0 + out.size(0)) from what head_stats kept
 void head_grad(const Tensor& kept, const Tensor& maxima, const Tensor& labels, const OptT& mask, const Tensor& lse, const Tensor& entropy, const OptT& g_logp,
                const OptT& g_entropy, double inv_temp, Tensor out, int64_t row0, const OptT& peak) {
@@ -418,9 +408,21 @@ void head_dhidden(const Tensor& d, const Tensor& w, Tensor out, int64_t splits, 
                   w.stride(1) == 1 && out.is_contiguous() && out.dim() == 2 && out.size(0) == d.size(0) && out.size(1) == w.size(1), op, ": bad shapes");
   TORCH_CHECK(d.scalar_type() == w.scalar_type() && out.scalar_type() == w.scalar_type() && w.element_size() == 2, op, ": 16-bit operands of one type");
   c10::cuda::CUDAGuard guard(d.device());
-  Tensor parts = at::empty({splits, d.size(0), w.size(1)}, d.options().dtype(at::kFloat));
+  Tensor parts = at::empty({splits > 1 ? splits : 0, d.size(0), w.size(1)}, d.options().dtype(at::kFloat));
   const int rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), d.stride(0), w.stride(0), peak_of(peak, d, op), parts.data_ptr<float>(), out.data_ptr(), (int)d.size(0),
                                  (int)w.size(1), (int)d.size(1), (int)splits, dtype_code(d), (int)num_sms, stream());
+  TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+}
+
+// out [vocabulary, H], of the operands' type or fp32, = or with `add` += d^T x h, fp16, taken back from the scale of d
+void head_dweight(const Tensor& d, const Tensor& h, Tensor out, bool add, int64_t num_sms, const Tensor& peak) {
+  const char* op = "head_dweight";
+  TORCH_CHECK(d.is_cuda() && h.device() == d.device() && out.device() == d.device() && d.dim() == 2 && h.dim() == 2 && d.size(0) == h.size(0) && d.stride(1) == 1 &&
+                  h.stride(1) == 1 && out.is_contiguous() && out.dim() == 2 && out.size(0) == d.size(1) && out.size(1) == h.size(1), op, ": bad shapes");
+  TORCH_CHECK(d.scalar_type() == at::kHalf && h.scalar_type() == at::kHalf, op, ": fp16 operands");
+  c10::cuda::CUDAGuard guard(d.device());
+  const int rc = rb_head_dweight(d.data_ptr(), h.data_ptr(), d.stride(0), h.stride(0), peak_of(peak, d, op), out.data_ptr(), (int)d.size(0), (int)h.size(1), (int)d.size(1),
+                                 dtype_code(d), dtype_code(out), add, (int)num_sms, stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
 }
 
@@ -503,12 +505,12 @@ class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> 
     Tensor dh = need_h ? at::empty({T, H}, h.options()) : Tensor(), dw, buffer, parts;
     if (need_w) {
       buffer = flat_gradient(w, ctx->saved_data["flat"].toBool());
-      if (buffer.defined() && buffer.scalar_type() != at::kFloat && T > step && !pk) buffer = Tensor();      // (16 bits would be rounded once a chunk)
-      dw = buffer.defined() && !pk ? buffer
-           : T > step || T == 0    ? at::zeros({V, H}, h.options().dtype(at::kFloat))
-                                   : at::empty({V, H}, pk ? h.options().dtype(at::kFloat) : h.options());
+      if (buffer.defined() && buffer.scalar_type() != at::kFloat && T > step) buffer = Tensor();      // (16 bits would be rounded once a chunk)
+      dw = buffer.defined()   ? buffer
+           : T > step || T == 0 ? at::zeros({V, H}, h.options().dtype(at::kFloat))
+                                : at::empty({V, H}, h.options());
     }
-    const bool add = need_w && (pk ? T > step : buffer.defined() || dw.scalar_type() == at::kFloat);
+    const bool add = need_w && (buffer.defined() || dw.scalar_type() == at::kFloat);
     const uint8_t* m = mask.defined() ? mask.data_ptr<uint8_t>() : nullptr;
     auto at_row = [](const Tensor& t, int64_t s) { return t.defined() ? t.data_ptr<float>() + s : nullptr; };
     if (pk) {
@@ -532,27 +534,23 @@ class HeadLogprobEntropy : public torch::autograd::Function<HeadLogprobEntropy> 
         void* to = static_cast<char*>(dh.data_ptr()) + s * H * 2;
         const int splits = rb_head_dhidden_splits((int)n, (int)H, (int)V, num_sms);
         if (splits > 1 || pk) {
-          if (!parts.defined() || parts.numel() < splits * n * H) parts = at::empty({splits * n * H}, h.options().dtype(at::kFloat));
-          rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), pitch, w.stride(0), pk, parts.data_ptr<float>(), to, (int)n, (int)H, (int)V, splits, dt, num_sms, stream());
+          if (splits > 1 && (!parts.defined() || parts.numel() < splits * n * H)) parts = at::empty({splits * n * H}, h.options().dtype(at::kFloat));
+          rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), pitch, w.stride(0), pk, splits > 1 ? parts.data_ptr<float>() : nullptr, to, (int)n, (int)H, (int)V, splits, dt, num_sms, stream());
         } else {
           rc = rb_gemm_tcgen05(d.data_ptr(), w.data_ptr(), to, nullptr, (int)n, (int)H, (int)V, pitch, w.stride(0), H, 0, 1, dt, dt, 0, 0, num_sms, -1, stream());
         }
         TORCH_CHECK(rc == 0, op, ": d hidden failed with code ", rc);
-        unseen_launches += splits > 1 || pk ? 2 : 1;
+        unseen_launches += splits > 1 ? 2 : 1;
       }
       if (need_w) {       // [n, V]^T x [n, H]
-        rc = rb_gemm_tcgen05(d.data_ptr(), hs, dw.data_ptr(), nullptr, (int)V, (int)H, (int)n, pitch, h.stride(0), H, 1, 1, dt, dtype_code(dw), add, 0, num_sms, -1,
-                             stream());
+        if (pk)
+          rc = rb_head_dweight(d.data_ptr(), hs, pitch, h.stride(0), pk, dw.data_ptr(), (int)n, (int)H, (int)V, dt, dtype_code(dw), add, num_sms, stream());
+        else
+          rc = rb_gemm_tcgen05(d.data_ptr(), hs, dw.data_ptr(), nullptr, (int)V, (int)H, (int)n, pitch, h.stride(0), H, 1, 1, dt, dtype_code(dw), add, 0, num_sms, -1,
+                               stream());
         TORCH_CHECK(rc == 0, op, ": d weight failed with code ", rc);
         ++unseen_launches;
       }
-    }
-    if (need_w && pk) {
-      const Tensor to = buffer.defined() ? buffer : at::empty({V, H}, h.options());
-      const int rc = rb_head_unscale(dw.data_ptr<float>(), pk, to.data_ptr(), V * H, dtype_code(to), buffer.defined(), stream());
-      TORCH_CHECK(rc == 0, op, ": d weight failed with code ", rc);
-      ++unseen_launches;
-      dw = to;
     }
     if (need_h) out[0] = once(dh, op);
     if (need_w && !buffer.defined()) out[1] = once(dw.scalar_type() == w.scalar_type() ? dw : dw.to(w.scalar_type()), op);
@@ -601,7 +599,7 @@ void register_vocab_ops(torch::Library& m) {
   m.def("head_grad(Tensor kept, Tensor maxima, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, Tensor(a!) out, "
         "int row0, Tensor? peak=None) -> ()", &head_grad);
   m.def("head_grad_peak(Tensor labels, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp) -> Tensor", &head_grad_peak);
-  m.def("head_unscale(Tensor x, Tensor peak, Tensor(a!) out, bool add) -> ()", &head_unscale);
+  m.def("head_dweight(Tensor d, Tensor h, Tensor(a!) out, bool add, int num_sms, Tensor peak) -> ()", &head_dweight);
   m.def("head_stats_bwd(Tensor h, Tensor w, Tensor labels, Tensor? mask, Tensor lse, Tensor entropy, Tensor? g_logp, Tensor? g_entropy, float inv_temp, "
         "Tensor(a!) out, int num_sms, Tensor? peak=None, bool rounded=False) -> ()", &head_stats_bwd);
   m.def("head_dhidden(Tensor d, Tensor w, Tensor(a!) out, int splits, int num_sms, Tensor? peak=None) -> ()", &head_dhidden);

@@ -8,8 +8,8 @@
 //   from the weights e^{x - m} that the forward pass kept, m the maximum of the lane's 128 columns, as fp16 times 2^15: 11 bits for weights down to 2^-29, so that what is kept is
 //   rounded by an eighth of what d logits in bf16 are (T V more numbers of 16 bits between the passes).
 // `rounded`: each accumulator is rounded to the operands' type first, in both passes, so that log-probabilities are those of stored logits (a ratio of two has to be of one kind).
-// In fp16 d logits are stored times a power of two that a bound of all of them gives (vocab_rows.cuh, grad_scale), and both products are taken back from it in fp32: with row gradients
-// of 1 / T nearly all of them lie below fp16's smallest number.
+// In fp16 d logits are stored times a power of two that a bound of all of them gives (vocab_rows.cuh, grad_scale), and both products are taken back from it in fp32, in their epilogues
+// where their sum is whole: with row gradients of 1 / T nearly all of them lie below fp16's smallest number.
 // d h with few tiles: the sum over the vocabulary in parts, fp32 tiles that a second kernel adds up in order (16 rows of 4096 x 32000: 167 us undivided).
 // An epilogue takes 32768 exponentials a CTA, 2048 cycles at least, beside 8 H cycles of products.
 // 8192 x 4096 x 32000 bf16, us: forward 1320 .. 1350 (the plain product 1320 .. 1400), d logits 206 from kept weights, 1380 from the product.
@@ -43,6 +43,7 @@ struct HeadParams {
   void* out;
   int64_t ld_out;
   int splits;           // d hidden: parts of the sum over the vocabulary, out fp32 [splits, M, N]
+  int direct, add;      // gradients of hidden states and weight straight into `out`, over grad_scale: 1 of the operands' type, 2 fp32; add: to what it holds
   int* status;
 };
 
@@ -97,7 +98,7 @@ template <typename T> RB_DEVICE void store_cols(uint32_t stage, const float (&x)
 // (kernels that have no 64 columns)
 template <typename T> RB_DEVICE void store_cols(uint32_t, const float (&)[32], T*, int64_t, int, int) {}
 
-enum HeadMode { kStats, kStatsKeep, kLogitGrad, kHiddenGrad };
+enum HeadMode { kStats, kStatsKeep, kLogitGrad, kHiddenGrad, kWeightGrad };
 constexpr float kKeepScale = 32768.f;
 
 template <typename T, int kFmt, HeadMode kMode>
@@ -111,9 +112,9 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
   uint64_t *full_bar = bars, *empty_bar = bars + kHeadStages, *tmem_full = bars + 2 * kHeadStages, *tmem_empty = tmem_full + 2;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr bool kBwd = kMode == kLogitGrad, kSplit = kMode == kHiddenGrad;
+  constexpr bool kBwd = kMode == kLogitGrad, kAMN = kMode == kWeightGrad, kSplit = kMode == kHiddenGrad || kAMN;
   constexpr bool kKeep = kMode == kStatsKeep;
-  constexpr int kCols = kBwd || kKeep ? 64 : 32;            // columns an epilogue warp holds at once
+  constexpr int kCols = kBwd || kKeep || kAMN ? 64 : 32;    // columns an epilogue warp holds at once
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
@@ -165,9 +166,15 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
           const uint32_t fb_local = ptx::smem_u32(&full_bar[stage]);
           if (leader) ptx::mbar_arrive_expect_tx(fb_local, 2 * kHeadStage);
           const uint32_t fb = mapa_u32(fb_local, 0);
-          tma_load_2d_cg2(ptx::smem_u32(smem_a + stage * kHeadA), &tma_a, fb, kb * BK, m0);
+          const uint32_t sa = ptx::smem_u32(smem_a + stage * kHeadA);
+          if constexpr (kAMN) {            // d logits as [T, V]: the sum runs over its rows
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) tma_load_2d_cg2(sa + j * (BK * 128), &tma_a, fb, m0 + 64 * j, kb * BK);
+          } else {
+            tma_load_2d_cg2(sa, &tma_a, fb, kb * BK, m0);
+          }
           const uint32_t sb = ptx::smem_u32(smem_b + stage * kHeadB);
-          if constexpr (kSplit) {          // W as [V, H]: the sum runs over its rows
+          if constexpr (kSplit) {          // W as [V, H], h as [T, H]: the sum runs over its rows
 #pragma unroll
             for (int j = 0; j < HN / 2 / 64; ++j) tma_load_2d_cg2(sb + j * (BK * 128), &tma_b, fb, n0 + 64 * j, kb * BK);
           } else {
@@ -179,8 +186,8 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
     }
   } else if (warp == 1) {
     if (leader) {      // the warp runs converged, one elected lane issues
-      constexpr uint32_t idesc = ptx::make_idesc_f16(kFmt, 2 * BM, HN, 0, kSplit ? 1 : 0);
-      constexpr uint32_t kBStep = (kSplit ? 2048 : 32) >> 4;          // 16 elements of the sum further, in descriptor units
+      constexpr uint32_t idesc = ptx::make_idesc_f16(kFmt, 2 * BM, HN, kAMN ? 1 : 0, kSplit ? 1 : 0);
+      constexpr uint32_t kAStep = (kAMN ? 2048 : 32) >> 4, kBStep = (kSplit ? 2048 : 32) >> 4;          // 16 elements of the sum further, in descriptor units
       const uint32_t tm = (uint32_t)ptx::uniform((int)tmem_base);
       int stage = 0, as = 0;
       uint32_t phase = 0, aphase = 0;
@@ -196,11 +203,11 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
           bounded_wait(ptx::smem_u32(&full_bar[stage]), phase, &dead);
           __syncwarp();
           ptx::tc_fence_after();
-          const uint64_t da = ptx::make_smem_desc_sw128(ptx::smem_u32(smem_a + stage * kHeadA), 16, 1024);
+          const uint64_t da = ptx::make_smem_desc_sw128(ptx::smem_u32(smem_a + stage * kHeadA), kAMN ? BK * 128 : 16, 1024);
           const uint64_t db = ptx::make_smem_desc_sw128(ptx::smem_u32(smem_b + stage * kHeadB), kSplit ? BK * 128 : 16, 1024);
           if (ptx::elect_one()) {
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k) tc_mma_f16_cg2(d_tmem, da + k * 2, db + k * kBStep, idesc, (kb | k) != 0 ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) tc_mma_f16_cg2(d_tmem, da + k * kAStep, db + k * kBStep, idesc, (kb | k) != 0 ? 1u : 0u);
             tc_commit_cg2(ptx::smem_u32(&empty_bar[stage]), 0b11);
           }
           __syncwarp();
@@ -291,8 +298,30 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
         }
         const int at = label - c;
         if constexpr (kSplit) {
-          store_rows32<float>(stage_out, x, reinterpret_cast<float*>(p.out) + ((int64_t)part * p.M + row0) * p.N + col, p.N, p.M - row0, min(32, p.N - col), true,
-                              false);
+          if (p.direct) {
+            const float down = p.peak ? rb::grad_unscale(*p.peak) : 1.f;
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) x[i] *= down;
+            const int64_t to = (int64_t)row0 * p.N + col;
+            if (kCols == 64 && p.direct == 1 && !p.add) {
+              store_cols<T>(stage_out, x, reinterpret_cast<T*>(p.out) + to, p.N, p.M - row0, p.N - col);
+              continue;
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < kCols; c0 += 32) {
+              float v[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = x[c0 + i];
+              const int cols = min(32, p.N - col - c0);
+              if (cols <= 0) break;
+              if (p.direct == 2) store_rows32<float>(stage_out, v, reinterpret_cast<float*>(p.out) + to + c0, p.N, p.M - row0, cols, true, p.add);
+              else store_rows32<T>(stage_out, v, reinterpret_cast<T*>(p.out) + to + c0, p.N, p.M - row0, cols, true, p.add);
+            }
+            continue;
+          }
+          if constexpr (kCols == 32)
+            store_rows32<float>(stage_out, x, reinterpret_cast<float*>(p.out) + ((int64_t)part * p.M + row0) * p.N + col, p.N, p.M - row0, min(32, p.N - col), true,
+                                false);
         } else if constexpr (kKeep) {
           if (gone | gone_hi) {
 #pragma unroll
@@ -562,24 +591,6 @@ __global__ void __launch_bounds__(256) head_grad_peak_kernel(const int64_t* __re
   rb::raise_peak(peak, v * inv_temp);
 }
 
-// out (+)= products, n numbers, taken back from the scale of their d logits; kAdd: to what `out` holds
-template <typename T, bool kAdd> __global__ void __launch_bounds__(256) head_unscale_kernel(const float* __restrict__ x, const uint32_t* __restrict__ peak, T* __restrict__ out,
-                                                                                            int64_t n) {
-  const float down = rb::grad_unscale(*peak);
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i + 4 <= n) {
-    const float4 v = *reinterpret_cast<const float4*>(x + i);
-    rb::Pack<T, 4> o;
-    if (kAdd) o = *reinterpret_cast<const rb::Pack<T, 4>*>(out + i);
-    const float a[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o.v[e] = rb::from_f<T>(kAdd ? fmaf(a[e], down, rb::to_f(o.v[e])) : a[e] * down);
-    *reinterpret_cast<rb::Pack<T, 4>*>(out + i) = o;
-  } else {
-    for (int64_t j = i; j < n; ++j) out[j] = rb::from_f<T>(kAdd ? fmaf(x[j], down, rb::to_f(out[j])) : x[j] * down);
-  }
-}
-
 // parts [splits, n] -> their sum, rounded once; n a multiple of 8; peak: taken back from the scale of d logits
 template <typename T> __global__ void __launch_bounds__(256) head_sum_kernel(const float* __restrict__ parts, const uint32_t* __restrict__ peak, T* __restrict__ out, int splits,
                                                                              int64_t n) {
@@ -675,20 +686,6 @@ int rb_head_grad_peak(const int64_t* labels, const float* entropy, const float* 
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
-// out [n] of type dt (0 fp32, 2 fp16) = x, or add: += x, over the scale; both 16-byte aligned
-int rb_head_unscale(const float* x, const uint32_t* peak, void* out, int64_t n, int dt, int add, cudaStream_t s) {
-  if (n <= 0) return 0;
-  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) return -12;
-  const int64_t blocks = RB_CEIL_DIV(n, 256 * 4);
-  if (blocks > 0x7fffffffLL) return -3;
-#define RB_L(T, A) head_unscale_kernel<T, A><<<(unsigned)blocks, 256, 0, s>>>(x, peak, (T*)out, n)
-  if (dt == 0) { if (add) RB_L(float, true); else RB_L(float, false); }
-  else if (dt == 2) { if (add) RB_L(__half, true); else RB_L(__half, false); }
-  else return -10;
-#undef RB_L
-  return cudaGetLastError() == cudaSuccess ? 0 : -3;
-}
-
 // out: d logits [M, N] of the operands' type, rows ld_out apart (a multiple of 8), 16-byte aligned; peak: see HeadParams
 int rb_head_stats_bwd(const void* h, const void* w, int64_t ld_h, int64_t ld_w, const int64_t* labels, const uint8_t* mask, int64_t mask_stride, const float* lse,
                       const float* entropy, const float* g_logp, const float* g_entropy, const uint32_t* peak, void* out, int64_t ld_out, int M, int N, int K, float inv_temp,
@@ -744,7 +741,8 @@ int rb_head_dhidden_splits(int M, int N, int V, int num_sms) {
   return best;
 }
 
-// d [M, V] (rows ld_d apart, a multiple of 8), w [V, N], parts: fp32 [splits, M, N], out [M, N] contiguous; N a multiple of 8.  peak: that d is scaled by, or null.
+// d [M, V] (rows ld_d apart, a multiple of 8), w [V, N], parts: fp32 [splits, M, N] (one split: null), out [M, N] contiguous; N a multiple of 8.  peak: that d is scaled by, or
+// null.
 int rb_head_dhidden(const void* d, const void* w, int64_t ld_d, int64_t ld_w, const uint32_t* peak, float* parts, void* out, int M, int N, int V, int splits, int in_dt,
                     int num_sms, cudaStream_t s) {
   if (M <= 0) return 0;
@@ -756,17 +754,41 @@ int rb_head_dhidden(const void* d, const void* w, int64_t ld_d, int64_t ld_w, co
   if (!make_tmap(&tb, w, in_dt == 1, (uint64_t)V, (uint64_t)N, (uint64_t)ld_w, 64, BK)) return -13;
   HeadParams p{};
   p.M = M; p.N = N; p.K = V;
-  p.out = parts;
+  p.out = splits > 1 ? parts : out;
   p.splits = splits;
+  p.direct = splits == 1;
+  p.peak = peak;
   p.status = rb_attn_status();
   if (p.status == nullptr) return -14;
   const int rc = in_dt == 1 ? launch_head<__nv_bfloat16, 1, kHiddenGrad>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kHiddenGrad>(ta, tb, p, num_sms, s);
-  if (rc) return rc;
+  if (rc || splits == 1) return rc;
   const int64_t n = (int64_t)M * N;
   const unsigned blocks = (unsigned)RB_CEIL_DIV(n, 256 * 8);
   if (in_dt == 1) head_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(parts, peak, (__nv_bfloat16*)out, splits, n);
   else head_sum_kernel<__half><<<blocks, 256, 0, s>>>(parts, peak, (__half*)out, splits, n);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+// out [V, N] contiguous, of the operands' type or fp32 (out_dt 0), = or add: += d^T h over the scale of d; d [M, V] (rows ld_d apart), h [M, N], in fp16 (the general product takes
+// what has no scale)
+int rb_head_dweight(const void* d, const void* h, int64_t ld_d, int64_t ld_h, const uint32_t* peak, void* out, int M, int N, int V, int in_dt, int out_dt, int add, int num_sms,
+                    cudaStream_t s) {
+  if (M <= 0) return 0;
+  if (in_dt != 2 || (out_dt != 0 && out_dt != in_dt)) return -10;
+  if (N % 8 || ld_d % 8 || ld_h % 8 || ((reinterpret_cast<uintptr_t>(d) | reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(out)) & 15)) return -11;
+  CUtensorMap ta, tb;
+  if (!make_tmap(&ta, d, false, (uint64_t)M, (uint64_t)V, (uint64_t)ld_d, 64, BK)) return -13;
+  if (!make_tmap(&tb, h, false, (uint64_t)M, (uint64_t)N, (uint64_t)ld_h, 64, BK)) return -13;
+  HeadParams p{};
+  p.M = V; p.N = N; p.K = M;
+  p.out = out;
+  p.splits = 1;
+  p.direct = out_dt == 0 ? 2 : 1;
+  p.add = add;
+  p.peak = peak;
+  p.status = rb_attn_status();
+  if (p.status == nullptr) return -14;
+  return launch_head<__half, 0, kWeightGrad>(ta, tb, p, num_sms, s);
 }
 
 }  // extern "C"

@@ -638,10 +638,7 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of, peak=None):
     if needs[1]:
         own = bool(getattr(weight, "_main_grad_hooked", False)) and len(weight._post_accumulate_grad_hooks or ()) == 1
         buffer = _row_grad_buffer(weight) if G is not None and weight.is_leaf and lib().gradient_goes_past(weight, own) else None
-        if peak is not None:
-            buffer = buffer if buffer is not None and buffer.dtype in (torch.float32, weight.dtype) else None
-            dw = (torch.zeros if T > chunk or T == 0 else torch.empty)(weight.shape, dtype=torch.float32, device=weight.device)
-        elif buffer is not None and (buffer.dtype == torch.float32 or T <= chunk):
+        if buffer is not None and (buffer.dtype == torch.float32 or (buffer.dtype == weight.dtype and T <= chunk)):
             dw = buffer              # the products' fp32 sums are added to it; one of 16 bits would be rounded once a chunk
         elif G is None or T > chunk or T == 0:
             dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device)
@@ -654,8 +651,8 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of, peak=None):
             if dw is not None:
                 dw += d.float().t() @ hidden[s:e].float()
             continue
+        sms = G._sms(weight.device)
         if dh is not None:                                                                   # [t, V] x [V, H]
-            sms = G._sms(weight.device)
             splits = lib().head_dhidden_splits(e - s, weight.shape[1], weight.shape[0], sms)
             if splits > 1 or peak is not None:
                 lib().head_dhidden(d, weight, dh[s:e], splits, sms, peak)
@@ -663,14 +660,14 @@ def _head_backward(hidden, weight, needs, chunk: int, dlogits_of, peak=None):
                 G.gemm(d, weight, out=dh[s:e], b_mn=True)
         if needs[1]:
             h = G.tma_rows(hidden[s:e])
-            if dw is None:
+            if peak is not None:
+                whole = torch.empty_like(weight, memory_format=torch.contiguous_format) if dw is None else None
+                lib().head_dweight(d, h, whole if dw is None else dw, dw is not None, sms, peak)
+            elif dw is None:
                 whole = G.gemm(d, h, a_mn=True, b_mn=True)                                   # [t, V]^T x [t, H], rounded once
             else:
-                G.gemm(d, h, out=dw, a_mn=True, b_mn=True, accumulate=peak is None or T > chunk)
-    if peak is not None and dw is not None:
-        whole = None if buffer is not None else torch.empty_like(dw, dtype=weight.dtype)
-        lib().head_unscale(dw, peak, buffer if whole is None else whole, whole is None)
-    elif dw is not None and dw is not buffer:
+                G.gemm(d, h, out=dw, a_mn=True, b_mn=True, accumulate=True)
+    if dw is not None and dw is not buffer:
         whole = dw.to(weight.dtype)
     return dh, whole
 
