@@ -10,7 +10,7 @@
 // A negative id is an unused place; an id given again counts where it stands first; an id beyond the vocabulary makes the row's loss NaN.
 // p_b = 0 and q_b = 0 contribute 0.
 //
-// Bound by memory, one read forward and one read and write backward: 8192 x 32000 bf16 with 64 tokens 101 and 165 us (5.2 and 6.3 TB/s).  The forward pass leaves what a row's gradient
+// Bound by memory, one read forward and one read and write backward: 8192 x 32000 bf16 with 64 tokens 101 and 165 .. 170 us (5.2 and 6.2 TB/s).  The forward pass leaves what a row's gradient
 // needs beside its logits: the listed tokens' own gradients, the rest's and its log-sum-exp.
 #include "vocab_rows.cuh"
 
@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
   const int seg = blockIdx.x - (int)(row * segs);
   const T* lr = logits + row * row_stride;
   O* orow = out + row * out_stride;
-  const float g = g_loss[row] * inv_temp * (peak ? rb::grad_scale(*peak) : 1.f);
+  float g = g_loss[row] * inv_temp;
+  if constexpr (std::is_same_v<T, float> && std::is_same_v<O, __half>) g *= peak ? rb::grad_scale(*peak) : 1.f;
   const bool zero = g == 0.f;
   const int id0 = threadIdx.x < k ? ids[row * k + threadIdx.x] : -1;         // (asked for beside the logits, as the block ends with them)
   const float listed0 = threadIdx.x < k ? grad_listed[row * k + threadIdx.x] : 0.f;
@@ -260,7 +261,7 @@ int rb_distill_peak(const float* grad_rest, const float* grad_listed, const floa
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-// out: [rows, V] of type out_dt (dt, or a 16-bit one for fp32 logits), may be the logits themselves; peak: gradients leave times grad_scale of it, or null
+// out: [rows, V] of type out_dt (dt, or a 16-bit one for fp32 logits), may be the logits themselves; peak (fp32 logits, fp16 gradients): they leave times grad_scale of it, or null
 int rb_distill_bwd(const void* logits, int64_t row_stride, const float* lse_rest, const float* grad_rest, const float* grad_listed, const int* ids,
                    const float* g_loss, const uint32_t* peak, void* out, int64_t out_stride, int64_t rows, int V, int k, float inv_temp, int dt, int out_dt,
                    cudaStream_t s) {
@@ -271,6 +272,7 @@ int rb_distill_bwd(const void* logits, int64_t row_stride, const float* lse_rest
 #define RB_L(T, O)                                                                                                                                     \
   distill_bwd_kernel<T, O><<<(unsigned)(rows * segs), kBwdThreads, 0, s>>>((const T*)logits, row_stride, lse_rest, grad_rest, grad_listed, ids, g_loss, peak,  \
                                                                            (O*)out, out_stride, V, k, inv_temp, (int)segs)
+  if (peak && !(dt == 0 && out_dt == 2)) return -1;
   if (dt == 0 && out_dt == 0) RB_L(float, float);
   else if (dt == 0 && out_dt == 1) RB_L(float, __nv_bfloat16);
   else if (dt == 0 && out_dt == 2) RB_L(float, __half);

@@ -12,7 +12,8 @@
 // where their sum is whole: with row gradients of 1 / T nearly all of them lie below fp16's smallest number.
 // d h with few tiles: the sum over the vocabulary in parts, fp32 tiles that a second kernel adds up in order (16 rows of 4096 x 32000: 167 us undivided).
 // An epilogue takes 32768 exponentials a CTA, 2048 cycles at least, beside 8 H cycles of products.
-// 8192 x 4096 x 32000 bf16, us: forward 1320 .. 1350 (the plain product 1320 .. 1400), d logits 206 from kept weights, 1380 from the product.
+// 8192 x 4096 x 32000 bf16, us: forward 1320 .. 1350 (the plain product 1320 .. 1400), d logits 206 from kept weights, 1380 from the product.  fp16: d weight 1570 (the general
+// product 1563), d hidden 1514 (1520); the bound of d logits 5 us for 2048 rows.
 #include "attn_common.cuh"
 #include "cta_pair.cuh"
 #include "vocab_rows.cuh"
@@ -30,7 +31,6 @@ constexpr int kHeadBand = 8;                                // row tiles walked 
 
 struct HeadParams {
   int M, N, K;
-  int rounded;          // logits are rounded to the operands' type, as a product that stores them leaves them
   float inv_temp;
   const int64_t* labels;
   const uint8_t* mask;
@@ -39,7 +39,7 @@ struct HeadParams {
   float *part_m, *part_s, *part_w, *target;
   // backward
   const float *lse, *entropy, *g_logp, *g_entropy;
-  const uint32_t* peak; // d logits leave times grad_scale of it; null: as they are
+  const uint32_t* peak; // fp16: d logits leave times grad_scale of it; null: as they are
   void* out;
   int64_t ld_out;
   int splits;           // d hidden: parts of the sum over the vocabulary, out fp32 [splits, M, N]
@@ -101,7 +101,8 @@ template <typename T> RB_DEVICE void store_cols(uint32_t, const float (&)[32], T
 enum HeadMode { kStats, kStatsKeep, kLogitGrad, kHiddenGrad, kWeightGrad };
 constexpr float kKeepScale = 32768.f;
 
-template <typename T, int kFmt, HeadMode kMode>
+// kRound: logits are rounded to the operands' type, as a product that stores them leaves them (a variant of its own: asked at run time, it cost every narrow head 3 %)
+template <typename T, int kFmt, HeadMode kMode, bool kRound = false>
 __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                                                                  const HeadParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -239,8 +240,8 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
         if (p.g_logp && given >= 0) gl = p.g_logp[row] * p.inv_temp;
         if (p.g_entropy) ge = p.g_entropy[row] * p.inv_temp;
         if (gl != 0.f && given >= p.N) gl = NAN;
-        if (p.peak) {
-          const float up = rb::grad_scale(*p.peak);
+        if constexpr (std::is_same_v<T, __half>) {
+          const float up = p.peak ? rb::grad_scale(*p.peak) : 1.f;
           gl *= up;
           ge *= up;
         }
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < 32; ++i) m = rb::max_nan(m, __uint_as_float(r[i]));
         }
-        if (p.rounded) {
+        if (kRound) {
           float same = m;
           round_pair<T>(m, same);
         }
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kHeadThreads, 1) head_stats_kernel(const __gri
         float x[kCols];
 #pragma unroll
         for (int i = 0; i < kCols; ++i) x[i] = __uint_as_float(r[i]);
-        if (!kSplit && p.rounded) {
+        if (kRound) {
 #pragma unroll
           for (int i = 0; i < kCols; i += 2) round_pair<T>(x[i], x[i + 1]);
         }
@@ -499,8 +500,8 @@ __global__ void __launch_bounds__(kGradThreads) head_grad_kernel(const __half* _
   float ge = p.g_entropy ? p.g_entropy[whole] * p.inv_temp : 0.f;
   float gl = p.g_logp && given >= 0 ? p.g_logp[whole] * p.inv_temp : 0.f;
   if (gl != 0.f && given >= p.N) gl = NAN;
-  if (p.peak) {
-    const float up = rb::grad_scale(*p.peak);
+  if constexpr (std::is_same_v<T, __half>) {
+    const float up = p.peak ? rb::grad_scale(*p.peak) : 1.f;
     gl *= up;
     ge *= up;
   }
@@ -614,8 +615,8 @@ template <typename T> __global__ void __launch_bounds__(256) head_sum_kernel(con
   *reinterpret_cast<rb::Pack<T, 8>*>(out + i) = o;
 }
 
-template <typename T, int kFmt, HeadMode kMode> int launch_head(const CUtensorMap& ta, const CUtensorMap& tb, const HeadParams& p, int num_sms, cudaStream_t s) {
-  auto kern = head_stats_kernel<T, kFmt, kMode>;
+template <typename T, int kFmt, HeadMode kMode, bool kRound = false> int launch_head(const CUtensorMap& ta, const CUtensorMap& tb, const HeadParams& p, int num_sms, cudaStream_t s) {
+  auto kern = head_stats_kernel<T, kFmt, kMode, kRound>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeadSmem) != cudaSuccess) return -2;
   const int tiles = RB_CEIL_DIV(p.M, 2 * BM) * RB_CEIL_DIV(p.N, HN) * (kMode == kHiddenGrad ? p.splits : 1), pairs = num_sms / 2;
   cudaLaunchConfig_t cfg{};
@@ -632,6 +633,13 @@ template <typename T, int kFmt, HeadMode kMode> int launch_head(const CUtensorMa
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, kern, ta, tb, p) != cudaSuccess) return -3;
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+// bf16 or fp16, logits as they are or rounded
+template <HeadMode kMode> int launch_logits(const CUtensorMap& ta, const CUtensorMap& tb, const HeadParams& p, int in_dt, bool rounded, int num_sms, cudaStream_t s) {
+  if (in_dt == 1)
+    return rounded ? launch_head<__nv_bfloat16, 1, kMode, true>(ta, tb, p, num_sms, s) : launch_head<__nv_bfloat16, 1, kMode>(ta, tb, p, num_sms, s);
+  return rounded ? launch_head<__half, 0, kMode, true>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kMode>(ta, tb, p, num_sms, s);
 }
 
 int head_maps(const void* h, const void* w, int64_t ld_h, int64_t ld_w, int M, int N, int K, int in_dt, CUtensorMap& ta, CUtensorMap& tb) {
@@ -660,7 +668,6 @@ int rb_head_stats(const void* h, const void* w, int64_t ld_h, int64_t ld_w, cons
   const int tiles_n = RB_CEIL_DIV(N, HN);
   HeadParams p{};
   p.M = M; p.N = N; p.K = K;
-  p.rounded = rounded;
   p.inv_temp = inv_temp;
   p.labels = labels; p.mask = mask; p.mask_stride = mask_stride;
   p.part_m = scratch;
@@ -672,8 +679,7 @@ int rb_head_stats(const void* h, const void* w, int64_t ld_h, int64_t ld_w, cons
   if (kept && (ld_kept % 8 || (reinterpret_cast<uintptr_t>(kept) & 15))) return -12;
   p.out = kept;
   p.ld_out = ld_kept;
-  const int rc = kept ? (in_dt == 1 ? launch_head<__nv_bfloat16, 1, kStatsKeep>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kStatsKeep>(ta, tb, p, num_sms, s))
-                      : (in_dt == 1 ? launch_head<__nv_bfloat16, 1, kStats>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kStats>(ta, tb, p, num_sms, s));
+  const int rc = kept ? launch_logits<kStatsKeep>(ta, tb, p, in_dt, rounded, num_sms, s) : launch_logits<kStats>(ta, tb, p, in_dt, rounded, num_sms, s);
   if (rc) return rc;
   head_merge_kernel<<<RB_CEIL_DIV(M, kMergeRows), kMergeRows * kMergeSlices, 0, s>>>(p, 2 * tiles_n, logp, entropy, lse);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
@@ -691,19 +697,19 @@ int rb_head_stats_bwd(const void* h, const void* w, int64_t ld_h, int64_t ld_w, 
                       const float* entropy, const float* g_logp, const float* g_entropy, const uint32_t* peak, void* out, int64_t ld_out, int M, int N, int K, float inv_temp,
                       int rounded, int in_dt, int num_sms, cudaStream_t s) {
   if (M <= 0) return 0;
+  if (peak && in_dt != 2) return -10;
   if (ld_out % 8 || (reinterpret_cast<uintptr_t>(out) & 15)) return -12;
   CUtensorMap ta, tb;
   if (const int rc = head_maps(h, w, ld_h, ld_w, M, N, K, in_dt, ta, tb)) return rc;
   HeadParams p{};
   p.M = M; p.N = N; p.K = K;
-  p.rounded = rounded;
   p.inv_temp = inv_temp;
   p.labels = labels; p.mask = mask; p.mask_stride = mask_stride;
   p.lse = lse; p.entropy = entropy; p.g_logp = g_logp; p.g_entropy = g_entropy; p.peak = peak;
   p.out = out; p.ld_out = ld_out;
   p.status = rb_attn_status();
   if (p.status == nullptr) return -14;
-  return in_dt == 1 ? launch_head<__nv_bfloat16, 1, kLogitGrad>(ta, tb, p, num_sms, s) : launch_head<__half, 0, kLogitGrad>(ta, tb, p, num_sms, s);
+  return launch_logits<kLogitGrad>(ta, tb, p, in_dt, rounded, num_sms, s);
 }
 
 // d logits [rows, N] of rows row0 .. of a forward pass over all_rows rows, from what it kept (`kept`: these rows; part_m, labels, mask and values a row: all rows); out as above
@@ -711,6 +717,7 @@ int rb_head_grad(const void* kept, int64_t ld_kept, const float* part_m, const i
                  const float* entropy, const float* g_logp, const float* g_entropy, const uint32_t* peak, void* out, int64_t ld_out, int row0, int rows, int all_rows, int N,
                  float inv_temp, int dt, cudaStream_t s) {
   if (rows <= 0) return 0;
+  if (peak && dt != 2) return -10;
   if (ld_out % 8 || ld_kept % 8 || ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(kept)) & 15) || row0 < 0 || row0 + rows > all_rows) return -12;
   HeadParams p{};
   p.M = rows; p.N = N;

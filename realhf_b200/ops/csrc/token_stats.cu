@@ -4,7 +4,7 @@
 // Backward, with y = x inv_temp - lse and p = e^y:   dx_j = inv_temp (g_logp (1[j = label] - p_j) - g_entropy p_j (y_j + H))
 // element by element, in segments of a row.
 //
-// Both are bound by memory: 8192 x 32000 bf16 forward 95 us (5.5 TB/s: the ends of rows of 64 KB), 8192 x 131072 340 (6.3); backward 156 and 636 (6.7 TB/s) with all loads of a
+// Both are bound by memory: 8192 x 32000 bf16 forward 95 us (5.5 TB/s: the ends of rows of 64 KB), 8192 x 131072 340 (6.3); backward 156 .. 160 and 636 .. 650 (6.6 TB/s) with all loads of a
 // thread ahead of the first use, streaming stores and f32x2 arithmetic (189 and 721 with a piece after the other).
 #include "vocab_rows.cuh"
 

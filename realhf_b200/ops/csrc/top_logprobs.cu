@@ -21,7 +21,7 @@
 //
 // A row of equal logits: 4096 x 32000 in 457 us, 896 before the descent left the digits out that a 16-bit type does not have.
 //
-// bf16, us: 8192 x 32000 with 20 / 64 / 256 alternatives 130 / 150 / 207, 4096 x 131072 with 64 212 (5.1 TB/s); the statistics alone take 95 and 170.  Bound by issue slots (66 %):
+// bf16, us: 8192 x 32000 with 20 / 64 / 256 alternatives 130 / 146 / 205, 4096 x 131072 with 64 212 .. 224 (4.8 .. 5.1 TB/s); the statistics alone take 95 and 170 .. 185.  Bound by issue slots (66 %):
 // ten instructions a logit, a fifth of them for bound, candidates and order.
 #include "vocab_rows.cuh"
 
