@@ -145,12 +145,13 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
   const int seg = blockIdx.x - (int)(row * segs);
   const T* lr = logits + row * row_stride;
   O* orow = out + row * out_stride;
-  float g = g_loss[row] * inv_temp;
-  if constexpr (std::is_same_v<T, float> && std::is_same_v<O, __half>) g *= peak ? rb::grad_scale(*peak) : 1.f;
+  const float g = g_loss[row] * inv_temp;
+  float up = 1.f;                                       // (of products with g, which the peak bounds: g times it may leave fp32)
+  if constexpr (std::is_same_v<T, float> && std::is_same_v<O, __half>) up = peak ? rb::grad_scale(*peak) : 1.f;
   const bool zero = g == 0.f;
   const int id0 = threadIdx.x < k ? ids[row * k + threadIdx.x] : -1;         // (asked for beside the logits, as the block ends with them)
   const float listed0 = threadIdx.x < k ? grad_listed[row * k + threadIdx.x] : 0.f;
-  const float a = zero ? 0.f : g * grad_rest[row], lr_rest = lse_rest_in[row];
+  const float a = zero ? 0.f : g * grad_rest[row] * up, lr_rest = lse_rest_in[row];
   const float ref = lr_rest == -INFINITY ? 0.f : lr_rest;
   auto grad = [&](float x) {
     const float e = rb::exp2_fast(fmaf(x, inv_temp, -ref) * rb::kLog2e);
@@ -204,10 +205,10 @@ __global__ void __launch_bounds__(kBwdThreads) distill_bwd_kernel(const T* logit
     for (int j = lo + threadIdx.x; j < hi; j += kBwdThreads) orow[j] = rb::from_f<O>(grad(rb::to_f(lr[j])));
   }
   __syncthreads();                                      // the listed tokens over what was just written
-  if (id0 >= lo && id0 < hi) orow[id0] = rb::from_f<O>(zero ? 0.f : g * listed0);
+  if (id0 >= lo && id0 < hi) orow[id0] = rb::from_f<O>(zero ? 0.f : g * listed0 * up);
   for (int i = threadIdx.x + kBwdThreads; i < k; i += kBwdThreads) {
     const int id = ids[row * k + i];
-    if (id >= lo && id < hi) orow[id] = rb::from_f<O>(zero ? 0.f : g * grad_listed[row * k + i]);
+    if (id >= lo && id < hi) orow[id] = rb::from_f<O>(zero ? 0.f : g * grad_listed[row * k + i] * up);
   }
 }
 

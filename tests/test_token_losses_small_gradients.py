@@ -242,3 +242,20 @@ def test_head_gradients_captured_gpu():
         graph.replay()
         for a, b in zip(out, work()):
             assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("keep_bytes", [0, 1 << 31])
+def test_head_distillation_gradients_that_are_next_to_nothing_gpu(keep_bytes):
+    """A student that has learnt its teacher: every gradient below 1e-33 of an incoming one of 100, for which the scale of d logits is the largest there is."""
+    T, H, V = 3, 64, 40
+    w = torch.zeros(V, H, dtype=torch.float16)
+    w[0, :] = 1.0
+    h = torch.full((T, H), 85.0 / 64, dtype=torch.float16)           # logits 85 and 0: the others hold e^-85 = 1e-37 of the mass each
+    hd, wd = h.cuda().requires_grad_(True), torch.nn.Parameter(w.cuda())
+    wd.main_grad = torch.zeros(V, H, device="cuda")
+    ids, t, tr = torch.zeros(T, 1, dtype=torch.long, device="cuda"), torch.zeros(T, 1, device="cuda"), torch.full((T,), -INF, device="cuda")
+    loss = OF.lm_head_distill_loss(hd, wd, ids, t, tr, keep_bytes=keep_bytes)
+    loss.backward(torch.full((T,), 100.0, device="cuda"))
+    assert loss.abs().max() < 1e-30 and not hd.grad.any()
+    assert wd.main_grad.isfinite().all() and wd.main_grad.abs().max() < 1e-30
