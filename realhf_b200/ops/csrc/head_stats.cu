@@ -12,7 +12,7 @@
 // where their sum is whole: with row gradients of 1 / T nearly all of them lie below fp16's smallest number.
 // d h with few tiles: the sum over the vocabulary in parts, fp32 tiles that a second kernel adds up in order (16 rows of 4096 x 32000: 167 us undivided).
 // An epilogue takes 32768 exponentials a CTA, 2048 cycles at least, beside 8 H cycles of products.
-// 8192 x 4096 x 32000 bf16, us: forward 1320 .. 1350 (the plain product 1320 .. 1400), d logits 206 from kept weights, 1380 from the product.  fp16: d weight 1570 (the general
+// 8192 x 4096 x 32000 bf16, us: forward 1320 .. 1350 (the plain product 1320 .. 1400), 1390 .. 1405 with kept weights, d logits 181 .. 206 from them, 1370 .. 1385 from the product.  fp16: d weight 1570 (the general
 // product 1563), d hidden 1514 (1520); the bound of d logits 5 us for 2048 rows.
 #include "attn_common.cuh"
 #include "cta_pair.cuh"
