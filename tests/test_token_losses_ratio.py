@@ -116,3 +116,37 @@ def test_rounded_statistics_beside_a_gradient_buffer_gpu():
         results.append((logp.detach(), ent.detach(), a.grad, (b.main_grad if own else b.grad).bfloat16()))
     for x, y in zip(*results):
         assert torch.equal(x, y)
+
+
+def check_capped(dev, dtype, softcap, scale):
+    """A capped or scaled head: both calls have the same log-probability, the cap's tanh apart (8 u of it)."""
+    h, w, labels = make_head(21, 64, 304, dtype, 2, dev)
+    out = ModelOutput(hidden=h, head_weight=w, ctx=None, softcap=softcap, logit_scale=scale)
+    with torch.no_grad():
+        old = out.logprobs(labels, None, 0.9)
+    logp, _ = out.logprobs_entropy(labels, None, 0.9, rounded=True)
+    z = out.logits.double() / 0.9
+    assert ((logp.double() - old.double()).abs() <= 4 * err(z, 304) + 32 * U * float(z.abs().max())).all()
+
+
+@pytest.mark.parametrize("softcap,scale", [(20.0, None), (20.0, 0.5), (None, 0.5)])
+def test_capped_and_scaled_heads_cpu(softcap, scale):
+    check_capped("cpu", torch.bfloat16, softcap, scale)
+
+
+def _sharded_logprobs(rank, world):
+    from realhf_b200.base.topology import ParallelContext, ProcessTopology
+    ctx = ParallelContext.build(ProcessTopology(1, 1, world), list(range(world)), rank, backend="gloo")
+    h, w, labels = make_head(9, 32, 64, torch.bfloat16, 2)
+    per = 64 // world
+    out = ModelOutput(hidden=h, head_weight=w[rank * per: (rank + 1) * per].clone(), ctx=ctx)
+    return out.logprobs(labels, None, 0.9).tolist(), out.logprobs_entropy(labels, None, 0.9, rounded=True)[0].tolist()
+
+
+@pytest.mark.distributed
+def test_sharded_head_cpu():
+    from realhf_b200.base.testing import run_distributed
+    h, w, _ = make_head(9, 32, 64, torch.bfloat16, 2)
+    z = h.double() @ w.double().t() / 0.9
+    for old, new in run_distributed(_sharded_logprobs, 2):
+        assert ((torch.tensor(old, dtype=torch.float64) - torch.tensor(new, dtype=torch.float64)).abs() <= 4 * err(z, 64)).all()
