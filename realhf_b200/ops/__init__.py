@@ -20,10 +20,10 @@ _host = None
 
 
 # kernels launched per op call (for the `gpu_launches` accounting of bench.py); the embedding's gradient, which a native backward pass launches without a call from
-# here, is counted by the library (`native_launches`)
+# here, is counted by the library (`native_launches`), and so are the products of the head's gradient, one kernel or two
 _KERNELS_PER_OP = {"rmsnorm_bwd": 2, "embedding_grad_": 0, "embedding_grad_tokens": 0, "gradient_goes_past": 0, "check_capture": 0, "adamw_step": 1, "decode_attention": 1, "attn_check": 0,
                    "attn_status": 0, "attn_wait_error": 0, "head_stats": 2,
-                   "head_dhidden": 2, "head_dhidden_splits": 0, "head_logprob_entropy": 2}
+                   "head_dhidden": 0, "head_dhidden_splits": 0, "head_logprob_entropy": 2}
 
 
 class _LaunchCounter:

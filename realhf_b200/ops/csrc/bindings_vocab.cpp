@@ -17,7 +17,7 @@ bool gradient_goes_past(const Tensor& leaf, bool own_hook);      // bindings.cpp
 void check_capture(const Tensor& leaf, c10::string_view op);     // bindings.cpp
 void attn_check();      // bindings_attn.cpp: an error once a bounded wait of an earlier kernel has run out
 
-// kernels launched where Python does not see the call (in a native backward pass), since the last question
+// kernels launched where Python does not see them (in a native backward pass, or one or two of them in a call), since the last question
 static std::atomic<int64_t> unseen_launches{0};
 
 extern "C" {
@@ -412,6 +412,7 @@ void head_dhidden(const Tensor& d, const Tensor& w, Tensor out, int64_t splits, 
   const int rc = rb_head_dhidden(d.data_ptr(), w.data_ptr(), d.stride(0), w.stride(0), peak_of(peak, d, op), parts.data_ptr<float>(), out.data_ptr(), (int)d.size(0),
                                  (int)w.size(1), (int)d.size(1), (int)splits, dtype_code(d), (int)num_sms, stream());
   TORCH_CHECK(rc == 0, op, " failed with code ", rc);
+  unseen_launches += splits > 1 ? 2 : 1;
 }
 
 // out [vocabulary, H], of the operands' type or fp32, = or with `add` += d^T x h, fp16, taken back from the scale of d

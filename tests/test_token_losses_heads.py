@@ -41,3 +41,20 @@ def test_head_alternatives_gpu(T, H, V, k, chunk, masked, temp, dtype):
     assert ((o.entropy.double() - H64).abs() <= 4 * e[:, 0] * (1 + H64) + U).all()
     want = y.gather(1, labels[:, None])[:, 0]
     assert ((o.logp.double() - want).abs() <= 2 * e[:, 0] + U * want.abs()).all()
+
+
+@gpu
+def test_kernels_of_d_hidden_are_counted_gpu():
+    from realhf_b200.ops import launches, lib
+    d, w = torch.randn(64, 2048, dtype=torch.float16, device="cuda"), torch.randn(2048, 256, dtype=torch.float16, device="cuda")
+    out = torch.empty(64, 256, dtype=torch.float16, device="cuda")
+    results = []
+    for splits, kernels in ((1, 1), (4, 2)):      # (parts are added up by a second kernel)
+        before = launches.total
+        lib().head_dhidden(d, w, out, splits, 148)
+        assert launches.total - before == kernels
+        results.append(out.double())
+    want = d.double() @ w.double()
+    size = d.double().abs() @ w.double().abs()
+    for got in results:       # the accumulator cuts off once for 16 terms, at most 2^-22 of their sizes' sum; the result is rounded once
+        assert ((got - want).abs() <= size * (2048 / 16 + 4) * 2.0 ** -22 + 2.0 ** -11 * want.abs() + 2.0 ** -25).all()
