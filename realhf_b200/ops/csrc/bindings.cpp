@@ -417,6 +417,7 @@ void register_seq_ops(torch::Library& m);      // bindings_seq.cpp
 void register_state_ops(torch::Library& m);    // bindings_state.cpp
 void register_mix_ops(torch::Library& m);      // bindings_mix.cpp
 void register_vocab_ops(torch::Library& m);    // bindings_vocab.cpp
+void register_int4_ops(torch::Library& m);     // bindings_int4.cpp
 
 static int64_t set_pdl(int64_t on) { const int old = rb_get_pdl(); if (on >= 0) rb_set_pdl((int)on); return old; }
 
@@ -451,4 +452,5 @@ TORCH_LIBRARY(realhf_b200, m) {
   register_state_ops(m);
   register_mix_ops(m);
   register_vocab_ops(m);
+  register_int4_ops(m);
 }

@@ -1,0 +1,98 @@
+// Keys and values of packed sequences into a 4-bit cache, and back (layout and rule: int4.cuh).
+//
+// One block per (tile of a sequence, head).  Read or write of the 16-bit side: 16 bytes a lane, a head's row by 8 or 16 lanes.
+#include "int4.cuh"
+
+#include <algorithm>
+
+namespace {
+
+constexpr int kThreads = 128;
+
+struct CacheParams {
+  void *k, *v;                      // [T, nkv, D], element (t, h, c) at t * ts + h * hs + c
+  int64_t kt, kh, vt, vh;
+  uint32_t* cache;                  // [slots, nkv, tiles, Tile<D>::kWords]
+  const int *cu, *slots, *start;    // [n + 1], [n] or null (sequence i: slot i), [n] or null (from row 0)
+  int n, nkv, n_slots, room, tiles, T;
+};
+
+template <typename T, int D, bool kStore>
+__global__ void __launch_bounds__(kThreads) cache_rows_kernel(CacheParams p) {
+  using Tl = q4::Tile<D>;
+  constexpr int LPR = D / 8, kGroups = kThreads / LPR;
+  rb::pdl_trigger();
+  rb::pdl_wait();
+  const int seq = blockIdx.x, head = blockIdx.y, sub = threadIdx.x % LPR;
+  const int tok0 = min(max(p.cu[seq], 0), p.T), tok1 = min(max(p.cu[seq + 1], tok0), p.T);
+  const int slot = p.slots ? p.slots[seq] : seq;
+  const int64_t start = p.start ? p.start[seq] : 0;
+  const bool there = slot >= 0 && slot < p.n_slots;
+  if (kStore && !there) return;
+  const int64_t first = (start < 0 ? start - 15 : start) / 16, last = start + (tok1 - tok0);   // tiles first .. ; rows below `last`
+  for (int64_t tile = first + blockIdx.z; tile * 16 < last; tile += gridDim.z) {
+    uint32_t* at = p.cache + (((int64_t)slot * p.nkv + head) * p.tiles + tile) * Tl::kWords;
+#pragma unroll 1
+    for (int r = threadIdx.x / LPR; r < 16; r += kGroups) {      // (a warp's lanes take the same turns)
+      const int64_t row = tile * 16 + r, tok = tok0 + (row - start);
+      const bool mine = row >= start && row < last, held = there && row >= 0 && row < p.room;
+      float x[8];
+      if constexpr (kStore) {
+        rb::Pack<T, 8> a{}, b{};
+        if (mine && held) {
+          a = *reinterpret_cast<const rb::Pack<T, 8>*>(reinterpret_cast<const T*>(p.k) + tok * p.kt + head * p.kh + sub * 8);
+          b = *reinterpret_cast<const rb::Pack<T, 8>*>(reinterpret_cast<const T*>(p.v) + tok * p.vt + head * p.vh + sub * 8);
+        }
+        float lo, hi;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = rb::to_f(a.v[i]);
+        q4::extremes<4>(x, lo, hi);
+        const uint32_t kg = q4::group_word<T>(lo, hi), kw = q4::pack8(x, q4::scale_of<T>(kg), lo);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = rb::to_f(b.v[i]);
+        q4::extremes<8>(x, lo, hi);
+        const uint32_t vg = q4::group_word<T>(lo, hi), vw = q4::pack8(x, q4::scale_of<T>(vg), lo);
+        if (mine && held) {
+          at[r * Tl::W + q4::word_place<Tl::J>(sub)] = kw;
+          at[Tl::kValues + sub * 16 + q4::place_of(r)] = vw;
+          if (sub % 4 == 0) at[Tl::kKeyScales + r * Tl::J + sub / 4] = kg;
+          if (sub % 8 == 0) at[Tl::kValueScales + r * Tl::H + sub / 8] = vg;
+        }
+      } else if (mine) {
+        rb::Pack<T, 8> a{}, b{};
+        if (held) {
+          const uint32_t kg = at[Tl::kKeyScales + r * Tl::J + sub / 4], vg = at[Tl::kValueScales + r * Tl::H + sub / 8];
+          q4::unpack8(at[r * Tl::W + q4::word_place<Tl::J>(sub)], q4::scale_of<T>(kg), q4::low_of<T>(kg), x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a.v[i] = rb::from_f<T>(x[i]);
+          q4::unpack8(at[Tl::kValues + sub * 16 + q4::place_of(r)], q4::scale_of<T>(vg), q4::low_of<T>(vg), x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b.v[i] = rb::from_f<T>(x[i]);
+        }
+        *reinterpret_cast<rb::Pack<T, 8>*>(reinterpret_cast<T*>(p.k) + tok * p.kt + head * p.kh + sub * 8) = a;
+        *reinterpret_cast<rb::Pack<T, 8>*>(reinterpret_cast<T*>(p.v) + tok * p.vt + head * p.vh + sub * 8) = b;
+      }
+    }
+  }
+}
+
+template <typename T, int D> int launch(const CacheParams& p, int store, int blocks, cudaStream_t s) {
+  const dim3 grid(p.n, p.nkv, blocks);
+  return (store ? rb::launch_pdl(cache_rows_kernel<T, D, true>, grid, dim3(kThreads), 0, s, p)
+                : rb::launch_pdl(cache_rows_kernel<T, D, false>, grid, dim3(kThreads), 0, s, p)) == cudaSuccess ? 0 : -3;
+}
+
+}  // namespace
+
+// `longest`: about the length of the longest sequence (how many blocks a sequence gets; any value is right).  dt: 1 bf16, 2 fp16.
+extern "C" int rb_int4_cache_rows(void* k, void* v, int64_t kt, int64_t kh, int64_t vt, int64_t vh, void* cache, const int* cu, const int* slots,
+                                  const int* start, int n, int nkv, int hd, int n_slots, int room, int T, int longest, int store, int dt, cudaStream_t s) {
+  if (n == 0 || nkv == 0 || T == 0) return 0;
+  const CacheParams p{k, v, kt, kh, vt, vh, reinterpret_cast<uint32_t*>(cache), cu, slots, start, n, nkv, n_slots, room, (room + 15) / 16, T};
+  const int blocks = (int)std::min<int64_t>((std::max<int64_t>(longest, 1) + 15) / 16 + (start != nullptr), 65535);
+  if (dt == 1 && hd == 128) return launch<__nv_bfloat16, 128>(p, store, blocks, s);
+  if (dt == 1 && hd == 64) return launch<__nv_bfloat16, 64>(p, store, blocks, s);
+  if (dt == 2 && hd == 128) return launch<__half, 128>(p, store, blocks, s);
+  if (dt == 2 && hd == 64) return launch<__half, 64>(p, store, blocks, s);
+  return -2;
+}

@@ -1,0 +1,359 @@
+"""Generation with keys, values and weights held in 4 bits.
+
+A group of numbers is held as codes 0 .. 15 with the group's lowest value and a step, both of the model's 16-bit type T:
+
+    low = min x,   scale = T((max x - low) / 15),   code = min(15, round_half_even((x - low) / scale))  (0 where scale is 0),   x ~ scale * code + low
+
+so a value is off by at most half a step (and 15 roundings of the step).  A group that holds an infinity or a NaN reads back as NaN.
+
+* `Int4KVCache`: a dense cache [slots, room, n_kv, hd] with groups of 32 channels of a key (after the rotation a few channels are far larger than the
+  others, and a small group keeps them to themselves) and of 64 channels of a value: 4.75 bits a number, 3.4 times less than 16.  `store` quantises the
+  keys and values of packed sequences, `load` reads them back, `decode_attention_int4` appends a token and attends to all rows as the cache holds them.
+* `Int4Linear`: a weight [N, K] with groups of 32, 64 or 128 along K and its products with rows of any number; made for the few rows of a decode step,
+  where the weights' bytes are the time.
+
+The layout in memory is `csrc/int4.cuh`'s; `Int4KVCache.store`, `.load`, `decode_attention_int4` and `Int4Linear` on CPU tensors are plain PyTorch over the
+same layout.  The reference generates in the training dtype only (`realhf/impl/model/nn/real_llm_generate.py`); both are opt-in
+(`GenerationHyperparameters.kv_cache_bits`, `.int4_weights`), since what is sampled then is the quantised policy's.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from realhf_b200.ops import lib, use_native
+
+KEY_GROUP, VALUE_GROUP, TILE_ROWS = 32, 64, 16
+HEAD_DIMS = (64, 128)
+GROUPS = (32, 64, 128)
+_SHIFT = [4 * (i >> 1) + 16 * (i & 1) for i in range(8)]   # where channel i of a word's eight has its bits
+
+
+# ------------------------------------------------------------------------------------------------ groups
+
+
+def quantize_groups(x: torch.Tensor, group: int, dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """x [..., n] of a 16-bit type (or of fp32, with the type of the steps in `dtype`) -> (codes uint8 [..., n], scale [..., n / group], low): the rule in plain
+    PyTorch."""
+    dtype = dtype or x.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"4-bit groups: steps are bfloat16 or float16, not {dtype}")
+    if group <= 0 or x.shape[-1] % group:
+        raise ValueError(f"4-bit groups: {x.shape[-1]} numbers in groups of {group}")
+    xg = x.to(dtype).float().unflatten(-1, (-1, group))
+    lo, hi = xg.amin(-1), xg.amax(-1)
+    # (by 1/16, an exact factor: the widest group of bfloat16 stays inside fp32; a tensor by a tensor is a correctly rounded division)
+    scale = ((hi * 0.0625 - lo * 0.0625) / torch.full_like(lo, 0.9375)).to(dtype)
+    fine = torch.isfinite(lo) & torch.isfinite(hi)
+    scale = torch.where(fine, scale, torch.full_like(scale, float("nan")))
+    low = torch.where(fine, lo, torch.full_like(lo, float("nan"))).to(dtype)
+    step = scale.float()[..., None]
+    c = (xg * 0.0625 - lo[..., None] * 0.0625) / torch.where(step > 0, step * 0.0625, torch.ones_like(step))
+    c = torch.where(step > 0, c.round().clamp(max=15), torch.zeros_like(c))
+    return c.to(torch.uint8).flatten(-2), scale, low
+
+
+def dequantize_groups(codes: torch.Tensor, scale: torch.Tensor, low: torch.Tensor) -> torch.Tensor:
+    """fp32 scale * code + low, rounded once."""
+    xg = codes.unflatten(-1, (scale.shape[-1], -1)).double()
+    return (xg * scale.double()[..., None] + low.double()[..., None]).float().flatten(-2)
+
+
+def _words(codes: torch.Tensor) -> torch.Tensor:
+    """uint8 [..., 8 n] -> int32 [..., n], channels in order."""
+    sh = torch.tensor(_SHIFT, dtype=torch.int64, device=codes.device)
+    w = (codes.unflatten(-1, (-1, 8)).long() << sh).sum(-1)
+    return torch.where(w >= 1 << 31, w - (1 << 32), w).int()
+
+
+def _codes(words: torch.Tensor) -> torch.Tensor:
+    sh = torch.tensor(_SHIFT, dtype=torch.int32, device=words.device)
+    return ((words[..., None] >> sh) & 15).to(torch.uint8).flatten(-2)
+
+
+def _group_words(scale: torch.Tensor, low: torch.Tensor) -> torch.Tensor:
+    return (scale.view(torch.int16).int() << 16) | (low.view(torch.int16).int() & 0xFFFF)
+
+
+def _group_numbers(words: torch.Tensor, dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    low = words & 0xFFFF
+    return (words >> 16).to(torch.int16).view(dtype), torch.where(low >= 1 << 15, low - (1 << 16), low).to(torch.int16).view(dtype)
+
+
+def _row_order(words: torch.Tensor) -> torch.Tensor:
+    """[..., 4 J] words of a row in the order of the channels -> the order in memory, (t, j) with word 4 j + t."""
+    return words.unflatten(-1, (-1, 4)).transpose(-1, -2).flatten(-2)
+
+
+def _channel_order(words: torch.Tensor) -> torch.Tensor:
+    return words.unflatten(-1, (4, -1)).transpose(-1, -2).flatten(-2)
+
+
+def _on16(x: torch.Tensor) -> torch.Tensor:
+    """x itself if its rows lie on 16 bytes with unit inner stride, else a packed copy (not `contiguous()`: a slice of one row counts as that wherever it starts)."""
+    if x.numel() and (x.stride(-1) != 1 or any(s % 8 for s in x.stride()[:-1]) or x.data_ptr() % 16):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+# ------------------------------------------------------------------------------------------------ cache
+
+
+class Int4KVCache:
+    """Keys and values of `slots` sequences of up to `room` tokens, in 4 bits.  `dtype`: the model's type."""
+
+    __slots__ = ("data", "slots", "room", "n_kv", "hd", "dtype")
+
+    def __init__(self, slots: int, room: int, n_kv: int, hd: int, dtype=torch.bfloat16, device="cuda"):
+        if hd not in HEAD_DIMS:
+            raise ValueError(f"Int4KVCache: heads of 64 or 128 channels, not {hd}")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"Int4KVCache: bfloat16 or float16, not {dtype}")
+        if slots < 0 or room < 0 or n_kv <= 0:
+            raise ValueError(f"Int4KVCache: {slots} slots of {room} tokens, {n_kv} heads")
+        self.slots, self.room, self.n_kv, self.hd, self.dtype = int(slots), int(room), int(n_kv), int(hd), dtype
+        words = TILE_ROWS * (hd // 4 + hd // KEY_GROUP + hd // VALUE_GROUP)
+        self.data = torch.zeros(slots, n_kv, -(-room // TILE_ROWS), words, dtype=torch.int32, device=device)
+
+    @property
+    def shape(self) -> Tuple[int, int, int, int]:
+        """The shape of a 16-bit cache of the same rows."""
+        return (self.slots, self.room, self.n_kv, self.hd)
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def nbytes(self) -> int:
+        return self.data.numel() * 4
+
+    def _fields(self):
+        """Views: key words [slots, n_kv, tiles, 16, W], value words [.., W, 16], key groups [.., 16, hd / 32], value groups [.., 16, hd / 64]."""
+        W, a = self.hd // 8, TILE_ROWS * self.hd // 8
+        kg, vg = self.hd // KEY_GROUP, self.hd // VALUE_GROUP
+        d = self.data
+        return (d[..., :a].unflatten(-1, (TILE_ROWS, W)), d[..., a:2 * a].unflatten(-1, (W, TILE_ROWS)),
+                d[..., 2 * a:2 * a + TILE_ROWS * kg].unflatten(-1, (TILE_ROWS, kg)), d[..., 2 * a + TILE_ROWS * kg:].unflatten(-1, (TILE_ROWS, vg)))
+
+    def _check(self, cu_seqlens, slots, start):
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise ValueError("Int4KVCache: cu_seqlens holds one number more than there are sequences")
+        n = cu_seqlens.numel() - 1
+        for name, t in (("slots", slots), ("start", start)):
+            if t is not None and tuple(t.shape) != (n,):
+                raise ValueError(f"Int4KVCache: `{name}` holds one number a sequence ({n}), not {tuple(t.shape)}")
+        i = lambda t: None if t is None else t.to(device=self.device, dtype=torch.int32).contiguous()   # noqa: E731
+        return i(cu_seqlens), i(slots), i(start)
+
+    def _rows(self, cu, slots, start, tokens: int):
+        """(token, slot, row) of every packed token whose row is inside the cache."""
+        tok = torch.arange(tokens, device=cu.device)
+        seq = torch.searchsorted(cu[1:].long().contiguous(), tok, right=True)
+        inside = (seq < cu.numel() - 1) & (tok >= int(cu[0]))
+        tok, seq = tok[inside], seq[inside]
+        row = tok - cu.long()[seq] + (start.long()[seq] if start is not None else 0)
+        slot = slots.long()[seq] if slots is not None else seq
+        ok = (slot >= 0) & (slot < self.slots) & (row >= 0) & (row < self.room)
+        return tok[ok], slot[ok], row[ok]
+
+    def store(self, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: Optional[int] = None, slots: Optional[torch.Tensor] = None,
+              start: Optional[torch.Tensor] = None) -> None:
+        """Writes packed keys (rotated) and values [T, n_kv, hd]: the tokens cu_seqlens[i] .. of sequence i go to the rows start[i] .. (0 ..) of slot slots[i] (i).
+        Rows and slots outside the cache are left out, all others of the cache keep what they hold.  No row may be named twice in a call.  `max_seqlen` sets the
+        size of the launch alone."""
+        if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (self.n_kv, self.hd):
+            raise ValueError(f"Int4KVCache.store: keys and values [tokens, {self.n_kv}, {self.hd}], not {tuple(k.shape)} and {tuple(v.shape)}")
+        if k.dtype != self.dtype or v.dtype != self.dtype or k.device != self.device or v.device != self.device:
+            raise ValueError(f"Int4KVCache.store: keys and values are {self.dtype} on {self.device}, as the cache")
+        cu, slots, start = self._check(cu_seqlens, slots, start)
+        if use_native(k):
+            n = max_seqlen if max_seqlen is not None else k.shape[0] // max(1, cu.numel() - 1)
+            lib().int4_cache_store(_on16(k), _on16(v), self.data, cu, slots, start, self.room, n)
+            return
+        tok, slot, row = self._rows(cu, slots, start, k.shape[0])
+        self._put(k[tok], v[tok], slot, row)
+
+    def _put(self, k, v, slot, row):
+        kw, vw, kg, vg = self._fields()
+        tile, r = row // TILE_ROWS, row % TILE_ROWS
+        c, s, lo = quantize_groups(k, KEY_GROUP)
+        heads = torch.arange(self.n_kv, device=k.device)
+        at = (slot[:, None], heads[None], tile[:, None])
+        kw[at + (r[:, None],)] = _row_order(_words(c))
+        kg[at + (r[:, None],)] = _group_words(s, lo)
+        c, s, lo = quantize_groups(v, VALUE_GROUP)
+        place = 4 * ((r & 7) >> 1) + (r & 1) + 2 * (r >> 3)
+        vw.transpose(-1, -2)[at + (place[:, None],)] = _words(c)
+        vg[at + (r[:, None],)] = _group_words(s, lo)
+
+    def _get(self, slot, row):
+        kw, vw, kg, vg = self._fields()
+        tile, r = row // TILE_ROWS, row % TILE_ROWS
+        at = (slot[:, None], torch.arange(self.n_kv, device=slot.device)[None], tile[:, None])
+        place = 4 * ((r & 7) >> 1) + (r & 1) + 2 * (r >> 3)
+        k = dequantize_groups(_codes(_channel_order(kw[at + (r[:, None],)])), *_group_numbers(kg[at + (r[:, None],)], self.dtype))
+        v = dequantize_groups(_codes(vw.transpose(-1, -2)[at + (place[:, None],)]), *_group_numbers(vg[at + (r[:, None],)], self.dtype))
+        return k, v
+
+    def load(self, cu_seqlens: torch.Tensor, tokens: int, max_seqlen: Optional[int] = None, slots: Optional[torch.Tensor] = None,
+             start: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The reverse of `store`: keys and values [tokens, n_kv, hd] of the cache's type, each number rounded once.  Tokens whose row or slot is outside the cache,
+        or that belong to no sequence, are 0."""
+        if tokens < 0:
+            raise ValueError(f"Int4KVCache.load: {tokens} tokens")
+        cu, slots, start = self._check(cu_seqlens, slots, start)
+        if use_native(self.data):
+            n = max_seqlen if max_seqlen is not None else tokens // max(1, cu.numel() - 1)
+            k, v = lib().int4_cache_load(self.data, cu, slots, start, self.room, self.hd, tokens, n, self.dtype)
+            return k, v
+        out = torch.zeros(2, tokens, self.n_kv, self.hd, dtype=self.dtype, device=self.device)
+        tok, slot, row = self._rows(cu, slots, start, tokens)
+        k, v = self._get(slot, row)
+        out[0, tok], out[1, tok] = k.to(self.dtype), v.to(self.dtype)
+        return out[0], out[1]
+
+
+# ------------------------------------------------------------------------------------------------ attention
+
+
+def _rotated(x, cos, sin, rot_dim: int, interleaved: bool):
+    """fp32 x [B, heads, hd], cos / sin [B, rot_dim / 2]."""
+    c, s = cos[:, None], sin[:, None]
+    a, b = (x[..., 0:rot_dim:2], x[..., 1:rot_dim:2]) if interleaved else (x[..., : rot_dim // 2], x[..., rot_dim // 2: rot_dim])
+    y = (a * c - b * s, b * c + a * s)
+    y = torch.stack(y, -1).flatten(-2) if interleaved else torch.cat(y, -1)
+    return torch.cat([y, x[..., rot_dim:]], -1)
+
+
+def decode_attention_int4_ref(qkv, cache: Int4KVCache, cache_lens, n_q: int, n_kv: int, hd: int, scale: float, cos=None, sin=None, rot_dim: Optional[int] = None,
+                              interleaved: bool = False):
+    """`decode_attention_int4` in plain PyTorch, on any device and for fp32 projections too."""
+    B, lens = qkv.shape[0], cache_lens.long()
+    live = (lens >= 0) & (lens < cache.room)
+    q, k, v = (t.reshape(B, -1, hd).float() for t in qkv.split([n_q * hd, n_kv * hd, n_kv * hd], 1))
+    if cos is not None:
+        at = lens.clamp(0, max(cache.room - 1, 0))
+        q, k = (_rotated(t, cos[at], sin[at], rot_dim or hd, interleaved) for t in (q, k))
+    slot = torch.nonzero(live).flatten()
+    cache._put(k[slot].to(cache.dtype), v[slot].to(cache.dtype), slot, lens[slot])
+    out = torch.zeros(B, n_q, hd, dtype=torch.float32, device=qkv.device)
+    for b in slot.tolist():
+        n = int(lens[b]) + 1
+        kk, vv = (t.repeat_interleave(n_q // n_kv, 1) for t in cache._get(torch.full((n,), b, device=qkv.device), torch.arange(n, device=qkv.device)))
+        out[b] = torch.einsum("hn,nhd->hd", torch.softmax(torch.einsum("hd,nhd->hn", q[b], kk) * scale, -1), vv)
+    return out.reshape(B, n_q * hd).to(qkv.dtype)
+
+
+def decode_attention_int4(qkv: torch.Tensor, cache: Int4KVCache, cache_lens: torch.Tensor, n_q: int, n_kv: int, hd: int, scale: Optional[float] = None, cos=None,
+                          sin=None, rot_dim: Optional[int] = None, interleaved: bool = False) -> torch.Tensor:
+    """One decode step over a 4-bit cache, as `attention.decode_attention` over a 16-bit one: row b of qkv [slots, (n_q + 2 n_kv) * hd] is the fused projection of
+    the token at position cache_lens[b] of slot b.  Its queries and key are rotated (cos / sin [room or more, rot_dim / 2] given), the key is rounded to the cache's
+    type, key and value are quantised and written, and the queries attend to the rows [0, cache_lens[b]] as the cache holds them, the new one among them.
+    Returns [slots, n_q * hd].  A row whose length is not in [0, room) changes nothing and returns 0.  Does not advance cache_lens."""
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    if (n_kv, hd) != (cache.n_kv, cache.hd) or n_q <= 0 or n_q % n_kv:
+        raise ValueError(f"decode_attention_int4: {n_q} query heads over {n_kv} of {hd} channels, a cache of {cache.n_kv} heads of {cache.hd}")
+    if tuple(qkv.shape) != (cache.slots, (n_q + 2 * n_kv) * hd) or tuple(cache_lens.shape) != (cache.slots,):
+        raise ValueError(f"decode_attention_int4: projections [{cache.slots}, {(n_q + 2 * n_kv) * hd}] and as many lengths, not {tuple(qkv.shape)} and "
+                         f"{tuple(cache_lens.shape)}")
+    rot = rot_dim or hd
+    if (cos is None) != (sin is None) or (cos is not None and (rot > hd or rot % (2 if interleaved else 16) or tuple(cos.shape[1:]) != (rot // 2,) or
+                                                               cos.shape != sin.shape or cos.shape[0] < cache.room)):
+        raise ValueError(f"decode_attention_int4: cosines and sines are tables [{cache.room} or more, {rot // 2}], both or neither")
+    if use_native(qkv):
+        if qkv.dtype != cache.dtype or qkv.device != cache.device:
+            raise ValueError(f"decode_attention_int4: projections are {cache.dtype} on {cache.device}, as the cache")
+        return lib().decode_attention_int4(_on16(qkv), cache.data, cache_lens.int().contiguous(), n_q, n_kv, hd, cache.room, scale, cos, sin, rot, interleaved)
+    return decode_attention_int4_ref(qkv, cache, cache_lens, n_q, n_kv, hd, scale, cos, sin, rot, interleaved)
+
+
+# ------------------------------------------------------------------------------------------------ weights
+
+
+class Int4Linear:
+    """One weight matrix [N, K] in 4 bits, groups of `group` along K (+ optional bias).  `__call__(x)`: x @ w^T + bias for x [..., K] of the weight's type."""
+
+    __slots__ = ("q", "bias", "N", "K", "group", "dtype")
+
+    def __init__(self, w: torch.Tensor, bias: Optional[torch.Tensor] = None, group: int = 128):
+        self._plan(w.shape, group, w.dtype, w.device, bias)
+        self.requantize(w)
+
+    def _plan(self, shape, group: int, dtype, device, bias):
+        if len(shape) != 2 or group not in GROUPS or shape[0] <= 0 or shape[1] <= 0 or shape[1] % group:
+            raise ValueError(f"Int4Linear: a weight [N, K] with groups of 32, 64 or 128 along K, not {tuple(shape)} in groups of {group}")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"Int4Linear: bfloat16 or float16, not {dtype}")
+        self.N, self.K, self.group, self.dtype = int(shape[0]), int(shape[1]), int(group), dtype
+        if bias is not None and (tuple(bias.shape) != (self.N,) or bias.dtype != dtype):
+            raise ValueError(f"Int4Linear: a bias [{self.N}] of {dtype}")
+        self.bias = bias
+        self.q = torch.zeros(-(-self.N // TILE_ROWS), -(-self.K // 128), TILE_ROWS * 16 + TILE_ROWS * (128 // group), dtype=torch.int32, device=device)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scale: torch.Tensor, low: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int4Linear":
+        """codes uint8 [N, K] (0 .. 15), scale and low [N, K / group] of the model's type: a weight that was quantised elsewhere."""
+        if codes.dim() != 2 or codes.dtype != torch.uint8 or scale.shape != low.shape or scale.dtype != low.dtype or scale.dim() != 2 or scale.shape[0] != codes.shape[0] \
+                or scale.shape[1] == 0 or codes.shape[1] % scale.shape[1]:
+            raise ValueError("Int4Linear.from_codes: codes uint8 [N, K], scale and low [N, K / group] of one type")
+        if codes.numel() and int(codes.max()) > 15:
+            raise ValueError("Int4Linear.from_codes: a code is 0 .. 15")
+        self = cls.__new__(cls)
+        self._plan(codes.shape, codes.shape[1] // scale.shape[1], scale.dtype, codes.device, bias)
+        self._fill(codes, scale, low)
+        return self
+
+    def _fill(self, codes, scale, low):
+        nt, kb, _ = self.q.shape
+        self.q.zero_()
+        w = torch.zeros(nt * TILE_ROWS, kb * 16, dtype=torch.int32, device=codes.device)
+        w[: self.N, : self.K // 8] = _words(codes)
+        self.q[..., :256] = _row_order(w.view(nt, TILE_ROWS, kb, 16)).transpose(1, 2).flatten(-2)
+        g = torch.zeros(nt * TILE_ROWS, kb * (128 // self.group), dtype=torch.int32, device=codes.device)
+        g[: self.N, : self.K // self.group] = _group_words(scale.contiguous(), low.contiguous())
+        self.q[..., 256:] = g.view(nt, TILE_ROWS, kb, -1).transpose(1, 2).flatten(-2)
+
+    def requantize(self, w: torch.Tensor):
+        """Refresh the 4-bit copy in place after the weight changed (same buffers: a kept CUDA graph stays valid)."""
+        if tuple(w.shape) != (self.N, self.K) or w.dtype != self.dtype or w.device != self.q.device:
+            raise ValueError(f"Int4Linear: a weight [{self.N}, {self.K}] of {self.dtype} on {self.q.device}")
+        if use_native(w):
+            lib().int4_quantize(_on16(w), self.q, self.group)
+        else:
+            self._fill(*quantize_groups(w, self.group))
+
+    def codes(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """(codes uint8 [N, K], scale, low [N, K / group])."""
+        nt, kb, _ = self.q.shape
+        w = _channel_order(self.q[..., :256].unflatten(-1, (TILE_ROWS, 16))).transpose(1, 2).reshape(nt * TILE_ROWS, kb * 16)
+        g = self.q[..., 256:].unflatten(-1, (TILE_ROWS, -1)).transpose(1, 2).reshape(nt * TILE_ROWS, -1)
+        return (_codes(w[: self.N, : self.K // 8]),) + _group_numbers(g[: self.N, : self.K // self.group], self.dtype)
+
+    def dequantize(self) -> torch.Tensor:
+        """fp32 [N, K]."""
+        return dequantize_groups(*self.codes())
+
+    def __call__(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if x.dim() == 0 or x.shape[-1] != self.K:
+            raise ValueError(f"Int4Linear: rows of {self.K}, not {tuple(x.shape)}")
+        bias = self.bias if bias is None else bias
+        x2 = x.reshape(-1, self.K)
+        if use_native(x):
+            if x.dtype != self.dtype or x.device != self.q.device:
+                raise ValueError(f"Int4Linear: rows of {self.dtype} on {self.q.device}")
+            y = lib().int4_linear(_on16(x2), self.q, bias, self.N, self.group)
+        else:
+            y = x2.float() @ self.dequantize().t()
+            y = (y if bias is None else y + bias.float()).to(x.dtype)
+        return y.view(*x.shape[:-1], self.N)
+
+    def nbytes(self) -> int:
+        return 4 * self.q.numel()
+
+
+def supported(w: torch.Tensor, group: int = 128) -> bool:
+    """Weights that a 4-bit copy can be made of."""
+    return bool(w.dim() == 2 and w.dtype in (torch.bfloat16, torch.float16) and w.shape[0] > 0 and w.shape[1] > 0 and w.shape[1] % group == 0)
