@@ -1,15 +1,17 @@
 // Numbers in groups of 4-bit codes: x ~ scale * c + low with low = min x, scale = T((max x - low) / 15), c = 0 .. 15 (T: the 16-bit type of the model).
 //
-// Eight neighbouring channels are one 32-bit word, channel 2i in bits 4i .. 4i + 3, channel 2i + 1 in bits 16 + 4i ..: a mask over both halves of a word leaves
-// a pair of neighbouring channels, and in the low 10 bits of an fp16 number a code is a subnormal, c 2^-24 (from bits 0 .. 3) or 16 c 2^-24 (from bits 4 .. 7).
-// A matrix instruction multiplies those exactly: no conversion, one shift for four pairs, and the powers of two go where they cost nothing.
-// A group's numbers are one word: scale in its upper half, low in its lower half.
+// A group's numbers are one word: scale in its upper half, low in its lower half.  Codes go to matrix instructions as they are, so each kind of operand has the order of
+// nibbles that costs the fewest instructions to take apart:
+//   key words     eight channels c, at bits 8 (c & 3) + 4 (c >> 2): two masks and a shift leave two operands of four bytes.
+//   value halves  four channels c of one row at bits 4 c of a half-word, a row's neighbour in the other half: masks and one shift leave pairs of neighbouring rows, and in the low
+//                 ten bits of an fp16 number a code is a subnormal, c 2^-24 (from bits 0 .. 3) or 16 c 2^-24 (from bits 4 .. 7).
+//   weight words  eight channels c, at bits 4 (c >> 1) + 16 (c & 1): pairs of neighbouring channels, as fp16 subnormals too.
 //
 // A row of n words (n / 4 = channels / 32 = J) is stored as [t = 0 .. 3][j < J], word (t, j) holding the channels 32 j + 8 t ..: the four lanes of a row in a matrix
 // instruction's operand take 16 neighbouring bytes each, and what they take together for step j lies in one group of 32.
 //
-// A cache is tiles of 16 rows of one head: key words [row][t][j], value words [word 0 .. D / 8 - 1][place of the row], the keys' group words [row][D / 32], the
-// values' [row][D / 64].  The place of row r, 4 ((r & 7) >> 1) + (r & 1) + 2 (r >> 3), brings the four rows whose weights a lane holds together.
+// A cache is tiles of 16 rows of one head: key words [row][t][j], the values, the keys' group words [row][D / 32], the values' [row][D / 64].  The values of a tile are
+// [channels / 8][t = 0 .. 3][row / 8][quad of channels][row & 1] halves, t = (row & 7) / 2: a lane's four rows and eight channels are 16 neighbouring bytes.
 #pragma once
 #include "common.cuh"
 
@@ -27,7 +29,8 @@ template <int D> struct Tile {
   static constexpr int kBytes = kWords * 4;
 };
 
-RB_DEVICE int place_of(int r) { return 4 * ((r & 7) >> 1) + (r & 1) + 2 * (r >> 3); }
+// the first of the two halves (the other is two further) that hold the channels 8 w .. of row r
+RB_DEVICE int half_place(int w, int r) { return 32 * w + 8 * ((r & 7) >> 1) + 4 * (r >> 3) + (r & 1); }
 // the place of word w (channels 8 w ..) in a row
 template <int J> RB_DEVICE int word_place(int w) { return (w & 3) * J + (w >> 2); }
 
@@ -52,21 +55,30 @@ template <typename T> RB_DEVICE uint32_t group_word(float lo, float hi) {
   if (!(fabsf(lo) <= kMost && fabsf(hi) <= kMost)) return bits16<T>(__int_as_float(0x7fc00000)) * 0x10001u;
   return bits16<T>(__fdiv_rn(__fsub_rn(hi * 0.0625f, lo * 0.0625f), 0.9375f)) << 16 | bits16<T>(lo);
 }
-// The code of x in a group with this scale and low: the quotient rounded to the nearest whole number, halves to the even one.
-RB_DEVICE uint32_t code_of(float x, float scale, float low) {
-  if (!(scale > 0.f)) return 0;
-  return (uint32_t)__float2int_rn(fminf(__fdiv_rn(__fsub_rn(x * 0.0625f, low * 0.0625f), scale * 0.0625f), 15.f));
-}
-RB_DEVICE uint32_t pack8(const float (&x)[8], float scale, float low) {
-  uint32_t w = 0;
+// The codes of eight numbers of a group: (x - low) / scale rounded to the nearest whole number, halves to the even one.  The quotient is correctly rounded: a product with the
+// correctly rounded reciprocal, corrected once by its remainder (Markstein's theorem), so that ties are ties.
+RB_DEVICE void codes8(const float (&x)[8], float scale, float low, uint32_t (&c)[8]) {
+  const float s = scale * 0.0625f, l = low * 0.0625f, r = __frcp_rn(s);
+  const bool any = scale > 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w |= code_of(x[i], scale, low) << (4 * (i >> 1) + 16 * (i & 1));
+  for (int i = 0; i < 8; ++i) {
+    const float a = fmaf(x[i], 0.0625f, -l), q = __fmul_rn(a, r), e = fmaf(fmaf(-q, s, a), r, q);
+    c[i] = any ? __float_as_uint(__fadd_rn(fminf(e, 15.f), 12582912.f)) & 15u : 0u;   // (1.5 2^23: the sum's last bits are the whole number)
+  }
+}
+constexpr int kKey = 0, kValue = 1, kWeight = 2;
+template <int kKind> RB_DEVICE int bit_of(int c) { return kKind == kKey ? 8 * (c & 3) + 4 * (c >> 2) : kKind == kValue ? 4 * c : 4 * (c >> 1) + 16 * (c & 1); }
+template <int kKind> RB_DEVICE uint32_t pack8(const float (&x)[8], float scale, float low) {
+  uint32_t c[8], w = 0;
+  codes8(x, scale, low, c);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w |= c[i] << bit_of<kKind>(i);
   return w;
 }
 // fp32 values of a word's channels: scale * c is exact, one rounding
-RB_DEVICE void unpack8(uint32_t w, float scale, float low, float (&x)[8]) {
+template <int kKind> RB_DEVICE void unpack8(uint32_t w, float scale, float low, float (&x)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = fmaf(scale, (float)(w >> (4 * (i >> 1) + 16 * (i & 1)) & 15u), low);
+  for (int i = 0; i < 8; ++i) x[i] = fmaf(scale, (float)(w >> bit_of<kKind>(i) & 15u), low);
 }
 
 // The extremes over a group that kLanes neighbouring lanes hold, eight channels each.

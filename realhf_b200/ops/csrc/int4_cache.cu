@@ -1,6 +1,7 @@
 // Keys and values of packed sequences into a 4-bit cache, and back (layout and rule: int4.cuh).
 //
-// One block per (tile of a sequence, head).  Read or write of the 16-bit side: 16 bytes a lane, a head's row by 8 or 16 lanes.
+// One block per (tile of a sequence, head).  The 16-bit side: 16 bytes a lane, a head's row by 8 or 16 lanes.  The 4-bit side: a tile is put together in shared memory and
+// copied whole, 16 bytes a lane; where a sequence begins or ends inside it, its rows' words are written one by one and the others left alone.
 #include "int4.cuh"
 
 #include <algorithm>
@@ -20,7 +21,8 @@ struct CacheParams {
 template <typename T, int D, bool kStore>
 __global__ void __launch_bounds__(kThreads) cache_rows_kernel(CacheParams p) {
   using Tl = q4::Tile<D>;
-  constexpr int LPR = D / 8, kGroups = kThreads / LPR;
+  constexpr int LPR = D / 8, kGroups = kThreads / LPR, kTurns = 16 / kGroups;
+  __shared__ __align__(16) uint32_t tile_words[Tl::kWords];
   rb::pdl_trigger();
   rb::pdl_wait();
   const int seq = blockIdx.x, head = blockIdx.y, sub = threadIdx.x % LPR;
@@ -32,46 +34,73 @@ __global__ void __launch_bounds__(kThreads) cache_rows_kernel(CacheParams p) {
   const int64_t first = (start < 0 ? start - 15 : start) / 16, last = start + (tok1 - tok0);   // tiles first .. ; rows below `last`
   for (int64_t tile = first + blockIdx.z; tile * 16 < last; tile += gridDim.z) {
     uint32_t* at = p.cache + (((int64_t)slot * p.nkv + head) * p.tiles + tile) * Tl::kWords;
-#pragma unroll 1
-    for (int r = threadIdx.x / LPR; r < 16; r += kGroups) {      // (a warp's lanes take the same turns)
-      const int64_t row = tile * 16 + r, tok = tok0 + (row - start);
-      const bool mine = row >= start && row < last, held = there && row >= 0 && row < p.room;
-      float x[8];
-      if constexpr (kStore) {
-        rb::Pack<T, 8> a{}, b{};
-        if (mine && held) {
-          a = *reinterpret_cast<const rb::Pack<T, 8>*>(reinterpret_cast<const T*>(p.k) + tok * p.kt + head * p.kh + sub * 8);
-          b = *reinterpret_cast<const rb::Pack<T, 8>*>(reinterpret_cast<const T*>(p.v) + tok * p.vt + head * p.vh + sub * 8);
-        }
-        float lo, hi;
+    const bool held = there && tile >= 0 && tile < p.tiles;        // (rows at or beyond `room` are looked at one by one)
+    const bool whole = held && tile * 16 >= start && tile * 16 + 16 <= last && tile * 16 + 16 <= p.room;
+    if constexpr (kStore) {
+      if (!held) continue;
+      rb::Pack<T, 8> a[kTurns], b[kTurns];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = rb::to_f(a.v[i]);
+      for (int i = 0; i < kTurns; ++i) {
+        const int64_t row = tile * 16 + threadIdx.x / LPR + i * kGroups, tok = tok0 + (row - start);
+        a[i] = b[i] = rb::Pack<T, 8>{};
+        if (row >= start && row < last && row < p.room) {
+          a[i] = *reinterpret_cast<const rb::Pack<T, 8>*>(reinterpret_cast<const T*>(p.k) + tok * p.kt + head * p.kh + sub * 8);
+          b[i] = *reinterpret_cast<const rb::Pack<T, 8>*>(reinterpret_cast<const T*>(p.v) + tok * p.vt + head * p.vh + sub * 8);
+        }
+      }
+      uint32_t* to = whole ? tile_words : at;
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int r = threadIdx.x / LPR + i * kGroups;
+        const int64_t row = tile * 16 + r;
+        float x[8], lo, hi;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = rb::to_f(a[i].v[e]);
         q4::extremes<4>(x, lo, hi);
-        const uint32_t kg = q4::group_word<T>(lo, hi), kw = q4::pack8(x, q4::scale_of<T>(kg), lo);
+        const uint32_t kg = q4::group_word<T>(lo, hi), kw = q4::pack8<q4::kKey>(x, q4::scale_of<T>(kg), lo);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = rb::to_f(b.v[i]);
+        for (int e = 0; e < 8; ++e) x[e] = rb::to_f(b[i].v[e]);
         q4::extremes<8>(x, lo, hi);
-        const uint32_t vg = q4::group_word<T>(lo, hi), vw = q4::pack8(x, q4::scale_of<T>(vg), lo);
-        if (mine && held) {
-          at[r * Tl::W + q4::word_place<Tl::J>(sub)] = kw;
-          at[Tl::kValues + sub * 16 + q4::place_of(r)] = vw;
-          if (sub % 4 == 0) at[Tl::kKeyScales + r * Tl::J + sub / 4] = kg;
-          if (sub % 8 == 0) at[Tl::kValueScales + r * Tl::H + sub / 8] = vg;
+        const uint32_t vg = q4::group_word<T>(lo, hi), vw = q4::pack8<q4::kValue>(x, q4::scale_of<T>(vg), lo);
+        if (row >= start && row < last && row < p.room) {
+          uint16_t* halves = reinterpret_cast<uint16_t*>(to + Tl::kValues) + q4::half_place(sub, r);
+          to[r * Tl::W + q4::word_place<Tl::J>(sub)] = kw;
+          halves[0] = (uint16_t)vw;
+          halves[2] = (uint16_t)(vw >> 16);
+          if (sub % 4 == 0) to[Tl::kKeyScales + r * Tl::J + sub / 4] = kg;
+          if (sub % 8 == 0) to[Tl::kValueScales + r * Tl::H + sub / 8] = vg;
         }
-      } else if (mine) {
+      }
+      if (whole) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < Tl::kWords / 4; i += kThreads) reinterpret_cast<uint4*>(at)[i] = reinterpret_cast<const uint4*>(tile_words)[i];
+        __syncthreads();
+      }
+    } else {
+      if (held)
+        for (int i = threadIdx.x; i < Tl::kWords / 4; i += kThreads) reinterpret_cast<uint4*>(tile_words)[i] = reinterpret_cast<const uint4*>(at)[i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int r = threadIdx.x / LPR + i * kGroups;
+        const int64_t row = tile * 16 + r, tok = tok0 + (row - start);
+        if (row < start || row >= last) continue;
         rb::Pack<T, 8> a{}, b{};
-        if (held) {
-          const uint32_t kg = at[Tl::kKeyScales + r * Tl::J + sub / 4], vg = at[Tl::kValueScales + r * Tl::H + sub / 8];
-          q4::unpack8(at[r * Tl::W + q4::word_place<Tl::J>(sub)], q4::scale_of<T>(kg), q4::low_of<T>(kg), x);
+        if (held && row < p.room) {
+          float x[8];
+          const uint16_t* halves = reinterpret_cast<const uint16_t*>(tile_words + Tl::kValues) + q4::half_place(sub, r);
+          const uint32_t kg = tile_words[Tl::kKeyScales + r * Tl::J + sub / 4], vg = tile_words[Tl::kValueScales + r * Tl::H + sub / 8];
+          q4::unpack8<q4::kKey>(tile_words[r * Tl::W + q4::word_place<Tl::J>(sub)], q4::scale_of<T>(kg), q4::low_of<T>(kg), x);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) a.v[i] = rb::from_f<T>(x[i]);
-          q4::unpack8(at[Tl::kValues + sub * 16 + q4::place_of(r)], q4::scale_of<T>(vg), q4::low_of<T>(vg), x);
+          for (int e = 0; e < 8; ++e) a.v[e] = rb::from_f<T>(x[e]);
+          q4::unpack8<q4::kValue>(halves[0] | (uint32_t)halves[2] << 16, q4::scale_of<T>(vg), q4::low_of<T>(vg), x);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) b.v[i] = rb::from_f<T>(x[i]);
+          for (int e = 0; e < 8; ++e) b.v[e] = rb::from_f<T>(x[e]);
         }
         *reinterpret_cast<rb::Pack<T, 8>*>(reinterpret_cast<T*>(p.k) + tok * p.kt + head * p.kh + sub * 8) = a;
         *reinterpret_cast<rb::Pack<T, 8>*>(reinterpret_cast<T*>(p.v) + tok * p.vt + head * p.vh + sub * 8) = b;
       }
+      __syncthreads();
     }
   }
 }

@@ -1,6 +1,6 @@
 // Products of a few rows with a weight held in 4 bits: y[m, n] = sum_k x[m, k] w[n, k] (+ bias[n]), w ~ scale c + low by groups of 32, 64 or 128 along K (int4.cuh).
 //
-// A weight is tiles of 16 output rows x 128 channels, the tiles of 16 rows one behind the other along K: code words [row][t][j] as a cache's keys of 128 channels,
+// A weight is tiles of 16 output rows x 128 channels, the tiles of 16 rows one behind the other along K: weight words [row][t][j] of 128 channels,
 // then the group words [row][group].  Rows beyond N and channels beyond K hold codes, scales and lowest values of 0.
 //
 // One warp per output row: its lanes walk along K, eight rows of x at a time.
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ w, 
     q4::extremes<G / 8>(x, lo, hi);
     const uint32_t g = mine ? q4::group_word<T>(lo, hi) : 0u;
     uint32_t* at = q + ((int64_t)blockIdx.x * kblocks + kb) * WTile<G>::kWords;
-    at[r * 16 + q4::word_place<4>(sub)] = mine ? q4::pack8(x, q4::scale_of<T>(g), lo) : 0u;
+    at[r * 16 + q4::word_place<4>(sub)] = mine ? q4::pack8<q4::kWeight>(x, q4::scale_of<T>(g), lo) : 0u;
     if (sub % (G / 8) == 0) at[256 + r * WTile<G>::kGroups + sub / (G / 8)] = g;
   }
 }
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kThreads) linear_kernel(const T* __restrict__ 
       const uint32_t* at = q + ((int64_t)(n / 16) * kblocks + kw / 16) * WTile<G>::kWords;
       const uint32_t g = at[256 + n % 16 * WTile<G>::kGroups + kw % 16 / (G / 8)];
       float w[8];
-      q4::unpack8(at[n % 16 * 16 + q4::word_place<4>(kw % 16)], q4::scale_of<T>(g), q4::low_of<T>(g), w);
+      q4::unpack8<q4::kWeight>(at[n % 16 * 16 + q4::word_place<4>(kw % 16)], q4::scale_of<T>(g), q4::low_of<T>(g), w);
       for (int m = 0; m < 8 && m0 + m < M; ++m)
         for (int i = 0; i < 8; ++i) acc[m] = fmaf(rb::to_f(x[(m0 + m) * ldx + kw * 8 + i]), w[i], acc[m]);
     }

@@ -29,7 +29,8 @@ from realhf_b200.ops import lib, use_native
 KEY_GROUP, VALUE_GROUP, TILE_ROWS = 32, 64, 16
 HEAD_DIMS = (64, 128)
 GROUPS = (32, 64, 128)
-_SHIFT = [4 * (i >> 1) + 16 * (i & 1) for i in range(8)]   # where channel i of a word's eight has its bits
+# where channel i of a word's eight has its bits, in a key's, a value's and a weight's word
+_KEY, _VALUE, _WEIGHT = [8 * (i & 3) + 4 * (i >> 2) for i in range(8)], [4 * i for i in range(8)], [4 * (i >> 1) + 16 * (i & 1) for i in range(8)]
 
 
 # ------------------------------------------------------------------------------------------------ groups
@@ -62,15 +63,15 @@ def dequantize_groups(codes: torch.Tensor, scale: torch.Tensor, low: torch.Tenso
     return (xg * scale.double()[..., None] + low.double()[..., None]).float().flatten(-2)
 
 
-def _words(codes: torch.Tensor) -> torch.Tensor:
+def _words(codes: torch.Tensor, shifts) -> torch.Tensor:
     """uint8 [..., 8 n] -> int32 [..., n], channels in order."""
-    sh = torch.tensor(_SHIFT, dtype=torch.int64, device=codes.device)
+    sh = torch.tensor(shifts, dtype=torch.int64, device=codes.device)
     w = (codes.unflatten(-1, (-1, 8)).long() << sh).sum(-1)
     return torch.where(w >= 1 << 31, w - (1 << 32), w).int()
 
 
-def _codes(words: torch.Tensor) -> torch.Tensor:
-    sh = torch.tensor(_SHIFT, dtype=torch.int32, device=words.device)
+def _codes(words: torch.Tensor, shifts) -> torch.Tensor:
+    sh = torch.tensor(shifts, dtype=torch.int32, device=words.device)
     return ((words[..., None] >> sh) & 15).to(torch.uint8).flatten(-2)
 
 
@@ -131,11 +132,12 @@ class Int4KVCache:
         return self.data.numel() * 4
 
     def _fields(self):
-        """Views: key words [slots, n_kv, tiles, 16, W], value words [.., W, 16], key groups [.., 16, hd / 32], value groups [.., 16, hd / 64]."""
+        """Views: key words [slots, n_kv, tiles, 16, W], value halves int16 [.., W, 4, 2, 2, 2] (channels / 8, (row & 7) / 2, row / 8, quad of channels, row & 1), key groups
+        [.., 16, hd / 32], value groups [.., 16, hd / 64]."""
         W, a = self.hd // 8, TILE_ROWS * self.hd // 8
         kg, vg = self.hd // KEY_GROUP, self.hd // VALUE_GROUP
         d = self.data
-        return (d[..., :a].unflatten(-1, (TILE_ROWS, W)), d[..., a:2 * a].unflatten(-1, (W, TILE_ROWS)),
+        return (d[..., :a].unflatten(-1, (TILE_ROWS, W)), d.view(torch.int16)[..., 2 * a:4 * a].unflatten(-1, (W, 4, 2, 2, 2)),
                 d[..., 2 * a:2 * a + TILE_ROWS * kg].unflatten(-1, (TILE_ROWS, kg)), d[..., 2 * a + TILE_ROWS * kg:].unflatten(-1, (TILE_ROWS, vg)))
 
     def _check(self, cu_seqlens, slots, start):
@@ -176,27 +178,28 @@ class Int4KVCache:
         tok, slot, row = self._rows(cu, slots, start, k.shape[0])
         self._put(k[tok], v[tok], slot, row)
 
+    def _at(self, slot, row):
+        """Index of rows in the fields of keys and of the groups, and in the values with the row's three dims in front."""
+        tile, r = row // TILE_ROWS, row % TILE_ROWS
+        at = (slot[:, None], torch.arange(self.n_kv, device=slot.device)[None], tile[:, None])
+        return at + (r[:, None],), at + ((r[:, None] & 7) >> 1, r[:, None] >> 3, r[:, None] & 1)
+
     def _put(self, k, v, slot, row):
         kw, vw, kg, vg = self._fields()
-        tile, r = row // TILE_ROWS, row % TILE_ROWS
+        at, place = self._at(slot, row)
         c, s, lo = quantize_groups(k, KEY_GROUP)
-        heads = torch.arange(self.n_kv, device=k.device)
-        at = (slot[:, None], heads[None], tile[:, None])
-        kw[at + (r[:, None],)] = _row_order(_words(c))
-        kg[at + (r[:, None],)] = _group_words(s, lo)
+        kw[at] = _row_order(_words(c, _KEY))
+        kg[at] = _group_words(s, lo)
         c, s, lo = quantize_groups(v, VALUE_GROUP)
-        place = 4 * ((r & 7) >> 1) + (r & 1) + 2 * (r >> 3)
-        vw.transpose(-1, -2)[at + (place[:, None],)] = _words(c)
-        vg[at + (r[:, None],)] = _group_words(s, lo)
+        vw.permute(0, 1, 2, 4, 5, 7, 3, 6)[place] = _words(c, _VALUE).view(torch.int16).unflatten(-1, (-1, 2))
+        vg[at] = _group_words(s, lo)
 
     def _get(self, slot, row):
         kw, vw, kg, vg = self._fields()
-        tile, r = row // TILE_ROWS, row % TILE_ROWS
-        at = (slot[:, None], torch.arange(self.n_kv, device=slot.device)[None], tile[:, None])
-        place = 4 * ((r & 7) >> 1) + (r & 1) + 2 * (r >> 3)
-        k = dequantize_groups(_codes(_channel_order(kw[at + (r[:, None],)])), *_group_numbers(kg[at + (r[:, None],)], self.dtype))
-        v = dequantize_groups(_codes(vw.transpose(-1, -2)[at + (place[:, None],)]), *_group_numbers(vg[at + (r[:, None],)], self.dtype))
-        return k, v
+        at, place = self._at(slot, row)
+        k = dequantize_groups(_codes(_channel_order(kw[at]), _KEY), *_group_numbers(kg[at], self.dtype))
+        words = vw.permute(0, 1, 2, 4, 5, 7, 3, 6)[place].contiguous().flatten(-2).view(torch.int32)
+        return k, dequantize_groups(_codes(words, _VALUE), *_group_numbers(vg[at], self.dtype))
 
     def load(self, cu_seqlens: torch.Tensor, tokens: int, max_seqlen: Optional[int] = None, slots: Optional[torch.Tensor] = None,
              start: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -310,7 +313,7 @@ class Int4Linear:
         nt, kb, _ = self.q.shape
         self.q.zero_()
         w = torch.zeros(nt * TILE_ROWS, kb * 16, dtype=torch.int32, device=codes.device)
-        w[: self.N, : self.K // 8] = _words(codes)
+        w[: self.N, : self.K // 8] = _words(codes, _WEIGHT)
         self.q[..., :256] = _row_order(w.view(nt, TILE_ROWS, kb, 16)).transpose(1, 2).flatten(-2)
         g = torch.zeros(nt * TILE_ROWS, kb * (128 // self.group), dtype=torch.int32, device=codes.device)
         g[: self.N, : self.K // self.group] = _group_words(scale.contiguous(), low.contiguous())
@@ -330,7 +333,7 @@ class Int4Linear:
         nt, kb, _ = self.q.shape
         w = _channel_order(self.q[..., :256].unflatten(-1, (TILE_ROWS, 16))).transpose(1, 2).reshape(nt * TILE_ROWS, kb * 16)
         g = self.q[..., 256:].unflatten(-1, (TILE_ROWS, -1)).transpose(1, 2).reshape(nt * TILE_ROWS, -1)
-        return (_codes(w[: self.N, : self.K // 8]),) + _group_numbers(g[: self.N, : self.K // self.group], self.dtype)
+        return (_codes(w[: self.N, : self.K // 8], _WEIGHT),) + _group_numbers(g[: self.N, : self.K // self.group], self.dtype)
 
     def dequantize(self) -> torch.Tensor:
         """fp32 [N, K]."""
