@@ -20,6 +20,7 @@ constexpr int kWarps = 4, kDecThreads = kWarps * 32;
 constexpr int ctas_of(int rep) { return rep <= 4 ? 4 : 3; }                       // CTAs an SM
 template <int D> constexpr int slots_of() { return 9728 / (2 * q4::Tile<D>::kBytes); }   // steps of a warp's ring: 2 or 4
 constexpr size_t kRing = 9728, kSmem = kWarps * kRing;
+constexpr float kSlack = 4.f;                                                     // how far (in powers of two) a maximum grows before the sums are corrected: weights up to 2^4
 constexpr int kMaxSplits = 8;                                                     // CTAs of a portable cluster
 
 struct StepParams {
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   float m = -INFINITY, l = 0.f, z[H];               // of head `head`, over the lane's keys: maximum, sum of weights, sums of weights times lowest values
 #pragma unroll
   for (int h = 0; h < H; ++h) z[h] = 0.f;
-  int top = -100;                                   // scaled weights are in units of 2^(top - 14); every scale so far is below 2^top
+  int top = -100;                                   // scaled weights are in units of 2^(top - 10); every scale so far is below 2^top
   uint32_t bound = 0;                               // the group word of that scale
   int slot = 0;
   uint32_t round = 0;                               // parity of the ring's current round
@@ -297,8 +298,13 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
         for (int c = 0; c < kScores; ++c) {
           int d[4];                                 // 1.5 2^23 as fp32's bits, plus the sum: a number whose difference from 1.5 2^23 is the sum
           mma_s8(d, w0[j] & kLow, w1[j] & kLow, w0[j] >> 4 & kLow, w1[j] >> 4 & kLow, qb[j][c][0], qb[j][c][1], 0x4b400000);
+          float n[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[c][i] = fmaf(i < 2 ? f0 : f1, __int_as_float(d[i]) - 12582912.f, x[c][i]);
+          for (int i = 0; i < 4; ++i) n[i] = __int_as_float(d[i]);
+          add_pair(n[0], n[1], -12582912.f, -12582912.f);
+          add_pair(n[2], n[3], -12582912.f, -12582912.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[c][i] = fmaf(i < 2 ? f0 : f1, n[i], x[c][i]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
             for (int h = 0; h < H; ++h) vg[u][i][h] = 0;
           }
     }
-    // ---- running softmax; the accumulators are corrected only where a maximum or the unit moved
+    // ---- running softmax; the accumulators are corrected only where a maximum has grown by more than kSlack or the unit moved
     float mx = m;
     uint32_t most = 0;
 #pragma unroll
@@ -370,9 +376,8 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
       }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float zero = mx == -INFINITY ? 0.f : mx;
-    if (__any_sync(0xffffffffu, mx != m || most >= bound)) {
-      const float corr = ex2(m - zero);
+    if (__any_sync(0xffffffffu, mx > m + kSlack || most >= bound)) {
+      const float corr = ex2(m - (mx == -INFINITY ? 0.f : mx));
       l *= corr;
 #pragma unroll
       for (int h = 0; h < H; ++h) z[h] *= corr;
@@ -398,7 +403,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
 #pragma unroll
       for (int j = 0; j < 4 * H; ++j) { o[j][0] *= ce * f; o[j][1] *= co * f; o[j][2] *= ce * f; o[j][3] *= co * f; }
     }
-    const float into = power2(14 - top);
+    const float into = power2(14 - (int)kSlack - top), zero = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float w[4];
@@ -458,7 +463,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i][j] = o[4 * h + j][i] * 64.f * power2(top);      // 2^20 of the subnormals, 2^-14 of the weights
+        x[i][j] = o[4 * h + j][i] * 1024.f * power2(top);    // 2^20 of the subnormals, 2^-10 of the weights
         if constexpr (REP == 2 || REP == 4) x[i][j] += __shfl_xor_sync(0xffffffffu, x[i][j], REP / 2);
       }
       if constexpr (REP == 1) { x[0][j] += x[1][j]; x[2][j] += x[3][j]; }

@@ -15,6 +15,8 @@
 #pragma once
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace q4 {
 
 constexpr int kRows = 16;            // rows of a tile
@@ -41,12 +43,14 @@ template <typename T> RB_DEVICE uint32_t bits16(float x) {
   const T v = rb::from_f<T>(x);
   return *reinterpret_cast<const uint16_t*>(&v);
 }
-template <typename T> RB_DEVICE float from_bits16(uint32_t b) {
-  const uint16_t h = (uint16_t)b;
-  return rb::to_f(*reinterpret_cast<const T*>(&h));
+template <typename T> RB_DEVICE float scale_of(uint32_t w) {
+  if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) return __uint_as_float(w & 0xffff0000u);   // (bf16: fp32's upper half)
+  return __high2float(*reinterpret_cast<const __half2*>(&w));
 }
-template <typename T> RB_DEVICE float scale_of(uint32_t w) { return from_bits16<T>(w >> 16); }
-template <typename T> RB_DEVICE float low_of(uint32_t w) { return from_bits16<T>(w & 0xffffu); }
+template <typename T> RB_DEVICE float low_of(uint32_t w) {
+  if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) return __uint_as_float(w << 16);
+  return __low2float(*reinterpret_cast<const __half2*>(&w));
+}
 
 // The group word of a group whose extremes are lo and hi; a group that holds an infinity or a NaN is NaN throughout.  Everything is taken by 1/16, an exact factor,
 // so that the widest group of bf16 does not leave fp32.
