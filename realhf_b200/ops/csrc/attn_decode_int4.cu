@@ -44,6 +44,13 @@ RB_DEVICE void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32
   asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c));
 }
+// [16 x 8] times [8 x 8] of the model's type
+template <typename T> RB_DEVICE void mma_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};" : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b));
+  else
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};" : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b));
+}
 // The codes in nibble i of both halves of a word, in bits 4 .. 7: as fp16 2^-20 times the codes.
 RB_DEVICE uint32_t nibbles(uint32_t w, int i) { return (i == 0 ? w << 4 : w >> (4 * i - 4)) & 0x00f000f0u; }
 template <int N> RB_DEVICE void ld_words(uint32_t (&w)[N], uint32_t addr) {
@@ -116,9 +123,10 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   extern __shared__ __align__(128) unsigned char ring[];
   __shared__ __align__(8) uint64_t bar[kWarps][NS];
   __shared__ uint32_t dead_flag;
-  __shared__ __align__(16) uint32_t sbytes[kWarps][4][REP][D / 4 + 2];   // the queries' three bytes, lowest first, and zeros
+  __shared__ __align__(16) uint32_t sbytes[kWarps][3][REP][D / 4 + 2];   // the queries' three bytes, lowest first
+  __shared__ uint16_t ssums[kWarps][3][REP][J];                     // their sums over a key group in three parts of the model's type
   __shared__ __align__(16) float sk[kWarps][D], sv[kWarps][D];      // the new token's key and value as the cache holds them
-  __shared__ float s_unit[kWarps][REP], s_qsum[kWarps][REP][J];     // the queries' power of two inverted; their sums over a key group, in base-2 units
+  __shared__ float s_unit[kWarps][REP];                             // the queries' power of two inverted
   __shared__ float sm_m[kWarps][REP], sm_l[kWarps][REP], sm_z[kWarps][H][REP], sm_new[kWarps][REP];
   __shared__ float cta_m[REP], cta_l[REP], cta_acc[REP][D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -229,9 +237,17 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     }
     const int ex = (int)(__float_as_uint(most) >> 23), up = max(min(21 + 127 - ex, 100), -100);
     if (r < REP) {                                   // (heads beyond the set repeat its last one and are not stored)
-      if (sub % 4 == 0) s_qsum[warp][r][sub / 4] = sum;
       if (sub == 0) { s_unit[warp][r] = ex == 255 ? __int_as_float(0x7fc00000) : power2(-up); sm_new[warp][r] = dot; }   // (an infinity or a NaN: every score is NaN)
       const float f = power2(up);
+      if (sub % 4 == 0) {
+        float rest = sum * power2(up - 12);          // 32 numbers below 2^22: below 2^15
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+          const T x = rb::from_f<T>(rest);
+          ssums[warp][d][r][sub / 4] = *reinterpret_cast<const uint16_t*>(&x);
+          rest -= rb::to_f(x);
+        }
+      }
       uint32_t bytes[3][2] = {};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -241,7 +257,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
         bytes[2][e / 4] |= (uint32_t)(uint8_t)d2 << (8 * (e & 3));
       }
 #pragma unroll
-      for (int d = 0; d < 4; ++d) *reinterpret_cast<uint2*>(&sbytes[warp][d][r][sub * 2]) = d < 3 ? make_uint2(bytes[d][0], bytes[d][1]) : make_uint2(0u, 0u);
+      for (int d = 0; d < 3; ++d) *reinterpret_cast<uint2*>(&sbytes[warp][d][r][sub * 2]) = make_uint2(bytes[d][0], bytes[d][1]);
     }
   }
   __syncwarp();
@@ -249,12 +265,17 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   // ---- the queries as column operands: column g of product c is (byte, head g % REP); of the weights, (part g / REP, head g % REP): columns beyond the parts are never looked at
   const int head = g % REP, part = min(g / REP, 1);
   auto byte_of = [](int c, int col) { return min(REP == 8 ? c : REP == 4 ? 2 * c + col / 4 : col / REP, 3); };
-  uint32_t qb[J][kScores][2];
-  float unit[kScores][2], qs[J][2];                 // of the columns 2t, 2t + 1: the unit, and the sums of the queries (beside the lowest byte alone)
+  uint32_t qb[J][kScores][2], sb[kScores];          // sb: the sums of group t
+  float unit[kScores][2], unit_low[2];              // of the columns 2t, 2t + 1
 #pragma unroll
   for (int c = 0; c < kScores; ++c) {
+    const int mine = byte_of(c, g);
 #pragma unroll
-    for (int j = 0; j < J; ++j) ld_words(qb[j][c], ptx::smem_u32(&sbytes[warp][byte_of(c, g)][head][8 * j + 2 * t]));
+    for (int j = 0; j < J; ++j) {
+      ld_words(qb[j][c], ptx::smem_u32(&sbytes[warp][min(mine, 2)][head][8 * j + 2 * t]));
+      if (mine > 2) qb[j][c][0] = qb[j][c][1] = 0;
+    }
+    sb[c] = mine < 3 && t < J ? ssums[warp][mine][head][t % J] : 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int byte = byte_of(c, 2 * t + i);
@@ -262,17 +283,15 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < J; ++j) qs[j][i] = 2 * t + i < REP ? s_qsum[warp][(2 * t + i) % REP][j] : 0.f;
+  for (int i = 0; i < 2; ++i) unit_low[i] = s_unit[warp][(2 * t + i) % REP] * 4096.f;
 
   float o[4 * H][4];
 #pragma unroll
   for (int j = 0; j < 4 * H; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m = -INFINITY, l = 0.f, z[H];               // of head `head`, over the lane's keys: maximum, sum of weights, sums of weights times lowest values
+  float m = -INFINITY, l = 0.f, z[H];               // of head `head`, over the lane's keys: maximum, sum of weights, sums of weights times lowest values, in the weights' unit
 #pragma unroll
   for (int h = 0; h < H; ++h) z[h] = 0.f;
-  int top = -100;                                   // scaled weights are in units of 2^(top - 10); every scale so far is below 2^top
+  int top = -100;                                   // weights are in units of 2^(top - 10); every value scale so far is below 2^top
   uint32_t bound = 0;                               // the group word of that scale
   int slot = 0;
   uint32_t round = 0;                               // parity of the ring's current round
@@ -290,9 +309,16 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
       ld_words(s0, at + u * Tl::kBytes + Tl::kKeyScales * 4 + g * (J * 4));
       ld_words(s1, at + u * Tl::kBytes + Tl::kKeyScales * 4 + (g + 8) * (J * 4));
       float x[kScores][4] = {}, y[4] = {};
+      {
+        uint32_t a0, a1;                            // the group words as operands: lowest values, and scales that meet zeros
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(a0) : "r"(at + u * Tl::kBytes + Tl::kKeyScales * 4 + g * (J * 4) + t % J * 4) : "memory");
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(a1) : "r"(at + u * Tl::kBytes + Tl::kKeyScales * 4 + (g + 8) * (J * 4) + t % J * 4) : "memory");
+#pragma unroll
+        for (int c = 0; c < kScores; ++c) mma_k8<T>(y, a0, a1, sb[c]);
+      }
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const float f0 = q4::scale_of<T>(s0[j]), f1 = q4::scale_of<T>(s1[j]), l0 = q4::low_of<T>(s0[j]), l1 = q4::low_of<T>(s1[j]);
+        const float f0 = q4::scale_of<T>(s0[j]), f1 = q4::scale_of<T>(s1[j]);
         constexpr uint32_t kLow = 0x0f0f0f0fu;
 #pragma unroll
         for (int c = 0; c < kScores; ++c) {
@@ -306,14 +332,11 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[c][i] = fmaf(i < 2 ? f0 : f1, n[i], x[c][i]);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (REP > 1 || i % 2 == 0) y[i] = fmaf(i < 2 ? l0 : l1, qs[j][i & 1], y[i]);
       }
       float v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[i] = fmaf(x[0][i], unit[0][i & 1], y[i]);
+        v[i] = fmaf(x[0][i], unit[0][i & 1], y[i] * unit_low[i & 1]);
 #pragma unroll
         for (int c = 1; c < kScores; ++c) v[i] = fmaf(x[c][i], unit[c][i & 1], v[i]);
       }
@@ -377,11 +400,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     if (__any_sync(0xffffffffu, mx > m + kSlack || most >= bound)) {
-      const float corr = ex2(m - (mx == -INFINITY ? 0.f : mx));
-      l *= corr;
-#pragma unroll
-      for (int h = 0; h < H; ++h) z[h] *= corr;
-      const float ce = __shfl_sync(0xffffffffu, corr, 8 * t), co = __shfl_sync(0xffffffffu, corr, 8 * t + 4);   // of columns 2t, 2t + 1
+      float corr = ex2(m - (mx == -INFINITY ? 0.f : mx));
       m = mx;
       constexpr uint32_t kNan = std::is_same<T, __half>::value ? 0x7c000000u : 0x7f800000u;   // infinities and NaN: no unit holds them
       most = 0;
@@ -392,18 +411,21 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
 #pragma unroll
           for (int h = 0; h < H; ++h) most = max(most, vg[u][i][h] < kNan ? vg[u][i][h] : 0u);
       most = __reduce_max_sync(0xffffffffu, most);
-      float f = 1.f;
       if (most >= bound) {                          // two bits of room, so that it seldom moves
         constexpr int kShift = std::is_same<T, __half>::value ? 26 : 23, kBias = std::is_same<T, __half>::value ? 15 : 127;
         const int ex = min((int)(most >> kShift) + 3, (int)(kNan >> kShift)), was = top;
         top = max(min(ex - kBias, 127), -100);
         bound = (uint32_t)ex << kShift;
-        f = power2(max(was - top, -126));
+        corr *= power2(max(was - top, -126));
       }
+      l *= corr;
 #pragma unroll
-      for (int j = 0; j < 4 * H; ++j) { o[j][0] *= ce * f; o[j][1] *= co * f; o[j][2] *= ce * f; o[j][3] *= co * f; }
+      for (int h = 0; h < H; ++h) z[h] *= corr;
+      const float ce = __shfl_sync(0xffffffffu, corr, 8 * t), co = __shfl_sync(0xffffffffu, corr, 8 * t + 4);   // of columns 2t, 2t + 1
+#pragma unroll
+      for (int j = 0; j < 4 * H; ++j) { o[j][0] *= ce; o[j][1] *= co; o[j][2] *= ce; o[j][3] *= co; }
     }
-    const float into = power2(14 - (int)kSlack - top), zero = m == -INFINITY ? 0.f : m;
+    const float zero = (m == -INFINITY ? 0.f : m) - (float)(14 - (int)kSlack - top);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float w[4];
@@ -417,7 +439,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t g0 = vg[u][2 * e][h], g1 = vg[u][2 * e + 1][h];
-          const float a = w[2 * e] * into * q4::scale_of<T>(g0), c = w[2 * e + 1] * into * q4::scale_of<T>(g1);
+          const float a = w[2 * e] * q4::scale_of<T>(g0), c = w[2 * e + 1] * q4::scale_of<T>(g1);
           z[h] = fmaf(w[2 * e], q4::low_of<T>(g0), z[h]);
           z[h] = fmaf(w[2 * e + 1], q4::low_of<T>(g1), z[h]);
           const uint32_t p0 = pack2<__half>(a, c);
@@ -450,11 +472,12 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     z[h] += __shfl_xor_sync(0xffffffffu, z[h], 1);
     z[h] += __shfl_xor_sync(0xffffffffu, z[h], 2);
   }
+  const float back = power2(top - 14 + (int)kSlack);
   if (g < REP && t == 0) {
     sm_m[warp][head] = m;
-    sm_l[warp][head] = l;
+    sm_l[warp][head] = l * back;
 #pragma unroll
-    for (int h = 0; h < H; ++h) sm_z[warp][h][head] = z[h];
+    for (int h = 0; h < H; ++h) sm_z[warp][h][head] = z[h] * back;
   }
 #pragma unroll
   for (int h = 0; h < H; ++h) {
@@ -463,7 +486,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i][j] = o[4 * h + j][i] * 1024.f * power2(top);    // 2^20 of the subnormals, 2^-10 of the weights
+        x[i][j] = o[4 * h + j][i] * 1048576.f * back;        // 2^20 of the subnormals
         if constexpr (REP == 2 || REP == 4) x[i][j] += __shfl_xor_sync(0xffffffffu, x[i][j], REP / 2);
       }
       if constexpr (REP == 1) { x[0][j] += x[1][j]; x[2][j] += x[3][j]; }
