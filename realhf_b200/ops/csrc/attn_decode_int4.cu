@@ -105,10 +105,11 @@ template <int D> RB_DEVICE void rotate8(float (&x)[8], int sub, const Turn& t, c
   } else {
     const int off = half / 8;                  // the partner channel is `half` away: so many lanes
     const bool first = d0 < half, active = d0 < p.rot_dim;
+    const int from = !active ? sub : first ? sub + off : sub - off;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float up = __shfl_down_sync(0xffffffffu, x[i], off, D / 8), dn = __shfl_up_sync(0xffffffffu, x[i], off, D / 8);
-      if (active) x[i] = first ? __fsub_rn(__fmul_rn(x[i], t.c[i]), __fmul_rn(up, t.s[i])) : __fadd_rn(__fmul_rn(x[i], t.c[i]), __fmul_rn(dn, t.s[i]));
+      const float other = __shfl_sync(0xffffffffu, x[i], from, D / 8), a = __fmul_rn(x[i], t.c[i]), b = __fmul_rn(other, t.s[i]);
+      if (active) x[i] = first ? __fsub_rn(a, b) : __fadd_rn(a, b);
     }
   }
 }
@@ -125,10 +126,11 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   __shared__ uint32_t dead_flag;
   __shared__ __align__(16) uint32_t sbytes[kWarps][3][REP][D / 4 + 2];   // the queries' three bytes, lowest first
   __shared__ uint16_t ssums[kWarps][3][REP][J];                     // their sums over a key group in three parts of the model's type
-  __shared__ __align__(16) float sk[kWarps][D], sv[kWarps][D];      // the new token's key and value as the cache holds them
   __shared__ float s_unit[kWarps][REP];                             // the queries' power of two inverted
-  __shared__ float sm_m[kWarps][REP], sm_l[kWarps][REP], sm_z[kWarps][H][REP], sm_new[kWarps][REP];
-  __shared__ float cta_m[REP], cta_l[REP], cta_acc[REP][D];
+  __shared__ float sm_m[kWarps][REP], sm_l[kWarps][REP], sm_z[kWarps][H][REP];
+  __shared__ uint2 s_new[kWarps][32];                               // the new row: a lane's word and its group's
+  __shared__ float cta_m[REP], cta_l[REP];
+  __shared__ __align__(16) float cta_acc[REP][D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   volatile uint32_t* dead = &dead_flag;
   if (threadIdx.x == 0) *dead = 0;
@@ -144,20 +146,20 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   const int b = (int)(work / (p.nkv * sets)), hkv = (int)(work / sets % p.nkv), h0 = (int)(work % sets) * REP, heads = min(REP, rep - h0);
   const int share = blockIdx.y * p.wide + warp % p.wide, shares = p.splits * p.wide;
   const int len = p.lens[b], pos = len < p.room ? len : -1;
-  const bool live = pos >= 0 && at_work < all, first = share == 0;
-  // ---- its queries (a group of D / 8 lanes has one) and, for the first share, the new key and value; asked for ahead of the tiles
+  const bool live = pos >= 0 && at_work < all;
+  // ---- its queries (a group of D / 8 lanes has one; the warps of a work share them) and the new key and value, asked for ahead of the tiles
   const T* qkv = reinterpret_cast<const T*>(p.qkv) + b * p.qkv_stride;
-  const int sub = lane % LPR;
+  const int sub = lane % LPR, wi = warp % p.wide, w0 = warp - wi;
   float xn[kTurns][8], kv[8];
 #pragma unroll
-  for (int i = 0; i < kTurns; ++i) load8(qkv + (int64_t)(hkv * rep + h0 + min(lane / LPR + i * RPT, heads - 1)) * D + sub * 8, xn[i]);
-  const bool of_value = lane / LPR % 2;             // of the new token, lanes of even rows have the key, of odd rows the value
-  if (first) load8(qkv + (int64_t)(p.nq + (of_value ? p.nkv : 0) + hkv) * D + sub * 8, kv);
+  for (int i = 0; i < kTurns; ++i)
+    if (i % p.wide == wi) load8(qkv + (int64_t)(hkv * rep + h0 + min(lane / LPR + i * RPT, heads - 1)) * D + sub * 8, xn[i]);
+  // steps of two tiles of the rows [0, pos]; who has the last one has the new row: of it lanes of even groups have the key, of odd ones the value
+  const int n_tiles = live ? pos / 16 + 1 : 0, n_steps = (n_tiles + 1) / 2;
+  const bool fresh = live && (n_steps - 1) % shares == share, of_value = lane / LPR % 2;
+  if (fresh) load8(qkv + (int64_t)(p.nq + (of_value ? p.nkv : 0) + hkv) * D + sub * 8, kv);
   Turn turn;
   if (p.cos && live) load_turn(turn, sub, p, pos);
-
-  // ---- this share's steps of the cached rows [0, pos) (the new one is handled from registers); the first of them are asked for
-  const int n_tiles = live ? RB_CEIL_DIV(pos, 16) : 0, n_steps = (n_tiles + 1) / 2;
   uint32_t* cache = p.cache + ((int64_t)b * p.nkv + hkv) * p.tiles * Tl::kWords;
   const uint32_t base = ptx::smem_u32(ring) + warp * (uint32_t)kRing;
   auto fetch = [&](int step, int slot) {
@@ -171,7 +173,53 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
 #pragma unroll
   for (int n = 0; n < NS; ++n) fetch(share + n * shares, n);
 
-  if (first) {                                      // the new row: quantised, written, and its numbers as the cache holds them
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    if (i % p.wide != wi) continue;
+    const int r = lane / LPR + i * RPT;
+    if (p.cos) rotate8<D>(xn[i], sub, turn, p);
+    // sums over the key groups, then whole numbers: the largest element to 2^21 .. 2^22
+    float sum = 0.f, most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      xn[i][e] *= p.scale;
+      sum += xn[i][e];
+      most = q4::max_nan(most, fabsf(xn[i][e]));
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) most = q4::max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const int ex = (int)(__float_as_uint(most) >> 23), up = max(min(21 + 127 - ex, 100), -100);
+    if (r < REP) {                                   // (heads beyond the set repeat its last one and are not stored)
+      if (sub == 0) s_unit[w0][r] = ex == 255 ? __int_as_float(0x7fc00000) : power2(-up);   // (an infinity or a NaN: every score is NaN)
+      if (sub % 4 == 0) {
+        float rest = sum * power2(up - 12);          // 32 numbers below 2^22: below 2^15
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+          const T x = rb::from_f<T>(rest);
+          ssums[w0][d][r][sub / 4] = *reinterpret_cast<const uint16_t*>(&x);
+          rest -= rb::to_f(x);
+        }
+      }
+      // n = d0 + 256 d1 + 65536 d2 with signed bytes: the bytes of n + 0x808080, each less 128.  n is read off the last bits of 1.5 2^23 + n.
+      uint32_t n[8];
+      const float f = power2(up);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) n[e] = __float_as_uint(fmaf(xn[i][e], f, 12582912.f)) + (0x808080u - 0x4b400000u);
+      uint32_t bytes[3][2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t a = __byte_perm(n[4 * q], n[4 * q + 1], 0x5140), c = __byte_perm(n[4 * q + 2], n[4 * q + 3], 0x5140);
+        bytes[0][q] = __byte_perm(a, c, 0x5410) ^ 0x80808080u;
+        bytes[1][q] = __byte_perm(a, c, 0x7632) ^ 0x80808080u;
+        bytes[2][q] = __byte_perm(__byte_perm(n[4 * q], n[4 * q + 1], 0x0062), __byte_perm(n[4 * q + 2], n[4 * q + 3], 0x0062), 0x5410) ^ 0x80808080u;
+      }
+#pragma unroll
+      for (int d = 0; d < 3; ++d) *reinterpret_cast<uint2*>(&sbytes[w0][d][r][sub * 2]) = make_uint2(bytes[d][0], bytes[d][1]);
+    }
+  }
+  if (fresh) {                                      // the new row: quantised and written; it goes into the last tile when that has come
     if (p.cos) {
       float turned[8];
 #pragma unroll
@@ -183,84 +231,28 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     float klo, khi;
     q4::extremes<4>(kv, klo, khi);
     const float vlo = q4::min_nan(klo, __shfl_xor_sync(0xffffffffu, klo, 4)), vhi = q4::max_nan(khi, __shfl_xor_sync(0xffffffffu, khi, 4));
-    const uint32_t gw = q4::group_word<T>(of_value ? vlo : klo, of_value ? vhi : khi);
-    const float scale = q4::scale_of<T>(gw), low = q4::low_of<T>(gw);
-    uint32_t code[8], kw = 0, vw = 0;
-    q4::codes8(kv, scale, low, code);
+    const uint32_t new_group = q4::group_word<T>(of_value ? vlo : klo, of_value ? vhi : khi);
+    uint32_t code[8], new_word = 0;
+    q4::codes8(kv, q4::scale_of<T>(new_group), q4::low_of<T>(new_group), code);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      kw |= code[e] << q4::bit_of<q4::kKey>(e);
-      vw |= code[e] << q4::bit_of<q4::kValue>(e);
-      kv[e] = fmaf(scale, (float)code[e], low);
-    }
-    if (live && h0 == 0 && lane < 2 * LPR) {
-      uint32_t* at = cache + (int64_t)(pos / 16) * Tl::kWords;
-      const int r = pos % 16;
-      if (of_value) {
-        uint16_t* halves = reinterpret_cast<uint16_t*>(at + Tl::kValues) + q4::half_place(sub, r);
-        halves[0] = (uint16_t)vw;
-        halves[2] = (uint16_t)(vw >> 16);
-      } else {
-        at[r * Tl::W + q4::word_place<J>(sub)] = kw;
-      }
-      if (sub % (of_value ? 8 : 4) == 0) at[of_value ? Tl::kValueScales + r * H + sub / 8 : Tl::kKeyScales + r * J + sub / 4] = gw;
-    }
-    if (lane < 2 * LPR) {
-      float* to = of_value ? sv[warp] : sk[warp];
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) *reinterpret_cast<float4*>(to + sub * 8 + e) = make_float4(kv[e], kv[e + 1], kv[e + 2], kv[e + 3]);
-    }
-    __syncwarp();
+    for (int e = 0; e < 8; ++e) new_word |= code[e] << (of_value ? q4::bit_of<q4::kValue>(e) : q4::bit_of<q4::kKey>(e));
+    s_new[warp][lane] = make_uint2(new_word, new_group);
   }
-#pragma unroll
-  for (int i = 0; i < kTurns; ++i) {
-    const int r = lane / LPR + i * RPT;
-    if (p.cos) rotate8<D>(xn[i], sub, turn, p);
-    // sums over the key groups, the new row's score, then whole numbers: the largest element to 2^21 .. 2^22
-    float sum = 0.f, most = 0.f, dot = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      xn[i][e] *= p.scale;
-      sum += xn[i][e];
-      most = q4::max_nan(most, fabsf(xn[i][e]));
+  auto put_row = [&](uint32_t* tile) {              // the new row's words and groups into its tile, in global or in shared memory
+    const int r = pos % 16;
+    const uint32_t new_word = s_new[warp][lane].x, new_group = s_new[warp][lane].y;
+    if (lane >= 2 * LPR) return;
+    if (of_value) {
+      uint16_t* halves = reinterpret_cast<uint16_t*>(tile + Tl::kValues) + q4::half_place(sub, r);
+      halves[0] = (uint16_t)new_word;
+      halves[2] = (uint16_t)(new_word >> 16);
+    } else {
+      tile[r * Tl::W + q4::word_place<J>(sub)] = new_word;
     }
-    if (first) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dot = fmaf(xn[i][e], sk[warp][sub * 8 + e], dot);
-    }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) {
-      most = q4::max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-      dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    }
-    const int ex = (int)(__float_as_uint(most) >> 23), up = max(min(21 + 127 - ex, 100), -100);
-    if (r < REP) {                                   // (heads beyond the set repeat its last one and are not stored)
-      if (sub == 0) { s_unit[warp][r] = ex == 255 ? __int_as_float(0x7fc00000) : power2(-up); sm_new[warp][r] = dot; }   // (an infinity or a NaN: every score is NaN)
-      const float f = power2(up);
-      if (sub % 4 == 0) {
-        float rest = sum * power2(up - 12);          // 32 numbers below 2^22: below 2^15
-#pragma unroll
-        for (int d = 0; d < 3; ++d) {
-          const T x = rb::from_f<T>(rest);
-          ssums[warp][d][r][sub / 4] = *reinterpret_cast<const uint16_t*>(&x);
-          rest -= rb::to_f(x);
-        }
-      }
-      uint32_t bytes[3][2] = {};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int n = __float2int_rn(xn[i][e] * f), d0 = (int8_t)n, n1 = (n - d0) >> 8, d1 = (int8_t)n1, d2 = (n1 - d1) >> 8;
-        bytes[0][e / 4] |= (uint32_t)(uint8_t)d0 << (8 * (e & 3));
-        bytes[1][e / 4] |= (uint32_t)(uint8_t)d1 << (8 * (e & 3));
-        bytes[2][e / 4] |= (uint32_t)(uint8_t)d2 << (8 * (e & 3));
-      }
-#pragma unroll
-      for (int d = 0; d < 3; ++d) *reinterpret_cast<uint2*>(&sbytes[warp][d][r][sub * 2]) = make_uint2(bytes[d][0], bytes[d][1]);
-    }
-  }
-  __syncwarp();
+    if (sub % (of_value ? 8 : 4) == 0) tile[of_value ? Tl::kValueScales + r * H + sub / 8 : Tl::kKeyScales + r * J + sub / 4] = new_group;
+  };
+  if (fresh && h0 == 0) put_row(cache + (int64_t)(pos / 16) * Tl::kWords);
+  if (p.wide == 1) __syncwarp(); else __syncthreads();
 
   // ---- the queries as column operands: column g of product c is (byte, head g % REP); of the weights, (part g / REP, head g % REP): columns beyond the parts are never looked at
   const int head = g % REP, part = min(g / REP, 1);
@@ -272,18 +264,18 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     const int mine = byte_of(c, g);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      ld_words(qb[j][c], ptx::smem_u32(&sbytes[warp][min(mine, 2)][head][8 * j + 2 * t]));
+      ld_words(qb[j][c], ptx::smem_u32(&sbytes[w0][min(mine, 2)][head][8 * j + 2 * t]));
       if (mine > 2) qb[j][c][0] = qb[j][c][1] = 0;
     }
-    sb[c] = mine < 3 && t < J ? ssums[warp][mine][head][t % J] : 0;
+    sb[c] = mine < 3 && t < J ? ssums[w0][mine][head][t % J] : 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int byte = byte_of(c, 2 * t + i);
-      unit[c][i] = byte < 3 ? s_unit[warp][(2 * t + i) % REP] * (byte == 0 ? 1.f : byte == 1 ? 256.f : 65536.f) : 0.f;
+      unit[c][i] = byte < 3 ? s_unit[w0][(2 * t + i) % REP] * (byte == 0 ? 1.f : byte == 1 ? 256.f : 65536.f) : 0.f;
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) unit_low[i] = s_unit[warp][(2 * t + i) % REP] * 4096.f;
+  for (int i = 0; i < 2; ++i) unit_low[i] = s_unit[w0][(2 * t + i) % REP] * 4096.f;
 
   float o[4 * H][4];
 #pragma unroll
@@ -299,6 +291,10 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   for (int step = share; step < n_steps; step += shares) {
     bounded_wait(ptx::smem_u32(&bar[warp][slot]), round, dead);
     const uint32_t at = base + slot * (2 * Tl::kBytes);
+    if (fresh && step == n_steps - 1) {
+      put_row(reinterpret_cast<uint32_t*>(ring + warp * kRing + slot * (2 * Tl::kBytes)) + (pos / 16 - 2 * step) * Tl::kWords);
+      __syncwarp();
+    }
     // ---- scores of 2 x 16 keys: lane (g, t) gets keys g and g + 8 of columns 2t and 2t + 1, then the keys 2t, 2t + 1, 2t + 8, 2t + 9 of head g % REP
     float s[2][4];
 #pragma unroll
@@ -375,12 +371,12 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
 #pragma unroll
         for (int h = 0; h < H; ++h) { vg[u][i][h] = a[i * H + h]; vg[u][2 + i][h] = c[i * H + h]; }
     }
-    if (step * 32 + 32 > pos) {                     // rows behind the length may hold anything
+    if (step * 32 + 32 > pos + 1) {                    // rows behind the length may hold anything
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (step * 32 + u * 16 + 2 * t + (i & 1) + (i >> 1) * 8 >= pos) {
+          if (step * 32 + u * 16 + 2 * t + (i & 1) + (i >> 1) * 8 > pos) {
             s[u][i] = -INFINITY;
 #pragma unroll
             for (int h = 0; h < H; ++h) vg[u][i][h] = 0;
@@ -472,7 +468,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     z[h] += __shfl_xor_sync(0xffffffffu, z[h], 1);
     z[h] += __shfl_xor_sync(0xffffffffu, z[h], 2);
   }
-  const float back = power2(top - 14 + (int)kSlack);
+  const float back = power2(top - 14 + (int)kSlack), up = back * 1048576.f;   // 2^20 of the subnormals
   if (g < REP && t == 0) {
     sm_m[warp][head] = m;
     sm_l[warp][head] = l * back;
@@ -486,7 +482,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i][j] = o[4 * h + j][i] * 1048576.f * back;        // 2^20 of the subnormals
+        x[i][j] = o[4 * h + j][i] * up;
         if constexpr (REP == 2 || REP == 4) x[i][j] += __shfl_xor_sync(0xffffffffu, x[i][j], REP / 2);
       }
       if constexpr (REP == 1) { x[0][j] += x[1][j]; x[2][j] += x[3][j]; }
@@ -503,23 +499,30 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     }
   }
   if (p.wide == 1) __syncwarp(); else __syncthreads();
-  const int w0 = warp / p.wide * p.wide;            // the work's first warp
-  const bool fresh = blockIdx.y == 0;               // its share 0 is here: the new row is one more set of sums
   T* out = reinterpret_cast<T*>(p.out) + (int64_t)b * p.nq * D + (int64_t)(hkv * rep + h0) * D;
-  for (int idx = (warp - w0) * 32 + lane; idx < heads * D; idx += p.wide * 32) {
-    const int r = idx / D, d = idx % D;
-    float mg = fresh ? sm_new[w0][r] : -INFINITY;
+  auto write4 = [&](int at4, const float (&a)[4], float l4) {
+    rb::Pack<T, 4> x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.v[i] = rb::from_f<T>(live ? a[i] / l4 : 0.f);
+    *reinterpret_cast<rb::Pack<T, 4>*>(out + at4 * 4) = x;
+  };
+  for (int c4 = wi * 32 + lane; c4 < heads * (D / 4); c4 += p.wide * 32) {   // four channels a lane
+    const int r = c4 / (D / 4), d = c4 % (D / 4) * 4;
+    float mg = -INFINITY, lg = 0.f, ag[4] = {};
     for (int w = w0; w < w0 + p.wide; ++w) mg = fmaxf(mg, sm_m[w][r]);
-    float lg = fresh ? ex2(sm_new[w0][r] - mg) : 0.f, ag = fresh ? sv[w0][d] * lg : 0.f;
     for (int w = w0; w < w0 + p.wide; ++w) {
-      const float c = sm_m[w][r] == -INFINITY ? 0.f : ex2(sm_m[w][r] - mg);
+      const float c = sm_m[w][r] == -INFINITY ? 0.f : ex2(sm_m[w][r] - mg), zw = sm_z[w][d / 64][r];
+      const float4 x = reinterpret_cast<const float4*>(ring + w * kRing)[c4];
       lg = fmaf(sm_l[w][r], c, lg);
-      ag = fmaf(reinterpret_cast<const float*>(ring + w * kRing)[idx] + sm_z[w][d / 64][r], c, ag);
+      ag[0] = fmaf(x.x + zw, c, ag[0]);
+      ag[1] = fmaf(x.y + zw, c, ag[1]);
+      ag[2] = fmaf(x.z + zw, c, ag[2]);
+      ag[3] = fmaf(x.w + zw, c, ag[3]);
     }
     if (p.splits == 1) {
-      if (at_work < all) out[idx] = rb::from_f<T>(live ? ag / lg : 0.f);
+      if (at_work < all) write4(c4, ag, lg);
     } else {
-      cta_acc[r][d] = ag;
+      *reinterpret_cast<float4*>(&cta_acc[r][d]) = make_float4(ag[0], ag[1], ag[2], ag[3]);
       if (d == 0) { cta_m[r] = mg; cta_l[r] = lg; }
     }
   }
@@ -541,17 +544,24 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
     return f;
   };
-  for (int idx = blockIdx.y * kDecThreads + threadIdx.x; idx < heads * D; idx += p.splits * kDecThreads) {
-    const int r = idx / D, d = idx % D;
-    float mg = -INFINITY;
+  const int each = RB_CEIL_DIV(heads * (D / 4), p.splits);
+  for (int i = threadIdx.x; i < each; i += kDecThreads) {
+    const int c4 = blockIdx.y * each + i, r = c4 / (D / 4), d = c4 % (D / 4) * 4;
+    if (c4 >= heads * (D / 4)) break;
+    float mg = -INFINITY, lg = 0.f, ag[4] = {};
+#pragma unroll 4
     for (int c = 0; c < p.splits; ++c) mg = fmaxf(mg, peer(&cta_m[r], c));
-    float lg = 0.f, ag = 0.f;
+#pragma unroll 4
     for (int c = 0; c < p.splits; ++c) {
       const float mc = peer(&cta_m[r], c), w = mc == -INFINITY ? 0.f : ex2(mc - mg);
+      const float4 x = ptx::ld_cluster_f4(ptx::smem_u32(&cta_acc[r][d]), c);
       lg = fmaf(peer(&cta_l[r], c), w, lg);
-      ag = fmaf(peer(&cta_acc[r][d], c), w, ag);
+      ag[0] = fmaf(x.x, w, ag[0]);
+      ag[1] = fmaf(x.y, w, ag[1]);
+      ag[2] = fmaf(x.z, w, ag[2]);
+      ag[3] = fmaf(x.w, w, ag[3]);
     }
-    out[idx] = rb::from_f<T>(live ? ag / lg : 0.f);
+    write4(c4, ag, lg);
   }
   ptx::cluster_sync();  // nobody leaves while its sums are being read
 }
