@@ -31,6 +31,7 @@ struct StepParams {
   const float *cos, *sin;   // [room or more, rot_dim / 2] or null
   int64_t qkv_stride;
   int B, nq, nkv, room, tiles, rot_dim, interleaved;
+  int longest_first;
   int wide, splits;         // warps of a block, blocks of a cluster that share the rows of one (sequence, kv head, set of query heads)
   float scale;              // times log2 e
   int* status;              // rb_attn_status()
@@ -63,6 +64,39 @@ template <int N> RB_DEVICE void ld_words(uint32_t (&w)[N], uint32_t addr) {
 RB_DEVICE float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }   // 2^x, 2 ulp
 RB_DEVICE float2 unpack_half2(uint32_t r) { return __half22float2(*reinterpret_cast<const __half2*>(&r)); }
 RB_DEVICE float power2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // e = -126 .. 127
+
+// The sequence that comes `rank`-th when the longest comes first: lengths in 32 classes, sequences of one class in their order.  A whole warp; B <= kRanked.
+constexpr int kRanked = 256;
+RB_DEVICE int sequence_of(const int* lens, int B, int room, int rank, int& len) {
+  const int lane = threadIdx.x & 31, down = max(27 - __clz(room), 0);      // classes 0 .. 31
+  int raw[kRanked / 32], v[kRanked / 32];
+#pragma unroll
+  for (int j = 0; j < kRanked / 32; ++j) raw[j] = j * 32 + lane < B ? lens[j * 32 + lane] : 0;
+#pragma unroll
+  for (int j = 0; j < kRanked / 32; ++j) v[j] = j * 32 + lane < B ? min(max(raw[j], 0), room) >> down : -1;
+  int cls = 0, before = 0;                          // the class of that sequence: the largest with more than `rank` sequences in it and above
+#pragma unroll
+  for (int bit = 16; bit > 0; bit >>= 1) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < kRanked / 32; ++j)
+      if (j * 32 < B) n += __popc(__ballot_sync(0xffffffffu, v[j] >= cls + bit));
+    if (n > rank) cls += bit; else before = n;      // (`before` ends as the number of sequences above the class)
+  }
+  int left = rank - before, b = 0;
+#pragma unroll
+  for (int j = 0; j < kRanked / 32; ++j)
+    if (j * 32 < B) {
+      const uint32_t hit = __ballot_sync(0xffffffffu, v[j] == cls);
+      const uint32_t it = __ballot_sync(0xffffffffu, v[j] == cls && __popc(hit & ((1u << lane) - 1)) == left);
+      if (it != 0) {
+        b = j * 32 + __ffs(it) - 1;
+        len = __shfl_sync(0xffffffffu, raw[j], __ffs(it) - 1);
+      }
+      left -= __popc(hit);
+    }
+  return b;
+}
 
 template <typename T> RB_DEVICE void load8(const T* p, float (&f)[8]) {
   const rb::Pack<T, 8> v = *reinterpret_cast<const rb::Pack<T, 8>*>(p);
@@ -141,11 +175,13 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   rb::pdl_wait();
   // ---- the warp's work: share `share` of `shares` of the rows of one (sequence, kv head, set of REP query heads)
   const int rep = p.nq / p.nkv, sets = RB_CEIL_DIV(rep, REP);
-  const int64_t all = (int64_t)p.B * p.nkv * sets, at_work = (int64_t)blockIdx.x * (kWarps / p.wide) + warp / p.wide;
-  const int64_t work = min(at_work, all - 1);       // (the last block's warps beyond the work go along and store nothing)
-  const int b = (int)(work / (p.nkv * sets)), hkv = (int)(work / sets % p.nkv), h0 = (int)(work % sets) * REP, heads = min(REP, rep - h0);
+  const unsigned all = (unsigned)p.B * p.nkv * sets, at_work = blockIdx.x * (kWarps / p.wide) + warp / p.wide;
+  const unsigned work = min(at_work, all - 1), pair = work / sets, nth = pair / p.nkv;     // (the last block's warps beyond the work go along and store nothing)
+  const int hkv = (int)(pair % p.nkv), h0 = (int)(work % sets) * REP, heads = min(REP, rep - h0);
+  int b = nth, len;
+  if (p.longest_first) b = sequence_of(p.lens, p.B, p.room, nth, len); else len = p.lens[b];
   const int share = blockIdx.y * p.wide + warp % p.wide, shares = p.splits * p.wide;
-  const int len = p.lens[b], pos = len < p.room ? len : -1;
+  const int pos = len < p.room ? len : -1;
   const bool live = pos >= 0 && at_work < all;
   // ---- its queries (a group of D / 8 lanes has one; the warps of a work share them) and the new key and value, asked for ahead of the tiles
   const T* qkv = reinterpret_cast<const T*>(p.qkv) + b * p.qkv_stride;
@@ -602,6 +638,9 @@ template <typename T, int D> int launch(StepParams p, cudaStream_t s) {
   const int64_t works = (int64_t)p.B * p.nkv * RB_CEIL_DIV(rep, heads), places = (int64_t)rb::kNumSMs * ctas_of(heads) * kWarps;
   p.wide = p.splits = 1;
   while (p.wide * p.splits < kWarps * kMaxSplits && works * p.wide * p.splits * 2 <= places && p.tiles >= 8 * p.wide * p.splits) (p.wide < kWarps ? p.wide : p.splits) *= 2;
+  // The longest sequences first, where there are more works than places: the last to begin are short ones then.
+  p.longest_first = p.B > 1 && p.B <= kRanked && works > places;
+  if (works * p.wide > 0x7fffffff) return -1;
   return heads == 1 ? launch_one<T, D, 1>(p, s) : heads == 2 ? launch_one<T, D, 2>(p, s) : heads == 4 ? launch_one<T, D, 4>(p, s) : launch_one<T, D, 8>(p, s);
 }
 
@@ -611,7 +650,7 @@ template <typename T, int D> int launch(StepParams p, cudaStream_t s) {
 extern "C" int rb_decode_attention_int4(const void* qkv, void* cache, const int* lens, void* out, const float* cos, const float* sin, int64_t qkv_stride, int B, int nq,
                                         int nkv, int hd, int room, int rot_dim, int interleaved, float scale, int dt, cudaStream_t s) {
   if (B == 0) return 0;
-  const StepParams p{qkv, reinterpret_cast<uint32_t*>(cache), lens, out, cos, sin, qkv_stride, B, nq, nkv, room, (room + 15) / 16, rot_dim, interleaved, 1, 1,
+  const StepParams p{qkv, reinterpret_cast<uint32_t*>(cache), lens, out, cos, sin, qkv_stride, B, nq, nkv, room, (room + 15) / 16, rot_dim, interleaved, 0, 1, 1,
                  scale * 1.4426950408889634f, rb_attn_status()};
   if (p.status == nullptr) return -5;
   if (dt == 1 && hd == 128) return launch<__nv_bfloat16, 128>(p, s);

@@ -318,7 +318,8 @@ def test_decode_values_of_any_size(dtype, power):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("B,nq,nkv,hd,room", [(1, 8, 1, 128, 9000), (2, 4, 4, 64, 5001), (1, 32, 8, 128, 4096), (300, 2, 2, 64, 40), (64, 32, 32, 128, 130)])
+@pytest.mark.parametrize("B,nq,nkv,hd,room", [(1, 8, 1, 128, 9000), (2, 4, 4, 64, 5001), (1, 32, 8, 128, 4096), (300, 2, 2, 64, 40), (64, 32, 32, 128, 130), (200, 4, 4, 64, 300), (256, 8, 2, 128, 33),
+                                               (33, 64, 64, 64, 50)])
 def test_decode_long_and_wide(dtype, B, nq, nkv, hd, room):
     """Few long sequences (split over blocks) and many short ones."""
     g = torch.Generator().manual_seed(B + room)
