@@ -32,8 +32,15 @@ class GenerationHyperparameters:
     # B200 addition (no reference counterpart): decode with e4m3 weights / activations on the fp8 tensor cores.  Sampled
     # tokens and the returned log-probs are those of the quantised policy (see docs/generation_fp8.md).
     fp8_weights: bool = False
+    # B200 additions: keys and values held in 4 bits (4; 16: the model's type), and the decode loop's weights (docs/generation_int4.md)
+    kv_cache_bits: int = 16
+    int4_weights: bool = False
 
     def __post_init__(self):
+        if self.kv_cache_bits not in (4, 16):
+            raise ValueError("kv_cache_bits must be 4 or 16")
+        if self.int4_weights and self.fp8_weights:
+            raise ValueError("int4_weights and fp8_weights exclude each other")
         if self.temperature == 0.0:
             self.greedy, self.temperature = True, 1.0
         if not (0.0 < self.top_p <= 1.0):

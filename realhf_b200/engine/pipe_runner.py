@@ -238,7 +238,7 @@ class PipelineRunner:
                 hidden = buf
             out = m(input_ids=ids, cu_seqlens=cu, max_seqlen=mx, kv_sink=kv) if self.first else \
                 m(hidden=hidden, cu_seqlens=cu, max_seqlen=mx, kv_sink=kv)
-            st = gen.DecodeState(m, B, mx + g.max_new_tokens)
+            st = gen.DecodeState(m, B, mx + g.max_new_tokens, g.kv_cache_bits)
             st.fill_from_prefill(kv, cu, lens)
             states.append(st)
             unfinished.append(torch.ones(B, dtype=torch.bool, device=dev))

@@ -22,7 +22,7 @@ import torch
 from realhf_b200.api.model import GenerationHyperparameters
 from realhf_b200.models.real_model import ReaLModel
 from realhf_b200.ops import functional as OF
-from realhf_b200.ops import launches
+from realhf_b200.ops import int4, launches
 from realhf_b200.parallel import tp as TP
 
 
@@ -104,13 +104,22 @@ def genstep(logits: torch.Tensor, g: GenerationHyperparameters, step: int, eos_i
 class DecodeState:
     """Static buffers of one decode session (fixed addresses => CUDA-graph replayable)."""
 
-    def __init__(self, model: ReaLModel, B: int, S: int):
+    def __init__(self, model: ReaLModel, B: int, S: int, kv_bits: int = 16):
+        """kv_bits: 16 (caches of the model's type) or 4 (`ops/int4.py`; homogeneous stacks with heads of 64 or 128 channels)."""
         c = model.config
         nq, nkv = model._local_heads()
         dev, dt = model.device, model.dtype
         nb = model.n_local_blocks()
         self.hetero = c.blocks is not None
-        if self.hetero:
+        self.kv_bits = int(kv_bits)
+        if self.kv_bits not in (4, 16):
+            raise ValueError(f"kv_cache_bits is 4 or 16, not {kv_bits}")
+        if self.kv_bits == 4 and (self.hetero or c.head_dim not in int4.HEAD_DIMS or (dev.type == "cuda" and dt not in (torch.bfloat16, torch.float16))):
+            raise ValueError("kv_cache_bits=4 needs a homogeneous stack with heads of 64 or 128 channels, on a GPU in bfloat16 or float16")
+        if self.kv_bits == 4:
+            # one cache a block holds its keys and values (a model in fp32, CPU tests: steps in bfloat16)
+            self.k = self.v = [int4.Int4KVCache(B, S, nkv, c.head_dim, dt if dt in (torch.bfloat16, torch.float16) else torch.bfloat16, dev) for _ in range(nb)]
+        elif self.hetero:
             # per block: the latent ring [B, R, rank] (a block that reads another block's latent holds that block's tensor) and
             # the convolution state [2, B, taps - 1, H] fp32 (mixer / feed-forward inputs); see models/hetero_block.py
             from realhf_b200.models import hetero_block as HB
@@ -236,6 +245,11 @@ class DecodeState:
 
     def fill_from_prefill(self, kv: List[Tuple[torch.Tensor, torch.Tensor]], cu_seqlens: torch.Tensor, lens: torch.Tensor):
         """Scatter the packed prefill K/V of every block into the dense caches."""
+        if self.kv_bits == 4:
+            for c, (k, v) in zip(self.k, kv):
+                c.store(k.to(c.dtype), v.to(c.dtype), cu_seqlens)
+            self.cache_lens.copy_(lens.int())
+            return
         dev = cu_seqlens.device
         T = int(kv[0][0].shape[0])
         tok = torch.arange(T, device=dev)
@@ -254,7 +268,8 @@ def _final_logits(model: ReaLModel, hidden: torch.Tensor) -> torch.Tensor:
         return f8(hidden)
     if model.config.logit_scale is not None and model.ctx.tp_size == 1:
         return OF.linear_f32(hidden, model.head_weight()).mul_(model.config.logit_scale)   # fp32 out of the GEMM, scaled in place
-    lg = OF.linear(hidden, model.head_weight())
+    q4 = model._int4.get("head") if model._int4_active and model._int4 else None
+    lg = q4(hidden) if q4 is not None and hidden.shape[0] <= 128 else OF.linear(hidden, model.head_weight())
     if model.ctx.tp_size > 1:
         lg = TP._gather_last_dim(lg, model.ctx)
     if model.config.logit_scale is not None:
@@ -279,12 +294,16 @@ def prefill_into_state(model: ReaLModel, state: DecodeState, slots: List[int], i
     else:
         kv: List[Tuple[torch.Tensor, torch.Tensor]] = []
         out = model(input_ids=input_ids, cu_seqlens=cu, max_seqlen=max_seqlen, kv_sink=kv)
-        tok = torch.arange(int(input_ids.shape[0]), device=cu.device)
-        seq = torch.searchsorted(cu[1:].long().contiguous(), tok, right=True)
-        pos = tok - cu.long()[seq]
-        for li, (k, v) in enumerate(kv):
-            state.k[li][idx[seq], pos] = k
-            state.v[li][idx[seq], pos] = v
+        if state.kv_bits == 4:
+            for c, (k, v) in zip(state.k, kv):
+                c.store(k.to(c.dtype), v.to(c.dtype), cu, max_seqlen, slots=idx.int())
+        else:
+            tok = torch.arange(int(input_ids.shape[0]), device=cu.device)
+            seq = torch.searchsorted(cu[1:].long().contiguous(), tok, right=True)
+            pos = tok - cu.long()[seq]
+            for li, (k, v) in enumerate(kv):
+                state.k[li][idx[seq], pos] = k
+                state.v[li][idx[seq], pos] = v
     state.cache_lens[idx] = lens
     return out.hidden
 
@@ -392,8 +411,8 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
             marks.append((name, e))
     mark("start")
     # ---- prefill
-    if state is None or state.B != B or state.S < S:
-        state = DecodeState(model, B, S)
+    if state is None or state.B != B or state.S < S or state.kv_bits != g.kv_cache_bits:
+        state = DecodeState(model, B, S, g.kv_cache_bits)
     state.free_slots = list(range(B))
     hidden = prefill_into_state(model, state, state.alloc(B), input_ids, cu, max_prompt)
     last = (cu[1:] - 1).long()
@@ -409,6 +428,10 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
     use_fp8 = (g.fp8_weights or os.environ.get("REAL_GEN_FP8", "0") == "1") and B <= 128 and model.fp8_decode_supported()
     if use_fp8:
         model.enable_fp8_decode()
+    # opt-in 4-bit weights (ops/int4.py), the same way: the prefill ran in the model's type
+    use_int4 = g.int4_weights and not use_fp8 and B <= 128 and model.int4_decode_supported()
+    if use_int4:
+        model.enable_int4_decode()
     V = logits.shape[1]
     # the fused sampler can run as the tail of the captured step: then a decode step is ONE graph replay and nothing else
     # (no eager copy of the next token, no cache_lens += 1, no sampling launch, no per-step python bookkeeping)
@@ -420,7 +443,7 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
         return _final_logits(model, h)
 
     sig = (in_graph, g.max_new_tokens, g.min_new_tokens, g.top_k, g.top_p, g.temperature, g.greedy, need_mask, eos_id, pad_id,
-           int(model.flat_param.data_ptr()), use_fp8)
+           int(model.flat_param.data_ptr()), use_fp8, use_int4)
     if state.graph is not None and state.graph_sig != sig:
         state.graph = None  # sampling options changed, or the flat parameter buffer moved (realloc / offload reload / ZeRO-3)
     if in_graph:
@@ -499,6 +522,8 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
     mark("decode")
     if use_fp8:  # a graph kept for the next call holds pointers into the e4m3 buffers: then they stay (re-quantised in place)
         model.disable_fp8_decode(free=not (use_graph and state.graph is not None and not g.force_cudagraph_recapture))
+    if use_int4:
+        model.disable_int4_decode(free=not (use_graph and state.graph is not None and not g.force_cudagraph_recapture))
     if timing:
         torch.cuda.synchronize(dev)
         LAST_TIMING.clear()
@@ -573,7 +598,7 @@ class InflightBatchingGenerator:
                  max_prompt_len: int):
         assert model.is_first_stage and model.is_last_stage
         self.model, self.g, self.eos_id, self.pad_id, self.B = model, g, eos_id, pad_id, n_slots
-        self.state = DecodeState(model, n_slots, max_prompt_len + g.max_new_tokens)
+        self.state = DecodeState(model, n_slots, max_prompt_len + g.max_new_tokens, g.kv_cache_bits)
         self.slot_seq = [-1] * n_slots                 # which request a slot serves
         self.slot_tokens: List[List[int]] = [[] for _ in range(n_slots)]
         self.slot_logprobs: List[List[float]] = [[] for _ in range(n_slots)]

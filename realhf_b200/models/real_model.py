@@ -31,6 +31,7 @@ from realhf_b200.models import sharding
 from realhf_b200.models.sharding import ParamSpec
 from realhf_b200.ops import attention as attn_ops
 from realhf_b200.ops import functional as OF
+from realhf_b200.ops import int4
 from realhf_b200.parallel import tp as TP
 
 
@@ -580,6 +581,41 @@ class ReaLModel(nn.Module):
         if free:
             self._fp8 = None
 
+    # ---- 4-bit weights for decode (ops/int4.py): copies of the same weights, used the same way
+    _int4 = None
+    _int4_active = False
+
+    def int4_decode_supported(self) -> bool:
+        c = self.config
+        return bool(self.ctx.tp_size == 1 and c.mlp_type == "llama" and c.blocks is None and self.dtype in (torch.bfloat16, torch.float16) and self.instantiated)
+
+    def enable_int4_decode(self) -> int:
+        """Quantise (or, when the buffers exist already, re-quantise in place) every local block linear and the LM head, in the largest groups that divide their
+        inputs.  Returns the bytes held by the copies."""
+        from realhf_b200.ops import int4
+        names = [f"{i}.{n}.weight" for i in self.layers if 1 <= i <= self.config.n_layers for n in ("attn.qkv", "attn.o", "mlp.gate_up", "mlp.down")]
+        ws = {n: self.p[n] for n in names if n in self.p}
+        if self.is_last_stage and self.head_weight() is not None and self.config.logit_scale is None:   # (a fixed factor goes with logits in fp32)
+            ws["head"] = self.head_weight()
+        old, new = self._int4 or {}, {}
+        for n, w in ws.items():
+            group = next((g for g in (128, 64, 32) if int4.supported(w, g)), None)
+            if group is None:
+                continue
+            f = old.get(n)
+            if f is not None and (f.N, f.K, f.group, f.dtype) == (*w.shape, group, w.dtype) and f.q.device == w.device:
+                f.requantize(w)
+            else:
+                f = int4.Int4Linear(w, group=group)
+            new[n] = f
+        self._int4, self._int4_active = new, True
+        return sum(f.nbytes() for f in new.values())
+
+    def disable_int4_decode(self, free: bool = True):
+        self._int4_active = False
+        if free:
+            self._int4 = None
+
     def tied_embedding_params(self) -> List[torch.Tensor]:
         """Parameters whose gradients must be summed over the embedding group (tied embeddings with pp > 1)."""
         c = self.config
@@ -716,7 +752,7 @@ class ReaLModel(nn.Module):
                     cache_lens: torch.Tensor, hidden: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
                     m_caches: Optional[list] = None) -> torch.Tensor:
         """input_ids [B] -> final hidden [B, H] (last stage: after ln_f).  Appends K/V at `cache_lens` in place.
-        Caches: one [B, S, nkv_local, hd] tensor per local block.  Capturable in a CUDA graph (no host sync).
+        Caches: one [B, S, nkv_local, hd] tensor per local block, or one `Int4KVCache` in both lists.  Capturable in a CUDA graph (no host sync).
         Heterogeneous stacks: the caches are the per-block state tensors of `DecodeState` (see models/hetero_block.py) and
         `slots` [B] int32 names the state slot of every row (None: row b is slot b; `cache_lens` is indexed by slot); `m_caches`
         is `DecodeState.m`, what the blocks with more than two state tensors hold beside them."""
@@ -759,9 +795,11 @@ class ReaLModel(nn.Module):
         d_sym = None  # same, but still a per-rank partial sum in symmetric memory (tensor-parallel decode)
         # W8A8 decode: e4m3 weights + per-token e4m3 activations on tcgen05 kind::f8f6f4 (`enable_fp8_decode`, <= 128 rows)
         fp8 = self._fp8 if (self._fp8_active and self._fp8 and self.ctx.tp_size == 1) else None
+        int4w = self._int4 if (self._int4_active and self._int4 and fp8 is None) else None   # 4-bit weights (`enable_int4_decode`)
+        low = fp8 if fp8 is not None else int4w
 
         def q8(h_, wname, bname=None):
-            f = fp8.get(wname) if fp8 is not None and h_.shape[0] <= 128 else None
+            f = low.get(wname) if low is not None and h_.shape[0] <= 128 else None
             return None if f is None else f(h_, self._w(bname) if bname else None)
 
         def norm_q8(x_, ln_name, wname, bname=None):
@@ -802,9 +840,14 @@ class ReaLModel(nn.Module):
                     qkv, x = fq
                 else:
                     h, x = add_norm(x, f"{i}.attn.ln.weight")
-                    qkv = TP.col_linear(h, self.p[f"{i}.attn.qkv.weight"], self._w(f"{i}.attn.qkv.bias"), self.ctx, False)
-                o = attn_ops.decode_attention(qkv, k_caches[li], v_caches[li], cache_lens, nq, nkv, hd, self._attn_scale(i),
-                                              cos, sin, hd, c.rotary_interleaved)
+                    qkv = q8(h, f"{i}.attn.qkv.weight", f"{i}.attn.qkv.bias") if int4w is not None else None
+                    if qkv is None:
+                        qkv = TP.col_linear(h, self.p[f"{i}.attn.qkv.weight"], self._w(f"{i}.attn.qkv.bias"), self.ctx, False)
+                if isinstance(k_caches[li], int4.Int4KVCache):
+                    o = int4.decode_attention_int4(qkv, k_caches[li], cache_lens, nq, nkv, hd, self._attn_scale(i), cos, sin, hd, c.rotary_interleaved)
+                else:
+                    o = attn_ops.decode_attention(qkv, k_caches[li], v_caches[li], cache_lens, nq, nkv, hd, self._attn_scale(i),
+                                                  cos, sin, hd, c.rotary_interleaved)
                 li += 1
                 if tp_fused:
                     d_sym = fused.gemm_partial(o, self.p[f"{i}.attn.o.weight"])
@@ -829,7 +872,8 @@ class ReaLModel(nn.Module):
                         d = TP.row_linear(OF.gated_act(gu, c.activation_function), self.p[f"{i}.mlp.down.weight"], None, self.ctx, False)
                 else:
                     h2, x = add_norm(x, f"{i}.mlp.ln.weight")
-                    d = self._mlp(i, x, h2)
+                    gu = q8(h2, f"{i}.mlp.gate_up.weight") if int4w is not None and f"{i}.mlp.down.weight" in int4w else None
+                    d = self._mlp(i, x, h2) if gu is None else q8(OF.gated_act(gu, c.activation_function), f"{i}.mlp.down.weight")
                 if i == c.n_layers:
                     x, _ = add_norm(x, f"{i}.ln_f.weight")
         if d_sym is not None:  # a pipeline stage that does not end with ln_f hands on the summed residual stream
