@@ -29,6 +29,12 @@ int type_of(const Tensor& t, const char* op) {
   return t.scalar_type() == at::kBFloat16 ? 1 : 2;
 }
 bool on16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+// t itself if its rows lie on 16 bytes with unit inner stride, else a packed copy (not `contiguous()`: a slice of one row counts as that wherever it starts)
+Tensor rows16(const Tensor& t) {
+  bool ok = t.numel() == 0 || (t.stride(-1) == 1 && on16(t));
+  for (int64_t i = 0; ok && t.numel() > 0 && i + 1 < t.dim(); ++i) ok = t.stride(i) % 8 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 
 // int32 [n] on the device of `like`, or null
 const int* whole(const OptT& t, int64_t n, const Tensor& like, const char* op, const char* what) {
@@ -48,36 +54,45 @@ CacheDims cache_dims(const Tensor& cache, int64_t room, int64_t hd, const char* 
   return {cache.size(0), cache.size(1), cache.size(2)};
 }
 
-void cache_rows(Tensor k, Tensor v, Tensor cache, const Tensor& cu, const OptT& slots, const OptT& start, int64_t room, int64_t longest, bool store, const char* op) {
+void cache_rows(Tensor k, Tensor v, Tensor cache, const Tensor& cu, const OptT& slots, const OptT& start, int64_t room, int64_t hd, int64_t longest, bool store,
+                const char* op) {
   TORCH_CHECK_VALUE(k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == cache.device() &&
                         v.device() == cache.device(), op, ": keys and values [tokens, heads, channels] of one type beside the cache");
   const int dt = type_of(k, op);
-  const auto d = cache_dims(cache, room, k.size(2), op);
-  TORCH_CHECK_VALUE(k.size(1) == d.nkv && k.size(0) <= kInt, op, ": ", k.size(1), " heads for a cache of ", d.nkv);
-  for (const Tensor& t : {k, v})
-    TORCH_CHECK_VALUE(k.numel() == 0 || (t.stride(2) == 1 && t.stride(1) % 8 == 0 && t.stride(0) % 8 == 0 && on16(t)), op, ": rows on 16 bytes with unit inner stride");
+  const auto d = cache_dims(cache, room, hd, op);
+  TORCH_CHECK_VALUE(k.size(1) == d.nkv && k.size(2) == hd && k.size(0) <= kInt, op, ": ", k.size(1), " heads of ", k.size(2), " channels for a cache of ", d.nkv, " of ", hd);
   TORCH_CHECK_VALUE(cu.dim() == 1 && cu.size(0) >= 1, op, ": cu_seqlens holds one number more than there are sequences");
   const int64_t n = cu.size(0) - 1;
   const int *cp = whole(cu, n + 1, cache, op, "cu_seqlens"), *sp = whole(slots, n, cache, op, "slots"), *bp = whole(start, n, cache, op, "start");
   c10::cuda::CUDAGuard guard(cache.device());
+  if (store) {
+    k = rows16(k);
+    v = rows16(v);
+  }
+  if (longest <= 0) longest = k.size(0) / std::max<int64_t>(n, 1);
   const int rc = rb_int4_cache_rows(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), cache.data_ptr(), cp, sp, bp, (int)n, (int)d.nkv,
                                     (int)k.size(2), (int)d.slots, (int)room, (int)k.size(0), (int)std::min(std::max<int64_t>(longest, 1), kInt), store, dt,
                                     at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, op, ": the kernel could not be launched (", rc, ")");
 }
 
-void int4_cache_store(const Tensor& k, const Tensor& v, Tensor cache, const Tensor& cu, const OptT& slots, const OptT& start, int64_t room, int64_t longest) {
-  cache_rows(k, v, cache, cu, slots, start, room, longest, true, "int4_cache_store");
+void int4_cache_store(const Tensor& k, const Tensor& v, Tensor cache, const Tensor& cu, const OptT& slots, const OptT& start, int64_t room, int64_t hd,
+                      int64_t longest) {
+  cache_rows(k, v, cache, cu, slots, start, room, hd, longest, true, "int4_cache_store");
 }
 
-// Every token inside a sequence of `cu` is written; the others hold 0.
+// Tokens that belong to no sequence, or whose row or slot is not there, are 0.
 std::vector<Tensor> int4_cache_load(const Tensor& cache, const Tensor& cu, const OptT& slots, const OptT& start, int64_t room, int64_t hd, int64_t tokens, int64_t longest,
                                     at::ScalarType dtype) {
   cache_dims(cache, room, hd, "int4_cache_load");
   TORCH_CHECK_VALUE(tokens >= 0, "int4_cache_load: ", tokens, " tokens");
   c10::cuda::CUDAGuard guard(cache.device());
-  auto k = at::zeros({tokens, cache.size(1), hd}, cache.options().dtype(dtype)), v = at::zeros_like(k);
-  cache_rows(k, v, cache, cu, slots, start, room, longest, false, "int4_cache_load");
+  auto k = at::empty({tokens, cache.size(1), hd}, cache.options().dtype(dtype)), v = at::empty_like(k);
+  cache_rows(k, v, cache, cu, slots, start, room, hd, longest, false, "int4_cache_load");
+  if (cu.size(0) == 1) {   // (no sequence: no block wrote anything)
+    k.zero_();
+    v.zero_();
+  }
   return {k, v};
 }
 
@@ -89,7 +104,6 @@ Tensor decode_attention_int4(const Tensor& qkv, Tensor cache, const Tensor& lens
   TORCH_CHECK_VALUE(nkv == d.nkv && nkv > 0 && nq > 0 && nq % nkv == 0 && nq <= 65535, op, ": ", nq, " query heads over ", nkv, " key heads, a cache of ", d.nkv);
   TORCH_CHECK_VALUE(qkv.dim() == 2 && qkv.device() == cache.device() && qkv.size(0) == d.slots && qkv.size(1) == (nq + 2 * nkv) * hd, op,
                     ": the fused projection's output [slots, (n_q + 2 n_kv) * hd] beside the cache");
-  TORCH_CHECK_VALUE(qkv.numel() == 0 || (qkv.stride(1) == 1 && qkv.stride(0) % 8 == 0 && on16(qkv)), op, ": rows on 16 bytes with unit inner stride");
   const int* lp = whole(lens, d.slots, cache, op, "cache_lens");
   TORCH_CHECK_VALUE(cos.has_value() == sin.has_value(), op, ": cosines and sines go together");
   if (cos.has_value()) {
@@ -100,9 +114,10 @@ Tensor decode_attention_int4(const Tensor& qkv, Tensor cache, const Tensor& lens
   }
   attn_check();
   c10::cuda::CUDAGuard guard(qkv.device());
+  const Tensor rows = rows16(qkv);
   auto out = at::empty({qkv.size(0), nq * hd}, qkv.options());
-  const int rc = rb_decode_attention_int4(qkv.data_ptr(), cache.data_ptr(), lp, out.data_ptr(), cos.has_value() ? cos->data_ptr<float>() : nullptr,
-                                          sin.has_value() ? sin->data_ptr<float>() : nullptr, qkv.stride(0), (int)qkv.size(0), (int)nq, (int)nkv, (int)hd, (int)room,
+  const int rc = rb_decode_attention_int4(rows.data_ptr(), cache.data_ptr(), lp, out.data_ptr(), cos.has_value() ? cos->data_ptr<float>() : nullptr,
+                                          sin.has_value() ? sin->data_ptr<float>() : nullptr, rows.stride(0), (int)qkv.size(0), (int)nq, (int)nkv, (int)hd, (int)room,
                                           (int)rot_dim, interleaved, (float)scale, dt, at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, op, ": the kernel could not be launched (", rc, ")");
   return out;
@@ -122,9 +137,9 @@ void int4_quantize(const Tensor& w, Tensor q, int64_t group) {
   TORCH_CHECK_VALUE(w.dim() == 2 && w.device() == q.device(), op, ": a weight [N, K] beside its packed form");
   const int dt = type_of(w, op);
   check_weight(q, w.size(0), w.size(1), group, op);
-  TORCH_CHECK_VALUE(w.stride(1) == 1 && w.stride(0) % 8 == 0 && on16(w), op, ": rows on 16 bytes with unit inner stride");
   c10::cuda::CUDAGuard guard(w.device());
-  const int rc = rb_int4_quantize(w.data_ptr(), q.data_ptr(), (int)w.size(0), (int)w.size(1), w.stride(0), (int)group, dt, at::cuda::getCurrentCUDAStream().stream());
+  const Tensor rows = rows16(w);
+  const int rc = rb_int4_quantize(rows.data_ptr(), q.data_ptr(), (int)w.size(0), (int)w.size(1), rows.stride(0), (int)group, dt, at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, op, ": the kernel could not be launched (", rc, ")");
 }
 
@@ -134,12 +149,12 @@ Tensor int4_linear(const Tensor& x, const Tensor& q, const OptT& bias, int64_t N
   const int dt = type_of(x, op);
   const int64_t M = x.size(0), K = x.size(1);
   check_weight(q, N, K, group, op);
-  TORCH_CHECK_VALUE(M == 0 || (x.stride(1) == 1 && x.stride(0) % 8 == 0 && on16(x)), op, ": rows on 16 bytes with unit inner stride");
   TORCH_CHECK_VALUE(!bias.has_value() || (bias->scalar_type() == x.scalar_type() && bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous() && bias->device() == x.device()),
                     op, ": a bias [", N, "] of the rows' type");
   c10::cuda::CUDAGuard guard(x.device());
+  const Tensor rows = rows16(x);
   auto y = at::empty({M, N}, x.options());
-  const int rc = rb_int4_linear(x.data_ptr(), q.data_ptr(), bias.has_value() ? bias->data_ptr() : nullptr, y.data_ptr(), (int)M, (int)N, (int)K, x.stride(0), N, (int)group, dt,
+  const int rc = rb_int4_linear(rows.data_ptr(), q.data_ptr(), bias.has_value() ? bias->data_ptr() : nullptr, y.data_ptr(), (int)M, (int)N, (int)K, rows.stride(0), N, (int)group, dt,
                                 at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, op, ": the kernel could not be launched (", rc, ")");
   return y;
@@ -148,7 +163,7 @@ Tensor int4_linear(const Tensor& x, const Tensor& q, const OptT& bias, int64_t N
 }  // namespace
 
 void register_int4_ops(torch::Library& m) {
-  m.def("int4_cache_store(Tensor k, Tensor v, Tensor(a!) cache, Tensor cu_seqlens, Tensor? slots, Tensor? start, int room, int longest) -> ()", &int4_cache_store);
+  m.def("int4_cache_store(Tensor k, Tensor v, Tensor(a!) cache, Tensor cu_seqlens, Tensor? slots, Tensor? start, int room, int hd, int longest) -> ()", &int4_cache_store);
   m.def("int4_cache_load(Tensor cache, Tensor cu_seqlens, Tensor? slots, Tensor? start, int room, int hd, int tokens, int longest, ScalarType dtype) -> Tensor[]",
         &int4_cache_load);
   m.def("decode_attention_int4(Tensor qkv, Tensor(a!) cache, Tensor cache_lens, int nq, int nkv, int hd, int room, float scale, Tensor? cos, Tensor? sin, int rot_dim, "

@@ -31,6 +31,14 @@ __global__ void __launch_bounds__(kThreads) cache_rows_kernel(CacheParams p) {
   const int64_t start = p.start ? p.start[seq] : 0;
   const bool there = slot >= 0 && slot < p.n_slots;
   if (kStore && !there) return;
+  if constexpr (!kStore) {                          // tokens before the first sequence and behind the last belong to none
+    const int lo = seq == p.n - 1 ? tok1 : 0, hi = seq == p.n - 1 ? p.T : 0, front = seq == 0 ? tok0 : 0;
+    for (int i = blockIdx.z * kGroups + threadIdx.x / LPR; i < front + (hi - lo); i += gridDim.z * kGroups) {
+      const int64_t tok = i < front ? i : lo + (i - front);
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.k) + tok * p.kt + head * p.kh + sub * 8) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.v) + tok * p.vt + head * p.vh + sub * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
   const int64_t first = (start < 0 ? start - 15 : start) / 16, last = start + (tok1 - tok0);   // tiles first .. ; rows below `last`
   for (int64_t tile = first + blockIdx.z; tile * 16 < last; tile += gridDim.z) {
     uint32_t* at = p.cache + (((int64_t)slot * p.nkv + head) * p.tiles + tile) * Tl::kWords;

@@ -93,13 +93,6 @@ def _channel_order(words: torch.Tensor) -> torch.Tensor:
     return words.unflatten(-1, (4, -1)).transpose(-1, -2).flatten(-2)
 
 
-def _on16(x: torch.Tensor) -> torch.Tensor:
-    """x itself if its rows lie on 16 bytes with unit inner stride, else a packed copy (not `contiguous()`: a slice of one row counts as that wherever it starts)."""
-    if x.numel() and (x.stride(-1) != 1 or any(s % 8 for s in x.stride()[:-1]) or x.data_ptr() % 16):
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
 # ------------------------------------------------------------------------------------------------ cache
 
 
@@ -147,8 +140,13 @@ class Int4KVCache:
         for name, t in (("slots", slots), ("start", start)):
             if t is not None and tuple(t.shape) != (n,):
                 raise ValueError(f"Int4KVCache: `{name}` holds one number a sequence ({n}), not {tuple(t.shape)}")
-        i = lambda t: None if t is None else t.to(device=self.device, dtype=torch.int32).contiguous()   # noqa: E731
-        return i(cu_seqlens), i(slots), i(start)
+        return self._whole(cu_seqlens), self._whole(slots), self._whole(start)
+
+    def _whole(self, t):
+        """int32 beside the cache."""
+        if t is None or (t.dtype is torch.int32 and t.device == self.data.device and t.is_contiguous()):
+            return t
+        return t.to(device=self.data.device, dtype=torch.int32).contiguous()
 
     def _rows(self, cu, slots, start, tokens: int):
         """(token, slot, row) of every packed token whose row is inside the cache."""
@@ -166,15 +164,14 @@ class Int4KVCache:
         """Writes packed keys (rotated) and values [T, n_kv, hd]: the tokens cu_seqlens[i] .. of sequence i go to the rows start[i] .. (0 ..) of slot slots[i] (i).
         Rows and slots outside the cache are left out, all others of the cache keep what they hold.  No row may be named twice in a call.  `max_seqlen` sets the
         size of the launch alone."""
+        if use_native(self.data) and k.dtype is self.dtype and k.is_cuda:      # (the op checks the rest)
+            lib().int4_cache_store(k, v, self.data, self._whole(cu_seqlens), self._whole(slots), self._whole(start), self.room, self.hd, max_seqlen or 0)
+            return
         if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (self.n_kv, self.hd):
             raise ValueError(f"Int4KVCache.store: keys and values [tokens, {self.n_kv}, {self.hd}], not {tuple(k.shape)} and {tuple(v.shape)}")
         if k.dtype != self.dtype or v.dtype != self.dtype or k.device != self.device or v.device != self.device:
             raise ValueError(f"Int4KVCache.store: keys and values are {self.dtype} on {self.device}, as the cache")
         cu, slots, start = self._check(cu_seqlens, slots, start)
-        if use_native(k):
-            n = max_seqlen if max_seqlen is not None else k.shape[0] // max(1, cu.numel() - 1)
-            lib().int4_cache_store(_on16(k), _on16(v), self.data, cu, slots, start, self.room, n)
-            return
         tok, slot, row = self._rows(cu, slots, start, k.shape[0])
         self._put(k[tok], v[tok], slot, row)
 
@@ -205,13 +202,12 @@ class Int4KVCache:
              start: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """The reverse of `store`: keys and values [tokens, n_kv, hd] of the cache's type, each number rounded once.  Tokens whose row or slot is outside the cache,
         or that belong to no sequence, are 0."""
+        if use_native(self.data):
+            k, v = lib().int4_cache_load(self.data, self._whole(cu_seqlens), self._whole(slots), self._whole(start), self.room, self.hd, tokens, max_seqlen or 0, self.dtype)
+            return k, v
         if tokens < 0:
             raise ValueError(f"Int4KVCache.load: {tokens} tokens")
         cu, slots, start = self._check(cu_seqlens, slots, start)
-        if use_native(self.data):
-            n = max_seqlen if max_seqlen is not None else tokens // max(1, cu.numel() - 1)
-            k, v = lib().int4_cache_load(self.data, cu, slots, start, self.room, self.hd, tokens, n, self.dtype)
-            return k, v
         out = torch.zeros(2, tokens, self.n_kv, self.hd, dtype=self.dtype, device=self.device)
         tok, slot, row = self._rows(cu, slots, start, tokens)
         k, v = self._get(slot, row)
@@ -257,6 +253,8 @@ def decode_attention_int4(qkv: torch.Tensor, cache: Int4KVCache, cache_lens: tor
     type, key and value are quantised and written, and the queries attend to the rows [0, cache_lens[b]] as the cache holds them, the new one among them.
     Returns [slots, n_q * hd].  A row whose length is not in [0, room) changes nothing and returns 0.  Does not advance cache_lens."""
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    if use_native(qkv) and qkv.dtype is cache.dtype:                           # (the op checks the rest)
+        return lib().decode_attention_int4(qkv, cache.data, cache._whole(cache_lens), n_q, n_kv, hd, cache.room, scale, cos, sin, rot_dim or hd, interleaved)
     if (n_kv, hd) != (cache.n_kv, cache.hd) or n_q <= 0 or n_q % n_kv:
         raise ValueError(f"decode_attention_int4: {n_q} query heads over {n_kv} of {hd} channels, a cache of {cache.n_kv} heads of {cache.hd}")
     if tuple(qkv.shape) != (cache.slots, (n_q + 2 * n_kv) * hd) or tuple(cache_lens.shape) != (cache.slots,):
@@ -266,10 +264,8 @@ def decode_attention_int4(qkv: torch.Tensor, cache: Int4KVCache, cache_lens: tor
     if (cos is None) != (sin is None) or (cos is not None and (rot > hd or rot % (2 if interleaved else 16) or tuple(cos.shape[1:]) != (rot // 2,) or
                                                                cos.shape != sin.shape or cos.shape[0] < cache.room)):
         raise ValueError(f"decode_attention_int4: cosines and sines are tables [{cache.room} or more, {rot // 2}], both or neither")
-    if use_native(qkv):
-        if qkv.dtype != cache.dtype or qkv.device != cache.device:
-            raise ValueError(f"decode_attention_int4: projections are {cache.dtype} on {cache.device}, as the cache")
-        return lib().decode_attention_int4(_on16(qkv), cache.data, cache_lens.int().contiguous(), n_q, n_kv, hd, cache.room, scale, cos, sin, rot, interleaved)
+    if use_native(qkv) or use_native(cache.data):
+        raise ValueError(f"decode_attention_int4: projections are {cache.dtype} on {cache.device}, as the cache")
     return decode_attention_int4_ref(qkv, cache, cache_lens, n_q, n_kv, hd, scale, cos, sin, rot, interleaved)
 
 
@@ -324,7 +320,7 @@ class Int4Linear:
         if tuple(w.shape) != (self.N, self.K) or w.dtype != self.dtype or w.device != self.q.device:
             raise ValueError(f"Int4Linear: a weight [{self.N}, {self.K}] of {self.dtype} on {self.q.device}")
         if use_native(w):
-            lib().int4_quantize(_on16(w), self.q, self.group)
+            lib().int4_quantize(w, self.q, self.group)
         else:
             self._fill(*quantize_groups(w, self.group))
 
@@ -343,12 +339,14 @@ class Int4Linear:
         if x.dim() == 0 or x.shape[-1] != self.K:
             raise ValueError(f"Int4Linear: rows of {self.K}, not {tuple(x.shape)}")
         bias = self.bias if bias is None else bias
-        x2 = x.reshape(-1, self.K)
         if use_native(x):
-            if x.dtype != self.dtype or x.device != self.q.device:
+            if x.dtype is not self.dtype or x.device != self.q.device:
                 raise ValueError(f"Int4Linear: rows of {self.dtype} on {self.q.device}")
-            y = lib().int4_linear(_on16(x2), self.q, bias, self.N, self.group)
+            if x.dim() == 2:
+                return lib().int4_linear(x, self.q, bias, self.N, self.group)
+            y = lib().int4_linear(x.reshape(-1, self.K), self.q, bias, self.N, self.group)
         else:
+            x2 = x.reshape(-1, self.K)
             y = x2.float() @ self.dequantize().t()
             y = (y if bias is None else y + bias.float()).to(x.dtype)
         return y.view(*x.shape[:-1], self.N)

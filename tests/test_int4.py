@@ -559,4 +559,4 @@ def test_refusals_of_the_kernels():
     with pytest.raises(ValueError):
         lib().int4_linear(torch.zeros(1, 128, device="cuda", dtype=torch.bfloat16), c.data, None, 4, 128)
     with pytest.raises(ValueError):
-        lib().int4_cache_store(torch.zeros(1, 1, 64), torch.zeros(1, 1, 64), c.data, torch.zeros(2, dtype=torch.int32), None, None, 8, 1)
+        lib().int4_cache_store(torch.zeros(1, 1, 64), torch.zeros(1, 1, 64), c.data, torch.zeros(2, dtype=torch.int32), None, None, 8, 64, 1)
