@@ -151,6 +151,7 @@ Tensor int4_linear(const Tensor& x, const Tensor& q, const OptT& bias, int64_t N
   check_weight(q, N, K, group, op);
   TORCH_CHECK_VALUE(!bias.has_value() || (bias->scalar_type() == x.scalar_type() && bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous() && bias->device() == x.device()),
                     op, ": a bias [", N, "] of the rows' type");
+  attn_check();
   c10::cuda::CUDAGuard guard(x.device());
   const Tensor rows = rows16(x);
   auto y = at::empty({M, N}, x.options());

@@ -7,10 +7,14 @@
 // leaves SMs idle, the blocks of a cluster share K.  Codes become exact 16-bit numbers (a mask that leaves a code in the low bits of 128 or 1024, and a subtraction) and are the
 // left operand, 16 output rows at a time; rows of x, read from L2 and L1 as the operands' lanes want them, are the right one, eight at a time.  Scale and lowest value stay out: a
 // group's product is scaled in fp32 when its channels are through, and the lowest value times the sum of x over the group (one more product, with ones) is added.
-#include "gemm_common.cuh"
+// More rows: a block has 128 output rows and all rows of x (in pieces of 128), and the products run on tcgen05.  Eight warps turn a block of 128 channels of codes into a swizzled
+// operand tile in shared memory, rows of x come by TMA, one warp issues the products of a group of channels into an accumulator of its own in tensor memory, and eight warps
+// scale it into sums in registers (and add the lowest values times the sums of x, which they take from the operand tile) while the next group is multiplied.
+#include "attn_common.cuh"
 #include "int4.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace {
 
@@ -78,6 +82,7 @@ struct LinearParams {
   void* y;
   int M, N, K, kblocks, tiles, splits;
   int64_t ldx, ldy;
+  int* status;              // rb_attn_status()
 };
 
 RB_DEVICE uint4 load_stream(const uint32_t* p) {
@@ -229,11 +234,300 @@ template <typename T, int G, int NT> int few_rows(LinearParams p, cudaStream_t s
   return cudaLaunchKernelEx(&cfg, few_rows_kernel<T, G, NT>, p) == cudaSuccess ? 0 : -3;
 }
 
+// ---------------------------------------------------------------------------------------------- many rows
+
+constexpr int kManyRows = 128, kExpand = 4, kScale = 8, kStages = 3;                 // output rows; warps that expand, that scale
+constexpr int kLoadWarp = kExpand + kScale, kMmaWarp = kLoadWarp + 1, kManyThreads = (kMmaWarp + 1) * 32;
+constexpr int kCodeBytes = kManyRows * 256;                                          // 128 rows x 128 channels of 16 bits: two halves of 64 channels
+constexpr int kBufs = 4;                                                             // accumulators
+template <int NP> constexpr size_t kManySmem = 1024 + kStages * (kCodeBytes + NP * 256);
+
+RB_DEVICE void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
+template <typename T> RB_DEVICE float2 pair_of(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// NP: rows of x, padded (rows beyond M read as zeros)
+template <typename T, int G, int NP>
+__global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid_constant__ CUtensorMap xmap, const LinearParams p) {
+  constexpr int NG = 128 / G, ND = kBufs, kCols = NP / 2, kX = NP * 256;
+  extern __shared__ unsigned char raw[];
+  __shared__ __align__(8) uint64_t code_full[kStages], x_full[kStages], empty[kStages], d_full[ND], d_empty[ND];
+  __shared__ __align__(16) float xsum[2][NG][NP];
+  __shared__ uint32_t tmem_ptr, dead_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile uint32_t* dead = &dead_flag;
+  const uint32_t base = (ptx::smem_u32(raw) + 1023u) & ~1023u, codes = base, xs = base + kStages * kCodeBytes;
+  auto bar = [](uint64_t* b, int i) { return ptx::smem_u32(&b[i]); };
+  if (threadIdx.x == 0) {
+    *dead = 0;
+    for (int i = 0; i < kStages; ++i) {
+      ptx::mbar_init(bar(code_full, i), kExpand);
+      ptx::mbar_init(bar(x_full, i), 1);
+      ptx::mbar_init(bar(empty, i), 1 + kScale);
+    }
+    for (int i = 0; i < ND; ++i) {
+      ptx::mbar_init(bar(d_full, i), 1);
+      ptx::mbar_init(bar(d_empty, i), kScale);
+    }
+    ptx::fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(ptx::smem_u32(&tmem_ptr), ND * NP);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_ptr);
+  rb::pdl_trigger();
+  rb::pdl_wait();
+  // this block's part of the channels
+  const int per = RB_CEIL_DIV(p.kblocks, p.splits), k0 = min(p.kblocks, (int)blockIdx.y * per), k1 = min(p.kblocks, k0 + per);
+  auto tile_of = [&](int i) { return p.q + (int64_t)min((int)blockIdx.x * (kManyRows / 16) + i, p.tiles - 1) * p.kblocks * WTile<G>::kWords; };
+  float acc[kCols];
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+
+  if (warp < kExpand) {
+    // ---- codes to operands: warp w has rows 16 w .. and 64 + 16 w .., a lane the words of rows g and g + 8 of its four steps; odd rows store them in another order, so that the eight
+    // lanes of a store meet all banks
+    const int g = lane >> 2, t = lane & 3, odd = g & 1;
+    const uint32_t* tile[2] = {tile_of(warp), tile_of(warp + 4)};
+    uint4 next[2][2];
+    auto ask = [&](int kb) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) next[u][h] = load_stream(tile[u] + (int64_t)kb * WTile<G>::kWords + h * 128 + lane * 4);
+    };
+    if (k0 < k1) ask(k0);
+    int st = 0;
+    uint32_t turn = 1;                              // (the first round of a ring is free)
+    for (int kb = k0; kb < k1; ++kb) {
+      uint32_t w[2][2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) { w[u][h][0] = next[u][h].x; w[u][h][1] = next[u][h].y; w[u][h][2] = next[u][h].z; w[u][h][3] = next[u][h].w; }
+      if (kb + 1 < k1) ask(kb + 1);
+      bounded_wait(bar(empty, st), turn, dead);
+      const uint32_t to = codes + st * kCodeBytes + (warp * 16 + g) * 128;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) {
+            uint32_t e[4];
+            expand<T>(odd ? w[u][h][jj ^ 1] : w[u][h][jj], e);
+            const int j = jj ^ odd;                 // channels 32 j + 8 t ..: piece 4 (j & 1) + t of half j >> 1
+            st_shared_v4(to + u * (64 * 128) + h * (8 * 128) + (j >> 1) * (kManyRows * 128) + ((((j & 1) * 4 + t) ^ g) << 4), e[0], e[1], e[2], e[3]);
+          }
+      ptx::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(code_full, st));
+      if (++st == kStages) { st = 0; turn ^= 1; }
+    }
+  } else if (warp < kLoadWarp) {
+    // ---- sums: warp has 32 output rows (a quarter of the lanes of tensor memory) and half of the rows of x
+    const int e = warp - kExpand, quarter = warp % 4, half = e / 4, tid = e * 32 + lane;
+    constexpr int kEach = 2 * 128 / NP, kPieces = 16 / kEach;      // threads a row of x, 16-byte pieces a thread of its 128 channels
+    const int col = tid / kEach, sub = tid % kEach, row = quarter * 32 + lane;
+    const uint32_t* tile = tile_of(row / 16) + 256 + row % 16 * NG;
+    uint32_t next[NG];
+    auto ask = [&](int kb) {
+#pragma unroll
+      for (int q = 0; q < NG; ++q) next[q] = __ldg(tile + (int64_t)kb * WTile<G>::kWords + q);
+    };
+    if (k0 < k1) ask(k0);
+    int st = 0, buf = 0;
+    uint32_t turn = 0, dturn = 0;
+    for (int kb = k0; kb < k1; ++kb) {
+      uint32_t word[NG];
+#pragma unroll
+      for (int q = 0; q < NG; ++q) word[q] = next[q];
+      if (kb + 1 < k1) ask(kb + 1);
+      // the sums of x over the groups: a thread's pieces lie in one group, or are whole groups
+      bounded_wait(bar(x_full, st), turn, dead);
+      constexpr int kSpan = kPieces * 8, kOwn = kSpan > G ? kSpan / G : 1, kShare = kSpan < G ? G / kSpan : 1;   // channels of a thread, groups that it sums alone, threads of a group
+      float s[kOwn];
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) s[i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int piece = sub * kPieces + i;
+        const uint4 v = ld_shared_v4(xs + st * kX + (piece >> 3) * (NP * 128) + col * 128 + (((piece & 7) ^ (col & 7)) << 4));
+        const float2 a = pair_of<T>(v.x), b = pair_of<T>(v.y), c = pair_of<T>(v.z), d = pair_of<T>(v.w);
+        s[i * kOwn / kPieces] += ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
+      }
+      if constexpr (kSpan < G) {
+#pragma unroll
+        for (int o = 1; o < kShare; o <<= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+      }
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i)
+        if (sub % kShare == 0) xsum[kb & 1][sub / kShare * kOwn + i][col] = s[i];
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(empty, st));
+      if (++st == kStages) { st = 0; turn ^= 1; }
+      asm volatile("bar.sync 1, %0;" ::"n"(kScale * 32) : "memory");
+#pragma unroll
+      for (int q = 0; q < NG; ++q) {
+        bounded_wait(bar(d_full, buf), dturn, dead);
+        ptx::tc_fence_after();
+        const float scale = q4::scale_of<T>(word[q]), low = q4::low_of<T>(word[q]);
+#pragma unroll
+        for (int c = 0; c < kCols; c += 16) {
+          uint32_t d[16];
+          tc_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + buf * NP + half * kCols + c, d);
+          ptx::tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(&xsum[kb & 1][q][half * kCols + c + i]);
+            acc[c + i] = fmaf(scale, __uint_as_float(d[i]), fmaf(low, x.x, acc[c + i]));
+            acc[c + i + 1] = fmaf(scale, __uint_as_float(d[i + 1]), fmaf(low, x.y, acc[c + i + 1]));
+            acc[c + i + 2] = fmaf(scale, __uint_as_float(d[i + 2]), fmaf(low, x.z, acc[c + i + 2]));
+            acc[c + i + 3] = fmaf(scale, __uint_as_float(d[i + 3]), fmaf(low, x.w, acc[c + i + 3]));
+          }
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(d_empty, buf));
+        if (++buf == ND) { buf = 0; dturn ^= 1; }
+      }
+    }
+  } else if (warp == kLoadWarp) {
+    int st = 0;
+    uint32_t turn = 1;
+    for (int kb = k0; kb < k1; ++kb) {
+      bounded_wait(bar(empty, st), turn, dead);
+      if (ptx::elect_one()) {
+        ptx::mbar_arrive_expect_tx(bar(x_full, st), kX);
+        ptx::tma_load_2d(xs + st * kX, &xmap, bar(x_full, st), kb * 128, 0);
+        ptx::tma_load_2d(xs + st * kX + NP * 128, &xmap, bar(x_full, st), kb * 128 + 64, 0);
+      }
+      if (++st == kStages) { st = 0; turn ^= 1; }
+    }
+  } else {
+    constexpr uint32_t idesc = ptx::make_idesc_f16(std::is_same<T, __half>::value ? 0 : 1, 128, NP, 0, 0);
+    const uint32_t el = ptx::elect_one() ? 1u : 0u;
+    int st = 0, buf = 0;
+    uint32_t turn = 0, dturn = 1;
+    for (int kb = k0; kb < k1; ++kb) {
+      bounded_wait(bar(code_full, st), turn, dead);
+      bounded_wait(bar(x_full, st), turn, dead);
+      const uint32_t a = ptx::desc_lo(codes + st * kCodeBytes, 16), b = ptx::desc_lo(xs + st * kX, 16);
+#pragma unroll
+      for (int q = 0; q < NG; ++q) {
+        bounded_wait(bar(d_empty, buf), dturn, dead);
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 8 / NG; ++k) {          // 16 channels, 32 bytes of a swizzled row
+          const int at = q * (8 / NG) + k;
+          ptx::tc_mma_f16_if(el, tmem + buf * NP, a + (at >> 2) * (kManyRows * 128 >> 4) + (at & 3) * 2, b + (at >> 2) * (NP * 128 >> 4) + (at & 3) * 2, idesc, k != 0);
+        }
+        ptx::tc_commit_if(el, bar(d_full, buf));
+        if (++buf == ND) { buf = 0; dturn ^= 1; }
+      }
+      ptx::tc_commit_if(el, bar(empty, st));
+      __syncwarp();
+      if (++st == kStages) { st = 0; turn ^= 1; }
+    }
+  }
+  // ---- all products have been read: the ring's place holds the sums where a cluster shares the channels
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, ND * NP);
+  const bool sums = warp >= kExpand && warp < kLoadWarp;
+  const int quarter = warp % 4, half = (warp - kExpand) / 4, r = quarter * 32 + lane, n = blockIdx.x * kManyRows + r;
+  T* y = reinterpret_cast<T*>(p.y);
+  const float bias = p.bias && n < p.N ? rb::to_f(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
+  if (p.splits == 1) {
+    if (sums && n < p.N) {
+#pragma unroll
+      for (int i = 0; i < kCols; ++i)
+        if (half * kCols + i < p.M) y[(half * kCols + i) * p.ldy + n] = rb::from_f<T>(acc[i] + bias);
+    }
+  } else {
+    float* part = reinterpret_cast<float*>(raw + (base - ptx::smem_u32(raw)));    // [NP][128]
+    if (sums) {
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) part[(half * kCols + i) * kManyRows + r] = acc[i];
+    }
+    ptx::cluster_sync();
+    if (sums) {                                       // rows of x are dealt out to the cluster's blocks and the eight warps' halves
+      for (int m = blockIdx.y * 2 + half; m < p.M; m += p.splits * 2) {
+        float v = bias;
+        for (int c = 0; c < p.splits; ++c) {
+          uint32_t a;
+          float f;
+          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(base + (m * kManyRows + r) * 4), "r"(c));
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+          v += f;
+        }
+        if (n < p.N) y[m * p.ldy + n] = rb::from_f<T>(v);
+      }
+    }
+  }
+  rb::report_given_up(dead, p.status);
+  if (p.splits > 1) ptx::cluster_sync();              // nobody leaves while its sums are being read
+}
+
+template <typename T, int G, int NP> int many_rows(LinearParams p, cudaStream_t s) {
+  static std::atomic<uint64_t> opted_in{0};           // the attribute is the kernel's on one device: a bit per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -3;
+  if (dev >= 64 || !(opted_in.load(std::memory_order_relaxed) >> dev & 1)) {
+    if (cudaFuncSetAttribute(many_rows_kernel<T, G, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kManySmem<NP>) != cudaSuccess) return -3;
+    if (dev < 64) opted_in.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  }
+  CUtensorMap xmap;
+  if (!make_tmap(&xmap, p.x, std::is_same<T, __nv_bfloat16>::value, p.M, p.K, p.ldx, 64, NP)) return -4;
+  // Blocks of a cluster: the number whose rounds over the SMs, each a fixed part (about eight blocks' time) and its blocks of channels, take the least
+  const int tiles = RB_CEIL_DIV(p.N, kManyRows);
+  int64_t best = INT64_MAX;
+  for (int c = 1; c <= kMaxSplits && c <= p.kblocks; ++c) {
+    const int64_t cost = (int64_t)RB_CEIL_DIV(tiles * (int64_t)c, rb::kNumSMs) * (RB_CEIL_DIV(p.kblocks, c) + 8);
+    if (cost < best) { best = cost; p.splits = c; }
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(tiles, p.splits);
+  cfg.blockDim = dim3(kManyThreads);
+  cfg.dynamicSmemBytes = kManySmem<NP>;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (p.splits > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = attr[n].val.clusterDim.z = 1;
+    attr[n++].val.clusterDim.y = p.splits;
+  }
+  if (rb::pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, many_rows_kernel<T, G, NP>, xmap, p) == cudaSuccess ? 0 : -3;
+}
+
 template <typename T, int G> int run(const void* x, const void* q, const void* bias, void* y, int M, int N, int K, int64_t ldx, int64_t ldy, cudaStream_t s) {
-  for (int m0 = 0; m0 < M; m0 += 16) {
-    const LinearParams p{(const T*)x + m0 * ldx, bias, (const uint32_t*)q, (T*)y + m0 * ldy, std::min(M - m0, 16), N, K, RB_CEIL_DIV(K, 128), RB_CEIL_DIV(N, 16), 1, ldx, ldy};
-    const int rc = p.M <= 8 ? few_rows<T, G, 1>(p, s) : few_rows<T, G, 2>(p, s);
+  int* status = rb_attn_status();
+  if (status == nullptr) return -5;
+  for (int m0 = 0; m0 < M;) {
+    const int rows = std::min(M - m0, 128);
+    const LinearParams p{(const T*)x + m0 * ldx, bias, (const uint32_t*)q, (T*)y + m0 * ldy, rows, N, K, RB_CEIL_DIV(K, 128), RB_CEIL_DIV(N, 16), 1, ldx, ldy, status};
+    const int rc = rows <= 8 ? few_rows<T, G, 1>(p, s) : rows <= 16 ? few_rows<T, G, 2>(p, s) : rows <= 32 ? many_rows<T, G, 32>(p, s) : rows <= 64 ? many_rows<T, G, 64>(p, s)
+                                                                                                            : many_rows<T, G, 128>(p, s);
     if (rc != 0) return rc;
+    m0 += rows;
   }
   return 0;
 }
