@@ -123,7 +123,7 @@ Tensor decode_attention_int4(const Tensor& qkv, Tensor cache, const Tensor& lens
   return out;
 }
 
-int64_t weight_words(int64_t N, int64_t K, int64_t group) { return (N + 15) / 16 * ((K + 127) / 128) * (256 + 16 * (128 / group)); }
+int64_t weight_words(int64_t N, int64_t K, int64_t group) { return (N + 127) / 128 * 8 * ((K + 127) / 128) * (256 + 16 * (128 / group)); }
 
 void check_weight(const Tensor& q, int64_t N, int64_t K, int64_t group, const char* op) {
   TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128, op, ": groups of 32, 64 or 128, not ", group);

@@ -1,7 +1,8 @@
 // Products of a few rows with a weight held in 4 bits: y[m, n] = sum_k x[m, k] w[n, k] (+ bias[n]), w ~ scale c + low by groups of 32, 64 or 128 along K (int4.cuh).
 //
-// A weight is tiles of 16 output rows x 128 channels, the tiles of 16 rows one behind the other along K: weight words [row][t][j] of 128 channels,
-// then the group words [row][group].  Rows beyond N and channels beyond K hold codes, scales and lowest values of 0.
+// A weight is tiles of 16 output rows x 128 channels: weight words [row][t][j] of 128 channels, then the group words [row][group].  Eight tiles of 128 rows lie one behind
+// the other, then those of the next 128 channels (a copy of the eight is one of 9 KB: eight copies of 1 KB each streamed 2.8 TB/s where one streamed 4.4), then the next rows'.
+// Rows beyond N and channels beyond K hold codes, scales and lowest values of 0.
 //
 // Few rows (up to 16): a block of eight warps has 32 output rows, its warps walk along K in blocks of 128 channels, one in eight each, and add their sums up at the end; where that
 // leaves SMs idle, the blocks of a cluster share K.  Codes become exact 16-bit numbers (a mask that leaves a code in the low bits of 128 or 1024, and a subtraction) and are the
@@ -25,6 +26,9 @@ template <int G> struct WTile {
   static constexpr int kGroups = 128 / G, kWords = 16 * 16 + 16 * kGroups;
 };
 
+// where tile i of block kb begins
+template <int G> RB_DEVICE int64_t tile_at(int i, int kb, int kblocks) { return (((int64_t)(i >> 3) * kblocks + kb) * 8 + (i & 7)) * WTile<G>::kWords; }
+
 template <typename T, int G>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ w, uint32_t* __restrict__ q, int N, int K, int64_t ld) {
   const int r = threadIdx.x / 16, sub = threadIdx.x % 16, n = blockIdx.x * 16 + r, kblocks = RB_CEIL_DIV(K, 128);
@@ -40,7 +44,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ w, 
     for (int i = 0; i < 8; ++i) x[i] = rb::to_f(a.v[i]);
     q4::extremes<G / 8>(x, lo, hi);
     const uint32_t g = mine ? q4::group_word<T>(lo, hi) : 0u;
-    uint32_t* at = q + ((int64_t)blockIdx.x * kblocks + kb) * WTile<G>::kWords;
+    uint32_t* at = q + tile_at<G>(blockIdx.x, kb, kblocks);
     at[r * 16 + q4::word_place<4>(sub)] = mine ? q4::pack8<q4::kWeight>(x, q4::scale_of<T>(g), lo) : 0u;
     if (sub % (G / 8) == 0) at[256 + r * WTile<G>::kGroups + sub / (G / 8)] = g;
   }
@@ -80,7 +84,7 @@ struct LinearParams {
   const void *x, *bias;
   const uint32_t* q;
   void* y;
-  int M, N, K, kblocks, tiles, splits;
+  int M, N, K, kblocks, splits;
   int64_t ldx, ldy;
   int* status;              // rb_attn_status()
 };
@@ -115,14 +119,14 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const LinearParam
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   rb::pdl_trigger();
   const int tile0 = blockIdx.x * MT, step = kFewWarps * p.splits, first = blockIdx.y * kFewWarps + warp;
-  const uint32_t* tile[MT];
+  const uint32_t* tile[MT];                         // (tiles are padded to whole sets of eight)
 #pragma unroll
-  for (int i = 0; i < MT; ++i) tile[i] = p.q + (int64_t)min(tile0 + i, p.tiles - 1) * p.kblocks * WTile<G>::kWords;
+  for (int i = 0; i < MT; ++i) tile[i] = p.q + tile_at<G>(tile0 + i, 0, p.kblocks);
   rb::pdl_wait();
   Block<G> next[MT];
   if (first < p.kblocks)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) next[i].load(tile[i] + (int64_t)first * WTile<G>::kWords, lane);
+    for (int i = 0; i < MT; ++i) next[i].load(tile[i] + (int64_t)first * (8 * WTile<G>::kWords), lane);
   float acc[MT][NT][4] = {};
   const T* x = reinterpret_cast<const T*>(p.x);
   for (int kb = first; kb < p.kblocks; kb += step) {
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const LinearParam
       }
     if (kb + step < p.kblocks)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) next[i].load(tile[i] + (int64_t)(kb + step) * WTile<G>::kWords, lane);
+      for (int i = 0; i < MT; ++i) next[i].load(tile[i] + (int64_t)(kb + step) * (8 * WTile<G>::kWords), lane);
 #pragma unroll
     for (int q = 0; q < NG; ++q) {                  // a group
       float c[MT][NT][4] = {}, one[NT][4] = {};
@@ -236,16 +240,24 @@ template <typename T, int G, int NT> int few_rows(LinearParams p, cudaStream_t s
 
 // ---------------------------------------------------------------------------------------------- many rows
 
-constexpr int kManyRows = 128, kExpand = 4, kScale = 8, kStages = 3;                 // output rows; warps that expand, that scale
+constexpr int kManyRows = 128, kTeams = 2, kExpand = 4 * kTeams, kScale = 8;         // output rows; warps that expand (a team of four has every second block), that scale
 constexpr int kLoadWarp = kExpand + kScale, kMmaWarp = kLoadWarp + 1, kManyThreads = (kMmaWarp + 1) * 32;
 constexpr int kCodeBytes = kManyRows * 256;                                          // 128 rows x 128 channels of 16 bits: two halves of 64 channels
 constexpr int kBufs = 4;                                                             // accumulators
-template <int NP> constexpr size_t kManySmem = 1024 + kStages * (kCodeBytes + NP * 256);
+template <int NP> constexpr int kManyStages = NP == 32 ? 4 : NP == 64 ? 3 : 2;       // operand tiles
+template <int NP> constexpr int kRaw = NP == 32 ? 5 : 6;                             // blocks of packed codes, 9 or 10 KB each
+template <int G> constexpr int kRawBytes = 8 * WTile<G>::kWords * 4;
+template <int G, int NP> constexpr size_t kManySmem = 1024 + kManyStages<NP> * (kCodeBytes + NP * 256) + kRaw<NP> * kRawBytes<G>;
 
 RB_DEVICE void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
                  "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
+// (x0, x1) <- (x0, x1) + (m, m) * (a0, a1), one instruction
+RB_DEVICE void fma2(float2& x, float m, float a0, float a1) {
+  asm("{\n\t.reg .b64 x, m, a;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 a, {%3, %4};\n\tfma.rn.f32x2 x, m, a, x;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x.x), "+f"(x.y) : "f"(m), "f"(a0), "f"(a1));
 }
 template <typename T> RB_DEVICE float2 pair_of(uint32_t w) {
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -255,25 +267,32 @@ template <typename T> RB_DEVICE float2 pair_of(uint32_t w) {
 // NP: rows of x, padded (rows beyond M read as zeros)
 template <typename T, int G, int NP>
 __global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid_constant__ CUtensorMap xmap, const LinearParams p) {
-  constexpr int NG = 128 / G, ND = kBufs, kCols = NP / 2, kX = NP * 256;
+  constexpr int NG = 128 / G, ND = kBufs, kCols = NP / 2, kX = NP * 256, kStages = kManyStages<NP>, kR = kRaw<NP>, kSums = 3;
   extern __shared__ unsigned char raw[];
-  __shared__ __align__(8) uint64_t code_full[kStages], x_full[kStages], empty[kStages], d_full[ND], d_empty[ND];
-  __shared__ __align__(16) float xsum[2][NG][NP];
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], d_full[ND], d_empty[ND], raw_full[kR], raw_empty[kR];
+  __shared__ __align__(16) float xsum[kSums][NG][NP];
+  __shared__ uint32_t groups[kStages][kManyRows * NG];
   __shared__ uint32_t tmem_ptr, dead_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile uint32_t* dead = &dead_flag;
-  const uint32_t base = (ptx::smem_u32(raw) + 1023u) & ~1023u, codes = base, xs = base + kStages * kCodeBytes;
+  const uint32_t base = (ptx::smem_u32(raw) + 1023u) & ~1023u, codes = base, xs = base + kStages * kCodeBytes, packed = xs + kStages * kX;
   auto bar = [](uint64_t* b, int i) { return ptx::smem_u32(&b[i]); };
+  // ring slot n % size, in its (n / size)-th round: what fills it waits for the other parity
+  auto wait_full = [&](uint64_t* b, int n, int size) { bounded_wait(ptx::smem_u32(&b[n % size]), n / size & 1, dead); };
+  auto wait_empty = [&](uint64_t* b, int n, int size) { bounded_wait(ptx::smem_u32(&b[n % size]), (n / size & 1) ^ 1, dead); };
   if (threadIdx.x == 0) {
     *dead = 0;
     for (int i = 0; i < kStages; ++i) {
-      ptx::mbar_init(bar(code_full, i), kExpand);
-      ptx::mbar_init(bar(x_full, i), 1);
+      ptx::mbar_init(bar(full, i), kExpand / kTeams + 1);       // the codes' warps and the copy of x
       ptx::mbar_init(bar(empty, i), 1 + kScale);
     }
     for (int i = 0; i < ND; ++i) {
       ptx::mbar_init(bar(d_full, i), 1);
       ptx::mbar_init(bar(d_empty, i), kScale);
+    }
+    for (int i = 0; i < kR; ++i) {
+      ptx::mbar_init(bar(raw_full, i), 1);
+      ptx::mbar_init(bar(raw_empty, i), kExpand / kTeams);
     }
     ptx::fence_barrier_init();
   }
@@ -288,156 +307,168 @@ __global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid
   rb::pdl_trigger();
   rb::pdl_wait();
   // this block's part of the channels
-  const int per = RB_CEIL_DIV(p.kblocks, p.splits), k0 = min(p.kblocks, (int)blockIdx.y * per), k1 = min(p.kblocks, k0 + per);
-  auto tile_of = [&](int i) { return p.q + (int64_t)min((int)blockIdx.x * (kManyRows / 16) + i, p.tiles - 1) * p.kblocks * WTile<G>::kWords; };
-  float acc[kCols];
+  const int per = RB_CEIL_DIV(p.kblocks, p.splits), k0 = min(p.kblocks, (int)blockIdx.y * per), blocks = min(p.kblocks, k0 + per) - k0;
+  float2 acc[kCols / 2];
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+  for (int i = 0; i < kCols / 2; ++i) acc[i] = make_float2(0.f, 0.f);
 
   if (warp < kExpand) {
-    // ---- codes to operands: warp w has rows 16 w .. and 64 + 16 w .., a lane the words of rows g and g + 8 of its four steps; odd rows store them in another order, so that the eight
-    // lanes of a store meet all banks
-    const int g = lane >> 2, t = lane & 3, odd = g & 1;
-    const uint32_t* tile[2] = {tile_of(warp), tile_of(warp + 4)};
-    uint4 next[2][2];
-    auto ask = [&](int kb) {
+    // ---- codes to operands: a team of four warps has every second block (its waits, fences and stores pass beside the other's arithmetic), a warp two tiles of it, a lane the words
+    // of rows g and g + 8 of their four steps; odd rows store them in another order, so that the eight lanes of a store meet all banks
+    constexpr int kMine = 8 / (kExpand / kTeams);
+    const int g = lane >> 2, t = lane & 3, odd = g & 1, w0 = warp / kTeams * kMine;
+    for (int n = warp % kTeams; n < blocks; n += kTeams) {
+      wait_full(raw_full, n, kR);
+      const uint32_t from = packed + n % kR * kRawBytes<G> + w0 * (WTile<G>::kWords * 4) + lane * 16;
+      wait_empty(empty, n, kStages);
+      const uint32_t to = codes + n % kStages * kCodeBytes + (w0 * 16 + g) * 128;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < kMine; ++u) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) next[u][h] = load_stream(tile[u] + (int64_t)kb * WTile<G>::kWords + h * 128 + lane * 4);
-    };
-    if (k0 < k1) ask(k0);
-    int st = 0;
-    uint32_t turn = 1;                              // (the first round of a ring is free)
-    for (int kb = k0; kb < k1; ++kb) {
-      uint32_t w[2][2][4];
+        for (int i = lane; i < 16 * NG; i += 32) {
+          uint32_t word;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(word) : "r"(from - lane * 16 + u * (WTile<G>::kWords * 4) + 1024 + i * 4) : "memory");
+          groups[n % kStages][(w0 + u) * 16 * NG + i] = word;
+        }
+        uint4 v[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int h = 0; h < 2; ++h) v[h] = ld_shared_v4(from + u * (WTile<G>::kWords * 4) + h * 512);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) { w[u][h][0] = next[u][h].x; w[u][h][1] = next[u][h].y; w[u][h][2] = next[u][h].z; w[u][h][3] = next[u][h].w; }
-      if (kb + 1 < k1) ask(kb + 1);
-      bounded_wait(bar(empty, st), turn, dead);
-      const uint32_t to = codes + st * kCodeBytes + (warp * 16 + g) * 128;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj) {
             uint32_t e[4];
-            expand<T>(odd ? w[u][h][jj ^ 1] : w[u][h][jj], e);
+            expand<T>(odd ? w[jj ^ 1] : w[jj], e);
             const int j = jj ^ odd;                 // channels 32 j + 8 t ..: piece 4 (j & 1) + t of half j >> 1
-            st_shared_v4(to + u * (64 * 128) + h * (8 * 128) + (j >> 1) * (kManyRows * 128) + ((((j & 1) * 4 + t) ^ g) << 4), e[0], e[1], e[2], e[3]);
+            st_shared_v4(to + u * (16 * 128) + h * (8 * 128) + (j >> 1) * (kManyRows * 128) + ((((j & 1) * 4 + t) ^ g) << 4), e[0], e[1], e[2], e[3]);
           }
+        }
+      }
       ptx::fence_proxy_async();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(code_full, st));
-      if (++st == kStages) { st = 0; turn ^= 1; }
+      if (lane == 0) {
+        ptx::mbar_arrive(bar(full, n % kStages));
+        ptx::mbar_arrive(bar(raw_empty, n % kR));
+      }
     }
   } else if (warp < kLoadWarp) {
-    // ---- sums: warp has 32 output rows (a quarter of the lanes of tensor memory) and half of the rows of x
-    const int e = warp - kExpand, quarter = warp % 4, half = e / 4, tid = e * 32 + lane;
-    constexpr int kEach = 2 * 128 / NP, kPieces = 16 / kEach;      // threads a row of x, 16-byte pieces a thread of its 128 channels
+    // ---- sums: a warp has 32 output rows, a quarter of the lanes of tensor memory, and half of the rows of x
+    const int quarter = warp % 4, half = (warp - kExpand) / 4, tid = (warp - kExpand) * 32 + lane;
+    constexpr int kEach = kScale * 32 / NP, kPieces = 16 / kEach;                // threads a row of x, 16-byte pieces a thread of its 128 channels
+    constexpr int kSpan = kPieces * 8, kOwn = kSpan > G ? kSpan / G : 1, kShare = kSpan < G ? G / kSpan : 1;   // channels of a thread, groups that it sums alone, threads of a group
     const int col = tid / kEach, sub = tid % kEach, row = quarter * 32 + lane;
-    const uint32_t* tile = tile_of(row / 16) + 256 + row % 16 * NG;
-    uint32_t next[NG];
-    auto ask = [&](int kb) {
+    // the sums of x over the groups of block n, one block ahead of the products' use: a thread's pieces lie in one group, or are whole groups
+    auto sums_of = [&](int n, uint32_t (&word)[NG]) {
+      if (n >= blocks) return;
+      wait_full(full, n, kStages);
+      float2 s[kOwn];
 #pragma unroll
-      for (int q = 0; q < NG; ++q) next[q] = __ldg(tile + (int64_t)kb * WTile<G>::kWords + q);
-    };
-    if (k0 < k1) ask(k0);
-    int st = 0, buf = 0;
-    uint32_t turn = 0, dturn = 0;
-    for (int kb = k0; kb < k1; ++kb) {
-      uint32_t word[NG];
-#pragma unroll
-      for (int q = 0; q < NG; ++q) word[q] = next[q];
-      if (kb + 1 < k1) ask(kb + 1);
-      // the sums of x over the groups: a thread's pieces lie in one group, or are whole groups
-      bounded_wait(bar(x_full, st), turn, dead);
-      constexpr int kSpan = kPieces * 8, kOwn = kSpan > G ? kSpan / G : 1, kShare = kSpan < G ? G / kSpan : 1;   // channels of a thread, groups that it sums alone, threads of a group
-      float s[kOwn];
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) s[i] = 0.f;
+      for (int i = 0; i < kOwn; ++i) s[i] = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int piece = sub * kPieces + i;
-        const uint4 v = ld_shared_v4(xs + st * kX + (piece >> 3) * (NP * 128) + col * 128 + (((piece & 7) ^ (col & 7)) << 4));
-        const float2 a = pair_of<T>(v.x), b = pair_of<T>(v.y), c = pair_of<T>(v.z), d = pair_of<T>(v.w);
-        s[i * kOwn / kPieces] += ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
-      }
-      if constexpr (kSpan < G) {
+        const uint4 v = ld_shared_v4(xs + n % kStages * kX + (piece >> 3) * (NP * 128) + col * 128 + (((piece & 7) ^ (col & 7)) << 4));
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int o = 1; o < kShare; o <<= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = pair_of<T>(u[e]);
+          add_pair(s[i * kOwn / kPieces].x, s[i * kOwn / kPieces].y, a.x, a.y);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < kOwn; ++i)
-        if (sub % kShare == 0) xsum[kb & 1][sub / kShare * kOwn + i][col] = s[i];
+      for (int i = 0; i < kOwn; ++i) {
+        float total = s[i].x + s[i].y;
+#pragma unroll
+        for (int o = 1; o < kShare; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (sub % kShare == 0) xsum[n % kSums][sub / kShare * kOwn + i][col] = total;
+      }
+#pragma unroll
+      for (int q = 0; q < NG; ++q) word[q] = groups[n % kStages][row * NG + q];
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(empty, st));
-      if (++st == kStages) { st = 0; turn ^= 1; }
-      asm volatile("bar.sync 1, %0;" ::"n"(kScale * 32) : "memory");
+      if (lane == 0) ptx::mbar_arrive(bar(empty, n % kStages));
+    };
+    uint32_t next[NG];
+    sums_of(0, next);
+    for (int n = 0; n < blocks; ++n) {
+      uint32_t word[NG];
+#pragma unroll
+      for (int q = 0; q < NG; ++q) word[q] = next[q];
+      sums_of(n + 1, next);
+      asm volatile("bar.sync 1, %0;" ::"n"(kScale * 32) : "memory");             // (sums of block n are there, and those of n - 2 are done with: three sets)
 #pragma unroll
       for (int q = 0; q < NG; ++q) {
-        bounded_wait(bar(d_full, buf), dturn, dead);
+        const int d_at = n * NG + q;
+        wait_full(d_full, d_at, ND);
         ptx::tc_fence_after();
         const float scale = q4::scale_of<T>(word[q]), low = q4::low_of<T>(word[q]);
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + d_at % ND * NP + half * kCols;
+        uint32_t d[2][16];
+        tc_ld16(from, d[0]);
 #pragma unroll
-        for (int c = 0; c < kCols; c += 16) {
-          uint32_t d[16];
-          tc_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + buf * NP + half * kCols + c, d);
+        for (int c = 0; c < kCols / 16; ++c) {
           ptx::tc_wait_ld();
+          if (c + 1 < kCols / 16) tc_ld16(from + (c + 1) * 16, d[(c + 1) & 1]);
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(&xsum[kb & 1][q][half * kCols + c + i]);
-            acc[c + i] = fmaf(scale, __uint_as_float(d[i]), fmaf(low, x.x, acc[c + i]));
-            acc[c + i + 1] = fmaf(scale, __uint_as_float(d[i + 1]), fmaf(low, x.y, acc[c + i + 1]));
-            acc[c + i + 2] = fmaf(scale, __uint_as_float(d[i + 2]), fmaf(low, x.z, acc[c + i + 2]));
-            acc[c + i + 3] = fmaf(scale, __uint_as_float(d[i + 3]), fmaf(low, x.w, acc[c + i + 3]));
+            const float4 x = *reinterpret_cast<const float4*>(&xsum[n % kSums][q][half * kCols + c * 16 + i]);
+            float2 &u = acc[c * 8 + i / 2], &v = acc[c * 8 + i / 2 + 1];
+            fma2(u, low, x.x, x.y);
+            fma2(v, low, x.z, x.w);
+            fma2(u, scale, __uint_as_float(d[c & 1][i]), __uint_as_float(d[c & 1][i + 1]));
+            fma2(v, scale, __uint_as_float(d[c & 1][i + 2]), __uint_as_float(d[c & 1][i + 3]));
           }
         }
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(d_empty, buf));
-        if (++buf == ND) { buf = 0; dturn ^= 1; }
+        if (lane == 0) ptx::mbar_arrive(bar(d_empty, d_at % ND));
       }
     }
   } else if (warp == kLoadWarp) {
-    int st = 0;
-    uint32_t turn = 1;
-    for (int kb = k0; kb < k1; ++kb) {
-      bounded_wait(bar(empty, st), turn, dead);
-      if (ptx::elect_one()) {
-        ptx::mbar_arrive_expect_tx(bar(x_full, st), kX);
-        ptx::tma_load_2d(xs + st * kX, &xmap, bar(x_full, st), kb * 128, 0);
-        ptx::tma_load_2d(xs + st * kX + NP * 128, &xmap, bar(x_full, st), kb * 128 + 64, 0);
+    // ---- copies: codes run ahead of x by what their rings differ in depth
+    constexpr int kLead = kR - kStages;
+    const uint32_t* from = p.q + tile_at<G>(blockIdx.x * 8, k0, p.kblocks);
+    for (int n = 0; n < blocks + kLead; ++n) {
+      if (n < blocks) {
+        wait_empty(raw_empty, n, kR);
+        if (ptx::elect_one()) {
+          ptx::mbar_arrive_expect_tx(bar(raw_full, n % kR), kRawBytes<G>);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(packed + n % kR * kRawBytes<G> + i * (kRawBytes<G> / 2)),
+                         "l"(from + (int64_t)n * (8 * WTile<G>::kWords) + i * (4 * WTile<G>::kWords)), "r"(kRawBytes<G> / 2), "r"(bar(raw_full, n % kR)) : "memory");
+        }
       }
-      if (++st == kStages) { st = 0; turn ^= 1; }
+      const int m = n - kLead;
+      if (m >= 0) {
+        wait_empty(empty, m, kStages);
+        if (ptx::elect_one()) {
+          ptx::mbar_arrive_expect_tx(bar(full, m % kStages), kX);
+          ptx::tma_load_2d(xs + m % kStages * kX, &xmap, bar(full, m % kStages), (k0 + m) * 128, 0);
+          ptx::tma_load_2d(xs + m % kStages * kX + NP * 128, &xmap, bar(full, m % kStages), (k0 + m) * 128 + 64, 0);
+        }
+      }
     }
   } else {
     constexpr uint32_t idesc = ptx::make_idesc_f16(std::is_same<T, __half>::value ? 0 : 1, 128, NP, 0, 0);
     const uint32_t el = ptx::elect_one() ? 1u : 0u;
-    int st = 0, buf = 0;
-    uint32_t turn = 0, dturn = 1;
-    for (int kb = k0; kb < k1; ++kb) {
-      bounded_wait(bar(code_full, st), turn, dead);
-      bounded_wait(bar(x_full, st), turn, dead);
-      const uint32_t a = ptx::desc_lo(codes + st * kCodeBytes, 16), b = ptx::desc_lo(xs + st * kX, 16);
+    for (int n = 0; n < blocks; ++n) {
+      wait_full(full, n, kStages);
+      const uint32_t a = ptx::desc_lo(codes + n % kStages * kCodeBytes, 16), b = ptx::desc_lo(xs + n % kStages * kX, 16);
 #pragma unroll
       for (int q = 0; q < NG; ++q) {
-        bounded_wait(bar(d_empty, buf), dturn, dead);
+        const int d_at = n * NG + q;
+        wait_empty(d_empty, d_at, ND);
         ptx::tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 8 / NG; ++k) {          // 16 channels, 32 bytes of a swizzled row
           const int at = q * (8 / NG) + k;
-          ptx::tc_mma_f16_if(el, tmem + buf * NP, a + (at >> 2) * (kManyRows * 128 >> 4) + (at & 3) * 2, b + (at >> 2) * (NP * 128 >> 4) + (at & 3) * 2, idesc, k != 0);
+          ptx::tc_mma_f16_if(el, tmem + d_at % ND * NP, a + (at >> 2) * (kManyRows * 128 >> 4) + (at & 3) * 2, b + (at >> 2) * (NP * 128 >> 4) + (at & 3) * 2, idesc, k != 0);
         }
-        ptx::tc_commit_if(el, bar(d_full, buf));
-        if (++buf == ND) { buf = 0; dturn ^= 1; }
+        ptx::tc_commit_if(el, bar(d_full, d_at % ND));
       }
-      ptx::tc_commit_if(el, bar(empty, st));
+      ptx::tc_commit_if(el, bar(empty, n % kStages));
       __syncwarp();
-      if (++st == kStages) { st = 0; turn ^= 1; }
     }
   }
   // ---- all products have been read: the ring's place holds the sums where a cluster shares the channels
@@ -446,34 +477,35 @@ __global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid
   ptx::tc_fence_after();
   if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, ND * NP);
   const bool sums = warp >= kExpand && warp < kLoadWarp;
-  const int quarter = warp % 4, half = (warp - kExpand) / 4, r = quarter * 32 + lane, n = blockIdx.x * kManyRows + r;
+  const int r = warp % 4 * 32 + lane, half = (warp - kExpand) / 4, n = blockIdx.x * kManyRows + r;
   T* y = reinterpret_cast<T*>(p.y);
   const float bias = p.bias && n < p.N ? rb::to_f(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
   if (p.splits == 1) {
     if (sums && n < p.N) {
 #pragma unroll
       for (int i = 0; i < kCols; ++i)
-        if (half * kCols + i < p.M) y[(half * kCols + i) * p.ldy + n] = rb::from_f<T>(acc[i] + bias);
+        if (half * kCols + i < p.M) y[(half * kCols + i) * p.ldy + n] = rb::from_f<T>((i & 1 ? acc[i / 2].y : acc[i / 2].x) + bias);
     }
   } else {
     float* part = reinterpret_cast<float*>(raw + (base - ptx::smem_u32(raw)));    // [NP][128]
     if (sums) {
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) part[(half * kCols + i) * kManyRows + r] = acc[i];
+      for (int i = 0; i < kCols; ++i) part[(half * kCols + i) * kManyRows + r] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
     }
     ptx::cluster_sync();
-    if (sums) {                                       // rows of x are dealt out to the cluster's blocks and the eight warps' halves
-      for (int m = blockIdx.y * 2 + half; m < p.M; m += p.splits * 2) {
-        float v = bias;
-        for (int c = 0; c < p.splits; ++c) {
-          uint32_t a;
-          float f;
-          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(base + (m * kManyRows + r) * 4), "r"(c));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
-          v += f;
-        }
-        if (n < p.N) y[m * p.ldy + n] = rb::from_f<T>(v);
+    // rows of x are dealt out to the cluster's blocks and their warps
+    for (int i = threadIdx.x / kManyRows; i * p.splits + blockIdx.y < p.M; i += kManyThreads / kManyRows) {
+      const int m = i * p.splits + blockIdx.y, c128 = threadIdx.x % kManyRows, out = blockIdx.x * kManyRows + c128;
+      if (threadIdx.x >= kManyThreads / kManyRows * kManyRows) break;
+      float v = p.bias && out < p.N ? rb::to_f(reinterpret_cast<const T*>(p.bias)[out]) : 0.f;
+      for (int c = 0; c < p.splits; ++c) {
+        uint32_t a;
+        float f;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(base + (m * kManyRows + c128) * 4), "r"(c));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+        v += f;
       }
+      if (out < p.N) y[m * p.ldy + out] = rb::from_f<T>(v);
     }
   }
   rb::report_given_up(dead, p.status);
@@ -485,7 +517,7 @@ template <typename T, int G, int NP> int many_rows(LinearParams p, cudaStream_t 
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -3;
   if (dev >= 64 || !(opted_in.load(std::memory_order_relaxed) >> dev & 1)) {
-    if (cudaFuncSetAttribute(many_rows_kernel<T, G, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kManySmem<NP>) != cudaSuccess) return -3;
+    if (cudaFuncSetAttribute(many_rows_kernel<T, G, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kManySmem<G, NP>) != cudaSuccess) return -3;
     if (dev < 64) opted_in.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
   }
   CUtensorMap xmap;
@@ -500,7 +532,7 @@ template <typename T, int G, int NP> int many_rows(LinearParams p, cudaStream_t 
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tiles, p.splits);
   cfg.blockDim = dim3(kManyThreads);
-  cfg.dynamicSmemBytes = kManySmem<NP>;
+  cfg.dynamicSmemBytes = kManySmem<G, NP>;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -523,16 +555,16 @@ template <typename T, int G> int run(const void* x, const void* q, const void* b
   if (status == nullptr) return -5;
   for (int m0 = 0; m0 < M;) {
     const int rows = std::min(M - m0, 128);
-    const LinearParams p{(const T*)x + m0 * ldx, bias, (const uint32_t*)q, (T*)y + m0 * ldy, rows, N, K, RB_CEIL_DIV(K, 128), RB_CEIL_DIV(N, 16), 1, ldx, ldy, status};
-    const int rc = rows <= 8 ? few_rows<T, G, 1>(p, s) : rows <= 16 ? few_rows<T, G, 2>(p, s) : rows <= 32 ? many_rows<T, G, 32>(p, s) : rows <= 64 ? many_rows<T, G, 64>(p, s)
-                                                                                                            : many_rows<T, G, 128>(p, s);
+    const LinearParams p{(const T*)x + m0 * ldx, bias, (const uint32_t*)q, (T*)y + m0 * ldy, rows, N, K, RB_CEIL_DIV(K, 128), 1, ldx, ldy, status};
+    const int rc = rows <= 8 ? few_rows<T, G, 1>(p, s) : rows <= 16 ? few_rows<T, G, 2>(p, s) : rows <= 32 ? many_rows<T, G, 32>(p, s)
+                                          : rows <= 64 ? many_rows<T, G, 64>(p, s) : many_rows<T, G, 128>(p, s);
     if (rc != 0) return rc;
     m0 += rows;
   }
   return 0;
 }
 template <typename T, int G> int quantize(const void* w, void* q, int N, int K, int64_t ld, cudaStream_t s) {
-  return rb::launch_pdl(quantize_kernel<T, G>, dim3(RB_CEIL_DIV(N, 16), min(RB_CEIL_DIV(K, 128), 65535)), dim3(256), 0, s, (const T*)w, (uint32_t*)q, N, K, ld) ==
+  return rb::launch_pdl(quantize_kernel<T, G>, dim3(RB_CEIL_DIV(N, 128) * 8, min(RB_CEIL_DIV(K, 128), 65535)), dim3(256), 0, s, (const T*)w, (uint32_t*)q, N, K, ld) ==
                  cudaSuccess ? 0 : -3;
 }
 

@@ -290,7 +290,7 @@ class Int4Linear:
         if bias is not None and (tuple(bias.shape) != (self.N,) or bias.dtype != dtype):
             raise ValueError(f"Int4Linear: a bias [{self.N}] of {dtype}")
         self.bias = bias
-        self.q = torch.zeros(-(-self.N // TILE_ROWS), -(-self.K // 128), TILE_ROWS * 16 + TILE_ROWS * (128 // group), dtype=torch.int32, device=device)
+        self.q = torch.zeros(-(-self.N // 128), -(-self.K // 128), 8, TILE_ROWS * 16 + TILE_ROWS * (128 // group), dtype=torch.int32, device=device)
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scale: torch.Tensor, low: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int4Linear":
@@ -306,14 +306,14 @@ class Int4Linear:
         return self
 
     def _fill(self, codes, scale, low):
-        nt, kb, _ = self.q.shape
+        nt, kb, _, _ = self.q.shape
         self.q.zero_()
-        w = torch.zeros(nt * TILE_ROWS, kb * 16, dtype=torch.int32, device=codes.device)
+        w = torch.zeros(nt * 128, kb * 16, dtype=torch.int32, device=codes.device)
         w[: self.N, : self.K // 8] = _words(codes, _WEIGHT)
-        self.q[..., :256] = _row_order(w.view(nt, TILE_ROWS, kb, 16)).transpose(1, 2).flatten(-2)
-        g = torch.zeros(nt * TILE_ROWS, kb * (128 // self.group), dtype=torch.int32, device=codes.device)
+        self.q[..., :256] = _row_order(w.view(nt, 8, TILE_ROWS, kb, 16)).permute(0, 3, 1, 2, 4).flatten(-2)
+        g = torch.zeros(nt * 128, kb * (128 // self.group), dtype=torch.int32, device=codes.device)
         g[: self.N, : self.K // self.group] = _group_words(scale.contiguous(), low.contiguous())
-        self.q[..., 256:] = g.view(nt, TILE_ROWS, kb, -1).transpose(1, 2).flatten(-2)
+        self.q[..., 256:] = g.view(nt, 8, TILE_ROWS, kb, -1).permute(0, 3, 1, 2, 4).flatten(-2)
 
     def requantize(self, w: torch.Tensor):
         """Refresh the 4-bit copy in place after the weight changed (same buffers: a kept CUDA graph stays valid)."""
@@ -326,9 +326,9 @@ class Int4Linear:
 
     def codes(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """(codes uint8 [N, K], scale, low [N, K / group])."""
-        nt, kb, _ = self.q.shape
-        w = _channel_order(self.q[..., :256].unflatten(-1, (TILE_ROWS, 16))).transpose(1, 2).reshape(nt * TILE_ROWS, kb * 16)
-        g = self.q[..., 256:].unflatten(-1, (TILE_ROWS, -1)).transpose(1, 2).reshape(nt * TILE_ROWS, -1)
+        nt, kb, _, _ = self.q.shape
+        w = _channel_order(self.q[..., :256].unflatten(-1, (TILE_ROWS, 16))).permute(0, 2, 3, 1, 4).reshape(nt * 128, kb * 16)
+        g = self.q[..., 256:].unflatten(-1, (TILE_ROWS, -1)).permute(0, 2, 3, 1, 4).reshape(nt * 128, -1)
         return (_codes(w[: self.N, : self.K // 8], _WEIGHT),) + _group_numbers(g[: self.N, : self.K // self.group], self.dtype)
 
     def dequantize(self) -> torch.Tensor:
