@@ -58,14 +58,25 @@ template <typename T> RB_DEVICE void mma16(float (&c)[4], uint32_t a0, uint32_t 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same onto zeros
+template <typename T> RB_DEVICE void mma16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 template <typename T> constexpr uint32_t kOnes = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
 
-// The codes of a word as pairs of neighbouring channels of type T, exact.
-template <typename T> RB_DEVICE void expand(uint32_t w, uint32_t (&h)[4]) {
+// The codes of a word as pairs of neighbouring channels of type T, exact.  `magic`, 1024 or 128 in both halves, comes as a number that the compiler does not know: mask and
+// magic as two immediates are two instructions where an immediate and a register are one.
+template <typename T> constexpr uint32_t kMagic = std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u;
+template <typename T> RB_DEVICE void expand(uint32_t w, uint32_t (&h)[4], uint32_t magic) {
   if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t u = (i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu) | 0x64006400u;       // 1024 + c, or 1024 + 16 c
+      const uint32_t u = (i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu) | magic;       // 1024 + c, or 1024 + 16 c
       const __half2 x = *reinterpret_cast<const __half2*>(&u);
       const __half2 y = i & 1 ? __hfma2(x, __float2half2_rn(0.0625f), __float2half2_rn(-64.f)) : __hadd2(x, __float2half2_rn(-1024.f));
       h[i] = *reinterpret_cast<const uint32_t*>(&y);
@@ -73,7 +84,7 @@ template <typename T> RB_DEVICE void expand(uint32_t w, uint32_t (&h)[4]) {
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t u = w >> (4 * i) & 0x000f000fu | 0x43004300u;                                       // 128 + c
+      const uint32_t u = w >> (4 * i) & 0x000f000fu | magic;                                       // 128 + c
       const __nv_bfloat162 y = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&u), __float2bfloat162_rn(-128.f));
       h[i] = *reinterpret_cast<const uint32_t*>(&y);
     }
@@ -87,79 +98,112 @@ struct LinearParams {
   int M, N, K, kblocks, splits;
   int64_t ldx, ldy;
   int* status;              // rb_attn_status()
+  uint32_t magic;           // kMagic<T>
 };
 
-RB_DEVICE uint4 load_stream(const uint32_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
-// One block of 128 channels of 16 rows: a lane's words of rows g and g + 8, and their groups'.
+// One block of 128 channels of 16 rows: a lane's words of rows g and g + 8, and their groups', from a tile in shared memory.
 template <int G> struct Block {
   uint32_t w[2][4], g[2][128 / G];
-  RB_DEVICE void load(const uint32_t* tile, int lane) {
+  RB_DEVICE void load(uint32_t tile, int lane) {
     const int r = lane >> 2;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint4 v = load_stream(tile + h * 128 + lane * 4);
+      const uint4 v = ld_shared_v4(tile + h * 512 + lane * 16);
       w[h][0] = v.x; w[h][1] = v.y; w[h][2] = v.z; w[h][3] = v.w;
 #pragma unroll
-      for (int i = 0; i < 128 / G; ++i) g[h][i] = __ldg(tile + 256 + (r + 8 * h) * (128 / G) + i);
+      for (int i = 0; i < 128 / G; ++i)
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(g[h][i]) : "r"(tile + 1024 + ((r + 8 * h) * (128 / G) + i) * 4) : "memory");
     }
   }
 };
+// A warp's ring of blocks on their way, 2176 to 2560 bytes each (registers hold one ahead, and 35 KB an SM were on their way: 2.1 TB/s at any number of rows)
+constexpr int kFewRing = 4;
+template <int G> constexpr int kFewBytes = kFewRows / 16 * WTile<G>::kWords * 4;
+template <int G> constexpr size_t kFewSmem = kFewWarps * kFewRing * kFewBytes<G>;
 
 // NT: sets of eight rows of x
 template <typename T, int G, int NT>
-__global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const LinearParams p) {
+__global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const LinearParams p) {
   constexpr int MT = kFewRows / 16, NG = 128 / G;
-  __shared__ __align__(16) float sums[kFewWarps][NT * 8][kFewRows + 1];
+  extern __shared__ __align__(128) unsigned char few_ring[];
+  __shared__ __align__(16) float sums[2][kFewWarps][NT * 8][kFewRows + 1];    // (of a tile of rows and of the next: a warp may be that far ahead)
   __shared__ float part[NT * 8][kFewRows];
+  __shared__ __align__(8) uint64_t bar[kFewWarps][kFewRing];
+  __shared__ uint32_t dead_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  volatile uint32_t* dead = &dead_flag;
+  if (threadIdx.x == 0) *dead = 0;
+  if (lane < kFewRing) ptx::mbar_init(ptx::smem_u32(&bar[warp][lane]), 1);
+  ptx::fence_barrier_init();
+  __syncthreads();
   rb::pdl_trigger();
-  const int tile0 = blockIdx.x * MT, step = kFewWarps * p.splits, first = blockIdx.y * kFewWarps + warp;
-  const uint32_t* tile[MT];                         // (tiles are padded to whole sets of eight)
-#pragma unroll
-  for (int i = 0; i < MT; ++i) tile[i] = p.q + tile_at<G>(tile0 + i, 0, p.kblocks);
+  // the warp's blocks of a set of 32 output rows, then those of the next set of this block of threads: one sequence, whose copies run ahead of the sums at a set's end
+  const int step = kFewWarps * p.splits, first = blockIdx.y * kFewWarps + warp, sets = RB_CEIL_DIV(p.N, kFewRows);
+  const uint32_t ring = ptx::smem_u32(few_ring) + warp * (kFewRing * kFewBytes<G>);
+  int ask_set = first < p.kblocks ? blockIdx.x : sets, ask_kb = first;
+  auto fetch = [&](int slot) {
+    if (ask_set >= sets) return;
+    if (ptx::elect_one()) {
+      const uint32_t full = ptx::smem_u32(&bar[warp][slot]);
+      ptx::mbar_arrive_expect_tx(full, kFewBytes<G>);
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring + slot * kFewBytes<G>),
+                   "l"(p.q + tile_at<G>(ask_set * MT, ask_kb, p.kblocks)), "r"(kFewBytes<G>), "r"(full) : "memory");
+    }
+    ask_kb += step;
+    if (ask_kb >= p.kblocks) { ask_kb = first; ask_set += gridDim.x; }
+  };
   rb::pdl_wait();
-  Block<G> next[MT];
-  if (first < p.kblocks)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) next[i].load(tile[i] + (int64_t)first * (8 * WTile<G>::kWords), lane);
-  float acc[MT][NT][4] = {};
-  const T* x = reinterpret_cast<const T*>(p.x);
+  for (int i = 0; i < kFewRing; ++i) fetch(i);
+  // rows beyond M repeat the last one and are not stored; channels beyond K read the row's first ones: they meet codes, scales and lowest values of 0
+  const T* x[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) x[n] = reinterpret_cast<const T*>(p.x) + min(n * 8 + g, p.M - 1) * p.ldx + 8 * t;
+  const int cols = min(p.M, NT * 8);
+  int slot = 0, half = 0;
+  uint32_t round = 0;
+#pragma unroll 1
+  for (int set = blockIdx.x; set < sets; set += gridDim.x, half ^= 1) {
+    float acc[MT][NT][4] = {};
+#pragma unroll 1
   for (int kb = first; kb < p.kblocks; kb += step) {
-    Block<G> cur[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) cur[i] = next[i];
     uint4 xv[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int m = n * 8 + g, k = kb * 128 + 32 * j + 8 * t;
-        xv[n][j] = m < p.M && k < p.K ? *reinterpret_cast<const uint4*>(x + m * p.ldx + k) : make_uint4(0, 0, 0, 0);
+        const int k = kb * 128 + 32 * j;
+        xv[n][j] = __ldg(reinterpret_cast<const uint4*>(x[n] + (k < p.K ? k : 0)));      // (K is a multiple of 32)
       }
-    if (kb + step < p.kblocks)
+    bounded_wait(ptx::smem_u32(&bar[warp][slot]), round, dead);
+    Block<G> cur[MT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) next[i].load(tile[i] + (int64_t)(kb + step) * (8 * WTile<G>::kWords), lane);
+    for (int i = 0; i < MT; ++i) cur[i].load(ring + slot * kFewBytes<G> + i * (WTile<G>::kWords * 4), lane);
+    __syncwarp();
+    fetch(slot);
+    if (++slot == kFewRing) { slot = 0; round ^= 1; }
 #pragma unroll
     for (int q = 0; q < NG; ++q) {                  // a group
-      float c[MT][NT][4] = {}, one[NT][4] = {};
+      float c[MT][NT][4], one[NT][4];
 #pragma unroll
       for (int j = q * 4 / NG; j < (q + 1) * 4 / NG; ++j) {
         uint32_t e0[MT][4], e1[MT][4];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          expand<T>(cur[i].w[0][j], e0[i]);
-          expand<T>(cur[i].w[1][j], e1[i]);
+          expand<T>(cur[i].w[0][j], e0[i], p.magic);
+          expand<T>(cur[i].w[1][j], e1[i], p.magic);
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const uint32_t b0 = s ? xv[n][j].z : xv[n][j].x, b1 = s ? xv[n][j].w : xv[n][j].y;
+            if (j == q * 4 / NG && s == 0) {
+              mma16_first<T>(one[n], kOnes<T>, kOnes<T>, kOnes<T>, kOnes<T>, b0, b1);
+#pragma unroll
+              for (int i = 0; i < MT; ++i) mma16_first<T>(c[i][n], e0[i][0], e1[i][0], e0[i][1], e1[i][1], b0, b1);
+              continue;
+            }
             mma16<T>(one[n], kOnes<T>, kOnes<T>, kOnes<T>, kOnes<T>, b0, b1);
 #pragma unroll
             for (int i = 0; i < MT; ++i) mma16<T>(c[i][n], e0[i][2 * s], e1[i][2 * s], e0[i][2 * s + 1], e1[i][2 * s + 1], b0, b1);
@@ -183,22 +227,21 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const LinearParam
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sums[warp][n * 8 + 2 * t + (e & 1)][i * 16 + g + 8 * (e >> 1)] = acc[i][n][e];
+      for (int e = 0; e < 4; ++e) sums[half][warp][n * 8 + 2 * t + (e & 1)][i * 16 + g + 8 * (e >> 1)] = acc[i][n][e];
   __syncthreads();
-  const int cols = min(p.M, NT * 8);
   auto finish = [&](int m, int r, float v) {
-    const int n = blockIdx.x * kFewRows + r;
+    const int n = set * kFewRows + r;
     if (n < p.N) reinterpret_cast<T*>(p.y)[m * p.ldy + n] = rb::from_f<T>(v + (p.bias ? rb::to_f(reinterpret_cast<const T*>(p.bias)[n]) : 0.f));
   };
   for (int i = threadIdx.x; i < cols * kFewRows; i += kFewThreads) {
     const int m = i / kFewRows, r = i % kFewRows;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) v += sums[w][m][r];
+    for (int w = 0; w < kFewWarps; ++w) v += sums[half][w][m][r];
     if (p.splits == 1) finish(m, r, v); else part[m][r] = v;
   }
-  if (p.splits == 1) return;
-  ptx::cluster_sync();
+  if (p.splits == 1) continue;
+  ptx::cluster_sync();                              // (a cluster has one set)
   for (int i = blockIdx.y * kFewThreads + threadIdx.x; i < cols * kFewRows; i += p.splits * kFewThreads) {
     const int m = i / kFewRows, r = i % kFewRows;
     float v = 0.f;
@@ -211,16 +254,26 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const LinearParam
     }
     finish(m, r, v);
   }
-  ptx::cluster_sync();  // nobody leaves while its sums are being read
+  }
+  rb::report_given_up(dead, p.status);
+  if (p.splits > 1) ptx::cluster_sync();  // nobody leaves while its sums are being read
 }
 
 template <typename T, int G, int NT> int few_rows(LinearParams p, cudaStream_t s) {
-  const int blocks = RB_CEIL_DIV(p.N, kFewRows);
+  static std::atomic<uint64_t> opted_in{0};           // the attribute is the kernel's on one device: a bit per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -3;
+  if (dev >= 64 || !(opted_in.load(std::memory_order_relaxed) >> dev & 1)) {
+    if (cudaFuncSetAttribute(few_rows_kernel<T, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewSmem<G>) != cudaSuccess) return -3;
+    if (dev < 64) opted_in.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  }
+  const int sets = RB_CEIL_DIV(p.N, kFewRows), blocks = std::min(sets, 2 * rb::kNumSMs);
   p.splits = 1;
-  while (p.splits < kMaxSplits && blocks * p.splits * 2 <= 2 * rb::kNumSMs && p.kblocks >= kFewWarps * p.splits * 2) p.splits *= 2;
+  while (p.splits < kMaxSplits && sets * p.splits * 2 <= 2 * rb::kNumSMs && p.kblocks >= kFewWarps * p.splits * 2) p.splits *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(blocks, p.splits);
   cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = kFewSmem<G>;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -339,7 +392,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj) {
             uint32_t e[4];
-            expand<T>(odd ? w[jj ^ 1] : w[jj], e);
+            expand<T>(odd ? w[jj ^ 1] : w[jj], e, p.magic);
             const int j = jj ^ odd;                 // channels 32 j + 8 t ..: piece 4 (j & 1) + t of half j >> 1
             st_shared_v4(to + u * (16 * 128) + h * (8 * 128) + (j >> 1) * (kManyRows * 128) + ((((j & 1) * 4 + t) ^ g) << 4), e[0], e[1], e[2], e[3]);
           }
@@ -555,7 +608,7 @@ template <typename T, int G> int run(const void* x, const void* q, const void* b
   if (status == nullptr) return -5;
   for (int m0 = 0; m0 < M;) {
     const int rows = std::min(M - m0, 128);
-    const LinearParams p{(const T*)x + m0 * ldx, bias, (const uint32_t*)q, (T*)y + m0 * ldy, rows, N, K, RB_CEIL_DIV(K, 128), 1, ldx, ldy, status};
+    const LinearParams p{(const T*)x + m0 * ldx, bias, (const uint32_t*)q, (T*)y + m0 * ldy, rows, N, K, RB_CEIL_DIV(K, 128), 1, ldx, ldy, status, kMagic<T>};
     const int rc = rows <= 8 ? few_rows<T, G, 1>(p, s) : rows <= 16 ? few_rows<T, G, 2>(p, s) : rows <= 32 ? many_rows<T, G, 32>(p, s)
                                           : rows <= 64 ? many_rows<T, G, 64>(p, s) : many_rows<T, G, 128>(p, s);
     if (rc != 0) return rc;
