@@ -141,16 +141,22 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const LinearPa
   const int step = kFewWarps * p.splits, first = blockIdx.y * kFewWarps + warp, sets = RB_CEIL_DIV(p.N, kFewRows);
   const uint32_t ring = ptx::smem_u32(few_ring) + warp * (kFewRing * kFewBytes<G>);
   int ask_set = first < p.kblocks ? blockIdx.x : sets, ask_kb = first;
+  const uint32_t* ask = p.q + tile_at<G>(ask_set * MT, first, p.kblocks);
   auto fetch = [&](int slot) {
     if (ask_set >= sets) return;
     if (ptx::elect_one()) {
       const uint32_t full = ptx::smem_u32(&bar[warp][slot]);
       ptx::mbar_arrive_expect_tx(full, kFewBytes<G>);
       asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring + slot * kFewBytes<G>),
-                   "l"(p.q + tile_at<G>(ask_set * MT, ask_kb, p.kblocks)), "r"(kFewBytes<G>), "r"(full) : "memory");
+                   "l"(ask), "r"(kFewBytes<G>), "r"(full) : "memory");
     }
     ask_kb += step;
-    if (ask_kb >= p.kblocks) { ask_kb = first; ask_set += gridDim.x; }
+    ask += step * (8 * WTile<G>::kWords);
+    if (ask_kb >= p.kblocks) {
+      ask_kb = first;
+      ask_set += gridDim.x;
+      ask = p.q + tile_at<G>(ask_set * MT, first, p.kblocks);
+    }
   };
   rb::pdl_wait();
 #pragma unroll
@@ -168,13 +174,19 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const LinearPa
 #pragma unroll 1
   for (int kb = first; kb < p.kblocks; kb += step) {
     uint4 xv[NT][4];
+    if (kb * 128 + 128 <= p.K) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        const uint4* from = reinterpret_cast<const uint4*>(x[n] + kb * 128);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = kb * 128 + 32 * j;
-        xv[n][j] = __ldg(reinterpret_cast<const uint4*>(x[n] + (k < p.K ? k : 0)));      // (K is a multiple of 32)
+        for (int j = 0; j < 4; ++j) xv[n][j] = __ldg(from + 4 * j);
       }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xv[n][j] = __ldg(reinterpret_cast<const uint4*>(x[n] + (kb * 128 + 32 * j < p.K ? kb * 128 + 32 * j : 0)));   // (K is a multiple of 32)
+    }
     bounded_wait(ptx::smem_u32(&bar[warp][slot]), round, dead);
     Block<G> cur[MT];
 #pragma unroll
