@@ -305,8 +305,9 @@ template <typename T, int G, int NT> int few_rows(LinearParams p, cudaStream_t s
 
 // ---------------------------------------------------------------------------------------------- many rows
 
-constexpr int kManyRows = 128, kTeams = 2, kExpand = 4 * kTeams, kScale = 8;         // output rows; warps that expand (a team of four has every second block), that scale
-constexpr int kLoadWarp = kExpand + kScale, kMmaWarp = kLoadWarp + 1, kManyThreads = (kMmaWarp + 1) * 32;
+constexpr int kManyRows = 128, kTeams = 2, kScale = 8;                               // output rows; teams of warps that expand (each has every second block), warps that scale
+template <int NP> constexpr int kTeam = NP == 128 ? 2 : 4;                           // warps of a team (128 rows: scaling takes longer, and needs the registers)
+template <int NP> constexpr int kManyThreads = (kTeams * kTeam<NP> + kScale + 2) * 32;
 constexpr int kCodeBytes = kManyRows * 256;                                          // 128 rows x 128 channels of 16 bits: two halves of 64 channels
 constexpr int kBufs = 4;                                                             // accumulators
 template <int NP> constexpr int kManyStages = NP == 32 ? 4 : NP == 64 ? 3 : 2;       // operand tiles
@@ -331,8 +332,9 @@ template <typename T> RB_DEVICE float2 pair_of(uint32_t w) {
 
 // NP: rows of x, padded (rows beyond M read as zeros)
 template <typename T, int G, int NP>
-__global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid_constant__ CUtensorMap xmap, const LinearParams p) {
+__global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __grid_constant__ CUtensorMap xmap, const LinearParams p) {
   constexpr int NG = 128 / G, ND = kBufs, kCols = NP / 2, kX = NP * 256, kStages = kManyStages<NP>, kR = kRaw<NP>, kSums = 3;
+  constexpr int kExpand = kTeams * kTeam<NP>, kLoadWarp = kExpand + kScale, kMmaWarp = kLoadWarp + 1;
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], d_full[ND], d_empty[ND], raw_full[kR], raw_empty[kR];
   __shared__ __align__(16) float xsum[kSums][NG][NP];
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid
   if (threadIdx.x == 0) {
     *dead = 0;
     for (int i = 0; i < kStages; ++i) {
-      ptx::mbar_init(bar(full, i), kExpand / kTeams + 1);       // the codes' warps and the copy of x
+      ptx::mbar_init(bar(full, i), kTeam<NP> + 1);       // the codes' warps and the copy of x
       ptx::mbar_init(bar(empty, i), 1 + kScale);
     }
     for (int i = 0; i < ND; ++i) {
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid
     }
     for (int i = 0; i < kR; ++i) {
       ptx::mbar_init(bar(raw_full, i), 1);
-      ptx::mbar_init(bar(raw_empty, i), kExpand / kTeams);
+      ptx::mbar_init(bar(raw_empty, i), kTeam<NP>);
     }
     ptx::fence_barrier_init();
   }
@@ -378,9 +380,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid
   for (int i = 0; i < kCols / 2; ++i) acc[i] = make_float2(0.f, 0.f);
 
   if (warp < kExpand) {
-    // ---- codes to operands: a team of four warps has every second block (its waits, fences and stores pass beside the other's arithmetic), a warp two tiles of it, a lane the words
+    // ---- codes to operands: a team of warps has every second block (its waits, fences and stores pass beside the other's arithmetic), a warp two or four tiles of it, a lane the words
     // of rows g and g + 8 of their four steps; odd rows store them in another order, so that the eight lanes of a store meet all banks
-    constexpr int kMine = 8 / (kExpand / kTeams);
+    constexpr int kMine = 8 / (kTeam<NP>);
     const int g = lane >> 2, t = lane & 3, odd = g & 1, w0 = warp / kTeams * kMine;
     for (int n = warp % kTeams; n < blocks; n += kTeams) {
       wait_full(raw_full, n, kR);
@@ -468,20 +470,20 @@ __global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid
         ptx::tc_fence_after();
         const float scale = q4::scale_of<T>(word[q]), low = q4::low_of<T>(word[q]);
         const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + d_at % ND * NP + half * kCols;
-        uint32_t d[2][16];
-        tc_ld16(from, d[0]);
+        constexpr int kAtOnce = kCols < 32 ? kCols : 32;     // (a wait is for all loads, and takes as long for 32 columns as for 16)
 #pragma unroll
-        for (int c = 0; c < kCols / 16; ++c) {
+        for (int c = 0; c < kCols; c += kAtOnce) {
+          uint32_t d[kAtOnce];
+          if constexpr (kAtOnce == 32) ptx::tc_ld_32x32(from + c, d); else tc_ld16(from + c, d);
           ptx::tc_wait_ld();
-          if (c + 1 < kCols / 16) tc_ld16(from + (c + 1) * 16, d[(c + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(&xsum[n % kSums][q][half * kCols + c * 16 + i]);
-            float2 &u = acc[c * 8 + i / 2], &v = acc[c * 8 + i / 2 + 1];
+          for (int i = 0; i < kAtOnce; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(&xsum[n % kSums][q][half * kCols + c + i]);
+            float2 &u = acc[(c + i) / 2], &v = acc[(c + i) / 2 + 1];
             fma2(u, low, x.x, x.y);
             fma2(v, low, x.z, x.w);
-            fma2(u, scale, __uint_as_float(d[c & 1][i]), __uint_as_float(d[c & 1][i + 1]));
-            fma2(v, scale, __uint_as_float(d[c & 1][i + 2]), __uint_as_float(d[c & 1][i + 3]));
+            fma2(u, scale, __uint_as_float(d[i]), __uint_as_float(d[i + 1]));
+            fma2(v, scale, __uint_as_float(d[i + 2]), __uint_as_float(d[i + 3]));
           }
         }
         ptx::tc_fence_before();
@@ -559,9 +561,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) many_rows_kernel(const __grid
     }
     ptx::cluster_sync();
     // rows of x are dealt out to the cluster's blocks and their warps
-    for (int i = threadIdx.x / kManyRows; i * p.splits + blockIdx.y < p.M; i += kManyThreads / kManyRows) {
+    for (int i = threadIdx.x / kManyRows; i * p.splits + blockIdx.y < p.M; i += kManyThreads<NP> / kManyRows) {
       const int m = i * p.splits + blockIdx.y, c128 = threadIdx.x % kManyRows, out = blockIdx.x * kManyRows + c128;
-      if (threadIdx.x >= kManyThreads / kManyRows * kManyRows) break;
+      if (threadIdx.x >= kManyThreads<NP> / kManyRows * kManyRows) break;
       float v = p.bias && out < p.N ? rb::to_f(reinterpret_cast<const T*>(p.bias)[out]) : 0.f;
       for (int c = 0; c < p.splits; ++c) {
         uint32_t a;
@@ -596,7 +598,7 @@ template <typename T, int G, int NP> int many_rows(LinearParams p, cudaStream_t 
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tiles, p.splits);
-  cfg.blockDim = dim3(kManyThreads);
+  cfg.blockDim = dim3(kManyThreads<NP>);
   cfg.dynamicSmemBytes = kManySmem<G, NP>;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
