@@ -15,6 +15,7 @@ int rb_int4_cache_rows(void* k, void* v, int64_t kt, int64_t kh, int64_t vt, int
 int rb_decode_attention_int4(const void* qkv, void* cache, const int* lens, void* out, const float* cos, const float* sin, int64_t qkv_stride, int B, int nq, int nkv,
                              int hd, int room, int rot_dim, int interleaved, float scale, int dt, cudaStream_t s);
 int rb_int4_quantize(const void* w, void* q, int N, int K, int64_t ld, int group, int dt, cudaStream_t s);
+int rb_int4_pack(const void* codes, const void* scale, const void* low, void* q, int N, int K, int group, cudaStream_t s);
 int rb_int4_linear(const void* x, const void* q, const void* bias, void* y, int M, int N, int K, int64_t ldx, int64_t ldy, int group, int dt, cudaStream_t s);
 }
 
@@ -143,6 +144,21 @@ void int4_quantize(const Tensor& w, Tensor q, int64_t group) {
   TORCH_CHECK(rc == 0, op, ": the kernel could not be launched (", rc, ")");
 }
 
+void int4_pack(const Tensor& codes, const Tensor& scale, const Tensor& low, Tensor q, int64_t group) {
+  const char* op = "int4_pack";
+  TORCH_CHECK_VALUE(codes.dim() == 2 && codes.scalar_type() == at::kByte && codes.device() == q.device(), op, ": codes uint8 [N, K] beside the packed form");
+  check_weight(q, codes.size(0), codes.size(1), group, op);
+  type_of(scale, op);
+  for (const Tensor& t : {scale, low})
+    TORCH_CHECK_VALUE(t.scalar_type() == scale.scalar_type() && t.dim() == 2 && t.size(0) == codes.size(0) && t.size(1) == codes.size(1) / group && t.device() == q.device(), op,
+                      ": steps and lowest values [N, K / group] of one 16-bit type beside the codes");
+  c10::cuda::CUDAGuard guard(q.device());
+  const Tensor c = codes.is_contiguous() && (reinterpret_cast<uintptr_t>(codes.data_ptr()) & 7) == 0 ? codes : codes.clone(at::MemoryFormat::Contiguous);
+  const Tensor s = scale.contiguous(), l = low.contiguous();
+  const int rc = rb_int4_pack(c.data_ptr(), s.data_ptr(), l.data_ptr(), q.data_ptr(), (int)codes.size(0), (int)codes.size(1), (int)group, at::cuda::getCurrentCUDAStream().stream());
+  TORCH_CHECK(rc == 0, op, ": the kernel could not be launched (", rc, ")");
+}
+
 Tensor int4_linear(const Tensor& x, const Tensor& q, const OptT& bias, int64_t N, int64_t group) {
   const char* op = "int4_linear";
   TORCH_CHECK_VALUE(x.dim() == 2 && x.device() == q.device() && x.size(0) <= kInt - 256, op, ": rows [M, K] beside the weight");
@@ -170,5 +186,6 @@ void register_int4_ops(torch::Library& m) {
   m.def("decode_attention_int4(Tensor qkv, Tensor(a!) cache, Tensor cache_lens, int nq, int nkv, int hd, int room, float scale, Tensor? cos, Tensor? sin, int rot_dim, "
         "bool interleaved) -> Tensor", &decode_attention_int4);
   m.def("int4_quantize(Tensor w, Tensor(a!) q, int group) -> ()", &int4_quantize);
+  m.def("int4_pack(Tensor codes, Tensor scale, Tensor low, Tensor(a!) q, int group) -> ()", &int4_pack);
   m.def("int4_linear(Tensor x, Tensor q, Tensor? bias, int n, int group) -> Tensor", &int4_linear);
 }

@@ -37,16 +37,37 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ w, 
   for (int kb = blockIdx.y; kb < kblocks; kb += gridDim.y) {
     const int k = kb * 128 + sub * 8;
     const bool mine = n < N && k < K;
-    rb::Pack<T, 8> a{};
-    if (mine) a = *reinterpret_cast<const rb::Pack<T, 8>*>(w + n * ld + k);
-    float x[8], lo, hi;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = rb::to_f(a.v[i]);
-    q4::extremes<G / 8>(x, lo, hi);
-    const uint32_t g = mine ? q4::group_word<T>(lo, hi) : 0u;
+    uint4 a = make_uint4(0, 0, 0, 0);
+    if (mine) a = *reinterpret_cast<const uint4*>(w + n * ld + k);
+    float lo, hi;
+    q4::extremes<T, G / 8>(a, lo, hi);
+    const q4::Coded c = q4::code8<T, q4::kWeight>(a, lo, hi);
     uint32_t* at = q + tile_at<G>(blockIdx.x, kb, kblocks);
-    at[r * 16 + q4::word_place<4>(sub)] = mine ? q4::pack8<q4::kWeight>(x, q4::scale_of<T>(g), lo) : 0u;
-    if (sub % (G / 8) == 0) at[256 + r * WTile<G>::kGroups + sub / (G / 8)] = g;
+    at[r * 16 + q4::word_place<4>(sub)] = mine ? c.word : 0u;
+    if (sub % (G / 8) == 0) at[256 + r * WTile<G>::kGroups + sub / (G / 8)] = mine ? c.group : 0u;
+  }
+}
+
+// The same from codes, a byte each, and 16-bit steps and lowest values.
+template <int G> __global__ void __launch_bounds__(256) pack_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scale, const uint16_t* __restrict__ low,
+                                                                    uint32_t* __restrict__ q, int N, int K) {
+  const int r = threadIdx.x / 16, sub = threadIdx.x % 16, n = blockIdx.x * 16 + r, kblocks = RB_CEIL_DIV(K, 128);
+  rb::pdl_trigger();
+  rb::pdl_wait();
+  for (int kb = blockIdx.y; kb < kblocks; kb += gridDim.y) {
+    const int k = kb * 128 + sub * 8;
+    const bool mine = n < N && k < K;
+    uint2 c = make_uint2(0, 0);
+    if (mine) c = *reinterpret_cast<const uint2*>(codes + (int64_t)n * K + k);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (c.x >> (8 * i) & 15u) << q4::bit_of<q4::kWeight>(i) | (c.y >> (8 * i) & 15u) << q4::bit_of<q4::kWeight>(4 + i);
+    uint32_t* at = q + tile_at<G>(blockIdx.x, kb, kblocks);
+    at[r * 16 + q4::word_place<4>(sub)] = w;
+    if (sub % (G / 8) == 0) {
+      const int64_t g = (int64_t)n * (K / G) + k / G;
+      at[256 + r * WTile<G>::kGroups + sub / (G / 8)] = mine ? (uint32_t)scale[g] << 16 | low[g] : 0u;
+    }
   }
 }
 
@@ -634,6 +655,10 @@ template <typename T, int G> int quantize(const void* w, void* q, int N, int K, 
   return rb::launch_pdl(quantize_kernel<T, G>, dim3(RB_CEIL_DIV(N, 128) * 8, min(RB_CEIL_DIV(K, 128), 65535)), dim3(256), 0, s, (const T*)w, (uint32_t*)q, N, K, ld) ==
                  cudaSuccess ? 0 : -3;
 }
+template <int G> int pack(const void* codes, const void* scale, const void* low, void* q, int N, int K, cudaStream_t s) {
+  return rb::launch_pdl(pack_kernel<G>, dim3(RB_CEIL_DIV(N, 128) * 8, min(RB_CEIL_DIV(K, 128), 65535)), dim3(256), 0, s, (const uint8_t*)codes, (const uint16_t*)scale,
+                        (const uint16_t*)low, (uint32_t*)q, N, K) == cudaSuccess ? 0 : -3;
+}
 
 }  // namespace
 
@@ -643,6 +668,12 @@ extern "C" int rb_int4_quantize(const void* w, void* q, int N, int K, int64_t ld
 #define RB_G(T) (group == 32 ? quantize<T, 32>(w, q, N, K, ld, s) : group == 64 ? quantize<T, 64>(w, q, N, K, ld, s) : group == 128 ? quantize<T, 128>(w, q, N, K, ld, s) : -1)
   return dt == 1 ? RB_G(__nv_bfloat16) : dt == 2 ? RB_G(__half) : -2;
 #undef RB_G
+}
+
+// codes [N, K] and steps and lowest values [N, K / group], contiguous; codes on 8 bytes
+extern "C" int rb_int4_pack(const void* codes, const void* scale, const void* low, void* q, int N, int K, int group, cudaStream_t s) {
+  if (N == 0 || K == 0) return 0;
+  return group == 32 ? pack<32>(codes, scale, low, q, N, K, s) : group == 64 ? pack<64>(codes, scale, low, q, N, K, s) : group == 128 ? pack<128>(codes, scale, low, q, N, K, s) : -1;
 }
 
 extern "C" int rb_int4_linear(const void* x, const void* q, const void* bias, void* y, int M, int N, int K, int64_t ldx, int64_t ldy, int group, int dt, cudaStream_t s) {

@@ -302,7 +302,10 @@ class Int4Linear:
             raise ValueError("Int4Linear.from_codes: a code is 0 .. 15")
         self = cls.__new__(cls)
         self._plan(codes.shape, codes.shape[1] // scale.shape[1], scale.dtype, codes.device, bias)
-        self._fill(codes, scale, low)
+        if use_native(codes):
+            lib().int4_pack(codes, scale, low, self.q, self.group)
+        else:
+            self._fill(codes, scale, low)
         return self
 
     def _fill(self, codes, scale, low):

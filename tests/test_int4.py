@@ -172,6 +172,35 @@ def test_cache_bits_are_the_same_on_both_devices(dtype, hd):
     assert kb[6, 0, :32].isnan().all() and not kb[6, 0, 32:].isnan().any() and vb[7, 2, :64].isnan().all() and vb[8, 1, :64].isnan().all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_group_bits_at_any_size(dtype):
+    """Groups of every power of two of the type, the smallest numbers and the widest range among them, word for word as on the CPU: in a cache and in a weight."""
+    g = torch.Generator().manual_seed(3)
+    bits = torch.randint(0, 1 << 15, (256, 2, 64), generator=g).short().view(dtype)                # numbers of any size, side by side
+    bits = torch.where(torch.isfinite(bits), bits, torch.ones_like(bits))
+    info = torch.finfo(dtype)
+    powers = range(int(math.log2(info.smallest_normal)) - 8, int(math.log2(info.max)) - 3)
+    scaled = torch.stack([(rows(g, 2, 64, dtype=torch.float32, device="cpu").double() * 2.0 ** p).to(dtype) for p in powers])
+    ties = torch.stack([(torch.randint(-30, 31, (2, 64), generator=g).double() / 2 * 2.0 ** p).to(dtype) for p in powers])
+    ends = torch.zeros(4, 2, 64, dtype=dtype)
+    ends[0, :, ::2], ends[1, :, ::2], ends[1, :, 1::2], ends[2], ends[3, :, :5] = info.max, info.max, -info.max, -0.0, info.smallest_normal
+    x = torch.cat([bits, -bits, scaled, scaled + 1, ties, ends])
+    n = x.shape[0]
+    a, b = (int4.Int4KVCache(1, n, 2, 64, dtype, d) for d in ("cpu", "cuda"))
+    a.store(x, x.flip(0), packed([n], "cpu"))
+    b.store(x.cuda(), x.flip(0).cuda(), packed([n], "cuda"))
+    for p, q in zip(a.load(packed([n], "cpu"), n), b.load(packed([n], "cuda"), n)):
+        assert torch.equal(p, q.cpu())
+    for p, q in zip(a._fields()[:2], b._fields()[:2]):
+        assert torch.equal(p, q.cpu())
+    for group in int4.GROUPS:
+        w = x.reshape(-1, 128)
+        p, q = int4.Int4Linear(w, group=group), int4.Int4Linear(w.cuda(), group=group)
+        for s, t in zip(p.codes(), q.codes()):
+            assert torch.equal(s, t.cpu())
+
+
 # ------------------------------------------------------------------------------------------------ attention
 
 
@@ -408,6 +437,19 @@ def test_weight_round_trip(device, dtype, N, K, group):
     assert torch.equal(again.q, lin.q)
     lin.requantize(w * 2)
     check_groups(lin.dequantize(), w * 2, group, dtype, rounded=False)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,K,group", [(1, 32, 32), (33, 192, 64), (130, 384, 128), (300, 160, 32)])
+def test_weights_of_codes(device, dtype, N, K, group):
+    g = torch.Generator().manual_seed(N)
+    c = torch.randint(0, 16, (N, K + 3), generator=g, dtype=torch.uint8).to(device)[:, 3:]          # strided, off by three bytes
+    s, lo = (rows(g, K // group, N, dtype=dtype, device=device).t() for _ in range(2))
+    lin = int4.Int4Linear.from_codes(c, s, lo)
+    for a, b in zip(lin.codes(), (c, s, lo)):
+        assert torch.equal(a, b)
+    assert torch.equal(lin.q.cpu(), int4.Int4Linear.from_codes(c.cpu(), s.cpu(), lo.cpu()).q)       # ... and zeros beyond N and K
 
 
 def check_linear(lin, x, bias=None):
