@@ -169,7 +169,8 @@ Tensor int4_linear(const Tensor& x, const Tensor& q, const OptT& bias, int64_t N
                     op, ": a bias [", N, "] of the rows' type");
   attn_check();
   c10::cuda::CUDAGuard guard(x.device());
-  const Tensor rows = rows16(x);
+  // (a row repeated by a stride of 0, or rows that overlap, are copied: a tensor map does not take them)
+  const Tensor rows = M > 1 && x.stride(0) < K ? x.clone(at::MemoryFormat::Contiguous) : rows16(x);
   auto y = at::empty({M, N}, x.options());
   const int rc = rb_int4_linear(rows.data_ptr(), q.data_ptr(), bias.has_value() ? bias->data_ptr() : nullptr, y.data_ptr(), (int)M, (int)N, (int)K, rows.stride(0), N, (int)group, dt,
                                 at::cuda::getCurrentCUDAStream().stream());

@@ -10,7 +10,7 @@ so a value is off by at most half a step (and 15 roundings of the step).  A grou
   others, and a small group keeps them to themselves) and of 64 channels of a value: 4.75 bits a number, 3.4 times less than 16.  `store` quantises the
   keys and values of packed sequences, `load` reads them back, `decode_attention_int4` appends a token and attends to all rows as the cache holds them.
 * `Int4Linear`: a weight [N, K] with groups of 32, 64 or 128 along K and its products with rows of any number; made for the few rows of a decode step,
-  where the weights' bytes are the time.
+  where the weights' bytes are the time.  None of these has a gradient.
 
 The layout in memory is `csrc/int4.cuh`'s; `Int4KVCache.store`, `.load`, `decode_attention_int4` and `Int4Linear` on CPU tensors are plain PyTorch over the
 same layout.  The reference generates in the training dtype only (`realhf/impl/model/nn/real_llm_generate.py`); both are opt-in
@@ -96,6 +96,11 @@ def _channel_order(words: torch.Tensor) -> torch.Tensor:
 # ------------------------------------------------------------------------------------------------ cache
 
 
+def _inference_only(x: torch.Tensor, name: str) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or on detached tensors")
+
+
 class Int4KVCache:
     """Keys and values of `slots` sequences of up to `room` tokens, in 4 bits.  `dtype`: the model's type."""
 
@@ -173,7 +178,7 @@ class Int4KVCache:
             raise ValueError(f"Int4KVCache.store: keys and values are {self.dtype} on {self.device}, as the cache")
         cu, slots, start = self._check(cu_seqlens, slots, start)
         tok, slot, row = self._rows(cu, slots, start, k.shape[0])
-        self._put(k[tok], v[tok], slot, row)
+        self._put(k.detach()[tok], v.detach()[tok], slot, row)
 
     def _at(self, slot, row):
         """Index of rows in the fields of keys and of the groups, and in the values with the row's three dims in front."""
@@ -251,7 +256,8 @@ def decode_attention_int4(qkv: torch.Tensor, cache: Int4KVCache, cache_lens: tor
     """One decode step over a 4-bit cache, as `attention.decode_attention` over a 16-bit one: row b of qkv [slots, (n_q + 2 n_kv) * hd] is the fused projection of
     the token at position cache_lens[b] of slot b.  Its queries and key are rotated (cos / sin [room or more, rot_dim / 2] given), the key is rounded to the cache's
     type, key and value are quantised and written, and the queries attend to the rows [0, cache_lens[b]] as the cache holds them, the new one among them.
-    Returns [slots, n_q * hd].  A row whose length is not in [0, room) changes nothing and returns 0.  Does not advance cache_lens."""
+    Returns [slots, n_q * hd], with no gradient (a call that would need one is refused).  A row whose length is not in [0, room) changes nothing and returns 0.  Does not advance cache_lens."""
+    _inference_only(qkv, "decode_attention_int4")
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     if use_native(qkv) and qkv.dtype is cache.dtype:                           # (the op checks the rest)
         return lib().decode_attention_int4(qkv, cache.data, cache._whole(cache_lens), n_q, n_kv, hd, cache.room, scale, cos, sin, rot_dim or hd, interleaved)
@@ -322,6 +328,7 @@ class Int4Linear:
         """Refresh the 4-bit copy in place after the weight changed (same buffers: a kept CUDA graph stays valid)."""
         if tuple(w.shape) != (self.N, self.K) or w.dtype != self.dtype or w.device != self.q.device:
             raise ValueError(f"Int4Linear: a weight [{self.N}, {self.K}] of {self.dtype} on {self.q.device}")
+        w = w.detach()
         if use_native(w):
             lib().int4_quantize(w, self.q, self.group)
         else:
@@ -341,6 +348,7 @@ class Int4Linear:
     def __call__(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
         if x.dim() == 0 or x.shape[-1] != self.K:
             raise ValueError(f"Int4Linear: rows of {self.K}, not {tuple(x.shape)}")
+        _inference_only(x, "Int4Linear")
         bias = self.bias if bias is None else bias
         if use_native(x):
             if x.dtype is not self.dtype or x.device != self.q.device:

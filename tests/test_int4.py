@@ -512,6 +512,50 @@ def test_linear_rows_of_any_size(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,group", [(17, 32), (40, 128), (100, 64)])
+def test_many_rows_of_any_size(dtype, M, group):
+    g = torch.Generator().manual_seed(M)
+    lin = int4.Int4Linear(rows(g, 200, 1152 + group, dtype=dtype, device="cuda"), group=group)
+    x = rows(g, M, lin.K, dtype=dtype, device="cuda").float()
+    x *= (2.0 ** torch.randint(-12, 4, (M, 1), generator=g)).cuda()
+    x[4] = 0
+    check_linear(lin, x.to(dtype))
+    x[8, 100], x[10, 3], x[M - 1, lin.K - 1] = float("inf"), float("nan"), -float("inf")
+    y = lin(x.to(dtype))
+    bad = [8, 10, M - 1]
+    assert not torch.isfinite(y[bad]).any()
+    keep = [i for i in range(M) if i not in bad]
+    x[bad] = 0
+    assert torch.isfinite(y[keep]).all() and torch.equal(y[keep], lin(x.to(dtype))[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [5, 20, 64, 150])
+def test_linear_captured_on_two_streams(M):
+    """Two graphs of one weight, replayed at once, and a weight quantised anew between the replays."""
+    g = torch.Generator().manual_seed(M)
+    w = [rows(g, 700, 2048, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    lin, xs = int4.Int4Linear(w[0]), [rows(g, M, 2048, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    want = [[int4.Int4Linear(v)(x) for x in xs] for v in w]
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    lin(xs[0])
+    for gr, x in zip(graphs, xs):
+        with torch.cuda.graph(gr):
+            outs.append(lin(x))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for v, ref in zip(w, want):
+        lin.requantize(v)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for gr, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], ref[0]) and torch.equal(outs[1], ref[1])
+
+
+@pytest.mark.gpu
 def test_linear_of_leading_dimensions_streams_and_graphs():
     g = torch.Generator().manual_seed(5)
     lin = int4.Int4Linear(rows(g, 500, 512, dtype=torch.bfloat16, device="cuda"), rows(g, 500, 1, dtype=torch.bfloat16, device="cuda")[:, 0])
@@ -585,6 +629,32 @@ def test_refusals(device):
     for codes, s in ((z(4, 128, dtype=torch.uint8) + 16, z(4, 1)), (z(4, 128, dtype=torch.int32), z(4, 1)), (z(4, 128, dtype=torch.uint8), z(4, 3)), (z(4, 128, dtype=torch.uint8), z(3, 1))):
         with pytest.raises(ValueError):
             int4.Int4Linear.from_codes(codes, s, s)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_gradient_is_refused_not_lost(device):
+    z = lambda *s: torch.zeros(*s, device=device, dtype=torch.bfloat16)   # noqa: E731
+    w = z(16, 128).requires_grad_()
+    lin, c, lens = int4.Int4Linear(w), int4.Int4KVCache(1, 8, 1, 64, torch.bfloat16, device), torch.zeros(1, dtype=torch.int32, device=device)
+    lin.requantize(w)
+    c.store(z(3, 1, 64).requires_grad_(), z(3, 1, 64), packed([3], device))
+    for f, x in ((lin, z(2, 128).requires_grad_()), (lambda t: int4.decode_attention_int4(t, c, lens, 2, 1, 64), z(1, 256).requires_grad_())):
+        with pytest.raises(RuntimeError):
+            f(x)
+        with torch.no_grad():
+            assert not f(x).requires_grad
+        f(x.detach())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("M", [3, 20, 70, 130])
+def test_linear_of_repeated_and_overlapping_rows(device, M):
+    g = torch.Generator().manual_seed(M)
+    lin = int4.Int4Linear(rows(g, 48, 256, dtype=torch.bfloat16, device=device) * 0.1, group=64)
+    flat = rows(g, 256 + 8 * M, dtype=torch.bfloat16, device=device)
+    check_linear(lin, flat[:256].expand(M, 256))
+    check_linear(lin, flat.as_strided((M, 256), (8, 1)))
+    check_linear(lin, flat[:256].expand(2, M, 256))
 
 
 @pytest.mark.gpu
