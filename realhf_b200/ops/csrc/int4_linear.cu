@@ -326,15 +326,14 @@ template <typename T, int G, int NT> int few_rows(LinearParams p, cudaStream_t s
 
 // ---------------------------------------------------------------------------------------------- many rows
 
-constexpr int kManyRows = 128, kTeams = 2, kScale = 8;                               // output rows; teams of warps that expand (each has every second block), warps that scale
-template <int NP> constexpr int kTeam = NP == 128 ? 2 : 4;                           // warps of a team (128 rows: scaling takes longer, and needs the registers)
-template <int NP> constexpr int kManyThreads = (kTeams * kTeam<NP> + kScale + 2) * 32;
-constexpr int kCodeBytes = kManyRows * 256;                                          // 128 rows x 128 channels of 16 bits: two halves of 64 channels
-constexpr int kBufs = 4;                                                             // accumulators
-template <int NP> constexpr int kManyStages = NP == 32 ? 4 : NP == 64 ? 3 : 2;       // operand tiles
-template <int NP> constexpr int kRaw = NP == 32 ? 5 : 6;                             // blocks of packed codes, 9 or 10 KB each
+constexpr int kManyRows = 128, kTeam = 4, kLows = 8;                                 // output rows; warps of a team that expands, a quarter of the rows each; warps of the lowest values
+template <int NP> constexpr int kTeams = NP == 128 ? 2 : 3;                          // teams: every second or third block each (128 rows: the registers of the lowest values' sums)
+template <int NP> constexpr int kManyThreads = (kTeams<NP> * kTeam + kLows + 2) * 32;
+constexpr int kWStages = 3, kWCols = 128;                                            // operand tiles in tensor memory; 64 columns of the larger parts, 64 of the smaller ones
+template <int NP> constexpr int kXStages = NP == 128 ? 4 : 6;                        // blocks of x in shared memory
+constexpr int kRaw = 6;                                                              // blocks of packed codes, 9 or 10 KB each
 template <int G> constexpr int kRawBytes = 8 * WTile<G>::kWords * 4;
-template <int G, int NP> constexpr size_t kManySmem = 1024 + kManyStages<NP> * (kCodeBytes + NP * 256) + kRaw<NP> * kRawBytes<G>;
+template <int G, int NP> constexpr size_t kManySmem = 1024 + kXStages<NP> * NP * 256 + kRaw * kRawBytes<G>;
 
 RB_DEVICE void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -351,41 +350,85 @@ template <typename T> RB_DEVICE float2 pair_of(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// The numbers c - 8 of a word, as pairs of neighbouring channels of type T
+template <typename T> RB_DEVICE void expand_centred(uint32_t w, uint32_t (&h)[4], uint32_t magic) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __half>::value) {
+      const uint32_t u = (i < 2 ? w : w >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu) | magic;       // 1024 + c, or 1024 + 16 c
+      const __half2 x = *reinterpret_cast<const __half2*>(&u);
+      const __half2 y = i & 1 ? __hfma2(x, __float2half2_rn(0.0625f), __float2half2_rn(-72.f)) : __hadd2(x, __float2half2_rn(-1032.f));
+      h[i] = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+      const uint32_t u = w >> (4 * i) & 0x000f000fu | magic;                                       // 128 + c
+      const __nv_bfloat162 y = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&u), __float2bfloat162_rn(-136.f));
+      h[i] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+  }
+}
+// scale * e as two numbers of T whose sum it is: a product, and what its rounding left (scale has 8 or 11 bits and e = c - 8 three, or is a power of two, so that fits).  Steps beyond
+// an eighth of T's largest number could overflow: there the larger part is half of it, and the smaller one is off by half a step of T at most.
+template <typename T> struct Step {
+  uint32_t all, first;
+  RB_DEVICE explicit Step(uint32_t group) {
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    all = __byte_perm(group, 0, 0x3232);
+    first = (all & 0x7fffu) > (kHalf ? 0x6fffu : 0x7dffu) ? all - (kHalf ? 0x04000400u : 0x00800080u) : all;
+  }
+  RB_DEVICE void parts(uint32_t e, uint32_t& hi, uint32_t& lo) const {
+    if constexpr (std::is_same<T, __half>::value) {
+      const __half2 x = *reinterpret_cast<const __half2*>(&e), h = __hmul2_rn(*reinterpret_cast<const __half2*>(&first), x);
+      const __half2 l = __hfma2(*reinterpret_cast<const __half2*>(&all), x, __hneg2(h));
+      hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&l);
+    } else {
+      const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&e), h = __hmul2_rn(*reinterpret_cast<const __nv_bfloat162*>(&first), x);
+      const __nv_bfloat162 l = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&all), x, __hneg2(h));
+      hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&l);
+    }
+  }
+};
+template <int N> RB_DEVICE void words_of(uint32_t at, uint32_t (&w)[N]) {
+  if constexpr (N == 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+  else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+  else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
+}
+
 // NP: rows of x, padded (rows beyond M read as zeros)
 template <typename T, int G, int NP>
 __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __grid_constant__ CUtensorMap xmap, const LinearParams p) {
-  constexpr int NG = 128 / G, ND = kBufs, kCols = NP / 2, kX = NP * 256, kStages = kManyStages<NP>, kR = kRaw<NP>, kSums = 3;
-  constexpr int kExpand = kTeams * kTeam<NP>, kLoadWarp = kExpand + kScale, kMmaWarp = kLoadWarp + 1;
+  constexpr int NG = 128 / G, kX = NP * 256, kXS = kXStages<NP>, kR = kRaw, kSums = 3, kTms = kTeams<NP>;
+  constexpr int kExpand = kTms * kTeam, kLoadWarp = kExpand + kLows, kMmaWarp = kLoadWarp + 1;
+  constexpr int kRows = 8, kCols = NP / 16;            // a thread's sums of the lowest values: rows, columns
   extern __shared__ unsigned char raw[];
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], d_full[ND], d_empty[ND], raw_full[kR], raw_empty[kR];
-  __shared__ __align__(16) float xsum[kSums][NG][NP];
-  __shared__ uint32_t groups[kStages][kManyRows * NG];
+  __shared__ __align__(8) uint64_t w_full[kWStages], w_empty[kWStages], x_full[kXS], x_empty[kXS], raw_full[kR], raw_empty[kR], done;
+  __shared__ __align__(16) float xsum[kSums][NG][NP], lows[kSums][NG][kManyRows];
   __shared__ uint32_t tmem_ptr, dead_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile uint32_t* dead = &dead_flag;
-  const uint32_t base = (ptx::smem_u32(raw) + 1023u) & ~1023u, codes = base, xs = base + kStages * kCodeBytes, packed = xs + kStages * kX;
+  const uint32_t base = (ptx::smem_u32(raw) + 1023u) & ~1023u, xs = base, packed = xs + kXS * kX;
   auto bar = [](uint64_t* b, int i) { return ptx::smem_u32(&b[i]); };
   // ring slot n % size, in its (n / size)-th round: what fills it waits for the other parity
   auto wait_full = [&](uint64_t* b, int n, int size) { bounded_wait(ptx::smem_u32(&b[n % size]), n / size & 1, dead); };
   auto wait_empty = [&](uint64_t* b, int n, int size) { bounded_wait(ptx::smem_u32(&b[n % size]), (n / size & 1) ^ 1, dead); };
   if (threadIdx.x == 0) {
     *dead = 0;
-    for (int i = 0; i < kStages; ++i) {
-      ptx::mbar_init(bar(full, i), kTeam<NP> + 1);       // the codes' warps and the copy of x
-      ptx::mbar_init(bar(empty, i), 1 + kScale);
+    for (int i = 0; i < kWStages; ++i) {
+      ptx::mbar_init(bar(w_full, i), kTeam);
+      ptx::mbar_init(bar(w_empty, i), 1);
     }
-    for (int i = 0; i < ND; ++i) {
-      ptx::mbar_init(bar(d_full, i), 1);
-      ptx::mbar_init(bar(d_empty, i), kScale);
+    for (int i = 0; i < kXS; ++i) {
+      ptx::mbar_init(bar(x_full, i), 1);
+      ptx::mbar_init(bar(x_empty, i), 1 + kLows);      // the products, and the sums
     }
     for (int i = 0; i < kR; ++i) {
       ptx::mbar_init(bar(raw_full, i), 1);
-      ptx::mbar_init(bar(raw_empty, i), kTeam<NP>);
+      ptx::mbar_init(bar(raw_empty, i), kTeam + kLows);
     }
+    ptx::mbar_init(bar(&done, 0), 1);
     ptx::fence_barrier_init();
   }
   if (warp == kMmaWarp) {
-    ptx::tmem_alloc(ptx::smem_u32(&tmem_ptr), ND * NP);
+    ptx::tmem_alloc(ptx::smem_u32(&tmem_ptr), 512);    // sums in columns 0 .. NP - 1, operand tiles from 128 on
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before();
@@ -396,67 +439,73 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
   rb::pdl_wait();
   // this block's part of the channels
   const int per = RB_CEIL_DIV(p.kblocks, p.splits), k0 = min(p.kblocks, (int)blockIdx.y * per), blocks = min(p.kblocks, k0 + per) - k0;
-  float2 acc[kCols / 2];
-#pragma unroll
-  for (int i = 0; i < kCols / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+  float* part = reinterpret_cast<float*>(raw + (base - ptx::smem_u32(raw)));    // [NP][128]: the block's sums, in the place of x once all products are done
 
   if (warp < kExpand) {
-    // ---- codes to operands: a team of warps has every second block (its waits, fences and stores pass beside the other's arithmetic), a warp two or four tiles of it, a lane the words
-    // of rows g and g + 8 of their four steps; odd rows store them in another order, so that the eight lanes of a store meet all banks
-    constexpr int kMine = 8 / (kTeam<NP>);
-    const int g = lane >> 2, t = lane & 3, odd = g & 1, w0 = warp / kTeams * kMine;
-    for (int n = warp % kTeams; n < blocks; n += kTeams) {
+    // ---- codes to operands in tensor memory: a lane has a row, whose 16 words it reads in an order that depends on the lane (eight lanes meet all banks) and puts right again
+    const int quarter = warp % 4, team = warp / kTeam, row = quarter * 32 + lane, turn = lane >> 1 & 3;
+    const uint32_t into = tmem + ((uint32_t)(quarter * 32) << 16) + 128;
+    for (int n = team; n < blocks; n += kTms) {
       wait_full(raw_full, n, kR);
-      const uint32_t from = packed + n % kR * kRawBytes<G> + w0 * (WTile<G>::kWords * 4) + lane * 16;
-      wait_empty(empty, n, kStages);
-      const uint32_t to = codes + n % kStages * kCodeBytes + (w0 * 16 + g) * 128;
+      const uint32_t tile = packed + n % kR * kRawBytes<G> + (row >> 4) * (WTile<G>::kWords * 4);
+      uint32_t w[4][4], group[NG];                     // [t][j]
 #pragma unroll
-      for (int u = 0; u < kMine; ++u) {
-#pragma unroll
-        for (int i = lane; i < 16 * NG; i += 32) {
-          uint32_t word;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(word) : "r"(from - lane * 16 + u * (WTile<G>::kWords * 4) + 1024 + i * 4) : "memory");
-          groups[n % kStages][(w0 + u) * 16 * NG + i] = word;
-        }
-        uint4 v[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) v[h] = ld_shared_v4(from + u * (WTile<G>::kWords * 4) + h * 512);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
-#pragma unroll
-          for (int jj = 0; jj < 4; ++jj) {
-            uint32_t e[4];
-            expand<T>(odd ? w[jj ^ 1] : w[jj], e, p.magic);
-            const int j = jj ^ odd;                 // channels 32 j + 8 t ..: piece 4 (j & 1) + t of half j >> 1
-            st_shared_v4(to + u * (16 * 128) + h * (8 * 128) + (j >> 1) * (kManyRows * 128) + ((((j & 1) * 4 + t) ^ g) << 4), e[0], e[1], e[2], e[3]);
-          }
-        }
+      for (int i = 0; i < 4; ++i) {
+        const uint4 v = ld_shared_v4(tile + (row & 15) * 64 + ((i + turn) & 3) * 16);
+        w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
       }
-      ptx::fence_proxy_async();
+      words_of(tile + 1024 + (row & 15) * (NG * 4), group);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {                    // w[i] holds piece i + turn: turned on by two and by one
+        const uint32_t a0 = turn & 2 ? w[2][j] : w[0][j], a1 = turn & 2 ? w[3][j] : w[1][j], a2 = turn & 2 ? w[0][j] : w[2][j], a3 = turn & 2 ? w[1][j] : w[3][j];
+        w[0][j] = turn & 1 ? a3 : a0, w[1][j] = turn & 1 ? a0 : a1, w[2][j] = turn & 1 ? a1 : a2, w[3][j] = turn & 1 ? a2 : a3;
+      }
+      wait_empty(w_empty, n, kWStages);
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const Step<T> step(group[j * NG / 4]);
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          uint32_t e[4];
+          expand_centred<T>(w[t][j], e, p.magic);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) step.parts(e[i], hi[4 * t + i], lo[4 * t + i]);
+        }
+        ptx::tc_st_32x16(into + n % kWStages * kWCols + j * 16, hi);
+        ptx::tc_st_32x16(into + n % kWStages * kWCols + 64 + j * 16, lo);
+      }
+      ptx::tc_wait_st();
+      ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        ptx::mbar_arrive(bar(full, n % kStages));
+        ptx::mbar_arrive(bar(w_full, n % kWStages));
         ptx::mbar_arrive(bar(raw_empty, n % kR));
       }
     }
   } else if (warp < kLoadWarp) {
-    // ---- sums: a warp has 32 output rows, a quarter of the lanes of tensor memory, and half of the rows of x
-    const int quarter = warp % 4, half = (warp - kExpand) / 4, tid = (warp - kExpand) * 32 + lane;
-    constexpr int kEach = kScale * 32 / NP, kPieces = 16 / kEach;                // threads a row of x, 16-byte pieces a thread of its 128 channels
+    // ---- lowest values times sums of x, added up in registers: a thread has eight rows and some columns, so that what it reads serves several products
+    const int tid = (warp - kExpand) * 32 + lane;
+    constexpr int kEach = kLows * 32 / NP, kPieces = 16 / kEach;                 // threads a row of x, 16-byte pieces a thread of its 128 channels
     constexpr int kSpan = kPieces * 8, kOwn = kSpan > G ? kSpan / G : 1, kShare = kSpan < G ? G / kSpan : 1;   // channels of a thread, groups that it sums alone, threads of a group
-    const int col = tid / kEach, sub = tid % kEach, row = quarter * 32 + lane;
-    // the sums of x over the groups of block n, one block ahead of the products' use: a thread's pieces lie in one group, or are whole groups
-    auto sums_of = [&](int n, uint32_t (&word)[NG]) {
-      if (n >= blocks) return;
-      wait_full(full, n, kStages);
+    const int col = tid / kEach, sub = tid % kEach, row0 = tid % 16 * kRows, col0 = tid / 16 * kCols;
+    float2 acc[kRows][kCols / 2];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int c = 0; c < kCols / 2; ++c) acc[r][c] = make_float2(0.f, 0.f);
+#pragma unroll 1
+    for (int n = 0; n < blocks; ++n) {
+      // the block's sums of x: a thread's pieces lie in one group, or are whole groups
+      wait_full(x_full, n, kXS);
       float2 s[kOwn];
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) s[i] = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int piece = sub * kPieces + i;
-        const uint4 v = ld_shared_v4(xs + n % kStages * kX + (piece >> 3) * (NP * 128) + col * 128 + (((piece & 7) ^ (col & 7)) << 4));
+        const uint4 v = ld_shared_v4(xs + n % kXS * kX + (piece >> 3) * (NP * 128) + col * 128 + (((piece & 7) ^ (col & 7)) << 4));
         const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -471,51 +520,60 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
         for (int o = 1; o < kShare; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         if (sub % kShare == 0) xsum[n % kSums][sub / kShare * kOwn + i][col] = total;
       }
+      wait_full(raw_full, n, kR);
+      if (tid < kManyRows) {                           // (the products are of c - 8)
+        uint32_t word[NG];
+        words_of(packed + n % kR * kRawBytes<G> + (tid >> 4) * (WTile<G>::kWords * 4) + 1024 + (tid & 15) * (NG * 4), word);
 #pragma unroll
-      for (int q = 0; q < NG; ++q) word[q] = groups[n % kStages][row * NG + q];
+        for (int q = 0; q < NG; ++q) lows[n % kSums][q][tid] = fmaf(8.f, q4::scale_of<T>(word[q]), q4::low_of<T>(word[q]));
+      }
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(empty, n % kStages));
-    };
-    uint32_t next[NG];
-    sums_of(0, next);
-    for (int n = 0; n < blocks; ++n) {
-      uint32_t word[NG];
-#pragma unroll
-      for (int q = 0; q < NG; ++q) word[q] = next[q];
-      sums_of(n + 1, next);
-      asm volatile("bar.sync 1, %0;" ::"n"(kScale * 32) : "memory");             // (sums of block n are there, and those of n - 2 are done with: three sets)
+      if (lane == 0) {
+        ptx::mbar_arrive(bar(x_empty, n % kXS));
+        ptx::mbar_arrive(bar(raw_empty, n % kR));
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kLows * 32) : "memory");              // (sums of block n are there, and those of n - 2 are done with: three sets)
 #pragma unroll
       for (int q = 0; q < NG; ++q) {
-        const int d_at = n * NG + q;
-        wait_full(d_full, d_at, ND);
-        ptx::tc_fence_after();
-        const float scale = q4::scale_of<T>(word[q]), low = q4::low_of<T>(word[q]);
-        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + d_at % ND * NP + half * kCols;
-        constexpr int kAtOnce = kCols < 32 ? kCols : 32;     // (a wait is for all loads, and takes as long for 32 columns as for 16)
+        float low[kRows];
+        float2 x[kCols / 2];
 #pragma unroll
-        for (int c = 0; c < kCols; c += kAtOnce) {
-          uint32_t d[kAtOnce];
-          if constexpr (kAtOnce == 32) ptx::tc_ld_32x32(from + c, d); else tc_ld16(from + c, d);
-          ptx::tc_wait_ld();
+        for (int r = 0; r < kRows; r += 4) *reinterpret_cast<float4*>(&low[r]) = *reinterpret_cast<const float4*>(&lows[n % kSums][q][row0 + r]);
 #pragma unroll
-          for (int i = 0; i < kAtOnce; i += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(&xsum[n % kSums][q][half * kCols + c + i]);
-            float2 &u = acc[(c + i) / 2], &v = acc[(c + i) / 2 + 1];
-            fma2(u, low, x.x, x.y);
-            fma2(v, low, x.z, x.w);
-            fma2(u, scale, __uint_as_float(d[i]), __uint_as_float(d[i + 1]));
-            fma2(v, scale, __uint_as_float(d[i + 2]), __uint_as_float(d[i + 3]));
-          }
-        }
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(d_empty, d_at % ND));
+        for (int c = 0; c < kCols / 2; ++c) x[c] = *reinterpret_cast<const float2*>(&xsum[n % kSums][q][col0 + 2 * c]);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int c = 0; c < kCols / 2; ++c) fma2(acc[r][c], low[r], x[c].x, x[c].y);
       }
     }
+    if (blocks > 0) bounded_wait(bar(&done, 0), 0, dead);
+    ptx::tc_fence_after();
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int r = 0; r < kRows; r += 4) {
+        auto of = [&](int i) { return c & 1 ? acc[r + i][c / 2].y : acc[r + i][c / 2].x; };
+        *reinterpret_cast<float4*>(&part[(col0 + c) * kManyRows + row0 + r]) = make_float4(of(0), of(1), of(2), of(3));
+      }
+    asm volatile("bar.sync 1, %0;" ::"n"(kLows * 32) : "memory");
+    // ---- and the products: a warp has 32 rows, a quarter of the lanes of tensor memory, and half of the columns
+    if (blocks > 0) {
+      const int quarter = warp % 4, half = (warp - kExpand) / 4;
+#pragma unroll 1
+      for (int c = half * (NP / 2); c < (half + 1) * (NP / 2); c += 16) {
+        uint32_t d[16];
+        tc_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c, d);
+        ptx::tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[(c + i) * kManyRows + quarter * 32 + lane] += __uint_as_float(d[i]);
+      }
+      ptx::tc_fence_before();
+    }
   } else if (warp == kLoadWarp) {
-    // ---- copies: codes run ahead of x by what their rings differ in depth
-    constexpr int kLead = kR - kStages;
+    // ---- copies
     const uint32_t* from = p.q + tile_at<G>(blockIdx.x * 8, k0, p.kblocks);
+    constexpr int kLead = kR > kXS ? kR - kXS : 0;       // codes run ahead of x by what their rings differ in depth
     for (int n = 0; n < blocks + kLead; ++n) {
       if (n < blocks) {
         wait_empty(raw_empty, n, kR);
@@ -529,11 +587,11 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
       }
       const int m = n - kLead;
       if (m >= 0) {
-        wait_empty(empty, m, kStages);
+        wait_empty(x_empty, m, kXS);
         if (ptx::elect_one()) {
-          ptx::mbar_arrive_expect_tx(bar(full, m % kStages), kX);
-          ptx::tma_load_2d(xs + m % kStages * kX, &xmap, bar(full, m % kStages), (k0 + m) * 128, 0);
-          ptx::tma_load_2d(xs + m % kStages * kX + NP * 128, &xmap, bar(full, m % kStages), (k0 + m) * 128 + 64, 0);
+          ptx::mbar_arrive_expect_tx(bar(x_full, m % kXS), kX);
+          ptx::tma_load_2d(xs + m % kXS * kX, &xmap, bar(x_full, m % kXS), (k0 + m) * 128, 0);
+          ptx::tma_load_2d(xs + m % kXS * kX + NP * 128, &xmap, bar(x_full, m % kXS), (k0 + m) * 128 + 64, 0);
         }
       }
     }
@@ -541,59 +599,47 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
     constexpr uint32_t idesc = ptx::make_idesc_f16(std::is_same<T, __half>::value ? 0 : 1, 128, NP, 0, 0);
     const uint32_t el = ptx::elect_one() ? 1u : 0u;
     for (int n = 0; n < blocks; ++n) {
-      wait_full(full, n, kStages);
-      const uint32_t a = ptx::desc_lo(codes + n % kStages * kCodeBytes, 16), b = ptx::desc_lo(xs + n % kStages * kX, 16);
+      wait_full(w_full, n, kWStages);
+      wait_full(x_full, n, kXS);
+      ptx::tc_fence_after();
+      const uint32_t a = tmem + 128 + n % kWStages * kWCols, b = ptx::desc_lo(xs + n % kXS * kX, 16);
 #pragma unroll
-      for (int q = 0; q < NG; ++q) {
-        const int d_at = n * NG + q;
-        wait_empty(d_empty, d_at, ND);
-        ptx::tc_fence_after();
+      for (int k = 0; k < 8; ++k)                     // 16 channels: eight columns of a part, 32 bytes of a swizzled row of x
 #pragma unroll
-        for (int k = 0; k < 8 / NG; ++k) {          // 16 channels, 32 bytes of a swizzled row
-          const int at = q * (8 / NG) + k;
-          ptx::tc_mma_f16_if(el, tmem + d_at % ND * NP, a + (at >> 2) * (kManyRows * 128 >> 4) + (at & 3) * 2, b + (at >> 2) * (NP * 128 >> 4) + (at & 3) * 2, idesc, k != 0);
-        }
-        ptx::tc_commit_if(el, bar(d_full, d_at % ND));
-      }
-      ptx::tc_commit_if(el, bar(empty, n % kStages));
+        for (int half = 0; half < 2; ++half)
+          ptx::tc_mma_f16_ts_if(el, tmem, a + half * 64 + k * 8, b + (k >> 2) * (NP * 128 >> 4) + (k & 3) * 2, idesc, n + k + half != 0);
+      ptx::tc_commit_if(el, bar(w_empty, n % kWStages));
+      ptx::tc_commit_if(el, bar(x_empty, n % kXS));
       __syncwarp();
     }
+    if (blocks > 0) ptx::tc_commit_if(el, bar(&done, 0));
+    __syncwarp();
   }
-  // ---- all products have been read: the ring's place holds the sums where a cluster shares the channels
+  // ---- the block's sums lie in shared memory; a cluster's are added up, rows of x dealt out to its blocks and their warps
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, ND * NP);
-  const bool sums = warp >= kExpand && warp < kLoadWarp;
-  const int r = warp % 4 * 32 + lane, half = (warp - kExpand) / 4, n = blockIdx.x * kManyRows + r;
+  if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, 512);
+  if (p.splits > 1) ptx::cluster_sync();
   T* y = reinterpret_cast<T*>(p.y);
-  const float bias = p.bias && n < p.N ? rb::to_f(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
-  if (p.splits == 1) {
-    if (sums && n < p.N) {
-#pragma unroll
-      for (int i = 0; i < kCols; ++i)
-        if (half * kCols + i < p.M) y[(half * kCols + i) * p.ldy + n] = rb::from_f<T>((i & 1 ? acc[i / 2].y : acc[i / 2].x) + bias);
-    }
-  } else {
-    float* part = reinterpret_cast<float*>(raw + (base - ptx::smem_u32(raw)));    // [NP][128]
-    if (sums) {
-#pragma unroll
-      for (int i = 0; i < kCols; ++i) part[(half * kCols + i) * kManyRows + r] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
-    }
-    ptx::cluster_sync();
-    // rows of x are dealt out to the cluster's blocks and their warps
-    for (int i = threadIdx.x / kManyRows; i * p.splits + blockIdx.y < p.M; i += kManyThreads<NP> / kManyRows) {
-      const int m = i * p.splits + blockIdx.y, c128 = threadIdx.x % kManyRows, out = blockIdx.x * kManyRows + c128;
-      if (threadIdx.x >= kManyThreads<NP> / kManyRows * kManyRows) break;
-      float v = p.bias && out < p.N ? rb::to_f(reinterpret_cast<const T*>(p.bias)[out]) : 0.f;
-      for (int c = 0; c < p.splits; ++c) {
-        uint32_t a;
-        float f;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(base + (m * kManyRows + c128) * 4), "r"(c));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
-        v += f;
+  constexpr int kPasses = kManyThreads<NP> / kManyRows;
+  const int r = threadIdx.x % kManyRows, n = blockIdx.x * kManyRows + r;
+  if (threadIdx.x < kPasses * kManyRows && n < p.N) {
+    const float bias = p.bias ? rb::to_f(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
+    for (int m = threadIdx.x / kManyRows * p.splits + blockIdx.y; m < p.M; m += kPasses * p.splits) {
+      float v = bias;
+      if (p.splits == 1) {
+        v += part[m * kManyRows + r];
+      } else {
+        for (int c = 0; c < p.splits; ++c) {
+          uint32_t at;
+          float f;
+          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + (m * kManyRows + r) * 4), "r"(c));
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(at) : "memory");
+          v += f;
+        }
       }
-      if (out < p.N) y[m * p.ldy + out] = rb::from_f<T>(v);
+      y[m * p.ldy + n] = rb::from_f<T>(v);
     }
   }
   rb::report_given_up(dead, p.status);
