@@ -1,7 +1,11 @@
 // Keys and values of packed sequences into a 4-bit cache, and back (layout and rule: int4.cuh).
 //
-// One block per (tile of a sequence, head).  The 16-bit side: 16 bytes a lane, a head's row by 8 or 16 lanes.  The 4-bit side: a tile is put together in shared memory and
-// copied whole, 16 bytes a lane; where a sequence begins or ends inside it, its rows' words are written one by one and the others left alone.
+// A warp has a tile of 16 rows of one head, so nothing waits for other warps: a row by 8 or 16 lanes, 16 bytes a lane of the 16-bit side, four turns' rows read ahead.  The 4-bit side
+// is put together in the warp's part of shared memory and copied whole, 16 bytes a lane; where a sequence begins or ends inside a tile, the words of its rows alone are written.
+//
+// Memory bounds reading back, memory and issue slots storing: keys and values of 128 x 128 tokens of 32 x 128 channels (348 MB both ways, 53 us at the copy's rate) are stored in 65 us
+// (5.4 TB/s; 14.8 instructions a number took 75, 27 with one number at a time and a division each took 124) and read back in 58 (6.0).  Calls of a few tokens are a chain of
+// latencies, 3.6 and 1.9 us.
 #include "int4.cuh"
 
 #include <algorithm>

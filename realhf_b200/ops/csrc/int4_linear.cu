@@ -8,9 +8,17 @@
 // leaves SMs idle, the blocks of a cluster share K.  Codes become exact 16-bit numbers (a mask that leaves a code in the low bits of 128 or 1024, and a subtraction) and are the
 // left operand, 16 output rows at a time; rows of x, read from L2 and L1 as the operands' lanes want them, are the right one, eight at a time.  Scale and lowest value stay out: a
 // group's product is scaled in fp32 when its channels are through, and the lowest value times the sum of x over the group (one more product, with ones) is added.
-// More rows: a block has 128 output rows and all rows of x (in pieces of 128), and the products run on tcgen05.  Eight warps turn a block of 128 channels of codes into a swizzled
-// operand tile in shared memory, rows of x come by TMA, one warp issues the products of a group of channels into an accumulator of its own in tensor memory, and eight warps
-// scale it into sums in registers (and add the lowest values times the sums of x, which they take from the operand tile) while the next group is multiplied.
+//   Bound: the weight's bytes.  1 x 4096 x 4096 takes 4.7 us (floor 1.4; 16-bit weights 9.8): launch, first bytes and the last sum.  7 x 1024 x 50257 in groups of 32 takes 13.7
+//   (floor 5.0; 27), 16 x 4096 x 22016 24.6 (floor 7.4; 30): copies of 2 KB alone stream 3.3 .. 3.6 TB/s, and products, arithmetic and loads of x fill a third to a half of their pipes
+//   each, one after the other in a warp.  Sets dealt out in halves, so that no block has more than others, changed nothing: an SM's two blocks even it out.
+// More rows: a block has 128 output rows and all rows of x (in pieces of 128), and the products run on tcgen05.  Teams of four warps turn a block of 128 channels of codes into an
+// operand in tensor memory: scale (c - 8) as two numbers of the type, exact, so that one accumulator takes all channels (c - 8 and not c: sums of codes that are all positive would leave
+// the accumulator's last places to cancel).  Rows of x come by TMA, one warp issues the products, and eight warps add up what is left, (lowest value + 8 scale) times the sums of x over a
+// group, eight output rows and some columns a thread.
+//   Bound: none alone.  128 x 11008 x 4096 in groups of 64 takes 36 us (floor 7.2; the 16-bit product 21), 32 rows 22: with half of the products left out 35, without the sums of x 29, with
+//   a quarter of the codes expanded 35: three chains of waits of about the same length a block of channels.  An accumulator a group, scaled out of tensor memory, took 45 (58 in groups
+//   of 32, now 42): a group's 64 KB leave tensor memory and its sums of x shared memory at 128 bytes a clock each.  The two parts in shared memory took 45 .. 53: 275 KB a block through it.
+// So a weight in 4 bits takes less time than one in 16 up to 16 rows, and less memory alone beyond.
 #include "attn_common.cuh"
 #include "int4.cuh"
 
@@ -687,6 +695,7 @@ template <typename T, int G, int NP> int many_rows(LinearParams p, cudaStream_t 
 template <typename T, int G> int run(const void* x, const void* q, const void* bias, void* y, int M, int N, int K, int64_t ldx, int64_t ldy, cudaStream_t s) {
   int* status = rb_attn_status();
   if (status == nullptr) return -5;
+  // (4096 x 11008 in groups of 128: 16 rows 15 us with few rows' kernel, 20 with the other; 32 rows take two passes of the former, one of 21 of the latter)
   for (int m0 = 0; m0 < M;) {
     const int rows = std::min(M - m0, 128);
     const LinearParams p{(const T*)x + m0 * ldx, bias, (const uint32_t*)q, (T*)y + m0 * ldy, rows, N, K, RB_CEIL_DIV(K, 128), 1, ldx, ldy, status, kMagic<T>};

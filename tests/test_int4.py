@@ -531,6 +531,29 @@ def test_many_rows_of_any_size(dtype, M, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [5, 20, 128])
+def test_linear_of_the_widest_groups(dtype, M):
+    """Steps beyond an eighth of the type's largest number, and of the smallest ones.  Where there are more than 16 rows, 8 steps would overflow there and are two halves, the second of
+    which is rounded to the type: off by EPS of half of |scale (c - 8)| <= 8 scale more than `check_linear` allows (and a factor 1 + EPS for the half that was rounded)."""
+    g = torch.Generator().manual_seed(M)
+    big = 0.97 * torch.finfo(dtype).max
+    w = (torch.rand(40, 256, generator=g).double() * 2 - 1) * big
+    w[:, ::32], w[:, 1::32] = big, -big
+    lin = int4.Int4Linear(w.to(dtype).cuda(), group=32)
+    limit = torch.finfo(dtype).max / 8
+    assert float(lin.codes()[1].double().min()) > limit
+    x = (torch.randn(M, 256, generator=g).double() * 2.0 ** (-14 if dtype == torch.float16 else -120)).to(dtype).cuda()
+    y, wd, x2 = lin(x).double().cpu(), lin.dequantize().double().cpu(), x.double().cpu()
+    ref, size = x2 @ wd.t(), 3 * x2.abs().sum(1, keepdim=True) * wd.abs().amax(1)
+    extra = EPS[dtype] / 2 * (1 + EPS[dtype]) * x2.abs().sum(1, keepdim=True) * 8 * lin.codes()[1].double().cpu().amax(1) if M > 16 else 0
+    assert bool(((y - ref).abs() <= EPS[dtype] * ref.abs() + SMALL[dtype] + 2.0 ** -22 * size + extra).all())
+    if dtype == torch.float16:                              # steps that are subnormal numbers: products are taken whole
+        lin = int4.Int4Linear((torch.randn(40, 256, generator=g) * 2.0 ** -17).to(dtype).cuda(), group=32)
+        check_linear(lin, torch.randn(M, 256, generator=g).to(dtype).cuda() * 64)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [5, 20, 64, 150])
 def test_linear_captured_on_two_streams(M):
     """Two graphs of one weight, replayed at once, and a weight quantised anew between the replays."""
