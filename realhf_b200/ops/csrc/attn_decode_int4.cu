@@ -11,8 +11,8 @@
 // (one shift less for every two operands) left errors of 6e-5 in outputs of size 1, in bits 4 .. 7 a sixteenth of that.
 //
 // Bound: the bytes of the cache, 152 a row of 128 channels (at the copy's rate 36 us for 128 sequences up to 639 rows of 32 heads, 16 for 32 sequences up to 4095 of 8 heads under 32
-// queries).  Taken: 57 us (4.2 TB/s; a 16-bit cache 122) and 41 (2.5 TB/s; 59): with four query heads a kv head the tensor pipe's legacy products and the arithmetic between them
-// take about as long as each other and do not overlap in full.  Few sequences are a chain of latencies: 1 x 3900 rows 10.4 us, of which 3 are a launch's.
+// queries).  Taken: 57 us (4.2 TB/s; a 16-bit cache 122) and 41 (2.5 TB/s; 59): issue slots 63 % and 51 %, the pipe of masks, minima and conversions 55 % and 38 %, and the 12 or 16 warps that
+// 128 registers leave an SM do not cover the rest.  Few sequences are a chain of latencies: 1 x 3900 rows 10.4 us, of which 3 are a launch's.
 #include "attn_common.cuh"
 #include "int4.cuh"
 
