@@ -13,12 +13,13 @@
 //   each, one after the other in a warp.  Sets dealt out in halves, so that no block has more than others, changed nothing: an SM's two blocks even it out.
 // More rows: a block has 128 output rows and all rows of x (in pieces of 128), and the products run on tcgen05.  Teams of four warps turn a block of 128 channels of codes into an
 // operand in tensor memory: scale (c - 8) as two numbers of the type, exact, so that one accumulator takes all channels (c - 8 and not c: sums of codes that are all positive would leave
-// the accumulator's last places to cancel).  Rows of x come by TMA, one warp issues the products, and eight warps add up what is left, (lowest value + 8 scale) times the sums of x over a
-// group, eight output rows and some columns a thread.
-//   Bound: none alone.  128 x 11008 x 4096 in groups of 64 takes 36 us (floor 7.2; the 16-bit product 21), 32 rows 22: with half of the products left out 35, without the sums of x 29, with
-//   a quarter of the codes expanded 35: three chains of waits of about the same length a block of channels.  An accumulator a group, scaled out of tensor memory, took 45 (58 in groups
-//   of 32, now 42): a group's 64 KB leave tensor memory and its sums of x shared memory at 128 bytes a clock each.  The two parts in shared memory took 45 .. 53: 275 KB a block through it.
-// So a weight in 4 bits takes less time than one in 16 up to 16 rows, and less memory alone beyond.
+// the accumulator's last places to cancel).  Rows of x come by TMA, one warp issues the products, four warps sum x over the groups (products with ones), and eight add up what is left,
+// (lowest value + 8 scale) times those sums, eight output rows and some columns a thread.
+//   Bound: none alone.  128 x 11008 x 4096 in groups of 64 takes 36 us (floor 7.2; the 16-bit product 21.3), 64 rows 22.7 (19.3), 32 rows 20.3 (18.4): chains of waits (operands,
+//   products, sums, lowest values) of about the same length a block of channels; with half of the products left out 128 rows took 35, with a quarter of the codes expanded 35.  An
+//   accumulator a group, scaled out of tensor memory, took 45 (58 in groups of 32, now 40): a group's 64 KB leave tensor memory and its sums of x shared memory at 128 bytes a clock each.
+//   The two parts in shared memory took 45 .. 53: 275 KB a block through it.  Sums of x by the lowest values' warps took 25.3 with 64 rows and 22.1 with 32.
+// So a weight in 4 bits takes less time than one in 16 up to 16 rows, about as long with 32, and saves memory alone beyond.
 #include "attn_common.cuh"
 #include "int4.cuh"
 
@@ -334,9 +335,10 @@ template <typename T, int G, int NT> int few_rows(LinearParams p, cudaStream_t s
 
 // ---------------------------------------------------------------------------------------------- many rows
 
-constexpr int kManyRows = 128, kTeam = 4, kLows = 8;                                 // output rows; warps of a team that expands, a quarter of the rows each; warps of the lowest values
+constexpr int kManyRows = 128, kTeam = 4, kLows = 8;                                 // output rows; warps of a team that expands, a quarter of the rows each; of the lowest values
 template <int NP> constexpr int kTeams = NP == 128 ? 2 : 3;                          // teams: every second or third block each (128 rows: the registers of the lowest values' sums)
-template <int NP> constexpr int kManyThreads = (kTeams<NP> * kTeam + kLows + 2) * 32;
+constexpr int kSumWarps = 4;                                                         // warps of the sums of x
+template <int NP> constexpr int kManyThreads = (kTeams<NP> * kTeam + kLows + kSumWarps + 2) * 32;
 constexpr int kWStages = 3, kWCols = 128;                                            // operand tiles in tensor memory; 64 columns of the larger parts, 64 of the smaller ones
 template <int NP> constexpr int kXStages = NP == 128 ? 4 : 6;                        // blocks of x in shared memory
 constexpr int kRaw = 6;                                                              // blocks of packed codes, 9 or 10 KB each
@@ -352,10 +354,6 @@ RB_DEVICE void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 RB_DEVICE void fma2(float2& x, float m, float a0, float a1) {
   asm("{\n\t.reg .b64 x, m, a;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 a, {%3, %4};\n\tfma.rn.f32x2 x, m, a, x;\n\tmov.b64 {%0, %1}, x;\n\t}"
       : "+f"(x.x), "+f"(x.y) : "f"(m), "f"(a0), "f"(a1));
-}
-template <typename T> RB_DEVICE float2 pair_of(uint32_t w) {
-  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
 // The numbers c - 8 of a word, as pairs of neighbouring channels of type T
@@ -404,11 +402,11 @@ template <int N> RB_DEVICE void words_of(uint32_t at, uint32_t (&w)[N]) {
 // NP: rows of x, padded (rows beyond M read as zeros)
 template <typename T, int G, int NP>
 __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __grid_constant__ CUtensorMap xmap, const LinearParams p) {
-  constexpr int NG = 128 / G, kX = NP * 256, kXS = kXStages<NP>, kR = kRaw, kSums = 3, kTms = kTeams<NP>;
-  constexpr int kExpand = kTms * kTeam, kLoadWarp = kExpand + kLows, kMmaWarp = kLoadWarp + 1;
+  constexpr int NG = 128 / G, kX = NP * 256, kXS = kXStages<NP>, kR = kRaw, kSums = 4, kTms = kTeams<NP>;
+  constexpr int kExpand = kTms * kTeam, kSumWarp = kExpand + kLows, kLoadWarp = kSumWarp + kSumWarps, kMmaWarp = kLoadWarp + 1;
   constexpr int kRows = 8, kCols = NP / 16;            // a thread's sums of the lowest values: rows, columns
   extern __shared__ unsigned char raw[];
-  __shared__ __align__(8) uint64_t w_full[kWStages], w_empty[kWStages], x_full[kXS], x_empty[kXS], raw_full[kR], raw_empty[kR], done;
+  __shared__ __align__(8) uint64_t w_full[kWStages], w_empty[kWStages], x_full[kXS], x_empty[kXS], raw_full[kR], raw_empty[kR], s_full[kSums], s_empty[kSums], done;
   __shared__ __align__(16) float xsum[kSums][NG][NP], lows[kSums][NG][kManyRows];
   __shared__ uint32_t tmem_ptr, dead_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -426,11 +424,15 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
     }
     for (int i = 0; i < kXS; ++i) {
       ptx::mbar_init(bar(x_full, i), 1);
-      ptx::mbar_init(bar(x_empty, i), 1 + kLows);      // the products, and the sums
+      ptx::mbar_init(bar(x_empty, i), 2);              // the products, and the sums
     }
     for (int i = 0; i < kR; ++i) {
       ptx::mbar_init(bar(raw_full, i), 1);
-      ptx::mbar_init(bar(raw_empty, i), kTeam + kLows);
+      ptx::mbar_init(bar(raw_empty, i), kTeam + 1);
+    }
+    for (int i = 0; i < kSums; ++i) {
+      ptx::mbar_init(bar(s_full, i), 1);
+      ptx::mbar_init(bar(s_empty, i), kLows);
     }
     ptx::mbar_init(bar(&done, 0), 1);
     ptx::fence_barrier_init();
@@ -492,12 +494,10 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
         ptx::mbar_arrive(bar(raw_empty, n % kR));
       }
     }
-  } else if (warp < kLoadWarp) {
+  } else if (warp < kSumWarp) {
     // ---- lowest values times sums of x, added up in registers: a thread has eight rows and some columns, so that what it reads serves several products
     const int tid = (warp - kExpand) * 32 + lane;
-    constexpr int kEach = kLows * 32 / NP, kPieces = 16 / kEach;                 // threads a row of x, 16-byte pieces a thread of its 128 channels
-    constexpr int kSpan = kPieces * 8, kOwn = kSpan > G ? kSpan / G : 1, kShare = kSpan < G ? G / kSpan : 1;   // channels of a thread, groups that it sums alone, threads of a group
-    const int col = tid / kEach, sub = tid % kEach, row0 = tid % 16 * kRows, col0 = tid / 16 * kCols;
+    const int row0 = tid % 16 * kRows, col0 = tid / 16 * kCols;
     float2 acc[kRows][kCols / 2];
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
@@ -505,55 +505,24 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
       for (int c = 0; c < kCols / 2; ++c) acc[r][c] = make_float2(0.f, 0.f);
 #pragma unroll 1
     for (int n = 0; n < blocks; ++n) {
-      // the block's sums of x: a thread's pieces lie in one group, or are whole groups
-      wait_full(x_full, n, kXS);
-      float2 s[kOwn];
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) s[i] = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int piece = sub * kPieces + i;
-        const uint4 v = ld_shared_v4(xs + n % kXS * kX + (piece >> 3) * (NP * 128) + col * 128 + (((piece & 7) ^ (col & 7)) << 4));
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 a = pair_of<T>(u[e]);
-          add_pair(s[i * kOwn / kPieces].x, s[i * kOwn / kPieces].y, a.x, a.y);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        float total = s[i].x + s[i].y;
-#pragma unroll
-        for (int o = 1; o < kShare; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (sub % kShare == 0) xsum[n % kSums][sub / kShare * kOwn + i][col] = total;
-      }
-      wait_full(raw_full, n, kR);
-      if (tid < kManyRows) {                           // (the products are of c - 8)
-        uint32_t word[NG];
-        words_of(packed + n % kR * kRawBytes<G> + (tid >> 4) * (WTile<G>::kWords * 4) + 1024 + (tid & 15) * (NG * 4), word);
-#pragma unroll
-        for (int q = 0; q < NG; ++q) lows[n % kSums][q][tid] = fmaf(8.f, q4::scale_of<T>(word[q]), q4::low_of<T>(word[q]));
-      }
-      __syncwarp();
-      if (lane == 0) {
-        ptx::mbar_arrive(bar(x_empty, n % kXS));
-        ptx::mbar_arrive(bar(raw_empty, n % kR));
-      }
-      asm volatile("bar.sync 1, %0;" ::"n"(kLows * 32) : "memory");              // (sums of block n are there, and those of n - 2 are done with: three sets)
-#pragma unroll
+      wait_full(s_full, n, kSums);
+#pragma unroll 1                                       // (unrolled, 128 rows in groups of 32 spill: 51 us against 40)
       for (int q = 0; q < NG; ++q) {
-        float low[kRows];
         float2 x[kCols / 2];
-#pragma unroll
-        for (int r = 0; r < kRows; r += 4) *reinterpret_cast<float4*>(&low[r]) = *reinterpret_cast<const float4*>(&lows[n % kSums][q][row0 + r]);
 #pragma unroll
         for (int c = 0; c < kCols / 2; ++c) x[c] = *reinterpret_cast<const float2*>(&xsum[n % kSums][q][col0 + 2 * c]);
 #pragma unroll
-        for (int r = 0; r < kRows; ++r)
+        for (int r = 0; r < kRows; r += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(&lows[n % kSums][q][row0 + r]);
+          const float low[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int c = 0; c < kCols / 2; ++c) fma2(acc[r][c], low[r], x[c].x, x[c].y);
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < kCols / 2; ++c) fma2(acc[r + i][c], low[i], x[c].x, x[c].y);
+        }
       }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(s_empty, n % kSums));
     }
     if (blocks > 0) bounded_wait(bar(&done, 0), 0, dead);
     ptx::tc_fence_after();
@@ -577,6 +546,46 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
         for (int i = 0; i < 16; ++i) part[(c + i) * kManyRows + quarter * 32 + lane] += __uint_as_float(d[i]);
       }
       ptx::tc_fence_before();
+    }
+  } else if (warp < kLoadWarp) {
+    // ---- a block's sums of x over its groups, products with ones 16 rows at a time, and its lowest values: every second block a warp
+    for (int n = warp - kSumWarp; n < blocks; n += kSumWarps) {
+      wait_empty(s_empty, n, kSums);
+      wait_full(x_full, n, kXS);
+#pragma unroll 4
+      for (int rows = 0; rows < NP; rows += 16) {
+        const int r = rows + (lane & 15);
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+          float c[4] = {};
+#pragma unroll
+          for (int k = q * (8 / NG); k < (q + 1) * (8 / NG); ++k) {
+            const int piece = 2 * k + (lane >> 4);
+            uint32_t a[4];
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                         : "r"(xs + n % kXS * kX + (piece >> 3) * (NP * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4)) : "memory");
+            mma16<T>(c, a[0], a[1], a[2], a[3], kOnes<T>, kOnes<T>);
+          }
+          if ((lane & 3) == 0) {
+            xsum[n % kSums][q][rows + (lane >> 2)] = c[0];
+            xsum[n % kSums][q][rows + (lane >> 2) + 8] = c[2];
+          }
+        }
+      }
+      wait_full(raw_full, n, kR);
+#pragma unroll
+      for (int row = lane; row < kManyRows; row += 32) {        // (the products are of c - 8)
+        uint32_t word[NG];
+        words_of(packed + n % kR * kRawBytes<G> + (row >> 4) * (WTile<G>::kWords * 4) + 1024 + (row & 15) * (NG * 4), word);
+#pragma unroll
+        for (int q = 0; q < NG; ++q) lows[n % kSums][q][row] = fmaf(8.f, q4::scale_of<T>(word[q]), q4::low_of<T>(word[q]));
+      }
+      __syncwarp();
+      if (lane == 0) {
+        ptx::mbar_arrive(bar(s_full, n % kSums));
+        ptx::mbar_arrive(bar(x_empty, n % kXS));
+        ptx::mbar_arrive(bar(raw_empty, n % kR));
+      }
     }
   } else if (warp == kLoadWarp) {
     // ---- copies
@@ -695,7 +704,7 @@ template <typename T, int G, int NP> int many_rows(LinearParams p, cudaStream_t 
 template <typename T, int G> int run(const void* x, const void* q, const void* bias, void* y, int M, int N, int K, int64_t ldx, int64_t ldy, cudaStream_t s) {
   int* status = rb_attn_status();
   if (status == nullptr) return -5;
-  // (4096 x 11008 in groups of 128: 16 rows 15 us with few rows' kernel, 20 with the other; 32 rows take two passes of the former, one of 21 of the latter)
+  // (4096 x 11008 in groups of 128: 16 rows 15 us with few rows' kernel, 20 with the other; 32 rows take two passes of the former, one of 19 of the latter)
   for (int m0 = 0; m0 < M;) {
     const int rows = std::min(M - m0, 128);
     const LinearParams p{(const T*)x + m0 * ldx, bias, (const uint32_t*)q, (T*)y + m0 * ldy, rows, N, K, RB_CEIL_DIV(K, 128), 1, ldx, ldy, status, kMagic<T>};
