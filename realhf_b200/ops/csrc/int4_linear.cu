@@ -17,7 +17,7 @@
 // (lowest value + 8 scale) times those sums, eight output rows and some columns a thread.
 //   Bound: none alone.  128 x 11008 x 4096 in groups of 64 takes 36 us (floor 7.2; the 16-bit product 21.3), 64 rows 22.7 (19.3), 32 rows 20.3 (18.4): chains of waits (operands,
 //   products, sums, lowest values) of about the same length a block of channels; with half of the products left out 128 rows took 35, with a quarter of the codes expanded 35.  An
-//   accumulator a group, scaled out of tensor memory, took 45 (58 in groups of 32, now 40): a group's 64 KB leave tensor memory and its sums of x shared memory at 128 bytes a clock each.
+//   accumulator a group, scaled out of tensor memory, took 45 (58 in groups of 32, now 39): a group's 64 KB leave tensor memory and its sums of x shared memory at 128 bytes a clock each.
 //   The two parts in shared memory took 45 .. 53: 275 KB a block through it.  Sums of x by the lowest values' warps took 25.3 with 64 rows and 22.1 with 32.
 // So a weight in 4 bits takes less time than one in 16 up to 16 rows, about as long with 32, and saves memory alone beyond.
 #include "attn_common.cuh"
@@ -336,7 +336,8 @@ template <typename T, int G, int NT> int few_rows(LinearParams p, cudaStream_t s
 // ---------------------------------------------------------------------------------------------- many rows
 
 constexpr int kManyRows = 128, kTeam = 4, kLows = 8;                                 // output rows; warps of a team that expands, a quarter of the rows each; of the lowest values
-template <int NP> constexpr int kTeams = NP == 128 ? 2 : 3;                          // teams: every second or third block each (128 rows: the registers of the lowest values' sums)
+template <int NP> constexpr int kTeams = NP == 128 ? 1 : 3;                          // teams: every third block each (32 rows 19.5 us, with two 20.5), or one, whose registers the lowest
+                                                                                     // values' sums of 128 rows need (39 us for groups of 32, with two 51)
 constexpr int kSumWarps = 4;                                                         // warps of the sums of x
 template <int NP> constexpr int kManyThreads = (kTeams<NP> * kTeam + kLows + kSumWarps + 2) * 32;
 constexpr int kWStages = 3, kWCols = 128;                                            // operand tiles in tensor memory; 64 columns of the larger parts, 64 of the smaller ones
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
 #pragma unroll 1
     for (int n = 0; n < blocks; ++n) {
       wait_full(s_full, n, kSums);
-#pragma unroll 1                                       // (unrolled, 128 rows in groups of 32 spill: 51 us against 40)
+#pragma unroll
       for (int q = 0; q < NG; ++q) {
         float2 x[kCols / 2];
 #pragma unroll
