@@ -406,6 +406,10 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
   constexpr int NG = 128 / G, kX = NP * 256, kXS = kXStages<NP>, kR = kRaw, kSums = 4, kTms = kTeams<NP>;
   constexpr int kExpand = kTms * kTeam, kSumWarp = kExpand + kLows, kLoadWarp = kSumWarp + kSumWarps, kMmaWarp = kLoadWarp + 1;
   constexpr int kRows = 8, kCols = NP / 16;            // a thread's sums of the lowest values: rows, columns
+  // A parity tells a round from the one before it, not from the one two before.  A warp that takes every k-th block knows that the block k before has come (its sums are used, or its
+  // product done), so a ring that it waits on has at least k places, or as many as there are teams that take turns.
+  static_assert(kXS >= kSumWarps && kR >= kSumWarps && kSums >= kSumWarps, "a warp of the sums of x could take the round before last for its own");
+  static_assert(kWStages >= kTms && kR >= kTms, "a team could take the round before last for its own");
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t w_full[kWStages], w_empty[kWStages], x_full[kXS], x_empty[kXS], raw_full[kR], raw_empty[kR], s_full[kSums], s_empty[kSums], done;
   __shared__ __align__(16) float xsum[kSums][NG][NP], lows[kSums][NG][kManyRows];
