@@ -320,11 +320,14 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   float o[4 * H][4];
 #pragma unroll
   for (int j = 0; j < 4 * H; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m = -INFINITY, l = 0.f, z[H];               // of head `head`, over the lane's keys: maximum, sum of weights, sums of weights times lowest values, in the weights' unit
+  float m = -INFINITY, l = 0.f, z[H];               // of head `head`, over the lane's keys: maximum, sum of weights, sums of weights times lowest values
 #pragma unroll
   for (int h = 0; h < H; ++h) z[h] = 0.f;
-  int top = -100;                                   // weights are in units of 2^(top - 10); every value scale so far is below 2^top
-  uint32_t bound = 0;                               // the group word of that scale
+  // A weight goes into the products as `unit_w` times it, 2^(10 - top); every value scale so far is below 2^top.  l and z are free of it: a lowest value may be any number of the
+  // type where steps are 0, and a factor made for small steps would take it past fp32.
+  constexpr int kRoom = 14 - (int)kSlack;
+  float unit_w = power2(kRoom + 100);               // (top = -100)
+  uint32_t bound = 0;                               // the group word of 2^top
   int slot = 0;
   uint32_t round = 0;                               // parity of the ring's current round
 #pragma unroll 1
@@ -436,7 +439,8 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     if (__any_sync(0xffffffffu, mx > m + kSlack || most >= bound)) {
-      float corr = ex2(m - (mx == -INFINITY ? 0.f : mx));
+      const float corr = ex2(m - (mx == -INFINITY ? 0.f : mx));
+      float corr_o = corr;
       m = mx;
       constexpr uint32_t kNan = std::is_same<T, __half>::value ? 0x7c000000u : 0x7f800000u;   // infinities and NaN: no unit holds them
       most = 0;
@@ -449,24 +453,27 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
       most = __reduce_max_sync(0xffffffffu, most);
       if (most >= bound) {                          // two bits of room, so that it seldom moves
         constexpr int kShift = std::is_same<T, __half>::value ? 26 : 23, kBias = std::is_same<T, __half>::value ? 15 : 127;
-        const int ex = min((int)(most >> kShift) + 3, (int)(kNan >> kShift)), was = top;
-        top = max(min(ex - kBias, 127), -100);
+        const int ex = min((int)(most >> kShift) + 3, (int)(kNan >> kShift)), was = kRoom + 127 - (int)(__float_as_uint(unit_w) >> 23), top = max(min(ex - kBias, 127), -100);
+        unit_w = power2(kRoom - top);
         bound = (uint32_t)ex << kShift;
-        corr *= power2(max(was - top, -126));
+        corr_o *= power2(max(was - top, -126));
       }
       l *= corr;
 #pragma unroll
       for (int h = 0; h < H; ++h) z[h] *= corr;
-      const float ce = __shfl_sync(0xffffffffu, corr, 8 * t), co = __shfl_sync(0xffffffffu, corr, 8 * t + 4);   // of columns 2t, 2t + 1
+      const float ce = __shfl_sync(0xffffffffu, corr_o, 8 * t), co = __shfl_sync(0xffffffffu, corr_o, 8 * t + 4);   // of columns 2t, 2t + 1
 #pragma unroll
       for (int j = 0; j < 4 * H; ++j) { o[j][0] *= ce; o[j][1] *= co; o[j][2] *= ce; o[j][3] *= co; }
     }
-    const float zero = (m == -INFINITY ? 0.f : m) - (float)(14 - (int)kSlack - top);
+    const float zero = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      float w[4];
+      float w[4], wu[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = ex2(s[u][i] - zero);
+      for (int i = 0; i < 4; ++i) {
+        w[i] = ex2(s[u][i] - zero);
+        wu[i] = w[i] * unit_w;
+      }
       l += (w[0] + w[1]) + (w[2] + w[3]);
       // ---- sums: codes^T times the weights' parts.  A lane's eight channels of four keys: rows g are the first quad of channels, rows g + 8 the second.
 #pragma unroll
@@ -475,7 +482,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t g0 = vg[u][2 * e][h], g1 = vg[u][2 * e + 1][h];
-          const float a = w[2 * e] * q4::scale_of<T>(g0), c = w[2 * e + 1] * q4::scale_of<T>(g1);
+          const float a = wu[2 * e] * q4::scale_of<T>(g0), c = wu[2 * e + 1] * q4::scale_of<T>(g1);
           z[h] = fmaf(w[2 * e], q4::low_of<T>(g0), z[h]);
           z[h] = fmaf(w[2 * e + 1], q4::low_of<T>(g1), z[h]);
           const uint32_t p0 = pack2<__half>(a, c);
@@ -508,12 +515,12 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     z[h] += __shfl_xor_sync(0xffffffffu, z[h], 1);
     z[h] += __shfl_xor_sync(0xffffffffu, z[h], 2);
   }
-  const float back = power2(top - 14 + (int)kSlack), up = back * 1048576.f;   // 2^20 of the subnormals
+  const float back = power2(127 - (int)(__float_as_uint(unit_w) >> 23)), up = back * 1048576.f;   // 2^20 of the subnormals
   if (g < REP && t == 0) {
     sm_m[warp][head] = m;
-    sm_l[warp][head] = l * back;
+    sm_l[warp][head] = l;
 #pragma unroll
-    for (int h = 0; h < H; ++h) sm_z[warp][h][head] = z[h] * back;
+    for (int h = 0; h < H; ++h) sm_z[warp][h][head] = z[h];
   }
 #pragma unroll
   for (int h = 0; h < H; ++h) {

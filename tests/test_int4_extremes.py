@@ -1,0 +1,40 @@
+"""4-bit caches whose numbers lie near the ends of their types, against 64 bits over what the cache holds."""
+import pytest
+import torch
+
+from realhf_b200.ops import int4
+from test_int4 import EPS, SMALL, TYPES, packed, rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("value", [100.0, -1000.0, 65504.0, 2.0 ** 100])
+def test_decode_of_many_rows_of_one_value(dtype, hd, value):
+    """Value groups with a step of 0 and a lowest value far from 0, thousands of them in one warp (more works than the GPU has places, so that none is split), some of them behind rows
+    of ordinary steps.  All weights are about the same: outputs are means of n rows.  Sums of n numbers of one size in fp32 are off by n 2^-24 relative at the very most, 1.8e-4 for
+    3000 rows, and the numbers of a lane, four warps' shares and so on are added up apart: a quarter of that."""
+    value = torch.tensor(value if dtype == torch.bfloat16 else max(min(value, 65504.0), -65504.0)).to(dtype).item()
+    g = torch.Generator().manual_seed(hd)
+    B, nq, nkv, room = 320, 4, 4, 3000
+    one = int4.Int4KVCache(1, room, nkv, hd, dtype, "cuda")
+    k, v = rows(g, room, nkv, hd, dtype=dtype, device="cuda"), torch.full((room, nkv, hd), value, dtype=dtype, device="cuda")
+    v[: room // 3, 2:] = rows(g, room // 3, nkv - 2, hd, dtype=dtype, device="cuda")
+    one.store(k, v, packed([room], "cuda"), room)
+    cache = int4.Int4KVCache(B, room, nkv, hd, dtype, "cuda")
+    cache.data.copy_(one.data.expand_as(cache.data))
+    qkv = rows(g, 1, nq + 2 * nkv, hd, dtype=dtype, device="cuda").view(1, -1) * 0.01
+    qkv[:, -nkv * hd:] = value
+    out = int4.decode_attention_int4(qkv.expand(B, -1), cache, torch.full((B,), room - 1, dtype=torch.int32, device="cuda"), nq, nkv, hd).view(B, nq, hd)
+    kk, vv = (t[0].double() for t in _held(cache, room))
+    w = torch.softmax(torch.einsum("hd,nhd->hn", qkv[0, : nq * hd].view(nq, hd).double(), kk) * hd ** -0.5, -1)
+    ref = torch.einsum("hn,nhd->hd", w, vv)
+    assert torch.isfinite(out).all()
+    assert bool(((out.double() - ref).abs() <= EPS[dtype] * ref.abs() + SMALL[dtype] + 4.5e-5 * vv.abs().amax()).all())
+
+
+def _held(cache, n):
+    """The numbers of the first n rows of slot 0, in 64 bits, [1, n, heads, channels]."""
+    c = int4.Int4KVCache(1, cache.room, cache.n_kv, cache.hd, cache.dtype, cache.device)
+    c.data.copy_(cache.data[:1])
+    return (t[None].double() for t in c._get(torch.zeros(n, dtype=torch.long, device=cache.device), torch.arange(n, device=cache.device)))
