@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     z[h] += __shfl_xor_sync(0xffffffffu, z[h], 1);
     z[h] += __shfl_xor_sync(0xffffffffu, z[h], 2);
   }
-  const float back = power2(127 - (int)(__float_as_uint(unit_w) >> 23)), up = back * 1048576.f;   // 2^20 of the subnormals
+  const float back = power2(127 - (int)(__float_as_uint(unit_w) >> 23));
   if (g < REP && t == 0) {
     sm_m[warp][head] = m;
     sm_l[warp][head] = l;
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i][j] = o[4 * h + j][i] * up;
+        x[i][j] = o[4 * h + j][i] * 1048576.f * back;   // 2^20 of the subnormals; apart, since the product of the two can leave fp32
         if constexpr (REP == 2 || REP == 4) x[i][j] += __shfl_xor_sync(0xffffffffu, x[i][j], REP / 2);
       }
       if constexpr (REP == 1) { x[0][j] += x[1][j]; x[2][j] += x[3][j]; }

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from realhf_b200.ops import int4
-from test_int4 import EPS, SMALL, TYPES, packed, rows
+from test_int4 import EPS, SMALL, TYPES, check_step, packed, rows
 
 
 @pytest.mark.gpu
@@ -38,3 +38,20 @@ def _held(cache, n):
     c = int4.Int4KVCache(1, cache.room, cache.n_kv, cache.hd, cache.dtype, cache.device)
     c.data.copy_(cache.data[:1])
     return (t[None].double() for t in c._get(torch.zeros(n, dtype=torch.long, device=cache.device), torch.arange(n, device=cache.device)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv", [(4, 4), (6, 3), (4, 1), (8, 1)])
+@pytest.mark.parametrize("power", [112, 116, 118, 120])
+def test_decode_of_the_largest_values(nq, nkv, power):
+    """Values up to 2^123 and steps beyond 2^114: sums of them stay inside fp32 (40 rows, weights of 2^4 at most: below 2^5.4 2^4 of a value, and most weights are far smaller)."""
+    g = torch.Generator().manual_seed(power + nq)
+    hd, room, B, dtype = 128, 40, 3, torch.bfloat16
+    cache = int4.Int4KVCache(B, room, nkv, hd, dtype, "cuda")
+    k, v = (rows(g, B * room, nkv, hd, dtype=dtype, device="cuda") for _ in range(2))
+    v[: B * room // 2] *= 2.0 ** power
+    v[B * room // 2:] *= 2.0 ** (power - 3)
+    cache.store(k, v, packed([room] * B, "cuda"), room)
+    qkv = rows(g, B, nq + 2 * nkv, hd, dtype=dtype, device="cuda").view(B, -1)
+    qkv[:, -nkv * hd:] *= 2.0 ** power
+    check_step(cache, qkv, [room - 1, 20, 0], nq, nkv, hd)
