@@ -223,18 +223,21 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       xn[i][e] *= p.scale;
-      sum += xn[i][e];
       most = q4::max_nan(most, fabsf(xn[i][e]));
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) most = q4::max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const int ex = (int)(__float_as_uint(most) >> 23), up = max(min(21 + 127 - ex, 100), -100);
+    // (ex is 254 at most in a finite query; the factors below stay normal numbers, and below 2^-105 a query's elements keep fewer bits)
+    const int ex = (int)(__float_as_uint(most) >> 23), up = max(min(21 + 127 - ex, 126), 21 + 127 - 254);
+    const float down = power2(up - 12);              // 32 numbers below 2^22: their sum, taken by 2^(up - 12), is below 2^15
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(xn[i][e], down, sum);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     if (r < REP) {                                   // (heads beyond the set repeat its last one and are not stored)
       if (sub == 0) s_unit[w0][r] = ex == 255 ? __int_as_float(0x7fc00000) : power2(-up);   // (an infinity or a NaN: every score is NaN)
       if (sub % 4 == 0) {
-        float rest = sum * power2(up - 12);          // 32 numbers below 2^22: below 2^15
+        float rest = sum;
 #pragma unroll
         for (int d = 0; d < 3; ++d) {
           const T x = rb::from_f<T>(rest);

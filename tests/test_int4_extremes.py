@@ -55,3 +55,22 @@ def test_decode_of_the_largest_values(nq, nkv, power):
     qkv = rows(g, B, nq + 2 * nkv, hd, dtype=dtype, device="cuda").view(B, -1)
     qkv[:, -nkv * hd:] *= 2.0 ** power
     check_step(cache, qkv, [room - 1, 20, 0], nq, nkv, hd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv", [(4, 4), (8, 2), (8, 1)])
+@pytest.mark.parametrize("power,one_value", [(122, False), (124, True), (119, False), (-78, False), (-100, False)])
+def test_decode_of_the_largest_and_smallest_queries(nq, nkv, power, one_value):
+    """Queries of 2^power against keys of 2^-power: scores of ordinary size.  With one value throughout, the sum of a query over 32 channels, which the keys' lowest values are taken by,
+    is 2^5 times an element."""
+    g = torch.Generator().manual_seed(power + 200 + nq)
+    hd, room, B, dtype = 128, 70, 3, torch.bfloat16
+    cache = int4.Int4KVCache(B, room, nkv, hd, dtype, "cuda")
+    k, v = (rows(g, B * room, nkv, hd, dtype=dtype, device="cuda") for _ in range(2))
+    cache.store(k * 2.0 ** -power, v, packed([room] * B, "cuda"), room)
+    qkv = rows(g, B, nq + 2 * nkv, hd, dtype=dtype, device="cuda").view(B, -1)
+    if one_value:
+        qkv[:, : nq * hd] = 1
+    qkv[:, : nq * hd] *= 2.0 ** power
+    qkv[:, nq * hd: (nq + nkv) * hd] *= 2.0 ** -power
+    check_step(cache, qkv, [room - 1, 31, 0], nq, nkv, hd, scale=1.0)
