@@ -189,6 +189,8 @@ class DecodeState:
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.graph_launches = 0
         self.graph_sig = None
+        # the copies of weights (e4m3, 4 bits) that the graph reads: held here, so that no other call frees them while the graph may be replayed
+        self.copies: Tuple[Optional[dict], Optional[dict]] = (None, None)
         self.B, self.S = B, S
         # in-graph sampling: per-row step counters, liveness flags, device-resident seed and the [B, n_gen] history buffers the
         # sampling kernel writes at column `step`
@@ -426,11 +428,15 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
     use_graph = g.use_cuda_graph and dev.type == "cuda"
     # opt-in W8A8 decode (ops/fp8.py): the prefill above ran in bf16; from here on block linears and the head read e4m3 copies
     use_fp8 = (g.fp8_weights or os.environ.get("REAL_GEN_FP8", "0") == "1") and B <= 128 and model.fp8_decode_supported()
+    # (a kept graph reads the copies that it was captured with: those are renewed, whatever other calls on the model have done with theirs)
+    kept = state.copies if state.graph is not None else (None, None)
     if use_fp8:
+        model._fp8 = kept[0] or model._fp8
         model.enable_fp8_decode()
     # opt-in 4-bit weights (ops/int4.py), the same way: the prefill ran in the model's type
     use_int4 = g.int4_weights and not use_fp8 and B <= 128 and model.int4_decode_supported()
     if use_int4:
+        model._int4 = kept[1] or model._int4
         model.enable_int4_decode()
     V = logits.shape[1]
     # the fused sampler can run as the tail of the captured step: then a decode step is ONE graph replay and nothing else
@@ -443,9 +449,10 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
         return _final_logits(model, h)
 
     sig = (in_graph, g.max_new_tokens, g.min_new_tokens, g.top_k, g.top_p, g.temperature, g.greedy, need_mask, eos_id, pad_id,
-           int(model.flat_param.data_ptr()), use_fp8, use_int4)
+           int(model.flat_param.data_ptr()), use_fp8, use_int4, model.copies_read())
     if state.graph is not None and state.graph_sig != sig:
-        state.graph = None  # sampling options changed, or the flat parameter buffer moved (realloc / offload reload / ZeRO-3)
+        # sampling options changed, or the flat parameter buffer (realloc / offload reload / ZeRO-3) or the copies of the weights moved
+        state.graph = None
     if in_graph:
         state.prepare_hist(g.max_new_tokens, V, need_mask)
         state.tok_hist[:, 0] = nxt
@@ -485,6 +492,7 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
         state.graph_launches = launches.end_capture()
         state.graph = graph
         state.graph_sig = sig
+        state.copies = (model._fp8 if use_fp8 else None, model._int4 if use_int4 else None)
     mark("capture")
     step = 1
     if in_graph:
@@ -540,6 +548,8 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
     if g.force_cudagraph_recapture and state.graph is not None:
         state.graph = None
         state.out = None
+    if state.graph is None:
+        state.copies = (None, None)
     model.train(was_training)
     model.sequence_parallel = sp_saved
     raise_if_gave_up(dev)

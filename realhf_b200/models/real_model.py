@@ -616,6 +616,12 @@ class ReaLModel(nn.Module):
         if free:
             self._int4 = None
 
+    def copies_read(self) -> Tuple[int, ...]:
+        """The addresses of the quantised weights that a decode step reads now: a captured step is good for these alone."""
+        fp8 = [t for f in self._fp8.values() for t in (f.qw, f.sw)] if self._fp8_active and self._fp8 else []
+        q4 = [f.q for f in self._int4.values()] if self._int4_active and self._int4 else []
+        return tuple(int(t.data_ptr()) for t in fp8 + q4)
+
     def tied_embedding_params(self) -> List[torch.Tensor]:
         """Parameters whose gradients must be summed over the embedding group (tied embeddings with pp > 1)."""
         c = self.config

@@ -1,0 +1,78 @@
+"""A captured decode step that is kept reads quantised copies of the weights: they live as long as the graph does, whatever other calls on the model do."""
+import pytest
+import torch
+
+from realhf_b200.api.model import GenerationHyperparameters
+from realhf_b200.models import generation as gen
+from realhf_b200.ops import int4
+from test_int4_generation import prompts, tiny
+
+
+def options(n, **kw):
+    return GenerationHyperparameters(max_new_tokens=n, min_new_tokens=n, greedy=True, **kw)
+
+
+def test_a_state_renews_the_copies_that_its_graph_reads(monkeypatch):
+    """(On the CPU nothing is captured: what stands in for a graph is a mark that there is one.)  A call with other options frees the model's copies, not the state's, and the next call with that
+    state reads the state's."""
+    m = tiny("cpu", torch.bfloat16)
+    ids, cu = prompts("cpu")
+    _, state = gen.generate(m, ids, cu, options(3), eos_id=None, pad_id=0)
+    m.enable_int4_decode()
+    copies = dict(m._int4)
+    read = m.copies_read()
+    assert len(read) == len(copies) == 9 and len(set(read)) == 9
+    state.graph, state.copies = object(), (None, m._int4)
+    m.disable_int4_decode(free=False)
+    assert m.copies_read() == ()
+    gen.generate(m, ids, cu, options(3, int4_weights=True), eos_id=None, pad_id=0)                 # another state
+    assert m._int4 is None
+    seen, real = [], int4.Int4Linear.__call__
+    monkeypatch.setattr(int4.Int4Linear, "__call__", lambda self, x, bias=None: (seen.append(self), real(self, x, bias))[1])
+    m.p["1.mlp.down.weight"].mul_(-1)
+    out, _ = gen.generate(m, ids, cu, options(3, int4_weights=True), eos_id=None, pad_id=0, state=state)
+    assert {id(f) for f in seen} == {id(f) for f in copies.values()}
+    fresh, _ = gen.generate(m, ids, cu, options(3, int4_weights=True), eos_id=None, pad_id=0)
+    assert torch.equal(out.tokens, fresh.tokens) and torch.equal(out.logprobs, fresh.logprobs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int4_weights", "fp8_weights"])
+def test_kept_graph_after_a_call_that_keeps_none(kind):
+    """Kept graph, a call with the default options on another state, then the kept state again, with memory that the allocator could have taken from freed copies."""
+    m = tiny("cuda", torch.bfloat16)
+    ids, cu = prompts("cuda")
+    keep = options(10, force_cudagraph_recapture=False, **{kind: True})
+    _, state = gen.generate(m, ids, cu, keep, eos_id=None, pad_id=0)
+    graph = state.graph
+    fresh, _ = gen.generate(m, ids, cu, options(10, **{kind: True}), eos_id=None, pad_id=0)
+    junk = [torch.full((1 << 18,), -1, dtype=torch.int8, device="cuda") for _ in range(64)]
+    out, state = gen.generate(m, ids, cu, keep, eos_id=None, pad_id=0, state=state)
+    assert state.graph is graph and len(junk) == 64
+    assert torch.equal(out.tokens, fresh.tokens)
+    torch.testing.assert_close(out.logprobs, fresh.logprobs, atol=1e-3, rtol=1e-3)
+    for n, p in m.p.items():
+        if n.endswith("mlp.down.weight"):
+            p.mul_(-1)
+    out, state = gen.generate(m, ids, cu, keep, eos_id=None, pad_id=0, state=state)
+    fresh, _ = gen.generate(m, ids, cu, options(10, **{kind: True}), eos_id=None, pad_id=0)
+    assert state.graph is graph and torch.equal(out.tokens, fresh.tokens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int4_weights", "fp8_weights"])
+def test_kept_graph_before_and_after_an_eager_call(kind, monkeypatch):
+    """One state in three calls whose sampling lies outside the graph: captured, eager, captured."""
+    monkeypatch.setenv("REAL_GEN_SAMPLE_IN_GRAPH", "0")
+    m = tiny("cuda", torch.bfloat16)
+    ids, cu = prompts("cuda")
+    state, outs = None, []
+    for graph in (True, False, True):
+        g = options(10, force_cudagraph_recapture=False, use_cuda_graph=graph, **{kind: True})
+        out, state = gen.generate(m, ids, cu, g, eos_id=None, pad_id=0, state=state)
+        outs.append(out)
+        junk = [torch.full((1 << 18,), -1, dtype=torch.int8, device="cuda") for _ in range(64)]
+        assert len(junk) == 64
+    for out in outs[1:]:
+        assert torch.equal(out.tokens, outs[0].tokens)
+        torch.testing.assert_close(out.logprobs, outs[0].logprobs, atol=1e-3, rtol=1e-3)
