@@ -388,6 +388,17 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
              eos_id: Optional[int], pad_id: int, generator: Optional[torch.Generator] = None,
              state: Optional[DecodeState] = None, sync_every: int = 16) -> Tuple[GenerationOutput, DecodeState]:
     """Generate for a packed batch of prompts on a single pipeline stage (pp == 1)."""
+    try:
+        return _generate(model, input_ids, cu_seqlens, g, eos_id, pad_id, generator, state, sync_every)
+    finally:
+        # after an error in the loop the copies of the weights would stay in use
+        if model._fp8_active:
+            model.disable_fp8_decode()
+        if model._int4_active:
+            model.disable_int4_decode()
+
+
+def _generate(model: ReaLModel, input_ids, cu_seqlens, g: GenerationHyperparameters, eos_id, pad_id, generator, state, sync_every):
     assert model.is_first_stage and model.is_last_stage, "pipelined generation goes through engine.pipe_runner"
     dev = model.device
     if generator is None and model.ctx.tp_size > 1 and not g.greedy and not fused_sampler_ok(dev, model.config.vocab_size):

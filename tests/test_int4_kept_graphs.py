@@ -76,3 +76,21 @@ def test_kept_graph_before_and_after_an_eager_call(kind, monkeypatch):
     for out in outs[1:]:
         assert torch.equal(out.tokens, outs[0].tokens)
         torch.testing.assert_close(out.logprobs, outs[0].logprobs, atol=1e-3, rtol=1e-3)
+
+
+@pytest.mark.parametrize("kind", ["int4_weights", "fp8_weights"])
+def test_an_error_in_the_loop_leaves_no_copies_in_use(kind, monkeypatch):
+    monkeypatch.setenv("REAL_FP8_EMULATE", "1")
+    m = tiny("cpu", torch.bfloat16)
+    ids, cu = prompts("cpu")
+    real = gen.genstep
+
+    def failing(logits, g, step, *a, **k):
+        if step == 2:
+            assert m._int4_active or m._fp8_active
+            raise KeyError("sampling")
+        return real(logits, g, step, *a, **k)
+    monkeypatch.setattr(gen, "genstep", failing)
+    with pytest.raises(KeyError):
+        gen.generate(m, ids, cu, GenerationHyperparameters(max_new_tokens=5, min_new_tokens=5, greedy=True, **{kind: True}), eos_id=None, pad_id=0)
+    assert not m._int4_active and not m._fp8_active and m._int4 is None and m._fp8 is None
