@@ -326,9 +326,11 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   float m = -INFINITY, l = 0.f, z[H];               // of head `head`, over the lane's keys: maximum, sum of weights, sums of weights times lowest values
 #pragma unroll
   for (int h = 0; h < H; ++h) z[h] = 0.f;
-  // A weight goes into the products as `unit_w` times it, 2^(10 - top); every value scale so far is below 2^top.  l and z are free of it: a lowest value may be any number of the
-  // type where steps are 0, and a factor made for small steps would take it past fp32.
-  constexpr int kRoom = 14 - (int)kSlack;
+  // Weights are 2^(s - m - kSpare): sums of the type's largest numbers over thousands of rows stay inside fp32, and so do the codes' part and the lowest values' part of a group that spans the
+  // whole type, which cancel; numbers of 2^-126 still keep the bits that bf16 has.  A weight goes into the products as `unit_w` times it, so that they are 2^(10 - top) 2^(s - m); every
+  // value scale so far is below 2^top.  l and z are free of that factor: a lowest value may be any number of the type where steps are 0, and a factor made for small steps would take
+  // it past fp32.
+  constexpr int kSpare = 12, kRoom = 14 - (int)kSlack + kSpare;
   float unit_w = power2(kRoom + 100);               // (top = -100)
   uint32_t bound = 0;                               // the group word of 2^top
   int slot = 0;
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
 #pragma unroll
       for (int j = 0; j < 4 * H; ++j) { o[j][0] *= ce; o[j][1] *= co; o[j][2] *= ce; o[j][3] *= co; }
     }
-    const float zero = m == -INFINITY ? 0.f : m;
+    const float zero = (m == -INFINITY ? 0.f : m) + (float)kSpare;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float w[4], wu[4];

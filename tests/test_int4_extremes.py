@@ -74,3 +74,24 @@ def test_decode_of_the_largest_and_smallest_queries(nq, nkv, power, one_value):
     qkv[:, : nq * hd] *= 2.0 ** power
     qkv[:, nq * hd: (nq + nkv) * hd] *= 2.0 ** -power
     check_step(cache, qkv, [room - 1, 31, 0], nq, nkv, hd, scale=1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,nkv", [(4, 4), (6, 2), (8, 1)])
+@pytest.mark.parametrize("room,low", [(1, -1.0), (40, -1.0), (1, 0.5), (500, 0.25), (1000, 1.0), (1000, -0.5)])
+def test_decode_of_sums_beyond_fp32(nq, nkv, room, low):
+    """Values up to 0.97 of bfloat16's largest number, groups that span the whole type among them: their means are finite, sums over rows are not in fp32.  The parts of a value (lowest value
+    and 15 steps) are rounded apart, 2^-23 of twice the largest number, on top of what `check_step` allows relative to it: 1e-5 covers it."""
+    g = torch.Generator().manual_seed(room + nq)
+    hd, B, dtype = 128, 160, torch.bfloat16
+    most = 0.97 * torch.finfo(dtype).max
+    one = int4.Int4KVCache(1, room, nkv, hd, dtype, "cuda")
+    k, v = rows(g, room, nkv, hd, dtype=dtype, device="cuda"), torch.full((room, nkv, hd), most, device="cuda")
+    v[..., ::3] *= low
+    one.store(k, v.to(dtype), packed([room], "cuda"), room)
+    cache = int4.Int4KVCache(B, room, nkv, hd, dtype, "cuda")
+    cache.data.copy_(one.data.expand_as(cache.data))
+    qkv = (rows(g, 1, nq + 2 * nkv, hd, dtype=dtype, device="cuda").view(1, -1) * 0.25).expand(B, -1).contiguous()
+    qkv[:, -nkv * hd:] = v[0].to(dtype).flatten()
+    check_step(cache, qkv, [room - 1] + [-1] * (B - 1), nq, nkv, hd)
+    check_step(cache, qkv, [room - 1] * 2 + [room // 2] * (B - 2), nq, nkv, hd)
