@@ -553,9 +553,14 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   if (p.wide == 1) __syncwarp(); else __syncthreads();
   T* out = reinterpret_cast<T*>(p.out) + (int64_t)b * p.nq * D + (int64_t)(hkv * rep + h0) * D;
   auto write4 = [&](int at4, const float (&a)[4], float l4) {
+    // (a mean of what the cache holds can lie above T's largest number by the rounding of a step: finite numbers stay finite)
+    constexpr float kMost = std::is_same<T, __half>::value ? 65504.f : 3.3895313892515355e38f;
     rb::Pack<T, 4> x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x.v[i] = rb::from_f<T>(live ? a[i] / l4 : 0.f);
+    for (int i = 0; i < 4; ++i) {
+      const float y = live ? a[i] / l4 : 0.f;
+      x.v[i] = rb::from_f<T>(fabsf(y) <= 3.4028234663852886e38f ? fminf(fmaxf(y, -kMost), kMost) : y);
+    }
     *reinterpret_cast<rb::Pack<T, 4>*>(out + at4 * 4) = x;
   };
   for (int c4 = wi * 32 + lane; c4 < heads * (D / 4); c4 += p.wide * 32) {   // four channels a lane

@@ -149,7 +149,8 @@ template <typename T, int kKind> RB_DEVICE Coded code8(const uint4& u, float lo,
   if ((__float_as_uint(lo) | __float_as_uint(hi)) == 0) return {0, 0};      // (zeros: rows of padding)
   return code8_long<T, kKind>(u, lo, hi);
 }
-// A word's channels as numbers of T, two a word: scale * c is exact, so two roundings, fp32's and T's.  `magic`: 2^23's bits, as a number that the compiler does not know
+// A word's channels as numbers of T, two a word: scale * c is exact, so two roundings, fp32's and T's.  A step that was rounded up can leave 15 steps above T's largest number, which is
+// what is read back then (NaN stays NaN).  `magic`: 2^23's bits, as a number that the compiler does not know
 // (a mask and a magic number as two immediates are two instructions where an immediate and a register are one).
 constexpr uint32_t kWholeMagic = 0x4b000000u;
 template <typename T, int kKind> RB_DEVICE uint4 unpack8(uint32_t w, uint32_t g, uint32_t magic) {
@@ -161,8 +162,8 @@ template <typename T, int kKind> RB_DEVICE uint4 unpack8(uint32_t w, uint32_t g,
     const uint64_t c = both(__uint_as_float(w >> bit_of<kKind>(2 * i) & 15u | magic), __uint_as_float(w >> bit_of<kKind>(2 * i + 1) & 15u | magic));
     float a, b;
     parts(fma2(add2(c, less), s2, l2), a, b);
-    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y[i]) : "f"(b), "f"(a));
-    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y[i]) : "f"(b), "f"(a));
+    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(y[i]) : "f"(b), "f"(a));
+    else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(y[i]) : "f"(b), "f"(a));
   }
   return make_uint4(y[0], y[1], y[2], y[3]);
 }

@@ -4,7 +4,8 @@ A group of numbers is held as codes 0 .. 15 with the group's lowest value and a 
 
     low = min x,   scale = T((max x - low) / 15),   code = min(15, round_half_even((x - low) / scale))  (0 where scale is 0),   x ~ scale * code + low
 
-so a value is off by at most half a step (and 15 roundings of the step).  A group that holds an infinity or a NaN reads back as NaN.
+so a value is off by at most half a step (and 15 roundings of the step).  A group that holds an infinity or a NaN reads back as NaN, finite numbers as finite ones: where the
+rounded step leaves a value above the type's largest number, that number is read back.
 
 * `Int4KVCache`: a dense cache [slots, room, n_kv, hd] with groups of 32 channels of a key (after the rotation a few channels are far larger than the
   others, and a small group keeps them to themselves) and of 64 channels of a value: 4.75 bits a number, 3.4 times less than 16.  `store` quantises the
@@ -61,6 +62,12 @@ def dequantize_groups(codes: torch.Tensor, scale: torch.Tensor, low: torch.Tenso
     """fp32 scale * code + low, rounded once."""
     xg = codes.unflatten(-1, (scale.shape[-1], -1)).double()
     return (xg * scale.double()[..., None] + low.double()[..., None]).float().flatten(-2)
+
+
+def _to_type(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Rounded to the type; finite numbers stay finite (a step that was rounded up can leave 15 steps above the type's largest number)."""
+    most = torch.finfo(dtype).max
+    return torch.where(torch.isfinite(x), x.clamp(-most, most), x).to(dtype)
 
 
 def _words(codes: torch.Tensor, shifts) -> torch.Tensor:
@@ -216,7 +223,7 @@ class Int4KVCache:
         out = torch.zeros(2, tokens, self.n_kv, self.hd, dtype=self.dtype, device=self.device)
         tok, slot, row = self._rows(cu, slots, start, tokens)
         k, v = self._get(slot, row)
-        out[0, tok], out[1, tok] = k.to(self.dtype), v.to(self.dtype)
+        out[0, tok], out[1, tok] = _to_type(k, self.dtype), _to_type(v, self.dtype)
         return out[0], out[1]
 
 
@@ -248,7 +255,7 @@ def decode_attention_int4_ref(qkv, cache: Int4KVCache, cache_lens, n_q: int, n_k
         n = int(lens[b]) + 1
         kk, vv = (t.repeat_interleave(n_q // n_kv, 1) for t in cache._get(torch.full((n,), b, device=qkv.device), torch.arange(n, device=qkv.device)))
         out[b] = torch.einsum("hn,nhd->hd", torch.softmax(torch.einsum("hd,nhd->hn", q[b], kk) * scale, -1), vv)
-    return out.reshape(B, n_q * hd).to(qkv.dtype)
+    return _to_type(out.reshape(B, n_q * hd), qkv.dtype)
 
 
 def decode_attention_int4(qkv: torch.Tensor, cache: Int4KVCache, cache_lens: torch.Tensor, n_q: int, n_kv: int, hd: int, scale: Optional[float] = None, cos=None,

@@ -95,3 +95,32 @@ def test_decode_of_sums_beyond_fp32(nq, nkv, room, low):
     qkv[:, -nkv * hd:] = v[0].to(dtype).flatten()
     check_step(cache, qkv, [room - 1] + [-1] * (B - 1), nq, nkv, hd)
     check_step(cache, qkv, [room - 1] * 2 + [room // 2] * (B - 2), nq, nkv, hd)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("low", [0.0, -1.0, -0.5, -0.25, -0.77, 0.3])
+def test_finite_numbers_read_back_finite(device, dtype, low):
+    """Groups up to the type's largest number whose step is rounded up: 15 steps above the lowest value are more than that number, off by 15 roundings of the step at most.  Outputs of
+    the attention, means of such values, are finite too; infinities stay NaN."""
+    most, nkv, hd, room = torch.finfo(dtype).max, 2, 64, 20
+    x = torch.full((room, nkv, hd), most)
+    x[..., ::2] *= low
+    x = x.to(dtype).to(device)
+    cache = int4.Int4KVCache(1, room, nkv, hd, dtype, device)
+    cu = packed([room], device)
+    cache.store(x, -x, cu, room)
+    k, v = cache.load(cu, room, room)
+    for got, want in ((k, x), (v, -x)):
+        assert torch.isfinite(got).all()
+        assert bool(((got.double() - want.double()).abs() <= 15 * EPS[dtype] * 2 * most / 15 + EPS[dtype] * most).all())
+    cache.store(torch.zeros_like(x), x, cu, room)
+    qkv = torch.cat([torch.zeros(1, 2 * nkv * hd, dtype=dtype, device=device), x[:1].reshape(1, -1)], 1)
+    out = int4.decode_attention_int4(qkv, cache, torch.tensor([room - 1], dtype=torch.int32, device=device), nkv, nkv, hd).view(nkv, hd)
+    assert torch.isfinite(out).all()
+    assert bool(((out.double() - x[0].double()).abs() <= 15 * EPS[dtype] * 2 * most / 15 + 2 * EPS[dtype] * most).all())
+    bad = x.clone()
+    bad[3, 1, 5] = float("inf")
+    cache.store(bad, bad, cu, room)
+    k, v = cache.load(cu, room, room)
+    assert k[3, 1, :32].isnan().all() and v[3, 1].isnan().all() and int(k.isnan().sum()) == 32 and int(v.isnan().sum()) == 64
