@@ -11,7 +11,10 @@ rounded step leaves a value above the type's largest number, that number is read
   others, and a small group keeps them to themselves) and of 64 channels of a value: 4.75 bits a number, 3.4 times less than 16.  `store` quantises the
   keys and values of packed sequences, `load` reads them back, `decode_attention_int4` appends a token and attends to all rows as the cache holds them.
 * `Int4Linear`: a weight [N, K] with groups of 32, 64 or 128 along K and its products with rows of any number; made for the few rows of a decode step,
-  where the weights' bytes are the time.  None of these has a gradient.
+  where the weights' bytes are the time.
+
+None of these has a gradient.  A product or an attention step whose rows, or whose call's bias, would need one is refused; `store`, a weight and the bias that is kept with it are taken
+as numbers.
 
 The layout in memory is `csrc/int4.cuh`'s; `Int4KVCache.store`, `.load`, `decode_attention_int4` and `Int4Linear` on CPU tensors are plain PyTorch over the
 same layout.  The reference generates in the training dtype only (`realhf/impl/model/nn/real_llm_generate.py`); both are opt-in
@@ -24,6 +27,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from realhf_b200.ops import lib, use_native
 
@@ -106,6 +110,8 @@ def _channel_order(words: torch.Tensor) -> torch.Tensor:
 def _inference_only(x: torch.Tensor, name: str) -> None:
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or on detached tensors")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError(f"{name} has no forward-mode derivative: call it on tensors without a tangent")
 
 
 class Int4KVCache:
@@ -175,7 +181,7 @@ class Int4KVCache:
               start: Optional[torch.Tensor] = None) -> None:
         """Writes packed keys (rotated) and values [T, n_kv, hd]: the tokens cu_seqlens[i] .. of sequence i go to the rows start[i] .. (0 ..) of slot slots[i] (i).
         Rows and slots outside the cache are left out, all others of the cache keep what they hold.  No row may be named twice in a call.  `max_seqlen` sets the
-        size of the launch alone."""
+        size of the launch alone.  What is stored is numbers: no gradient goes back to `k` and `v`."""
         if use_native(self.data) and k.dtype is self.dtype and k.is_cuda:      # (the op checks the rest)
             lib().int4_cache_store(k, v, self.data, self._whole(cu_seqlens), self._whole(slots), self._whole(start), self.room, self.hd, max_seqlen or 0)
             return
@@ -302,7 +308,7 @@ class Int4Linear:
         self.N, self.K, self.group, self.dtype = int(shape[0]), int(shape[1]), int(group), dtype
         if bias is not None and (tuple(bias.shape) != (self.N,) or bias.dtype != dtype):
             raise ValueError(f"Int4Linear: a bias [{self.N}] of {dtype}")
-        self.bias = bias
+        self.bias = None if bias is None else bias.detach()                    # (its numbers alone, as the weight's)
         self.q = torch.zeros(-(-self.N // 128), -(-self.K // 128), 8, TILE_ROWS * 16 + TILE_ROWS * (128 // group), dtype=torch.int32, device=device)
 
     @classmethod
@@ -356,7 +362,10 @@ class Int4Linear:
         if x.dim() == 0 or x.shape[-1] != self.K:
             raise ValueError(f"Int4Linear: rows of {self.K}, not {tuple(x.shape)}")
         _inference_only(x, "Int4Linear")
-        bias = self.bias if bias is None else bias
+        if bias is None:
+            bias = self.bias
+        else:
+            _inference_only(bias, "Int4Linear")
         if use_native(x):
             if x.dtype is not self.dtype or x.device != self.q.device:
                 raise ValueError(f"Int4Linear: rows of {self.dtype} on {self.q.device}")
