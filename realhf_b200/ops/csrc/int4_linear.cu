@@ -146,30 +146,34 @@ template <int G> struct Block {
     }
   }
 };
-// A warp's ring of blocks on their way, 2176 to 2560 bytes each (registers hold one ahead, and 35 KB an SM were on their way: 2.1 TB/s at any number of rows)
-constexpr int kFewRing = 4;
+// A warp's ring of blocks on their way, 2176 to 2560 bytes each (registers hold one ahead, and 35 KB an SM were on their way: 2.1 TB/s at any number of rows): four, or three where four would
+// leave an SM one block of threads (16 rows in groups of 32)
 template <int G> constexpr int kFewBytes = kFewRows / 16 * WTile<G>::kWords * 4;
-template <int G> constexpr size_t kFewSmem = kFewWarps * kFewRing * kFewBytes<G>;
+template <int NT> constexpr size_t kFewSums = 2 * kFewWarps * NT * 8 * (kFewRows + 1) * 4 + NT * 8 * kFewRows * 4;     // a tile of rows' sums and the next one's; a block's
+template <int G, int NT, int kRing> constexpr bool kTwoFit = 2 * (kFewWarps * kRing * (kFewBytes<G> + 8) + kFewSums<NT> + 1024 + 64) <= 228 * 1024;
+template <int G, int NT> constexpr int kFewRing = kTwoFit<G, NT, 4> ? 4 : 3;
+template <int G, int NT> constexpr size_t kFewSmem = kFewWarps * kFewRing<G, NT> * kFewBytes<G>;
 
 // NT: sets of eight rows of x
 template <typename T, int G, int NT>
 __global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const LinearParams p) {
-  constexpr int MT = kFewRows / 16, NG = 128 / G;
+  constexpr int MT = kFewRows / 16, NG = 128 / G, kRing = kFewRing<G, NT>;
+  static_assert(kTwoFit<G, NT, kRing>, "the grid and the splits count on two blocks an SM");
   extern __shared__ __align__(128) unsigned char few_ring[];
   __shared__ __align__(16) float sums[2][kFewWarps][NT * 8][kFewRows + 1];    // (of a tile of rows and of the next: a warp may be that far ahead)
   __shared__ float part[NT * 8][kFewRows];
-  __shared__ __align__(8) uint64_t bar[kFewWarps][kFewRing];
+  __shared__ __align__(8) uint64_t bar[kFewWarps][kRing];
   __shared__ uint32_t dead_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   volatile uint32_t* dead = &dead_flag;
   if (threadIdx.x == 0) *dead = 0;
-  if (lane < kFewRing) ptx::mbar_init(ptx::smem_u32(&bar[warp][lane]), 1);
+  if (lane < kRing) ptx::mbar_init(ptx::smem_u32(&bar[warp][lane]), 1);
   ptx::fence_barrier_init();
   __syncthreads();
   rb::pdl_trigger();
   // the warp's blocks of a set of 32 output rows, then those of the next set of this block of threads: one sequence, whose copies run ahead of the sums at a set's end
   const int step = kFewWarps * p.splits, first = blockIdx.y * kFewWarps + warp, sets = RB_CEIL_DIV(p.N, kFewRows);
-  const uint32_t ring = ptx::smem_u32(few_ring) + warp * (kFewRing * kFewBytes<G>);
+  const uint32_t ring = ptx::smem_u32(few_ring) + warp * (kRing * kFewBytes<G>);
   int ask_set = first < p.kblocks ? blockIdx.x : sets, ask_kb = first;
   const uint32_t* ask = p.q + tile_at<G>(ask_set * MT, first, p.kblocks);
   auto fetch = [&](int slot) {
@@ -190,7 +194,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const LinearPa
   };
   rb::pdl_wait();
 #pragma unroll
-  for (int i = 0; i < kFewRing; ++i) fetch(i);
+  for (int i = 0; i < kRing; ++i) fetch(i);
   // rows beyond M repeat the last one and are not stored; channels beyond K read the row's first ones: they meet codes, scales and lowest values of 0
   const T* x[NT];
 #pragma unroll
@@ -223,7 +227,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const LinearPa
     for (int i = 0; i < MT; ++i) cur[i].load(ring + slot * kFewBytes<G> + i * (WTile<G>::kWords * 4), lane);
     __syncwarp();
     fetch(slot);
-    if (++slot == kFewRing) { slot = 0; round ^= 1; }
+    if (++slot == kRing) { slot = 0; round ^= 1; }
 #pragma unroll
     for (int q = 0; q < NG; ++q) {                  // a group
       float c[MT][NT][4], one[NT][4];
@@ -306,7 +310,7 @@ template <typename T, int G, int NT> int few_rows(LinearParams p, cudaStream_t s
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -3;
   if (dev >= 64 || !(opted_in.load(std::memory_order_relaxed) >> dev & 1)) {
-    if (cudaFuncSetAttribute(few_rows_kernel<T, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewSmem<G>) != cudaSuccess) return -3;
+    if (cudaFuncSetAttribute(few_rows_kernel<T, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewSmem<G, NT>) != cudaSuccess) return -3;
     if (dev < 64) opted_in.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
   }
   const int sets = RB_CEIL_DIV(p.N, kFewRows), blocks = std::min(sets, 2 * rb::kNumSMs);
@@ -315,7 +319,7 @@ template <typename T, int G, int NT> int few_rows(LinearParams p, cudaStream_t s
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(blocks, p.splits);
   cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = kFewSmem<G>;
+  cfg.dynamicSmemBytes = kFewSmem<G, NT>;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   int n = 0;
