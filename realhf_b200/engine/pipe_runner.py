@@ -213,6 +213,8 @@ class PipelineRunner:
     def generate(self, input_: SequenceSample, g: GenerationHyperparameters, eos_id, pad_id, n_mbs: int,
                  sync_every: int = 16) -> List[gen.GenerationOutput]:
         m, dev = self.m, self.m.device
+        if g.int4_weights:
+            gen.say_ignored("int4_weights", "pipelined generation has no 4-bit weights")
         mbs = self._split(input_, self.pp * n_mbs)
         M = len(mbs)
         metas = [_mb_inputs(mb, dev) for mb in mbs]

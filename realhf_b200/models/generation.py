@@ -20,6 +20,7 @@ from typing import List, Optional, Tuple
 import torch
 
 from realhf_b200.api.model import GenerationHyperparameters
+from realhf_b200.base import logging
 from realhf_b200.models.real_model import ReaLModel
 from realhf_b200.ops import functional as OF
 from realhf_b200.ops import int4, launches
@@ -383,6 +384,25 @@ def raise_if_gave_up(dev: torch.device) -> None:
         lib().attn_check()
 
 
+_SAID = set()
+
+
+def say_ignored(option: str, why: str) -> None:
+    """Once per option and reason: generation goes on without an option that was asked for."""
+    if (option, why) not in _SAID:
+        _SAID.add((option, why))
+        logging.getLogger("generation").warning(f"{option} is not used: {why}; the loop reads the weights of the model's type")
+
+
+def _why_no_int4(model: ReaLModel, B: int, use_fp8: bool) -> Optional[str]:
+    """Why a decode loop of B sequences cannot read 4-bit copies of the weights; None where it can."""
+    if use_fp8:
+        return "fp8_weights is on"
+    if B > 128:
+        return "there are more than 128 sequences"
+    return None if model.int4_decode_supported() else "it takes a dense model with a gated feed-forward in bfloat16 or float16 that is not sharded"
+
+
 @torch.no_grad()
 def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor, g: GenerationHyperparameters,
              eos_id: Optional[int], pad_id: int, generator: Optional[torch.Generator] = None,
@@ -445,7 +465,12 @@ def _generate(model: ReaLModel, input_ids, cu_seqlens, g: GenerationHyperparamet
         model._fp8 = kept[0] or model._fp8
         model.enable_fp8_decode()
     # opt-in 4-bit weights (ops/int4.py), the same way: the prefill ran in the model's type
-    use_int4 = g.int4_weights and not use_fp8 and B <= 128 and model.int4_decode_supported()
+    use_int4 = False
+    if g.int4_weights:
+        why = _why_no_int4(model, B, use_fp8)
+        use_int4 = why is None
+        if not use_int4:
+            say_ignored("int4_weights", why)
     if use_int4:
         model._int4 = kept[1] or model._int4
         model.enable_int4_decode()
@@ -619,6 +644,8 @@ class InflightBatchingGenerator:
                  max_prompt_len: int):
         assert model.is_first_stage and model.is_last_stage
         self.model, self.g, self.eos_id, self.pad_id, self.B = model, g, eos_id, pad_id, n_slots
+        if g.int4_weights:
+            say_ignored("int4_weights", "in-flight batching has no 4-bit weights")
         self.state = DecodeState(model, n_slots, max_prompt_len + g.max_new_tokens, g.kv_cache_bits)
         self.slot_seq = [-1] * n_slots                 # which request a slot serves
         self.slot_tokens: List[List[int]] = [[] for _ in range(n_slots)]
