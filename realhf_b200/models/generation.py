@@ -192,6 +192,7 @@ class DecodeState:
         self.graph_sig = None
         # the copies of weights (e4m3, 4 bits) that the graph reads: held here, so that no other call frees them while the graph may be replayed
         self.copies: Tuple[Optional[dict], Optional[dict]] = (None, None)
+        self.tables = None   # ... and the rotation's tables, which the model replaces when a longer sequence comes
         self.B, self.S = B, S
         # in-graph sampling: per-row step counters, liveness flags, device-resident seed and the [B, n_gen] history buffers the
         # sampling kernel writes at column `step`
@@ -529,6 +530,7 @@ def _generate(model: ReaLModel, input_ids, cu_seqlens, g: GenerationHyperparamet
         state.graph = graph
         state.graph_sig = sig
         state.copies = (model._fp8 if use_fp8 else None, model._int4 if use_int4 else None)
+        state.tables = model._rope
     mark("capture")
     step = 1
     if in_graph:
@@ -585,7 +587,7 @@ def _generate(model: ReaLModel, input_ids, cu_seqlens, g: GenerationHyperparamet
         state.graph = None
         state.out = None
     if state.graph is None:
-        state.copies = (None, None)
+        state.copies, state.tables = (None, None), None
     model.train(was_training)
     model.sequence_parallel = sp_saved
     raise_if_gave_up(dev)

@@ -9,7 +9,7 @@ from test_int4_generation import prompts, tiny
 
 
 def options(n, **kw):
-    return GenerationHyperparameters(max_new_tokens=n, min_new_tokens=n, greedy=True, **kw)
+    return GenerationHyperparameters(max_new_tokens=n, min_new_tokens=n, greedy=True, **{"use_cuda_graph": True, **kw})
 
 
 def test_a_state_renews_the_copies_that_its_graph_reads(monkeypatch):
@@ -45,6 +45,7 @@ def test_kept_graph_after_a_call_that_keeps_none(kind):
     keep = options(10, force_cudagraph_recapture=False, **{kind: True})
     _, state = gen.generate(m, ids, cu, keep, eos_id=None, pad_id=0)
     graph = state.graph
+    assert graph is not None
     fresh, _ = gen.generate(m, ids, cu, options(10, **{kind: True}), eos_id=None, pad_id=0)
     junk = [torch.full((1 << 18,), -1, dtype=torch.int8, device="cuda") for _ in range(64)]
     out, state = gen.generate(m, ids, cu, keep, eos_id=None, pad_id=0, state=state)
@@ -71,6 +72,7 @@ def test_kept_graph_before_and_after_an_eager_call(kind, monkeypatch):
         g = options(10, force_cudagraph_recapture=False, use_cuda_graph=graph, **{kind: True})
         out, state = gen.generate(m, ids, cu, g, eos_id=None, pad_id=0, state=state)
         outs.append(out)
+        assert state.graph is not None
         junk = [torch.full((1 << 18,), -1, dtype=torch.int8, device="cuda") for _ in range(64)]
         assert len(junk) == 64
     for out in outs[1:]:
@@ -94,3 +96,24 @@ def test_an_error_in_the_loop_leaves_no_copies_in_use(kind, monkeypatch):
     with pytest.raises(KeyError):
         gen.generate(m, ids, cu, GenerationHyperparameters(max_new_tokens=5, min_new_tokens=5, greedy=True, **{kind: True}), eos_id=None, pad_id=0)
     assert not m._int4_active and not m._fp8_active and m._int4 is None and m._fp8 is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 16])
+def test_kept_graph_after_a_longer_sequence(bits):
+    """A sequence beyond the tables of cosines and sines makes the model take longer ones: the kept graph's live on, with the same numbers."""
+    import weakref
+    m = tiny("cuda", torch.bfloat16)
+    ids, cu = prompts("cuda")
+    keep = options(10, force_cudagraph_recapture=False, kv_cache_bits=bits)
+    want, state = gen.generate(m, ids, cu, keep, eos_id=None, pad_id=0)
+    graph, table, n = state.graph, weakref.ref(m._rope[0]), m._rope[0].shape[0]
+    assert graph is not None
+    m.rope_tables(2 * n)
+    junk = [torch.full((n, 32), 7.0, device="cuda") for _ in range(16)]
+    assert m._rope[0].shape[0] >= 2 * n and table() is not None and table() is not m._rope[0] and len(junk) == 16
+    out, state = gen.generate(m, ids, cu, keep, eos_id=None, pad_id=0, state=state)
+    assert state.graph is graph and torch.equal(out.tokens, want.tokens)
+    torch.testing.assert_close(out.logprobs, want.logprobs, atol=1e-3, rtol=1e-3)
+    _, state = gen.generate(m, ids, cu, options(10, kv_cache_bits=bits), eos_id=None, pad_id=0, state=state)      # (keeps none)
+    assert state.graph is None and table() is None
