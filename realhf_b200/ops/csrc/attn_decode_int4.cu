@@ -5,14 +5,19 @@
 // copy of 4864 bytes (heads of 64 channels: 2432) into a ring of its own, and the codes themselves are operands on the tensor cores:
 //   scores  codes, as bytes, [16 keys x 32 channels of a group] times q [32 x 8 columns] in whole numbers: a query is a 23-bit whole number (with one power of two a head), three signed
 //           bytes, (byte, head) pairs in the columns.  A sum is exact; the group's scale times it, and the lowest value times the query's sum over the group, are added in fp32.
-//   sums    codes^T, as fp16 subnormals, [16 channels x 16 keys] times weights [16 x 8 columns]: a row's softmax weight times its value group's scale, two fp16 parts (22 bits) of it,
+//   sums    codes^T, as small fp16 numbers, [16 channels x 16 keys] times weights [16 x 8 columns]: a row's softmax weight times its value group's scale, two fp16 parts (22 bits) of it,
 //           (part, head) pairs in the columns, in units of a power of two above all scales so far (it moves as a softmax's maximum does).  The lowest values are summed beside.
 // So nothing is converted on the way from the cache to a product.  The tensor core aligns subnormals as if they were 2^-14 and cuts off some 23 bits below: codes in bits 0 .. 3
-// (one shift less for every two operands) left errors of 6e-5 in outputs of size 1, in bits 4 .. 7 a sixteenth of that.
+// (one shift less for every two operands) left errors of 6e-5 in outputs of size 1.  In bits 7 .. 10, where 8 is 2^-14, nothing of a code is below that (32 x 4095 rows: errors of 5.5e-6
+// of the outputs' size before their rounding, in bits 4 .. 7 8.6e-6, 0.5 % less time).
 //
 // Bound: the bytes of the cache, 152 a row of 128 channels (at the copy's rate 36 us for 128 sequences up to 639 rows of 32 heads, 16 for 32 sequences up to 4095 of 8 heads under 32
-// queries).  Taken: 57 us (4.2 TB/s; a 16-bit cache 122) and 41 (2.5 TB/s; 59): issue slots 63 % and 51 %, the pipe of masks, minima and conversions 55 % and 38 %, and the 12 or 16 warps that
-// 128 registers leave an SM do not cover the rest.  Few sequences are a chain of latencies: 1 x 3900 rows 10.4 us, of which 3 are a launch's.
+// queries).  Taken: 58.6 us (4.05 TB/s; a 16-bit cache 122) and 41.5 (2.5 TB/s; 59): issue slots 66 % and 53 %, the pipe of masks, minima and conversions 55 % and 38 %, and the
+// warps that are there do not cover the rest: 128 registers allow an SM 16 (with eight queries 12), and where all blocks begin at once those of short sequences end early (32 sequences of 1300 ..
+// 4095 rows: 12 on average, the longest has 16 steps a warp where the mean is 10).  Few sequences are a chain of latencies: 1 x 3900 rows 10.4 us, of which 3 are a launch's.
+//
+// Precision: queries keep 22 or 23 bits below the largest of a head, softmax weights times steps 22 (two fp16 parts), sums are fp32's.  Errors before the outputs' rounding: 0.4 .. 1.2e-5 of
+// their size (fp32 throughout 0.2 .. 0.4e-5); by arithmetic most of it comes from scores, whose codes' part and lowest values' part cancel where keys have channels far larger than others.
 #include "attn_common.cuh"
 #include "int4.cuh"
 
@@ -56,8 +61,8 @@ template <typename T> RB_DEVICE void mma_k8(float (&c)[4], uint32_t a0, uint32_t
   else
     asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};" : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b));
 }
-// The codes in nibble i of both halves of a word, in bits 4 .. 7: as fp16 2^-20 times the codes.
-RB_DEVICE uint32_t nibbles(uint32_t w, int i) { return (i == 0 ? w << 4 : w >> (4 * i - 4)) & 0x00f000f0u; }
+// The codes in nibble i of both halves of a word, in bits 7 .. 10: as fp16 2^-17 times the codes (8 is 2^-14, the first normal number, so there is no gap).
+RB_DEVICE uint32_t nibbles(uint32_t w, int i) { return (i < 2 ? w << (7 - 4 * i) : w >> (4 * i - 7)) & 0x07800780u; }
 template <int N> RB_DEVICE void ld_words(uint32_t (&w)[N], uint32_t addr) {
   static_assert(N == 2 || N == 4, "");
   if constexpr (N == 4)
@@ -159,6 +164,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
   constexpr int J = Tl::J, H = Tl::H, NS = slots_of<D>();
   constexpr int kProd = REP == 8 ? 2 : 1;          // products of weights: (part, head) pairs fill 8 columns, or each part has its own
   constexpr int kScores = REP == 8 ? 3 : REP == 4 ? 2 : 1;   // products of queries: (byte, head) pairs
+  constexpr int kTogether = REP == 1 ? 1 : 2;      // tiles whose products are added to the sums at once (128 x 639 rows with one query a key head 59.1 us, both at once 59.7; 32 x 4095 with four 42.1, 41.4)
   extern __shared__ __align__(128) unsigned char ring[];
   __shared__ __align__(8) uint64_t bar[kWarps][NS];
   __shared__ uint32_t dead_flag;
@@ -471,37 +477,51 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
       for (int j = 0; j < 4 * H; ++j) { o[j][0] *= ce; o[j][1] *= co; o[j][2] *= ce; o[j][3] *= co; }
     }
     const float zero = (m == -INFINITY ? 0.f : m) + (float)kSpare;
+    // ---- sums: codes^T times the weights' parts.  A lane's eight channels of four keys: rows g are the first quad of channels, rows g + 8 the second.  Products begin at zero and are added
+    // to the sums in fp32: the tensor core cuts off what it adds to an accumulator instead of rounding it, and sums of codes, which are all positive, fall behind (128 x 639 rows: errors of 3.8e-5
+    // of the outputs' size before their rounding, so 0.9e-5).
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float w[4], wu[4];
+    for (int u0 = 0; u0 < 2; u0 += kTogether) {
+      float w[kTogether][4], wu[kTogether][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = ex2(s[u][i] - zero);
-        wu[i] = w[i] * unit_w;
+      for (int u = 0; u < kTogether; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[u][i] = ex2(s[u0 + u][i] - zero);
+          wu[u][i] = w[u][i] * unit_w;
+        }
+        l += (w[u][0] + w[u][1]) + (w[u][2] + w[u][3]);
       }
-      l += (w[0] + w[1]) + (w[2] + w[3]);
-      // ---- sums: codes^T times the weights' parts.  A lane's eight channels of four keys: rows g are the first quad of channels, rows g + 8 the second.
 #pragma unroll
       for (int h = 0; h < H; ++h) {
-        uint32_t pb[kProd][2];
+        uint32_t pb[kTogether][kProd][2], w4[kTogether][4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t g0 = vg[u][2 * e][h], g1 = vg[u][2 * e + 1][h];
-          const float a = wu[2 * e] * q4::scale_of<T>(g0), c = wu[2 * e + 1] * q4::scale_of<T>(g1);
-          z[h] = fmaf(w[2 * e], q4::low_of<T>(g0), z[h]);
-          z[h] = fmaf(w[2 * e + 1], q4::low_of<T>(g1), z[h]);
-          const uint32_t p0 = pack2<__half>(a, c);
-          const float2 f0 = unpack_half2(p0);
-          const uint32_t p1 = pack2<__half>(a - f0.x, c - f0.y);
-          if constexpr (REP == 8) { pb[0][e] = p0; pb[1][e] = p1; } else pb[0][e] = part ? p1 : p0;
+        for (int u = 0; u < kTogether; ++u) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t g0 = vg[u0 + u][2 * e][h], g1 = vg[u0 + u][2 * e + 1][h];
+            const float a = wu[u][2 * e] * q4::scale_of<T>(g0), c = wu[u][2 * e + 1] * q4::scale_of<T>(g1);
+            z[h] = fmaf(w[u][2 * e], q4::low_of<T>(g0), z[h]);
+            z[h] = fmaf(w[u][2 * e + 1], q4::low_of<T>(g1), z[h]);
+            const uint32_t p0 = pack2<__half>(a, c);
+            const float2 f0 = unpack_half2(p0);
+            const uint32_t p1 = pack2<__half>(a - f0.x, c - f0.y);
+            if constexpr (REP == 8) { pb[u][0][e] = p0; pb[u][1][e] = p1; } else pb[u][0][e] = part ? p1 : p0;
+          }
+          ld_words(w4[u], at + (u0 + u) * Tl::kBytes + Tl::kValues * 4 + h * 512 + g * 64 + t * 16);
         }
-        uint32_t w4[4];
-        ld_words(w4, at + u * Tl::kBytes + Tl::kValues * 4 + h * 512 + g * 64 + t * 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+          float x[4] = {};
 #pragma unroll
-          for (int f = 0; f < kProd; ++f)
-            mma_f16(o[4 * h + i], nibbles(w4[0], i), nibbles(w4[1], i), nibbles(w4[2], i), nibbles(w4[3], i), pb[f][0], pb[f][1]);
+          for (int u = 0; u < kTogether; ++u)
+#pragma unroll
+            for (int f = 0; f < kProd; ++f)
+              mma_f16(x, nibbles(w4[u][0], i), nibbles(w4[u][1], i), nibbles(w4[u][2], i), nibbles(w4[u][3], i), pb[u][f][0], pb[u][f][1]);
+          float(&to)[4] = o[4 * h + i];
+          add_pair(to[0], to[1], x[0], x[1]);
+          add_pair(to[2], to[3], x[2], x[3]);
+        }
       }
     }
     __syncwarp();
@@ -534,7 +554,7 @@ __global__ void __launch_bounds__(kDecThreads, ctas_of(REP)) decode_int4_kernel(
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i][j] = o[4 * h + j][i] * 1048576.f * back;   // 2^20 of the subnormals; apart, since the product of the two can leave fp32
+        x[i][j] = o[4 * h + j][i] * 131072.f * back;   // 2^17 of the codes; apart, since the product of the two can leave fp32
         if constexpr (REP == 2 || REP == 4) x[i][j] += __shfl_xor_sync(0xffffffffu, x[i][j], REP / 2);
       }
       if constexpr (REP == 1) { x[0][j] += x[1][j]; x[2][j] += x[3][j]; }

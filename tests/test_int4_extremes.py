@@ -124,3 +124,29 @@ def test_finite_numbers_read_back_finite(device, dtype, low):
     cache.store(bad, bad, cu, room)
     k, v = cache.load(cu, room, room)
     assert k[3, 1, :32].isnan().all() and v[3, 1].isnan().all() and int(k.isnan().sum()) == 32 and int(v.isnan().sum()) == 64
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nq,nkv", [(4, 4), (8, 4), (8, 2), (8, 1)])
+def test_decode_sums_are_rounded_not_cut(nq, nkv, hd):
+    """Means of 4000 rows of one warp whose values cancel to a thousandth of their size, so that fp16 shows the sums' own errors.  A value is a code times its step and the lowest value, summed
+    apart: 2.5 of either a row at most here.  250 partial sums rounded to nearest are off by 2^-24 of that each at most, at random: 2^-24 / sqrt(3) sqrt(250) is a standard deviation, of which six
+    are allowed for each of the two sums; what is cut off within a tile's products, 2^-23 of them and two parts, is a bias of 2^-22 of a sum.  Weights of equal scores are equal.  The mean error
+    over all channels has a standard deviation smaller by the root of their number: what is left of it is a bias."""
+    g = torch.Generator().manual_seed(nq + hd)
+    B, room, dtype = 1300 // nkv + 20, 4000, torch.float16
+    x = rows(g, room // 2, nkv, hd, dtype=dtype, device="cuda")
+    one = int4.Int4KVCache(1, room, nkv, hd, dtype, "cuda")
+    one.store(rows(g, room, nkv, hd, dtype=dtype, device="cuda"), torch.stack([x, -x], 1).flatten(0, 1), packed([room], "cuda"), room)
+    cache = int4.Int4KVCache(B, room, nkv, hd, dtype, "cuda")
+    cache.data.copy_(one.data.expand_as(cache.data))
+    qkv = torch.zeros(B, (nq + 2 * nkv) * hd, dtype=dtype, device="cuda")
+    qkv[:, -nkv * hd:] = -x[-1].flatten()
+    out = int4.decode_attention_int4(qkv, cache, torch.full((B,), room - 1, dtype=torch.int32, device="cuda"), nq, nkv, hd).view(B, nq, hd)
+    ref = next(t for i, t in enumerate(_held(cache, room)) if i)[0].mean(0).repeat_interleave(nq // nkv, 0)
+    bound = 2.5 * (2 * 6 * 2.0 ** -24 * (250 / 3) ** 0.5 + 2 * 2.0 ** -22)
+    worst = float(((out.double() - ref).abs() - EPS[dtype] * ref.abs()).max())
+    bias, most = abs(float((out.double() - ref)[0].mean())), 2.5 * (2 * 6 * 2.0 ** -24 * (250 / 3) ** 0.5 / (nkv * hd) ** 0.5 + 2 * 2.0 ** -22)
+    assert bias <= most, (bias, most)
+    assert worst <= bound + SMALL[dtype], (worst, bound)
