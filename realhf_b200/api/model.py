@@ -32,7 +32,7 @@ class GenerationHyperparameters:
     # B200 addition (no reference counterpart): decode with e4m3 weights / activations on the fp8 tensor cores.  Sampled
     # tokens and the returned log-probs are those of the quantised policy (see docs/generation_fp8.md).
     fp8_weights: bool = False
-    # B200 additions: keys and values held in 4 bits (4; 16: the model's type), and the decode loop's weights (docs/generation_int4.md)
+    # B200 additions: keys and values held in 4 bits (4; 16: the model's type), and the decode loop's weights, up to 16 sequences (docs/generation_int4.md)
     kv_cache_bits: int = 16
     int4_weights: bool = False
 

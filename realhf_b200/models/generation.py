@@ -399,8 +399,8 @@ def _why_no_int4(model: ReaLModel, B: int, use_fp8: bool) -> Optional[str]:
     """Why a decode loop of B sequences cannot read 4-bit copies of the weights; None where it can."""
     if use_fp8:
         return "fp8_weights is on"
-    if B > 128:
-        return "there are more than 128 sequences"
+    if B > int4.FAST_ROWS:   # (the 16-bit weights stay beside the copies, so that there is no memory to gain)
+        return f"with more than {int4.FAST_ROWS} sequences the weights of the model's type take less time"
     return None if model.int4_decode_supported() else "it takes a dense model with a gated feed-forward in bfloat16 or float16 that is not sharded"
 
 

@@ -34,6 +34,9 @@ from realhf_b200.ops import lib, use_native
 KEY_GROUP, VALUE_GROUP, TILE_ROWS = 32, 64, 16
 HEAD_DIMS = (64, 128)
 GROUPS = (32, 64, 128)
+# Rows up to which a product with a 4-bit weight takes less time than with a 16-bit one (4096 -> 11008: 16 rows 14.8 us against 17.6, 17 rows 23.8 against 17.9; 11008 -> 4096: 14.6
+# against 17.7, 18.7 against 18.0; 4096 -> 12288: 17.7 against 19.0, 34.6 against 19.1)
+FAST_ROWS = 16
 # where channel i of a word's eight has its bits, in a key's, a value's and a weight's word
 _KEY, _VALUE, _WEIGHT = [8 * (i & 3) + 4 * (i >> 2) for i in range(8)], [4 * i for i in range(8)], [4 * (i >> 1) + 16 * (i & 1) for i in range(8)]
 

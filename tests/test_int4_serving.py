@@ -5,6 +5,7 @@ import torch
 from realhf_b200.api.model import GenerationHyperparameters, ReaLModelConfig
 from realhf_b200.models import generation as gen
 from realhf_b200.models.real_model import ReaLModel
+from realhf_b200.ops import int4
 from test_int4_generation import DEVICES, prompts, tiny
 
 
@@ -17,10 +18,12 @@ def said(monkeypatch):
 
 @pytest.mark.parametrize("why", ["supported", "fp8", "sequences", "type", "batching"])
 def test_a_loop_that_cannot_use_4_bit_weights_says_so(why, monkeypatch):
-    lines = said(monkeypatch)
+    lines, calls = said(monkeypatch), []
+    real = int4.Int4Linear.__call__
+    monkeypatch.setattr(int4.Int4Linear, "__call__", lambda self, x, bias=None: (calls.append(x.shape[0]), real(self, x, bias))[1])
     m = tiny("cpu", torch.float32 if why == "type" else torch.bfloat16)
     g = GenerationHyperparameters(max_new_tokens=2, min_new_tokens=2, greedy=True, int4_weights=True)
-    ids, cu = prompts("cpu", lens=(2,) * 129) if why == "sequences" else prompts("cpu")
+    ids, cu = prompts("cpu", lens=(2,) * 17) if why == "sequences" else prompts("cpu", lens=(2,) * 16) if why == "supported" else prompts("cpu")
     if why == "fp8":
         monkeypatch.setenv("REAL_FP8_EMULATE", "1")
         monkeypatch.setenv("REAL_GEN_FP8", "1")
@@ -30,6 +33,7 @@ def test_a_loop_that_cannot_use_4_bit_weights_says_so(why, monkeypatch):
         else:
             gen.generate(m, ids, cu, g, eos_id=None, pad_id=0)
     assert len(lines) == (why != "supported") and all("int4_weights is not used" in line for line in lines)
+    assert set(calls) == ({16} if why == "supported" else set())
 
 
 class Checked(gen.InflightBatchingGenerator):
