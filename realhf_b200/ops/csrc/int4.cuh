@@ -3,9 +3,9 @@
 // A group's numbers are one word: scale in its upper half, low in its lower half.  Codes go to matrix instructions as they are, so each kind of operand has the order of
 // nibbles that costs the fewest instructions to take apart:
 //   key words     eight channels c, at bits 8 (c & 3) + 4 (c >> 2): two masks and a shift leave two operands of four bytes.
-//   value halves  four channels c of one row at bits 4 c of a half-word, a row's neighbour in the other half: masks and one shift leave pairs of neighbouring rows, and in the low
-//                 ten bits of an fp16 number a code is a subnormal, c 2^-24 (from bits 0 .. 3) or 16 c 2^-24 (from bits 4 .. 7).
-//   weight words  eight channels c, at bits 4 (c >> 1) + 16 (c & 1): pairs of neighbouring channels, as fp16 subnormals too.
+//   value halves  four channels c of one row at bits 4 c of a half-word, a row's neighbour in the other half: a shift and a mask leave pairs of neighbouring rows in bits 7 .. 10, where a code
+//                 is the fp16 number c 2^-17.
+//   weight words  eight channels c, at bits 4 (c >> 1) + 16 (c & 1): pairs of neighbouring channels, which a mask and a larger number's bits make exact 16-bit numbers.
 //
 // A row of n words (n / 4 = channels / 32 = J) is stored as [t = 0 .. 3][j < J], word (t, j) holding the channels 32 j + 8 t ..: the four lanes of a row in a matrix
 // instruction's operand take 16 neighbouring bytes each, and what they take together for step j lies in one group of 32.

@@ -9,8 +9,8 @@
 // left operand, 16 output rows at a time; rows of x, read from L2 and L1 as the operands' lanes want them, are the right one, eight at a time.  Scale and lowest value stay out: a
 // group's product is scaled in fp32 when its channels are through, and the lowest value times the sum of x over the group (one more product, with ones) is added.
 //   Bound: the weight's bytes.  1 x 4096 x 4096 takes 4.7 us (floor 1.4; 16-bit weights 9.8): launch, first bytes and the last sum.  7 x 1024 x 50257 in groups of 32 takes 13.7
-//   (floor 5.0; 27), 16 x 4096 x 22016 24.6 (floor 7.4; 30): copies of 2 KB alone stream 3.3 .. 3.6 TB/s, and products, arithmetic and loads of x fill a third to a half of their pipes
-//   each, one after the other in a warp.  Sets dealt out in halves, so that no block has more than others, changed nothing: an SM's two blocks even it out.
+//   (floor 5.0; 27), 16 x 4096 x 22016 24.6 (floor 7.4; 30) and in groups of 32 29.1: copies of 2 KB alone stream 3.3 .. 3.6 TB/s, and products, arithmetic and loads of x fill a third to a
+//   half of their pipes each, one after the other in a warp; two of the six products of 16 channels of 16 rows are the sums of x, which each set of 32 output rows forms anew.  Sets dealt out in halves, so that no block has more than others, changed nothing: an SM's two blocks even it out.
 // More rows: a block has 128 output rows and all rows of x (in pieces of 128), and the products run on tcgen05.  Teams of four warps turn a block of 128 channels of codes into an
 // operand in tensor memory: scale (c - 8) as two numbers of the type, exact, so that one accumulator takes all channels (c - 8 and not c: sums of codes that are all positive would leave
 // the accumulator's last places to cancel).  Rows of x come by TMA, one warp issues the products, four warps sum x over the groups (products with ones), and eight add up what is left,
@@ -19,7 +19,11 @@
 //   products, sums, lowest values) of about the same length a block of channels; with half of the products left out 128 rows took 35, with a quarter of the codes expanded 35.  An
 //   accumulator a group, scaled out of tensor memory, took 45 (58 in groups of 32, now 39): a group's 64 KB leave tensor memory and its sums of x shared memory at 128 bytes a clock each.
 //   The two parts in shared memory took 45 .. 53: 275 KB a block through it.  Sums of x by the lowest values' warps took 25.3 with 64 rows and 22.1 with 32.
-// So a weight in 4 bits takes less time than one in 16 up to 16 rows, about as long with 32, and saves memory alone beyond.
+// So a weight in 4 bits takes less time than one in 16 up to 16 rows and more beyond (17 rows of 4096 -> 11008 23.8 us against 17.9, of 11008 -> 4096 18.7 against 18.0); it saves memory
+// where no 16-bit weight is kept beside it.
+//
+// Codes and rows are summed over a group before the step goes in: 15 x 128 numbers of a row have to stay inside fp32, so bf16's up to 1e35 do.  A row that holds an infinity or a NaN gives
+// numbers that are not finite, which ones is not said (sums that cancel, channels of padding that read the row's first ones against codes of 0).
 #include "attn_common.cuh"
 #include "int4.cuh"
 
@@ -557,7 +561,7 @@ __global__ void __launch_bounds__(kManyThreads<NP>, 1) many_rows_kernel(const __
       ptx::tc_fence_before();
     }
   } else if (warp < kLoadWarp) {
-    // ---- a block's sums of x over its groups, products with ones 16 rows at a time, and its lowest values: every second block a warp
+    // ---- a block's sums of x over its groups, products with ones 16 rows at a time, and its lowest values: every fourth block a warp
     for (int n = warp - kSumWarp; n < blocks; n += kSumWarps) {
       wait_empty(s_empty, n, kSums);
       wait_full(x_full, n, kXS);
