@@ -392,7 +392,7 @@ def say_ignored(option: str, why: str) -> None:
     """Once per option and reason: generation goes on without an option that was asked for."""
     if (option, why) not in _SAID:
         _SAID.add((option, why))
-        logging.getLogger("generation").warning(f"{option} is not used: {why}; the loop reads the weights of the model's type")
+        logging.getLogger("generation").warning(f"{option} is not used: {why}")
 
 
 def _why_no_int4(model: ReaLModel, B: int, use_fp8: bool) -> Optional[str]:
@@ -409,14 +409,16 @@ def generate(model: ReaLModel, input_ids: torch.Tensor, cu_seqlens: torch.Tensor
              eos_id: Optional[int], pad_id: int, generator: Optional[torch.Generator] = None,
              state: Optional[DecodeState] = None, sync_every: int = 16) -> Tuple[GenerationOutput, DecodeState]:
     """Generate for a packed batch of prompts on a single pipeline stage (pp == 1)."""
+    fp8_was, int4_was = model._fp8_active, model._int4_active
     try:
         return _generate(model, input_ids, cu_seqlens, g, eos_id, pad_id, generator, state, sync_every)
-    finally:
-        # after an error in the loop the copies of the weights would stay in use
-        if model._fp8_active:
+    except BaseException:
+        # after an error in the loop the copies that it made of the weights would stay in use
+        if model._fp8_active and not fp8_was:
             model.disable_fp8_decode()
-        if model._int4_active:
+        if model._int4_active and not int4_was:
             model.disable_int4_decode()
+        raise
 
 
 def _generate(model: ReaLModel, input_ids, cu_seqlens, g: GenerationHyperparameters, eos_id, pad_id, generator, state, sync_every):

@@ -10,7 +10,8 @@
 // group's product is scaled in fp32 when its channels are through, and the lowest value times the sum of x over the group (one more product, with ones) is added.
 //   Bound: the weight's bytes.  1 x 4096 x 4096 takes 4.7 us (floor 1.4; 16-bit weights 9.8): launch, first bytes and the last sum.  7 x 1024 x 50257 in groups of 32 takes 13.7
 //   (floor 5.0; 27), 16 x 4096 x 22016 24.6 (floor 7.4; 30) and in groups of 32 29.1: copies of 2 KB alone stream 3.3 .. 3.6 TB/s, and products, arithmetic and loads of x fill a third to a
-//   half of their pipes each, one after the other in a warp; two of the six products of 16 channels of 16 rows are the sums of x, which each set of 32 output rows forms anew.  Sets dealt out in halves, so that no block has more than others, changed nothing: an SM's two blocks even it out.
+//   half of their pipes each, one after the other in a warp; two of the six products of 16 channels of 16 rows are the sums of x, which each set of 32 output rows forms anew.  Sets dealt
+//   out in halves, so that no block has more than others, changed nothing: an SM's two blocks even it out.
 // More rows: a block has 128 output rows and all rows of x (in pieces of 128), and the products run on tcgen05.  Teams of four warps turn a block of 128 channels of codes into an
 // operand in tensor memory: scale (c - 8) as two numbers of the type, exact, so that one accumulator takes all channels (c - 8 and not c: sums of codes that are all positive would leave
 // the accumulator's last places to cancel).  Rows of x come by TMA, one warp issues the products, four warps sum x over the groups (products with ones), and eight add up what is left,

@@ -117,3 +117,16 @@ def test_kept_graph_after_a_longer_sequence(bits):
     torch.testing.assert_close(out.logprobs, want.logprobs, atol=1e-3, rtol=1e-3)
     _, state = gen.generate(m, ids, cu, options(10, kv_cache_bits=bits), eos_id=None, pad_id=0, state=state)      # (keeps none)
     assert state.graph is None and table() is None
+
+
+def test_copies_that_were_in_use_before_a_call_stay_in_use():
+    """Copies that a program has put to use by hand are its own: a call without the option leaves them so, with an error too."""
+    m = tiny("cpu", torch.bfloat16)
+    ids, cu = prompts("cpu")
+    m.enable_int4_decode()
+    copies = m._int4
+    gen.generate(m, ids, cu, options(3), eos_id=None, pad_id=0)
+    assert m._int4_active and m._int4 is copies
+    with pytest.raises(AttributeError):
+        gen.generate(m, ids, cu, None, eos_id=None, pad_id=0)
+    assert m._int4_active and m._int4 is copies
